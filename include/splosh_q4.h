@@ -410,6 +410,81 @@ int splosh_emit_operand(const float *hidden, int64_t ld_hidden, const uint16_t *
 int splosh_row_inv(const float *squares, int64_t rows, int64_t groups, int64_t dim, float eps, float *inv,
                    hipStream_t stream);
 
+/* ---- Per-request operators of a packed step ----------------------------------------------------
+ *
+ * A step packs rows of several requests into one GEMM (Runtime/BatchScheduler.swift:975). These two
+ * serve what differs from request to request in it, and have no counterpart among the reference's
+ * kernels: low-rank adapters beside a shared projection, and the choice of each row's next token. */
+
+/* Low-rank adapters of one projection, any weight format: slot s holds a_s bf16 [ranks[s]][inner] at
+ * a + s a_slot_stride (rows a_row_stride apart) and b_s bf16 [rows][ranks[s]] at b + s b_slot_stride
+ * (rows b_row_stride apart), strides in elements, and the factor scales[s]. Room for max_rank rows of
+ * a and columns of b is there in every slot (1 <= max_rank <= SPLOSH_MAX_RANK); what lies past a slot's
+ * rank is never used. ranks and scales are device arrays of `count` values; ranks NULL: max_rank for
+ * all; scales NULL: 1. A rank below 0 counts as 0, one above max_rank as max_rank. */
+#define SPLOSH_MAX_RANK 256
+typedef struct splosh_adapters {
+    const uint16_t *a;
+    const uint16_t *b;
+    const int32_t *ranks;
+    const float *scales;
+    int64_t count;
+    int64_t max_rank;
+    int64_t rows;                  /* the projection's outputs N */
+    int64_t inner;                 /* its inputs K */
+    int64_t a_slot_stride;
+    int64_t a_row_stride;
+    int64_t b_slot_stride;
+    int64_t b_row_stride;
+} splosh_adapters;
+
+/* The workspace a call needs for `rows` activation rows: the fp32 products with a. */
+size_t splosh_adapters_workspace_bytes(const splosh_adapters *adapters, int count, int64_t rows);
+
+/* out[m][n] += scales[s] sum_j t[m][j] b_s[n][j], t[m][j] = sum_k x[m][k] a_s[j][k], s = slots[m]: the
+ * adapters' part of a projection whose shared part out (fp32 or bf16) already holds. x is the
+ * projection's activation, bf16 with row stride ldx. slots: one id a row, on the device; a row whose
+ * id is negative or >= count is left as it is. t is kept in fp32, and the sum is rounded once to
+ * out's type. An infinite or NaN x gives its own row's outputs infinities or NaN; an infinite element
+ * of b may give NaN where the product would be infinite. out must not overlap x or the workspace. The
+ * workspace need not be zeroed; its first 16 KiB stay as they are, so one that other calls use serves
+ * here too, in stream order. */
+int splosh_adapters_add(const splosh_adapters *adapters, const uint16_t *x, int64_t ldx, void *out, int64_t ldc,
+                        int out_dtype, const int32_t *slots, int64_t rows, void *workspace, size_t workspace_bytes,
+                        hipStream_t stream);
+/* Several projections of one activation at once (q, k and v; gate and up), as splosh_q4_gemm_group:
+ * adapters[i] adds to outs[i] (row stride ldcs[i]) for i < count (count <= SPLOSH_MAX_GROUP). All share
+ * inner and slots; an id that is past one projection's count leaves that projection's row as it is.
+ * The outputs must not overlap. */
+int splosh_adapters_add_group(const splosh_adapters *adapters, int count, const uint16_t *x, int64_t ldx,
+                              void *const *outs, const int64_t *ldcs, int out_dtype, const int32_t *slots,
+                              int64_t rows, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The workspace a sampling call needs (0: the shape is not valid). */
+size_t splosh_sample_workspace_bytes(int64_t rows, int64_t vocab);
+
+/* The next token of each row from its logits (fp32 or bf16, [rows][vocab], row stride ld), as the ids
+ * the embedding lookups take. Per row, with T = temperature, k = top_k, p = top_p, q = min_p,
+ * u = uniforms (device arrays of `rows` values):
+ *   - NaN and -inf entries are never chosen; a row without any other gets id 0xffffffff (a row of zeros in
+ *     the embedding lookups) and logprob -inf. With +inf among them, the entries of +inf alone have
+ *     weight, the same each.
+ *   - T <= 0 or NaN: the largest entry, the first of equal ones; logprob 0.
+ *   - Else the entries in order, larger logits first and of equal ones the lower index, with weights
+ *     w = exp((logit - max) / T). k >= 1 keeps the first k. Of these, p < 1 keeps the shortest run
+ *     from the start that has p or more of their weight (one entry at least). Of these, q > 0 keeps
+ *     those with w >= q (q above 1 as 1). The token is the lowest index i whose running weight over
+ *     the kept entries in index order, i included, exceeds u times their whole weight (u below 0 or
+ *     NaN as 0, u >= 1: the last kept entry with weight); its logprob is ln(w / whole weight).
+ * temperature NULL: 1; top_k, top_p, min_p NULL: off; uniforms NULL: every row as with T = 0.
+ * logprobs may be NULL. Weights are summed in 64-bit fixed point, 2^-40 of the largest weight (less
+ * counts as none), so the result depends on no order of additions. vocab <= 2^23. The workspace is
+ * zero-filled before its first use and shared as splosh_workspace_bytes describes (its arrival
+ * counters are zero between calls). */
+int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float *uniforms,
+                  const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                  uint32_t *tokens, float *logprobs, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,12 @@ class Q5KWeight(ctypes.Structure):
     _fields_ = [("plane0", _vp), ("plane1", _vp), ("meta", _vp), ("rows", _i64), ("inner", _i64)]
 
 
+class Adapters(ctypes.Structure):
+    _fields_ = [("a", _vp), ("b", _vp), ("ranks", _vp), ("scales", _vp), ("count", _i64), ("max_rank", _i64),
+                ("rows", _i64), ("inner", _i64), ("a_slot_stride", _i64), ("a_row_stride", _i64),
+                ("b_slot_stride", _i64), ("b_row_stride", _i64)]
+
+
 # name -> (restype, argtypes); every symbol include/splosh_q4.h declares.
 SIGNATURES = {
     "splosh_q4_layout_init": (_int, [_i64, _i64, _int, _i64, _i64, ctypes.POINTER(Layout)]),
@@ -118,6 +124,12 @@ SIGNATURES = {
     "splosh_prepare_operand": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "splosh_silu_mul_operand": (_int, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
     "splosh_emit_operand": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "splosh_adapters_workspace_bytes": (_sz, [ctypes.POINTER(Adapters), _int, _i64]),
+    "splosh_adapters_add": (_int, [ctypes.POINTER(Adapters), _vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _sz, _vp]),
+    "splosh_adapters_add_group": (_int, [ctypes.POINTER(Adapters), _int, _vp, _i64, ctypes.POINTER(_vp),
+                                         ctypes.POINTER(_i64), _int, _vp, _i64, _vp, _sz, _vp]),
+    "splosh_sample_workspace_bytes": (_sz, [_i64, _i64]),
+    "splosh_sample": (_int, [_vp, _i64, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "splosh_row_inv": (_int, [_vp, _i64, _i64, _i64, ctypes.c_float, _vp, _vp]),
 }
 

@@ -1165,3 +1165,102 @@ int splosh_row_inv(const float *squares, int64_t rows, int64_t groups, int64_t d
 }
 
 }  // extern "C"
+
+// ---- per-request operators -------------------------------------------------------------------
+
+namespace {
+
+int check_adapters(const splosh_adapters *w) {
+    if (!w->a || !w->b) return fail(SPLOSH_ERR_NULL_POINTER, "null adapter matrices");
+    if (w->count <= 0 || w->rows <= 0 || w->inner <= 0 || w->max_rank <= 0)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "adapters: count, max_rank, rows and inner must be positive");
+    if (w->max_rank > SPLOSH_MAX_RANK)
+        return fail(SPLOSH_ERR_UNSUPPORTED, "max_rank above " + std::to_string(SPLOSH_MAX_RANK));
+    if (w->count > INT32_MAX || w->rows > INT32_MAX / 2 || w->inner > INT32_MAX / 2)
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "adapters: size overflows");
+    if (w->a_row_stride < w->inner || w->b_row_stride < w->max_rank || w->a_slot_stride < 0 || w->b_slot_stride < 0)
+        return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "adapter stride shorter than its rows");
+    if (mul_overflows(w->max_rank, w->a_row_stride) || mul_overflows(w->rows, w->b_row_stride) ||
+        mul_overflows(w->count, w->a_slot_stride) || mul_overflows(w->count, w->b_slot_stride))
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "adapters: size overflows");
+    if (!aligned(w->a, 2) || !aligned(w->b, 2) || !aligned(w->ranks, 4) || !aligned(w->scales, 4))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "adapter arrays are not aligned to their elements");
+    return SPLOSH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t splosh_adapters_workspace_bytes(const splosh_adapters *adapters, int count, int64_t rows) {
+    if (!adapters || count < 1 || count > SPLOSH_MAX_GROUP || rows <= 0 || rows > splosh::kAdapterMaxRows) return 0;
+    for (int i = 0; i < count; ++i)
+        if (adapters[i].max_rank <= 0 || adapters[i].max_rank > SPLOSH_MAX_RANK || adapters[i].inner <= 0) return 0;
+    return splosh::adapters_workspace_bytes(adapters, count, rows);
+}
+
+int splosh_adapters_add_group(const splosh_adapters *adapters, int count, const uint16_t *x, int64_t ldx,
+                              void *const *outs, const int64_t *ldcs, int out_dtype, const int32_t *slots,
+                              int64_t rows, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (!adapters || !outs || !ldcs) return fail(SPLOSH_ERR_NULL_POINTER, "null adapters, output or ldc list");
+    if (!slots) return fail(SPLOSH_ERR_NULL_POINTER, "null slots");
+    if (count < 1 || count > SPLOSH_MAX_GROUP)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "count must be 1.." + std::to_string(SPLOSH_MAX_GROUP));
+    int st;
+    for (int i = 0; i < count; ++i) {
+        if ((st = check_adapters(&adapters[i]))) return st;
+        if (adapters[i].inner != adapters[0].inner)
+            return fail(SPLOSH_ERR_INVALID_SHAPE, "grouped adapters must share inner");
+        if ((st = check_io(x, ldx, outs[i], ldcs[i], out_dtype, rows, adapters[i].rows, adapters[i].inner))) return st;
+        if (!aligned(x, 2) || !aligned(outs[i], out_dtype == SPLOSH_F32 ? 4 : 2) || !aligned(slots, 4))
+            return fail(SPLOSH_ERR_UNSUPPORTED, "operands are not aligned to their elements");
+        for (int j = 0; j < i; ++j)
+            if (outs[i] == outs[j]) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "grouped outputs must not overlap");
+    }
+    if (rows > splosh::kAdapterMaxRows) return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows for one launch");
+    const size_t need = splosh::adapters_workspace_bytes(adapters, count, rows);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SPLOSH_ERR_WORKSPACE_TOO_SMALL,
+                    "adapters need a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return hip_status(splosh::launch_adapters(adapters, count, x, ldx, outs, ldcs, out_dtype, slots, rows, workspace,
+                                              stream),
+                      "adapters launch");
+}
+
+int splosh_adapters_add(const splosh_adapters *adapters, const uint16_t *x, int64_t ldx, void *out, int64_t ldc,
+                        int out_dtype, const int32_t *slots, int64_t rows, void *workspace, size_t workspace_bytes,
+                        hipStream_t stream) {
+    return splosh_adapters_add_group(adapters, 1, x, ldx, &out, &ldc, out_dtype, slots, rows, workspace,
+                                     workspace_bytes, stream);
+}
+
+size_t splosh_sample_workspace_bytes(int64_t rows, int64_t vocab) {
+    if (rows <= 0 || rows > INT32_MAX || vocab <= 0 || vocab > splosh::kSampleMaxVocab) return 0;
+    return splosh::sample_workspace_bytes(rows, vocab);
+}
+
+int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float *uniforms,
+                  const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                  uint32_t *tokens, float *logprobs, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (!logits || !tokens) return fail(SPLOSH_ERR_NULL_POINTER, "null logits or tokens");
+    if (rows <= 0 || vocab <= 0) return fail(SPLOSH_ERR_INVALID_SHAPE, "rows and vocab must be positive");
+    if (ld < vocab) return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "ld is shorter than vocab");
+    if (dtype != SPLOSH_F32 && dtype != SPLOSH_BF16) return fail(SPLOSH_ERR_UNSUPPORTED, "unknown logits dtype");
+    if (vocab > splosh::kSampleMaxVocab) return fail(SPLOSH_ERR_UNSUPPORTED, "vocab above 2^23");
+    if (mul_overflows(rows, ld)) return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "size overflows");
+    if (rows > INT32_MAX) return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows");
+    if (!aligned(logits, dtype == SPLOSH_F32 ? 4 : 2) || !aligned(tokens, 4) || !aligned(logprobs, 4) ||
+        !aligned(uniforms, 4) || !aligned(temperature, 4) || !aligned(top_k, 4) || !aligned(top_p, 4) ||
+        !aligned(min_p, 4))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "operands are not aligned to their elements");
+    const size_t need = splosh::sample_workspace_bytes(rows, vocab);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SPLOSH_ERR_WORKSPACE_TOO_SMALL,
+                    "sampling needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return hip_status(splosh::launch_sample(logits, ld, dtype, rows, vocab,
+                                            {uniforms, temperature, top_k, top_p, min_p}, tokens, logprobs, workspace,
+                                            stream),
+                      "sample launch");
+}
+
+}  // extern "C"

@@ -293,4 +293,23 @@ hipError_t launch_q5k_gemm_scalar(const splosh_q5k_weight &w, const uint16_t *a,
                                   int64_t ldc, int out_dtype, const void *residual, int64_t rows,
                                   hipStream_t stream);
 
+// Low-rank adapters beside a projection (adapters.hip): `group` projections of one activation.
+constexpr int64_t kAdapterMaxRows = 1 << 21;
+size_t adapters_workspace_bytes(const splosh_adapters *adapters, int group, int64_t rows);
+hipError_t launch_adapters(const splosh_adapters *adapters, int group, const uint16_t *x, int64_t ldx,
+                           void *const *outs, const int64_t *ldcs, int out_dtype, const int32_t *slots, int64_t rows,
+                           void *workspace, hipStream_t stream);
+
+// Sampling (sample.hip).
+constexpr int64_t kSampleMaxVocab = 1 << 23;
+struct SampleParams {
+    const float *uniforms, *temperature;  // null uniforms: greedy
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+};
+size_t sample_workspace_bytes(int64_t rows, int64_t vocab);
+hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab,
+                         const SampleParams &params, uint32_t *tokens, float *logprobs, void *workspace,
+                         hipStream_t stream);
+
 }  // namespace splosh

@@ -7,6 +7,8 @@ libsplosh_q4.so through its C ABI. The names follow the reference's host API:
 * ``Engine.gemm`` / ``Engine.mlp_in`` -- Runtime/Engine.swift:1652, :1911 (stream-ordered).
 * ``dequant``, ``tile128``, ``q5k_repack`` -- DequantOracle.dequantize, Converter.tile,
   GgufPlanes.repack on the device.
+* ``add_adapters`` / ``sample`` -- what differs between the requests of a packed step: low-rank
+  adapters beside a projection, and the choice of each row's next token.
 
 Buffer-size checks (GemmQ4Error.bufferTooSmall) happen here because the C ABI sees raw pointers.
 """
@@ -589,3 +591,160 @@ def embed(w, tokens, out=None, out_dtype=torch.float32, stream=None):
     _lib.check(fn(ctypes.byref(wc), _ptr(tokens), count, _ptr(out), out.stride(0), _dtype_code(out.dtype),
                   _stream(stream)))
     return out
+
+
+# ---- per-request operators of a packed step ------------------------------------------------------
+
+
+def _device(t, stream):
+    """The context a call on `t` is launched in: nothing to enter when its device is the current one
+    or a stream is named (the kernels go to the stream's device)."""
+    if t.device.index in (None, torch.cuda.current_device()):
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _vector(t, rows, dtype, device, name):
+    """A per-row array: contiguous, of at least `rows` values, on the operands' device (None: none)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
+        raise SploshError(13, f"{name} must be a contiguous {dtype} vector")
+    if t.numel() < rows:
+        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows}, observed: {t.numel()})")
+    if t.device != device:
+        raise SploshError(13, f"{name} is on {t.device}, the operands on {device}")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _matrix(t, rows, columns, device, name):
+    """A [rows, columns] operand: contiguous rows of at least `columns` on the operands' device."""
+    if not t.is_cuda:
+        raise SploshError(12, f"{name} is not a device tensor")
+    if t.dim() != 2 or t.stride(1) != 1 or t.device != device:
+        raise SploshError(13, f"{name} must be [rows, columns] with contiguous rows, on {device}")
+    if t.shape[1] < columns:
+        raise GemmQ4Error(1, f"{name} has {t.shape[1]} columns, {columns} are needed")
+    if t.shape[0] < rows:
+        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows} rows, observed: {t.shape[0]})")
+
+
+@dataclass
+class Adapters:
+    """The low-rank adapters of one projection (splosh_adapters): ``a`` bf16 [count, max_rank, inner]
+    and ``b`` bf16 [count, rows, max_rank] (last dimensions contiguous), ``scales`` fp32 [count]
+    (None: 1) and ``ranks`` int32 [count] (None: max_rank for all). Slot s adds
+    scales[s] * b[s][:, :r] @ (a[s][:r] @ x), r = ranks[s]. The tensors are taken as they are: adapters
+    are exchanged by writing into them."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scales: torch.Tensor = None
+    ranks: torch.Tensor = None
+
+    def __post_init__(self):
+        a, b = self.a, self.b
+        if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+            raise SploshError(13, "adapter matrices must be bf16")
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or 0 in a.shape + b.shape:
+            raise GemmQ4Error(1, "adapters are a [count, max_rank, inner] and b [count, rows, max_rank]")
+        if a.stride(2) != 1 or b.stride(2) != 1:
+            raise SploshError(13, "adapter rows must be contiguous")
+        if not a.is_cuda:
+            raise SploshError(12, "a is not a device tensor")
+        if b.device != a.device:
+            raise SploshError(13, f"b is on {b.device}, a on {a.device}")
+        self.count, self.max_rank, self.inner = a.shape
+        self.rows = b.shape[1]
+        scales = _vector(self.scales, self.count, torch.float32, a.device, "scales")
+        ranks = _vector(self.ranks, self.count, torch.int32, a.device, "ranks")
+        self._c = _lib.Adapters(a.data_ptr(), b.data_ptr(), ranks, scales, self.count, self.max_rank, self.rows,
+                                self.inner, a.stride(0), a.stride(1), b.stride(0), b.stride(1))
+
+    def c(self):
+        return self._c
+
+
+def adapters_workspace_bytes(adapters, rows):
+    """splosh_adapters_workspace_bytes: the scratch a call on these projections' adapters needs."""
+    adapters = [adapters] if isinstance(adapters, Adapters) else list(adapters)
+    cs = (_lib.Adapters * len(adapters))(*[w.c() for w in adapters])
+    return _lib.lib().splosh_adapters_workspace_bytes(cs, len(adapters), rows)
+
+
+def add_adapters_group(outs, a, adapters, slots, rows=None, stream=None, workspace=None):
+    """splosh_adapters_add_group: the adapters' part of several projections of one activation,
+    outs[i][m] += adapters[i] of slots[m] on a[m], in place. ``a`` is the projections' bf16 activation
+    [rows, inner], ``outs`` their outputs (gemm_group's; fp32 or bf16), ``slots`` int32 [rows], the
+    adapter of each row (negative or past the count: none). Returns the outputs."""
+    rows = a.shape[0] if rows is None else rows
+    if a.dtype != torch.bfloat16:
+        raise SploshError(13, "activations must be bf16")
+    outs, adapters = list(outs), list(adapters)
+    if len(outs) != len(adapters) or not outs:
+        raise GemmQ4Error(1, "one output for each projection's adapters")
+    n = len(outs)
+    if rows <= 0:
+        raise GemmQ4Error(1, "rows must be positive")
+    _matrix(a, rows, adapters[0].inner, a.device, "a")
+    for w, o in zip(adapters, outs):
+        if o.dtype != outs[0].dtype:
+            raise SploshError(13, "grouped outputs must share one dtype")
+        _matrix(o, rows, w.rows, a.device, "output")
+        if w.a.device != a.device:
+            raise SploshError(13, f"adapters are on {w.a.device}, the activations on {a.device}")
+    slot_ptr = _vector(slots, rows, torch.int32, a.device, "slots")
+    cs = (_lib.Adapters * n)(*[w.c() for w in adapters])
+    out_ptrs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+    ldcs = (ctypes.c_int64 * n)(*[o.stride(0) for o in outs])
+    with _device(a, stream):
+        if workspace is None:
+            with _allocating(stream):
+                workspace = torch.empty(max(1, _lib.lib().splosh_adapters_workspace_bytes(cs, n, rows)),
+                                        dtype=torch.uint8, device=a.device)
+        _lib.check(_lib.lib().splosh_adapters_add_group(cs, n, _ptr(a), a.stride(0), out_ptrs, ldcs,
+                                                        _dtype_code(outs[0].dtype), slot_ptr, rows, _ptr(workspace),
+                                                        workspace.numel() * workspace.element_size(), _stream(stream)))
+    return outs
+
+
+def add_adapters(out, a, adapters, slots, rows=None, stream=None, workspace=None):
+    """splosh_adapters_add: add_adapters_group for one projection. Returns ``out``."""
+    return add_adapters_group([out], a, [adapters], slots, rows, stream, workspace)[0]
+
+
+def sample_workspace_bytes(rows, vocab):
+    """splosh_sample_workspace_bytes: the scratch a sampling call needs (0: not a valid shape)."""
+    return _lib.lib().splosh_sample_workspace_bytes(rows, vocab)
+
+
+def sample(logits, uniforms=None, temperature=None, top_k=None, top_p=None, min_p=None, out=None, logprobs=None,
+           stream=None, workspace=None):
+    """splosh_sample: the next token of each row of ``logits`` (fp32 or bf16 [rows, vocab]), and the
+    natural logarithm of the probability it was drawn with. The parameters are fp32 (top_k: int32)
+    device vectors [rows]; None leaves that one off. uniforms None: the largest logit of every row
+    (as temperature 0 in one row). Returns (tokens int32, logprobs fp32); a row with nothing to choose
+    gets token -1, which embed turns into zeros."""
+    device = logits.device
+    _matrix(logits, 0, 0, device, "logits")
+    rows, vocab = logits.shape
+    if rows == 0 or vocab == 0:
+        raise GemmQ4Error(1, "rows and vocab must be positive")
+    params = [_vector(t, rows, dt, device, name) for t, dt, name in
+              ((uniforms, torch.float32, "uniforms"), (temperature, torch.float32, "temperature"),
+               (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"))]
+    with _device(logits, stream):
+        with _allocating(stream):
+            if out is None:
+                out = torch.empty(rows, dtype=torch.int32, device=device)
+            if logprobs is None:
+                logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+            if workspace is None:
+                workspace = torch.empty(max(1, sample_workspace_bytes(rows, vocab)), dtype=torch.uint8, device=device)
+                workspace[:WORKSPACE_COUNTER_BYTES].zero_()
+        _lib.check(_lib.lib().splosh_sample(_ptr(logits), logits.stride(0), _dtype_code(logits.dtype), rows, vocab,
+                                            *params, _vector(out, rows, torch.int32, device, "out"),
+                                            _vector(logprobs, rows, torch.float32, device, "logprobs"),
+                                            _ptr(workspace), workspace.numel() * workspace.element_size(),
+                                            _stream(stream)))
+    return out, logprobs
