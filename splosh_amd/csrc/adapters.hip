@@ -1,13 +1,17 @@
 // adapters.hip -- low-rank adapters of many requests beside a shared projection.
 //
 // out[m] += c_s b_s (a_s x[m]) for the adapter s = slots[m] of row m, in two launches: the products
-// t = a_s x (fp32 partial sums over slices of K, in the workspace), then out += b_s (c_s t).
+// t = c_s a_s x (fp32 partial sums over slices of K, in the workspace), then out += b_s t.
 //
 // Both walk the rows in chunks of 64. A chunk's rows are taken adapter by adapter: the lanes of a wave
 // hold the chunk's slots, a ballot gives the rows of one adapter, and these meet the adapter's matrix as
-// the columns of v_mfma_f32_16x16x32_bf16, sixteen at a time, whatever places they have in the batch. So
-// an adapter's matrices are read once a chunk, no sorted order of the rows is asked for, and an adapter
-// no row uses costs nothing.
+// the columns of v_mfma_f32_16x16x32_bf16, whatever places they have in the batch. So no sorted order of
+// the rows is asked for, an adapter's matrices are read once a chunk, and one no row uses costs nothing.
+// The first launch leaves the chunks' lists of adapters and rows for the second.
+//
+// FAST kernels are for operands whose every 16-byte piece is whole, aligned and within a buffer
+// descriptor's reach (the usual case): their loads have no branches, since an offset out of a descriptor's
+// range reads zeros and writes nothing. The others take elements one by one where a piece is not whole.
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -17,40 +21,42 @@ namespace splosh {
 constexpr size_t kAdapterCounterBytes = 16384;
 constexpr int kChunk = 64;       // rows of a chunk
 constexpr int kDownRanks = 64;   // rows of a that a workgroup of the first launch takes
-constexpr int kUpColumns = 256;  // outputs of a workgroup of the second
-constexpr int kUpRanks = 64;     // ranks it stages at a time
+constexpr int kUpColumns = 256;  // outputs of a tile of the second
+// An offset past every descriptor, and still so with another one added.
+constexpr uint32_t kNowhere = 0x40000000u;
+
+// One chunk's adapters for one projection.
+struct ChunkList {
+    struct Part {
+        int32_t slot;
+        uint16_t rank;       // 0: past the last part
+        uint8_t first, count;  // its rows: order[first ..]
+    } part[kChunk];
+    uint8_t order[kChunk];
+};
 
 struct AdapterWeight {
     splosh_adapters w;
     void *out;
     int64_t ldc;
     int t_offset;  // its first column of t
-    int first;     // its first workgroup column of the launch
 };
 
 struct AdapterArgs {
-    AdapterWeight w[SPLOSH_MAX_GROUP];
-    int group;
     const uint16_t *x;
-    int64_t ldx;
+    int64_t ldx, rows;
     const int32_t *slots;
-    float *t;     // [slices][rows][t_cols]
-    int t_cols, slices;
-    int64_t rows;
+    ChunkList *lists;  // [projection][chunk]
+    float *t;          // [slices][rows][t_cols]
+    int t_cols, slices, slice_steps;
+    int tiles;    // tiles of outputs a workgroup of the second launch takes
+    int turns;    // workgroups that share a chunk's adapters
+    AdapterWeight w[SPLOSH_MAX_GROUP];
 };
 
-// The projection a workgroup column belongs to.
-__device__ __forceinline__ int projection_of(const AdapterArgs &args, int column) {
-    int i = 0;
-    while (i + 1 < args.group && column >= args.w[i + 1].first) ++i;
-    return i;
-}
-
-// Elements [0, n) of eight from p, zero past them; ALIGNED: p is 16-byte aligned.
-template <bool ALIGNED>
+// Elements [0, n) of the eight at p, zero past them.
 __device__ __forceinline__ u32x4 load8(const uint16_t *p, int n) {
     u32x4 v = {0, 0, 0, 0};
-    if (ALIGNED && n >= 8) return *(const u32x4 *)p;
     if (n > 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -58,95 +64,66 @@ __device__ __forceinline__ u32x4 load8(const uint16_t *p, int n) {
     }
     return v;
 }
-
-// The rows of a chunk, adapter by adapter: every lane holds its row's slot and rank (0: no adapter), and
-// next() leaves in `mine` the i-th row of the next adapter's for lane i (the other rows after them).
-struct ChunkRows {
-    int slot, rank, seen, mine, count;
-    uint64_t todo;
-    int group_slot, group_rank;
-
-    __device__ __forceinline__ ChunkRows(const AdapterArgs &args, const splosh_adapters &w, int64_t base) {
-        const int lane = threadIdx.x & 63;
-        const int64_t row = base + lane;
-        slot = row < args.rows ? args.slots[row] : -1;
-        const bool known = slot >= 0 && slot < w.count;
-        rank = known ? (w.ranks ? w.ranks[slot] : (int)w.max_rank) : 0;
-        rank = rank < (int)w.max_rank ? rank : (int)w.max_rank;
-        todo = __ballot(rank > 0);
-        seen = 0;
-    }
-
-    // The next adapter whose turn is `z` of `turns`; false past the last.
-    __device__ __forceinline__ bool next(int z, int turns) {
-        while (todo) {
-            const int first = __builtin_ctzll(todo);
-            group_slot = __builtin_amdgcn_readlane(slot, first);
-            const uint64_t rows = __ballot(rank > 0 && slot == group_slot);
-            todo &= ~rows;
-            if (seen++ % turns != z) continue;
-            group_rank = __builtin_amdgcn_readlane(rank, first);
-            count = __builtin_popcountll(rows);
-            const int lane = threadIdx.x & 63;
-            const uint64_t below = ((uint64_t)1 << lane) - 1;
-            const int place = rows >> lane & 1 ? __builtin_popcountll(rows & below)
-                                               : count + __builtin_popcountll(~rows & below);
-            mine = __builtin_amdgcn_ds_permute(place * 4, lane);
-            return true;
-        }
-        return false;
-    }
-
-    // The chunk row at place i of the adapter's.
-    __device__ __forceinline__ int row_at(int i) const { return __builtin_amdgcn_ds_bpermute(i * 4, mine); }
-};
+__device__ __forceinline__ u32x4 keep8(u32x4 v, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 2 * i + 1 < n ? v[i] : 2 * i < n ? v[i] & 0xffffu : 0u;
+    return v;
+}
 
 // ---- t = a x --------------------------------------------------------------------------------------
 //
-// A workgroup: one chunk, up to 64 rows of one projection's a, one slice of K. Its four waves take the
-// slice's steps of 32 k in turn, kSteps of them with every load in flight, and add their sums in LDS.
-// a's rows are the MFMA's rows and the activation rows its columns: the sum's four registers are then
-// four neighbouring ranks of one activation row, a 16-byte store.
+// A workgroup: one adapter's rows of a chunk, up to 64 rows of one projection's a, one slice of K. Its eight
+// waves take the slice's steps of 32 k in turn, kSteps of them with every load in flight, and add their
+// sums in LDS. a's rows are the MFMA's rows and the activation rows its columns: the sum's four registers
+// are then four neighbouring ranks of one activation row, a 16-byte store.
 
-constexpr int kSteps = 4;
+constexpr int kDownWaves = 8;
 
-template <int RB, int P, bool ALIGNED>
-__device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args, const AdapterWeight &g, const ChunkRows &rows,
-                                          int64_t base, int rank0, int slice, f32x4 *sums) {
+// 16 RB of the adapter's rows: `mine` is the chunk row that lane i holds as the adapter's i-th.
+template <int RB, int P, bool FAST>
+__device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args, const AdapterWeight &g, int slot,
+                                                         int rank, float scale, int mine, int count, int64_t base,
+                                                         int rank0, int slice, f32x4 *sums) {
+    constexpr int kSteps = RB == 1 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
     const int inner = (int)g.w.inner, steps = (inner + 31) / 32;
-    const int from = (int)((int64_t)steps * slice / args.slices), to = (int)((int64_t)steps * (slice + 1) / args.slices);
-    const uint16_t *a = g.w.a + rows.group_slot * g.w.a_slot_stride;
-    const uint16_t *xr[RB], *ar[P];
-    bool xv[RB], av[P];
-    int64_t out_row[RB];
+    const int from = slice * args.slice_steps, to = from + args.slice_steps < steps ? from + args.slice_steps : steps;
+    const uint16_t *a = g.w.a + slot * g.w.a_slot_stride, *x = args.x + base * args.ldx;
+    const rsrc_t ra = make_rsrc(a, FAST ? (uint32_t)(g.w.max_rank * g.w.a_row_stride * 2) : 0);
+    const rsrc_t rx = make_rsrc(x, FAST ? (uint32_t)(kChunk * args.ldx * 2) : 0);
+    uint32_t xo[RB], ao[P];
+    int xr[RB];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-        xv[i] = i * 16 + m < rows.count;
-        const int at = rows.row_at(i * 16 + m);
-        out_row[i] = base + (xv[i] ? at : 0);
-        xr[i] = args.x + out_row[i] * args.ldx;
+        xr[i] = __builtin_amdgcn_ds_bpermute(((i * 16 + m) & 63) * 4, mine);
+        if (i * 16 + m >= count) xr[i] = -1;
+        xo[i] = xr[i] < 0 ? kNowhere : (uint32_t)(xr[i] * args.ldx * 2);
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         const int r = rank0 + p * 16 + m;
-        av[p] = r < rows.group_rank;
-        ar[p] = a + (av[p] ? r : 0) * g.w.a_row_stride;
+        ao[p] = r < rank ? (uint32_t)(r * g.w.a_row_stride * 2) : kNowhere;
     }
     f32x4 acc[RB][P];
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
         for (int p = 0; p < P; ++p) acc[i][p] = f32x4{0, 0, 0, 0};
-    for (int s = from + wave; s < to; s += 4 * kSteps) {
+    for (int s = from + wave; s < to; s += kDownWaves * kSteps) {
         u32x4 xs[kSteps][RB], as[kSteps][P];
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-            const int step = s + 4 * j, k = step * 32 + q * 8, n = step < to ? inner - k : 0;
+            const int step = s + kDownWaves * j, k = step * 32 + q * 8, n = step < to ? inner - k : 0;
+            const uint32_t ko = n > 0 ? (uint32_t)k * 2 : kNowhere;
 #pragma unroll
-            for (int i = 0; i < RB; ++i) xs[j][i] = load8<ALIGNED>(xr[i] + k, xv[i] ? n : 0);
+            for (int i = 0; i < RB; ++i)
+                xs[j][i] = FAST ? buffer_load16(rx, xo[i] + ko, 0)
+                                : load8(x + (xr[i] < 0 ? 0 : xr[i]) * args.ldx + k, xr[i] < 0 ? 0 : n);
 #pragma unroll
-            for (int p = 0; p < P; ++p) as[j][p] = load8<ALIGNED>(ar[p] + k, av[p] ? n : 0);
+            for (int p = 0; p < P; ++p) {
+                const int r = rank0 + p * 16 + m;
+                as[j][p] = FAST ? buffer_load16(ra, ao[p] + ko, 0) : load8(a + r * g.w.a_row_stride + k, r < rank ? n : 0);
+            }
         }
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
@@ -157,208 +134,270 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
                     acc[i][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(as[j][p]), as_bf16x8(xs[j][i]),
                                                                          acc[i][p], 0, 0, 0);
     }
-    // The waves' sums, panel by panel: [wave][row block][lane].
+    // The waves' sums, a panel at a time: [row block][wave][lane].
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RB; ++i) sums[(wave * RB + i) * 64 + lane] = acc[i][p];
+        for (int i = 0; i < RB; ++i) sums[(i * kDownWaves + wave) * 64 + lane] = acc[i][p];
         __syncthreads();
-        if (wave < RB) {
-            f32x4 v = sums[wave * 64 + lane];
+        if (wave >= RB) continue;
+        f32x4 v = sums[wave * kDownWaves * 64 + lane];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) v += sums[(w * RB + wave) * 64 + lane];
-            const int r = rank0 + p * 16 + q * 4;
-            int64_t row = out_row[0];
-            bool live = xv[0];
+        for (int w = 1; w < kDownWaves; ++w) v += sums[(wave * kDownWaves + w) * 64 + lane];
+        int row = xr[0];
 #pragma unroll
-            for (int i = 1; i < RB; ++i)
-                if (wave == i) row = out_row[i], live = xv[i];
-            if (live && r < rows.group_rank)
-                *(f32x4 *)(args.t + ((int64_t)slice * args.rows + row) * args.t_cols + g.t_offset + r) = v;
-        }
+        for (int i = 1; i < RB; ++i) row = wave == i ? xr[i] : row;
+        const int r = rank0 + p * 16 + q * 4;
+        if (row >= 0 && r < rank)
+            *(f32x4 *)(args.t + ((int64_t)slice * args.rows + base + row) * args.t_cols + g.t_offset + r) = v * scale;
     }
 }
 
-template <int RBMAX, int P, bool ALIGNED>
-__global__ void __launch_bounds__(256, 2) adapter_down_kernel(AdapterArgs args) {
-    __shared__ f32x4 sums[4 * RBMAX * 64];
+template <int RBMAX, int P, bool FAST>
+__global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(AdapterArgs args) {
+    __shared__ f32x4 sums[RBMAX * kDownWaves * 64];
+    const int which = blockIdx.z / args.turns, turn = blockIdx.z % args.turns;
     const int column = blockIdx.x / args.slices, slice = blockIdx.x % args.slices;
-    const AdapterWeight &g = args.w[projection_of(args, column)];
-    const int rank0 = (column - g.first) * kDownRanks;
-    const int64_t base = (int64_t)blockIdx.y * kChunk;
-    ChunkRows rows(args, g.w, base);
-    while (rows.next(blockIdx.z, gridDim.z)) {
-        if (rank0 >= rows.group_rank) continue;
-        if (RBMAX == 1 || rows.count <= 16)
-            down_rows<1, P, ALIGNED>(args, g, rows, base, rank0, slice, sums);
-        else if (rows.count <= 32)
-            down_rows<RBMAX == 1 ? 1 : 2, P, ALIGNED>(args, g, rows, base, rank0, slice, sums);
-        else
-            down_rows<RBMAX, P, ALIGNED>(args, g, rows, base, rank0, slice, sums);
+    const AdapterWeight &g = args.w[which];
+    const int rank0 = column * kDownRanks, lane = threadIdx.x & 63;
+    if (rank0 >= g.w.max_rank) return;
+    // Every lane its row's slot, rank (0: no adapter) and scale.
+    const int64_t base = (int64_t)blockIdx.y * kChunk, my_row = base + lane;
+    const int slot = my_row < args.rows ? args.slots[my_row] : -1;
+    const bool known = slot >= 0 && slot < g.w.count;
+    int rank = known ? (g.w.ranks ? g.w.ranks[slot] : (int)g.w.max_rank) : 0;
+    const float scale = known && g.w.scales ? g.w.scales[slot] : 1.0f;
+    rank = rank < (int)g.w.max_rank ? rank : (int)g.w.max_rank;
+    const uint64_t all = __ballot(rank > 0), below = ((uint64_t)1 << lane) - 1;
+    uint64_t todo = all;
+    for (int part = 0; todo; ++part) {
+        const int lead = __builtin_ctzll(todo);
+        const int group_slot = __builtin_amdgcn_readlane(slot, lead), group_rank = __builtin_amdgcn_readlane(rank, lead);
+        const uint64_t rows = __ballot(rank > 0 && slot == group_slot);
+        todo &= ~rows;
+        if (part % args.turns != turn || rank0 >= group_rank) continue;
+        const int count = __builtin_popcountll(rows);
+        const int place = rows >> lane & 1 ? __builtin_popcountll(rows & below)
+                                           : count + __builtin_popcountll(~rows & below);
+        int mine = __builtin_amdgcn_ds_permute(place * 4, lane);
+        const float group_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), lead));
+        if (RBMAX == 1 || count <= 16) {
+            for (int left = count; left > 0; left -= 16) {
+                down_rows<1, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, left, base, rank0, slice, sums);
+                mine = __builtin_amdgcn_ds_bpermute(((lane + 16) & 63) * 4, mine);
+            }
+        } else {
+            down_rows<RBMAX, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, count, base, rank0, slice, sums);
+        }
     }
+    // The list for the second launch, by one wave of the chunk.
+    if (blockIdx.x != 0 || turn != 0 || threadIdx.x >= 64) return;
+    ChunkList &list = args.lists[which * (int64_t)gridDim.y + blockIdx.y];
+    int first = 0, part = 0;
+    for (todo = all; todo; ++part) {
+        const int lead = __builtin_ctzll(todo), group_slot = __builtin_amdgcn_readlane(slot, lead);
+        const uint64_t rows = __ballot(rank > 0 && slot == group_slot);
+        todo &= ~rows;
+        if (rows >> lane & 1) list.order[first + __builtin_popcountll(rows & below)] = (uint8_t)lane;
+        const int count = __builtin_popcountll(rows);
+        if (lane == lead) list.part[part] = {group_slot, (uint16_t)rank, (uint8_t)first, (uint8_t)count};
+        first += count;
+    }
+    if (lane >= part) list.part[lane].rank = 0;
 }
 
 // ---- out += b t -----------------------------------------------------------------------------------
 //
-// A workgroup: one chunk, 256 outputs of one projection, 64 a wave. t's slices are summed, scaled, and
-// laid down in LDS as MFMA operands, in two bf16 pieces for a bf16 output and three for an fp32 one (a
-// piece takes eight more bits, so the products keep 16 or 24 of t's); b's rows are the MFMA's rows,
-// dealt so that a lane's sixteen sums of one output row are sixteen neighbouring outputs: row 4 q + i of
-// block j is output 16 q + 4 j + i.
+// A workgroup: one adapter's rows of a chunk, a run of tiles of 256 outputs of one projection, 64 outputs
+// a wave. t's slices are summed and laid down in LDS as MFMA operands, in two bf16 pieces for a bf16
+// output and three for an fp32 one (a piece takes eight more bits, so the products keep 16 or 24 of t's).
+// b's rows are the MFMA's rows and stay in registers while the adapter's rows go by, sixteen at a time. Their
+// sums pass through LDS, so that a wave reads and writes runs of 64 neighbouring outputs of a row: with
+// the MFMA's own layout, neighbouring lanes hold different rows, and four times the cache lookups.
 
-template <typename OUT>
-__device__ __forceinline__ void load_out16(const OUT *p, int n, bool vector, uint32_t (&v)[16 * sizeof(OUT) / 4]) {
-    constexpr int kPer = 4 / sizeof(OUT);
-    if (vector && n >= 16) {
+// Orders a wave's own LDS operations for the compiler (the hardware does them in order).
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kUpSumStride = 68;  // floats of a row of sums in LDS: 64 and a step of four banks
+
+// The part's rows of t summed over the slices, as operands in LDS: [piece][panel of 32 ranks][row block]
+// [lane] x 16 bytes. Four ranks of one row a thread.
+template <int PIECES>
+__device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWeight &g, int mine, int count,
+                                        int blocks, int64_t base, int rank, u32x2 *pieces) {
+    constexpr int kAtOnce = 8;
+    const int panels = (rank + 31) / 32, quads = panels * 8;
+    const int64_t slice_floats = args.rows * args.t_cols;
+    for (int item = threadIdx.x; item < blocks * 16 * quads; item += 256) {
+        const int i = item / quads, r = (item - i * quads) * 4;
+        f32x4 v = {0, 0, 0, 0};
+        const int chunk_row = __builtin_amdgcn_ds_bpermute(i * 4, mine);
+        if (i < count && r < rank) {
+            const float *t = args.t + (base + chunk_row) * args.t_cols + g.t_offset + r;
+            for (int s = 0; s < args.slices; s += kAtOnce) {
+                f32x4 part[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(OUT); ++i) {
-            const u32x4 w = *(const u32x4 *)((const char *)p + 16 * i);
+                for (int e = 0; e < kAtOnce; ++e)
+                    part[e] = *(const f32x4 *)(t + (s + e < args.slices ? s + e : s) * slice_floats);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * i + e] = w[e];
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 16 / kPer; ++i) {
-        v[i] = 0;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            if (i * kPer + e < n) {
-                if constexpr (sizeof(OUT) == 4) v[i] = __float_as_uint(p[i]);
-                else v[i] |= (uint32_t)p[i * kPer + e] << (16 * e);
+                for (int e = 0; e < kAtOnce; ++e)
+                    if (s + e < args.slices) v += part[e];
             }
+        }
+        float piece[PIECES][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float rest = r + e < rank ? v[e] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < PIECES; ++c) {
+                piece[c][e] = rest;
+                const float top = bf16_bits_to_f32(f32_to_bf16(rest));
+                rest = __builtin_fabsf(top) < __builtin_inff() ? rest - top : 0.0f;
+            }
+        }
+        const int at = ((r >> 5) * blocks + (i >> 4)) * 64 + ((r >> 3) & 3) * 16 + (i & 15);
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c)
+            pieces[(c * panels * blocks * 64 + at) * 2 + ((r >> 2) & 1)] =
+                u32x2{f32x2_to_bf16x2(piece[c][0], piece[c][1]), f32x2_to_bf16x2(piece[c][2], piece[c][3])};
     }
 }
 
-template <int RB, typename OUT, bool ALIGNED>
-__device__ __attribute__((always_inline)) void up_rows(const AdapterArgs &args, const AdapterWeight &g, const ChunkRows &rows,
-                                        int64_t base, int column0, u32x2 *pieces) {
-    constexpr int kPieces = sizeof(OUT) == 4 ? 3 : 2, kPanels = kUpRanks / 32;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, q = lane >> 4;
-    const int n0 = column0 + wave * 64, columns = (int)g.w.rows, rank = rows.group_rank;
-    // The outputs to add to, asked for first.
-    OUT *out[RB];
-    bool live[RB];
-    uint32_t old[RB][16 * sizeof(OUT) / 4];
-    const int left = columns - n0 - q * 16;
-    const bool vector = (g.ldc * sizeof(OUT)) % 16 == 0 && ((uintptr_t)g.out & 15) == 0;
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        live[i] = i * 16 + m < rows.count;
-        const int at = rows.row_at(i * 16 + m);
-        out[i] = (OUT *)g.out + (base + (live[i] ? at : 0)) * g.ldc + n0 + q * 16;
-        load_out16<OUT>(out[i], live[i] ? left : 0, vector, old[i]);
-    }
-    const uint16_t *b = g.w.b + rows.group_slot * g.w.b_slot_stride;
-    const float scale = g.w.scales ? g.w.scales[rows.group_slot] : 1.0f;
-    f32x4 acc[RB][4];
-#pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    for (int rank0 = 0; rank0 < rank; rank0 += kUpRanks) {
-        u32x4 bs[kPanels][4];
-#pragma unroll
-        for (int p = 0; p < kPanels; ++p)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + (m >> 2) * 16 + j * 4 + (m & 3), r = rank0 + p * 32 + q * 8;
-                bs[p][j] = load8<ALIGNED>(b + (int64_t)n * g.w.b_row_stride + r, n < columns ? rank - r : 0);
-            }
-        if (rank0) __syncthreads();
-        // Four ranks of one row a thread: [piece][panel][row block][lane of the operand] x 16 bytes.
-        const int ranks = rank - rank0 < kUpRanks ? rank - rank0 : kUpRanks, quads = (ranks + 31) / 32 * 8;
-        for (int item = tid; item < RB * 16 * quads; item += 256) {
-            const int i = item / quads, r = (item % quads) * 4;
-            f32x4 v = {0, 0, 0, 0};
-            const int chunk_row = rows.row_at(i & 63);
-            if (i < rows.count && rank0 + r < rank) {
-                const float *t = args.t + (base + chunk_row) * args.t_cols + g.t_offset + rank0 + r;
-                for (int s = 0; s < args.slices; ++s) v += *(const f32x4 *)(t + (int64_t)s * args.rows * args.t_cols);
-            }
-            float piece[kPieces][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float rest = rank0 + r + e < rank ? v[e] * scale : 0.0f;
-#pragma unroll
-                for (int c = 0; c < kPieces; ++c) {
-                    piece[c][e] = rest;
-                    const float top = bf16_bits_to_f32(f32_to_bf16(rest));
-                    rest = __builtin_fabsf(top) < __builtin_inff() ? rest - top : 0.0f;
-                }
-            }
-            const int at = ((r >> 5) * RB + (i >> 4)) * 64 + ((r >> 3) & 3) * 16 + (i & 15);
-#pragma unroll
-            for (int c = 0; c < kPieces; ++c)
-                pieces[(c * kPanels * RB * 64 + at) * 2 + ((r >> 2) & 1)] =
-                    u32x2{f32x2_to_bf16x2(piece[c][0], piece[c][1]), f32x2_to_bf16x2(piece[c][2], piece[c][3])};
-        }
-        __syncthreads();
-#pragma unroll
-        for (int p = 0; p < kPanels; ++p) {
-            if (p * 32 >= ranks) break;
-#pragma unroll
-            for (int c = 0; c < kPieces; ++c)
-#pragma unroll
-                for (int i = 0; i < RB; ++i) {
-                    const u32x4 t = *(const u32x4 *)&pieces[(((c * kPanels + p) * RB + i) * 64 + lane) * 2];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(bs[p][j]), as_bf16x8(t), acc[i][j],
-                                                                             0, 0, 0);
-                }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        if (!live[i]) continue;
-        if constexpr (sizeof(OUT) == 4) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(old[i][4 * j + e]) + acc[i][j][e];
-                if (vector && left >= 16) *(f32x4 *)(out[i] + 4 * j) = v;
-                else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (4 * j + e < left) out[i][4 * j + e] = v[e];
-                }
-            }
-        } else {
-            uint32_t v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[e] = f32x2_to_bf16x2(bf16_bits_to_f32(old[i][e] & 0xffffu) + acc[i][e >> 1][2 * (e & 1)],
-                                       bf16_bits_to_f32(old[i][e] >> 16) + acc[i][e >> 1][2 * (e & 1) + 1]);
-            if (vector && left >= 16) {
-                *(u32x4 *)out[i] = u32x4{v[0], v[1], v[2], v[3]};
-                *(u32x4 *)(out[i] + 8) = u32x4{v[4], v[5], v[6], v[7]};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (e < left) out[i][e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-            }
-        }
-    }
-    __syncthreads();  // (the next adapter stages into the same LDS)
-}
-
-template <int RBMAX, typename OUT, bool ALIGNED>
-__global__ void __launch_bounds__(256, 2) adapter_up_kernel(AdapterArgs args) {
-    __shared__ u32x4 pieces[3 * (kUpRanks / 32) * RBMAX * 64];
-    const AdapterWeight &g = args.w[projection_of(args, blockIdx.x)];
-    const int column0 = ((int)blockIdx.x - g.first) * kUpColumns;
+// NP: panels of 32 ranks held in registers; 0: any number of them, read again for each block of rows.
+template <int NP, typename OUT, bool FAST>
+__global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(AdapterArgs args) {
+    constexpr int kPieces = sizeof(OUT) == 4 ? 3 : 2, kLoads = sizeof(OUT), kPer = 16 / sizeof(OUT), kHeld = NP ? NP : 1;
+    extern __shared__ u32x4 pieces[];
+    __shared__ float sums[4][16 * kUpSumStride];
+    const int which = blockIdx.z / args.turns, turn = blockIdx.z % args.turns;
+    const AdapterWeight &g = args.w[which];
+    const int column0 = (int)blockIdx.x * args.tiles * kUpColumns, columns = (int)g.w.rows;
+    if (column0 >= columns) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
     const int64_t base = (int64_t)blockIdx.y * kChunk;
-    ChunkRows rows(args, g.w, base);
-    while (rows.next(blockIdx.z, gridDim.z)) {
-        if (RBMAX == 1 || rows.count <= 16)
-            up_rows<1, OUT, ALIGNED>(args, g, rows, base, column0, (u32x2 *)pieces);
-        else if (rows.count <= 32)
-            up_rows<RBMAX == 1 ? 1 : 2, OUT, ALIGNED>(args, g, rows, base, column0, (u32x2 *)pieces);
-        else
-            up_rows<RBMAX, OUT, ALIGNED>(args, g, rows, base, column0, (u32x2 *)pieces);
+    const ChunkList &list = args.lists[which * (int64_t)gridDim.y + blockIdx.y];
+    const u32x2 record = *(const u32x2 *)&list.part[lane];
+    const int order = list.order[lane], parts = __builtin_popcountll(__ballot((record.y & 0xffffu) != 0));
+    OUT *out = (OUT *)g.out + base * g.ldc;
+    const rsrc_t ro = make_rsrc(out, FAST ? (uint32_t)(kChunk * g.ldc * sizeof(OUT)) : 0);
+    for (int part = turn; part < parts; part += args.turns) {
+        const int slot = __builtin_amdgcn_readlane(record.x, part);
+        const uint32_t rest = __builtin_amdgcn_readlane(record.y, part);
+        const int rank = rest & 0xffffu, first = (rest >> 16) & 0xffu, count = rest >> 24;
+        const int blocks = (count + 15) / 16, panels = (rank + 31) / 32;
+        const int mine = __builtin_amdgcn_ds_bpermute(((first + lane) & 63) * 4, order);
+        const uint16_t *b = g.w.b + slot * g.w.b_slot_stride;
+        const rsrc_t rb = make_rsrc(b, FAST ? (uint32_t)(g.w.rows * g.w.b_row_stride * 2) : 0);
+        for (int tile = 0; tile < args.tiles; ++tile) {
+            const int n0 = column0 + tile * kUpColumns + wave * 64;
+            if (n0 - wave * 64 >= columns) break;
+            u32x4 bs[kHeld][4];
+            auto load_b = [&](int p, u32x4(&v)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = n0 + j * 16 + m, r = p * 32 + q * 8;
+                    if constexpr (FAST)
+                        v[j] = buffer_load16(
+                            rb, n < columns && r < rank ? (uint32_t)((n * g.w.b_row_stride + r) * 2) : kNowhere, 0);
+                    else
+                        v[j] = load8(b + n * g.w.b_row_stride + r, n < columns ? rank - r : 0);
+                }
+            };
+            auto past_rank = [&](int p, u32x4(&v)[4]) {
+                if (FAST && (rank & 7)) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = keep8(v[j], rank - p * 32 - q * 8);
+                }
+            };
+#pragma unroll
+            for (int p = 0; p < NP; ++p) load_b(p, bs[p]);
+            if (tile == 0) {
+                __syncthreads();  // (the operands before them have been read)
+                stage_t<kPieces>(args, g, mine, count, blocks, base, rank, (u32x2 *)pieces);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int p = 0; p < NP; ++p) past_rank(p, bs[p]);
+#pragma unroll 1
+            for (int i = 0; i < blocks; ++i) {
+                // The outputs to add to: 16 bytes a lane, runs of 64 outputs of a row.
+                u32x4 old[kLoads];
+                uint32_t at[kLoads];
+                int row[kLoads];
+#pragma unroll
+                for (int c = 0; c < kLoads; ++c) {
+                    const int place = i * 16 + (c * 64 + lane) * kPer / 64, n = n0 + lane * kPer % 64;
+                    row[c] = __builtin_amdgcn_ds_bpermute(place * 4, mine);
+                    if (place >= count) row[c] = -1;
+                    if constexpr (FAST) {
+                        at[c] = row[c] >= 0 && n < columns ? (uint32_t)((row[c] * g.ldc + n) * sizeof(OUT)) : kNowhere;
+                        old[c] = buffer_load16(ro, at[c], 0);
+                    }
+                }
+                f32x4 acc[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = f32x4{0, 0, 0, 0};
+                auto multiply = [&](int p, const u32x4(&v)[4]) {
+#pragma unroll
+                    for (int c = 0; c < kPieces; ++c) {
+                        const u32x4 t = pieces[((c * panels + p) * blocks + i) * 64 + lane];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(v[j]), as_bf16x8(t), acc[j], 0, 0, 0);
+                    }
+                };
+                if constexpr (NP > 0) {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        if (p < panels) multiply(p, bs[p]);
+                } else {
+                    for (int p = 0; p < panels; ++p) {
+                        load_b(p, bs[0]);
+                        past_rank(p, bs[0]);
+                        multiply(p, bs[0]);
+                    }
+                }
+                // Column m of the MFMA is a row of the sums here, registers j, e its outputs 16 j + 4 q + e. (A
+                // wave's LDS operations are done in order.)
+                float *mine_sums = sums[wave];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *(f32x4 *)(mine_sums + m * kUpSumStride + j * 16 + q * 4) = acc[j];
+                wave_fence();
+#pragma unroll
+                for (int c = 0; c < kLoads; ++c) {
+                    const float *from = mine_sums + (c * 64 + lane) * kPer / 64 * kUpSumStride + lane * kPer % 64;
+                    f32x4 v[kPer / 4];
+#pragma unroll
+                    for (int e = 0; e < kPer / 4; ++e) v[e] = *(const f32x4 *)(from + 4 * e);
+                    if constexpr (FAST) {
+                        u32x4 w;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (sizeof(OUT) == 4)
+                                w[e] = __float_as_uint(__uint_as_float(old[c][e]) + v[0][e]);
+                            else
+                                w[e] = f32x2_to_bf16x2(bf16_bits_to_f32(old[c][e] & 0xffffu) + v[e >> 1][2 * (e & 1)],
+                                                       bf16_bits_to_f32(old[c][e] >> 16) + v[e >> 1][2 * (e & 1) + 1]);
+                        }
+                        __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)at[c], 0, 0);
+                    } else if (row[c] >= 0) {
+                        OUT *p = out + row[c] * g.ldc;
+#pragma unroll
+                        for (int e = 0; e < kPer; ++e) {
+                            const int n = n0 + lane * kPer % 64 + e;
+                            if (n >= columns) continue;
+                            if constexpr (sizeof(OUT) == 4) p[n] += v[0][e];
+                            else p[n] = f32_to_bf16(bf16_bits_to_f32(p[n]) + v[e >> 2][e & 3]);
+                        }
+                    }
+                }
+                wave_fence();
+            }
+        }
     }
 }
 
@@ -370,100 +409,133 @@ static int t_columns(const splosh_adapters *w, int group) {
     return cols;
 }
 
-static int down_columns(const splosh_adapters *w, int group) {
-    int columns = 0;
-    for (int i = 0; i < group; ++i) columns += (int)(w[i].max_rank + kDownRanks - 1) / kDownRanks;
-    return columns;
+static int down_columns(const splosh_adapters &w) { return (int)(w.max_rank + kDownRanks - 1) / kDownRanks; }
+static int64_t up_tiles(const splosh_adapters &w) { return (w.rows + kUpColumns - 1) / kUpColumns; }
+
+// Steps of 32 k a slice of K, whole rounds of the workgroup's waves: a workgroup a CU from the chunks and
+// projections alone, eight slices at most (the second launch adds them up; K17408, 64 rows of 28 adapters,
+// both launches: 4 slices 31.5 us, 8 24.6, 16 29.8).
+struct SlicePlan {
+    int steps, slices;
+};
+static SlicePlan plan_slices(const splosh_adapters *w, int group, int64_t rows) {
+    const int64_t chunks = (rows + kChunk - 1) / kChunk, steps = (w[0].inner + 31) / 32;
+    int64_t others = 0;
+    for (int i = 0; i < group; ++i) others += chunks * down_columns(w[i]);
+    int64_t want = (256 - 1 + others) / others;
+    want = want < 8 ? want : 8;
+    const int64_t rounds = (steps + kDownWaves - 1) / kDownWaves, per = (rounds + want - 1) / want;
+    return {(int)(per * kDownWaves), (int)((rounds + per - 1) / per)};
 }
 
-// Slices of K: 512 workgroups from the chunks and projections alone, of 16 steps of 32 or more each (four
-// a wave).
-static int plan_slices(const splosh_adapters *w, int group, int64_t rows) {
-    const int64_t chunks = (rows + kChunk - 1) / kChunk, steps = (w[0].inner + 31) / 32;
-    const int64_t want = (511 + chunks * down_columns(w, group)) / (chunks * down_columns(w, group));
-    int64_t slices = steps / 16 < want ? steps / 16 : want;
-    slices = slices < 32 ? slices : 32;
-    return slices < 1 ? 1 : (int)slices;
+static size_t lists_bytes(int group, int64_t rows) {
+    return (size_t)group * ((rows + kChunk - 1) / kChunk) * sizeof(ChunkList);
 }
 
 size_t adapters_workspace_bytes(const splosh_adapters *w, int group, int64_t rows) {
-    return kAdapterCounterBytes + (size_t)plan_slices(w, group, rows) * rows * t_columns(w, group) * sizeof(float);
+    return kAdapterCounterBytes + lists_bytes(group, rows) +
+           (size_t)plan_slices(w, group, rows).slices * rows * t_columns(w, group) * sizeof(float);
 }
 
-// The adapters of a chunk go to up to this many workgroups: all of its rows' where the launch is small, one
-// where it fills the device anyway.
-static unsigned turns(const splosh_adapters *w, int group, int64_t rows, int64_t others) {
-    int64_t most = rows < kChunk ? rows : kChunk, count = 1;
+// A chunk has this many adapters at most (rows and slots bound them).
+static int64_t most_parts(const splosh_adapters *w, int group, int64_t rows) {
+    int64_t count = 1;
     for (int i = 0; i < group; ++i) count = w[i].count > count ? w[i].count : count;
-    most = count < most ? count : most;
-    const int64_t n = 4096 / others;
-    return (unsigned)(n < 1 ? 1 : n < most ? n : most);
+    const int64_t most = rows < kChunk ? rows : kChunk;
+    return count < most ? count : most;
 }
 
-template <int RBMAX, bool ALIGNED>
+// The adapters of a chunk go to up to this many workgroups: each its own where the launch is small, one for
+// all where it fills the device anyway.
+static int plan_turns(int64_t parts, int64_t others) {
+    const int64_t n = 2048 / others;
+    return (int)(n < 1 ? 1 : n < parts ? n : parts);
+}
+
+template <int RB, bool FAST>
 static void launch_down(const AdapterArgs &args, int panels, dim3 grid, hipStream_t stream) {
-    if (panels == 1) hipLaunchKernelGGL((adapter_down_kernel<RBMAX, 1, ALIGNED>), grid, dim3(256), 0, stream, args);
-    else if (panels == 2) hipLaunchKernelGGL((adapter_down_kernel<RBMAX, 2, ALIGNED>), grid, dim3(256), 0, stream, args);
-    else hipLaunchKernelGGL((adapter_down_kernel<RBMAX, 4, ALIGNED>), grid, dim3(256), 0, stream, args);
+    if (panels == 1) hipLaunchKernelGGL((adapter_down_kernel<RB, 1, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
+    else if (panels == 2) hipLaunchKernelGGL((adapter_down_kernel<RB, 2, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
+    else hipLaunchKernelGGL((adapter_down_kernel<RB, 4, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
 }
 
-template <int RBMAX, typename OUT>
-static void launch_up(const AdapterArgs &args, bool aligned, dim3 grid, hipStream_t stream) {
-    if (aligned) hipLaunchKernelGGL((adapter_up_kernel<RBMAX, OUT, true>), grid, dim3(256), 0, stream, args);
-    else hipLaunchKernelGGL((adapter_up_kernel<RBMAX, OUT, false>), grid, dim3(256), 0, stream, args);
+// LDS of the operands: three pieces (of an fp32 output) of whole panels of ranks for a chunk's rows; past the
+// default limit of 64 KB with what the kernel has of its own, the limit is raised once.
+constexpr int kUpMaxLds = 3 * (SPLOSH_MAX_RANK / 32) * (kChunk / 16) * 1024;
+
+template <int NP, typename OUT, bool FAST>
+static hipError_t launch_up(const AdapterArgs &args, int lds, dim3 grid, hipStream_t stream) {
+    if (NP == 0) {
+        static const hipError_t raised = hipFuncSetAttribute((const void *)adapter_up_kernel<NP, OUT, FAST>,
+                                                             hipFuncAttributeMaxDynamicSharedMemorySize, kUpMaxLds);
+        if (raised != hipSuccess) return raised;
+    }
+    hipLaunchKernelGGL((adapter_up_kernel<NP, OUT, FAST>), grid, dim3(256), lds, stream, args);
+    return hipGetLastError();
+}
+template <typename OUT>
+static hipError_t launch_up(const AdapterArgs &args, int panels, bool fast, int lds, dim3 grid, hipStream_t stream) {
+    if (!fast) return launch_up<0, OUT, false>(args, lds, grid, stream);
+    if (panels == 1) return launch_up<1, OUT, true>(args, lds, grid, stream);
+    if (panels == 2) return launch_up<2, OUT, true>(args, lds, grid, stream);
+    return launch_up<0, OUT, true>(args, lds, grid, stream);
 }
 
 hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *x, int64_t ldx, void *const *outs,
                            const int64_t *ldcs, int out_dtype, const int32_t *slots, int64_t rows, void *workspace,
                            hipStream_t stream) {
     AdapterArgs args{};
-    args.group = group;
     args.x = x;
     args.ldx = ldx;
     args.slots = slots;
-    args.t = (float *)((char *)workspace + kAdapterCounterBytes);
+    args.lists = (ChunkList *)((char *)workspace + kAdapterCounterBytes);
+    args.t = (float *)((char *)workspace + kAdapterCounterBytes + lists_bytes(group, rows));
     args.t_cols = t_columns(w, group);
-    args.slices = plan_slices(w, group, rows);
+    const SlicePlan plan = plan_slices(w, group, rows);
+    args.slices = plan.slices;
+    args.slice_steps = plan.steps;
     args.rows = rows;
+    const int64_t esize = out_dtype == SPLOSH_F32 ? 4 : 2;
     auto aligned16 = [](const void *p, int64_t a, int64_t b) { return (uintptr_t)p % 16 == 0 && a % 8 == 0 && b % 8 == 0; };
-    bool down_aligned = aligned16(x, ldx, 0), up_aligned = true;
+    auto near = [](int64_t elements, int64_t size) { return elements < (int64_t)kNowhere / size; };
+    bool down_fast = aligned16(x, ldx, w[0].inner) && near(kChunk * ldx, 2), up_fast = true;
     int at = 0, columns = 0;
-    int64_t most_rank = 0;
+    int64_t most_rank = 0, tiles = 0, most_tiles = 0;
     for (int i = 0; i < group; ++i) {
-        args.w[i] = AdapterWeight{w[i], outs[i], ldcs[i], at, columns};
+        args.w[i] = AdapterWeight{w[i], outs[i], ldcs[i], at};
         at += (int)(w[i].max_rank + 15) / 16 * 16;
-        columns += (int)(w[i].max_rank + kDownRanks - 1) / kDownRanks;
+        columns = columns > down_columns(w[i]) ? columns : down_columns(w[i]);
         most_rank = w[i].max_rank > most_rank ? w[i].max_rank : most_rank;
-        down_aligned = down_aligned && aligned16(w[i].a, w[i].a_slot_stride, w[i].a_row_stride);
-        up_aligned = up_aligned && aligned16(w[i].b, w[i].b_slot_stride, w[i].b_row_stride);
+        tiles += up_tiles(w[i]);
+        most_tiles = up_tiles(w[i]) > most_tiles ? up_tiles(w[i]) : most_tiles;
+        down_fast = down_fast && aligned16(w[i].a, w[i].a_slot_stride, w[i].a_row_stride) &&
+                    near(w[i].max_rank * w[i].a_row_stride, 2);
+        up_fast = up_fast && (uintptr_t)outs[i] % 16 == 0 && ldcs[i] * esize % 16 == 0 && w[i].rows % 16 == 0 &&
+                  w[i].max_rank % 8 == 0 && near(kChunk * ldcs[i], esize) &&
+                  aligned16(w[i].b, w[i].b_slot_stride, w[i].b_row_stride) && near(w[i].rows * w[i].b_row_stride, 2);
     }
     const unsigned chunks = (unsigned)((rows + kChunk - 1) / kChunk);
     const unsigned down_x = (unsigned)(columns * args.slices);
-    const dim3 down(down_x, chunks, turns(w, group, rows, (int64_t)down_x * chunks));
+    const int64_t parts = most_parts(w, group, rows);
+    args.turns = plan_turns(parts, (int64_t)down_x * chunks * group);
+    const dim3 down(down_x, chunks, (unsigned)(group * args.turns));
     const int panels = most_rank <= 16 ? 1 : most_rank <= 32 ? 2 : 4;
-    if (rows <= 16) {
-        if (down_aligned) launch_down<1, true>(args, panels, down, stream);
-        else launch_down<1, false>(args, panels, down, stream);
-    } else {
-        if (down_aligned) launch_down<4, true>(args, panels, down, stream);
-        else launch_down<4, false>(args, panels, down, stream);
-    }
+    if (!down_fast) launch_down<1, false>(args, panels, down, stream);
+    else if (rows <= 16) launch_down<1, true>(args, panels, down, stream);
+    else launch_down<4, true>(args, panels, down, stream);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    unsigned up_x = 0;
-    for (int i = 0; i < group; ++i) {
-        args.w[i].first = (int)up_x;
-        up_x += (unsigned)((w[i].rows + kUpColumns - 1) / kUpColumns);
-    }
-    const dim3 up(up_x, chunks, turns(w, group, rows, (int64_t)up_x * chunks));
-    if (rows <= 16) {
-        if (out_dtype == SPLOSH_F32) launch_up<1, float>(args, up_aligned, up, stream);
-        else launch_up<1, uint16_t>(args, up_aligned, up, stream);
-    } else {
-        if (out_dtype == SPLOSH_F32) launch_up<4, float>(args, up_aligned, up, stream);
-        else launch_up<4, uint16_t>(args, up_aligned, up, stream);
-    }
-    return hipGetLastError();
+    // Tiles a workgroup, for which t is staged once: so many that six workgroups a CU are left (2048 rows,
+    // N17408: 33.4 us, with three a CU 35.7).
+    const int64_t share = (tiles * chunks * (chunks == 1 ? parts : 1) + 1535) / 1536;
+    args.tiles = (int)(share < most_tiles ? share : most_tiles);
+    const unsigned up_x = (unsigned)((most_tiles + args.tiles - 1) / args.tiles);
+    args.turns = plan_turns(parts, (int64_t)up_x * chunks * group);
+    const dim3 up(up_x, chunks, (unsigned)(group * args.turns));
+    const int up_panels = (int)(most_rank + 31) / 32, blocks = rows < kChunk ? (int)(rows + 15) / 16 : kChunk / 16;
+    const int lds = (out_dtype == SPLOSH_F32 ? 3 : 2) * up_panels * blocks * 1024;
+    return out_dtype == SPLOSH_F32 ? launch_up<float>(args, up_panels, up_fast, lds, up, stream)
+                                   : launch_up<uint16_t>(args, up_panels, up_fast, lds, up, stream);
 }
 
 }  // namespace splosh
