@@ -7,21 +7,22 @@
 // complement of the index. Weights are integers (2^40 for the largest logit of what they are measured
 // against), so that their sums do not depend on the order of the additions.
 //
-// Two launches over pieces of 8192 logits, a workgroup each, the last of a row's to arrive going on with
-// the row (no workgroup waits for another):
-//   scan    -- a piece's largest logit and its weight, and for rows with a cut how many elements and how
-//              much weight fall into each of 512 value bins below its largest. The row: greedy ones and
-//              those with the temperature alone are settled here, from one piece more; else the bins that
-//              the cut can be in.
-//   collect -- the weight above these bins, and the elements in them as a list. The row: the list sorted,
-//              the cut found on running sums, the piece the draw falls into and the token in it.
-// A row whose cut lies below its bins, or in bins of more elements than the list holds, is settled by one
-// workgroup with a radix search over the whole row.
+// Four launches; a workgroup takes a piece of 8192 logits, or a row:
+//   scan    (pieces) the piece's largest logit and its weight, and for rows with a cut how many elements
+//           and how much weight fall into each of 512 value bins below its largest;
+//   settle  (rows)   greedy rows and those with the temperature alone are settled, from one piece more;
+//           for the others, the bins that the cut can be in;
+//   collect (pieces) the weight above these bins, and the elements in them as a list;
+//   finish  (rows)   the cut, by a radix search in the list, the piece the draw falls into and the token
+//           in it. A row whose cut lies below its bins, or in bins of more elements than the list
+//           holds, is searched whole.
+// The launches over pieces hold nothing but what they stream, so that four workgroups share a CU.
 #include "common.hpp"
 #include "launch.hpp"
 
 namespace splosh {
 
+// The workspace's first 16 KiB belong to the arrival counters of the kernels that have any.
 constexpr size_t kSampleCounterBytes = 16384;
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kPer = 16;                     // logits a thread
@@ -56,18 +57,34 @@ __device__ __forceinline__ u64 order_key(float v, uint32_t index) {
     return key ? (u64)key << 32 | (0xffffffffu - index) : 0;
 }
 
-// exp((v - top) / T) in units of 2^-40, c = log2(e) / T: the exponent in 64 bits, its fraction's power
-// by the hardware's (1 ulp of fp32, 2^-24 .. 2^-23 relative). The largest logit weighs 2^40 also where
-// it is infinite.
-__device__ __forceinline__ u64 logit_weight(float v, float top, double c) {
-    if (v == top) return (u64)1 << kWeightBits;
-    const double t = ((double)v - (double)top) * c;
-    if (!(t > -(kWeightBits + 2.0))) return 0;
-    const double n = __builtin_rint(t);
-    const uint32_t e = (uint32_t)(__builtin_amdgcn_exp2f((float)(t - n)) * 16777216.0f);
-    const int shift = (int)n + kWeightBits - 24;
-    return shift >= 0 ? (u64)e << shift : (u64)(((e >> (-shift - 1)) + 1) >> 1);
-}
+// exp((v - top) / T) in units of 2^-40, downwards, c = log2(e) / T. The exponent (v - s) c - (top - s) c is kept
+// in two fp32 numbers (its product's rounding error by an fma, c in two as well), of which the larger one's
+// whole part is the shift; the fraction's power is the hardware's (1 ulp). s is 0, and top where the exponent
+// at top is so large that its fraction would be lost: then v - top is exact for every v that has weight.
+struct Weights {
+    float top, s, c_high, c_low, whole, fraction;
+
+    __device__ __forceinline__ Weights(float top_, double c) : top(top_) {
+        double at = (double)top * c;
+        s = 0.0f;
+        if (!(__builtin_fabs(at) < (double)(1 << 21))) s = top, at = 0.0;
+        c_high = (float)c;
+        c_low = c_high < __builtin_inff() ? (float)(c - (double)c_high) : 0.0f;
+        const double n = __builtin_rint(at);
+        whole = (float)n;
+        fraction = (float)(at - n);
+    }
+    __device__ __forceinline__ u64 operator()(float v) const {
+#pragma clang fp contract(off)  // (high is the rounded product wherever it stands)
+        const float d = v - s, high = d * c_high;
+        const float low = __builtin_fmaf(d, c_low, __builtin_fmaf(d, c_high, -high));
+        const float n = __builtin_rintf(high), left = n - whole;  // (left: at most 1)
+        const float e = __builtin_amdgcn_exp2f(((high - n) + low) - fraction);
+        const int shift = 1 - (int)left;
+        const u64 w = ((u64)(uint32_t)(e * 16777216.0f) << (kWeightBits - 23)) >> (shift > 0 ? shift : 0);
+        return v == top ? (u64)1 << kWeightBits : left > -(kWeightBits + 4.0f) ? w : 0;
+    }
+};
 
 // w >= q for min-p, low = log2(q).
 __device__ __forceinline__ bool weighs(float v, float top, double c, double low) {
@@ -82,27 +99,40 @@ __device__ __forceinline__ int value_bin(float v) {
 }
 
 // ---- across a workgroup ---------------------------------------------------------------------------
+//
+// Reductions and running sums over the lanes by DPP moves (a move within a row of 16, then its last lane to
+// the rows after it), over the waves through LDS. Zero is neutral in all of them.
 
-template <typename V>
-__device__ __forceinline__ V shuffle_xor(V v, int d) {
-    if constexpr (sizeof(V) == 8) return (V)__shfl_xor((u64)v, d, 64);
-    else return __shfl_xor(v, d, 64);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_move(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_move(u64 v) {
+    return (u64)dpp_move<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp_move<CTRL, ROWS>((uint32_t)v);
 }
 struct MaxOp {
     template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
-struct MinOp {
-    template <typename V> __device__ V operator()(V a, V b) const { return a < b ? a : b; }
-};
 struct SumOp {
     template <typename V> __device__ V operator()(V a, V b) const { return a + b; }
 };
+// Over the lanes up to this one; lane 63 has the wave's.
+template <typename V, typename F>
+__device__ __forceinline__ V wave_scan(V v, F op) {
+    v = op(v, dpp_move<0x111, 0xf>(v));
+    v = op(v, dpp_move<0x112, 0xf>(v));
+    v = op(v, dpp_move<0x114, 0xf>(v));
+    v = op(v, dpp_move<0x118, 0xf>(v));
+    v = op(v, dpp_move<0x142, 0xa>(v));
+    v = op(v, dpp_move<0x143, 0xc>(v));
+    return v;
+}
 template <typename V, typename F>
 __device__ __forceinline__ V block_reduce(V v, F op, u64 *scratch) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = op(v, shuffle_xor(v, d));
+    v = wave_scan(v, op);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = (u64)v;
+    if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = (u64)v;
     __syncthreads();
     v = (V)scratch[0];
 #pragma unroll
@@ -111,14 +141,10 @@ __device__ __forceinline__ V block_reduce(V v, F op, u64 *scratch) {
 }
 // The sum over the threads up to this one.
 __device__ __forceinline__ u64 block_scan(u64 v, u64 *scratch) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 up = __shfl_up(v, d, 64);
-        if (lane >= d) v += up;
-    }
+    const int wave = threadIdx.x >> 6;
+    v = wave_scan(v, SumOp());
     __syncthreads();
-    if (lane == 63) scratch[wave] = v;
+    if ((threadIdx.x & 63) == 63) scratch[wave] = v;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kWaves - 1; ++i)
@@ -127,16 +153,6 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 *scratch) {
 }
 
 // ---- what the launches leave for each other ---------------------------------------------------------
-//
-// What a workgroup of the same launch reads is written and read past the L2s (agent scope), which are one an
-// XCD and not coherent.
-
-__device__ __forceinline__ void put(u64 *p, u64 v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ u64 get(const u64 *p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 
 enum RowState : int { kSettled = 0, kCollect = 1, kSearch = 2 };
 
@@ -146,9 +162,9 @@ struct RowPlan {
     u64 total;         // the whole row's weight, of the largest logit
     uint32_t above;    // elements in the bins above the list's
     uint32_t listed;   // elements of the list so far
-    uint32_t valid, reserved;
+    uint32_t valid, reserved;  // valid: elements that can be chosen
 };
-// A piece. key: its largest logit's << 32 | the index of that.
+// A piece. key: its largest logit's << 32 | the index of that (greedy rows).
 struct PieceHead {
     u64 key, weight, valid;  // scan: its weight, of its own largest logit; its elements that can be chosen
     u64 above, kept;         // collect: the weight above the list's bins, and of it what min-p leaves
@@ -165,7 +181,6 @@ struct SampleArgs {
     SampleParams p;
     uint32_t *tokens;
     float *logprobs;
-    int *arrivals;
     char *rows;
     size_t row_bytes;
 };
@@ -212,19 +227,6 @@ __device__ __forceinline__ u64 draw_of(float u, u64 total) {
     return target < total ? target : total - 1;
 }
 
-// The last workgroup of `parts` to arrive. What each has put before is then there for it.
-__device__ __forceinline__ bool last_to_arrive(int *counter, int parts, int *shared) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (old == parts - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *shared = old;
-    }
-    __syncthreads();
-    return *shared == parts - 1;
-}
-
 // A thread's sixteen logits of the piece at `base`: v, and their indexes through index_of. Past the vocabulary
 // and NaN: -inf. VECTOR: rows whose 16-byte pieces are aligned.
 template <typename T, bool VECTOR>
@@ -232,48 +234,53 @@ __device__ __forceinline__ int index_of(int e) {
     constexpr int kRun = VECTOR ? 16 / (int)sizeof(T) : 1;
     return e / kRun * (kThreads * kRun) + (int)threadIdx.x * kRun + e % kRun;
 }
+template <typename T, bool VECTOR, int RUN>
+__device__ __forceinline__ void load_run(const T *row, int i, int vocab, float *v) {
+    if (VECTOR && i + RUN <= vocab) {
+        const u32x4 w = *(const u32x4 *)(row + i);
+#pragma unroll
+        for (int j = 0; j < RUN; ++j)
+            v[j] = sizeof(T) == 4 ? __uint_as_float(w[j & 3])
+                                  : bf16_bits_to_f32(j & 1 ? w[(j >> 1) & 3] >> 16 : w[(j >> 1) & 3] & 0xffffu);
+    } else {
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) v[j] = i + j < vocab ? logit_of(row[i + j]) : -__builtin_inff();
+    }
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) v[j] = v[j] != v[j] ? -__builtin_inff() : v[j];
+}
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void load_piece(const T *row, int base, int vocab, float (&v)[kPer]) {
     constexpr int kRun = VECTOR ? 16 / (int)sizeof(T) : 1;
 #pragma unroll
-    for (int e = 0; e < kPer; e += kRun) {
-        const int i = base + index_of<T, VECTOR>(e);
-        if (VECTOR && i + kRun <= vocab) {
-            const u32x4 w = *(const u32x4 *)(row + i);
-#pragma unroll
-            for (int j = 0; j < kRun; ++j)
-                v[e + j] = sizeof(T) == 4 ? __uint_as_float(w[j & 3])
-                                          : bf16_bits_to_f32(j & 1 ? w[(j >> 1) & 3] >> 16 : w[(j >> 1) & 3] & 0xffffu);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kRun; ++j) v[e + j] = i + j < vocab ? logit_of(row[i + j]) : -__builtin_inff();
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = v[e] != v[e] ? -__builtin_inff() : v[e];
+    for (int e = 0; e < kPer; e += kRun)
+        load_run<T, VECTOR, kRun>(row, base + index_of<T, VECTOR>(e), vocab, &v[e]);
 }
 
 struct Shared {
     u64 scratch[kWaves];
-    int arrival;
     int chosen;
     u64 rest;
     int cuts[4];
     u64 weights[4];
 };
 
-// The token of a settled piece: the first index of the piece whose running weight over the kept elements
-// (order key >= cut, weight of `top` at least 2^low) exceeds `target`. probability: its weight times `scale`.
-template <typename T>
-__device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int piece, float top, double c, u64 cut,
-                                       double low, u64 target, double scale, Shared &sh) {
+// The token of the row: the first index of the piece whose running weight over the kept elements (order key
+// >= cut, weight of the row's largest at least 2^low) exceeds `target`. Its probability: its weight times scale.
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int piece, float top, double c,
+                                       u64 cut, double low, u64 target, double scale, Shared &sh) {
+    constexpr int kRun = 16 / (int)sizeof(T);
     const int first = piece * kPiece + (int)threadIdx.x * kPer;
+    const Weights weigh(top, c);
+    float v[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; e += kRun) load_run<T, VECTOR, kRun>(row, first + e, args.vocab, &v[e]);
     u64 w[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        const float v = first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
-        const u64 key = order_key(v, first + e);
-        w[e] = key && key >= cut && weighs(v, top, c, low) ? logit_weight(v, top, c) : 0;
+        const u64 key = order_key(v[e], first + e);
+        w[e] = key && key >= cut && weighs(v[e], top, c, low) ? weigh(v[e]) : 0;
         sum += w[e];
     }
     u64 run = block_scan(sum, sh.scratch) - sum;
@@ -302,166 +309,85 @@ __device__ __forceinline__ u64 choose_piece(u64 weight, float u, Shared &sh) {
     return total;
 }
 
-// ---- the radix search over a whole row ---------------------------------------------------------------
-
-constexpr int kDigitBits = 11;
-
-// The smallest run from the start of the order, of keys >= limit, with `k` elements, or with weight >= share
-// where k is 0: its last key; *weight its weight. counts and sums: 2^kDigitBits each.
-template <typename T>
-__device__ __noinline__ u64 find_cut(const T *row, int vocab, float top, double c, u64 limit, u64 k, double share,
-                                     u64 *weight, uint32_t *counts, u64 *sums, Shared &sh) {
-    const int tid = threadIdx.x;
-    u64 prefix = 0, base_weight = 0, base_count = 0;
-    for (int shift = 64 - kDigitBits, bits = kDigitBits;; shift -= bits) {
-        const u64 above = shift + bits >= 64 ? 0 : ~(u64)0 << (shift + bits);
-        for (int d = tid; d < 1 << bits; d += kThreads) counts[d] = 0, sums[d] = 0;
-        __syncthreads();
-        for (int i = tid; i < vocab; i += kThreads) {
-            const float v = logit_of(row[i]);
-            const u64 key = order_key(v, i);
-            if (key == 0 || key < limit || ((key ^ prefix) & above)) continue;
-            const int d = (int)(key >> shift) & ((1 << bits) - 1);
-            atomicAdd(&counts[d], 1u);
-            atomicAdd(&sums[d], logit_weight(v, top, c));
-        }
-        __syncthreads();
-        // The digits from the largest down, a run of them a thread; the first that the run can end in, or where
-        // rounding leaves none the last there is.
-        const int per = (1 << bits) / kThreads, high = (1 << bits) - 1 - tid * per;
-        u64 own_count = 0, own_weight = 0;
-        for (int d = high; d > high - per; --d) own_count += counts[d], own_weight += sums[d];
-        u64 n = base_count + block_scan(own_count, sh.scratch) - own_count;
-        u64 w = base_weight + block_scan(own_weight, sh.scratch) - own_weight;
-        if (tid == 0) sh.cuts[0] = -1, sh.cuts[1] = 1 << bits;
-        __syncthreads();
-        for (int pass = 0; pass < 2; ++pass) {
-            for (int d = high; d > high - per; --d) {
-                if (counts[d] == 0) continue;
-                const bool before = (k ? n >= k : (double)w >= share) && n != base_count;
-                n += counts[d];
-                w += sums[d];
-                if (pass == 0) atomicMin(&sh.cuts[1], d);
-                if (pass == 0 ? !before && (k ? n >= k : (double)w >= share) : d == sh.cuts[1]) {
-                    sh.cuts[0] = d;
-                    sh.weights[0] = w - sums[d];
-                    sh.weights[1] = n - counts[d];
-                    sh.weights[2] = w;
-                }
-            }
-            __syncthreads();
-            if (sh.cuts[0] >= 0) break;
-        }
-        if (tid == 0) sh.rest = prefix | (u64)sh.cuts[0] << shift;
-        __syncthreads();
-        prefix = sh.rest;
-        base_weight = sh.weights[0];
-        base_count = sh.weights[1];
-        *weight = sh.weights[2];
-        if (shift == 0) return prefix;
-        if (shift < kDigitBits) bits = shift;
-    }
-}
-
-template <typename T>
-__device__ __noinline__ void search_row(const SampleArgs &args, int64_t r, const T *row, const RowPlan &plan,
-                                        const RowParams &rp, u64 *memory, Shared &sh) {
-    uint32_t *counts = (uint32_t *)memory;
-    u64 *sums = memory + (1 << kDigitBits) / 2;
-    const float top = key_logit(plan.top_key);
-    const double low = rp.low();
-    u64 cut = 1, weight = plan.total;
-    if (rp.k && (uint32_t)rp.k < plan.valid)
-        cut = find_cut(row, args.vocab, top, rp.c, cut, (u64)rp.k, 0.0, &weight, counts, sums, sh);
-    if (rp.p < 1.0f)
-        cut = find_cut(row, args.vocab, top, rp.c, cut, 0, (double)rp.p * (double)weight, &weight, counts, sums, sh);
-    // The pieces' kept weights, thread by thread.
-    u64 mine = 0;
-    for (int piece = 0; piece < args.pieces; ++piece) {
-        float v[kPer];
-        load_piece<T, false>(row, piece * kPiece, args.vocab, v);
-        u64 kept = 0;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const u64 key = order_key(v[e], piece * kPiece + index_of<T, false>(e));
-            if (key && key >= cut && weighs(v[e], top, rp.c, low)) kept += logit_weight(v[e], top, rp.c);
-        }
-        kept = block_reduce(kept, SumOp(), sh.scratch);
-        if ((int)threadIdx.x == piece) mine = kept;
-    }
-    const u64 total = choose_piece(mine, rp.u, sh);
-    locate<T>(args, r, row, sh.chosen, top, rp.c, cut, low, sh.rest, 1.0 / (double)total, sh);
-}
-
 // ---- scan -------------------------------------------------------------------------------------------
+
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) {
+    __shared__ u64 scratch[kWaves];
+    __shared__ u64 bins[kBins];
+    const int tid = threadIdx.x, piece = blockIdx.x;
+    const int64_t r = blockIdx.y;
+    float v[kPer];
+    load_piece<T, VECTOR>((const T *)args.logits + r * args.ld, piece * kPiece, args.vocab, v);
+    const RowParams rp = row_params(args, r);
+    const bool cut = !rp.greedy && (rp.k || rp.p < 1.0f);
+    RowScratch &row = row_scratch(args, (int)r);
+    if (cut) bins[tid] = 0;
+    float best = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) best = __builtin_fmaxf(best, v[e]);
+    const uint32_t best_key = block_reduce(logit_key(best), MaxOp(), scratch);
+    u64 weight = 0, index = 0;
+    uint32_t valid = 0;
+    const float top = key_logit(best_key);
+    if (rp.greedy) {
+        uint32_t at = 0;  // (the complement: the first index is the largest)
+#pragma unroll
+        for (int e = kPer - 1; e >= 0; --e)
+            if (v[e] == top) at = ~(uint32_t)(piece * kPiece + index_of<T, VECTOR>(e));
+        index = ~block_reduce(at, MaxOp(), scratch);
+    } else if (best_key) {
+        const int top_bin = value_bin(top);
+        const Weights weigh(top, rp.c);
+        if (cut) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const u64 w = weigh(v[e]);
+                weight += w;
+                const bool live = v[e] > -__builtin_inff();
+                valid += __builtin_popcountll(__ballot(live));
+                const int below = top_bin - value_bin(v[e]);
+                if (live && below < kBins) atomicAdd(&bins[below], (u64)1 << kBinShift | w >> kBinUnit);
+            }
+            valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) weight += weigh(v[e]);
+        }
+        weight = block_reduce(weight, SumOp(), scratch);
+    }
+    if (tid == 0) {
+        row.heads[piece].key = (u64)best_key << 32 | index;
+        row.heads[piece].weight = weight;
+        row.heads[piece].valid = valid;
+    }
+    if (cut) row_bins(args, row)[(size_t)piece * kBins + tid] = bins[tid];
+}
+
+// ---- settle -----------------------------------------------------------------------------------------
 
 // 2^t for t <= 0, in 64 bits.
 __device__ __forceinline__ double power_of(double t) { return t > -1000.0 ? exp2(t) : 0.0; }
 
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) {
+__global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args) {
     __shared__ Shared sh;
-    __shared__ u64 bins[kBins];
-    const int tid = threadIdx.x, piece = blockIdx.x;
-    const int64_t r = blockIdx.y;
-    const T *row = (const T *)args.logits + r * args.ld;
-    float v[kPer];
-    load_piece<T, VECTOR>(row, piece * kPiece, args.vocab, v);
-    const RowParams rp = row_params(args, r);
-    const bool cut = !rp.greedy && (rp.k || rp.p < 1.0f);
-    RowScratch &scratch = row_scratch(args, (int)r);
-    bins[tid] = 0;
-    uint32_t best = 0;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const uint32_t key = logit_key(v[e]);
-        best = best > key ? best : key;
-    }
-    best = block_reduce(best, MaxOp(), sh.scratch);
-    u64 weight = 0, valid = 0, index = 0;
-    if (rp.greedy) {
-        uint32_t at = 0xffffffffu;
-#pragma unroll
-        for (int e = kPer - 1; e >= 0; --e)
-            if (logit_key(v[e]) == best) at = (uint32_t)(piece * kPiece + index_of<T, VECTOR>(e));
-        index = block_reduce(at, MinOp(), sh.scratch);
-    } else if (best) {
-        const float top = key_logit(best);
-        const int top_bin = value_bin(top);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const u64 w = logit_weight(v[e], top, rp.c);
-            weight += w;
-            if (cut && logit_key(v[e])) {
-                ++valid;
-                const int below = top_bin - value_bin(v[e]);
-                if (below < kBins) atomicAdd(&bins[below], (u64)1 << kBinShift | w >> kBinUnit);
-            }
-        }
-        // (Sixteen times 512 weights of 2^40 at most, and 2^13 elements: one sum of both.)
-        weight = block_reduce(weight, SumOp(), sh.scratch);
-        if (cut) valid = block_reduce(valid, SumOp(), sh.scratch);
-    }
-    if (tid == 0) {
-        put(&scratch.heads[piece].key, (u64)best << 32 | index);
-        put(&scratch.heads[piece].weight, weight);
-        put(&scratch.heads[piece].valid, valid);
-    }
-    u64 *all_bins = row_bins(args, scratch);
-    if (cut) put(&all_bins[(size_t)piece * kBins + tid], bins[tid]);
-    if (!last_to_arrive(args.arrivals + r, args.pieces, &sh.arrival)) return;
-
-    // The row: one piece a thread.
     __shared__ float factors[kThreads];  // the pieces' weights in the row's
     __shared__ int top_bins[kThreads];
-    const u64 key = tid < args.pieces ? get(&scratch.heads[tid].key) : 0;
-    const u64 piece_weight = tid < args.pieces ? get(&scratch.heads[tid].weight) : 0;
-    const u64 piece_valid = tid < args.pieces ? get(&scratch.heads[tid].valid) : 0;
-    const uint32_t top_key = block_reduce((uint32_t)(key >> 32), MaxOp(), sh.scratch);
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const T *row = (const T *)args.logits + r * args.ld;
+    RowScratch &scratch = row_scratch(args, (int)r);
+    const RowParams rp = row_params(args, r);
+    const bool cut = !rp.greedy && (rp.k || rp.p < 1.0f);
+    // One piece a thread.
+    PieceHead head = {0, 0, 0, 0, 0};
+    if (tid < args.pieces) head.key = scratch.heads[tid].key, head.weight = scratch.heads[tid].weight, head.valid = scratch.heads[tid].valid;
+    const uint32_t piece_key = (uint32_t)(head.key >> 32), top_key = block_reduce(piece_key, MaxOp(), sh.scratch);
     RowPlan &plan = scratch.plan;
     if (rp.greedy || top_key == 0) {
-        // The first piece that has the largest has its first index.
-        const uint32_t at = block_reduce((uint32_t)(key >> 32) == top_key ? (uint32_t)key : 0xffffffffu, MinOp(), sh.scratch);
+        // Of the pieces that have the largest, the first index.
+        const uint32_t at = ~block_reduce(piece_key == top_key ? ~(uint32_t)head.key : 0u, MaxOp(), sh.scratch);
         if (tid == 0) {
             args.tokens[r] = top_key ? at : 0xffffffffu;
             if (args.logprobs) args.logprobs[r] = top_key ? 0.0f : -__builtin_inff();
@@ -469,43 +395,47 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
         }
         return;
     }
-    const float top = key_logit(top_key), piece_top = key_logit((uint32_t)(key >> 32));
-    const double factor = key >> 32 == 0 ? 0.0
-                          : piece_top == top ? 1.0 : power_of(((double)piece_top - (double)top) * rp.c);
-    const u64 row_weight = (u64)((double)piece_weight * factor);
+    const float top = key_logit(top_key), piece_top = key_logit(piece_key);
+    const double factor = piece_key == 0 ? 0.0
+                          : piece_key == top_key ? 1.0 : power_of(((double)piece_top - (double)top) * rp.c);
+    const u64 row_weight = (u64)((double)head.weight * factor);
     if (!cut && rp.q == 0.0f) {  // the temperature alone
         const u64 total = choose_piece(row_weight, rp.u, sh);
         __shared__ double chosen_factor;
-        __shared__ u64 chosen_weight, chosen_key;
-        if (tid == sh.chosen) chosen_factor = factor, chosen_weight = piece_weight, chosen_key = key;
+        __shared__ u64 chosen_weight;
+        __shared__ uint32_t chosen_key;
+        if (tid == sh.chosen) chosen_factor = factor, chosen_weight = head.weight, chosen_key = piece_key;
         __syncthreads();
         u64 target = (u64)((double)sh.rest / chosen_factor);
         target = target < chosen_weight ? target : chosen_weight - 1;
-        locate<T>(args, r, row, sh.chosen, key_logit((uint32_t)(chosen_key >> 32)), rp.c, 1, -__builtin_inf(), target,
-                  chosen_factor / (double)total, sh);
+        locate<T, VECTOR>(args, r, row, sh.chosen, key_logit(chosen_key), rp.c, 1, -__builtin_inf(), target,
+                          chosen_factor / (double)total, sh);
         if (tid == 0) plan.state = kSettled;
         return;
     }
     const u64 total = block_reduce(row_weight, SumOp(), sh.scratch);
-    const u64 all_valid = block_reduce(piece_valid, SumOp(), sh.scratch);
-    if (!cut) {  // min-p alone: everything is above the list
-        if (tid == 0) plan = {kCollect, -0x7fffffff, -0x7fffffff, top_key, total, 0, 0, (uint32_t)all_valid, 0};
+    const u64 valid = block_reduce(head.valid, SumOp(), sh.scratch);
+    const bool by_count = rp.k && (u64)rp.k < valid, by_share = rp.p < 1.0f;
+    if (!by_count && !by_share) {  // min-p alone, or with a k past what the row has: everything is above the list
+        if (tid == 0) plan = {kCollect, -0x7fffffff, -0x7fffffff, top_key, total, 0, 0, (uint32_t)valid, 0};
         return;
     }
     // The row's bins: thread j the j-th below that of its largest logit.
     const int top_bin = value_bin(top);
     factors[tid] = (float)factor;
-    top_bins[tid] = key >> 32 ? value_bin(piece_top) : -0x40000000;
+    top_bins[tid] = piece_key ? value_bin(piece_top) : -0x40000000;
+    if (tid < 4) sh.cuts[tid] = kBins;
     __syncthreads();
+    const u64 *bins = row_bins(args, scratch);
     u64 count = 0;
     double bin_weight = 0.0;
-    constexpr int kAtOnce = 8;
+    constexpr int kAtOnce = 16;
     for (int first = 0; first < args.pieces; first += kAtOnce) {
         u64 entry[kAtOnce];
 #pragma unroll
         for (int e = 0; e < kAtOnce; ++e) {
             const int below = first + e < args.pieces ? tid - (top_bin - top_bins[first + e]) : -1;
-            entry[e] = below >= 0 ? get(&all_bins[(size_t)(first + e) * kBins + below]) : 0;
+            entry[e] = below >= 0 ? bins[(size_t)(first + e) * kBins + below] : 0;
         }
 #pragma unroll
         for (int e = 0; e < kAtOnce; ++e) {
@@ -516,43 +446,32 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
     }
     const u64 own_weight = (u64)bin_weight, run_count = block_scan(count, sh.scratch),
               run_weight = block_scan(own_weight, sh.scratch);
-    // cuts: the bins of the k-th element, and those between which the run ends that has the share p.
-    if (tid < 4) sh.cuts[tid] = kBins;
-    __syncthreads();
-    const bool by_count = rp.k && (u64)rp.k < all_valid;
+    // cuts: the bin of the k-th element, and those between which the run ends that has the share p.
     if (by_count && run_count >= (u64)rp.k && run_count - count < (u64)rp.k) {
         sh.cuts[0] = tid;
         sh.weights[0] = run_weight - own_weight;
         sh.weights[1] = run_weight;
     }
     __syncthreads();
-    const bool found = !by_count || sh.cuts[0] < kBins;
-    if (rp.p < 1.0f && found) {
+    if (by_share && (!by_count || sh.cuts[0] < kBins)) {
         // (The bins' weights are exact to 2^-22 or better: piece factors in fp32, entries in 2^-35.)
         constexpr double kSlack = 1.0 / (1 << 20);
         const double least = (double)rp.p * (double)(by_count ? sh.weights[0] : total) * (1.0 - kSlack);
         const double most = (double)rp.p * (double)(by_count ? sh.weights[1] : total) * (1.0 + kSlack);
-        if (count && (double)run_weight >= least && ((double)(run_weight - own_weight) < least || run_count == count))
-            sh.cuts[1] = tid;
-        if (count && (double)run_weight >= most && ((double)(run_weight - own_weight) < most || run_count == count))
-            sh.cuts[2] = tid;
+        const double before = (double)(run_weight - own_weight);
+        if (count && (double)run_weight >= least && (before < least || run_count == count)) sh.cuts[1] = tid;
+        if (count && (double)run_weight >= most && (before < most || run_count == count)) sh.cuts[2] = tid;
     }
     __syncthreads();
     // The list: from the first bin that the cut can be in to the last that matters.
-    const int from = rp.p < 1.0f ? sh.cuts[1] : sh.cuts[0];
-    const int to = by_count ? sh.cuts[0] : rp.p < 1.0f ? sh.cuts[2] : sh.cuts[0];
-    const bool none = !by_count && !(rp.p < 1.0f);  // k is past what the row has
-    if (none) {
-        if (tid == 0) plan = {kCollect, -0x7fffffff, -0x7fffffff, top_key, total, 0, 0, (uint32_t)all_valid, 0};
-        return;
-    }
-    if (from < kBins && tid == from) sh.weights[2] = run_count - count;
-    if (to < kBins && tid == to) sh.weights[3] = run_count;
+    const int from = by_share ? sh.cuts[1] : sh.cuts[0], to = by_count ? sh.cuts[0] : sh.cuts[2];
+    if (tid == from) sh.weights[2] = run_count - count;
+    if (tid == to) sh.weights[3] = run_count;
     __syncthreads();
     if (tid == 0) {
         const bool fits = from < kBins && to < kBins && sh.weights[3] - sh.weights[2] <= kList;
         plan = {fits ? kCollect : kSearch, top_bin - from + 1, top_bin - to, top_key, total,
-                fits ? (uint32_t)sh.weights[2] : 0, 0, (uint32_t)all_valid, 0};
+                fits ? (uint32_t)sh.weights[2] : 0, 0, (uint32_t)valid, 0};
     }
 }
 
@@ -560,146 +479,191 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs args) {
-    __shared__ Shared sh;
-    __shared__ u64 list[kList];
-    const int tid = threadIdx.x, piece = blockIdx.x, lane = tid & 63;
+    __shared__ u64 scratch[kWaves];
+    const int piece = blockIdx.x, lane = threadIdx.x & 63;
     const int64_t r = blockIdx.y;
-    RowScratch &scratch = row_scratch(args, (int)r);
-    const RowPlan plan = scratch.plan;
-    const u64 piece_key = scratch.heads[piece].key >> 32;
-    if (plan.state == kSettled) return;
-    const T *row = (const T *)args.logits + r * args.ld;
+    RowScratch &row = row_scratch(args, (int)r);
+    const int state = row.plan.state, low_bin = row.plan.low_bin, above_bin = row.plan.above_bin;
+    const uint32_t top_key = row.plan.top_key, piece_key = (uint32_t)(row.heads[piece].key >> 32);
+    if (state != kCollect) return;
     const RowParams rp = row_params(args, r);
-    if (plan.state == kSearch) {
-        if (piece == 0) search_row<T>(args, r, row, plan, rp, list, sh);
-        return;
-    }
-    const float top = key_logit(plan.top_key), piece_top = key_logit((uint32_t)piece_key);
+    const float top = key_logit(top_key), piece_top = key_logit(piece_key);
     const double low = rp.low();
-    u64 *row_list_at = row_list(args, scratch);
     u64 above = 0, kept = 0;
     // (A piece whose largest is below the list's bins, or below min-p with no list, has nothing to give.)
-    if (piece_key && value_bin(piece_top) >= plan.low_bin &&
-        (plan.low_bin != -0x7fffffff || weighs(piece_top, top, rp.c, low))) {
+    if (piece_key && value_bin(piece_top) >= low_bin &&
+        (low_bin != -0x7fffffff || weighs(piece_top, top, rp.c, low))) {
+        const Weights weigh(top, rp.c);
         float v[kPer];
-        load_piece<T, VECTOR>(row, piece * kPiece, args.vocab, v);
-        int mine = 0;
+        load_piece<T, VECTOR>((const T *)args.logits + r * args.ld, piece * kPiece, args.vocab, v);
         uint32_t listed = 0;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
-            if (logit_key(v[e]) == 0) continue;
             const int bin = value_bin(v[e]);
-            if (bin >= plan.above_bin) {
-                const u64 w = logit_weight(v[e], top, rp.c);
-                above += w;
-                if (weighs(v[e], top, rp.c, low)) kept += w;
-            } else if (bin >= plan.low_bin) {
-                listed |= 1u << e;
-                ++mine;
+            if (v[e] > -__builtin_inff() && bin >= low_bin) {
+                if (bin >= above_bin) {
+                    const u64 w = weigh(v[e]);
+                    above += w;
+                    if (weighs(v[e], top, rp.c, low)) kept += w;
+                } else {
+                    listed |= 1u << e;
+                }
             }
         }
         // Places in the row's list, a wave at a time.
-        if (__ballot(mine != 0)) {
-            int run = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int up = __shfl_up(run, d, 64);
-                if (lane >= d) run += up;
-            }
+        if (__ballot(listed != 0)) {
+            const uint32_t mine = __builtin_popcount(listed), run = wave_scan(mine, SumOp());
             uint32_t at = 0;
             if (lane == 63)
-                at = __hip_atomic_fetch_add(&scratch.plan.listed, (uint32_t)run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            at = __builtin_amdgcn_readlane(at, 63) + (uint32_t)(run - mine);
+                at = __hip_atomic_fetch_add(&row.plan.listed, run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            at = __builtin_amdgcn_readlane(at, 63) + run - mine;
+            u64 *list = row_list(args, row);
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
                 if (listed >> e & 1) {
-                    if (at < kList) put(&row_list_at[at], order_key(v[e], piece * kPiece + index_of<T, VECTOR>(e)));
+                    if (at < kList) list[at] = order_key(v[e], piece * kPiece + index_of<T, VECTOR>(e));
                     ++at;
                 }
         }
-        above = block_reduce(above, SumOp(), sh.scratch);
-        kept = block_reduce(kept, SumOp(), sh.scratch);
+        above = block_reduce(above, SumOp(), scratch);
+        kept = block_reduce(kept, SumOp(), scratch);
     }
-    if (tid == 0) {
-        put(&scratch.heads[piece].above, above);
-        put(&scratch.heads[piece].kept, kept);
+    if (threadIdx.x == 0) {
+        row.heads[piece].above = above;
+        row.heads[piece].kept = kept;
     }
-    if (!last_to_arrive(args.arrivals + r, args.pieces, &sh.arrival)) return;
+}
 
-    // The row. The list in order, larger keys first.
-    const uint32_t listed = __hip_atomic_load(&scratch.plan.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int n = listed < (uint32_t)kList ? (int)listed : kList;
-    u64 piece_kept = tid < args.pieces ? get(&scratch.heads[tid].kept) : 0;
-    const u64 piece_above = tid < args.pieces ? get(&scratch.heads[tid].above) : 0;
-    u64 cut = 1;
-    if (n) {
-        int size = 64;
-        while (size < n) size *= 2;
-        for (int i = tid; i < size; i += kThreads) list[i] = i < n ? get(&row_list_at[i]) : 0;
-        for (int width = 2; width <= size; width *= 2)
-            for (int step = width / 2; step > 0; step /= 2) {
-                __syncthreads();
-                for (int i = tid; i < size / 2; i += kThreads) {
-                    const int a = 2 * i - (i & (step - 1)), b = a + step;
-                    const u64 x = list[a], y = list[b];
-                    if ((x < y) == ((a & width) == 0)) list[a] = y, list[b] = x;
-                }
-            }
-        const u64 row_above = block_reduce(piece_above, SumOp(), sh.scratch);
-        // Running weights over runs of the list, one a thread.
-        const int per = (n + kThreads - 1) / kThreads, first = tid * per;
-        u64 sum = 0;
-        for (int i = first; i < first + per && i < n; ++i) sum += logit_weight(key_logit((uint32_t)(list[i] >> 32)), top, rp.c);
-        const u64 before = row_above + block_scan(sum, sh.scratch) - sum;
-        // The k-th element, and the weight up to it.
-        const bool by_count = rp.k && (uint32_t)rp.k < plan.valid;
-        int last = n - 1;
-        if (by_count) {
-            const int64_t at = (int64_t)rp.k - plan.above - 1;
-            last = at < 0 ? 0 : at < n ? (int)at : n - 1;
-        }
-        if (tid == 0) sh.cuts[0] = last;
-        if (by_count && last >= first && last < first + per) {
-            u64 run = before;
-            for (int i = first; i <= last; ++i) run += logit_weight(key_logit((uint32_t)(list[i] >> 32)), top, rp.c);
-            sh.weights[0] = run;
+// ---- finish -----------------------------------------------------------------------------------------
+
+// Among the keys of a source (key(i) for i < n, 0 and those below `limit` not counted), which `base_count`
+// elements of weight `base_weight` come before: the smallest run from the start of the order with `k`
+// elements, or with weight >= share where k is 0. Returns its last key, *weight its weight. Nine bits of the
+// key at a time, from the first in which the keys between `least` and `most` differ.
+template <typename Source>
+__device__ __forceinline__ u64 find_cut(const Source &key_at, int n, u64 most, u64 least, const Weights &weigh, u64 limit,
+                                        u64 base_count, u64 base_weight, u64 k, double share, u64 *weight, u64 *counts,
+                                        u64 *sums, Shared &sh) {
+    constexpr int kBits = 9;
+    static_assert(1 << kBits == kThreads, "a digit a thread");
+    const int tid = threadIdx.x, digit = kThreads - 1 - tid;
+    const int top_bit = most == least ? 0 : 63 - __builtin_clzll(most ^ least);
+    int shift = top_bit < kBits ? 0 : top_bit - kBits + 1;
+    u64 above = top_bit == 63 ? 0 : ~(u64)0 << (top_bit + 1), prefix = most & above;
+    for (;;) {
+        __syncthreads();
+        counts[tid] = 0;
+        sums[tid] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid; i < n; i += kThreads) {
+            const u64 key = key_at(i);
+            if (key == 0 || key < limit || ((key ^ prefix) & above)) continue;
+            const int d = (int)(key >> shift) & (int)(~above >> shift) & (kThreads - 1);
+            atomicAdd(&counts[d], (u64)1);
+            atomicAdd(&sums[d], weigh(key_logit((uint32_t)(key >> 32))));
         }
         __syncthreads();
-        if (rp.p < 1.0f) {
-            const double share = (double)rp.p * (double)(by_count ? sh.weights[0] : plan.total);
-            u64 run = before;
-            for (int i = first; i < first + per && i <= last; ++i) {
-                const u64 w = logit_weight(key_logit((uint32_t)(list[i] >> 32)), top, rp.c);
-                run += w;
-                // (The first that reaches the share; where rounding has the elements above reach it, the first.)
-                if ((double)run >= share && ((double)(run - w) < share || i == 0)) sh.cuts[0] = i;
-            }
+        // The first digit from the largest down that the run can end in; where rounding leaves none, the last.
+        const u64 count = counts[digit], sum = sums[digit];
+        const u64 run = base_count + block_scan(count, sh.scratch), w = base_weight + block_scan(sum, sh.scratch);
+        const bool reached = k ? run >= k : (double)w >= share;
+        const bool before = run != base_count + count && (k ? run - count >= k : (double)(w - sum) >= share);
+        const int last = (int)block_reduce(count ? (uint32_t)tid + 1 : 0u, MaxOp(), sh.scratch) - 1;
+        if (count && !before && (reached || tid == last)) {
+            sh.cuts[0] = digit;
+            sh.weights[0] = run - count;
+            sh.weights[1] = w - sum;
+            sh.weights[2] = w;
         }
         __syncthreads();
-        cut = list[sh.cuts[0]];
-        // What min-p leaves of the list's kept elements, to their pieces.
-        u64 *extra = (u64 *)list;  // (kept apart by the barriers)
-        const int end = sh.cuts[0] + 1;
-        u64 keys[kList / kThreads];
-#pragma unroll
-        for (int j = 0; j < kList / kThreads; ++j) {
-            const int i = tid + j * kThreads;
-            keys[j] = i < end ? list[i] : 0;
-        }
-        __syncthreads();
-        extra[tid] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kList / kThreads; ++j) {
-            const float v = key_logit((uint32_t)(keys[j] >> 32));
-            if (keys[j] && weighs(v, top, rp.c, low))
-                atomicAdd(&extra[(0xffffffffu - (uint32_t)keys[j]) / kPiece], logit_weight(v, top, rp.c));
-        }
-        __syncthreads();
-        piece_kept += extra[tid];
+        prefix |= (u64)(uint32_t)sh.cuts[0] << shift;
+        base_count = sh.weights[0];
+        base_weight = sh.weights[1];
+        if (shift == 0) break;
+        above = ~(u64)0 << shift;
+        shift = shift < kBits ? 0 : shift - kBits;
     }
-    const u64 total = choose_piece(piece_kept, rp.u, sh);
-    locate<T>(args, r, row, sh.chosen, top, rp.c, cut, low, sh.rest, 1.0 / (double)total, sh);
+    *weight = sh.weights[2];
+    return prefix;
+}
+
+// The cuts of top-k and, among its elements, of top-p.
+template <typename Source>
+__device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, u64 most, u64 least, const Weights &weigh,
+                                         const RowPlan &plan, const RowParams &rp, u64 base_weight, u64 *memory, Shared &sh) {
+    u64 cut = 1, weight = plan.total;
+    for (int pass = 0; pass < 2; ++pass) {
+        const bool by_count = pass == 0;
+        if (by_count ? !(rp.k && (uint32_t)rp.k < plan.valid) : !(rp.p < 1.0f)) continue;
+        cut = find_cut(key_at, n, most, least, weigh, cut, plan.above, base_weight, by_count ? (u64)rp.k : 0,
+                       (double)rp.p * (double)weight, &weight, memory, memory + kThreads, sh);
+    }
+    return cut;
+}
+
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args) {
+    __shared__ Shared sh;
+    __shared__ u64 list[kList], memory[2 * kThreads];
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    RowScratch &scratch = row_scratch(args, (int)r);
+    const RowPlan plan = scratch.plan;
+    if (plan.state == kSettled) return;
+    u64 kept = 0, above = 0;
+    if (tid < args.pieces) kept = scratch.heads[tid].kept, above = scratch.heads[tid].above;
+    const T *row = (const T *)args.logits + r * args.ld;
+    const RowParams rp = row_params(args, r);
+    const float top = key_logit(plan.top_key);
+    const double low = rp.low();
+    const Weights weigh(top, rp.c);
+    u64 cut = 1;
+    if (plan.state == kCollect) {
+        const int n = (int)plan.listed;
+        if (n) {
+            u64 most = 0, least = 0;  // (least: the complement's largest)
+            for (int i = tid; i < n; i += kThreads) {
+                const u64 key = row_list(args, scratch)[i];
+                list[i] = key;
+                most = most > key ? most : key;
+                least = least > ~key ? least : ~key;
+            }
+            most = block_reduce(most, MaxOp(), sh.scratch);
+            least = ~block_reduce(least, MaxOp(), sh.scratch);
+            const u64 base_weight = block_reduce(above, SumOp(), sh.scratch);
+            cut = find_cuts([&](int i) { return list[i]; }, n, most, least, weigh, plan, rp, base_weight, memory, sh);
+            // What min-p leaves of the list's kept elements, to their pieces.
+            __syncthreads();
+            memory[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+                const u64 key = list[i];
+                const float v = key_logit((uint32_t)(key >> 32));
+                if (key >= cut && weighs(v, top, rp.c, low))
+                    atomicAdd(&memory[(0xffffffffu - (uint32_t)key) / kPiece], weigh(v));
+            }
+            __syncthreads();
+            kept += memory[tid];
+        }
+    } else {
+        cut = find_cuts([&](int i) { return order_key(logit_of(row[i]), i); }, args.vocab, ~(u64)0, 0, weigh, plan, rp, 0,
+                        memory, sh);
+        // The pieces' kept weights, thread by thread.
+        kept = 0;
+        for (int piece = 0; piece < args.pieces; ++piece) {
+            u64 sum = 0;
+            for (int i = piece * kPiece + tid; i < (piece + 1) * kPiece && i < args.vocab; i += kThreads) {
+                const float v = logit_of(row[i]);
+                const u64 key = order_key(v, i);
+                if (key >= cut && weighs(v, top, rp.c, low)) sum += weigh(v);
+            }
+            sum = block_reduce(sum, SumOp(), sh.scratch);
+            if (tid == piece) kept = sum;
+        }
+    }
+    const u64 total = choose_piece(kept, rp.u, sh);
+    locate<T, VECTOR>(args, r, row, sh.chosen, top, rp.c, cut, low, sh.rest, 1.0 / (double)total, sh);
 }
 
 // ---- host -------------------------------------------------------------------------------------------
@@ -717,10 +681,12 @@ size_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
 
 template <typename T, bool VECTOR>
 static void launch_batch(const SampleArgs &args, int rows, hipStream_t stream) {
-    const dim3 grid((unsigned)args.pieces, (unsigned)rows);
-    hipLaunchKernelGGL((sample_scan_kernel<T, VECTOR>), grid, dim3(kThreads), 0, stream, args);
-    if (args.p.uniforms)
-        hipLaunchKernelGGL((sample_collect_kernel<T, VECTOR>), grid, dim3(kThreads), 0, stream, args);
+    const dim3 pieces((unsigned)args.pieces, (unsigned)rows), whole((unsigned)rows);
+    hipLaunchKernelGGL((sample_scan_kernel<T, VECTOR>), pieces, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL((sample_settle_kernel<T, VECTOR>), whole, dim3(kThreads), 0, stream, args);
+    if (!args.p.uniforms || (!args.p.top_k && !args.p.top_p && !args.p.min_p)) return;  // every row is settled
+    hipLaunchKernelGGL((sample_collect_kernel<T, VECTOR>), pieces, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL((sample_finish_kernel<T, VECTOR>), whole, dim3(kThreads), 0, stream, args);
 }
 
 hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab,
@@ -739,7 +705,6 @@ hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows
         args.p = {from(params.uniforms), from(params.temperature), from(params.top_k), from(params.top_p), from(params.min_p)};
         args.tokens = tokens + at;
         args.logprobs = from(logprobs);
-        args.arrivals = (int *)workspace;
         args.rows = (char *)workspace + kSampleCounterBytes;
         args.row_bytes = row_bytes(vocab);
         if (dtype == SPLOSH_F32) {
