@@ -57,32 +57,37 @@ __device__ __forceinline__ u64 order_key(float v, uint32_t index) {
     return key ? (u64)key << 32 | (0xffffffffu - index) : 0;
 }
 
-// exp((v - top) / T) in units of 2^-40, downwards, c = log2(e) / T. The exponent (v - s) c - (top - s) c is kept
-// in two fp32 numbers (its product's rounding error by an fma, c in two as well), of which the larger one's
-// whole part is the shift; the fraction's power is the hardware's (1 ulp). s is 0, and top where the exponent
-// at top is so large that its fraction would be lost: then v - top is exact for every v that has weight.
+// exp((v - top) / T) in units of 2^-40, downwards, c = log2(e) / T. The exponent is (v - s) c - (top - s) c, its
+// parts kept apart: the whole number nearest to the fp32 product is the shift, what an fma leaves of the product
+// past it, the product with c's second fp32 part and top's fraction add up to the fraction, whose power is the
+// hardware's (1 ulp). s is 0, and top where the exponent at top is so large that its fraction would be lost:
+// then v - top is exact for every v that has weight. Where top is infinite, so is each that has weight.
 struct Weights {
-    float top, s, c_high, c_low, whole, fraction;
+    float s, c_high, c_low, shift0, fraction, infinite;
 
-    __device__ __forceinline__ Weights(float top_, double c) : top(top_) {
+    __device__ __forceinline__ Weights(float top, double c) {
         double at = (double)top * c;
         s = 0.0f;
         if (!(__builtin_fabs(at) < (double)(1 << 21))) s = top, at = 0.0;
         c_high = (float)c;
         c_low = c_high < __builtin_inff() ? (float)(c - (double)c_high) : 0.0f;
         const double n = __builtin_rint(at);
-        whole = (float)n;
+        shift0 = (float)n + (float)(kShift);
         fraction = (float)(at - n);
+        infinite = top == __builtin_inff() ? top : __builtin_nanf("");
     }
+    // m 2^32 (m: 24 bits and the power's) moved down to m 2^(40 - 24) at the exponent 0, or 1 less where the
+    // two whole numbers are rounded apart.
+    static constexpr int kShift = 32 - (kWeightBits - 24);
     __device__ __forceinline__ u64 operator()(float v) const {
-#pragma clang fp contract(off)  // (high is the rounded product wherever it stands)
-        const float d = v - s, high = d * c_high;
-        const float low = __builtin_fmaf(d, c_low, __builtin_fmaf(d, c_high, -high));
-        const float n = __builtin_rintf(high), left = n - whole;  // (left: at most 1)
-        const float e = __builtin_amdgcn_exp2f(((high - n) + low) - fraction);
-        const int shift = 1 - (int)left;
-        const u64 w = ((u64)(uint32_t)(e * 16777216.0f) << (kWeightBits - 23)) >> (shift > 0 ? shift : 0);
-        return v == top ? (u64)1 << kWeightBits : left > -(kWeightBits + 4.0f) ? w : 0;
+#pragma clang fp contract(off)  // (n is the rounded product's)
+        const float d = v - s, n = __builtin_rintf(d * c_high);
+        const float f = __builtin_fmaf(d, c_high, -n) + __builtin_fmaf(d, c_low, -fraction);
+        float e = __builtin_amdgcn_exp2f(f);
+        e = v == infinite ? 0.5f : e;
+        int shift = (int)(shift0 - n);
+        shift = shift < kShift - 1 ? kShift - 1 : shift > 63 ? 63 : shift;  // (an infinite one's: the least)
+        return (u64)(uint32_t)(e * 16777216.0f) << 32 >> shift;
     }
 };
 
@@ -163,6 +168,7 @@ struct RowPlan {
     uint32_t above;    // elements in the bins above the list's
     uint32_t listed;   // elements of the list so far
     uint32_t valid, reserved;  // valid: elements that can be chosen
+    double c, low;     // log2(e) / T; log2(min_p), -inf where it is off
 };
 // A piece. key: its largest logit's << 32 | the index of that (greedy rows).
 struct PieceHead {
@@ -202,8 +208,6 @@ struct RowParams {
     float p;   // 1: off
     float q;   // 0: off
     float u;
-    // log2(q), the least (v - top) c of what min-p keeps; -inf: off.
-    __device__ double low() const { return q > 0.0f ? log2((double)q) : -__builtin_inf(); }
 };
 __device__ __forceinline__ RowParams row_params(const SampleArgs &args, int64_t r) {
     const float t = args.p.temperature ? args.p.temperature[r] : 1.0f, p = args.p.top_p ? args.p.top_p[r] : 1.0f,
@@ -283,14 +287,16 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
         w[e] = key && key >= cut && weighs(v[e], top, c, low) ? weigh(v[e]) : 0;
         sum += w[e];
     }
-    u64 run = block_scan(sum, sh.scratch) - sum;
+    u64 run = block_scan(sum, sh.scratch) - sum, found = 0;
+    int at = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        if (run <= target && target < run + w[e]) {
-            args.tokens[r] = (uint32_t)(first + e);
-            if (args.logprobs) args.logprobs[r] = (float)log((double)w[e] * scale);
-        }
+        if (run <= target && target < run + w[e]) at = e, found = w[e];
         run += w[e];
+    }
+    if (found) {
+        args.tokens[r] = (uint32_t)(first + at);
+        if (args.logprobs) args.logprobs[r] = (float)log((double)found * scale);
     }
 }
 
@@ -415,9 +421,11 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     }
     const u64 total = block_reduce(row_weight, SumOp(), sh.scratch);
     const u64 valid = block_reduce(head.valid, SumOp(), sh.scratch);
+    // The least (v - top) c of what min-p keeps.
+    const double low = rp.q > 0.0f ? log2((double)rp.q) : -__builtin_inf();
     const bool by_count = rp.k && (u64)rp.k < valid, by_share = rp.p < 1.0f;
     if (!by_count && !by_share) {  // min-p alone, or with a k past what the row has: everything is above the list
-        if (tid == 0) plan = {kCollect, -0x7fffffff, -0x7fffffff, top_key, total, 0, 0, (uint32_t)valid, 0};
+        if (tid == 0) plan = {kCollect, -0x7fffffff, -0x7fffffff, top_key, total, 0, 0, (uint32_t)valid, 0, rp.c, low};
         return;
     }
     // The row's bins: thread j the j-th below that of its largest logit.
@@ -429,7 +437,7 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     const u64 *bins = row_bins(args, scratch);
     u64 count = 0;
     double bin_weight = 0.0;
-    constexpr int kAtOnce = 16;
+    constexpr int kAtOnce = 32;
     for (int first = 0; first < args.pieces; first += kAtOnce) {
         u64 entry[kAtOnce];
 #pragma unroll
@@ -471,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     if (tid == 0) {
         const bool fits = from < kBins && to < kBins && sh.weights[3] - sh.weights[2] <= kList;
         plan = {fits ? kCollect : kSearch, top_bin - from + 1, top_bin - to, top_key, total,
-                fits ? (uint32_t)sh.weights[2] : 0, 0, (uint32_t)valid, 0};
+                fits ? (uint32_t)sh.weights[2] : 0, 0, (uint32_t)valid, 0, rp.c, low};
     }
 }
 
@@ -483,17 +491,17 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
     const int piece = blockIdx.x, lane = threadIdx.x & 63;
     const int64_t r = blockIdx.y;
     RowScratch &row = row_scratch(args, (int)r);
-    const int state = row.plan.state, low_bin = row.plan.low_bin, above_bin = row.plan.above_bin;
-    const uint32_t top_key = row.plan.top_key, piece_key = (uint32_t)(row.heads[piece].key >> 32);
+    const RowPlan &plan = row.plan;
+    const int state = plan.state, low_bin = plan.low_bin, above_bin = plan.above_bin;
+    const uint32_t piece_key = (uint32_t)(row.heads[piece].key >> 32);
+    const float top = key_logit(plan.top_key), piece_top = key_logit(piece_key);
+    const double c = plan.c, low = plan.low;
     if (state != kCollect) return;
-    const RowParams rp = row_params(args, r);
-    const float top = key_logit(top_key), piece_top = key_logit(piece_key);
-    const double low = rp.low();
     u64 above = 0, kept = 0;
     // (A piece whose largest is below the list's bins, or below min-p with no list, has nothing to give.)
     if (piece_key && value_bin(piece_top) >= low_bin &&
-        (low_bin != -0x7fffffff || weighs(piece_top, top, rp.c, low))) {
-        const Weights weigh(top, rp.c);
+        (low_bin != -0x7fffffff || weighs(piece_top, top, c, low))) {
+        const Weights weigh(top, c);
         float v[kPer];
         load_piece<T, VECTOR>((const T *)args.logits + r * args.ld, piece * kPiece, args.vocab, v);
         uint32_t listed = 0;
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
                 if (bin >= above_bin) {
                     const u64 w = weigh(v[e]);
                     above += w;
-                    if (weighs(v[e], top, rp.c, low)) kept += w;
+                    if (weighs(v[e], top, c, low)) kept += w;
                 } else {
                     listed |= 1u << e;
                 }
@@ -564,14 +572,14 @@ __device__ __forceinline__ u64 find_cut(const Source &key_at, int n, u64 most, u
             atomicAdd(&sums[d], weigh(key_logit((uint32_t)(key >> 32))));
         }
         __syncthreads();
-        // The first digit from the largest down that the run can end in; where rounding leaves none, the last.
+        // The first digit from the largest down that the run can end in.
         const u64 count = counts[digit], sum = sums[digit];
         const u64 run = base_count + block_scan(count, sh.scratch), w = base_weight + block_scan(sum, sh.scratch);
         const bool reached = k ? run >= k : (double)w >= share;
         const bool before = run != base_count + count && (k ? run - count >= k : (double)(w - sum) >= share);
-        const int last = (int)block_reduce(count ? (uint32_t)tid + 1 : 0u, MaxOp(), sh.scratch) - 1;
-        if (count && !before && (reached || tid == last)) {
+        if (count && !before && reached) {
             sh.cuts[0] = digit;
+            sh.cuts[1] = count == 1;
             sh.weights[0] = run - count;
             sh.weights[1] = w - sum;
             sh.weights[2] = w;
@@ -582,6 +590,16 @@ __device__ __forceinline__ u64 find_cut(const Source &key_at, int n, u64 most, u
         base_weight = sh.weights[1];
         if (shift == 0) break;
         above = ~(u64)0 << shift;
+        if (sh.cuts[1]) {  // one element is left: its key
+#pragma unroll 4
+            for (int i = tid; i < n; i += kThreads) {
+                const u64 key = key_at(i);
+                if (key && ((key ^ prefix) & above) == 0) sh.rest = key;
+            }
+            __syncthreads();
+            prefix = sh.rest;
+            break;
+        }
         shift = shift < kBits ? 0 : shift - kBits;
     }
     *weight = sh.weights[2];
@@ -616,7 +634,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const T *row = (const T *)args.logits + r * args.ld;
     const RowParams rp = row_params(args, r);
     const float top = key_logit(plan.top_key);
-    const double low = rp.low();
+    const double low = plan.low;
     const Weights weigh(top, rp.c);
     u64 cut = 1;
     if (plan.state == kCollect) {
