@@ -4,7 +4,7 @@
 // Every filter keeps a run from the start of one total order, larger logits first and of equal ones
 // the lower index, so together they keep {element >= cut} of it (min-p a value bound of its own), and
 // one cut decides the row. The order is that of a 64-bit key: the logit's bits made monotone, then the
-// complement of the index. Weights are integers (2^40 for the largest logit of what they are measured
+// complement of the index in as many bits as the vocabulary takes. Weights are integers (2^40 for the largest logit of what they are measured
 // against), so that their sums do not depend on the order of the additions.
 //
 // Four launches; a workgroup takes a piece of 8192 logits, or a row:
@@ -31,7 +31,8 @@ constexpr int kBins = kThreads;              // value bins of a piece
 constexpr int kList = 8192;                  // elements of a row's list
 constexpr int kBatchRows = 256;              // rows of one launch
 constexpr int kWeightBits = 40;
-// A bin's entry: 15 bits of count (a piece has 2^13 elements) over 49 of weight in units of 2^-35.
+// A bin's entry while it is counted: 15 bits of count (a piece has 2^13 elements) over 49 of weight in units of
+// 2^-35; as it is left, the count over the fp32 weight.
 constexpr int kBinShift = 49, kBinUnit = kWeightBits - 35;
 
 static_assert((int64_t)kPiece * kThreads >= kSampleMaxVocab, "a row's pieces are one a thread");
@@ -52,10 +53,26 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 __device__ __forceinline__ float key_logit(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-__device__ __forceinline__ u64 order_key(float v, uint32_t index) {
-    const uint32_t key = logit_key(v);
-    return key ? (u64)key << 32 | (0xffffffffu - index) : 0;
-}
+// An element's place in the order, 0 for those that are never chosen: its logit's over `bits` bits of its
+// index's complement, of a bf16 logit the half that its bits are in.
+template <typename T>
+struct OrderKeys {
+    static constexpr int kLow = sizeof(T) == 2 ? 16 : 0;
+    int bits;
+    __device__ __forceinline__ explicit OrderKeys(int vocab) : bits(32 - __builtin_clz(vocab)) {}
+    __device__ __forceinline__ u64 operator()(float v, int index) const {
+        const uint32_t key = logit_key(v) >> kLow;
+        return key ? (u64)key << bits | (uint32_t)((1 << bits) - 1 - index) : 0;
+    }
+    __device__ __forceinline__ float logit(u64 key) const {
+        const uint32_t high = (uint32_t)(key >> bits);
+        return key_logit(kLow && !(high & 0x8000u) ? high << kLow | 0xffffu : high << kLow);
+    }
+    // The least and the most that a logit's keys can be.
+    __device__ __forceinline__ u64 least(float v) const { return (u64)(logit_key(v) >> kLow) << bits; }
+    __device__ __forceinline__ u64 most(float v) const { return least(v) | ((1u << bits) - 1); }
+    __device__ __forceinline__ int index(u64 key) const { return (1 << bits) - 1 - (int)((uint32_t)key & ((1u << bits) - 1)); }
+};
 
 // exp((v - top) / T) in units of 2^-40, downwards, c = log2(e) / T. The exponent is (v - s) c - (top - s) c, its
 // parts kept apart: the whole number nearest to the fp32 product is the shift, what an fma leaves of the product
@@ -101,6 +118,13 @@ __device__ __forceinline__ bool weighs(float v, float top, double c, double low)
 __device__ __forceinline__ int value_bin(float v) {
     const int bin = (int)(__float_as_uint(__builtin_fabsf(v) + 1.0f) >> 17) - (127 << 6);
     return v >= 0.0f ? bin : -1 - bin;
+}
+
+// The smallest value of a bin, to the rounding of 1 + |logit|.
+__device__ __forceinline__ float bin_edge(int bin) {
+    const int at = bin >= 0 ? bin : -bin;
+    const float v = __uint_as_float((uint32_t)((at < 8192 ? at : 8192) + (127 << 6)) << 17) - 1.0f;
+    return bin >= 0 ? v : -v;
 }
 
 // ---- across a workgroup ---------------------------------------------------------------------------
@@ -277,13 +301,14 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
     constexpr int kRun = 16 / (int)sizeof(T);
     const int first = piece * kPiece + (int)threadIdx.x * kPer;
     const Weights weigh(top, c);
+    const OrderKeys<T> keys(args.vocab);
     float v[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; e += kRun) load_run<T, VECTOR, kRun>(row, first + e, args.vocab, &v[e]);
     u64 w[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        const u64 key = order_key(v[e], first + e);
+        const u64 key = keys(v[e], first + e);
         w[e] = key && key >= cut && weighs(v[e], top, c, low) ? weigh(v[e]) : 0;
         sum += w[e];
     }
@@ -367,7 +392,11 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
         row.heads[piece].weight = weight;
         row.heads[piece].valid = valid;
     }
-    if (cut) row_bins(args, row)[(size_t)piece * kBins + tid] = bins[tid];
+    if (cut) {
+        const u64 entry = bins[tid];
+        const float w = (float)((entry & (((u64)1 << kBinShift) - 1)) << kBinUnit);
+        row_bins(args, row)[(size_t)piece * kBins + tid] = entry >> kBinShift << 32 | __float_as_uint(w);
+    }
 }
 
 // ---- settle -----------------------------------------------------------------------------------------
@@ -420,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
         return;
     }
     const u64 total = block_reduce(row_weight, SumOp(), sh.scratch);
-    const u64 valid = block_reduce(head.valid, SumOp(), sh.scratch);
+    const u64 valid = rp.k ? block_reduce(head.valid, SumOp(), sh.scratch) : 0;
     // The least (v - top) c of what min-p keeps.
     const double low = rp.q > 0.0f ? log2((double)rp.q) : -__builtin_inf();
     const bool by_count = rp.k && (u64)rp.k < valid, by_share = rp.p < 1.0f;
@@ -435,21 +464,20 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     if (tid < 4) sh.cuts[tid] = kBins;
     __syncthreads();
     const u64 *bins = row_bins(args, scratch);
-    u64 count = 0;
-    double bin_weight = 0.0;
+    uint32_t count = 0;
+    float bin_weight = 0.0f;
     constexpr int kAtOnce = 32;
     for (int first = 0; first < args.pieces; first += kAtOnce) {
         u64 entry[kAtOnce];
 #pragma unroll
         for (int e = 0; e < kAtOnce; ++e) {
-            const int below = first + e < args.pieces ? tid - (top_bin - top_bins[first + e]) : -1;
+            const int below = first + e < args.pieces ? tid - top_bin + top_bins[first + e] : -1;
             entry[e] = below >= 0 ? bins[(size_t)(first + e) * kBins + below] : 0;
         }
 #pragma unroll
         for (int e = 0; e < kAtOnce; ++e) {
-            count += entry[e] >> kBinShift;
-            bin_weight += (double)((entry[e] & (((u64)1 << kBinShift) - 1)) << kBinUnit) *
-                          (double)(first + e < args.pieces ? factors[first + e] : 0.0f);
+            count += (uint32_t)(entry[e] >> 32);
+            bin_weight = __builtin_fmaf(__uint_as_float((uint32_t)entry[e]), factors[(first + e) & (kThreads - 1)], bin_weight);
         }
     }
     const u64 own_weight = (u64)bin_weight, run_count = block_scan(count, sh.scratch),
@@ -462,8 +490,8 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     }
     __syncthreads();
     if (by_share && (!by_count || sh.cuts[0] < kBins)) {
-        // (The bins' weights are exact to 2^-22 or better: piece factors in fp32, entries in 2^-35.)
-        constexpr double kSlack = 1.0 / (1 << 20);
+        // (The bins' weights are fp32 sums of one product a piece: 2^-19 for a row of 32, 2^-15 for one of 512.)
+        constexpr double kSlack = 1.0 / (1 << 14);
         const double least = (double)rp.p * (double)(by_count ? sh.weights[0] : total) * (1.0 - kSlack);
         const double most = (double)rp.p * (double)(by_count ? sh.weights[1] : total) * (1.0 + kSlack);
         const double before = (double)(run_weight - own_weight);
@@ -526,10 +554,11 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
                 at = __hip_atomic_fetch_add(&row.plan.listed, run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             at = __builtin_amdgcn_readlane(at, 63) + run - mine;
             u64 *list = row_list(args, row);
+            const OrderKeys<T> keys(args.vocab);
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
                 if (listed >> e & 1) {
-                    if (at < kList) list[at] = order_key(v[e], piece * kPiece + index_of<T, VECTOR>(e));
+                    if (at < kList) list[at] = keys(v[e], piece * kPiece + index_of<T, VECTOR>(e));
                     ++at;
                 }
         }
@@ -544,78 +573,119 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
 
 // ---- finish -----------------------------------------------------------------------------------------
 
-// Among the keys of a source (key(i) for i < n, 0 and those below `limit` not counted), which `base_count`
-// elements of weight `base_weight` come before: the smallest run from the start of the order with `k`
-// elements, or with weight >= share where k is 0. Returns its last key, *weight its weight. Nine bits of the
-// key at a time, from the first in which the keys between `least` and `most` differ.
-template <typename Source>
-__device__ __forceinline__ u64 find_cut(const Source &key_at, int n, u64 most, u64 least, const Weights &weigh, u64 limit,
-                                        u64 base_count, u64 base_weight, u64 k, double share, u64 *weight, u64 *counts,
-                                        u64 *sums, Shared &sh) {
-    constexpr int kBits = 9;
-    static_assert(1 << kBits == kThreads, "a digit a thread");
-    const int tid = threadIdx.x, digit = kThreads - 1 - tid;
-    const int top_bit = most == least ? 0 : 63 - __builtin_clzll(most ^ least);
-    int shift = top_bit < kBits ? 0 : top_bit - kBits + 1;
-    u64 above = top_bit == 63 ? 0 : ~(u64)0 << (top_bit + 1), prefix = most & above;
-    for (;;) {
-        __syncthreads();
-        counts[tid] = 0;
-        sums[tid] = 0;
-        __syncthreads();
+// A step of the search for a cut among keys: how many there are with each digit of nine bits, and their weight.
+struct Digits {
+    u64 prefix, above;  // the bits above the digit, and where they are
+    int shift;
+    u64 base_count;     // elements before all of them
+    // Of this thread's digit (the largest in thread 0): its elements and weight, and with those before.
+    u64 count, weight, run_count, run_weight;
+};
+constexpr int kDigitBits = 9, kFew = 64;
+static_assert(1 << kDigitBits == kThreads, "a digit a thread");
+
+// The keys are those of a source, key(i) for i < n, from `limit` on (limit >= 1; a key of 0 is none).
+template <typename Source, typename Keys>
+__device__ __forceinline__ void count_digits(Digits &d, const Source &key_at, int n, const Keys &keys, const Weights &weigh,
+                                             u64 limit, u64 base_count, u64 base_weight, u64 *memory, Shared &sh) {
+    const int tid = threadIdx.x;
+    u64 *counts = memory, *sums = memory + kThreads;
+    __syncthreads();
+    counts[tid] = 0;
+    sums[tid] = 0;
+    __syncthreads();
 #pragma unroll 4
-        for (int i = tid; i < n; i += kThreads) {
-            const u64 key = key_at(i);
-            if (key == 0 || key < limit || ((key ^ prefix) & above)) continue;
-            const int d = (int)(key >> shift) & (int)(~above >> shift) & (kThreads - 1);
-            atomicAdd(&counts[d], (u64)1);
-            atomicAdd(&sums[d], weigh(key_logit((uint32_t)(key >> 32))));
-        }
-        __syncthreads();
-        // The first digit from the largest down that the run can end in.
-        const u64 count = counts[digit], sum = sums[digit];
-        const u64 run = base_count + block_scan(count, sh.scratch), w = base_weight + block_scan(sum, sh.scratch);
-        const bool reached = k ? run >= k : (double)w >= share;
-        const bool before = run != base_count + count && (k ? run - count >= k : (double)(w - sum) >= share);
-        if (count && !before && reached) {
-            sh.cuts[0] = digit;
-            sh.cuts[1] = count == 1;
-            sh.weights[0] = run - count;
-            sh.weights[1] = w - sum;
-            sh.weights[2] = w;
-        }
-        __syncthreads();
-        prefix |= (u64)(uint32_t)sh.cuts[0] << shift;
-        base_count = sh.weights[0];
-        base_weight = sh.weights[1];
-        if (shift == 0) break;
-        above = ~(u64)0 << shift;
-        if (sh.cuts[1]) {  // one element is left: its key
-#pragma unroll 4
-            for (int i = tid; i < n; i += kThreads) {
-                const u64 key = key_at(i);
-                if (key && ((key ^ prefix) & above) == 0) sh.rest = key;
-            }
-            __syncthreads();
-            prefix = sh.rest;
-            break;
-        }
-        shift = shift < kBits ? 0 : shift - kBits;
+    for (int i = tid; i < n; i += kThreads) {
+        const u64 key = key_at(i);
+        if (key < limit || ((key ^ d.prefix) & d.above)) continue;
+        const int digit = (int)((key & ~d.above) >> d.shift);
+        atomicAdd(&counts[digit], (u64)1);
+        atomicAdd(&sums[digit], weigh(keys.logit(key)));
     }
-    *weight = sh.weights[2];
-    return prefix;
+    __syncthreads();
+    d.base_count = base_count;
+    d.count = counts[kThreads - 1 - tid];
+    d.weight = sums[kThreads - 1 - tid];
+    d.run_count = base_count + block_scan(d.count, sh.scratch);
+    d.run_weight = base_weight + block_scan(d.weight, sh.scratch);
 }
 
-// The cuts of top-k and, among its elements, of top-p.
-template <typename Source>
-__device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, u64 most, u64 least, const Weights &weigh,
-                                         const RowPlan &plan, const RowParams &rp, u64 base_weight, u64 *memory, Shared &sh) {
+// The smallest run from the start of the order with `k` elements, or with weight >= share where k is 0: its last
+// key, of those >= limit; *weight its weight. `d`: the first step. Where rounding has what comes before the keys
+// reach the share already, the first key.
+template <typename Source, typename Keys>
+__device__ __forceinline__ u64 find_cut(Digits d, const Source &key_at, int n, const Keys &keys, const Weights &weigh, u64 limit,
+                                        u64 k, double share, u64 *weight, u64 *memory, Shared &sh) {
+    const int tid = threadIdx.x;
+    const auto ends = [&](u64 count, u64 sum) { return k ? count >= k : (double)sum >= share; };
+    u64 *few = memory;
+    for (;;) {
+        const u64 count_before = d.run_count - d.count, weight_before = d.run_weight - d.weight;
+        if (d.count && ends(d.run_count, d.run_weight) &&
+            (count_before == d.base_count || !ends(count_before, weight_before))) {
+            sh.cuts[0] = kThreads - 1 - tid;
+            sh.weights[0] = count_before;
+            sh.weights[1] = weight_before;
+            sh.weights[2] = d.run_weight;
+            sh.weights[3] = d.count;
+        }
+        if (tid == 0) sh.cuts[1] = 0;
+        __syncthreads();
+        const u64 base_count = sh.weights[0], base_weight = sh.weights[1], inside = sh.weights[3];
+        d.prefix |= (u64)(uint32_t)sh.cuts[0] << d.shift;
+        d.above = ~(u64)0 << d.shift;
+        if (d.shift == 0) {
+            *weight = sh.weights[2];
+            return d.prefix;
+        }
+        if (inside <= kFew) break;
+        d.shift = d.shift < kDigitBits ? 0 : d.shift - kDigitBits;
+        count_digits(d, key_at, n, keys, weigh, limit, base_count, base_weight, memory, sh);
+    }
+    // A wave's worth of keys: each lane counts what comes before its own.
+    const u64 base_count = sh.weights[0], base_weight = sh.weights[1];
+#pragma unroll 4
+    for (int i = tid; i < n; i += kThreads) {
+        const u64 key = key_at(i);
+        if (key >= limit && ((key ^ d.prefix) & d.above) == 0) few[atomicAdd(&sh.cuts[1], 1)] = key;
+    }
+    __syncthreads();
+    if (tid < 64) {
+        const int m = sh.cuts[1];
+        const u64 key = tid < m ? few[tid] : 0, own = tid < m ? weigh(keys.logit(key)) : 0;
+        u64 count = base_count + 1, sum = base_weight + own;
+        for (int i = 0; i < m; ++i) {
+            const u64 other = few[i], w = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(own >> 32), i) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)own, i);
+            if (other > key) ++count, sum += w;
+        }
+        if (tid < m && ends(count, sum) && (count == base_count + 1 || !ends(count - 1, sum - own))) {
+            sh.rest = key;
+            sh.weights[2] = sum;
+        }
+    }
+    __syncthreads();
+    *weight = sh.weights[2];
+    return sh.rest;
+}
+
+// The cuts of top-k and, among its elements, of top-p; the keys lie in [least, most], after `base_weight`.
+template <typename Source, typename Keys>
+__device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, const Keys &keys, u64 least, u64 most,
+                                         const Weights &weigh, const RowPlan &plan, const RowParams &rp, u64 base_weight,
+                                         u64 *memory, Shared &sh) {
+    const bool by_count = rp.k && (uint32_t)rp.k < plan.valid, by_share = rp.p < 1.0f;
     u64 cut = 1, weight = plan.total;
+    if (!by_count && !by_share) return cut;
+    const int top_bit = 63 - __builtin_clzll(most ^ least);
+    Digits d;
+    d.shift = top_bit < kDigitBits ? 0 : top_bit - kDigitBits + 1;
+    d.above = ~(u64)0 << top_bit << 1;
+    d.prefix = most & d.above;
+    count_digits(d, key_at, n, keys, weigh, cut, plan.above, base_weight, memory, sh);
     for (int pass = 0; pass < 2; ++pass) {
-        const bool by_count = pass == 0;
-        if (by_count ? !(rp.k && (uint32_t)rp.k < plan.valid) : !(rp.p < 1.0f)) continue;
-        cut = find_cut(key_at, n, most, least, weigh, cut, plan.above, base_weight, by_count ? (u64)rp.k : 0,
-                       (double)rp.p * (double)weight, &weight, memory, memory + kThreads, sh);
+        if (pass ? !by_share : !by_count) continue;
+        cut = find_cut(d, key_at, n, keys, weigh, cut, pass ? 0 : (u64)rp.k, (double)rp.p * (double)weight, &weight, memory, sh);
     }
     return cut;
 }
@@ -634,54 +704,48 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const T *row = (const T *)args.logits + r * args.ld;
     const RowParams rp = row_params(args, r);
     const float top = key_logit(plan.top_key);
-    const double low = plan.low;
-    const Weights weigh(top, rp.c);
+    const double c = plan.c, low = plan.low;
+    const Weights weigh(top, c);
+    const OrderKeys<T> keys(args.vocab);
     u64 cut = 1;
     if (plan.state == kCollect) {
         const int n = (int)plan.listed;
         if (n) {
-            u64 most = 0, least = 0;  // (least: the complement's largest)
-            for (int i = tid; i < n; i += kThreads) {
-                const u64 key = row_list(args, scratch)[i];
-                list[i] = key;
-                most = most > key ? most : key;
-                least = least > ~key ? least : ~key;
-            }
-            most = block_reduce(most, MaxOp(), sh.scratch);
-            least = ~block_reduce(least, MaxOp(), sh.scratch);
+            const u64 *from = row_list(args, scratch);
+            for (int i = tid; i < n; i += kThreads) list[i] = from[i];
             const u64 base_weight = block_reduce(above, SumOp(), sh.scratch);
-            cut = find_cuts([&](int i) { return list[i]; }, n, most, least, weigh, plan, rp, base_weight, memory, sh);
+            cut = find_cuts([&](int i) { return list[i]; }, n, keys, keys.least(bin_edge(plan.low_bin - 1)),
+                            keys.most(bin_edge(plan.above_bin + 1)), weigh, plan, rp, base_weight, memory, sh);
             // What min-p leaves of the list's kept elements, to their pieces.
             __syncthreads();
             memory[tid] = 0;
             __syncthreads();
             for (int i = tid; i < n; i += kThreads) {
                 const u64 key = list[i];
-                const float v = key_logit((uint32_t)(key >> 32));
-                if (key >= cut && weighs(v, top, rp.c, low))
-                    atomicAdd(&memory[(0xffffffffu - (uint32_t)key) / kPiece], weigh(v));
+                const float v = keys.logit(key);
+                if (key >= cut && weighs(v, top, c, low)) atomicAdd(&memory[keys.index(key) / kPiece], weigh(v));
             }
             __syncthreads();
             kept += memory[tid];
         }
     } else {
-        cut = find_cuts([&](int i) { return order_key(logit_of(row[i]), i); }, args.vocab, ~(u64)0, 0, weigh, plan, rp, 0,
-                        memory, sh);
+        cut = find_cuts([&](int i) { return keys(logit_of(row[i]), i); }, args.vocab, keys, 0, keys.most(__builtin_inff()),
+                        weigh, plan, rp, 0, memory, sh);
         // The pieces' kept weights, thread by thread.
         kept = 0;
         for (int piece = 0; piece < args.pieces; ++piece) {
             u64 sum = 0;
             for (int i = piece * kPiece + tid; i < (piece + 1) * kPiece && i < args.vocab; i += kThreads) {
                 const float v = logit_of(row[i]);
-                const u64 key = order_key(v, i);
-                if (key >= cut && weighs(v, top, rp.c, low)) sum += weigh(v);
+                const u64 key = keys(v, i);
+                if (key >= cut && weighs(v, top, c, low)) sum += weigh(v);
             }
             sum = block_reduce(sum, SumOp(), sh.scratch);
             if (tid == piece) kept = sum;
         }
     }
     const u64 total = choose_piece(kept, rp.u, sh);
-    locate<T, VECTOR>(args, r, row, sh.chosen, top, rp.c, cut, low, sh.rest, 1.0 / (double)total, sh);
+    locate<T, VECTOR>(args, r, row, sh.chosen, top, c, cut, low, sh.rest, 1.0 / (double)total, sh);
 }
 
 // ---- host -------------------------------------------------------------------------------------------
