@@ -255,34 +255,40 @@ __device__ __forceinline__ u64 draw_of(float u, u64 total) {
     return target < total ? target : total - 1;
 }
 
-// A thread's sixteen logits of the piece at `base`: v, and their indexes through index_of. Past the vocabulary
-// and NaN: -inf. VECTOR: rows whose 16-byte pieces are aligned.
+// A thread's sixteen logits of the piece at `base`, -inf past the vocabulary; their indexes in it are
+// index_of(e). VECTOR: rows whose 16-byte pieces are aligned. (Whole pieces without a branch, so that every load
+// is out before the first is waited for.)
 template <typename T, bool VECTOR>
 __device__ __forceinline__ int index_of(int e) {
     constexpr int kRun = VECTOR ? 16 / (int)sizeof(T) : 1;
     return e / kRun * (kThreads * kRun) + (int)threadIdx.x * kRun + e % kRun;
 }
-template <typename T, bool VECTOR, int RUN>
-__device__ __forceinline__ void load_run(const T *row, int i, int vocab, float *v) {
-    if (VECTOR && i + RUN <= vocab) {
-        const u32x4 w = *(const u32x4 *)(row + i);
+template <typename T, bool VECTOR, typename Index>
+__device__ __forceinline__ void load_logits(const T *row, int base, int vocab, const Index &index, float (&v)[kPer]) {
+    constexpr int kRun = 16 / (int)sizeof(T);
+    if (base + kPiece > vocab) {
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            v[j] = sizeof(T) == 4 ? __uint_as_float(w[j & 3])
-                                  : bf16_bits_to_f32(j & 1 ? w[(j >> 1) & 3] >> 16 : w[(j >> 1) & 3] & 0xffffu);
+        for (int e = 0; e < kPer; ++e) v[e] = base + index(e) < vocab ? logit_of(row[base + index(e)]) : -__builtin_inff();
+    } else if constexpr (VECTOR) {
+        u32x4 w[kPer / kRun];
+#pragma unroll
+        for (int e = 0; e < kPer; e += kRun) w[e / kRun] = *(const u32x4 *)(row + base + index(e));
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const uint32_t word = w[e / kRun][e % kRun * sizeof(T) / 4];
+            v[e] = sizeof(T) == 4 ? __uint_as_float(word) : bf16_bits_to_f32(e & 1 ? word >> 16 : word & 0xffffu);
+        }
     } else {
+        T w[kPer];
 #pragma unroll
-        for (int j = 0; j < RUN; ++j) v[j] = i + j < vocab ? logit_of(row[i + j]) : -__builtin_inff();
+        for (int e = 0; e < kPer; ++e) w[e] = row[base + index(e)];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[e] = logit_of(w[e]);
     }
-#pragma unroll
-    for (int j = 0; j < RUN; ++j) v[j] = v[j] != v[j] ? -__builtin_inff() : v[j];
 }
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void load_piece(const T *row, int base, int vocab, float (&v)[kPer]) {
-    constexpr int kRun = VECTOR ? 16 / (int)sizeof(T) : 1;
-#pragma unroll
-    for (int e = 0; e < kPer; e += kRun)
-        load_run<T, VECTOR, kRun>(row, base + index_of<T, VECTOR>(e), vocab, &v[e]);
+    load_logits<T, VECTOR>(row, base, vocab, [](int e) { return index_of<T, VECTOR>(e); }, v);
 }
 
 struct Shared {
@@ -298,13 +304,11 @@ struct Shared {
 template <typename T, bool VECTOR>
 __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int piece, float top, double c,
                                        u64 cut, double low, u64 target, double scale, Shared &sh) {
-    constexpr int kRun = 16 / (int)sizeof(T);
     const int first = piece * kPiece + (int)threadIdx.x * kPer;
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
     float v[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; e += kRun) load_run<T, VECTOR, kRun>(row, first + e, args.vocab, &v[e]);
+    load_logits<T, VECTOR>(row, piece * kPiece, args.vocab, [](int e) { return (int)threadIdx.x * kPer + e; }, v);
     u64 w[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
