@@ -4,16 +4,17 @@
 // Every filter keeps a run from the start of one total order, larger logits first and of equal ones
 // the lower index, so together they keep {element >= cut} of it (min-p a value bound of its own), and
 // one cut decides the row. The order is that of a 64-bit key: the logit's bits made monotone, then the
-// complement of the index in as many bits as the vocabulary takes. Weights are integers (2^40 for the largest logit of what they are measured
-// against), so that their sums do not depend on the order of the additions.
+// complement of the index in as many bits as the vocabulary takes. What decides between elements is summed in
+// integers (2^40 for the row's largest logit), so that no order of additions matters.
 //
 // Four launches; a workgroup takes a piece of 8192 logits, or a row:
-//   scan    (pieces) the piece's largest logit and its weight, and for rows with a cut how many elements
-//           and how much weight fall into each of 512 value bins below its largest;
-//   settle  (rows)   greedy rows and those with the temperature alone are settled, from one piece more;
+//   scan    (pieces) the piece's largest logit, the weight of each wave's strip of 1024 against it, and for
+//           rows with a cut how many elements and how much weight fall into each of 512 value bins
+//           below it;
+//   settle  (rows)   greedy rows and those with the temperature alone are settled, from one strip more;
 //           for the others, the bins that the cut can be in;
-//   collect (pieces) the weight above these bins, and the elements in them as a list;
-//   finish  (rows)   the cut, by a radix search in the list, the piece the draw falls into and the token
+//   collect (pieces) each strip's weight above these bins, and the elements in them as a list;
+//   finish  (rows)   the cut, by a radix search in the list, the strip the draw falls into and the token
 //           in it. A row whose cut lies below its bins, or in bins of more elements than the list
 //           holds, is searched whole.
 // The launches over pieces hold nothing but what they stream, so that four workgroups share a CU.
@@ -26,14 +27,16 @@ namespace splosh {
 constexpr size_t kSampleCounterBytes = 16384;
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kPer = 16;                     // logits a thread
+constexpr int kStrip = 64 * kPer;            // a wave
 constexpr int kPiece = kThreads * kPer;      // and a workgroup
 constexpr int kBins = kThreads;              // value bins of a piece
-constexpr int kList = 8192;                  // elements of a row's list
-constexpr int kBatchRows = 256;              // rows of one launch
 constexpr int kWeightBits = 40;
 // A bin's entry while it is counted: 15 bits of count (a piece has 2^13 elements) over 49 of weight in units of
-// 2^-35; as it is left, the count over the fp32 weight.
+// 2^-35; as it is left, the count over the fp32 weight in units of 2^-40.
 constexpr int kBinShift = 49, kBinUnit = kWeightBits - 35;
+constexpr int kMaxStrips = (int)(kSampleMaxVocab / kStrip);
+constexpr int kList = 8192;                  // elements of a row's list
+constexpr int kBatchRows = 256;              // rows of one launch
 
 static_assert((int64_t)kPiece * kThreads >= kSampleMaxVocab, "a row's pieces are one a thread");
 
@@ -96,6 +99,15 @@ struct Weights {
     // m 2^32 (m: 24 bits and the power's) moved down to m 2^(40 - 24) at the exponent 0, or 1 less where the
     // two whole numbers are rounded apart.
     static constexpr int kShift = 32 - (kWeightBits - 24);
+    // The same as a number, 1 at top; top finite. NaN and -inf weigh nothing.
+    __device__ __forceinline__ float relative(float v) const {
+#pragma clang fp contract(off)
+        const float d = v - s, n = __builtin_rintf(d * c_high);
+        const float f = __builtin_fmaf(d, c_high, -n) + __builtin_fmaf(d, c_low, -fraction);
+        // (Far below top f can be anything.)
+        const float e = __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_exp2f(f), 0.0f), 4.0f);
+        return __builtin_ldexpf(e, (int)__builtin_fmaxf(n - (shift0 - (float)kShift), -200.0f));
+    }
     __device__ __forceinline__ u64 operator()(float v) const {
 #pragma clang fp contract(off)  // (n is the rounded product's)
         const float d = v - s, n = __builtin_rintf(d * c_high);
@@ -183,6 +195,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 *scratch) {
 
 // ---- what the launches leave for each other ---------------------------------------------------------
 
+constexpr int kNoBin = -0x7fffffff;  // (as low_bin and above_bin: nothing goes to the list)
 enum RowState : int { kSettled = 0, kCollect = 1, kSearch = 2 };
 
 struct RowPlan {
@@ -194,14 +207,16 @@ struct RowPlan {
     uint32_t valid, reserved;  // valid: elements that can be chosen
     double c, low;     // log2(e) / T; log2(min_p), -inf where it is off
 };
-// A piece. key: its largest logit's << 32 | the index of that (greedy rows).
-struct PieceHead {
-    u64 key, weight, valid;  // scan: its weight, of its own largest logit; its elements that can be chosen
-    u64 above, kept;         // collect: the weight above the list's bins, and of it what min-p leaves
+// A wave's strip of a piece.
+struct Strip {
+    u64 weight;       // scan: of its piece's largest logit
+    u64 above, kept;  // collect: the weight above the list's bins, and of it what min-p leaves
 };
 struct RowScratch {
     RowPlan plan;
-    PieceHead heads[1];  // [pieces], then the bins u64 [pieces][kBins], then the list u64 [kList]
+    // [pieces] its largest logit's key << 32 | the index of that (greedy rows); [pieces] elements that can be chosen;
+    // [strips] Strip; [pieces][kBins] count << 32 | fp32 weight; [kList] the list.
+    u64 heads[1];
 };
 
 struct SampleArgs {
@@ -218,8 +233,12 @@ struct SampleArgs {
 __device__ __forceinline__ RowScratch &row_scratch(const SampleArgs &args, int r) {
     return *(RowScratch *)(args.rows + r * args.row_bytes);
 }
+__device__ __forceinline__ u64 *row_valid(const SampleArgs &args, RowScratch &row) { return row.heads + args.pieces; }
+__device__ __forceinline__ Strip *row_strips(const SampleArgs &args, RowScratch &row) {
+    return (Strip *)(row_valid(args, row) + args.pieces);
+}
 __device__ __forceinline__ u64 *row_bins(const SampleArgs &args, RowScratch &row) {
-    return (u64 *)&row.heads[args.pieces];
+    return (u64 *)(row_strips(args, row) + args.pieces * kWaves);
 }
 __device__ __forceinline__ u64 *row_list(const SampleArgs &args, RowScratch &row) {
     return row_bins(args, row) + (size_t)args.pieces * kBins;
@@ -256,15 +275,16 @@ __device__ __forceinline__ u64 draw_of(float u, u64 total) {
 }
 
 // A thread's sixteen logits of the piece at `base`, -inf past the vocabulary; their indexes in it are
-// index_of(e). VECTOR: rows whose 16-byte pieces are aligned. (Whole pieces without a branch, so that every load
+// index_of(e), a wave's a strip. VECTOR: rows whose 16-byte pieces are aligned. (Whole pieces without a branch, so that every load
 // is out before the first is waited for.)
 template <typename T, bool VECTOR>
 __device__ __forceinline__ int index_of(int e) {
     constexpr int kRun = VECTOR ? 16 / (int)sizeof(T) : 1;
-    return e / kRun * (kThreads * kRun) + (int)threadIdx.x * kRun + e % kRun;
+    return (int)(threadIdx.x >> 6) * kStrip + e / kRun * (64 * kRun) + (int)(threadIdx.x & 63) * kRun + e % kRun;
 }
-template <typename T, bool VECTOR, typename Index>
-__device__ __forceinline__ void load_logits(const T *row, int base, int vocab, const Index &index, float (&v)[kPer]) {
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load_piece(const T *row, int base, int vocab, float (&v)[kPer]) {
+    const auto index = [](int e) { return index_of<T, VECTOR>(e); };
     constexpr int kRun = 16 / (int)sizeof(T);
     if (base + kPiece > vocab) {
 #pragma unroll
@@ -286,40 +306,70 @@ __device__ __forceinline__ void load_logits(const T *row, int base, int vocab, c
         for (int e = 0; e < kPer; ++e) v[e] = logit_of(w[e]);
     }
 }
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void load_piece(const T *row, int base, int vocab, float (&v)[kPer]) {
-    load_logits<T, VECTOR>(row, base, vocab, [](int e) { return index_of<T, VECTOR>(e); }, v);
-}
-
 struct Shared {
     u64 scratch[kWaves];
     int chosen;
+    double fraction;
     u64 rest;
     int cuts[4];
     u64 weights[4];
 };
 
-// The token of the row: the first index of the piece whose running weight over the kept elements (order key
-// >= cut, weight of the row's largest at least 2^low) exceeds `target`. Its probability: its weight times scale.
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int piece, float top, double c,
-                                       u64 cut, double low, u64 target, double scale, Shared &sh) {
-    const int first = piece * kPiece + (int)threadIdx.x * kPer;
+// The strip the draw falls into, strips one after the other (weight_of(s) for s < strips): sh.chosen, and how far
+// into its weight. Returns the whole weight.
+template <typename F>
+__device__ __forceinline__ u64 choose_strip(const F &weight_of, int strips, float u, Shared &sh) {
+    const int each = (strips + kThreads - 1) / kThreads, first = (int)threadIdx.x * each;
+    u64 mine = 0;
+    for (int s = first; s < first + each && s < strips; ++s) mine += weight_of(s);
+    const u64 run = block_scan(mine, sh.scratch);
+    u64 total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) total += sh.scratch[i];
+    const u64 target = draw_of(u, total);
+    if (run > target && run - mine <= target) {
+        u64 rest = target - (run - mine);
+        int s = first;
+        u64 w = weight_of(s);
+        while (rest >= w) {
+            rest -= w;
+            w = weight_of(++s);
+        }
+        sh.chosen = s;
+        sh.fraction = (double)rest / (double)w;
+    }
+    __syncthreads();
+    return total;
+}
+
+// The token of the row: the first index of the strip whose running weight over the kept elements (order key
+// >= cut, weight of the row's largest at least 2^low) exceeds `fraction` of the strip's. Its probability: its
+// weight times scale.
+template <typename T>
+__device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int strip, float top, double c,
+                                       u64 cut, double low, double fraction, double scale, Shared &sh) {
+    constexpr int kEach = kStrip / kThreads;
+    const int first = strip * kStrip + (int)threadIdx.x * kEach;
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
-    float v[kPer];
-    load_logits<T, VECTOR>(row, piece * kPiece, args.vocab, [](int e) { return (int)threadIdx.x * kPer + e; }, v);
-    u64 w[kPer], sum = 0;
+    float v[kEach];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
+    for (int e = 0; e < kEach; ++e) v[e] = first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
+    u64 w[kEach], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
         const u64 key = keys(v[e], first + e);
         w[e] = key && key >= cut && weighs(v[e], top, c, low) ? weigh(v[e]) : 0;
         sum += w[e];
     }
-    u64 run = block_scan(sum, sh.scratch) - sum, found = 0;
+    u64 run = block_scan(sum, sh.scratch) - sum, total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) total += sh.scratch[i];
+    u64 target = (u64)(fraction * (double)total), found = 0;
+    target = target < total ? target : total - 1;
     int at = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
+    for (int e = 0; e < kEach; ++e) {
         if (run <= target && target < run + w[e]) at = e, found = w[e];
         run += w[e];
     }
@@ -327,21 +377,6 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
         args.tokens[r] = (uint32_t)(first + at);
         if (args.logprobs) args.logprobs[r] = (float)log((double)found * scale);
     }
-}
-
-// The piece the draw falls into, from its weight in thread `piece`; the rest of the target there.
-__device__ __forceinline__ u64 choose_piece(u64 weight, float u, Shared &sh) {
-    const u64 run = block_scan(weight, sh.scratch);
-    u64 total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) total += sh.scratch[i];
-    const u64 target = draw_of(u, total);
-    if (run > target && run - weight <= target) {
-        sh.chosen = (int)threadIdx.x;
-        sh.rest = target - (run - weight);
-    }
-    __syncthreads();
-    return total;
 }
 
 // ---- scan -------------------------------------------------------------------------------------------
@@ -362,19 +397,19 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 #pragma unroll
     for (int e = 0; e < kPer; ++e) best = __builtin_fmaxf(best, v[e]);
     const uint32_t best_key = block_reduce(logit_key(best), MaxOp(), scratch);
-    u64 weight = 0, index = 0;
-    uint32_t valid = 0;
     const float top = key_logit(best_key);
+    u64 index = 0, weight = 0;
+    uint32_t valid = 0;
     if (rp.greedy) {
         uint32_t at = 0;  // (the complement: the first index is the largest)
 #pragma unroll
         for (int e = kPer - 1; e >= 0; --e)
             if (v[e] == top) at = ~(uint32_t)(piece * kPiece + index_of<T, VECTOR>(e));
         index = ~block_reduce(at, MaxOp(), scratch);
-    } else if (best_key) {
-        const int top_bin = value_bin(top);
-        const Weights weigh(top, rp.c);
-        if (cut) {
+    } else if (cut) {
+        if (best_key) {
+            const int top_bin = value_bin(top);
+            const Weights weigh(top, rp.c);
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
                 const u64 w = weigh(v[e]);
@@ -384,19 +419,27 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
                 const int below = top_bin - value_bin(v[e]);
                 if (live && below < kBins) atomicAdd(&bins[below], (u64)1 << kBinShift | w >> kBinUnit);
             }
-            valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
-        } else {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) weight += weigh(v[e]);
         }
-        weight = block_reduce(weight, SumOp(), scratch);
+        if (rp.k) valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
+    } else if (best_key) {
+        // (A lane's sixteen in fp32, the lanes in integers. Where the largest is infinite, those that are.)
+        const bool infinite = top == __builtin_inff();
+        const Weights weigh(infinite ? 0.0f : top, rp.c);
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum += infinite ? (v[e] == top ? 1.0f : 0.0f) : weigh.relative(v[e]);
+        weight = (u64)(sum * (float)((u64)1 << kWeightBits));
+    }
+    if (!rp.greedy) {
+        weight = wave_scan(weight, SumOp());
+        if ((tid & 63) == 63) row_strips(args, row)[piece * kWaves + (tid >> 6)].weight = weight;
     }
     if (tid == 0) {
-        row.heads[piece].key = (u64)best_key << 32 | index;
-        row.heads[piece].weight = weight;
-        row.heads[piece].valid = valid;
+        row.heads[piece] = (u64)best_key << 32 | index;
+        row_valid(args, row)[piece] = valid;
     }
     if (cut) {
+        __syncthreads();
         const u64 entry = bins[tid];
         const float w = (float)((entry & (((u64)1 << kBinShift) - 1)) << kBinUnit);
         row_bins(args, row)[(size_t)piece * kBins + tid] = entry >> kBinShift << 32 | __float_as_uint(w);
@@ -408,25 +451,26 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 // 2^t for t <= 0, in 64 bits.
 __device__ __forceinline__ double power_of(double t) { return t > -1000.0 ? exp2(t) : 0.0; }
 
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args) {
     __shared__ Shared sh;
-    __shared__ float factors[kThreads];  // the pieces' weights in the row's
+    __shared__ double factors[kThreads];  // the pieces' weights in the row's
     __shared__ int top_bins[kThreads];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, strips = args.pieces * kWaves;
     const int64_t r = blockIdx.x;
     const T *row = (const T *)args.logits + r * args.ld;
     RowScratch &scratch = row_scratch(args, (int)r);
     const RowParams rp = row_params(args, r);
     const bool cut = !rp.greedy && (rp.k || rp.p < 1.0f);
     // One piece a thread.
-    PieceHead head = {0, 0, 0, 0, 0};
-    if (tid < args.pieces) head.key = scratch.heads[tid].key, head.weight = scratch.heads[tid].weight, head.valid = scratch.heads[tid].valid;
-    const uint32_t piece_key = (uint32_t)(head.key >> 32), top_key = block_reduce(piece_key, MaxOp(), sh.scratch);
+    const u64 head = tid < args.pieces ? scratch.heads[tid] : 0;
+    const u64 piece_valid = tid < args.pieces ? row_valid(args, scratch)[tid] : 0;
+    const u64 strip_weight = tid < strips ? row_strips(args, scratch)[tid].weight : 0;  // (the first 512)
+    const uint32_t piece_key = (uint32_t)(head >> 32), top_key = block_reduce(piece_key, MaxOp(), sh.scratch);
     RowPlan &plan = scratch.plan;
     if (rp.greedy || top_key == 0) {
         // Of the pieces that have the largest, the first index.
-        const uint32_t at = ~block_reduce(piece_key == top_key ? ~(uint32_t)head.key : 0u, MaxOp(), sh.scratch);
+        const uint32_t at = ~block_reduce(piece_key == top_key ? ~(uint32_t)head : 0u, MaxOp(), sh.scratch);
         if (tid == 0) {
             args.tokens[r] = top_key ? at : 0xffffffffu;
             if (args.logprobs) args.logprobs[r] = top_key ? 0.0f : -__builtin_inff();
@@ -435,35 +479,33 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
         return;
     }
     const float top = key_logit(top_key), piece_top = key_logit(piece_key);
-    const double factor = piece_key == 0 ? 0.0
-                          : piece_key == top_key ? 1.0 : power_of(((double)piece_top - (double)top) * rp.c);
-    const u64 row_weight = (u64)((double)head.weight * factor);
+    factors[tid] = piece_key == 0 ? 0.0
+                   : piece_key == top_key ? 1.0 : power_of(((double)piece_top - (double)top) * rp.c);
+    __syncthreads();
+    const auto weight_of = [&](int s) {
+        return (u64)((double)(s == tid ? strip_weight : row_strips(args, scratch)[s].weight) * factors[s / kWaves]);
+    };
     if (!cut && rp.q == 0.0f) {  // the temperature alone
-        const u64 total = choose_piece(row_weight, rp.u, sh);
-        __shared__ double chosen_factor;
-        __shared__ u64 chosen_weight;
-        __shared__ uint32_t chosen_key;
-        if (tid == sh.chosen) chosen_factor = factor, chosen_weight = head.weight, chosen_key = piece_key;
-        __syncthreads();
-        u64 target = (u64)((double)sh.rest / chosen_factor);
-        target = target < chosen_weight ? target : chosen_weight - 1;
-        locate<T, VECTOR>(args, r, row, sh.chosen, key_logit(chosen_key), rp.c, 1, -__builtin_inf(), target,
-                          chosen_factor / (double)total, sh);
+        const u64 total = choose_strip(weight_of, strips, rp.u, sh);
+        const int piece = sh.chosen / kWaves;
+        locate<T>(args, r, row, sh.chosen, key_logit((uint32_t)(scratch.heads[piece] >> 32)), rp.c, 1, -__builtin_inf(),
+                  sh.fraction, factors[piece] / (double)total, sh);
         if (tid == 0) plan.state = kSettled;
         return;
     }
+    u64 row_weight = 0;
+    for (int s = tid; s < strips; s += kThreads) row_weight += weight_of(s);
     const u64 total = block_reduce(row_weight, SumOp(), sh.scratch);
-    const u64 valid = rp.k ? block_reduce(head.valid, SumOp(), sh.scratch) : 0;
+    const u64 valid = rp.k ? block_reduce(piece_valid, SumOp(), sh.scratch) : 0;
     // The least (v - top) c of what min-p keeps.
     const double low = rp.q > 0.0f ? log2((double)rp.q) : -__builtin_inf();
     const bool by_count = rp.k && (u64)rp.k < valid, by_share = rp.p < 1.0f;
     if (!by_count && !by_share) {  // min-p alone, or with a k past what the row has: everything is above the list
-        if (tid == 0) plan = {kCollect, -0x7fffffff, -0x7fffffff, top_key, total, 0, 0, (uint32_t)valid, 0, rp.c, low};
+        if (tid == 0) plan = {kCollect, kNoBin, kNoBin, top_key, total, 0, 0, (uint32_t)valid, 0, rp.c, low};
         return;
     }
     // The row's bins: thread j the j-th below that of its largest logit.
     const int top_bin = value_bin(top);
-    factors[tid] = (float)factor;
     top_bins[tid] = piece_key ? value_bin(piece_top) : -0x40000000;
     if (tid < 4) sh.cuts[tid] = kBins;
     __syncthreads();
@@ -481,7 +523,7 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
 #pragma unroll
         for (int e = 0; e < kAtOnce; ++e) {
             count += (uint32_t)(entry[e] >> 32);
-            bin_weight = __builtin_fmaf(__uint_as_float((uint32_t)entry[e]), factors[(first + e) & (kThreads - 1)], bin_weight);
+            bin_weight = __builtin_fmaf(__uint_as_float((uint32_t)entry[e]), (float)factors[(first + e) & (kThreads - 1)], bin_weight);
         }
     }
     const u64 own_weight = (u64)bin_weight, run_count = block_scan(count, sh.scratch),
@@ -519,20 +561,19 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
 
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs args) {
-    __shared__ u64 scratch[kWaves];
     const int piece = blockIdx.x, lane = threadIdx.x & 63;
     const int64_t r = blockIdx.y;
     RowScratch &row = row_scratch(args, (int)r);
     const RowPlan &plan = row.plan;
     const int state = plan.state, low_bin = plan.low_bin, above_bin = plan.above_bin;
-    const uint32_t piece_key = (uint32_t)(row.heads[piece].key >> 32);
+    const uint32_t piece_key = (uint32_t)(row.heads[piece] >> 32);
     const float top = key_logit(plan.top_key), piece_top = key_logit(piece_key);
     const double c = plan.c, low = plan.low;
     if (state != kCollect) return;
     u64 above = 0, kept = 0;
     // (A piece whose largest is below the list's bins, or below min-p with no list, has nothing to give.)
-    if (piece_key && value_bin(piece_top) >= low_bin &&
-        (low_bin != -0x7fffffff || weighs(piece_top, top, c, low))) {
+    const bool listing = low_bin != kNoBin;
+    if (piece_key && value_bin(piece_top) >= low_bin && (listing || weighs(piece_top, top, c, low))) {
         const Weights weigh(top, c);
         float v[kPer];
         load_piece<T, VECTOR>((const T *)args.logits + r * args.ld, piece * kPiece, args.vocab, v);
@@ -542,9 +583,12 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
             const int bin = value_bin(v[e]);
             if (v[e] > -__builtin_inff() && bin >= low_bin) {
                 if (bin >= above_bin) {
-                    const u64 w = weigh(v[e]);
-                    above += w;
-                    if (weighs(v[e], top, c, low)) kept += w;
+                    const bool keep = weighs(v[e], top, c, low);
+                    if (keep || listing) {
+                        const u64 w = weigh(v[e]);
+                        above += w;
+                        kept += keep ? w : 0;
+                    }
                 } else {
                     listed |= 1u << e;
                 }
@@ -566,12 +610,13 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
                     ++at;
                 }
         }
-        above = block_reduce(above, SumOp(), scratch);
-        kept = block_reduce(kept, SumOp(), scratch);
+        above = wave_scan(above, SumOp());
+        kept = wave_scan(kept, SumOp());
     }
-    if (threadIdx.x == 0) {
-        row.heads[piece].above = above;
-        row.heads[piece].kept = kept;
+    if (lane == 63) {
+        Strip &strip = row_strips(args, row)[piece * kWaves + (threadIdx.x >> 6)];
+        strip.above = above;
+        strip.kept = kept;
     }
 }
 
@@ -694,17 +739,18 @@ __device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, const Keys
     return cut;
 }
 
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args) {
     __shared__ Shared sh;
-    __shared__ u64 list[kList], memory[2 * kThreads];
-    const int tid = threadIdx.x;
+    __shared__ u64 list[kList], memory[2 * kThreads], extra[kMaxStrips];
+    const int tid = threadIdx.x, strips = args.pieces * kWaves;
     const int64_t r = blockIdx.x;
     RowScratch &scratch = row_scratch(args, (int)r);
     const RowPlan plan = scratch.plan;
+    const Strip *of = row_strips(args, scratch);
+    const u64 strip_kept = tid < strips ? of[tid].kept : 0;  // (the first 512)
+    u64 above = tid < strips ? of[tid].above : 0;
     if (plan.state == kSettled) return;
-    u64 kept = 0, above = 0;
-    if (tid < args.pieces) kept = scratch.heads[tid].kept, above = scratch.heads[tid].above;
     const T *row = (const T *)args.logits + r * args.ld;
     const RowParams rp = row_params(args, r);
     const float top = key_logit(plan.top_key);
@@ -712,44 +758,31 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
     u64 cut = 1;
-    if (plan.state == kCollect) {
-        const int n = (int)plan.listed;
-        if (n) {
-            const u64 *from = row_list(args, scratch);
-            for (int i = tid; i < n; i += kThreads) list[i] = from[i];
-            const u64 base_weight = block_reduce(above, SumOp(), sh.scratch);
-            cut = find_cuts([&](int i) { return list[i]; }, n, keys, keys.least(bin_edge(plan.low_bin - 1)),
-                            keys.most(bin_edge(plan.above_bin + 1)), weigh, plan, rp, base_weight, memory, sh);
-            // What min-p leaves of the list's kept elements, to their pieces.
-            __syncthreads();
-            memory[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
-                const u64 key = list[i];
-                const float v = keys.logit(key);
-                if (key >= cut && weighs(v, top, c, low)) atomicAdd(&memory[keys.index(key) / kPiece], weigh(v));
-            }
-            __syncthreads();
-            kept += memory[tid];
-        }
-    } else {
+    const bool listed = plan.state == kCollect;
+    const int n = listed ? (int)plan.listed : 0;
+    for (int s = tid; s < strips; s += kThreads) extra[s] = 0;
+    if (n) {
+        const u64 *from = row_list(args, scratch);
+        for (int i = tid; i < n; i += kThreads) list[i] = from[i];
+        for (int s = tid + kThreads; s < strips; s += kThreads) above += of[s].above;
+        const u64 base_weight = block_reduce(above, SumOp(), sh.scratch);
+        cut = find_cuts([&](int i) { return list[i]; }, n, keys, keys.least(bin_edge(plan.low_bin - 1)),
+                        keys.most(bin_edge(plan.above_bin + 1)), weigh, plan, rp, base_weight, memory, sh);
+    } else if (!listed) {
         cut = find_cuts([&](int i) { return keys(logit_of(row[i]), i); }, args.vocab, keys, 0, keys.most(__builtin_inff()),
                         weigh, plan, rp, 0, memory, sh);
-        // The pieces' kept weights, thread by thread.
-        kept = 0;
-        for (int piece = 0; piece < args.pieces; ++piece) {
-            u64 sum = 0;
-            for (int i = piece * kPiece + tid; i < (piece + 1) * kPiece && i < args.vocab; i += kThreads) {
-                const float v = logit_of(row[i]);
-                const u64 key = keys(v, i);
-                if (key >= cut && weighs(v, top, c, low)) sum += weigh(v);
-            }
-            sum = block_reduce(sum, SumOp(), sh.scratch);
-            if (tid == piece) kept = sum;
-        }
     }
-    const u64 total = choose_piece(kept, rp.u, sh);
-    locate<T, VECTOR>(args, r, row, sh.chosen, top, c, cut, low, sh.rest, 1.0 / (double)total, sh);
+    // What min-p leaves of the kept elements of the list, or of the row, to their strips.
+    __syncthreads();
+    for (int i = tid; i < (listed ? n : args.vocab); i += kThreads) {
+        const u64 key = listed ? list[i] : keys(logit_of(row[i]), i);
+        const float v = keys.logit(key);
+        if (key >= cut && weighs(v, top, c, low)) atomicAdd(&extra[keys.index(key) / kStrip], weigh(v));
+    }
+    __syncthreads();
+    const u64 total = choose_strip(
+        [&](int s) { return extra[s] + (!listed ? 0 : s == tid ? strip_kept : of[s].kept); }, strips, rp.u, sh);
+    locate<T>(args, r, row, sh.chosen, top, c, cut, low, sh.fraction, 1.0 / (double)total, sh);
 }
 
 // ---- host -------------------------------------------------------------------------------------------
@@ -757,7 +790,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
 static int64_t pieces_of(int64_t vocab) { return (vocab + kPiece - 1) / kPiece; }
 static size_t row_bytes(int64_t vocab) {
     const int64_t pieces = pieces_of(vocab);
-    const size_t bytes = sizeof(RowPlan) + pieces * sizeof(PieceHead) + pieces * kBins * sizeof(u64) + kList * sizeof(u64);
+    const size_t bytes = sizeof(RowPlan) + pieces * (2 * sizeof(u64) + kWaves * sizeof(Strip) + kBins * sizeof(u64)) +
+                         kList * sizeof(u64);
     return (bytes + 255) / 256 * 256;
 }
 
@@ -769,10 +803,10 @@ template <typename T, bool VECTOR>
 static void launch_batch(const SampleArgs &args, int rows, hipStream_t stream) {
     const dim3 pieces((unsigned)args.pieces, (unsigned)rows), whole((unsigned)rows);
     hipLaunchKernelGGL((sample_scan_kernel<T, VECTOR>), pieces, dim3(kThreads), 0, stream, args);
-    hipLaunchKernelGGL((sample_settle_kernel<T, VECTOR>), whole, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL((sample_settle_kernel<T>), whole, dim3(kThreads), 0, stream, args);
     if (!args.p.uniforms || (!args.p.top_k && !args.p.top_p && !args.p.min_p)) return;  // every row is settled
     hipLaunchKernelGGL((sample_collect_kernel<T, VECTOR>), pieces, dim3(kThreads), 0, stream, args);
-    hipLaunchKernelGGL((sample_finish_kernel<T, VECTOR>), whole, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL((sample_finish_kernel<T>), whole, dim3(kThreads), 0, stream, args);
 }
 
 hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab,
