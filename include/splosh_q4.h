@@ -478,7 +478,7 @@ size_t splosh_sample_workspace_bytes(int64_t rows, int64_t vocab);
  *     NaN as 0, u >= 1: the last kept entry with weight); its logprob is ln(w / whole weight).
  * temperature NULL: 1; top_k, top_p, min_p NULL: off; uniforms NULL: every row as with T = 0.
  * logprobs may be NULL. Weights are summed in 64-bit fixed point, 2^-40 of the largest weight (less
- * counts as none), so the result depends on no order of additions. vocab <= 2^22. The workspace is
+ * counts as none), so the result depends on no order of additions. vocab <= 2^21. The workspace is
  * zero-filled before its first use and shared as splosh_workspace_bytes describes (its arrival
  * counters are zero between calls). */
 int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float *uniforms,

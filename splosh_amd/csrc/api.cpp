@@ -1246,7 +1246,7 @@ int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64
     if (rows <= 0 || vocab <= 0) return fail(SPLOSH_ERR_INVALID_SHAPE, "rows and vocab must be positive");
     if (ld < vocab) return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "ld is shorter than vocab");
     if (dtype != SPLOSH_F32 && dtype != SPLOSH_BF16) return fail(SPLOSH_ERR_UNSUPPORTED, "unknown logits dtype");
-    if (vocab > splosh::kSampleMaxVocab) return fail(SPLOSH_ERR_UNSUPPORTED, "vocab above 2^22");
+    if (vocab > splosh::kSampleMaxVocab) return fail(SPLOSH_ERR_UNSUPPORTED, "vocab above 2^21");
     if (mul_overflows(rows, ld)) return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "size overflows");
     if (rows > INT32_MAX) return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows");
     if (!aligned(logits, dtype == SPLOSH_F32 ? 4 : 2) || !aligned(tokens, 4) || !aligned(logprobs, 4) ||

@@ -301,7 +301,7 @@ hipError_t launch_adapters(const splosh_adapters *adapters, int group, const uin
                            void *workspace, hipStream_t stream);
 
 // Sampling (sample.hip).
-constexpr int64_t kSampleMaxVocab = 1 << 22;
+constexpr int64_t kSampleMaxVocab = 1 << 21;
 struct SampleParams {
     const float *uniforms, *temperature;  // null uniforms: greedy
     const int32_t *top_k;

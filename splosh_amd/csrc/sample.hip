@@ -34,11 +34,11 @@ constexpr int kWeightBits = 40;
 // A bin's entry while it is counted: 15 bits of count (a piece has 2^13 elements) over 49 of weight in units of
 // 2^-35; as it is left, the count over the fp32 weight in units of 2^-40.
 constexpr int kBinShift = 49, kBinUnit = kWeightBits - 35;
-constexpr int kMaxStrips = (int)(kSampleMaxVocab / kStrip);
+constexpr int kMaxStrips = kThreads * kWaves;
 constexpr int kList = 8192;                  // elements of a row's list
 constexpr int kBatchRows = 256;              // rows of one launch
 
-static_assert((int64_t)kPiece * kThreads >= kSampleMaxVocab, "a row's pieces are one a thread");
+static_assert((int64_t)kPiece * kThreads >= kSampleMaxVocab + 7, "a row's pieces are one a thread");
 
 typedef unsigned long long u64;
 
@@ -274,38 +274,54 @@ __device__ __forceinline__ u64 draw_of(float u, u64 total) {
     return target < total ? target : total - 1;
 }
 
-// A thread's sixteen logits of the piece at `base`, -inf past the vocabulary; their indexes in it are
-// index_of(e), a wave's a strip. VECTOR: rows whose 16-byte pieces are aligned. (Whole pieces without a branch, so that every load
-// is out before the first is waited for.)
-template <typename T, bool VECTOR>
+// The pieces of a row begin at the 16-byte boundary at or before it, `lead` elements early, so that their 16-byte
+// parts are aligned whatever the row's alignment.
+template <typename T>
+__device__ __forceinline__ int row_lead(const T *row) {
+    return (int)((uintptr_t)row % 16 / sizeof(T));
+}
+// A thread's sixteen logits of the piece at `base`, -inf outside the row; their indexes are base + index_of(e), a
+// wave's a strip. (Whole pieces without a branch, so that every load is out before the first is waited for.)
+template <typename T>
 __device__ __forceinline__ int index_of(int e) {
-    constexpr int kRun = VECTOR ? 16 / (int)sizeof(T) : 1;
+    constexpr int kRun = 16 / (int)sizeof(T);
     return (int)(threadIdx.x >> 6) * kStrip + e / kRun * (64 * kRun) + (int)(threadIdx.x & 63) * kRun + e % kRun;
 }
-template <typename T, bool VECTOR>
+template <typename T>
 __device__ __forceinline__ void load_piece(const T *row, int base, int vocab, float (&v)[kPer]) {
-    const auto index = [](int e) { return index_of<T, VECTOR>(e); };
     constexpr int kRun = 16 / (int)sizeof(T);
-    if (base + kPiece > vocab) {
+    u32x4 w[kPer / kRun];
+    const bool whole = base >= 0 && base + kPiece <= vocab;
+    if (whole) {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) v[e] = base + index(e) < vocab ? logit_of(row[base + index(e)]) : -__builtin_inff();
-    } else if constexpr (VECTOR) {
-        u32x4 w[kPer / kRun];
-#pragma unroll
-        for (int e = 0; e < kPer; e += kRun) w[e / kRun] = *(const u32x4 *)(row + base + index(e));
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const uint32_t word = w[e / kRun][e % kRun * sizeof(T) / 4];
-            v[e] = sizeof(T) == 4 ? __uint_as_float(word) : bf16_bits_to_f32(e & 1 ? word >> 16 : word & 0xffffu);
-        }
+        for (int e = 0; e < kPer; e += kRun) w[e / kRun] = *(const u32x4 *)(row + base + index_of<T>(e));
     } else {
-        T w[kPer];
+        constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) w[e] = row[base + index(e)];
+        for (int e = 0; e < kPer; e += kRun) {
+            const int i = base + index_of<T>(e);
+            w[e / kRun] = u32x4{kNone, kNone, kNone, kNone};
+            if (i >= 0 && i + kRun <= vocab) w[e / kRun] = *(const u32x4 *)(row + i);
+        }
+    }
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) v[e] = logit_of(w[e]);
+    for (int e = 0; e < kPer; ++e) {
+        const uint32_t word = w[e / kRun][e % kRun * sizeof(T) / 4];
+        v[e] = sizeof(T) == 4 ? __uint_as_float(word) : bf16_bits_to_f32(e & 1 ? word >> 16 : word & 0xffffu);
+    }
+    if (!whole) {  // the parts that the row begins or ends in
+#pragma unroll
+        for (int e = 0; e < kPer; e += kRun) {
+            const int i = base + index_of<T>(e);
+            if ((i < 0 && i + kRun > 0) || (i < vocab && i + kRun > vocab)) {
+#pragma unroll
+                for (int j = 0; j < kRun; ++j)
+                    if (i + j >= 0 && i + j < vocab) v[e + j] = logit_of(row[i + j]);
+            }
+        }
     }
 }
+
 struct Shared {
     u64 scratch[kWaves];
     int chosen;
@@ -349,12 +365,13 @@ template <typename T>
 __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int strip, float top, double c,
                                        u64 cut, double low, double fraction, double scale, Shared &sh) {
     constexpr int kEach = kStrip / kThreads;
-    const int first = strip * kStrip + (int)threadIdx.x * kEach;
+    const int first = strip * kStrip - row_lead(row) + (int)threadIdx.x * kEach;
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
     float v[kEach];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e] = first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
+    for (int e = 0; e < kEach; ++e)
+        v[e] = first + e >= 0 && first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
     u64 w[kEach], sum = 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -381,14 +398,16 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
 
 // ---- scan -------------------------------------------------------------------------------------------
 
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) {
     __shared__ u64 scratch[kWaves];
     __shared__ u64 bins[kBins];
     const int tid = threadIdx.x, piece = blockIdx.x;
     const int64_t r = blockIdx.y;
+    const T *logits = (const T *)args.logits + r * args.ld;
+    const int base = piece * kPiece - row_lead(logits);
     float v[kPer];
-    load_piece<T, VECTOR>((const T *)args.logits + r * args.ld, piece * kPiece, args.vocab, v);
+    load_piece(logits, base, args.vocab, v);
     const RowParams rp = row_params(args, r);
     const bool cut = !rp.greedy && (rp.k || rp.p < 1.0f);
     RowScratch &row = row_scratch(args, (int)r);
@@ -404,7 +423,7 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
         uint32_t at = 0;  // (the complement: the first index is the largest)
 #pragma unroll
         for (int e = kPer - 1; e >= 0; --e)
-            if (v[e] == top) at = ~(uint32_t)(piece * kPiece + index_of<T, VECTOR>(e));
+            if (v[e] == top) at = ~(uint32_t)(base + index_of<T>(e));
         index = ~block_reduce(at, MaxOp(), scratch);
     } else if (cut) {
         if (best_key) {
@@ -559,7 +578,7 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
 
 // ---- collect ----------------------------------------------------------------------------------------
 
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs args) {
     const int piece = blockIdx.x, lane = threadIdx.x & 63;
     const int64_t r = blockIdx.y;
@@ -575,8 +594,10 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
     const bool listing = low_bin != kNoBin;
     if (piece_key && value_bin(piece_top) >= low_bin && (listing || weighs(piece_top, top, c, low))) {
         const Weights weigh(top, c);
+        const T *logits = (const T *)args.logits + r * args.ld;
+        const int base = piece * kPiece - row_lead(logits);
         float v[kPer];
-        load_piece<T, VECTOR>((const T *)args.logits + r * args.ld, piece * kPiece, args.vocab, v);
+        load_piece(logits, base, args.vocab, v);
         uint32_t listed = 0;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
@@ -606,7 +627,7 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
                 if (listed >> e & 1) {
-                    if (at < kList) list[at] = keys(v[e], piece * kPiece + index_of<T, VECTOR>(e));
+                    if (at < kList) list[at] = keys(v[e], base + index_of<T>(e));
                     ++at;
                 }
         }
@@ -757,6 +778,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const double c = plan.c, low = plan.low;
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
+    const int lead = row_lead(row);
     u64 cut = 1;
     const bool listed = plan.state == kCollect;
     const int n = listed ? (int)plan.listed : 0;
@@ -777,7 +799,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     for (int i = tid; i < (listed ? n : args.vocab); i += kThreads) {
         const u64 key = listed ? list[i] : keys(logit_of(row[i]), i);
         const float v = keys.logit(key);
-        if (key >= cut && weighs(v, top, c, low)) atomicAdd(&extra[keys.index(key) / kStrip], weigh(v));
+        if (key >= cut && weighs(v, top, c, low)) atomicAdd(&extra[(keys.index(key) + lead) / kStrip], weigh(v));
     }
     __syncthreads();
     const u64 total = choose_strip(
@@ -787,7 +809,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
 
 // ---- host -------------------------------------------------------------------------------------------
 
-static int64_t pieces_of(int64_t vocab) { return (vocab + kPiece - 1) / kPiece; }
+// (With the elements that a piece may begin before its row.)
+static int64_t pieces_of(int64_t vocab) { return (vocab + 7 + kPiece - 1) / kPiece; }
 static size_t row_bytes(int64_t vocab) {
     const int64_t pieces = pieces_of(vocab);
     const size_t bytes = sizeof(RowPlan) + pieces * (2 * sizeof(u64) + kWaves * sizeof(Strip) + kBins * sizeof(u64)) +
@@ -799,21 +822,20 @@ size_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
     return kSampleCounterBytes + (size_t)(rows < kBatchRows ? rows : kBatchRows) * row_bytes(vocab);
 }
 
-template <typename T, bool VECTOR>
+template <typename T>
 static void launch_batch(const SampleArgs &args, int rows, hipStream_t stream) {
     const dim3 pieces((unsigned)args.pieces, (unsigned)rows), whole((unsigned)rows);
-    hipLaunchKernelGGL((sample_scan_kernel<T, VECTOR>), pieces, dim3(kThreads), 0, stream, args);
-    hipLaunchKernelGGL((sample_settle_kernel<T>), whole, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL(sample_scan_kernel<T>, pieces, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL(sample_settle_kernel<T>, whole, dim3(kThreads), 0, stream, args);
     if (!args.p.uniforms || (!args.p.top_k && !args.p.top_p && !args.p.min_p)) return;  // every row is settled
-    hipLaunchKernelGGL((sample_collect_kernel<T, VECTOR>), pieces, dim3(kThreads), 0, stream, args);
-    hipLaunchKernelGGL((sample_finish_kernel<T>), whole, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL(sample_collect_kernel<T>, pieces, dim3(kThreads), 0, stream, args);
+    hipLaunchKernelGGL(sample_finish_kernel<T>, whole, dim3(kThreads), 0, stream, args);
 }
 
 hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab,
                          const SampleParams &params, uint32_t *tokens, float *logprobs, void *workspace,
                          hipStream_t stream) {
     const int64_t esize = dtype == SPLOSH_F32 ? 4 : 2;
-    const bool vector = (uintptr_t)logits % 16 == 0 && ld * esize % 16 == 0;
     for (int64_t at = 0; at < rows; at += kBatchRows) {
         const int count = (int)(rows - at < kBatchRows ? rows - at : kBatchRows);
         SampleArgs args{};
@@ -827,13 +849,8 @@ hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows
         args.logprobs = from(logprobs);
         args.rows = (char *)workspace + kSampleCounterBytes;
         args.row_bytes = row_bytes(vocab);
-        if (dtype == SPLOSH_F32) {
-            if (vector) launch_batch<float, true>(args, count, stream);
-            else launch_batch<float, false>(args, count, stream);
-        } else {
-            if (vector) launch_batch<uint16_t, true>(args, count, stream);
-            else launch_batch<uint16_t, false>(args, count, stream);
-        }
+        if (dtype == SPLOSH_F32) launch_batch<float>(args, count, stream);
+        else launch_batch<uint16_t>(args, count, stream);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }

@@ -79,7 +79,7 @@ def sample(logits=LOGITS, ld=1000, dtype=_lib.F32, rows=4, vocab=1000, u=U, t=T,
 @pytest.mark.parametrize("change,case", [
     ({"logits": None}, "nullPointer"), ({"tokens": None}, "nullPointer"), ({"rows": 0}, "invalidShape"),
     ({"vocab": 0}, "invalidShape"), ({"ld": 999}, "invalidRowStride"), ({"dtype": 7}, "unsupported"),
-    ({"vocab": (1 << 22) + 1, "ld": 1 << 24}, "unsupported"), ({"rows": 1 << 40, "ld": 1 << 40}, "arithmeticOverflow"),
+    ({"vocab": (1 << 21) + 1, "ld": 1 << 24}, "unsupported"), ({"rows": 1 << 40, "ld": 1 << 40}, "arithmeticOverflow"),
     ({"rows": 1 << 40}, "unsupported"),
     ({"logits": ctypes.c_void_p(0x10002)}, "unsupported"), ({"u": ctypes.c_void_p(0x10002)}, "unsupported"),
     ({"logprobs": ctypes.c_void_p(0x10002)}, "unsupported"), ({"k": ctypes.c_void_p(0x10001)}, "unsupported"),
@@ -92,5 +92,5 @@ def test_sample_call(change, case):
 
 def test_sample_workspace():
     size = _lib.lib().splosh_sample_workspace_bytes
-    assert size(0, 10) == 0 and size(1, 0) == 0 and size(1, (1 << 22) + 1) == 0
+    assert size(0, 10) == 0 and size(1, 0) == 0 and size(1, (1 << 21) + 1) == 0
     assert size(1, 1) >= 16384 and size(64, 248320) >= size(1, 248320)
