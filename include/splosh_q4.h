@@ -477,10 +477,10 @@ size_t splosh_sample_workspace_bytes(int64_t rows, int64_t vocab);
  *     the kept entries in index order, i included, exceeds u times their whole weight (u below 0 or
  *     NaN as 0, u >= 1: the last kept entry with weight); its logprob is ln(w / whole weight).
  * temperature NULL: 1; top_k, top_p, min_p NULL: off; uniforms NULL: every row as with T = 0.
- * logprobs may be NULL. Weights are summed in 64-bit fixed point, 2^-40 of the largest weight (less
- * counts as none), so the result depends on no order of additions. vocab <= 2^21. The workspace is
- * zero-filled before its first use and shared as splosh_workspace_bytes describes (its arrival
- * counters are zero between calls). */
+ * logprobs may be NULL. What decides between two entries is summed in 64-bit fixed point, 2^-40 of the
+ * largest weight (less counts as none), so the result depends on no order of additions, on no other
+ * row and on no other call. vocab <= 2^21. The workspace need not be zeroed; its first 16 KiB stay as
+ * they are, so one that other calls use serves here too, in stream order. Rows go 256 at a time. */
 int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float *uniforms,
                   const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                   uint32_t *tokens, float *logprobs, void *workspace, size_t workspace_bytes, hipStream_t stream);

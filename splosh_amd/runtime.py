@@ -594,39 +594,57 @@ def embed(w, tokens, out=None, out_dtype=torch.float32, stream=None):
 
 
 # ---- per-request operators of a packed step ------------------------------------------------------
+#
+# The checks here ask a tensor for little and pass plain addresses: a call on one row takes about as long on
+# the host as its kernels on the device.
 
 
-def _device(t, stream):
-    """The context a call on `t` is launched in: nothing to enter when its device is the current one
-    or a stream is named (the kernels go to the stream's device)."""
-    if t.device.index in (None, torch.cuda.current_device()):
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
-def _vector(t, rows, dtype, device, name):
-    """A per-row array: contiguous, of at least `rows` values, on the operands' device (None: none)."""
-    if t is None:
-        return None
-    if t.dtype != dtype or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
-        raise SploshError(13, f"{name} must be a contiguous {dtype} vector")
-    if t.numel() < rows:
-        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows}, observed: {t.numel()})")
-    if t.device != device:
-        raise SploshError(13, f"{name} is on {t.device}, the operands on {device}")
-    return ctypes.c_void_p(t.data_ptr())
-
-
-def _matrix(t, rows, columns, device, name):
-    """A [rows, columns] operand: contiguous rows of at least `columns` on the operands' device."""
+def _index(t, name):
+    """The index of the device that a call's operands are on."""
     if not t.is_cuda:
         raise SploshError(12, f"{name} is not a device tensor")
-    if t.dim() != 2 or t.stride(1) != 1 or t.device != device:
-        raise SploshError(13, f"{name} must be [rows, columns] with contiguous rows, on {device}")
-    if t.shape[1] < columns:
-        raise GemmQ4Error(1, f"{name} has {t.shape[1]} columns, {columns} are needed")
-    if t.shape[0] < rows:
-        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows} rows, observed: {t.shape[0]})")
+    return t.get_device()
+
+
+def _launch(index, stream):
+    """What a call is launched in: its operands' device made the current one, where it is not."""
+    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _raw_stream(stream, index):
+    return stream.cuda_stream if stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _vector(t, rows, dtype, index, name):
+    """The address of a per-row array: contiguous, of at least `rows` values, on device `index` (None: none)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous():
+        raise SploshError(13, f"{name} must be a contiguous {dtype} vector")
+    if t.get_device() != index:
+        raise SploshError(13, f"{name} is on {t.device}, the operands on cuda:{index}")
+    if t.numel() < rows:
+        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows}, observed: {t.numel()})")
+    return t.data_ptr()
+
+
+def _matrix(t, rows, columns, index, name):
+    """The address of a [rows, columns] operand: contiguous rows of at least `columns`, on device `index`."""
+    if not t.is_cuda:
+        raise SploshError(12, f"{name} is not a device tensor")
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or t.get_device() != index:
+        raise SploshError(13, f"{name} must be [rows, columns] with contiguous rows, on cuda:{index}")
+    if shape[1] < columns:
+        raise GemmQ4Error(1, f"{name} has {shape[1]} columns, {columns} are needed")
+    if shape[0] < rows:
+        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows} rows, observed: {shape[0]})")
+    return t.data_ptr()
+
+
+def _row_stride(t):
+    """The row stride of a checked operand (a single row's can be anything)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
 @dataclass
@@ -648,18 +666,22 @@ class Adapters:
             raise SploshError(13, "adapter matrices must be bf16")
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or 0 in a.shape + b.shape:
             raise GemmQ4Error(1, "adapters are a [count, max_rank, inner] and b [count, rows, max_rank]")
-        if a.stride(2) != 1 or b.stride(2) != 1:
+        if (a.stride(2) != 1 and a.shape[2] > 1) or (b.stride(2) != 1 and b.shape[2] > 1):
             raise SploshError(13, "adapter rows must be contiguous")
-        if not a.is_cuda:
-            raise SploshError(12, "a is not a device tensor")
-        if b.device != a.device:
+        self.index = _index(a, "a")
+        if b.get_device() != self.index:
             raise SploshError(13, f"b is on {b.device}, a on {a.device}")
         self.count, self.max_rank, self.inner = a.shape
         self.rows = b.shape[1]
-        scales = _vector(self.scales, self.count, torch.float32, a.device, "scales")
-        ranks = _vector(self.ranks, self.count, torch.int32, a.device, "ranks")
+        scales = _vector(self.scales, self.count, torch.float32, self.index, "scales")
+        ranks = _vector(self.ranks, self.count, torch.int32, self.index, "ranks")
+
+        def stride(t, dim, least):  # (of a dimension of one, anything)
+            return t.stride(dim) if t.shape[dim] > 1 else max(t.stride(dim), least)
+
         self._c = _lib.Adapters(a.data_ptr(), b.data_ptr(), ranks, scales, self.count, self.max_rank, self.rows,
-                                self.inner, a.stride(0), a.stride(1), b.stride(0), b.stride(1))
+                                self.inner, stride(a, 0, 0), stride(a, 1, self.inner), stride(b, 0, 0),
+                                stride(b, 1, self.max_rank))
 
     def c(self):
         return self._c
@@ -668,7 +690,7 @@ class Adapters:
 def adapters_workspace_bytes(adapters, rows):
     """splosh_adapters_workspace_bytes: the scratch a call on these projections' adapters needs."""
     adapters = [adapters] if isinstance(adapters, Adapters) else list(adapters)
-    cs = (_lib.Adapters * len(adapters))(*[w.c() for w in adapters])
+    cs = (_lib.Adapters * len(adapters))(*[w._c for w in adapters])
     return _lib.lib().splosh_adapters_workspace_bytes(cs, len(adapters), rows)
 
 
@@ -677,40 +699,49 @@ def add_adapters_group(outs, a, adapters, slots, rows=None, stream=None, workspa
     outs[i][m] += adapters[i] of slots[m] on a[m], in place. ``a`` is the projections' bf16 activation
     [rows, inner], ``outs`` their outputs (gemm_group's; fp32 or bf16), ``slots`` int32 [rows], the
     adapter of each row (negative or past the count: none). Returns the outputs."""
-    rows = a.shape[0] if rows is None else rows
-    if a.dtype != torch.bfloat16:
-        raise SploshError(13, "activations must be bf16")
     outs, adapters = list(outs), list(adapters)
-    if len(outs) != len(adapters) or not outs:
-        raise GemmQ4Error(1, "one output for each projection's adapters")
     n = len(outs)
+    if n != len(adapters) or n == 0:
+        raise GemmQ4Error(1, "one output for each projection's adapters")
+    rows = a.shape[0] if rows is None else rows
     if rows <= 0:
         raise GemmQ4Error(1, "rows must be positive")
-    _matrix(a, rows, adapters[0].inner, a.device, "a")
+    if a.dtype != torch.bfloat16:
+        raise SploshError(13, "activations must be bf16")
+    index, dtype = _index(a, "a"), outs[0].dtype
+    x = _matrix(a, rows, adapters[0].inner, index, "a")
+    ptrs = []
     for w, o in zip(adapters, outs):
-        if o.dtype != outs[0].dtype:
+        if o.dtype != dtype:
             raise SploshError(13, "grouped outputs must share one dtype")
-        _matrix(o, rows, w.rows, a.device, "output")
-        if w.a.device != a.device:
-            raise SploshError(13, f"adapters are on {w.a.device}, the activations on {a.device}")
-    slot_ptr = _vector(slots, rows, torch.int32, a.device, "slots")
-    cs = (_lib.Adapters * n)(*[w.c() for w in adapters])
-    out_ptrs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
-    ldcs = (ctypes.c_int64 * n)(*[o.stride(0) for o in outs])
-    with _device(a, stream):
+        if w.index != index:
+            raise SploshError(13, f"adapters are on cuda:{w.index}, the activations on cuda:{index}")
+        ptrs.append(_matrix(o, rows, w.rows, index, "output"))
+    slot_ptr = _vector(slots, rows, torch.int32, index, "slots")
+    lib, code = _lib.lib(), _dtype_code(dtype)
+    if n > 1 or workspace is None:
+        cs = (_lib.Adapters * n)(*[w._c for w in adapters])
+    with _launch(index, stream):
         if workspace is None:
             with _allocating(stream):
-                workspace = torch.empty(max(1, _lib.lib().splosh_adapters_workspace_bytes(cs, n, rows)),
-                                        dtype=torch.uint8, device=a.device)
-        _lib.check(_lib.lib().splosh_adapters_add_group(cs, n, _ptr(a), a.stride(0), out_ptrs, ldcs,
-                                                        _dtype_code(outs[0].dtype), slot_ptr, rows, _ptr(workspace),
-                                                        workspace.numel() * workspace.element_size(), _stream(stream)))
+                workspace = torch.empty(max(1, lib.splosh_adapters_workspace_bytes(cs, n, rows)), dtype=torch.uint8,
+                                        device=a.device)
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if n == 1:
+            st = lib.splosh_adapters_add(ctypes.byref(adapters[0]._c), x, _row_stride(a), ptrs[0], _row_stride(outs[0]),
+                                         code, slot_ptr, rows, ws, ws_bytes, _raw_stream(stream, index))
+        else:
+            st = lib.splosh_adapters_add_group(cs, n, x, _row_stride(a), (ctypes.c_void_p * n)(*ptrs),
+                                               (ctypes.c_int64 * n)(*[_row_stride(o) for o in outs]), code, slot_ptr, rows,
+                                               ws, ws_bytes, _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
     return outs
 
 
 def add_adapters(out, a, adapters, slots, rows=None, stream=None, workspace=None):
     """splosh_adapters_add: add_adapters_group for one projection. Returns ``out``."""
-    return add_adapters_group([out], a, [adapters], slots, rows, stream, workspace)[0]
+    return add_adapters_group((out,), a, (adapters,), slots, rows, stream, workspace)[0]
 
 
 def sample_workspace_bytes(rows, vocab):
@@ -725,26 +756,27 @@ def sample(logits, uniforms=None, temperature=None, top_k=None, top_p=None, min_
     device vectors [rows]; None leaves that one off. uniforms None: the largest logit of every row
     (as temperature 0 in one row). Returns (tokens int32, logprobs fp32); a row with nothing to choose
     gets token -1, which embed turns into zeros."""
-    device = logits.device
-    _matrix(logits, 0, 0, device, "logits")
+    index = _index(logits, "logits")
+    ptr = _matrix(logits, 0, 0, index, "logits")
     rows, vocab = logits.shape
     if rows == 0 or vocab == 0:
         raise GemmQ4Error(1, "rows and vocab must be positive")
-    params = [_vector(t, rows, dt, device, name) for t, dt, name in
-              ((uniforms, torch.float32, "uniforms"), (temperature, torch.float32, "temperature"),
-               (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"))]
-    with _device(logits, stream):
-        with _allocating(stream):
-            if out is None:
-                out = torch.empty(rows, dtype=torch.int32, device=device)
-            if logprobs is None:
-                logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-            if workspace is None:
-                workspace = torch.empty(max(1, sample_workspace_bytes(rows, vocab)), dtype=torch.uint8, device=device)
-                workspace[:WORKSPACE_COUNTER_BYTES].zero_()
-        _lib.check(_lib.lib().splosh_sample(_ptr(logits), logits.stride(0), _dtype_code(logits.dtype), rows, vocab,
-                                            *params, _vector(out, rows, torch.int32, device, "out"),
-                                            _vector(logprobs, rows, torch.float32, device, "logprobs"),
-                                            _ptr(workspace), workspace.numel() * workspace.element_size(),
-                                            _stream(stream)))
+    f32, code = torch.float32, _dtype_code(logits.dtype)
+    params = (_vector(uniforms, rows, f32, index, "uniforms"), _vector(temperature, rows, f32, index, "temperature"),
+              _vector(top_k, rows, torch.int32, index, "top_k"), _vector(top_p, rows, f32, index, "top_p"),
+              _vector(min_p, rows, f32, index, "min_p"))
+    lib = _lib.lib()
+    with _launch(index, stream):
+        if out is None or logprobs is None or workspace is None:
+            with _allocating(stream):
+                out = torch.empty(rows, dtype=torch.int32, device=logits.device) if out is None else out
+                logprobs = torch.empty(rows, dtype=f32, device=logits.device) if logprobs is None else logprobs
+                if workspace is None:
+                    workspace = torch.empty(max(1, lib.splosh_sample_workspace_bytes(rows, vocab)), dtype=torch.uint8,
+                                            device=logits.device)
+        st = lib.splosh_sample(ptr, _row_stride(logits), code, rows, vocab, *params,
+                               _vector(out, rows, torch.int32, index, "out"), _vector(logprobs, rows, f32, index, "logprobs"),
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
     return out, logprobs
