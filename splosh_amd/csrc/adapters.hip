@@ -20,7 +20,7 @@ namespace splosh {
 // The workspace's first 16 KiB belong to the arrival counters of the kernels that have any.
 constexpr size_t kAdapterCounterBytes = 16384;
 constexpr int kChunk = 64;       // rows of a chunk
-constexpr int kDownRanks = 64;   // rows of a that a workgroup of the first launch takes
+constexpr int kDownRanks = 32;   // rows of a that a workgroup of the first launch takes
 constexpr int kUpColumns = 256;  // outputs of a tile of the second
 // An offset past every descriptor, and still so with another one added.
 constexpr uint32_t kNowhere = 0x40000000u;
@@ -51,6 +51,7 @@ struct AdapterArgs {
     int t_cols, slices, slice_steps;
     int tiles;    // tiles of outputs a workgroup of the second launch takes
     int turns;    // workgroups that share a chunk's adapters
+    int shares;   // workgroups of the second launch that share an adapter's rows, sixteen at a time
     AdapterWeight w[SPLOSH_MAX_GROUP];
 };
 
@@ -70,22 +71,36 @@ __device__ __forceinline__ u32x4 keep8(u32x4 v, int n) {
     return v;
 }
 
+// Orders a wave's own LDS operations for the compiler (the hardware does them in order).
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- t = a x --------------------------------------------------------------------------------------
 //
-// A workgroup: one adapter's rows of a chunk, up to 64 rows of one projection's a, one slice of K. Its eight
+// A workgroup: one adapter's rows of a chunk, up to 32 rows of one projection's a, one slice of K. Its four
 // waves take the slice's steps of 32 k in turn, kSteps of them with every load in flight, and add their
 // sums in LDS. a's rows are the MFMA's rows and the activation rows its columns: the sum's four registers
 // are then four neighbouring ranks of one activation row, a 16-byte store.
+//
+// A FAST load has the four lanes of a quad read the 64 bytes of one row, and goes through LDS to the MFMA's
+// order, in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache
+// lookup of its own.
 
-constexpr int kDownWaves = 8;
+constexpr int kDownWaves = 4;
 
 // 16 RB of the adapter's rows: `mine` is the chunk row that lane i holds as the adapter's i-th.
 template <int RB, int P, bool FAST>
 __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args, const AdapterWeight &g, int slot,
                                                          int rank, float scale, int mine, int count, int64_t base,
-                                                         int rank0, int slice, f32x4 *sums) {
+                                                         int rank0, int slice, u32x4 *memory) {
     constexpr int kSteps = RB == 1 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
+    // Where a lane's 16 bytes of a load lie: row and piece; and, spread over the banks, in LDS.
+    const int load_row = FAST ? lane >> 2 : m, load_piece = FAST ? lane & 3 : q;
+    u32x4 *stage = memory + wave * (RB + P) * 64;
+    const int put = lane ^ ((lane >> 4) & 3), get = m * 4 + (q ^ ((m >> 2) & 3));
     const int inner = (int)g.w.inner, steps = (inner + 31) / 32;
     const int from = slice * args.slice_steps, to = from + args.slice_steps < steps ? from + args.slice_steps : steps;
     const uint16_t *a = g.w.a + slot * g.w.a_slot_stride, *x = args.x + base * args.ldx;
@@ -97,11 +112,12 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
     for (int i = 0; i < RB; ++i) {
         xr[i] = __builtin_amdgcn_ds_bpermute(((i * 16 + m) & 63) * 4, mine);
         if (i * 16 + m >= count) xr[i] = -1;
-        xo[i] = xr[i] < 0 ? kNowhere : (uint32_t)(xr[i] * args.ldx * 2);
+        const int row = __builtin_amdgcn_ds_bpermute(((i * 16 + load_row) & 63) * 4, mine);
+        xo[i] = i * 16 + load_row < count ? (uint32_t)(row * args.ldx * 2) : kNowhere;
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const int r = rank0 + p * 16 + m;
+        const int r = rank0 + p * 16 + load_row;
         ao[p] = r < rank ? (uint32_t)(r * g.w.a_row_stride * 2) : kNowhere;
     }
     f32x4 acc[RB][P];
@@ -113,7 +129,7 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
         u32x4 xs[kSteps][RB], as[kSteps][P];
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-            const int step = s + kDownWaves * j, k = step * 32 + q * 8, n = step < to ? inner - k : 0;
+            const int step = s + kDownWaves * j, k = step * 32 + load_piece * 8, n = step < to ? inner - k : 0;
             const uint32_t ko = n > 0 ? (uint32_t)k * 2 : kNowhere;
 #pragma unroll
             for (int i = 0; i < RB; ++i)
@@ -126,14 +142,28 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
             }
         }
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j)
+        for (int j = 0; j < kSteps; ++j) {
+            if constexpr (FAST) {
+#pragma unroll
+                for (int i = 0; i < RB; ++i) stage[i * 64 + put] = xs[j][i];
+#pragma unroll
+                for (int p = 0; p < P; ++p) stage[(RB + p) * 64 + put] = as[j][p];
+                wave_fence();
+#pragma unroll
+                for (int i = 0; i < RB; ++i) xs[j][i] = stage[i * 64 + get];
+#pragma unroll
+                for (int p = 0; p < P; ++p) as[j][p] = stage[(RB + p) * 64 + get];
+                wave_fence();
+            }
 #pragma unroll
             for (int i = 0; i < RB; ++i)
 #pragma unroll
                 for (int p = 0; p < P; ++p)
                     acc[i][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(as[j][p]), as_bf16x8(xs[j][i]),
                                                                          acc[i][p], 0, 0, 0);
+        }
     }
+    f32x4 *sums = (f32x4 *)memory;
     // The waves' sums, a panel at a time: [row block][wave][lane].
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -156,7 +186,7 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
 
 template <int RBMAX, int P, bool FAST>
 __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(AdapterArgs args) {
-    __shared__ f32x4 sums[RBMAX * kDownWaves * 64];
+    __shared__ u32x4 memory[(RBMAX + P) * kDownWaves * 64];
     const int which = blockIdx.z / args.turns, turn = blockIdx.z % args.turns;
     const int column = blockIdx.x / args.slices, slice = blockIdx.x % args.slices;
     const AdapterWeight &g = args.w[which];
@@ -184,11 +214,11 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
         const float group_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), lead));
         if (RBMAX == 1 || count <= 16) {
             for (int left = count; left > 0; left -= 16) {
-                down_rows<1, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, left, base, rank0, slice, sums);
+                down_rows<1, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, left, base, rank0, slice, memory);
                 mine = __builtin_amdgcn_ds_bpermute(((lane + 16) & 63) * 4, mine);
             }
         } else {
-            down_rows<RBMAX, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, count, base, rank0, slice, sums);
+            down_rows<RBMAX, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, count, base, rank0, slice, memory);
         }
     }
     // The list for the second launch, by one wave of the chunk.
@@ -216,27 +246,23 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
 // sums pass through LDS, so that a wave reads and writes runs of 64 neighbouring outputs of a row: with
 // the MFMA's own layout, neighbouring lanes hold different rows, and four times the cache lookups.
 
-// Orders a wave's own LDS operations for the compiler (the hardware does them in order).
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 constexpr int kUpSumStride = 68;  // floats of a row of sums in LDS: 64 and a step of four banks
 
-// The part's rows of t summed over the slices, as operands in LDS: [piece][panel of 32 ranks][row block]
-// [lane] x 16 bytes. Four ranks of one row a thread.
+// The rows of t of a workgroup's blocks of sixteen (block j of its own: from the adapter's row 16 (share + j
+// shares) on), summed over the slices, as operands in LDS: [piece][panel of 32 ranks][block][lane] x 16 bytes.
+// Four ranks of one row a thread.
 template <int PIECES>
 __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWeight &g, int mine, int count,
-                                        int blocks, int64_t base, int rank, u32x2 *pieces) {
+                                        int blocks, int share, int64_t base, int rank, u32x2 *pieces) {
     constexpr int kAtOnce = 8;
     const int panels = (rank + 31) / 32, quads = panels * 8;
     const int64_t slice_floats = args.rows * args.t_cols;
     for (int item = threadIdx.x; item < blocks * 16 * quads; item += 256) {
         const int i = item / quads, r = (item - i * quads) * 4;
         f32x4 v = {0, 0, 0, 0};
-        const int chunk_row = __builtin_amdgcn_ds_bpermute(i * 4, mine);
-        if (i < count && r < rank) {
+        const int place = (share + (i >> 4) * args.shares) * 16 + (i & 15);
+        const int chunk_row = __builtin_amdgcn_ds_bpermute((place & 63) * 4, mine);
+        if (place < count && r < rank) {
             const float *t = args.t + (base + chunk_row) * args.t_cols + g.t_offset + r;
             for (int s = 0; s < args.slices; s += kAtOnce) {
                 f32x4 part[kAtOnce];
@@ -273,7 +299,8 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
     constexpr int kPieces = sizeof(OUT) == 4 ? 3 : 2, kLoads = sizeof(OUT), kPer = 16 / sizeof(OUT), kHeld = NP ? NP : 1;
     extern __shared__ u32x4 pieces[];
     __shared__ float sums[4][16 * kUpSumStride];
-    const int which = blockIdx.z / args.turns, turn = blockIdx.z % args.turns;
+    const int share = blockIdx.z % args.shares, z = blockIdx.z / args.shares;
+    const int which = z / args.turns, turn = z % args.turns;
     const AdapterWeight &g = args.w[which];
     const int column0 = (int)blockIdx.x * args.tiles * kUpColumns, columns = (int)g.w.rows;
     if (column0 >= columns) return;
@@ -288,7 +315,8 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
         const int slot = __builtin_amdgcn_readlane(record.x, part);
         const uint32_t rest = __builtin_amdgcn_readlane(record.y, part);
         const int rank = rest & 0xffffu, first = (rest >> 16) & 0xffu, count = rest >> 24;
-        const int blocks = (count + 15) / 16, panels = (rank + 31) / 32;
+        const int blocks = ((count + 15) / 16 - share + args.shares - 1) / args.shares, panels = (rank + 31) / 32;
+        if (blocks <= 0) continue;
         const int mine = __builtin_amdgcn_ds_bpermute(((first + lane) & 63) * 4, order);
         const uint16_t *b = g.w.b + slot * g.w.b_slot_stride;
         const rsrc_t rb = make_rsrc(b, FAST ? (uint32_t)(g.w.rows * g.w.b_row_stride * 2) : 0);
@@ -317,7 +345,7 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
             for (int p = 0; p < NP; ++p) load_b(p, bs[p]);
             if (tile == 0) {
                 __syncthreads();  // (the operands before them have been read)
-                stage_t<kPieces>(args, g, mine, count, blocks, base, rank, (u32x2 *)pieces);
+                stage_t<kPieces>(args, g, mine, count, blocks, share, base, rank, (u32x2 *)pieces);
                 __syncthreads();
             }
 #pragma unroll
@@ -330,8 +358,8 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
                 int row[kLoads];
 #pragma unroll
                 for (int c = 0; c < kLoads; ++c) {
-                    const int place = i * 16 + (c * 64 + lane) * kPer / 64, n = n0 + lane * kPer % 64;
-                    row[c] = __builtin_amdgcn_ds_bpermute(place * 4, mine);
+                    const int place = (share + i * args.shares) * 16 + (c * 64 + lane) * kPer / 64, n = n0 + lane * kPer % 64;
+                    row[c] = __builtin_amdgcn_ds_bpermute((place & 63) * 4, mine);
                     if (place >= count) row[c] = -1;
                     if constexpr (FAST) {
                         at[c] = row[c] >= 0 && n < columns ? (uint32_t)((row[c] * g.ldc + n) * sizeof(OUT)) : kNowhere;
@@ -455,8 +483,7 @@ static int plan_turns(int64_t parts, int64_t others) {
 template <int RB, bool FAST>
 static void launch_down(const AdapterArgs &args, int panels, dim3 grid, hipStream_t stream) {
     if (panels == 1) hipLaunchKernelGGL((adapter_down_kernel<RB, 1, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
-    else if (panels == 2) hipLaunchKernelGGL((adapter_down_kernel<RB, 2, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
-    else hipLaunchKernelGGL((adapter_down_kernel<RB, 4, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
+    else hipLaunchKernelGGL((adapter_down_kernel<RB, 2, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
 }
 
 // LDS of the operands: three pieces (of an fp32 output) of whole panels of ranks for a chunk's rows; past the
@@ -519,7 +546,7 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     const int64_t parts = most_parts(w, group, rows);
     args.turns = plan_turns(parts, (int64_t)down_x * chunks * group);
     const dim3 down(down_x, chunks, (unsigned)(group * args.turns));
-    const int panels = most_rank <= 16 ? 1 : most_rank <= 32 ? 2 : 4;
+    const int panels = most_rank <= 16 ? 1 : 2;
     if (!down_fast) launch_down<1, false>(args, panels, down, stream);
     else if (rows <= 16) launch_down<1, true>(args, panels, down, stream);
     else launch_down<4, true>(args, panels, down, stream);
@@ -530,8 +557,12 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     const int64_t share = (tiles * chunks * (chunks == 1 ? parts : 1) + 1535) / 1536;
     args.tiles = (int)(share < most_tiles ? share : most_tiles);
     const unsigned up_x = (unsigned)((most_tiles + args.tiles - 1) / args.tiles);
-    args.turns = plan_turns(parts, (int64_t)up_x * chunks * group);
-    const dim3 up(up_x, chunks, (unsigned)(group * args.turns));
+    // An adapter's rows in shares where there are fewer than three workgroups a CU and more than 16 rows an adapter
+    // (333 rows of three, K6144 -> N5120: 12.3 us whole, 9.3 in four).
+    const int64_t whole = tiles / args.tiles * chunks * (chunks == 1 ? parts : 1);
+    args.shares = rows <= 16 * parts || whole >= 768 ? 1 : whole >= 384 || rows <= 32 ? 2 : 4;
+    args.turns = plan_turns(parts, (int64_t)up_x * chunks * group * args.shares);
+    const dim3 up(up_x, chunks, (unsigned)(group * args.turns * args.shares));
     const int up_panels = (int)(most_rank + 31) / 32, blocks = rows < kChunk ? (int)(rows + 15) / 16 : kChunk / 16;
     const int lds = (out_dtype == SPLOSH_F32 ? 3 : 2) * up_panels * blocks * 1024;
     return out_dtype == SPLOSH_F32 ? launch_up<float>(args, up_panels, up_fast, lds, up, stream)
