@@ -11,7 +11,8 @@
 //
 // FAST kernels are for operands whose every 16-byte piece is whole, aligned and within a buffer
 // descriptor's reach (the usual case): their loads have no branches, since an offset out of a descriptor's
-// range reads zeros and writes nothing. The others take elements one by one where a piece is not whole.
+// range reads zeros and writes nothing. The others load pieces at any alignment, where they are whole, and
+// element by element where they are not.
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -55,13 +56,20 @@ struct AdapterArgs {
     AdapterWeight w[SPLOSH_MAX_GROUP];
 };
 
-// Elements [0, n) of the eight at p, zero past them.
+// Elements [0, n) of the eight at p, of any alignment; zero past them.
 __device__ __forceinline__ u32x4 load8(const uint16_t *p, int n) {
     u32x4 v = {0, 0, 0, 0};
-    if (n > 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    if (n >= 8) {
+        __builtin_memcpy(&v, p, 16);
+    } else if (n > 0) {
+        uint64_t low = 0, high = 0;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const uint64_t e = (uint64_t)p[i] << (16 * (i & 3));
+            low |= i < 4 ? e : 0;
+            high |= i < 4 ? 0 : e;
+        }
+        v = u32x4{(uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32)};
     }
     return v;
 }
@@ -84,8 +92,7 @@ __device__ __forceinline__ void wave_fence() {
 // sums in LDS. a's rows are the MFMA's rows and the activation rows its columns: the sum's four registers
 // are then four neighbouring ranks of one activation row, a 16-byte store.
 //
-// A FAST load has the four lanes of a quad read the 64 bytes of one row, and goes through LDS to the MFMA's
-// order, in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache
+// A load has the four lanes of a quad read the 64 bytes of one row, and goes through LDS to the MFMA's order, in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache
 // lookup of its own.
 
 constexpr int kDownWaves = 4;
@@ -98,7 +105,7 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
     constexpr int kSteps = RB == 1 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
     // Where a lane's 16 bytes of a load lie: row and piece; and, spread over the banks, in LDS.
-    const int load_row = FAST ? lane >> 2 : m, load_piece = FAST ? lane & 3 : q;
+    const int load_row = lane >> 2, load_piece = lane & 3;
     u32x4 *stage = memory + wave * (RB + P) * 64;
     const int put = lane ^ ((lane >> 4) & 3), get = m * 4 + (q ^ ((m >> 2) & 3));
     const int inner = (int)g.w.inner, steps = (inner + 31) / 32;
@@ -107,18 +114,24 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
     const rsrc_t ra = make_rsrc(a, FAST ? (uint32_t)(g.w.max_rank * g.w.a_row_stride * 2) : 0);
     const rsrc_t rx = make_rsrc(x, FAST ? (uint32_t)(kChunk * args.ldx * 2) : 0);
     uint32_t xo[RB], ao[P];
+    const uint16_t *xp[RB], *ap[P];
+    bool xv[RB], av[P];
     int xr[RB];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
         xr[i] = __builtin_amdgcn_ds_bpermute(((i * 16 + m) & 63) * 4, mine);
         if (i * 16 + m >= count) xr[i] = -1;
         const int row = __builtin_amdgcn_ds_bpermute(((i * 16 + load_row) & 63) * 4, mine);
-        xo[i] = i * 16 + load_row < count ? (uint32_t)(row * args.ldx * 2) : kNowhere;
+        xv[i] = i * 16 + load_row < count;
+        xo[i] = xv[i] ? (uint32_t)(row * args.ldx * 2) : kNowhere;
+        xp[i] = x + (xv[i] ? row : 0) * args.ldx;
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         const int r = rank0 + p * 16 + load_row;
-        ao[p] = r < rank ? (uint32_t)(r * g.w.a_row_stride * 2) : kNowhere;
+        av[p] = r < rank;
+        ao[p] = av[p] ? (uint32_t)(r * g.w.a_row_stride * 2) : kNowhere;
+        ap[p] = a + (av[p] ? r : 0) * g.w.a_row_stride;
     }
     f32x4 acc[RB][P];
 #pragma unroll
@@ -133,28 +146,23 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
             const uint32_t ko = n > 0 ? (uint32_t)k * 2 : kNowhere;
 #pragma unroll
             for (int i = 0; i < RB; ++i)
-                xs[j][i] = FAST ? buffer_load16(rx, xo[i] + ko, 0)
-                                : load8(x + (xr[i] < 0 ? 0 : xr[i]) * args.ldx + k, xr[i] < 0 ? 0 : n);
+                xs[j][i] = FAST ? buffer_load16(rx, xo[i] + ko, 0) : load8(xp[i] + k, xv[i] ? n : 0);
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int r = rank0 + p * 16 + m;
-                as[j][p] = FAST ? buffer_load16(ra, ao[p] + ko, 0) : load8(a + r * g.w.a_row_stride + k, r < rank ? n : 0);
-            }
+            for (int p = 0; p < P; ++p)
+                as[j][p] = FAST ? buffer_load16(ra, ao[p] + ko, 0) : load8(ap[p] + k, av[p] ? n : 0);
         }
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-            if constexpr (FAST) {
 #pragma unroll
-                for (int i = 0; i < RB; ++i) stage[i * 64 + put] = xs[j][i];
+            for (int i = 0; i < RB; ++i) stage[i * 64 + put] = xs[j][i];
 #pragma unroll
-                for (int p = 0; p < P; ++p) stage[(RB + p) * 64 + put] = as[j][p];
-                wave_fence();
+            for (int p = 0; p < P; ++p) stage[(RB + p) * 64 + put] = as[j][p];
+            wave_fence();
 #pragma unroll
-                for (int i = 0; i < RB; ++i) xs[j][i] = stage[i * 64 + get];
+            for (int i = 0; i < RB; ++i) xs[j][i] = stage[i * 64 + get];
 #pragma unroll
-                for (int p = 0; p < P; ++p) as[j][p] = stage[(RB + p) * 64 + get];
-                wave_fence();
-            }
+            for (int p = 0; p < P; ++p) as[j][p] = stage[(RB + p) * 64 + get];
+            wave_fence();
 #pragma unroll
             for (int i = 0; i < RB; ++i)
 #pragma unroll
@@ -210,16 +218,12 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
         const int count = __builtin_popcountll(rows);
         const int place = rows >> lane & 1 ? __builtin_popcountll(rows & below)
                                            : count + __builtin_popcountll(~rows & below);
-        int mine = __builtin_amdgcn_ds_permute(place * 4, lane);
+        const int mine = __builtin_amdgcn_ds_permute(place * 4, lane);
         const float group_scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), lead));
-        if (RBMAX == 1 || count <= 16) {
-            for (int left = count; left > 0; left -= 16) {
-                down_rows<1, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, left, base, rank0, slice, memory);
-                mine = __builtin_amdgcn_ds_bpermute(((lane + 16) & 63) * 4, mine);
-            }
-        } else {
+        if (RBMAX == 1 || count <= 16)
+            down_rows<1, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, count, base, rank0, slice, memory);
+        else
             down_rows<RBMAX, P, FAST>(args, g, group_slot, group_rank, group_scale, mine, count, base, rank0, slice, memory);
-        }
     }
     // The list for the second launch, by one wave of the chunk.
     if (blockIdx.x != 0 || turn != 0 || threadIdx.x >= 64) return;
@@ -364,11 +368,26 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
                     if constexpr (FAST) {
                         at[c] = row[c] >= 0 && n < columns ? (uint32_t)((row[c] * g.ldc + n) * sizeof(OUT)) : kNowhere;
                         old[c] = buffer_load16(ro, at[c], 0);
+                    } else if (row[c] >= 0 && n + kPer <= columns) {
+                        __builtin_memcpy(&old[c], out + row[c] * g.ldc + n, 16);
                     }
                 }
                 f32x4 acc[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[j] = f32x4{0, 0, 0, 0};
+                // Sixteen bytes of outputs and their sums, rounded once.
+                auto added = [](u32x4 o, const f32x4(&v)[kPer / 4]) {
+                    u32x4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (sizeof(OUT) == 4)
+                            w[e] = __float_as_uint(__uint_as_float(o[e]) + v[0][e]);
+                        else
+                            w[e] = f32x2_to_bf16x2(bf16_bits_to_f32(o[e] & 0xffffu) + v[e >> 1][2 * (e & 1)],
+                                                   bf16_bits_to_f32(o[e] >> 16) + v[e >> 1][2 * (e & 1) + 1]);
+                    }
+                    return w;
+                };
                 auto multiply = [&](int p, const u32x4(&v)[4]) {
 #pragma unroll
                     for (int c = 0; c < kPieces; ++c) {
@@ -402,24 +421,21 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
 #pragma unroll
                     for (int e = 0; e < kPer / 4; ++e) v[e] = *(const f32x4 *)(from + 4 * e);
                     if constexpr (FAST) {
-                        u32x4 w;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if constexpr (sizeof(OUT) == 4)
-                                w[e] = __float_as_uint(__uint_as_float(old[c][e]) + v[0][e]);
-                            else
-                                w[e] = f32x2_to_bf16x2(bf16_bits_to_f32(old[c][e] & 0xffffu) + v[e >> 1][2 * (e & 1)],
-                                                       bf16_bits_to_f32(old[c][e] >> 16) + v[e >> 1][2 * (e & 1) + 1]);
-                        }
+                        const u32x4 w = added(old[c], v);
                         __builtin_amdgcn_raw_buffer_store_b128(w, ro, (int)at[c], 0, 0);
                     } else if (row[c] >= 0) {
-                        OUT *p = out + row[c] * g.ldc;
+                        const int n = n0 + lane * kPer % 64;
+                        OUT *p = out + row[c] * g.ldc + n;
+                        if (n + kPer <= columns) {
+                            const u32x4 w = added(old[c], v);
+                            __builtin_memcpy(p, &w, 16);
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < kPer; ++e) {
-                            const int n = n0 + lane * kPer % 64 + e;
-                            if (n >= columns) continue;
-                            if constexpr (sizeof(OUT) == 4) p[n] += v[0][e];
-                            else p[n] = f32_to_bf16(bf16_bits_to_f32(p[n]) + v[e >> 2][e & 3]);
+                            for (int e = 0; e < kPer; ++e) {
+                                if (n + e >= columns) continue;
+                                if constexpr (sizeof(OUT) == 4) p[e] += v[0][e];
+                                else p[e] = f32_to_bf16(bf16_bits_to_f32(p[e]) + v[e >> 2][e & 3]);
+                            }
                         }
                     }
                 }
@@ -502,7 +518,8 @@ static hipError_t launch_up(const AdapterArgs &args, int lds, dim3 grid, hipStre
 }
 template <typename OUT>
 static hipError_t launch_up(const AdapterArgs &args, int panels, bool fast, int lds, dim3 grid, hipStream_t stream) {
-    if (!fast) return launch_up<0, OUT, false>(args, lds, grid, stream);
+    if (!fast) return panels == 1 ? launch_up<1, OUT, false>(args, lds, grid, stream)
+                                  : launch_up<0, OUT, false>(args, lds, grid, stream);
     if (panels == 1) return launch_up<1, OUT, true>(args, lds, grid, stream);
     if (panels == 2) return launch_up<2, OUT, true>(args, lds, grid, stream);
     return launch_up<0, OUT, true>(args, lds, grid, stream);
@@ -547,9 +564,13 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     args.turns = plan_turns(parts, (int64_t)down_x * chunks * group);
     const dim3 down(down_x, chunks, (unsigned)(group * args.turns));
     const int panels = most_rank <= 16 ? 1 : 2;
-    if (!down_fast) launch_down<1, false>(args, panels, down, stream);
-    else if (rows <= 16) launch_down<1, true>(args, panels, down, stream);
-    else launch_down<4, true>(args, panels, down, stream);
+    if (rows <= 16) {
+        if (down_fast) launch_down<1, true>(args, panels, down, stream);
+        else launch_down<1, false>(args, panels, down, stream);
+    } else {
+        if (down_fast) launch_down<4, true>(args, panels, down, stream);
+        else launch_down<4, false>(args, panels, down, stream);
+    }
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     // Tiles a workgroup, for which t is staged once: so many that six workgroups a CU are left (2048 rows,
