@@ -209,7 +209,8 @@ struct RowPlan {
 };
 // A wave's strip of a piece.
 struct Strip {
-    u64 weight;       // scan: of its piece's largest logit
+    u64 key;          // scan: its largest logit's
+    u64 weight;       // scan: its weight, of its piece's largest logit
     u64 above, kept;  // collect: the weight above the list's bins, and of it what min-p leaves
 };
 struct RowScratch {
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
     float best = -__builtin_inff();
 #pragma unroll
     for (int e = 0; e < kPer; ++e) best = __builtin_fmaxf(best, v[e]);
+    const uint32_t strip_key = wave_scan(logit_key(best), MaxOp());  // (in lane 63)
     const uint32_t best_key = block_reduce(logit_key(best), MaxOp(), scratch);
     const float top = key_logit(best_key);
     u64 index = 0, weight = 0;
@@ -451,7 +453,11 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
     }
     if (!rp.greedy) {
         weight = wave_scan(weight, SumOp());
-        if ((tid & 63) == 63) row_strips(args, row)[piece * kWaves + (tid >> 6)].weight = weight;
+        if ((tid & 63) == 63) {
+            Strip &strip = row_strips(args, row)[piece * kWaves + (tid >> 6)];
+            strip.key = strip_key;
+            strip.weight = weight;
+        }
     }
     if (tid == 0) {
         row.heads[piece] = (u64)best_key << 32 | index;
@@ -584,15 +590,16 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
     const int64_t r = blockIdx.y;
     RowScratch &row = row_scratch(args, (int)r);
     const RowPlan &plan = row.plan;
+    Strip &strip = row_strips(args, row)[piece * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
     const int state = plan.state, low_bin = plan.low_bin, above_bin = plan.above_bin;
-    const uint32_t piece_key = (uint32_t)(row.heads[piece] >> 32);
-    const float top = key_logit(plan.top_key), piece_top = key_logit(piece_key);
+    const uint32_t strip_key = (uint32_t)strip.key;
+    const float top = key_logit(plan.top_key), strip_top = key_logit(strip_key);
     const double c = plan.c, low = plan.low;
     if (state != kCollect) return;
     u64 above = 0, kept = 0;
-    // (A piece whose largest is below the list's bins, or below min-p with no list, has nothing to give.)
+    // (A strip whose largest is below the list's bins, or below min-p with no list, has nothing to give.)
     const bool listing = low_bin != kNoBin;
-    if (piece_key && value_bin(piece_top) >= low_bin && (listing || weighs(piece_top, top, c, low))) {
+    if (strip_key && value_bin(strip_top) >= low_bin && (listing || weighs(strip_top, top, c, low))) {
         const Weights weigh(top, c);
         const T *logits = (const T *)args.logits + r * args.ld;
         const int base = piece * kPiece - row_lead(logits);
@@ -635,7 +642,6 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
         kept = wave_scan(kept, SumOp());
     }
     if (lane == 63) {
-        Strip &strip = row_strips(args, row)[piece * kWaves + (threadIdx.x >> 6)];
         strip.above = above;
         strip.kept = kept;
     }
