@@ -339,6 +339,7 @@ __device__ __forceinline__ u64 choose_strip(const F &weight_of, int strips, floa
     const int each = (strips + kThreads - 1) / kThreads, first = (int)threadIdx.x * each;
     u64 mine = 0;
     for (int s = first; s < first + each && s < strips; ++s) mine += weight_of(s);
+    if (threadIdx.x == 0) sh.chosen = 0, sh.fraction = 0.0;
     const u64 run = block_scan(mine, sh.scratch);
     u64 total = 0;
 #pragma unroll
@@ -373,16 +374,19 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
         v[e] = first + e >= 0 && first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
-    u64 w[kEach], sum = 0;
+    u64 w[kEach], run = 0, total = 0;
+    for (int pass = 0; pass < 2 && total == 0; ++pass) {  // (again, by number, where what is left is less than a unit each)
+        u64 sum = 0;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const u64 key = keys(v[e], first + e);
-        w[e] = key && key >= cut && weighs(v[e], top, c, low) ? weigh(v[e]) : 0;
-        sum += w[e];
+        for (int e = 0; e < kEach; ++e) {
+            const u64 key = keys(v[e], first + e);
+            w[e] = key && key >= cut && weighs(v[e], top, c, low) ? pass ? 1 : weigh(v[e]) : 0;
+            sum += w[e];
+        }
+        run = block_scan(sum, sh.scratch) - sum;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) total += sh.scratch[i];
     }
-    u64 run = block_scan(sum, sh.scratch) - sum, total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) total += sh.scratch[i];
     u64 target = (u64)(fraction * (double)total), found = 0;
     target = target < total ? target : total - 1;
     int at = 0;
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
     if (cut) bins[tid] = 0;
     float best = -__builtin_inff();
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) best = __builtin_fmaxf(best, v[e]);
+    for (int e = 0; e < kPer; ++e) best = __builtin_fmaxf(best, __builtin_canonicalizef(v[e]));  // (a signalling NaN quiet)
     const uint32_t strip_key = wave_scan(logit_key(best), MaxOp());  // (in lane 63)
     const uint32_t best_key = block_reduce(logit_key(best), MaxOp(), scratch);
     const float top = key_logit(best_key);
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
                 const bool live = v[e] > -__builtin_inff();
                 valid += __builtin_popcountll(__ballot(live));
                 const int below = top_bin - value_bin(v[e]);
-                if (live && below < kBins) atomicAdd(&bins[below], (u64)1 << kBinShift | w >> kBinUnit);
+                if (live && (uint32_t)below < (uint32_t)kBins) atomicAdd(&bins[below], (u64)1 << kBinShift | w >> kBinUnit);
             }
         }
         if (rp.k) valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
@@ -723,11 +727,14 @@ __device__ __forceinline__ u64 find_cut(Digits d, const Source &key_at, int n, c
 #pragma unroll 4
     for (int i = tid; i < n; i += kThreads) {
         const u64 key = key_at(i);
-        if (key >= limit && ((key ^ d.prefix) & d.above) == 0) few[atomicAdd(&sh.cuts[1], 1)] = key;
+        if (key >= limit && ((key ^ d.prefix) & d.above) == 0) {
+            const int at = atomicAdd(&sh.cuts[1], 1);
+            if (at < kFew) few[at] = key;
+        }
     }
     __syncthreads();
     if (tid < 64) {
-        const int m = sh.cuts[1];
+        const int m = sh.cuts[1] < kFew ? sh.cuts[1] : kFew;
         const u64 key = tid < m ? few[tid] : 0, own = tid < m ? weigh(keys.logit(key)) : 0;
         u64 count = base_count + 1, sum = base_weight + own;
         for (int i = 0; i < m; ++i) {
@@ -787,7 +794,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const int lead = row_lead(row);
     u64 cut = 1;
     const bool listed = plan.state == kCollect;
-    const int n = listed ? (int)plan.listed : 0;
+    const int n = listed ? plan.listed < (uint32_t)kList ? (int)plan.listed : kList : 0;
     for (int s = tid; s < strips; s += kThreads) extra[s] = 0;
     if (n) {
         const u64 *from = row_list(args, scratch);

@@ -185,6 +185,27 @@ def test_masks(rt):
             assert tokens[7] == (17 if greedy else 4000)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_signalling_nans(rt, dtype):
+    """Every kind of NaN (signalling ones too, of both signs) beside the largest logits, in every place of a
+    thread's, a wave's and a piece's run: none hides another entry."""
+    vocab, rows = 9000, 4
+    logits = logits_of(rows, vocab, torch.float32, 61, 20).to(dtype)
+    bits = logits.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    kinds = ([0x7F800001, 0x7FA00000, 0x7FC00000, -0x7FFFFF, -1] if dtype == torch.float32 else
+             [0x7F81, 0x7FA0, 0x7FC0, -0x7F, -1])
+    top = torch.topk(logits.float(), 40).indices
+    for r in range(rows):
+        for i, at in enumerate(top[r].tolist()):
+            for step in (-1, 1, 2, 3):
+                if 0 <= at + step < vocab and at + step not in set(top[r].tolist()):
+                    bits[r, at + step] = kinds[(i + step) % len(kinds)]
+    u, params = params_of(rows, 62, (1, 1, 0, 0))
+    check_all(logits, u, params, *call(rt, logits, u, params))
+    tokens, _ = call(rt, logits, None, {})
+    assert torch.equal(tokens.long(), top[:, 0])
+
+
 def test_parameters_at_their_ends(rt):
     """top_k below 1 and past the vocabulary, top_p of 0, 1 and beyond, min_p of 1 and beyond, u of 0 and
     1 and beyond, and NaN for each."""
