@@ -469,7 +469,7 @@ size_t splosh_sample_workspace_bytes(int64_t rows, int64_t vocab);
  *   - NaN and -inf entries are never chosen; a row without any other gets id 0xffffffff (a row of zeros in
  *     the embedding lookups) and logprob -inf. With +inf among them, the entries of +inf alone have
  *     weight, the same each.
- *   - T <= 0 or NaN: the largest entry, the first of equal ones; logprob 0.
+ *   - T <= 0 or NaN: the largest entry, the first of equal ones; logprob 0. (T below 2^-126 as 2^-126.)
  *   - Else the entries in order, larger logits first and of equal ones the lower index, with weights
  *     w = exp((logit - max) / T). k >= 1 keeps the first k. Of these, p < 1 keeps the shortest run
  *     from the start that has p or more of their weight (one entry at least). Of these, q > 0 keeps

@@ -99,20 +99,22 @@ struct Weights {
     // m 2^32 (m: 24 bits and the power's) moved down to m 2^(40 - 24) at the exponent 0, or 1 less where the
     // two whole numbers are rounded apart.
     static constexpr int kShift = 32 - (kWeightBits - 24);
+    // 2^f. (Far below top f can be anything, and NaN for a NaN or -inf: none.)
+    static __device__ __forceinline__ float power(float f) {
+        return __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_exp2f(f), 0.0f), 4.0f);
+    }
     // The same as a number, 1 at top; top finite. NaN and -inf weigh nothing.
     __device__ __forceinline__ float relative(float v) const {
 #pragma clang fp contract(off)
         const float d = v - s, n = __builtin_rintf(d * c_high);
         const float f = __builtin_fmaf(d, c_high, -n) + __builtin_fmaf(d, c_low, -fraction);
-        // (Far below top f can be anything.)
-        const float e = __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_exp2f(f), 0.0f), 4.0f);
-        return __builtin_ldexpf(e, (int)__builtin_fmaxf(n - (shift0 - (float)kShift), -200.0f));
+        return __builtin_ldexpf(power(f), (int)__builtin_fmaxf(n - (shift0 - (float)kShift), -200.0f));
     }
     __device__ __forceinline__ u64 operator()(float v) const {
 #pragma clang fp contract(off)  // (n is the rounded product's)
         const float d = v - s, n = __builtin_rintf(d * c_high);
         const float f = __builtin_fmaf(d, c_high, -n) + __builtin_fmaf(d, c_low, -fraction);
-        float e = __builtin_amdgcn_exp2f(f);
+        float e = power(f);
         e = v == infinite ? 0.5f : e;
         int shift = (int)(shift0 - n);
         shift = shift < kShift - 1 ? kShift - 1 : shift > 63 ? 63 : shift;  // (an infinite one's: the least)
@@ -259,7 +261,7 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs &args, int64_t 
     const int k = args.p.top_k ? args.p.top_k[r] : 0;
     RowParams out;
     out.greedy = !args.p.uniforms || !(t > 0.0f);
-    out.c = 1.4426950408889634074 / (double)t;
+    out.c = 1.4426950408889634074 / (double)(t > 0x1p-126f ? t : 0x1p-126f);  // (so that fp32 holds it)
     out.k = k > 0 ? k : 0;
     out.p = p < 1.0f ? p : 1.0f;
     out.q = q > 0.0f ? (q < 1.0f ? q : 1.0f) : 0.0f;
@@ -692,7 +694,8 @@ __device__ __forceinline__ void count_digits(Digits &d, const Source &key_at, in
 
 // The smallest run from the start of the order with `k` elements, or with weight >= share where k is 0: its last
 // key, of those >= limit; *weight its weight. `d`: the first step. Where rounding has what comes before the keys
-// reach the share already, the first key.
+// reach the share already, the first key. Where no run reaches it (the pieces' weights, of which it is a share, hold
+// more of those below a unit of the row's), 0.
 template <typename Source, typename Keys>
 __device__ __forceinline__ u64 find_cut(Digits d, const Source &key_at, int n, const Keys &keys, const Weights &weigh, u64 limit,
                                         u64 k, double share, u64 *weight, u64 *memory, Shared &sh) {
@@ -711,6 +714,7 @@ __device__ __forceinline__ u64 find_cut(Digits d, const Source &key_at, int n, c
         }
         if (tid == 0) sh.cuts[1] = 0;
         __syncthreads();
+        if (sh.cuts[0] < 0) return 0;
         const u64 base_count = sh.weights[0], base_weight = sh.weights[1], inside = sh.weights[3];
         d.prefix |= (u64)(uint32_t)sh.cuts[0] << d.shift;
         d.above = ~(u64)0 << d.shift;
@@ -765,6 +769,7 @@ __device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, const Keys
     d.shift = top_bit < kDigitBits ? 0 : top_bit - kDigitBits + 1;
     d.above = ~(u64)0 << top_bit << 1;
     d.prefix = most & d.above;
+    if (threadIdx.x == 0) sh.cuts[0] = -1;
     count_digits(d, key_at, n, keys, weigh, cut, plan.above, base_weight, memory, sh);
     for (int pass = 0; pass < 2; ++pass) {
         if (pass ? !by_share : !by_count) continue;
@@ -803,9 +808,15 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
         const u64 base_weight = block_reduce(above, SumOp(), sh.scratch);
         cut = find_cuts([&](int i) { return list[i]; }, n, keys, keys.least(bin_edge(plan.low_bin - 1)),
                         keys.most(bin_edge(plan.above_bin + 1)), weigh, plan, rp, base_weight, memory, sh);
+        if (cut == 0) {  // the whole list
+            u64 last = 0;  // (the complement)
+            for (int i = tid; i < n; i += kThreads) last = last > ~list[i] ? last : ~list[i];
+            cut = ~block_reduce(last, MaxOp(), sh.scratch);
+        }
     } else if (!listed) {
         cut = find_cuts([&](int i) { return keys(logit_of(row[i]), i); }, args.vocab, keys, 0, keys.most(__builtin_inff()),
                         weigh, plan, rp, 0, memory, sh);
+        cut = cut ? cut : 1;
     }
     // What min-p leaves of the kept elements of the list, or of the row, to their strips.
     __syncthreads();

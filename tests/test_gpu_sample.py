@@ -1,5 +1,7 @@
 """splosh_sample against its definition in 64 bits, row by row: filters alone and together, ties, masks,
 values that are not finite, and every odd length and layout."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -200,8 +202,9 @@ def test_signalling_nans(rt, dtype):
             for step in (-1, 1, 2, 3):
                 if 0 <= at + step < vocab and at + step not in set(top[r].tolist()):
                     bits[r, at + step] = kinds[(i + step) % len(kinds)]
-    u, params = params_of(rows, 62, (1, 1, 0, 0))
-    check_all(logits, u, params, *call(rt, logits, u, params))
+    for on in ((1, 1, 0, 0), (1, 0, 1, 0), (1, 0, 0, 1), (1, 0, 0, 0)):
+        u, params = params_of(rows, 62, on)
+        run(rt, logits, u, params)
     tokens, _ = call(rt, logits, None, {})
     assert torch.equal(tokens.long(), top[:, 0])
 
@@ -227,6 +230,51 @@ def test_parameters_at_their_ends(rt):
         assert tokens[r] == best[r] and logprobs[r] == 0.0, r
     kept = kept_weights(logits[1].numpy())[0]
     assert int(tokens[1]) == int(np.nonzero(kept >= 2.0 ** -40)[0][-1])
+
+
+@pytest.mark.parametrize("far", [-27.4, -28.5])
+def test_a_share_of_weights_below_a_unit(rt, far):
+    """One large logit and 200000 that weigh about 2^-40 of it each, 2e-7 to 6e-8 together: with the largest
+    p below 1 the share is not reached before them. The token is the large one's for every u from 1e-6 to 1 - 1e-6."""
+    rows, vocab = 8, 200003
+    logits = (far + 0.01 * torch.rand(rows, vocab, generator=torch.Generator().manual_seed(63))).float()
+    at = torch.arange(rows) * 23456 + 7
+    logits[torch.arange(rows), at] = 0.0
+    u = torch.linspace(1e-6, 1.0 - 1e-6, rows)
+    top_p = torch.full((rows,), 1.0 - 2.0 ** -24)
+    for params in ({"top_p": top_p}, {"top_p": top_p, "min_p": torch.full((rows,), 0.01)},
+                   {"top_p": top_p, "top_k": torch.full((rows,), 5000, dtype=torch.int32)}):
+        tokens, logprobs = call(rt, logits, u, params)
+        assert torch.equal(tokens.long(), at) and (logprobs <= 0).all() and (logprobs >= -1e-6).all()
+
+
+@pytest.mark.parametrize("offset", [0.0, -3.0, 3.0])
+def test_temperatures_below_the_normal_numbers(rt, offset):
+    """The largest entry alone has weight; of two equal ones each half of it."""
+    rows, vocab = 4, 9001
+    logits = -1.0 - torch.rand(rows, vocab, generator=torch.Generator().manual_seed(64)) + offset
+    logits[:, [700, 8800]] = offset
+    u = torch.tensor([0.0, 0.49, 0.51, 1.0])
+    for t in (2.0 ** -149, 1e-40, 2.0 ** -126):
+        for params in ({}, {"top_p": torch.full((rows,), 0.9)}, {"min_p": torch.full((rows,), 0.5)},
+                       {"top_k": torch.full((rows,), 50, dtype=torch.int32)}):
+            tokens, logprobs = call(rt, logits, u, {"temperature": torch.full((rows,), t), **params})
+            assert tokens.tolist() == [700, 700, 8800, 8800]
+            assert (logprobs + math.log(2.0)).abs().max() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("vocab,dtype", [(524287, torch.float32), (600001, torch.bfloat16), (1 << 21, torch.float32),
+                                         (1 << 21, torch.bfloat16)])
+def test_largest_vocabularies(rt, vocab, dtype):
+    """More strips than a workgroup has threads; bf16's ties overflow the list, and the row is searched whole."""
+    rows = 2
+    logits = logits_of(rows, vocab, torch.float32, vocab, 48).to(dtype)
+    wide = torch.full((rows, vocab + 3), 1e4, dtype=dtype)
+    wide[:, 1 : 1 + vocab] = logits
+    for on in ((1, 0, 0, 0), (1, 1, 0, 1), (1, 0, 1, 0)):
+        u, params = params_of(rows, vocab + 1, on)
+        params = off_borders(logits.float().numpy(), params)
+        check_all(logits, u, params, *call(rt, wide.cuda()[:, 1 : 1 + vocab], u, params), f"{on}")
 
 
 def test_defaults(rt):
