@@ -92,8 +92,9 @@ __device__ __forceinline__ void wave_fence() {
 // sums in LDS. a's rows are the MFMA's rows and the activation rows its columns: the sum's four registers
 // are then four neighbouring ranks of one activation row, a 16-byte store.
 //
-// A load has the four lanes of a quad read the 64 bytes of one row, and goes through LDS to the MFMA's order, in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache
-// lookup of its own.
+// A load has the four lanes of a quad read the 64 bytes of one row, and goes through LDS to the MFMA's order,
+// in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache lookup of
+// its own.
 
 constexpr int kDownWaves = 4;
 
@@ -190,6 +191,7 @@ __device__ __attribute__((always_inline)) void down_rows(const AdapterArgs &args
         if (row >= 0 && r < rank)
             *(f32x4 *)(args.t + ((int64_t)slice * args.rows + base + row) * args.t_cols + g.t_offset + r) = v * scale;
     }
+    __syncthreads();  // (the next adapter's operands go where these sums were)
 }
 
 template <int RBMAX, int P, bool FAST>
@@ -541,8 +543,8 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     args.rows = rows;
     const int64_t esize = out_dtype == SPLOSH_F32 ? 4 : 2;
     auto aligned16 = [](const void *p, int64_t a, int64_t b) { return (uintptr_t)p % 16 == 0 && a % 8 == 0 && b % 8 == 0; };
-    auto near = [](int64_t elements, int64_t size) { return elements < (int64_t)kNowhere / size; };
-    bool down_fast = aligned16(x, ldx, w[0].inner) && near(kChunk * ldx, 2), up_fast = true;
+    auto near = [](int64_t n, int64_t stride, int64_t size) { return stride < (int64_t)kNowhere / size / n; };
+    bool down_fast = aligned16(x, ldx, w[0].inner) && near(kChunk, ldx, 2), up_fast = true;
     int at = 0, columns = 0;
     int64_t most_rank = 0, tiles = 0, most_tiles = 0;
     for (int i = 0; i < group; ++i) {
@@ -553,10 +555,10 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
         tiles += up_tiles(w[i]);
         most_tiles = up_tiles(w[i]) > most_tiles ? up_tiles(w[i]) : most_tiles;
         down_fast = down_fast && aligned16(w[i].a, w[i].a_slot_stride, w[i].a_row_stride) &&
-                    near(w[i].max_rank * w[i].a_row_stride, 2);
-        up_fast = up_fast && (uintptr_t)outs[i] % 16 == 0 && ldcs[i] * esize % 16 == 0 && w[i].rows % 16 == 0 &&
-                  w[i].max_rank % 8 == 0 && near(kChunk * ldcs[i], esize) &&
-                  aligned16(w[i].b, w[i].b_slot_stride, w[i].b_row_stride) && near(w[i].rows * w[i].b_row_stride, 2);
+                    near(w[i].max_rank, w[i].a_row_stride, 2);
+        up_fast = up_fast && (uintptr_t)outs[i] % 16 == 0 && ldcs[i] % (16 / esize) == 0 && w[i].rows % 16 == 0 &&
+                  w[i].max_rank % 8 == 0 && near(kChunk, ldcs[i], esize) &&
+                  aligned16(w[i].b, w[i].b_slot_stride, w[i].b_row_stride) && near(w[i].rows, w[i].b_row_stride, 2);
     }
     const unsigned chunks = (unsigned)((rows + kChunk - 1) / kChunk);
     const unsigned down_x = (unsigned)(columns * args.slices);

@@ -266,6 +266,57 @@ def test_graph_replays(rt):
         check(buf, nout, nx, nw, slots.cpu())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rank", [72, 256])
+def test_group_captured_first(rt, rank, dtype):
+    """A group with operands past 64 KB of LDS, captured before any eager call of its kind, replayed on buffers
+    that eager calls on the same workspace use in between."""
+    rows, outputs = 70, (96, 33)
+    cases = [host_case(rows, 200, n, rank, 3, dtype, 83 + n) for n in outputs]
+    x, slots = cases[0][0], slots_of(rows, 3, 83)
+    ws_of, xd, sl = [on_gpu(rt, c[1]) for c in cases], x.cuda(), slots.cuda()
+    outs = [c[2].cuda() for c in cases]
+    ws = torch.zeros(rt.adapters_workspace_bytes(ws_of, rows), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        rt.add_adapters_group(outs, xd, ws_of, sl, workspace=ws)
+    for _ in range(3):
+        for o, c in zip(outs, cases):
+            o.copy_(c[2])
+        rt.add_adapters(torch.zeros(5, outputs[1], dtype=dtype, device="cuda"), xd, ws_of[1], sl, rows=5, workspace=ws)
+        g.replay()
+        torch.cuda.synchronize()
+        for o, c in zip(outs, cases):
+            check(o, c[2], x, c[1], slots)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rank,count", [(16, 40), (48, 40), (48, 3)])
+def test_many_adapters_a_workgroup(rt, rank, count, dtype):
+    """More adapters in a chunk than workgroups take them one each: the next one's operands do not meet the
+    last one's sums."""
+    rows = 4000
+    case = host_case(rows, 96, 80, rank, count, dtype, 85)
+    slots = slots_of(rows, count, 85)
+    first = run(rt, case, slots)
+    for _ in range(3):
+        again = run(rt, case, slots)
+        assert torch.equal(again, first)
+
+
+def test_row_strides_past_every_product(rt):
+    """A single row: its stride can be anything that 63 bits hold, and is not multiplied by a chunk's 64 rows."""
+    case = host_case(1, 64, 48, 16, 2, torch.float32, 86)
+    x, adapters, out = case
+    slots = torch.tensor([1], dtype=torch.int32)
+    for stride in (1 << 56, 1 << 57, 1 << 58):
+        got = out.cuda()
+        rt.add_adapters(got.as_strided((1, 48), (stride, 1)), x.cuda().as_strided((1, 64), (stride, 1)), on_gpu(rt, adapters),
+                        slots.cuda())
+        check(got, out, x, adapters, slots)
+
+
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_repeatable(rt, rows):
     x, adapters, out = host_case(rows, 1280, 264, 32, 4, torch.float32, 81)
