@@ -32,8 +32,11 @@ constexpr int kPiece = kThreads * kPer;      // and a workgroup
 constexpr int kBins = kThreads;              // value bins of a piece
 constexpr int kWeightBits = 40;
 // A bin's entry while it is counted: 15 bits of count (a piece has 2^13 elements) over 49 of weight in units of
-// 2^-35; as it is left, the count over the fp32 weight in units of 2^-40.
-constexpr int kBinShift = 49, kBinUnit = kWeightBits - 35;
+// 2^-31, so that an element's fits 32 bits; as it is left, the count over the fp32 weight in units of 2^-40.
+constexpr int kBinShift = 49, kBinBits = 31;
+// Rows whose largest logit is in a bin below this one are searched whole: 512 bins further down NaN and -inf
+// (past bin -8192) would be among those that are counted.
+constexpr int kLowestBin = -7000;
 constexpr int kMaxStrips = kThreads * kWaves;
 constexpr int kList = 8192;                  // elements of a row's list
 constexpr int kBatchRows = 256;              // rows of one launch
@@ -103,13 +106,6 @@ struct Weights {
     static __device__ __forceinline__ float power(float f) {
         return __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_exp2f(f), 0.0f), 4.0f);
     }
-    // The same as a number, 1 at top; top finite. NaN and -inf weigh nothing.
-    __device__ __forceinline__ float relative(float v) const {
-#pragma clang fp contract(off)
-        const float d = v - s, n = __builtin_rintf(d * c_high);
-        const float f = __builtin_fmaf(d, c_high, -n) + __builtin_fmaf(d, c_low, -fraction);
-        return __builtin_ldexpf(power(f), (int)__builtin_fmaxf(n - (shift0 - (float)kShift), -200.0f));
-    }
     __device__ __forceinline__ u64 operator()(float v) const {
 #pragma clang fp contract(off)  // (n is the rounded product's)
         const float d = v - s, n = __builtin_rintf(d * c_high);
@@ -120,6 +116,25 @@ struct Weights {
         shift = shift < kShift - 1 ? kShift - 1 : shift > 63 ? 63 : shift;  // (an infinite one's: the least)
         return (u64)(uint32_t)(e * 16777216.0f) << 32 >> shift;
     }
+};
+
+// The same as a number, 1 at top, for sums over a piece: 2^x of the fp32 product x = (v - top) c and, to first
+// order, of what the product rounds off. Off by the power's last place and by v - top's half a one (2^-25 x).
+// NaN and -inf weigh `none`, which is 0 for all but the largest T. top finite.
+struct PieceWeights {
+    float top, c_high, c_low, least, none;
+    __device__ __forceinline__ PieceWeights(float top, double c) : top(top), c_high((float)c), c_low((float)(c - (double)c_high)) {
+        // (Past it a weight is 0.)
+        least = __builtin_fmaxf(-160.0f / c_high, -__FLT_MAX__);
+        none = of(least);
+    }
+    __device__ __forceinline__ float of(float d) const {
+#pragma clang fp contract(off)
+        const float x = d * c_high, rest = __builtin_fmaf(d, c_low, __builtin_fmaf(d, c_high, -x));
+        const float e = __builtin_amdgcn_exp2f(x);
+        return __builtin_fmaf(e, rest * 0.6931471805599453f, e);
+    }
+    __device__ __forceinline__ float operator()(float v) const { return of(__builtin_fmaxf(v - top, least)); }
 };
 
 // w >= q for min-p, low = log2(q).
@@ -433,29 +448,45 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
         for (int e = kPer - 1; e >= 0; --e)
             if (v[e] == top) at = ~(uint32_t)(base + index_of<T>(e));
         index = ~block_reduce(at, MaxOp(), scratch);
-    } else if (cut) {
-        if (best_key) {
-            const int top_bin = value_bin(top);
-            const Weights weigh(top, rp.c);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const u64 w = weigh(v[e]);
-                weight += w;
-                const bool live = v[e] > -__builtin_inff();
-                valid += __builtin_popcountll(__ballot(live));
-                const int below = top_bin - value_bin(v[e]);
-                if (live && (uint32_t)below < (uint32_t)kBins) atomicAdd(&bins[below], (u64)1 << kBinShift | w >> kBinUnit);
-            }
-        }
-        if (rp.k) valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
     } else if (best_key) {
-        // (A lane's sixteen in fp32, the lanes in integers. Where the largest is infinite, those that are.)
-        const bool infinite = top == __builtin_inff();
-        const Weights weigh(infinite ? 0.0f : top, rp.c);
-        float sum = 0.0f;
+        if (rp.k) {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum += infinite ? (v[e] == top ? 1.0f : 0.0f) : weigh.relative(v[e]);
-        weight = (u64)(sum * (float)((u64)1 << kWeightBits));
+            for (int e = 0; e < kPer; ++e) valid += __builtin_popcountll(__ballot(v[e] > -__builtin_inff()));
+        }
+        // Where the largest is infinite, those that are have weight.
+        const bool infinite = top == __builtin_inff();
+        if (infinite) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[e] = v[e] == top ? 0.0f : -__builtin_inff();
+        }
+        const PieceWeights weigh(infinite ? 0.0f : top, rp.c);
+        // A lane's sixteen in fp32, the lanes in integers.
+        float sum = 0.0f;
+        if (cut) {
+            const int top_bin = value_bin(top);
+            if (top_bin >= kLowestBin - kBins && !infinite) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const float w = weigh(v[e]);
+                    sum += w;
+                    const int below = top_bin - value_bin(v[e]);
+                    if ((uint32_t)below < (uint32_t)kBins)
+                        atomicAdd(&bins[below], (u64)1 << kBinShift | (uint32_t)__builtin_fmaf(w, (float)(1u << kBinBits), 0.5f));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) sum += weigh(v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) sum += weigh(v[e]);
+        }
+        if (weigh.none > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) sum -= v[e] > -__builtin_inff() ? 0.0f : weigh.none;
+        }
+        weight = (u64)(__builtin_fmaxf(sum, 0.0f) * (float)((u64)1 << kWeightBits));
+        if (rp.k) valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
     }
     if (!rp.greedy) {
         weight = wave_scan(weight, SumOp());
@@ -472,7 +503,7 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
     if (cut) {
         __syncthreads();
         const u64 entry = bins[tid];
-        const float w = (float)((entry & (((u64)1 << kBinShift) - 1)) << kBinUnit);
+        const float w = (float)((entry & (((u64)1 << kBinShift) - 1)) << (kWeightBits - kBinBits));
         row_bins(args, row)[(size_t)piece * kBins + tid] = entry >> kBinShift << 32 | __float_as_uint(w);
     }
 }
@@ -567,10 +598,12 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     }
     __syncthreads();
     if (by_share && (!by_count || sh.cuts[0] < kBins)) {
-        // (The bins' weights are fp32 sums of one product a piece: 2^-19 for a row of 32, 2^-15 for one of 512.)
+        // (The bins' weights are fp32 sums of one product a piece: 2^-19 for a row of 32, 2^-15 for one of 512;
+        // and of elements rounded to their units.)
         constexpr double kSlack = 1.0 / (1 << 14);
-        const double least = (double)rp.p * (double)(by_count ? sh.weights[0] : total) * (1.0 - kSlack);
-        const double most = (double)rp.p * (double)(by_count ? sh.weights[1] : total) * (1.0 + kSlack);
+        const double rounding = (double)args.vocab * (double)((u64)1 << (kWeightBits - kBinBits - 1));
+        const double least = (double)rp.p * (double)(by_count ? sh.weights[0] : total) * (1.0 - kSlack) - rounding;
+        const double most = (double)rp.p * (double)(by_count ? sh.weights[1] : total) * (1.0 + kSlack) + rounding;
         const double before = (double)(run_weight - own_weight);
         if (count && (double)run_weight >= least && (before < least || run_count == count)) sh.cuts[1] = tid;
         if (count && (double)run_weight >= most && (before < most || run_count == count)) sh.cuts[2] = tid;
@@ -582,7 +615,7 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     if (tid == to) sh.weights[3] = run_count;
     __syncthreads();
     if (tid == 0) {
-        const bool fits = from < kBins && to < kBins && sh.weights[3] - sh.weights[2] <= kList;
+        const bool fits = from < kBins && to < kBins && top_bin >= kLowestBin && top < __builtin_inff() && sh.weights[3] - sh.weights[2] <= kList;
         plan = {fits ? kCollect : kSearch, top_bin - from + 1, top_bin - to, top_key, total,
                 fits ? (uint32_t)sh.weights[2] : 0, 0, (uint32_t)valid, 0, rp.c, low};
     }

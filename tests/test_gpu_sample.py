@@ -263,6 +263,36 @@ def test_temperatures_below_the_normal_numbers(rt, offset):
             assert (logprobs + math.log(2.0)).abs().max() <= 2.0 ** -20
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1.0, 1e36, 3e38, float("inf")])
+def test_masks_at_the_largest_temperatures(rt, temperature, dtype):
+    """NaN and -inf weigh nothing where every other weight is the same, too."""
+    rows, vocab = 6, 20011
+    logits = logits_of(rows, vocab, torch.float32, 65).to(dtype)
+    mask = torch.rand(rows, vocab, generator=torch.Generator().manual_seed(66))
+    logits[mask < 0.5] = -math.inf
+    logits[mask < 0.1] = math.nan
+    for on in ((0, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (0, 1, 1, 0)):
+        u, params = params_of(rows, 67, on)
+        params["temperature"] = torch.full((rows,), temperature)
+        run(rt, logits, u, params, f"{on}")
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 100, 2.0 ** 112, 2.0 ** 120])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_logits_of_the_largest_sizes(rt, scale, sign):
+    """At both ends of fp32, where a bin is 2^-6 of a logit and the lowest bins are those of NaN and -inf."""
+    rows, vocab = 6, 9001
+    gen = torch.Generator().manual_seed(68)
+    logits = sign * scale * (1.0 + torch.rand(rows, vocab, generator=gen))
+    logits[torch.rand(rows, vocab, generator=gen) < 0.3] = -math.inf
+    logits[torch.rand(rows, vocab, generator=gen) < 0.1] = math.nan
+    for on in ((0, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 1, 1, 1)):
+        u, params = params_of(rows, 69, on)
+        params["temperature"] = torch.full((rows,), scale / 8)
+        run(rt, logits, u, params, f"{on}")
+
+
 @pytest.mark.parametrize("vocab,dtype", [(524287, torch.float32), (600001, torch.bfloat16), (1 << 21, torch.float32),
                                          (1 << 21, torch.bfloat16)])
 def test_largest_vocabularies(rt, vocab, dtype):
