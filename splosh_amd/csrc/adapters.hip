@@ -12,7 +12,12 @@
 // FAST kernels are for operands whose every 16-byte piece is whole, aligned and within a buffer
 // descriptor's reach (the usual case): their loads have no branches, since an offset out of a descriptor's
 // range reads zeros and writes nothing. The others load pieces at any alignment, where they are whole, and
-// element by element where they are not.
+// element by element where they are not (both launches on FAST operands: 64 rows, K5120 -> 2 x 17408: 15.3 us FAST,
+// 19.7 not; 2048 rows, K5120 -> N17408: 43 and 64).
+//
+// What has to move is the adapters' matrices in use, x, and out twice; the arithmetic, 2 rank (K + N) a row, is far
+// under the matrix core's rate. A step's small calls are two launches of 2 us, each with four dependent round
+// trips to memory (slots, ranks, operands, sums): 4.2 + 4.7 us for one row of K5120 -> N5120.
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -95,6 +100,11 @@ __device__ __forceinline__ void wave_fence() {
 // A load has the four lanes of a quad read the 64 bytes of one row, and goes through LDS to the MFMA's order,
 // in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache lookup of
 // its own.
+//
+// Bound by the reads of a: 64 rows of 32 adapters of ranks 16 to 64, K17408: 47 MB in 13.9 us (3.4 TB/s), 2 us of
+// it the launch. More loads in flight (the next steps' before this one's products; rows in runs of 128 bytes)
+// measured the same. One block of rows a workgroup (RBMAX 1, for up to 16 rows) saves the code and registers of the
+// other form: 4.9 us for 5.1 with eight rows on q, k and v. One panel of 16 ranks (P 1): 4.2 us for 4.7 with one row.
 
 constexpr int kDownWaves = 4;
 
@@ -251,6 +261,9 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
 // b's rows are the MFMA's rows and stay in registers while the adapter's rows go by, sixteen at a time. Their
 // sums pass through LDS, so that a wave reads and writes runs of 64 neighbouring outputs of a row: with
 // the MFMA's own layout, neighbouring lanes hold different rows, and four times the cache lookups.
+//
+// Bound by out, read and written: 2048 rows, N17408, bf16: 160 MB in 34 us (4.7 TB/s, a large copy's rate); 64 rows,
+// 2 x 17408, fp32, rank 16: 27 MB in 8.4 us.
 
 constexpr int kUpSumStride = 68;  // floats of a row of sums in LDS: 64 and a step of four banks
 
@@ -299,7 +312,8 @@ __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWe
     }
 }
 
-// NP: panels of 32 ranks held in registers; 0: any number of them, read again for each block of rows.
+// NP 1: ranks up to 32, b held in registers; NP 0: any rank, b read again for each block of rows (2048 rows of rank
+// 16: 34.2 us held, 38.6 read again; holding 64 ranks measured level with reading them again).
 template <int NP, typename OUT, bool FAST>
 __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(AdapterArgs args) {
     constexpr int kPieces = sizeof(OUT) == 4 ? 3 : 2, kLoads = sizeof(OUT), kPer = 16 / sizeof(OUT), kHeld = NP ? NP : 1;
@@ -459,8 +473,8 @@ static int down_columns(const splosh_adapters &w) { return (int)(w.max_rank + kD
 static int64_t up_tiles(const splosh_adapters &w) { return (w.rows + kUpColumns - 1) / kUpColumns; }
 
 // Steps of 32 k a slice of K, whole rounds of the workgroup's waves: a workgroup a CU from the chunks and
-// projections alone, eight slices at most (the second launch adds them up; K17408, 64 rows of 28 adapters,
-// both launches: 4 slices 31.5 us, 8 24.6, 16 29.8).
+// projections alone, eight slices at most (the second launch adds them up; K17408, 64 rows of 32 adapters,
+// both launches: 4 slices 23.1 us, 8 21.1, 16 23.2).
 struct SlicePlan {
     int steps, slices;
 };
@@ -491,8 +505,9 @@ static int64_t most_parts(const splosh_adapters *w, int group, int64_t rows) {
     return count < most ? count : most;
 }
 
-// The adapters of a chunk go to up to this many workgroups: each its own where the launch is small, one for
-// all where it fills the device anyway.
+// The adapters of a chunk go to up to this many workgroups: each its own where the launch is small, several to one
+// where it fills the device anyway: eight workgroups a CU (64 rows of eight, K5120 -> 2 x 17408, the second launch:
+// 8.4 us, two a CU 12.0).
 static int plan_turns(int64_t parts, int64_t others) {
     const int64_t n = 2048 / others;
     return (int)(n < 1 ? 1 : n < parts ? n : parts);
@@ -523,7 +538,6 @@ static hipError_t launch_up(const AdapterArgs &args, int panels, bool fast, int 
     if (!fast) return panels == 1 ? launch_up<1, OUT, false>(args, lds, grid, stream)
                                   : launch_up<0, OUT, false>(args, lds, grid, stream);
     if (panels == 1) return launch_up<1, OUT, true>(args, lds, grid, stream);
-    if (panels == 2) return launch_up<2, OUT, true>(args, lds, grid, stream);
     return launch_up<0, OUT, true>(args, lds, grid, stream);
 }
 
@@ -576,14 +590,13 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     // Tiles a workgroup, for which t is staged once: so many that six workgroups a CU are left (2048 rows,
-    // N17408: 33.4 us, with three a CU 35.7).
+    // N17408: two tiles 34.1 us, one 40.9, four 34.2; 64 rows, 2 x 17408: one tile 8.2, four 12.0).
     const int64_t share = (tiles * chunks * (chunks == 1 ? parts : 1) + 1535) / 1536;
     args.tiles = (int)(share < most_tiles ? share : most_tiles);
     const unsigned up_x = (unsigned)((most_tiles + args.tiles - 1) / args.tiles);
-    // An adapter's rows in shares where there are fewer than three workgroups a CU and more than 16 rows an adapter
-    // (333 rows of three, K6144 -> N5120: 12.3 us whole, 9.3 in four).
-    const int64_t whole = tiles / args.tiles * chunks * (chunks == 1 ? parts : 1);
-    args.shares = rows <= 16 * parts || whole >= 768 ? 1 : whole >= 384 || rows <= 32 ? 2 : 4;
+    // More than 16 rows an adapter: its rows in shares, a block of sixteen each (333 rows of three adapters of rank
+    // 64, K6144 -> N5120: 9.2 us, one workgroup for all of a chunk's rows 11.6; 500 of two, rank 128: 12.8 and 21.0).
+    args.shares = rows <= 16 * parts ? 1 : rows <= 32 ? 2 : 4;
     args.turns = plan_turns(parts, (int64_t)up_x * chunks * group * args.shares);
     const dim3 up(up_x, chunks, (unsigned)(group * args.turns * args.shares));
     const int up_panels = (int)(most_rank + 31) / 32, blocks = rows < kChunk ? (int)(rows + 15) / 16 : kChunk / 16;

@@ -17,7 +17,10 @@
 //   finish  (rows)   the cut, by a radix search in the list, the strip the draw falls into and the token
 //           in it. A row whose cut lies below its bins, or in bins of more elements than the list
 //           holds, is searched whole.
-// The launches over pieces hold nothing but what they stream, so that four workgroups share a CU.
+// The launches over pieces hold nothing but what they stream, so that four workgroups share a CU. The rows' launches
+// are chains of a few dependent round trips, about 1.5 us of each the launch's own: one row of 248320 with every
+// filter takes 5.2 + 6.9 + 4.2 + 7.3 us, and 64 of them 18 + 7.7 + 7.8 + 8.1. What has to move is the logits, once:
+// 64 rows of 248320 fp32, 64 MB, 13 us at the rate of a large copy.
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -419,6 +422,10 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
 }
 
 // ---- scan -------------------------------------------------------------------------------------------
+//
+// Bound by its vector instructions beside the read: 35 an element with bins (an exponential at a quarter of the rate,
+// an LDS atomic), 20 without. 64 rows of 248320: fp32 with bins 64 MB in 17-19 us (3.4-3.7 TB/s), bf16 with the
+// temperature alone 32 MB in 12.3 us (2.6 TB/s). 512 threads of sixteen logits each: with 256 or 1024 threads slower.
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) {
@@ -509,6 +516,9 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 }
 
 // ---- settle -----------------------------------------------------------------------------------------
+//
+// Latency: the pieces' heads, then their bins (at most 32 in flight a thread), then three scans over the workgroup;
+// 6.9 us for one row of 31 pieces, 7.7 for 64. Loading the bins before the heads are known measured slower.
 
 // 2^t for t <= 0, in 64 bits.
 __device__ __forceinline__ double power_of(double t) { return t > -1000.0 ? exp2(t) : 0.0; }
@@ -622,6 +632,10 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
 }
 
 // ---- collect ----------------------------------------------------------------------------------------
+//
+// Reads again what can be above the list or in it, strip by strip: nothing but the strips' records for rows that are
+// settled, few strips for rows with a peaked head (64 rows of 248320 fp32: 14 of 64 MB, 7.8 us), all of a flat row's
+// (16 of 100003 bf16 with top-p: 7.2 us).
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs args) {
@@ -687,6 +701,10 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
 }
 
 // ---- finish -----------------------------------------------------------------------------------------
+//
+// Latency: the plan, the list, one to three steps of the search, the strip; 7.3 us a row with a list of a few
+// elements, 9.3 with one of thousands. Up to 64 keys that share a digit are ranked by one wave, which saves the steps
+// below it.
 
 // A step of the search for a cut among keys: how many there are with each digit of nine bits, and their weight.
 struct Digits {
