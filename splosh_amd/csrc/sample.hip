@@ -172,6 +172,10 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ u64 dpp_move(u64 v) {
     return (u64)dpp_move<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp_move<CTRL, ROWS>((uint32_t)v);
 }
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
 struct MaxOp {
     template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
@@ -793,8 +797,7 @@ __device__ __forceinline__ u64 find_cut(Digits d, const Source &key_at, int n, c
         const u64 key = tid < m ? few[tid] : 0, own = tid < m ? weigh(keys.logit(key)) : 0;
         u64 count = base_count + 1, sum = base_weight + own;
         for (int i = 0; i < m; ++i) {
-            const u64 other = few[i], w = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(own >> 32), i) << 32 |
-                                          (uint32_t)__builtin_amdgcn_readlane((int)own, i);
+            const u64 other = few[i], w = lane_of(own, i);
             if (other > key) ++count, sum += w;
         }
         if (tid < m && ends(count, sum) && (count == base_count + 1 || !ends(count - 1, sum - own))) {
@@ -829,6 +832,43 @@ __device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, const Keys
     return cut;
 }
 
+// The same for a list of no more keys than a wave has lanes, lane i the i-th, in every wave: each wave counts what an
+// eighth of them adds before each key, and all add the eighths up. `above`: this thread's part of the weight above
+// the list's bins.
+__device__ __forceinline__ u64 rank_few(u64 key, u64 own, int n, u64 above, const RowPlan &plan, const RowParams &rp,
+                                        u64 *memory, Shared &sh) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    u64 count = 0, sum = 0;
+    for (int i = wave; i < n; i += kWaves)
+        if (lane_of(key, i) > key) ++count, sum += lane_of(own, i);
+    memory[threadIdx.x] = sum;
+    memory[kThreads + threadIdx.x] = count;
+    above = wave_scan(above, SumOp());
+    if (lane == 63) sh.scratch[wave] = above;
+    __syncthreads();
+    count = plan.above + 1;
+    sum = own;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        sum += memory[w * 64 + lane] + sh.scratch[w];
+        count += memory[kThreads + w * 64 + lane];
+    }
+    const bool any = lane < n;
+    u64 cut = 1, weight = plan.total, hit;
+    if (rp.k && (uint32_t)rp.k < plan.valid && (hit = __ballot(any && count == (u64)rp.k))) {
+        cut = lane_of(key, __builtin_ctzll(hit));
+        weight = lane_of(sum, __builtin_ctzll(hit));
+    }
+    if (rp.p < 1.0f) {
+        const double share = (double)rp.p * (double)weight;
+        hit = __ballot(any && (double)sum >= share && (count == plan.above + 1 || (double)(sum - own) < share));
+        if (!hit) hit = __ballot(any && count == (u64)plan.above + n);  // (no run reaches it: the whole list)
+        const u64 last = hit ? lane_of(key, __builtin_ctzll(hit)) : 1;
+        cut = last > cut ? last : cut;
+    }
+    return cut;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args) {
     __shared__ Shared sh;
@@ -840,6 +880,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const Strip *of = row_strips(args, scratch);
     const u64 strip_kept = tid < strips ? of[tid].kept : 0;  // (the first 512)
     u64 above = tid < strips ? of[tid].above : 0;
+    const u64 early = row_list(args, scratch)[tid & 63];  // (before it is known how many there are)
     if (plan.state == kSettled) return;
     const T *row = (const T *)args.logits + r * args.ld;
     const RowParams rp = row_params(args, r);
@@ -852,10 +893,20 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const bool listed = plan.state == kCollect;
     const int n = listed ? plan.listed < (uint32_t)kList ? (int)plan.listed : kList : 0;
     for (int s = tid; s < strips; s += kThreads) extra[s] = 0;
-    if (n) {
+    if (n)
+        for (int s = tid + kThreads; s < strips; s += kThreads) above += of[s].above;
+    const bool few = listed && n <= kFew;
+    if (few) {
+        if (n) {
+            const bool any = (tid & 63) < n;
+            const float v = keys.logit(early);
+            const u64 own = any ? weigh(v) : 0;
+            cut = rank_few(any ? early : 0, own, n, above, plan, rp, memory, sh);
+            if (tid < n && early >= cut && weighs(v, top, c, low)) atomicAdd(&extra[(keys.index(early) + lead) / kStrip], own);
+        }
+    } else if (n) {
         const u64 *from = row_list(args, scratch);
         for (int i = tid; i < n; i += kThreads) list[i] = from[i];
-        for (int s = tid + kThreads; s < strips; s += kThreads) above += of[s].above;
         const u64 base_weight = block_reduce(above, SumOp(), sh.scratch);
         cut = find_cuts([&](int i) { return list[i]; }, n, keys, keys.least(bin_edge(plan.low_bin - 1)),
                         keys.most(bin_edge(plan.above_bin + 1)), weigh, plan, rp, base_weight, memory, sh);
@@ -864,14 +915,14 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
             for (int i = tid; i < n; i += kThreads) last = last > ~list[i] ? last : ~list[i];
             cut = ~block_reduce(last, MaxOp(), sh.scratch);
         }
-    } else if (!listed) {
+    } else {
         cut = find_cuts([&](int i) { return keys(logit_of(row[i]), i); }, args.vocab, keys, 0, keys.most(__builtin_inff()),
                         weigh, plan, rp, 0, memory, sh);
         cut = cut ? cut : 1;
     }
     // What min-p leaves of the kept elements of the list, or of the row, to their strips.
     __syncthreads();
-    for (int i = tid; i < (listed ? n : args.vocab); i += kThreads) {
+    for (int i = tid; i < (few ? 0 : listed ? n : args.vocab); i += kThreads) {
         const u64 key = listed ? list[i] : keys(logit_of(row[i]), i);
         const float v = keys.logit(key);
         if (key >= cut && weighs(v, top, c, low)) atomicAdd(&extra[(keys.index(key) + lead) / kStrip], weigh(v));
