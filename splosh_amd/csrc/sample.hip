@@ -524,8 +524,11 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 // Latency: the pieces' heads, then their bins (at most 32 in flight a thread), then three scans over the workgroup;
 // 6.9 us for one row of 31 pieces, 7.7 for 64. Loading the bins before the heads are known measured slower.
 
-// 2^t for t <= 0, in 64 bits.
-__device__ __forceinline__ double power_of(double t) { return t > -1000.0 ? exp2(t) : 0.0; }
+// 2^t for t <= 0, to the hardware's 2^-23.
+__device__ __forceinline__ double power_of(double t) {
+    const double n = __builtin_rint(t);
+    return t > -1000.0 ? __builtin_ldexp((double)__builtin_amdgcn_exp2f((float)(t - n)), (int)n) : 0.0;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args) {
@@ -582,24 +585,31 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     }
     // The row's bins: thread j the j-th below that of its largest logit.
     const int top_bin = value_bin(top);
-    top_bins[tid] = piece_key ? value_bin(piece_top) : -0x40000000;
+    constexpr int kNoPiece = -0x4000000;
+    top_bins[tid] = piece_key ? value_bin(piece_top) : kNoPiece;
     if (tid < 4) sh.cuts[tid] = kBins;
     __syncthreads();
-    const u64 *bins = row_bins(args, scratch);
+    // (Lane e has where piece first + e's bins begin and its weight in the row's: a load and its use take a few
+    // instructions, and a bin above the piece's own is out of the descriptor's range: zero.)
+    const rsrc_t bins = make_rsrc(row_bins(args, scratch), (uint32_t)args.pieces * kBins * sizeof(u64));
     uint32_t count = 0;
     float bin_weight = 0.0f;
-    constexpr int kAtOnce = 32;
+    constexpr int kAtOnce = 16;  // (eight: 7.4 us for one row, 32: 6.4 and with four pieces 7.2 for 6.1)
     for (int first = 0; first < args.pieces; first += kAtOnce) {
-        u64 entry[kAtOnce];
+        const int piece = first + (tid & (kAtOnce - 1));
+        const int from = (piece < args.pieces ? top_bins[piece] : kNoPiece) - top_bin;
+        const uint32_t factor = __float_as_uint((float)factors[piece & (kThreads - 1)]);
+        u32x2 entry[kAtOnce];
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e)
+            entry[e] = __builtin_amdgcn_raw_buffer_load_b64(bins, (tid + __builtin_amdgcn_readlane(from, e)) * 8,
+                                                            (first + e < args.pieces ? first + e : 0) * kBins * 8, 0);
+        __builtin_amdgcn_sched_barrier(0);  // (every load out before the first is waited for)
 #pragma unroll
         for (int e = 0; e < kAtOnce; ++e) {
-            const int below = first + e < args.pieces ? tid - top_bin + top_bins[first + e] : -1;
-            entry[e] = below >= 0 ? bins[(size_t)(first + e) * kBins + below] : 0;
-        }
-#pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) {
-            count += (uint32_t)(entry[e] >> 32);
-            bin_weight = __builtin_fmaf(__uint_as_float((uint32_t)entry[e]), (float)factors[(first + e) & (kThreads - 1)], bin_weight);
+            count += entry[e].y;
+            bin_weight = __builtin_fmaf(__uint_as_float(entry[e].x),
+                                        __uint_as_float(__builtin_amdgcn_readlane(factor, e)), bin_weight);
         }
     }
     const u64 own_weight = (u64)bin_weight, run_count = block_scan(count, sh.scratch),
