@@ -19,7 +19,7 @@
 //           holds, is searched whole.
 // The launches over pieces hold nothing but what they stream, so that four workgroups share a CU. The rows' launches
 // are chains of a few dependent round trips, about 1.5 us of each the launch's own: one row of 248320 with every
-// filter takes 5.2 + 6.9 + 4.2 + 7.3 us, and 64 of them 18 + 7.7 + 7.8 + 8.1. What has to move is the logits, once:
+// filter takes 5.3 + 6.4 + 4.4 + 4.8 us, and 64 of them 18 + 7.0 + 7.5 + 5.5. What has to move is the logits, once:
 // 64 rows of 248320 fp32, 64 MB, 13 us at the rate of a large copy.
 #include "common.hpp"
 #include "launch.hpp"
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 
 // ---- settle -----------------------------------------------------------------------------------------
 //
-// Latency: the pieces' heads, then their bins (at most 32 in flight a thread), then three scans over the workgroup;
-// 6.9 us for one row of 31 pieces, 7.7 for 64. Loading the bins before the heads are known measured slower.
+// Latency: the pieces' heads, then their bins (sixteen pieces at a time, 4 KB each), then scans over the workgroup;
+// 6.4 us for one row of 31 pieces, 7.0 for 64. Loading the bins before the heads are known measured slower.
 
 // 2^t for t <= 0, to the hardware's 2^-23.
 __device__ __forceinline__ double power_of(double t) {
@@ -716,9 +716,9 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
 
 // ---- finish -----------------------------------------------------------------------------------------
 //
-// Latency: the plan, the list, one to three steps of the search, the strip; 7.3 us a row with a list of a few
-// elements, 9.3 with one of thousands. Up to 64 keys that share a digit are ranked by one wave, which saves the steps
-// below it.
+// Latency: the plan, the list, the cut, the strip. A list of up to 64 keys, of most rows with a peaked head, is
+// ranked at once (4.8 us a row; by digits 7.3); a longer one is searched by digits, and up to 64 keys that share one
+// are ranked by one wave, which saves the steps below it (9.5 us with lists of hundreds).
 
 // A step of the search for a cut among keys: how many there are with each digit of nine bits, and their weight.
 struct Digits {
