@@ -480,8 +480,9 @@ size_t splosh_sample_workspace_bytes(int64_t rows, int64_t vocab);
  * logprobs may be NULL. What decides between two entries is summed in 64-bit fixed point, 2^-40 of the
  * largest weight (less counts as none), the whole weight that p (without k) or, with T alone, u is a
  * share of in fp32 sums of sixteen and then so (to 2^-21). Nothing is added in an order that changes, so
- * the result depends on no other row and on no other call. vocab <= 2^21. The workspace need not be zeroed; its first 16 KiB stay as
- * they are, so one that other calls use serves here too, in stream order. Rows go 256 at a time. */
+ * the result depends on no other row and on no other call. vocab <= 2^21. The workspace need not be
+ * zeroed; its first 16 KiB stay as they are, so one that other calls use serves here too, in stream
+ * order. Rows go 256 at a time. */
 int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float *uniforms,
                   const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                   uint32_t *tokens, float *logprobs, void *workspace, size_t workspace_bytes, hipStream_t stream);

@@ -14,8 +14,8 @@
 //   settle  (rows)   greedy rows and those with the temperature alone are settled, from one strip more;
 //           for the others, the bins that the cut can be in;
 //   collect (pieces) each strip's weight above these bins, and the elements in them as a list;
-//   finish  (rows)   the cut, by a radix search in the list, the strip the draw falls into and the token
-//           in it. A row whose cut lies below its bins, or in bins of more elements than the list
+//   finish  (rows)   the cut, by ranking a short list or by a radix search in it, the strip the draw falls into and
+//           the token in it. A row whose cut lies below its bins, or in bins of more elements than the list
 //           holds, is searched whole.
 // The launches over pieces hold nothing but what they stream, so that four workgroups share a CU. The rows' launches
 // are chains of a few dependent round trips, about 1.5 us of each the launch's own: one row of 248320 with every
@@ -126,7 +126,8 @@ struct Weights {
 // NaN and -inf weigh `none`, which is 0 for all but the largest T. top finite.
 struct PieceWeights {
     float top, c_high, c_low, least, none;
-    __device__ __forceinline__ PieceWeights(float top, double c) : top(top), c_high((float)c), c_low((float)(c - (double)c_high)) {
+    __device__ __forceinline__ PieceWeights(float top, double c)
+        : top(top), c_high((float)c), c_low((float)(c - (double)c_high)) {
         // (Past it a weight is 0.)
         least = __builtin_fmaxf(-160.0f / c_high, -__FLT_MAX__);
         none = of(least);
@@ -639,7 +640,8 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
     if (tid == to) sh.weights[3] = run_count;
     __syncthreads();
     if (tid == 0) {
-        const bool fits = from < kBins && to < kBins && top_bin >= kLowestBin && top < __builtin_inff() && sh.weights[3] - sh.weights[2] <= kList;
+        const bool fits = from < kBins && to < kBins && top_bin >= kLowestBin && top < __builtin_inff() &&
+                          sh.weights[3] - sh.weights[2] <= kList;
         plan = {fits ? kCollect : kSearch, top_bin - from + 1, top_bin - to, top_key, total,
                 fits ? (uint32_t)sh.weights[2] : 0, 0, (uint32_t)valid, 0, rp.c, low};
     }
