@@ -16,7 +16,7 @@
 //   collect (pieces) each strip's weight above these bins, and the elements in them as a list;
 //   finish  (rows)   the cut, by ranking a short list or by a radix search in it, the strip the draw falls into and
 //           the token in it. A row whose cut lies below its bins, or in bins of more elements than the list
-//           holds, is searched whole (one workgroup, six passes: 2 ms for 248320 equal logits).
+//           holds, is searched whole (one workgroup, a pass for each nine bits of key: 2 ms for 248320 equal logits).
 // The launches over pieces hold nothing but what they stream, so that four workgroups share a CU. The rows' launches
 // are chains of a few dependent round trips, about 1.5 us of each the launch's own: one row of 248320 with every
 // filter takes 5.3 + 6.4 + 4.4 + 4.8 us, and 64 of them 18 + 7.0 + 7.5 + 5.5. What has to move is the logits, once:
