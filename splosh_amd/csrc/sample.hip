@@ -840,6 +840,7 @@ __device__ __forceinline__ u64 find_cuts(const Source &key_at, int n, const Keys
     for (int pass = 0; pass < 2; ++pass) {
         if (pass ? !by_share : !by_count) continue;
         cut = find_cut(d, key_at, n, keys, weigh, cut, pass ? 0 : (u64)rp.k, (double)rp.p * (double)weight, &weight, memory, sh);
+        __syncthreads();  // (every wave has read its results in sh, which the next one writes before a barrier of its own)
     }
     return cut;
 }

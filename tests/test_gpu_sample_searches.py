@@ -1,0 +1,34 @@
+"""splosh_sample where a row's cut is searched for in a long list or in the whole row, against its definition in
+64 bits."""
+import pytest
+import torch
+
+from sample_check import off_borders
+from test_gpu_sample import call, check_all, logits_of, params_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def rt():
+    from splosh_amd import runtime
+    return runtime
+
+
+@pytest.mark.parametrize("k,vocab,spread", [(65, 20011, 2.0), (150, 50021, 2.0), (600, 50021, 1.0), (600, 248320, 2.0),
+                                            (600, 9001, 0.0), (9000, 30011, 2.0)])
+def test_top_k_and_top_p_of_long_lists(rt, k, vocab, spread):
+    """Both cuts, one after the other, from more than 64 keys, or (equal logits, and more than 8192 keys between
+    the two cuts) from the whole row: the second search starts from the first one's results in every wave. The same
+    tokens and logprobs every time."""
+    rows = 48
+    logits = logits_of(rows, vocab, torch.float32, k, spread=spread)
+    u, params = params_of(rows, k, (1, 1, 1, 0))
+    params["top_k"] = k - torch.arange(rows, dtype=torch.int32) % 7
+    params = off_borders(logits.numpy(), params)
+    dev = logits.cuda()
+    first = call(rt, dev, u, params)
+    check_all(logits, u, params, *first)
+    for _ in range(8):
+        tokens, logprobs = call(rt, dev, u, params)
+        assert torch.equal(tokens, first[0]) and torch.equal(logprobs, first[1])
