@@ -493,11 +493,12 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 #pragma unroll
             for (int e = 0; e < kPer; ++e) sum += weigh(v[e]);
         }
-        if (weigh.none > 0.0f) {
+        if (weigh.none > 0.0f) {  // (added up without them: taken off again, their rounding would be left)
+            sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) sum -= v[e] > -__builtin_inff() ? 0.0f : weigh.none;
+            for (int e = 0; e < kPer; ++e) sum += v[e] > -__builtin_inff() ? weigh(v[e]) : 0.0f;
         }
-        weight = (u64)(__builtin_fmaxf(sum, 0.0f) * (float)((u64)1 << kWeightBits));
+        weight = (u64)(sum * (float)((u64)1 << kWeightBits));
         if (rp.k) valid = block_reduce(tid & 63 ? 0u : valid, SumOp(), scratch);
     }
     if (!rp.greedy) {

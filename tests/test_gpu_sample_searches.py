@@ -1,5 +1,8 @@
 """splosh_sample where a row's cut is searched for in a long list or in the whole row, against its definition in
 64 bits."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
@@ -32,3 +35,22 @@ def test_top_k_and_top_p_of_long_lists(rt, k, vocab, spread):
     for _ in range(8):
         tokens, logprobs = call(rt, dev, u, params)
         assert torch.equal(tokens, first[0]) and torch.equal(logprobs, first[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masked_stretches_weigh_nothing_at_the_largest_temperatures(rt, dtype):
+    """Stretches of -inf and NaN before the first entry that can be chosen, temperatures at which a weight far below
+    the largest is still a fraction of it: the draws of 0 and just above take the first entry that can be chosen."""
+    rows, vocab, first = 96, 9001, 3100
+    logits = logits_of(rows, vocab, torch.float32, 71).to(dtype)
+    logits[:, :first] = -math.inf
+    logits[:, 40:2000:3] = math.nan
+    logits[:, first + 20:] = -math.inf
+    u = torch.zeros(rows)
+    u[1::2] = 1e-9
+    params = {"temperature": torch.tensor(np.geomspace(4e36, 3.3e38, rows).astype(np.float32)),
+              "top_k": torch.zeros(rows, dtype=torch.int32), "top_p": torch.ones(rows), "min_p": torch.zeros(rows)}
+    out = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    tokens, logprobs = call(rt, logits, u, params, out=out)
+    assert tokens.tolist() == [first] * rows
+    check_all(logits, u, params, tokens, logprobs)
