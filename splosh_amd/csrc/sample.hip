@@ -853,8 +853,10 @@ __device__ __forceinline__ u64 rank_few(u64 key, u64 own, int n, u64 above, cons
                                         u64 *memory, Shared &sh) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     u64 count = 0, sum = 0;
-    for (int i = wave; i < n; i += kWaves)
-        if (lane_of(key, i) > key) ++count, sum += lane_of(own, i);
+    for (int i = wave; i < n; i += kWaves) {
+        const u64 other = lane_of(key, i), w = lane_of(own, i);  // (of lanes that the branch may leave out: before it)
+        if (other > key) ++count, sum += w;
+    }
     memory[threadIdx.x] = sum;
     memory[kThreads + threadIdx.x] = count;
     above = wave_scan(above, SumOp());

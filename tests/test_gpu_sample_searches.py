@@ -54,3 +54,26 @@ def test_masked_stretches_weigh_nothing_at_the_largest_temperatures(rt, dtype):
     tokens, logprobs = call(rt, logits, u, params, out=out)
     assert tokens.tolist() == [first] * rows
     check_all(logits, u, params, tokens, logprobs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_length_of_a_short_list(rt, dtype):
+    """Lists of 1 to 64 keys, ranked at once: k of them kept, and of these a share that ends at each place in turn,
+    between the sums before and after it."""
+    rows, vocab = 64, 9001
+    gen = torch.Generator().manual_seed(73)
+    logits = (-40.0 - torch.rand(rows, vocab, generator=gen)).to(dtype)
+    steps = (-0.0625 * torch.arange(rows)).to(dtype)  # (weights 6% apart)
+    for r in range(rows):
+        logits[r, torch.randperm(vocab, generator=gen)[:rows]] = steps
+    w = torch.exp(steps.double())
+    for shift in (0, 5, 40):
+        k = torch.arange(1, rows + 1)
+        ends = (k * 7 + shift) % k  # place of the last that the share keeps
+        run = torch.stack([w.cumsum(0)[e] for e in ends])
+        share = (run - 0.5 * w[ends]) / w.cumsum(0)[k - 1]
+        u = torch.rand(rows, generator=gen)
+        params = {"temperature": torch.ones(rows), "top_k": k.int(), "top_p": share.float(), "min_p": torch.zeros(rows)}
+        params["top_k"][::3] += 2  # (the cut past the share, and where the list is longer than k)
+        params = off_borders(logits.float().numpy(), params)
+        check_all(logits, u, params, *call(rt, logits, u, params), f"shift {shift}")
