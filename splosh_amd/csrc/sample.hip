@@ -40,11 +40,11 @@ constexpr int kBinShift = 49, kBinBits = 31;
 // Rows whose largest logit is in a bin below this one are searched whole: 512 bins further down NaN and -inf
 // (past bin -8192) would be among those that are counted.
 constexpr int kLowestBin = -7000;
-constexpr int kMaxStrips = kThreads * kWaves;
+constexpr int kMaxStrips = (int)(kSampleMaxVocab / kStrip);
 constexpr int kList = 8192;                  // elements of a row's list
 constexpr int kBatchRows = 256;              // rows of one launch
 
-static_assert((int64_t)kPiece * kThreads >= kSampleMaxVocab + 7, "a row's pieces are one a thread");
+static_assert((int64_t)kPiece * kThreads >= kSampleMaxVocab && kSampleMaxVocab % kPiece == 0, "a row's pieces are one a thread");
 
 typedef unsigned long long u64;
 
@@ -300,14 +300,10 @@ __device__ __forceinline__ u64 draw_of(float u, u64 total) {
     return target < total ? target : total - 1;
 }
 
-// The pieces of a row begin at the 16-byte boundary at or before it, `lead` elements early, so that their 16-byte
-// parts are aligned whatever the row's alignment.
-template <typename T>
-__device__ __forceinline__ int row_lead(const T *row) {
-    return (int)((uintptr_t)row % 16 / sizeof(T));
-}
-// A thread's sixteen logits of the piece at `base`, -inf outside the row; their indexes are base + index_of(e), a
-// wave's a strip. (Whole pieces without a branch, so that every load is out before the first is waited for.)
+// A thread's sixteen logits of the piece at `base`, -inf past the row's end; their indexes are base + index_of(e), a
+// wave's a strip. Pieces are counted from the row's first element whatever its alignment, so that which elements
+// share a sum does not depend on where the row lies: the 16-byte loads need no more than an element's alignment.
+// (Whole pieces without a branch, so that every load is out before the first is waited for.)
 template <typename T>
 __device__ __forceinline__ int index_of(int e) {
     constexpr int kRun = 16 / (int)sizeof(T);
@@ -317,17 +313,17 @@ template <typename T>
 __device__ __forceinline__ void load_piece(const T *row, int base, int vocab, float (&v)[kPer]) {
     constexpr int kRun = 16 / (int)sizeof(T);
     u32x4 w[kPer / kRun];
-    const bool whole = base >= 0 && base + kPiece <= vocab;
+    const bool whole = base + kPiece <= vocab;
     if (whole) {
 #pragma unroll
-        for (int e = 0; e < kPer; e += kRun) w[e / kRun] = *(const u32x4 *)(row + base + index_of<T>(e));
+        for (int e = 0; e < kPer; e += kRun) __builtin_memcpy(&w[e / kRun], row + base + index_of<T>(e), 16);
     } else {
         constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
         for (int e = 0; e < kPer; e += kRun) {
             const int i = base + index_of<T>(e);
             w[e / kRun] = u32x4{kNone, kNone, kNone, kNone};
-            if (i >= 0 && i + kRun <= vocab) w[e / kRun] = *(const u32x4 *)(row + i);
+            if (i + kRun <= vocab) __builtin_memcpy(&w[e / kRun], row + i, 16);
         }
     }
 #pragma unroll
@@ -335,14 +331,14 @@ __device__ __forceinline__ void load_piece(const T *row, int base, int vocab, fl
         const uint32_t word = w[e / kRun][e % kRun * sizeof(T) / 4];
         v[e] = sizeof(T) == 4 ? __uint_as_float(word) : bf16_bits_to_f32(e & 1 ? word >> 16 : word & 0xffffu);
     }
-    if (!whole) {  // the parts that the row begins or ends in
+    if (!whole) {  // the part that the row ends in
 #pragma unroll
         for (int e = 0; e < kPer; e += kRun) {
             const int i = base + index_of<T>(e);
-            if ((i < 0 && i + kRun > 0) || (i < vocab && i + kRun > vocab)) {
+            if (i < vocab && i + kRun > vocab) {
 #pragma unroll
                 for (int j = 0; j < kRun; ++j)
-                    if (i + j >= 0 && i + j < vocab) v[e + j] = logit_of(row[i + j]);
+                    if (i + j < vocab) v[e + j] = logit_of(row[i + j]);
             }
         }
     }
@@ -392,13 +388,13 @@ template <typename T>
 __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const T *row, int strip, float top, double c,
                                        u64 cut, double low, double fraction, double scale, Shared &sh) {
     constexpr int kEach = kStrip / kThreads;
-    const int first = strip * kStrip - row_lead(row) + (int)threadIdx.x * kEach;
+    const int first = strip * kStrip + (int)threadIdx.x * kEach;
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
     float v[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
-        v[e] = first + e >= 0 && first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
+        v[e] = first + e < args.vocab ? logit_of(row[first + e]) : -__builtin_inff();
     u64 w[kEach], run = 0, total = 0;
     for (int pass = 0; pass < 2 && total == 0; ++pass) {  // (again, by number, where what is left is less than a unit each)
         u64 sum = 0;
@@ -439,7 +435,7 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
     const int tid = threadIdx.x, piece = blockIdx.x;
     const int64_t r = blockIdx.y;
     const T *logits = (const T *)args.logits + r * args.ld;
-    const int base = piece * kPiece - row_lead(logits);
+    const int base = piece * kPiece;
     float v[kPer];
     load_piece(logits, base, args.vocab, v);
     const RowParams rp = row_params(args, r);
@@ -672,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs arg
     if (strip_key && value_bin(strip_top) >= low_bin && (listing || weighs(strip_top, top, c, low))) {
         const Weights weigh(top, c);
         const T *logits = (const T *)args.logits + r * args.ld;
-        const int base = piece * kPiece - row_lead(logits);
+        const int base = piece * kPiece;
         float v[kPer];
         load_piece(logits, base, args.vocab, v);
         uint32_t listed = 0;
@@ -904,7 +900,6 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     const double c = plan.c, low = plan.low;
     const Weights weigh(top, c);
     const OrderKeys<T> keys(args.vocab);
-    const int lead = row_lead(row);
     u64 cut = 1;
     const bool listed = plan.state == kCollect;
     const int n = listed ? plan.listed < (uint32_t)kList ? (int)plan.listed : kList : 0;
@@ -918,7 +913,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
             const float v = keys.logit(early);
             const u64 own = any ? weigh(v) : 0;
             cut = rank_few(any ? early : 0, own, n, above, plan, rp, memory, sh);
-            if (tid < n && early >= cut && weighs(v, top, c, low)) atomicAdd(&extra[(keys.index(early) + lead) / kStrip], own);
+            if (tid < n && early >= cut && weighs(v, top, c, low)) atomicAdd(&extra[keys.index(early) / kStrip], own);
         }
     } else if (n) {
         const u64 *from = row_list(args, scratch);
@@ -941,7 +936,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
     for (int i = tid; i < (few ? 0 : listed ? n : args.vocab); i += kThreads) {
         const u64 key = listed ? list[i] : keys(logit_of(row[i]), i);
         const float v = keys.logit(key);
-        if (key >= cut && weighs(v, top, c, low)) atomicAdd(&extra[(keys.index(key) + lead) / kStrip], weigh(v));
+        if (key >= cut && weighs(v, top, c, low)) atomicAdd(&extra[keys.index(key) / kStrip], weigh(v));
     }
     __syncthreads();
     const u64 total = choose_strip(
@@ -951,8 +946,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs args
 
 // ---- host -------------------------------------------------------------------------------------------
 
-// (With the elements that a piece may begin before its row.)
-static int64_t pieces_of(int64_t vocab) { return (vocab + 7 + kPiece - 1) / kPiece; }
+static int64_t pieces_of(int64_t vocab) { return (vocab + kPiece - 1) / kPiece; }
 static size_t row_bytes(int64_t vocab) {
     const int64_t pieces = pieces_of(vocab);
     const size_t bytes = sizeof(RowPlan) + pieces * (2 * sizeof(u64) + kWaves * sizeof(Strip) + kBins * sizeof(u64)) +

@@ -77,3 +77,22 @@ def test_every_length_of_a_short_list(rt, dtype):
         params["top_k"][::3] += 2  # (the cut past the share, and where the list is longer than k)
         params = off_borders(logits.float().numpy(), params)
         check_all(logits, u, params, *call(rt, logits, u, params), f"shift {shift}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [777, 12345, 40009])
+def test_the_same_row_at_every_alignment(rt, vocab, dtype):
+    """A row's token and the bits of its logprob do not depend on where the row begins."""
+    rows = 300
+    logits = logits_of(rows, vocab, torch.float32, 77, head=20, spread=3.0).to(dtype)
+    for on in ((1, 0, 0, 0), (1, 0, 1, 0), (1, 1, 1, 0), (1, 0, 0, 1), None):
+        u, params = params_of(rows, 78, on)
+        want = call(rt, logits, u, params)
+        places = 16 // dtype.itemsize
+        for at in range(places):
+            # (A stride of whole 16 bytes: every row begins at the same place in its 16 bytes.)
+            wide = torch.full((rows, (vocab + 2 * places) // places * places), 1e4, dtype=dtype, device="cuda")
+            wide[:, at : at + vocab] = logits.cuda()
+            got = call(rt, wide[:, at : at + vocab], u, params)
+            off = (got[0] != want[0]) | (got[1].view(torch.int32) != want[1].view(torch.int32))
+            assert int(off.sum()) == 0, f"{on} at {at}"
