@@ -256,8 +256,9 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
 // ---- out += b t -----------------------------------------------------------------------------------
 //
 // A workgroup: one adapter's rows of a chunk, a run of tiles of 256 outputs of one projection, 64 outputs
-// a wave. t's slices are summed and laid down in LDS as MFMA operands, in two bf16 pieces for a bf16
-// output and three for an fp32 one (a piece takes eight more bits, so the products keep 16 or 24 of t's).
+// a wave. t's slices are summed and laid down in LDS as MFMA operands, in three bf16 pieces of eight bits each, so
+// that the products keep all of t's 24. (Two pieces are enough for most bf16 outputs and save 0.3 of 41.4 us for 2048 rows,
+// N17408, rank 16; but one value in a thousand is then rounded the other way.)
 // b's rows are the MFMA's rows and stay in registers while the adapter's rows go by, sixteen at a time. Their
 // sums pass through LDS, so that a wave reads and writes runs of 64 neighbouring outputs of a row: with
 // the MFMA's own layout, neighbouring lanes hold different rows, and four times the cache lookups.
@@ -265,12 +266,12 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
 // Bound by out, read and written: 2048 rows, N17408, bf16: 160 MB in 34 us (4.7 TB/s, a large copy's rate); 64 rows,
 // 2 x 17408, fp32, rank 16: 27 MB in 8.4 us.
 
+constexpr int kPieces = 3;
 constexpr int kUpSumStride = 68;  // floats of a row of sums in LDS: 64 and a step of four banks
 
 // The rows of t of a workgroup's blocks of sixteen (block j of its own: from the adapter's row 16 (share + j
 // shares) on), summed over the slices, as operands in LDS: [piece][panel of 32 ranks][block][lane] x 16 bytes.
 // Four ranks of one row a thread.
-template <int PIECES>
 __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWeight &g, int mine, int count,
                                         int blocks, int share, int64_t base, int rank, u32x2 *pieces) {
     constexpr int kAtOnce = 8;
@@ -293,12 +294,12 @@ __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWe
                     if (s + e < args.slices) v += part[e];
             }
         }
-        float piece[PIECES][4];
+        float piece[kPieces][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float rest = r + e < rank ? v[e] : 0.0f;
 #pragma unroll
-            for (int c = 0; c < PIECES; ++c) {
+            for (int c = 0; c < kPieces; ++c) {
                 piece[c][e] = rest;
                 const float top = bf16_bits_to_f32(f32_to_bf16(rest));
                 rest = __builtin_fabsf(top) < __builtin_inff() ? rest - top : 0.0f;
@@ -306,7 +307,7 @@ __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWe
         }
         const int at = ((r >> 5) * blocks + (i >> 4)) * 64 + ((r >> 3) & 3) * 16 + (i & 15);
 #pragma unroll
-        for (int c = 0; c < PIECES; ++c)
+        for (int c = 0; c < kPieces; ++c)
             pieces[(c * panels * blocks * 64 + at) * 2 + ((r >> 2) & 1)] =
                 u32x2{f32x2_to_bf16x2(piece[c][0], piece[c][1]), f32x2_to_bf16x2(piece[c][2], piece[c][3])};
     }
@@ -316,7 +317,7 @@ __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWe
 // 16: 34.2 us held, 38.6 read again; holding 64 ranks measured level with reading them again).
 template <int NP, typename OUT, bool FAST>
 __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(AdapterArgs args) {
-    constexpr int kPieces = sizeof(OUT) == 4 ? 3 : 2, kLoads = sizeof(OUT), kPer = 16 / sizeof(OUT), kHeld = NP ? NP : 1;
+    constexpr int kLoads = sizeof(OUT), kPer = 16 / sizeof(OUT), kHeld = NP ? NP : 1;
     extern __shared__ u32x4 pieces[];
     __shared__ float sums[4][16 * kUpSumStride];
     const int share = blockIdx.z % args.shares, z = blockIdx.z / args.shares;
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(Adapte
             for (int p = 0; p < NP; ++p) load_b(p, bs[p]);
             if (tile == 0) {
                 __syncthreads();  // (the operands before them have been read)
-                stage_t<kPieces>(args, g, mine, count, blocks, share, base, rank, (u32x2 *)pieces);
+                stage_t(args, g, mine, count, blocks, share, base, rank, (u32x2 *)pieces);
                 __syncthreads();
             }
 #pragma unroll
@@ -519,9 +520,9 @@ static void launch_down(const AdapterArgs &args, int panels, dim3 grid, hipStrea
     else hipLaunchKernelGGL((adapter_down_kernel<RB, 2, FAST>), grid, dim3(64 * kDownWaves), 0, stream, args);
 }
 
-// LDS of the operands: three pieces (of an fp32 output) of whole panels of ranks for a chunk's rows; past the
-// default limit of 64 KB with what the kernel has of its own, the limit is raised once.
-constexpr int kUpMaxLds = 3 * (SPLOSH_MAX_RANK / 32) * (kChunk / 16) * 1024;
+// LDS of the operands: their pieces of whole panels of ranks for a chunk's rows; past the default limit of 64 KB with
+// what the kernel has of its own, the limit is raised once.
+constexpr int kUpMaxLds = kPieces * (SPLOSH_MAX_RANK / 32) * (kChunk / 16) * 1024;
 
 template <int NP, typename OUT, bool FAST>
 static hipError_t launch_up(const AdapterArgs &args, int lds, dim3 grid, hipStream_t stream) {
@@ -600,7 +601,7 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     args.turns = plan_turns(parts, (int64_t)up_x * chunks * group * args.shares);
     const dim3 up(up_x, chunks, (unsigned)(group * args.turns * args.shares));
     const int up_panels = (int)(most_rank + 31) / 32, blocks = rows < kChunk ? (int)(rows + 15) / 16 : kChunk / 16;
-    const int lds = (out_dtype == SPLOSH_F32 ? 3 : 2) * up_panels * blocks * 1024;
+    const int lds = kPieces * up_panels * ((blocks + args.shares - 1) / args.shares) * 1024;
     return out_dtype == SPLOSH_F32 ? launch_up<float>(args, up_panels, up_fast, lds, up, stream)
                                    : launch_up<uint16_t>(args, up_panels, up_fast, lds, up, stream);
 }
