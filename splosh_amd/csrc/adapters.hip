@@ -300,8 +300,9 @@ __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWe
             float rest = r + e < rank ? v[e] : 0.0f;
 #pragma unroll
             for (int c = 0; c < kPieces; ++c) {
-                piece[c][e] = rest;
-                const float top = bf16_bits_to_f32(f32_to_bf16(rest));
+                // (Cut off and not rounded: a finite value's piece is finite. Sums' NaNs are quiet ones, which stay NaN.)
+                const float top = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+                piece[c][e] = top;
                 rest = __builtin_fabsf(top) < __builtin_inff() ? rest - top : 0.0f;
             }
         }

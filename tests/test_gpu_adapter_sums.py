@@ -35,3 +35,16 @@ def test_every_bit_reaches_the_output(rt, sign, rows, rank, inner, outputs, dtyp
     got = add(rt, x, a, b, torch.full((rows, outputs), sign, dtype=dtype))
     want = 2.0 + 2.0 ** -6 if dtype == torch.bfloat16 else 2.0 + 2.0 ** -7 + 2.0 ** -19
     assert (got.float() == sign * want).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_products_at_the_end_of_fp32(rt, sign, dtype):
+    """t = 2^127 (1 + 0.99609375 + 2^-11), finite but nearer to 2^128 than to any bf16 number: 2^-126 of it is 4 - 2^-7 + 2^-10."""
+    x, a, b = torch.zeros(3, 8), torch.zeros(4, 8), torch.zeros(16, 4)
+    x[:, :3] = 2.0 ** 64
+    a[0, 0], a[0, 1], a[0, 2] = sign * 2.0 ** 63, sign * 0.99609375 * 2.0 ** 63, sign * 2.0 ** 52
+    b[:, 0] = 2.0 ** -126
+    got = add(rt, x, a, b, torch.zeros(3, 16, dtype=dtype))
+    want = torch.tensor(2.0 * (1.0 + 0.99609375 + 2.0 ** -11)).to(dtype)
+    assert (got == sign * want).all()
