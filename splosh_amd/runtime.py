@@ -646,6 +646,15 @@ def _matrix(t, rows, columns, index, name):
     return t.data_ptr()
 
 
+def _given_workspace(workspace, index):
+    """(address, bytes) of a caller's workspace on device `index`; one dense block, all of whose bytes are its own."""
+    if workspace.get_device() != index:
+        raise SploshError(13, f"workspace is on {workspace.device}, the operands on cuda:{index}")
+    if not workspace.is_contiguous():
+        raise SploshError(13, "workspace must be contiguous")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _row_stride(t):
     """The row stride of a checked operand (a single row's can be anything)."""
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
@@ -740,8 +749,7 @@ def add_adapters_group(outs, a, adapters, slots, rows=None, stream=None, workspa
                                         device=a.device)
         st = lib.splosh_adapters_add_group(cs, n, x, _row_stride(a), (ctypes.c_void_p * n)(*ptrs),
                                            (ctypes.c_int64 * n)(*[_row_stride(o) for o in outs]), code, slot_ptr, rows,
-                                           workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                           _raw_stream(stream, index))
+                                           *_given_workspace(workspace, index), _raw_stream(stream, index))
     if st:
         _lib.check(st)
     return outs
@@ -755,8 +763,8 @@ def add_adapters(out, a, adapters, slots, rows=None, stream=None, workspace=None
     ptr, slot_ptr = _added(out, adapters, rows, index), _vector(slots, rows, torch.int32, index, "slots")
     with _launch(index):
         st = _lib.lib().splosh_adapters_add(ctypes.byref(adapters._c), x, _row_stride(a), ptr, _row_stride(out),
-                                            _dtype_code(out.dtype), slot_ptr, rows, workspace.data_ptr(),
-                                            workspace.numel() * workspace.element_size(), _raw_stream(stream, index))
+                                            _dtype_code(out.dtype), slot_ptr, rows, *_given_workspace(workspace, index),
+                                            _raw_stream(stream, index))
     if st:
         _lib.check(st)
     return out
@@ -794,7 +802,7 @@ def sample(logits, uniforms=None, temperature=None, top_k=None, top_p=None, min_
                                             device=logits.device)
         st = lib.splosh_sample(ptr, _row_stride(logits), code, rows, vocab, *params,
                                _vector(out, rows, torch.int32, index, "out"), _vector(logprobs, rows, f32, index, "logprobs"),
-                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _raw_stream(stream, index))
+                               *_given_workspace(workspace, index), _raw_stream(stream, index))
     if st:
         _lib.check(st)
     return out, logprobs

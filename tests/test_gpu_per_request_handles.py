@@ -1,0 +1,31 @@
+"""The per-request operators' handles and workspaces on the device: what is refused leaves every output as it was."""
+import pytest
+import torch
+
+from test_gpu_adapters import host_case, on_gpu, slots_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def rt():
+    from splosh_amd import runtime
+    return runtime
+
+
+def test_workspaces_on_the_host(rt):
+    from splosh_amd._lib import SploshError
+    x, adapters, out = host_case(4, 64, 48, 8, 3, torch.float32, 1)
+    w, xd, od, slots = on_gpu(rt, adapters), x.cuda(), out.cuda(), slots_of(4, 3, 1).cuda()
+    logits = torch.randn(4, 100).cuda()
+    tokens = torch.full((4,), 7, dtype=torch.int32, device="cuda")
+    far = torch.zeros(1 << 22, dtype=torch.uint8)
+    one = torch.zeros(1, dtype=torch.uint8, device="cuda").expand(1 << 22)
+    for ws in (far, one):
+        for call in (lambda: rt.add_adapters(od, xd, w, slots, workspace=ws),
+                     lambda: rt.add_adapters_group([od], xd, [w], slots, workspace=ws),
+                     lambda: rt.sample(logits, out=tokens, workspace=ws)):
+            with pytest.raises(SploshError) as e:
+                call()
+            assert e.value.case == "unsupported"
+    assert torch.equal(od.cpu(), out) and (tokens == 7).all()
