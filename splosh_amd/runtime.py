@@ -660,13 +660,14 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-@dataclass
+@dataclass(frozen=True)
 class Adapters:
     """The low-rank adapters of one projection (splosh_adapters): ``a`` bf16 [count, max_rank, inner]
     and ``b`` bf16 [count, rows, max_rank] (last dimensions contiguous), ``scales`` fp32 [count]
     (None: 1) and ``ranks`` int32 [count] (None: max_rank for all). Slot s adds
     scales[s] * b[s][:, :r] @ (a[s][:r] @ x), r = ranks[s]. The tensors are taken as they are: adapters
-    are exchanged by writing into them."""
+    are exchanged by writing into them, and other tensors need a handle of their own (this one keeps the
+    addresses that it was made with, so its fields cannot be assigned)."""
 
     a: torch.Tensor
     b: torch.Tensor
@@ -681,20 +682,21 @@ class Adapters:
             raise GemmQ4Error(1, "adapters are a [count, max_rank, inner] and b [count, rows, max_rank]")
         if (a.stride(2) != 1 and a.shape[2] > 1) or (b.stride(2) != 1 and b.shape[2] > 1):
             raise SploshError(13, "adapter rows must be contiguous")
-        self.index = _index(a, "a")
-        if b.get_device() != self.index:
+        index = _index(a, "a")
+        if b.get_device() != index:
             raise SploshError(13, f"b is on {b.device}, a on {a.device}")
-        self.count, self.max_rank, self.inner = a.shape
-        self.rows = b.shape[1]
-        scales = _vector(self.scales, self.count, torch.float32, self.index, "scales")
-        ranks = _vector(self.ranks, self.count, torch.int32, self.index, "ranks")
+        count, max_rank, inner = a.shape
+        rows = b.shape[1]
+        scales = _vector(self.scales, count, torch.float32, index, "scales")
+        ranks = _vector(self.ranks, count, torch.int32, index, "ranks")
 
         def stride(t, dim, least):  # (of a dimension of one, anything)
             return t.stride(dim) if t.shape[dim] > 1 else max(t.stride(dim), least)
 
-        self._c = _lib.Adapters(a.data_ptr(), b.data_ptr(), ranks, scales, self.count, self.max_rank, self.rows,
-                                self.inner, stride(a, 0, 0), stride(a, 1, self.inner), stride(b, 0, 0),
-                                stride(b, 1, self.max_rank))
+        c = _lib.Adapters(a.data_ptr(), b.data_ptr(), ranks, scales, count, max_rank, rows, inner, stride(a, 0, 0),
+                          stride(a, 1, inner), stride(b, 0, 0), stride(b, 1, max_rank))
+        for name, value in dict(index=index, count=count, max_rank=max_rank, inner=inner, rows=rows, _c=c).items():
+            object.__setattr__(self, name, value)
 
     def c(self):
         return self._c
@@ -703,7 +705,7 @@ class Adapters:
 def adapters_workspace_bytes(adapters, rows):
     """splosh_adapters_workspace_bytes: the scratch a call on these projections' adapters needs."""
     adapters = [adapters] if isinstance(adapters, Adapters) else list(adapters)
-    cs = (_lib.Adapters * len(adapters))(*[w._c for w in adapters])
+    cs = (_lib.Adapters * len(adapters))(*[w.c() for w in adapters])
     return _lib.lib().splosh_adapters_workspace_bytes(cs, len(adapters), rows)
 
 
@@ -741,7 +743,7 @@ def add_adapters_group(outs, a, adapters, slots, rows=None, stream=None, workspa
     ptrs = [_added(o, w, rows, index) for w, o in zip(adapters, outs)]
     slot_ptr = _vector(slots, rows, torch.int32, index, "slots")
     lib, code = _lib.lib(), _dtype_code(dtype)
-    cs = (_lib.Adapters * n)(*[w._c for w in adapters])
+    cs = (_lib.Adapters * n)(*[w.c() for w in adapters])
     with _launch(index):
         if workspace is None:
             with _allocating(stream):
@@ -762,7 +764,7 @@ def add_adapters(out, a, adapters, slots, rows=None, stream=None, workspace=None
     rows, index, x = _adapted(a, adapters, rows)
     ptr, slot_ptr = _added(out, adapters, rows, index), _vector(slots, rows, torch.int32, index, "slots")
     with _launch(index):
-        st = _lib.lib().splosh_adapters_add(ctypes.byref(adapters._c), x, _row_stride(a), ptr, _row_stride(out),
+        st = _lib.lib().splosh_adapters_add(ctypes.byref(adapters.c()), x, _row_stride(a), ptr, _row_stride(out),
                                             _dtype_code(out.dtype), slot_ptr, rows, *_given_workspace(workspace, index),
                                             _raw_stream(stream, index))
     if st:

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from adapter_check import check
 from test_gpu_adapters import host_case, on_gpu, slots_of
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +30,19 @@ def test_workspaces_on_the_host(rt):
                 call()
             assert e.value.case == "unsupported"
     assert torch.equal(od.cpu(), out) and (tokens == 7).all()
+
+
+def test_adapters_keep_their_tensors(rt):
+    """A handle holds the addresses of the tensors that it was made from: none can be put in their place, and
+    writing into them is seen by the next call."""
+    x, adapters, out = host_case(6, 64, 48, 8, 3, torch.float32, 2)
+    w, slots = on_gpu(rt, adapters), slots_of(6, 3, 2)
+    for name in ("a", "b", "scales", "ranks"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name))
+    other = host_case(6, 64, 48, 8, 3, torch.float32, 3)[1]
+    for mine, new in zip((w.a, w.b, w.scales), other):
+        mine.copy_(new)
+    got = out.cuda()
+    rt.add_adapters(got, x.cuda(), w, slots.cuda())
+    check(got, out, x, other, slots)
