@@ -652,7 +652,7 @@ def _given_workspace(workspace, index):
         raise SploshError(13, f"workspace is on {workspace.device}, the operands on cuda:{index}")
     if not workspace.is_contiguous():
         raise SploshError(13, "workspace must be contiguous")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def _row_stride(t):
@@ -743,7 +743,7 @@ def add_adapters_group(outs, a, adapters, slots, rows=None, stream=None, workspa
     ptrs = [_added(o, w, rows, index) for w, o in zip(adapters, outs)]
     slot_ptr = _vector(slots, rows, torch.int32, index, "slots")
     lib, code = _lib.lib(), _dtype_code(dtype)
-    cs = (_lib.Adapters * n)(*[w.c() for w in adapters])
+    cs = (_lib.Adapters * n)(*[w._c for w in adapters])
     with _launch(index):
         if workspace is None:
             with _allocating(stream):
@@ -764,7 +764,7 @@ def add_adapters(out, a, adapters, slots, rows=None, stream=None, workspace=None
     rows, index, x = _adapted(a, adapters, rows)
     ptr, slot_ptr = _added(out, adapters, rows, index), _vector(slots, rows, torch.int32, index, "slots")
     with _launch(index):
-        st = _lib.lib().splosh_adapters_add(ctypes.byref(adapters.c()), x, _row_stride(a), ptr, _row_stride(out),
+        st = _lib.lib().splosh_adapters_add(ctypes.byref(adapters._c), x, _row_stride(a), ptr, _row_stride(out),
                                             _dtype_code(out.dtype), slot_ptr, rows, *_given_workspace(workspace, index),
                                             _raw_stream(stream, index))
     if st:
