@@ -48,3 +48,17 @@ def test_products_at_the_end_of_fp32(rt, sign, dtype):
     got = add(rt, x, a, b, torch.zeros(3, 16, dtype=dtype))
     want = torch.tensor(2.0 * (1.0 + 0.99609375 + 2.0 ** -11)).to(dtype)
     assert (got == sign * want).all()
+
+
+def test_the_most_rows(rt):
+    """2^21 rows, the entry points' limit: 32768 chunks."""
+    from adapter_check import check
+    from test_gpu_adapters import host_case, slots_of
+    rows = 1 << 21
+    x, adapters, out = host_case(rows, 8, 16, 3, 3, torch.bfloat16, 43)
+    slots = slots_of(rows, 3, 43)
+    got = rt.add_adapters(out.cuda(), x.cuda(), on_gpu(rt, adapters), slots.cuda())
+    pick = list(range(0, 200)) + list(range(rows // 2 - 100, rows // 2 + 100)) + list(range(rows - 200, rows))
+    check(got[pick], out[pick], x[pick], adapters, slots[pick])
+    idle = (slots < 0) | (slots >= 3)
+    assert torch.equal(got.cpu()[idle].view(torch.int16), out[idle].view(torch.int16))

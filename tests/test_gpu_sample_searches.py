@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from sample_check import off_borders
-from test_gpu_sample import call, check_all, logits_of, params_of
+from test_gpu_sample import call, check_all, logits_of, params_of, run
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,26 @@ def test_the_same_row_at_every_alignment(rt, vocab, dtype):
             got = call(rt, wide[:, at : at + vocab], u, params)
             off = (got[0] != want[0]) | (got[1].view(torch.int32) != want[1].view(torch.int32))
             assert int(off.sum()) == 0, f"{on} at {at}"
+
+
+@pytest.mark.parametrize("offset", [-300.0, -20.0, 15.0, 30.0, 100.0, 4000.0])
+def test_logits_about_another_value(rt, offset):
+    """A common offset: the bins about it are wider, the lists longer, and from some offset on rows are searched whole."""
+    rows, vocab = 8, 100003
+    logits = logits_of(rows, vocab, torch.float32, 79) + offset
+    for on in ((1, 0, 1, 0), (1, 1, 1, 0), (1, 0, 1, 1)):
+        u, params = params_of(rows, 80, on)
+        run(rt, logits, u, params, f"{offset} {on}")
+
+
+@pytest.mark.parametrize("head", [0, 40])
+@pytest.mark.parametrize("top_p", [0.9995, 0.9999, 0.99999, 1.0 - 2.0 ** -24])
+def test_shares_next_to_the_whole(rt, top_p, head):
+    """Shares that the bins cannot tell from the whole weight."""
+    rows, vocab = 8, 60013
+    logits = logits_of(rows, vocab, torch.float32, 81, head)
+    u, params = params_of(rows, 82, (1, 0, 1, 0))
+    params["top_p"] = torch.full((rows,), top_p)
+    run(rt, logits, u, params)
+    params["top_k"] = torch.full((rows,), 20000, dtype=torch.int32)
+    run(rt, logits, u, params)
