@@ -411,14 +411,20 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
     u64 target = (u64)(fraction * (double)total), found = 0;
     target = target < total ? target : total - 1;
     int at = 0;
+    float logit = top;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-        if (run <= target && target < run + w[e]) at = e, found = w[e];
+        if (run <= target && target < run + w[e]) at = e, found = w[e], logit = v[e];
         run += w[e];
     }
     if (found) {
         args.tokens[r] = (uint32_t)(first + at);
-        if (args.logprobs) args.logprobs[r] = (float)log((double)found * scale);
+        // (Below 2^24 units the weight's own unit would be seen in its logarithm: the exponent as it is.)
+        constexpr double kLn2 = 0.693147180559945309417;
+        const bool small = found >> 24 == 0 && logit != top;
+        const double weight = small ? (double)((u64)1 << kWeightBits) : (double)found;
+        const double power = small ? ((double)logit - (double)top) * c * kLn2 : 0.0;
+        if (args.logprobs) args.logprobs[r] = (float)(power + log(weight * scale));
     }
 }
 

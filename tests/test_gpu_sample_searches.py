@@ -119,3 +119,22 @@ def test_shares_next_to_the_whole(rt, top_p, head):
     run(rt, logits, u, params)
     params["top_k"] = torch.full((rows,), 20000, dtype=torch.int32)
     run(rt, logits, u, params)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("far", [-16.0, -22.0, -25.0])
+def test_logprobs_of_unlikely_tokens(rt, far, dtype):
+    """One large logit and 100000 of about e^far of its weight: a draw from among those has its own logprob, to fp32's
+    last places of it and 2^-20 for the whole weight."""
+    rows, vocab = 16, 100003
+    gen = torch.Generator().manual_seed(83)
+    logits = (far + 0.5 * torch.rand(rows, vocab, generator=gen)).to(dtype)
+    logits[:, 0] = 0.0
+    u = torch.full((rows,), 1.0 - 2.0 ** -22)
+    for params in ({}, {"min_p": torch.full((rows,), 2.0 ** -39)}, {"top_k": torch.full((rows,), 99000, dtype=torch.int32)}):
+        tokens, logprobs = call(rt, logits, u, params)
+        z = torch.gather(logits.double(), 1, tokens.long()[:, None])[:, 0]
+        kept = logits.double().exp() if "top_k" not in params else torch.topk(logits.double(), 99000).values.exp()
+        want = z - kept.sum(1).log()
+        assert (tokens > 0).all() and (z <= far + 0.5).all()
+        assert ((logprobs.double() - want).abs() <= 2.0 ** -20 + 2.0 ** -23 * want.abs()).all(), (logprobs.double() - want).abs().max()
