@@ -6,18 +6,19 @@
 // Both walk the rows in chunks of 64. A chunk's rows are taken adapter by adapter: the lanes of a wave
 // hold the chunk's slots, a ballot gives the rows of one adapter, and these meet the adapter's matrix as
 // the columns of v_mfma_f32_16x16x32_bf16, whatever places they have in the batch. So no sorted order of
-// the rows is asked for, an adapter's matrices are read once a chunk, and one no row uses costs nothing.
-// The first launch leaves the chunks' lists of adapters and rows for the second.
+// the rows is asked for, and an adapter that no row uses costs nothing. a is read once a chunk; b once for each of the
+// up to four workgroups that share an adapter's rows, and past 32 ranks once for each sixteen rows. The first launch
+// leaves the chunks' lists of adapters and rows for the second.
 //
 // FAST kernels are for operands whose every 16-byte piece is whole, aligned and within a buffer
 // descriptor's reach (the usual case): their loads have no branches, since an offset out of a descriptor's
 // range reads zeros and writes nothing. The others load pieces at any alignment, where they are whole, and
-// element by element where they are not (both launches on FAST operands: 64 rows, K5120 -> 2 x 17408: 15.3 us FAST,
-// 19.7 not; 2048 rows, K5120 -> N17408: 43 and 64).
+// element by element where they are not (both launches on FAST operands: 64 rows, K5120 -> 2 x 17408, fp32: 15.3 us
+// FAST, 19.6 not; 2048 rows, K5120 -> N17408, bf16: 44.0 and 57.6, and 66 with the odd sizes K5119 -> N17401).
 //
 // What has to move is the adapters' matrices in use, x, and out twice; the arithmetic, 2 rank (K + N) a row, is far
 // under the matrix core's rate. A step's small calls are two launches of 2 us, each with four dependent round
-// trips to memory (slots, ranks, operands, sums): 4.2 + 4.7 us for one row of K5120 -> N5120.
+// trips to memory (slots, ranks, operands, sums): 4.2 + 4.8 us for one row of K5120 -> N5120.
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -101,8 +102,9 @@ __device__ __forceinline__ void wave_fence() {
 // in which neighbouring lanes hold neighbouring rows: loaded in that order, every lane is a cache lookup of
 // its own.
 //
-// Bound by the reads of a: 64 rows of 32 adapters of ranks 16 to 64, K17408: 47 MB in 13.9 us (3.4 TB/s), 2 us of
-// it the launch. More loads in flight (the next steps' before this one's products; rows in runs of 128 bytes)
+// Bound by the reads of a where they are many, at up to 3.0 TB/s: 64 rows of 32 adapters, K17408, ranks 16 to 64
+// 47 MB in 15.7 us, 2 us of it the launch. Ranks of 64, 32, 16 and 8 leave workgroups of very uneven lengths, and the
+// longest decides: 36 MB in 15.1 us, and 31 MB in 13.9 where the rows use 27 of the 32 (2.2 TB/s). More loads in flight (the next steps' before this one's products; rows in runs of 128 bytes)
 // measured the same. One block of rows a workgroup (RBMAX 1, for up to 16 rows) saves the code and registers of the
 // other form: 4.9 us for 5.1 with eight rows on q, k and v. One panel of 16 ranks (P 1): 4.2 us for 4.7 with one row.
 
@@ -263,8 +265,8 @@ __global__ void __launch_bounds__(64 * kDownWaves, 2) adapter_down_kernel(Adapte
 // sums pass through LDS, so that a wave reads and writes runs of 64 neighbouring outputs of a row: with
 // the MFMA's own layout, neighbouring lanes hold different rows, and four times the cache lookups.
 //
-// Bound by out, read and written: 2048 rows, N17408, bf16: 160 MB in 34 us (4.7 TB/s, a large copy's rate); 64 rows,
-// 2 x 17408, fp32, rank 16: 27 MB in 8.4 us.
+// Bound by out, read and written, where it is large: 2048 rows, N17408, bf16: 160 MB in 34.6 us (4.6 TB/s, near a large
+// copy's 4.95); 64 rows, 2 x 17408, fp32, rank 16: 27 MB in 8.7 us (3.1 TB/s).
 
 constexpr int kPieces = 3;
 constexpr int kUpSumStride = 68;  // floats of a row of sums in LDS: 64 and a step of four banks
@@ -315,7 +317,7 @@ __device__ __forceinline__ void stage_t(const AdapterArgs &args, const AdapterWe
 }
 
 // NP 1: ranks up to 32, b held in registers; NP 0: any rank, b read again for each block of rows (2048 rows of rank
-// 16: 34.2 us held, 38.6 read again; holding 64 ranks measured level with reading them again).
+// 16: 34.6 us held, 35.6 read again; holding 64 ranks measured level with reading them again).
 template <int NP, typename OUT, bool FAST>
 __global__ void __launch_bounds__(256, NP == 1 ? 4 : 3) adapter_up_kernel(AdapterArgs args) {
     constexpr int kLoads = sizeof(OUT), kPer = 16 / sizeof(OUT), kHeld = NP ? NP : 1;
@@ -596,8 +598,8 @@ hipError_t launch_adapters(const splosh_adapters *w, int group, const uint16_t *
     const int64_t share = (tiles * chunks * (chunks == 1 ? parts : 1) + 1535) / 1536;
     args.tiles = (int)(share < most_tiles ? share : most_tiles);
     const unsigned up_x = (unsigned)((most_tiles + args.tiles - 1) / args.tiles);
-    // More than 16 rows an adapter: its rows in shares, a block of sixteen each (333 rows of three adapters of rank
-    // 64, K6144 -> N5120: 9.2 us, one workgroup for all of a chunk's rows 11.6; 500 of two, rank 128: 12.8 and 21.0).
+    // More than 16 rows an adapter: its rows in shares, a block of sixteen each (fp32, K6144 -> N5120: 333 rows of three
+    // adapters of rank 64: 9.5 us, one workgroup for all of a chunk's rows 15.2; 500 of two, rank 128: 16.2 and 23.5).
     args.shares = rows <= 16 * parts ? 1 : rows <= 32 ? 2 : 4;
     args.turns = plan_turns(parts, (int64_t)up_x * chunks * group * args.shares);
     const dim3 up(up_x, chunks, (unsigned)(group * args.turns * args.shares));

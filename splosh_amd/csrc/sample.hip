@@ -15,11 +15,12 @@
 //           for the others, the bins that the cut can be in;
 //   collect (pieces) each strip's weight above these bins, and the elements in them as a list;
 //   finish  (rows)   the cut, by ranking a short list or by a radix search in it, the strip the draw falls into and
-//           the token in it. A row whose cut lies below its bins, or in bins of more elements than the list
-//           holds, is searched whole (one workgroup, a pass for each nine bits of key: 2 ms for 248320 equal logits).
+//           the token in it. A row is searched whole where the bins cannot narrow its cut down to the list: by one
+//           workgroup, a pass over the row for each nine bits of key (248320 fp32: 0.4 to 0.9 ms, 64 rows of it 0.6 to
+//           1.2; all logits equal 2.1 and 2.3). Which rows those are: see settle.
 // The launches over pieces hold nothing but what they stream, so that four workgroups share a CU. The rows' launches
 // are chains of a few dependent round trips, about 1.5 us of each the launch's own: one row of 248320 with every
-// filter takes 5.3 + 6.4 + 4.4 + 4.8 us, and 64 of them 18 + 7.0 + 7.5 + 5.5. What has to move is the logits, once:
+// filter takes 5.2 + 6.4 + 4.9 + 4.8 us, and 64 of them 19 + 7.1 + 7.4 + 5.6. What has to move is the logits, once:
 // 64 rows of 248320 fp32, 64 MB, 13 us at the rate of a large copy.
 #include "common.hpp"
 #include "launch.hpp"
@@ -431,8 +432,8 @@ __device__ __forceinline__ void locate(const SampleArgs &args, int64_t r, const 
 // ---- scan -------------------------------------------------------------------------------------------
 //
 // Bound by its vector instructions beside the read: 35 an element with bins (an exponential at a quarter of the rate,
-// an LDS atomic), 20 without. 64 rows of 248320: fp32 with bins 64 MB in 17-19 us (3.4-3.7 TB/s), bf16 with the
-// temperature alone 32 MB in 12.3 us (2.6 TB/s). 512 threads of sixteen logits each: with 256 or 1024 threads slower.
+// an LDS atomic), 20 without. 64 rows of 248320: fp32 with bins 64 MB in 17-19 us (3.4-3.7 TB/s), greedy 11.8 (5.4),
+// bf16 with the temperature alone 32 MB in 12.2 us (2.6 TB/s). 512 threads of sixteen logits each: with 256 or 1024 threads slower.
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) {
@@ -526,7 +527,15 @@ __global__ void __launch_bounds__(kThreads) sample_scan_kernel(SampleArgs args) 
 // ---- settle -----------------------------------------------------------------------------------------
 //
 // Latency: the pieces' heads, then their bins (sixteen pieces at a time, 4 KB each), then scans over the workgroup;
-// 6.4 us for one row of 31 pieces, 7.0 for 64. Loading the bins before the heads are known measured slower.
+// 6.4 us for one row of 31 pieces, 7.1 for 64. Loading the bins before the heads are known measured slower.
+//
+// Rows that are left to be searched whole (measured with vocabularies of 248320, normal logits with a deviation of 2):
+//   - a share p that the bins cannot tell from the whole weight: p (1 + 2^-14) and half a bin's unit for each element
+//     of the vocabulary exceed it; p from 0.9999 on, 0.9998 with a head of likely tokens;
+//   - more than 8192 elements in the bins from the first that a cut can be in to the last that matters: equal logits;
+//     the cuts of top-p and of a top-k of ten thousands far apart; and logits about a value far from 0, since the bins
+//     are as wide as 1 + |logit| makes them: nuclei of p = 0.9 from an offset of 15 on, of 0.8 from 30 on;
+//   - cuts more than 512 bins below the largest logit.
 
 // 2^t for t <= 0, to the hardware's 2^-23.
 __device__ __forceinline__ double power_of(double t) {
@@ -653,8 +662,8 @@ __global__ void __launch_bounds__(kThreads) sample_settle_kernel(SampleArgs args
 // ---- collect ----------------------------------------------------------------------------------------
 //
 // Reads again what can be above the list or in it, strip by strip: nothing but the strips' records for rows that are
-// settled, few strips for rows with a peaked head (64 rows of 248320 fp32: 14 of 64 MB, 7.8 us), all of a flat row's
-// (16 of 100003 bf16 with top-p: 7.2 us).
+// settled, few strips for rows with a peaked head (64 rows of 248320 fp32: 14 of 64 MB, 7.4 us), all of a flat row's
+// (16 of 100003 bf16 with top-p: 7.5 us).
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs args) {
