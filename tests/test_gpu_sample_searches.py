@@ -138,3 +138,18 @@ def test_logprobs_of_unlikely_tokens(rt, far, dtype):
         want = z - kept.sum(1).log()
         assert (tokens > 0).all() and (z <= far + 0.5).all()
         assert ((logprobs.double() - want).abs() <= 2.0 ** -20 + 2.0 ** -23 * want.abs()).all(), (logprobs.double() - want).abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e-30, 0.7, 1e38, math.inf])
+def test_infinite_entries_with_every_filter(rt, temperature, dtype):
+    """+inf among the entries: those alone have weight, whatever filter they pass, in one piece or in several."""
+    rows, vocab = 6, 20011
+    logits = logits_of(rows, vocab, torch.float32, 84).to(dtype)
+    for r in range(rows):
+        logits[r, torch.randperm(vocab, generator=torch.Generator().manual_seed(r))[: 1 + 29 * r]] = math.inf
+    logits[:, 100:4000:3] = -math.inf
+    for on in ((1, 0, 0, 0), (1, 1, 0, 0), (1, 0, 1, 0), (1, 0, 0, 1), (1, 1, 1, 0), (1, 0, 1, 1), (1, 1, 1, 1)):
+        u, params = params_of(rows, 85, on)
+        params["temperature"] = torch.full((rows,), temperature)
+        run(rt, logits, u, params, f"{on}")
