@@ -491,6 +491,137 @@ int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64
                   const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                   uint32_t *tokens, float *logprobs, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- The attention layers of a packed step ------------------------------------------------------
+ *
+ * What lies between the q, k and v projections of a packed step and its out projection: norms of
+ * queries and keys over each head with the rotation by position, keys and values kept in 8 bits in a
+ * paged cache, and causal attention of the step's rows over that cache.
+ *
+ * How a step is packed: row m belongs to request r where starts[r] <= m < starts[r + 1] (starts[0] = 0,
+ * ascending; a request may have no row), and stands for that request's token at position
+ * lengths[r] - starts[r + 1] + m: lengths[r] counts the request's tokens in the cache once the step's own
+ * are in it. Position p of request r lies at place p % page_tokens of page table[r table_stride +
+ * p / page_tokens]. All three are device arrays that a kernel reads when it runs, so a captured call may
+ * find others at each replay. Rows from starts[requests] on belong to no request: what they would
+ * write is left as it was. A row with a negative position, or one past the table, has no place in the
+ * cache, and a page id that is negative or not below the cache's pages is no page: nothing is kept
+ * there, and what would be read from there is masked (attention) or zero (splosh_cache_read). starts below 0
+ * or above `rows` count as those. 1 <= requests <= SPLOSH_MAX_REQUESTS. */
+#define SPLOSH_MAX_REQUESTS 65535
+typedef struct splosh_packed {
+    const int32_t *starts;         /* requests + 1 */
+    const int32_t *lengths;        /* requests */
+    const int32_t *table;          /* requests rows of table_pages page ids */
+    int64_t requests;
+    int64_t table_stride;
+    int64_t table_pages;
+} splosh_packed;
+
+/* Keys and values of one layer in 8 bits, in pages of page_tokens tokens (a multiple of 32) for all
+ * `heads` key/value heads of dim 64, 128 or 256. Page i starts at data + i page_stride, page_stride >=
+ * splosh_cache_page_bytes(heads, dim, page_tokens) and a multiple of 16, data 16-byte aligned. A page holds for each
+ * head and each 32 tokens one record of 64 dim + 256 bytes: the int8 codes of the keys [32][dim], of the
+ * values [32][dim], the fp32 scales of the keys [32] and of the values [32]. A vector x is kept as
+ * code_i = rint(127 x_i / max|x|) and scale = max|x| / 127 and stands for code_i scale; where max|x| / 127 is below
+ * 2^-100, with that as the scale. One with an infinite or NaN element is kept as codes 0 and scale NaN, and
+ * stands for NaN. */
+typedef struct splosh_cache {
+    uint8_t *data;
+    int64_t pages;
+    int64_t page_stride;           /* bytes */
+    int64_t page_tokens;
+    int64_t heads;
+    int64_t dim;
+} splosh_cache;
+
+/* The bytes of one page (0: not a valid shape). */
+size_t splosh_cache_page_bytes(int64_t heads, int64_t dim, int64_t page_tokens);
+
+/* The heads of one projection: vector (row m, head h) of `dim` elements at x + m row_stride + h
+ * head_stride (elements of the call's dtype), so that queries may lie beside their gates. weight: bf16
+ * [dim], the norm's; NULL: no norm. out: bf16, dense rows of heads dim values, row stride ld_out;
+ * it may be x itself where x is bf16 with the same strides. */
+typedef struct splosh_heads {
+    const void *x;
+    int64_t row_stride;
+    int64_t head_stride;
+    int64_t heads;
+    const uint16_t *weight;
+    uint16_t *out;
+    int64_t ld_out;
+} splosh_heads;
+
+/* For every part i < count (queries and keys; count <= SPLOSH_MAX_GROUP), row and head, y = x / sqrt(mean(x^2) + eps) weight
+ * and then, for i < rotary / 2, the pair (y_i, y_{i + rotary/2}) turned by the angle positions[m]
+ * frequencies[i]: (a, b) -> (a cos - b sin, b cos + a sin). In fp32, angles in 64 bits, rounded once to bf16.
+ * x: fp32 or bf16 (dtype, that of all parts). frequencies: fp32 [rotary / 2], NULL with rotary 0: no
+ * rotation; rotary even, <= dim. dim 64, 128 or 256. */
+int splosh_rotate_heads(const splosh_heads *parts, int count, int dtype, int64_t rows, int64_t dim,
+                        const int32_t *positions, const float *frequencies, int64_t rotary, float eps,
+                        hipStream_t stream);
+
+/* A step's keys and values into the cache at their rows' places: keys as splosh_rotate_heads makes them
+ * (by the rows' own positions) but not rounded to bf16, values as they are. v's weight and the `out` of both must be NULL.
+ * q (NULL: none): the step's queries, to q->out as splosh_rotate_heads makes them, in the same launch. Two rows of one place
+ * (requests that share a page they both write) leave one or the other's bytes there. */
+int splosh_cache_write(const splosh_cache *cache, const splosh_packed *packed, const splosh_heads *k,
+                       const splosh_heads *v, const splosh_heads *q, int dtype, int64_t rows,
+                       const float *frequencies, int64_t rotary, float eps, hipStream_t stream);
+
+/* What the cache holds at the rows' places, as bf16 [rows][heads dim] (row strides ldk and ldv); k or v may
+ * be NULL. The rows of a read are those of a step: with starts[r + 1] - starts[r] = n the last n tokens of
+ * request r. */
+int splosh_cache_read(const splosh_cache *cache, const splosh_packed *packed, int64_t rows, uint16_t *k, int64_t ldk,
+                      uint16_t *v, int64_t ldv, hipStream_t stream);
+
+/* The workspace an attention call needs (0: not a valid shape). */
+size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_packed *packed, int64_t rows,
+                                     int64_t q_heads, int64_t shared);
+
+/* out[m][h] = sum_j w_j v_j, w = softmax over j <= position(m) of scale q[m][h] . k_j, keys and values those
+ * that head h / (q_heads / cache->heads) keeps for row m's request; the step's own have to be written before
+ * (splosh_cache_write). q: bf16, vector (m, h) at q + m row_stride + h head_stride; out: bf16, dense rows of q_heads dim
+ * values, row stride ld_out. A row that sees no key gets zeros.
+ * shared: the first `shared` tokens (a multiple of page_tokens, 0: none) are the same for all requests of the call: they
+ * are read through the pages of request 0, once for all rows; the table's entries of other requests for
+ * them are not used. Scores and sums are fp32, q's values enter the first product as they are, the weights the second one in fp16 (relative
+ * to the largest, 2^-11). Nothing is added in an order that changes: the result depends on the step's
+ * shape and on the device's count of CUs, and on no other call. The workspace need not be zeroed; its first
+ * 16 KiB stay as they are, so one that other calls use serves here too, in stream order. */
+int splosh_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
+                  const splosh_cache *cache, const splosh_packed *packed, int64_t rows, int64_t shared, float scale,
+                  uint16_t *out, int64_t ld_out, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---- Drafted tokens ------------------------------------------------------------------------------
+ *
+ * The end of a verify step: the rows of request r, starts[r] .. starts[r + 1] - 1, are the last token that
+ * it was given and the tokens drafted after it (tokens: the step's ids, those that were embedded), and
+ * the logits of row m (fp32 or bf16, row stride ld) judge the token of row m + 1. */
+
+/* The workspace a verification needs (0: not a valid shape). */
+size_t splosh_verify_workspace_bytes(int64_t rows, int64_t vocab, int64_t requests);
+
+/* With p_m = softmax(logits[m] / T) and q_m the draft's probabilities at row m (fp32 or bf16, row stride ld_draft; NULL: the drafted
+ * token's is 1), T = temperature[r], u = uniforms (one a row): going through the rows of request r but the last, the
+ * token t of row m + 1 is accepted if u_m q_m(t) < p_m(t), until one is not. accepted[r] = their count. After them one
+ * new token is drawn: at the row j whose token was not accepted from max(p_j - q_j, 0), or, all accepted, from p of
+ * the last row j: the lowest index whose running weight, itself included, exceeds u times the whole weight, u that
+ * of the request's last row. (Where max(p - q, 0) is 0 everywhere: from p.) out[starts[r] + i] is the i-th of the
+ * accepted tokens, then the new one, then -1 to the end of the request's rows, so that accepted[r] + 1 of them count.
+ *   - NaN and -inf entries have probability 0 (mask what a filter leaves out so); a row without any other has
+ *     none at all: its token is not accepted and the new one is -1. With +inf among them, the entries of +inf
+ *     alone have weight, the same each.
+ *   - T <= 0 or NaN: p is 1 at the largest entry, the first of equal ones. temperature NULL: 1.
+ *   - u below 0 or NaN counts as 0; u >= 1: the last entry with weight. A drafted id that is negative or not below
+ *     vocab is not accepted. A NaN q is not accepted and leaves no weight.
+ *   - A request without rows has accepted 0; rows of `out` past starts[requests] are left as they were.
+ * Weights and their sums are 64-bit floating point in a fixed order. vocab <= 2^21, rows and requests <= 65535.
+ * The workspace need not be zeroed; its first 16 KiB stay as they are. */
+int splosh_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const int32_t *tokens,
+                  const int32_t *starts, int64_t requests, const float *uniforms, const float *temperature,
+                  const void *draft, int64_t ld_draft, int draft_dtype, int32_t *out, int32_t *accepted, void *workspace,
+                  size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

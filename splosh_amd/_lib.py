@@ -72,6 +72,21 @@ class Adapters(ctypes.Structure):
                 ("b_slot_stride", _i64), ("b_row_stride", _i64)]
 
 
+class Packed(ctypes.Structure):
+    _fields_ = [("starts", _vp), ("lengths", _vp), ("table", _vp), ("requests", _i64), ("table_stride", _i64),
+                ("table_pages", _i64)]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [("data", _vp), ("pages", _i64), ("page_stride", _i64), ("page_tokens", _i64), ("heads", _i64),
+                ("dim", _i64)]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("x", _vp), ("row_stride", _i64), ("head_stride", _i64), ("heads", _i64), ("weight", _vp), ("out", _vp),
+                ("ld_out", _i64)]
+
+
 # name -> (restype, argtypes); every symbol include/splosh_q4.h declares.
 SIGNATURES = {
     "splosh_q4_layout_init": (_int, [_i64, _i64, _int, _i64, _i64, ctypes.POINTER(Layout)]),
@@ -130,6 +145,18 @@ SIGNATURES = {
                                          ctypes.POINTER(_i64), _int, _vp, _i64, _vp, _sz, _vp]),
     "splosh_sample_workspace_bytes": (_sz, [_i64, _i64]),
     "splosh_sample": (_int, [_vp, _i64, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "splosh_cache_page_bytes": (_sz, [_i64, _i64, _i64]),
+    "splosh_rotate_heads": (_int, [ctypes.POINTER(Heads), _int, _int, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp]),
+    "splosh_cache_write": (_int, [ctypes.POINTER(Cache), ctypes.POINTER(Packed), ctypes.POINTER(Heads),
+                                  ctypes.POINTER(Heads), ctypes.POINTER(Heads), _int, _i64, _vp, _i64, ctypes.c_float,
+                                  _vp]),
+    "splosh_cache_read": (_int, [ctypes.POINTER(Cache), ctypes.POINTER(Packed), _i64, _vp, _i64, _vp, _i64, _vp]),
+    "splosh_attend_workspace_bytes": (_sz, [ctypes.POINTER(Cache), ctypes.POINTER(Packed), _i64, _i64, _i64]),
+    "splosh_attend": (_int, [_vp, _i64, _i64, _i64, ctypes.POINTER(Cache), ctypes.POINTER(Packed), _i64, _i64,
+                             ctypes.c_float, _vp, _i64, _vp, _sz, _vp]),
+    "splosh_verify_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "splosh_verify": (_int, [_vp, _i64, _int, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _int, _vp, _vp, _vp, _sz,
+                             _vp]),
     "splosh_row_inv": (_int, [_vp, _i64, _i64, _i64, ctypes.c_float, _vp, _vp]),
 }
 

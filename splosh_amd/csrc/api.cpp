@@ -1264,3 +1264,210 @@ int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64
 }
 
 }  // extern "C"
+
+// ---- the attention layers of a packed step, and its drafted tokens -----------------------------
+
+namespace {
+
+constexpr int64_t kMaxStepRows = 1 << 22;      // rows of a launch
+constexpr int64_t kMaxCacheHeads = 1024;
+constexpr int64_t kMaxTableTokens = 1 << 30;   // positions stay far from 32 bits
+
+bool head_dim_ok(int64_t dim) { return dim == 64 || dim == 128 || dim == 256; }
+
+int check_rows(int64_t rows) {
+    if (rows <= 0) return fail(SPLOSH_ERR_INVALID_SHAPE, "rows must be positive");
+    if (rows > kMaxStepRows) return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows for one launch");
+    return SPLOSH_OK;
+}
+
+int check_cache(const splosh_cache *c) {
+    if (!c || !c->data) return fail(SPLOSH_ERR_NULL_POINTER, "null cache");
+    if (c->pages <= 0 || c->heads <= 0 || c->page_tokens <= 0 || c->dim <= 0)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "cache: pages, page_tokens, heads and dim must be positive");
+    const size_t bytes = splosh_cache_page_bytes(c->heads, c->dim, c->page_tokens);
+    if (!bytes)
+        return fail(SPLOSH_ERR_UNSUPPORTED, "cache: dim is 64, 128 or 256, page_tokens a multiple of 32");
+    if (c->page_stride < (int64_t)bytes || c->page_stride % 16 != 0)
+        return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "cache: page_stride is shorter than a page, or no multiple of 16");
+    if (c->pages > INT32_MAX || mul_overflows(c->pages, c->page_stride))
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "cache: size overflows");
+    if (!aligned(c->data, 16)) return fail(SPLOSH_ERR_UNSUPPORTED, "cache: data must be 16-byte aligned");
+    return SPLOSH_OK;
+}
+
+int check_packed(const splosh_packed *p, const splosh_cache &c) {
+    if (!p || !p->starts || !p->lengths || !p->table) return fail(SPLOSH_ERR_NULL_POINTER, "null starts, lengths or table");
+    if (p->requests <= 0 || p->table_pages <= 0)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "requests and table_pages must be positive");
+    if (p->requests > SPLOSH_MAX_REQUESTS) return fail(SPLOSH_ERR_UNSUPPORTED, "too many requests");
+    if (p->table_stride < p->table_pages && p->requests > 1)
+        return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "table_stride is shorter than table_pages");
+    if (p->table_stride < 0 || mul_overflows(p->requests, p->table_stride))
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "table: size overflows");
+    if (p->table_pages > kMaxTableTokens || p->table_pages * c.page_tokens > kMaxTableTokens)
+        return fail(SPLOSH_ERR_UNSUPPORTED, "more than 2^30 tokens a request");
+    if (!aligned(p->starts, 4) || !aligned(p->lengths, 4) || !aligned(p->table, 4))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "starts, lengths and table must be 4-byte aligned");
+    return SPLOSH_OK;
+}
+
+// `written`: whether the part has an output.
+int check_heads(const splosh_heads &h, int dtype, int64_t rows, int64_t dim, bool written) {
+    if (!h.x || (written && !h.out)) return fail(SPLOSH_ERR_NULL_POINTER, "null heads");
+    if (!written && h.out) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "keys and values of a cache have no other output");
+    if (h.heads <= 0) return fail(SPLOSH_ERR_INVALID_SHAPE, "heads must be positive");
+    if (h.heads > kMaxCacheHeads) return fail(SPLOSH_ERR_UNSUPPORTED, "too many heads");
+    if ((h.head_stride < dim && h.heads > 1) || h.head_stride < 0 || h.row_stride < 0 ||
+        (h.row_stride < dim && rows > 1) || (written && h.ld_out < h.heads * dim && rows > 1))
+        return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "heads: stride shorter than what it steps over");
+    if (mul_overflows(rows, h.row_stride) || mul_overflows(h.heads, h.head_stride) ||
+        (written && (h.ld_out < 0 || mul_overflows(rows, h.ld_out))))
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "heads: size overflows");
+    if (!aligned(h.x, dtype == SPLOSH_F32 ? 4 : 2) || !aligned(h.weight, 2) || !aligned(h.out, 2))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "heads are not aligned to their elements");
+    return SPLOSH_OK;
+}
+
+int check_rotation(int dtype, int64_t dim, const float *frequencies, int64_t rotary) {
+    if (dtype != SPLOSH_F32 && dtype != SPLOSH_BF16) return fail(SPLOSH_ERR_UNSUPPORTED, "unknown dtype");
+    if (rotary < 0 || rotary > dim || rotary % 2 != 0)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "rotary must be even, from 0 to dim");
+    if (rotary > 0 && !frequencies) return fail(SPLOSH_ERR_NULL_POINTER, "null frequencies");
+    if (!aligned(frequencies, 4)) return fail(SPLOSH_ERR_UNSUPPORTED, "frequencies must be 4-byte aligned");
+    return SPLOSH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t splosh_cache_page_bytes(int64_t heads, int64_t dim, int64_t page_tokens) {
+    if (heads <= 0 || heads > kMaxCacheHeads || !head_dim_ok(dim) || page_tokens <= 0 || page_tokens % 32 != 0 ||
+        page_tokens > kMaxTableTokens)
+        return 0;
+    return (size_t)(heads * (page_tokens / 32) * (64 * dim + 256));
+}
+
+int splosh_rotate_heads(const splosh_heads *parts, int count, int dtype, int64_t rows, int64_t dim,
+                        const int32_t *positions, const float *frequencies, int64_t rotary, float eps,
+                        hipStream_t stream) {
+    if (!parts) return fail(SPLOSH_ERR_NULL_POINTER, "null heads list");
+    if (count < 1 || count > SPLOSH_MAX_GROUP)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "count must be 1.." + std::to_string(SPLOSH_MAX_GROUP));
+    if (!head_dim_ok(dim)) return fail(SPLOSH_ERR_UNSUPPORTED, "dim is 64, 128 or 256");
+    int st;
+    if ((st = check_rows(rows)) || (st = check_rotation(dtype, dim, frequencies, rotary))) return st;
+    if (rotary > 0 && !positions) return fail(SPLOSH_ERR_NULL_POINTER, "null positions");
+    if (!aligned(positions, 4)) return fail(SPLOSH_ERR_UNSUPPORTED, "positions must be 4-byte aligned");
+    for (int i = 0; i < count; ++i) {
+        if ((st = check_heads(parts[i], dtype, rows, dim, true))) return st;
+        for (int j = 0; j < i; ++j)
+            if (parts[i].out == parts[j].out) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "outputs must not overlap");
+    }
+    return hip_status(splosh::launch_rotate_heads(parts, count, dtype, rows, dim, positions, frequencies, rotary, eps,
+                                                  stream),
+                      "rotate heads launch");
+}
+
+int splosh_cache_write(const splosh_cache *cache, const splosh_packed *packed, const splosh_heads *k,
+                       const splosh_heads *v, const splosh_heads *q, int dtype, int64_t rows,
+                       const float *frequencies, int64_t rotary, float eps, hipStream_t stream) {
+    int st;
+    if ((st = check_cache(cache)) || (st = check_packed(packed, *cache))) return st;
+    if (!k || !v) return fail(SPLOSH_ERR_NULL_POINTER, "null keys or values");
+    if ((st = check_rows(rows)) || (st = check_rotation(dtype, cache->dim, frequencies, rotary)) ||
+        (st = check_heads(*k, dtype, rows, cache->dim, false)) || (st = check_heads(*v, dtype, rows, cache->dim, false)) ||
+        (q && (st = check_heads(*q, dtype, rows, cache->dim, true))))
+        return st;
+    if (k->heads != cache->heads || v->heads != cache->heads)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "keys and values must have the cache's heads");
+    if (v->weight) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "values have no norm");
+    return hip_status(splosh::launch_cache_write(*cache, *packed, *k, *v, q, dtype, rows, frequencies, rotary, eps,
+                                                 stream),
+                      "cache write launch");
+}
+
+int splosh_cache_read(const splosh_cache *cache, const splosh_packed *packed, int64_t rows, uint16_t *k, int64_t ldk,
+                      uint16_t *v, int64_t ldv, hipStream_t stream) {
+    int st;
+    if ((st = check_cache(cache)) || (st = check_packed(packed, *cache)) || (st = check_rows(rows))) return st;
+    if (!k && !v) return fail(SPLOSH_ERR_NULL_POINTER, "null keys and values");
+    const int64_t columns = cache->heads * cache->dim;
+    if ((k && ldk < columns) || (v && ldv < columns))
+        return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "row stride shorter than a row");
+    if ((k && mul_overflows(rows, ldk)) || (v && mul_overflows(rows, ldv)))
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "size overflows");
+    if (k == v) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "outputs must not overlap");
+    if (!aligned(k, 2) || !aligned(v, 2)) return fail(SPLOSH_ERR_UNSUPPORTED, "outputs are not aligned to their elements");
+    return hip_status(splosh::launch_cache_read(*cache, *packed, rows, k, ldk, v, ldv, stream), "cache read launch");
+}
+
+size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_packed *packed, int64_t rows,
+                                     int64_t q_heads, int64_t shared) {
+    if (!cache || !packed || !splosh_cache_page_bytes(cache->heads, cache->dim, cache->page_tokens) || rows <= 0 ||
+        rows > kMaxStepRows || q_heads <= 0 || q_heads > kMaxCacheHeads || q_heads % cache->heads != 0 || shared < 0 ||
+        packed->requests <= 0 || packed->requests > SPLOSH_MAX_REQUESTS)
+        return 0;
+    return splosh::attend_workspace_bytes(*cache, packed->requests, rows, q_heads, shared);
+}
+
+int splosh_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
+                  const splosh_cache *cache, const splosh_packed *packed, int64_t rows, int64_t shared, float scale,
+                  uint16_t *out, int64_t ld_out, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    int st;
+    if ((st = check_cache(cache)) || (st = check_packed(packed, *cache)) || (st = check_rows(rows))) return st;
+    const splosh_heads part{q, row_stride, head_stride, q_heads, nullptr, out, ld_out};
+    if ((st = check_heads(part, SPLOSH_BF16, rows, cache->dim, true))) return st;
+    if (q_heads % cache->heads != 0)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "q_heads must be a multiple of the cache's heads");
+    if (shared < 0 || shared % cache->page_tokens != 0 || shared / cache->page_tokens > packed->table_pages)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "shared must be whole pages of the table");
+    if (!(scale > 0.0f) || scale > 3.0e38f) return fail(SPLOSH_ERR_INVALID_SHAPE, "scale must be positive and finite");
+    const size_t need = splosh::attend_workspace_bytes(*cache, packed->requests, rows, q_heads, shared);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SPLOSH_ERR_WORKSPACE_TOO_SMALL,
+                    "attention needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return hip_status(splosh::launch_attend(q, row_stride, head_stride, q_heads, *cache, *packed, rows, shared, scale, out,
+                                            ld_out, workspace, stream),
+                      "attention launch");
+}
+
+size_t splosh_verify_workspace_bytes(int64_t rows, int64_t vocab, int64_t requests) {
+    if (rows <= 0 || rows > splosh::kVerifyMaxRows || vocab <= 0 || vocab > splosh::kVerifyMaxVocab || requests <= 0 ||
+        requests > splosh::kVerifyMaxRows)
+        return 0;
+    return splosh::verify_workspace_bytes(rows, vocab, requests);
+}
+
+int splosh_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const int32_t *tokens,
+                  const int32_t *starts, int64_t requests, const float *uniforms, const float *temperature,
+                  const void *draft, int64_t ld_draft, int draft_dtype, int32_t *out, int32_t *accepted, void *workspace,
+                  size_t workspace_bytes, hipStream_t stream) {
+    if (!logits || !tokens || !starts || !uniforms || !out || !accepted)
+        return fail(SPLOSH_ERR_NULL_POINTER, "null logits, tokens, starts, uniforms or output");
+    if (rows <= 0 || vocab <= 0 || requests <= 0)
+        return fail(SPLOSH_ERR_INVALID_SHAPE, "rows, vocab and requests must be positive");
+    if (ld < vocab || (draft && ld_draft < vocab)) return fail(SPLOSH_ERR_INVALID_ROW_STRIDE, "ld is shorter than vocab");
+    if ((dtype != SPLOSH_F32 && dtype != SPLOSH_BF16) || (draft && draft_dtype != SPLOSH_F32 && draft_dtype != SPLOSH_BF16))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "unknown logits or draft dtype");
+    if (vocab > splosh::kVerifyMaxVocab) return fail(SPLOSH_ERR_UNSUPPORTED, "vocab above 2^21");
+    if (rows > splosh::kVerifyMaxRows || requests > splosh::kVerifyMaxRows)
+        return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows or requests for one launch");
+    if (mul_overflows(rows, ld) || (draft && mul_overflows(rows, ld_draft)))
+        return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "size overflows");
+    if (!aligned(logits, dtype == SPLOSH_F32 ? 4 : 2) || !aligned(draft, draft_dtype == SPLOSH_F32 ? 4 : 2) ||
+        !aligned(tokens, 4) || !aligned(starts, 4) || !aligned(uniforms, 4) || !aligned(temperature, 4) || !aligned(out, 4) ||
+        !aligned(accepted, 4))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "operands are not aligned to their elements");
+    if (out == tokens || accepted == out) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "outputs must not overlap the tokens");
+    const size_t need = splosh::verify_workspace_bytes(rows, vocab, requests);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SPLOSH_ERR_WORKSPACE_TOO_SMALL,
+                    "verification needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return hip_status(splosh::launch_verify(logits, ld, dtype, rows, vocab, tokens, starts, requests, uniforms, temperature,
+                                            draft, ld_draft, draft_dtype, out, accepted, workspace, stream),
+                      "verify launch");
+}
+
+}  // extern "C"

@@ -312,4 +312,28 @@ hipError_t launch_sample(const void *logits, int64_t ld, int dtype, int64_t rows
                          const SampleParams &params, uint32_t *tokens, float *logprobs, void *workspace,
                          hipStream_t stream);
 
+// The heads of a packed step, before its attention (heads.hip).
+hipError_t launch_rotate_heads(const splosh_heads *parts, int count, int dtype, int64_t rows, int64_t dim,
+                               const int32_t *positions, const float *frequencies, int64_t rotary, float eps,
+                               hipStream_t stream);
+hipError_t launch_cache_write(const splosh_cache &cache, const splosh_packed &packed, const splosh_heads &k,
+                              const splosh_heads &v, const splosh_heads *q, int dtype, int64_t rows,
+                              const float *frequencies, int64_t rotary, float eps, hipStream_t stream);
+hipError_t launch_cache_read(const splosh_cache &cache, const splosh_packed &packed, int64_t rows, uint16_t *k,
+                             int64_t ldk, uint16_t *v, int64_t ldv, hipStream_t stream);
+
+// Attention over the cache (attend.hip).
+size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t shared);
+hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
+                         const splosh_cache &cache, const splosh_packed &packed, int64_t rows, int64_t shared,
+                         float scale, uint16_t *out, int64_t ld_out, void *workspace, hipStream_t stream);
+
+// Drafted tokens (verify.hip).
+constexpr int64_t kVerifyMaxVocab = 1 << 21, kVerifyMaxRows = 65535;
+size_t verify_workspace_bytes(int64_t rows, int64_t vocab, int64_t requests);
+hipError_t launch_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const int32_t *tokens,
+                         const int32_t *starts, int64_t requests, const float *uniforms, const float *temperature,
+                         const void *draft, int64_t ld_draft, int draft_dtype, int32_t *out, int32_t *accepted,
+                         void *workspace, hipStream_t stream);
+
 }  // namespace splosh

@@ -1,0 +1,310 @@
+// verify.hip -- drafted tokens against the target's probabilities.
+//
+// A drafted token t is accepted if u q(t) < p(t); where one is not, the next token comes from max(p - q, 0). What has
+// to move is the step's logits, once, for the maximum and sum of each row's softmax; of each request one row more of
+// logits and draft for the new token. All that decides between two tokens is in 64-bit floating point, added in an
+// order that the shape alone gives: the neighbours of a draw on a vocabulary of 250000 lie 1e-9 of the weight apart, which fp32
+// would not tell.
+//
+// Three launches; a workgroup takes a piece of 8192 entries of a row, or a request:
+//   scan   (pieces of every row)         the piece's largest entry and the weight of its entries against it;
+//   rest   (pieces of every request's row) which row ends the request's accepted run, from the pieces' numbers and one
+//          probability a row, and the weights max(p - q, 0) and p of that row by strips of 1024;
+//   finish (requests)                    the strip that the draw falls into, and the token in it.
+#include <climits>
+
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace splosh {
+
+constexpr size_t kVerifyCounterBytes = 16384;  // the workspace's first bytes belong to other kernels' counters
+constexpr int kThreads = 512, kWaves = kThreads / 64, kPer = 16;
+constexpr int kStrip = 64 * kPer, kPiece = kThreads * kPer;
+
+struct PieceStats {
+    double sum;
+    float most;
+    int first;  // the first entry of that value
+};
+struct Decision {
+    int row, last, top;  // the row that ends the accepted run, whether it is the request's last, its first largest entry
+    float most;
+    double total, by;    // the row's weight; log2(e) / T, 0: greedy
+};
+struct StripSums {
+    double rest, whole;
+};
+
+struct VerifyArgs {
+    const void *logits;
+    int64_t ld;
+    int vocab, pieces, requests, rows;
+    const int32_t *tokens, *starts;
+    const float *uniforms, *temperature;
+    const void *draft;
+    int64_t ld_draft;
+    int draft_f32;
+    int32_t *out, *accepted;
+    PieceStats *stats;
+    Decision *decisions;
+    StripSums *strips;
+};
+
+// 2^x, x <= 0, to 1e-13: the whole part as the exponent, the fraction (|f| <= 1/2) by its series in f ln 2.
+__device__ __forceinline__ double power2(double x) {
+    if (!(x > -1000.0)) return 0.0;
+    const double n = __builtin_rint(x), f = (x - n) * 0.6931471805599453;
+    double e = 1.0 / 479001600.0;
+    e = e * f + 1.0 / 39916800.0;
+    e = e * f + 1.0 / 3628800.0;
+    e = e * f + 1.0 / 362880.0;
+    e = e * f + 1.0 / 40320.0;
+    e = e * f + 1.0 / 5040.0;
+    e = e * f + 1.0 / 720.0;
+    e = e * f + 1.0 / 120.0;
+    e = e * f + 1.0 / 24.0;
+    e = e * f + 1.0 / 6.0;
+    e = e * f + 0.5;
+    e = e * f + 1.0;
+    e = e * f + 1.0;
+    return __builtin_ldexp(e, (int)n);
+}
+
+// log2(e) / T; 0 where T asks for the largest entry.
+__device__ __forceinline__ double factor_of(const float *temperature, int request) {
+    const float t = temperature ? temperature[request] : 1.0f;
+    // (An infinite T: all entries alike.)
+    return t > 0.0f ? __builtin_fmax(1.4426950408889634 / (double)__builtin_fmaxf(t, 1.1754944e-38f), 1e-300) : 0.0;
+}
+
+// The weight of an entry against the largest, `most`; `first`: whether it is the first of that value.
+__device__ __forceinline__ double weight_of(float v, float most, double by, bool first) {
+    if (!(v > -__builtin_inff())) return 0.0;  // (NaN and -inf)
+    if (by == 0.0) return first ? 1.0 : 0.0;
+    if (v == most) return 1.0;
+    return most == __builtin_inff() ? 0.0 : power2(((double)v - (double)most) * by);
+}
+
+__device__ __forceinline__ float entry(const float *p) { return *p; }
+__device__ __forceinline__ float entry(const uint16_t *p) { return bf16_bits_to_f32(*p); }
+
+// The request of row `row`, -1: none.
+__device__ __forceinline__ int row_request(const int32_t *starts, int requests, int row) {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int base = 0; base <= requests; base += 64) {
+        const int i = base + lane, n = __popcll(__ballot(i <= requests && starts[i] <= row));
+        count += n;
+        if (n < 64) break;
+    }
+    return count - 1 < requests ? count - 1 : -1;
+}
+
+// (v, i): the larger value, of equal ones the lower index. NaN is no value.
+__device__ __forceinline__ void keep_first(float &v, int &i, float w, int j) {
+    if (w > v || (w == v && j < i)) v = w, i = j;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
+    __shared__ float wave_most[kWaves];
+    __shared__ int wave_first[kWaves];
+    __shared__ double wave_total[kWaves];
+    const int row = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int r = row_request(a.starts, a.requests, row);
+    if (r < 0) return;
+    const T *logits = (const T *)a.logits + row * a.ld;
+    const int begin = piece * kPiece + wave * kStrip + lane;
+    float v[kPer], most = -__builtin_inff();
+    int first = INT_MAX;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = begin + 64 * e < a.vocab ? entry(logits + begin + 64 * e) : -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) keep_first(most, first, v[e], begin + 64 * e);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) keep_first(most, first, __shfl_xor(most, m), __shfl_xor(first, m));
+    if (lane == 0) wave_most[wave] = most, wave_first[wave] = first;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) keep_first(most, first, wave_most[w], wave_first[w]);
+    const double by = factor_of(a.temperature, r);
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += weight_of(v[e], most, by, begin + 64 * e == first);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+    if (lane == 0) wave_total[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kWaves; ++w) sum += wave_total[w];
+        a.stats[(int64_t)row * a.pieces + piece] = {sum, most, first};
+    }
+}
+
+// The whole row from its pieces, by one wave: the largest entry, the first of that value, and the weight against it.
+__device__ __forceinline__ PieceStats row_stats(const VerifyArgs &a, int row, double by) {
+    const int lane = threadIdx.x & 63;
+    const PieceStats *stats = a.stats + (int64_t)row * a.pieces;
+    float most = -__builtin_inff();
+    int first = INT_MAX;
+    for (int i = lane; i < a.pieces; i += 64) keep_first(most, first, stats[i].most, stats[i].first);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) keep_first(most, first, __shfl_xor(most, m), __shfl_xor(first, m));
+    double sum = 0.0;
+    for (int i = lane; i < a.pieces; i += 64) sum += stats[i].sum * weight_of(stats[i].most, most, by, stats[i].first == first);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+    return {sum, most, first};
+}
+
+__device__ __forceinline__ double draft_of(const VerifyArgs &a, int row, int token, int drafted) {
+    if (!a.draft) return token == drafted ? 1.0 : 0.0;
+    const int64_t at = row * a.ld_draft + token;
+    return a.draft_f32 ? ((const float *)a.draft)[at] : bf16_bits_to_f32(((const uint16_t *)a.draft)[at]);
+}
+
+// u of a row: below 0 or NaN as 0.
+__device__ __forceinline__ double uniform_of(const VerifyArgs &a, int row) { return __builtin_fmax((double)a.uniforms[row], 0.0); }
+
+// (weight of max(p - q, 0), of p) of one entry of the decided row.
+template <typename T>
+__device__ __forceinline__ StripSums rest_of(const VerifyArgs &a, const Decision &d, int drafted, int token) {
+    if (token >= a.vocab || !(d.total > 0.0)) return {0.0, 0.0};
+    const double p = weight_of(entry((const T *)a.logits + d.row * a.ld + token), d.most, d.by, token == d.top) / d.total;
+    return {d.last ? p : __builtin_fmax(p - draft_of(a, d.row, token, drafted), 0.0), p};
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
+    __shared__ int stop;
+    __shared__ Decision decision;
+    const int r = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int begin = max(a.starts[r], 0), end = min(a.starts[r + 1], a.rows);
+    if (begin >= end) {
+        if (piece == 0 && tid == 0) a.accepted[r] = 0, a.decisions[r].row = -1;
+        return;
+    }
+    if (tid == 0) stop = end - 1;
+    __syncthreads();
+    const double by = factor_of(a.temperature, r);
+    for (int row = begin + wave; row < end - 1; row += kWaves) {
+        const PieceStats s = row_stats(a, row, by);
+        const int t = a.tokens[row + 1];
+        bool accept = t >= 0 && t < a.vocab;
+        if (accept) {
+            const double p = weight_of(entry((const T *)a.logits + row * a.ld + t), s.most, by, t == s.first);
+            accept = s.sum > 0.0 && uniform_of(a, row) * draft_of(a, row, t, t) < p / s.sum;
+        }
+        if (!accept && lane == 0) atomicMin(&stop, row);
+    }
+    __syncthreads();
+    if (wave == 0) {
+        const PieceStats s = row_stats(a, stop, by);
+        if (lane == 0) decision = {stop, stop == end - 1, s.first, s.most, s.sum, by};
+    }
+    __syncthreads();
+    const Decision d = decision;
+    const int drafted = d.last ? -1 : a.tokens[d.row + 1];
+    if (piece == 0) {
+        if (tid == 0) a.decisions[r] = d, a.accepted[r] = d.row - begin;
+        for (int row = begin + tid; row < end; row += kThreads)
+            if (row != d.row) a.out[row] = row < d.row ? a.tokens[row + 1] : -1;
+    }
+    StripSums sum{0.0, 0.0};
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const StripSums w = rest_of<T>(a, d, drafted, piece * kPiece + wave * kStrip + 64 * e + lane);
+        sum.rest += w.rest, sum.whole += w.whole;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) sum.rest += __shfl_xor(sum.rest, m), sum.whole += __shfl_xor(sum.whole, m);
+    if (lane == 0) a.strips[((int64_t)r * a.pieces + piece) * kWaves + wave] = sum;
+}
+
+// The wave's running sums over its lanes, each lane's own included.
+__device__ __forceinline__ double wave_running(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double w = __shfl_up(v, m);
+        if (lane >= m) v += w;
+    }
+    return v;
+}
+
+// One wave a request: strips by the lane, then the strip's entries 64 at a time.
+template <typename T>
+__global__ __launch_bounds__(64) void finish_kernel(VerifyArgs a) {
+    const int r = blockIdx.x, lane = threadIdx.x;
+    const Decision d = a.decisions[r];
+    if (d.row < 0) return;
+    const StripSums *strips = a.strips + (int64_t)r * a.pieces * kWaves;
+    const int count = a.pieces * kWaves, drafted = d.last ? -1 : a.tokens[d.row + 1];
+    double rest = 0.0, whole = 0.0;
+    for (int i = lane; i < count; i += 64) rest += strips[i].rest, whole += strips[i].whole;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) rest += __shfl_xor(rest, m), whole += __shfl_xor(whole, m);
+    const bool from_rest = rest > 0.0;
+    const double most = uniform_of(a, min(a.starts[r + 1], a.rows) - 1) * (from_rest ? rest : whole);
+    // The strip whose running weight passes the draw; the last one with weight if none does.
+    double before = 0.0, strip_before = 0.0;
+    int strip = -1;
+    for (int base = 0; base < count; base += 64) {
+        const int i = base + lane;
+        const double w = i < count ? (from_rest ? strips[i].rest : strips[i].whole) : 0.0;
+        const double running = before + wave_running(w);
+        const uint64_t passed = __ballot(w > 0.0 && running > most), with = __ballot(w > 0.0);
+        const int at = passed ? __builtin_ctzll(passed) : with ? 63 - __builtin_clzll(with) : -1;
+        if (at >= 0) strip = base + at, strip_before = __shfl(running - w, at);
+        if (passed) break;
+        before = __shfl(running, 63);
+    }
+    int token = -1;
+    if (strip >= 0) {
+        before = strip_before;
+        for (int e = 0; e < kPer; ++e) {
+            const StripSums s = rest_of<T>(a, d, drafted, strip * kStrip + 64 * e + lane);
+            const double w = from_rest ? s.rest : s.whole, running = before + wave_running(w);
+            const uint64_t passed = __ballot(w > 0.0 && running > most), with = __ballot(w > 0.0);
+            const int at = passed ? __builtin_ctzll(passed) : with ? 63 - __builtin_clzll(with) : -1;
+            if (at >= 0) token = strip * kStrip + 64 * e + at;
+            if (passed) break;
+            before = __shfl(running, 63);
+        }
+    }
+    if (lane == 0) a.out[d.row] = token;
+}
+
+static int64_t pieces_of(int64_t vocab) { return (vocab + kPiece - 1) / kPiece; }
+
+size_t verify_workspace_bytes(int64_t rows, int64_t vocab, int64_t requests) {
+    const int64_t pieces = pieces_of(vocab);
+    return kVerifyCounterBytes + rows * pieces * sizeof(PieceStats) + requests * sizeof(Decision) +
+           requests * pieces * kWaves * sizeof(StripSums);
+}
+
+hipError_t launch_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const int32_t *tokens,
+                         const int32_t *starts, int64_t requests, const float *uniforms, const float *temperature,
+                         const void *draft, int64_t ld_draft, int draft_dtype, int32_t *out, int32_t *accepted,
+                         void *workspace, hipStream_t stream) {
+    static_assert(sizeof(PieceStats) == 16 && sizeof(Decision) % 16 == 0 && sizeof(StripSums) == 16, "aligned arrays");
+    VerifyArgs a{logits, ld, (int)vocab, (int)pieces_of(vocab), (int)requests, (int)rows, tokens, starts, uniforms,
+                 temperature, draft, ld_draft, draft_dtype == SPLOSH_F32, out, accepted, nullptr, nullptr, nullptr};
+    uint8_t *at = static_cast<uint8_t *>(workspace) + kVerifyCounterBytes;
+    a.stats = reinterpret_cast<PieceStats *>(at);
+    at += rows * a.pieces * sizeof(PieceStats);
+    a.decisions = reinterpret_cast<Decision *>(at);
+    at += requests * sizeof(Decision);
+    a.strips = reinterpret_cast<StripSums *>(at);
+    const dim3 rows_grid(a.pieces, (unsigned)rows), requests_grid(a.pieces, (unsigned)requests);
+    auto go = [&](auto scan, auto rest, auto finish) {
+        scan<<<rows_grid, kThreads, 0, stream>>>(a);
+        rest<<<requests_grid, kThreads, 0, stream>>>(a);
+        finish<<<(unsigned)requests, 64, 0, stream>>>(a);
+    };
+    if (dtype == SPLOSH_F32) go(scan_kernel<float>, rest_kernel<float>, finish_kernel<float>);
+    else go(scan_kernel<uint16_t>, rest_kernel<uint16_t>, finish_kernel<uint16_t>);
+    return hipGetLastError();
+}
+
+}  // namespace splosh

@@ -9,6 +9,9 @@ libsplosh_q4.so through its C ABI. The names follow the reference's host API:
   GgufPlanes.repack on the device.
 * ``add_adapters`` / ``sample`` -- what differs between the requests of a packed step: low-rank
   adapters beside a projection, and the choice of each row's next token.
+* ``rotate_heads`` / ``cache_write`` / ``cache_read`` / ``attend`` -- a packed step's attention layers between their
+  projections: norms and rotation of the heads, the 8-bit paged cache, attention over it.
+* ``verify`` -- the drafted tokens of a verify step against the target's probabilities.
 
 Buffer-size checks (GemmQ4Error.bufferTooSmall) happen here because the C ABI sees raw pointers.
 """
@@ -808,3 +811,271 @@ def sample(logits, uniforms=None, temperature=None, top_k=None, top_p=None, min_
     if st:
         _lib.check(st)
     return out, logprobs
+
+
+# ---- the attention layers of a packed step, and its drafted tokens ---------------------------------
+
+
+def _same_device(t, index, name):
+    if not t.is_cuda:
+        raise SploshError(12, f"{name} is not a device tensor")
+    if t.get_device() != index:
+        raise SploshError(13, f"{name} is on {t.device}, the operands on cuda:{index}")
+
+
+@dataclass(frozen=True)
+class Packed:
+    """How a step's rows are packed (splosh_packed): ``starts`` int32 [requests + 1], the first row of each request
+    and their end; ``lengths`` int32 [requests], each request's tokens in the cache once the step's own are in it;
+    ``table`` int32 [requests, pages], its pages in order (contiguous rows). The tensors are taken as they are:
+    the next step's values are written into them, and other tensors need a handle of their own."""
+
+    starts: torch.Tensor
+    lengths: torch.Tensor
+    table: torch.Tensor
+
+    def __post_init__(self):
+        table = self.table
+        index = _index(table, "table")
+        if table.dtype != torch.int32 or table.dim() != 2 or 0 in table.shape or (table.stride(1) != 1 and table.shape[1] > 1):
+            raise SploshError(13, "table must be int32 [requests, pages] with contiguous rows")
+        requests, pages = table.shape
+        starts = _vector(self.starts, requests + 1, torch.int32, index, "starts")
+        lengths = _vector(self.lengths, requests, torch.int32, index, "lengths")
+        c = _lib.Packed(starts, lengths, table.data_ptr(), requests, _row_stride(table), pages)
+        for name, value in dict(index=index, requests=requests, _c=c).items():
+            object.__setattr__(self, name, value)
+
+    def c(self):
+        return self._c
+
+
+def cache_page_bytes(heads, dim, page_tokens):
+    """splosh_cache_page_bytes: the bytes of one page (0: not a valid shape)."""
+    return _lib.lib().splosh_cache_page_bytes(heads, dim, page_tokens)
+
+
+@dataclass(frozen=True)
+class Cache:
+    """Keys and values of one layer in 8 bits (splosh_cache): ``data`` uint8 [pages, bytes], a page a row of
+    cache_page_bytes(heads, dim, page_tokens) bytes or more, 16-byte aligned."""
+
+    data: torch.Tensor
+    page_tokens: int
+    heads: int
+    dim: int
+
+    def __post_init__(self):
+        data = self.data
+        index = _index(data, "data")
+        need = cache_page_bytes(self.heads, self.dim, self.page_tokens)
+        if not need:
+            raise SploshError(13, "a cache has dim 64, 128 or 256 and page_tokens a multiple of 32")
+        if data.dtype != torch.uint8 or data.dim() != 2 or 0 in data.shape or (data.stride(1) != 1 and data.shape[1] > 1):
+            raise SploshError(13, "data must be uint8 [pages, bytes] with contiguous pages")
+        if data.shape[1] < need:
+            raise GemmQ4Error(8, f"bufferTooSmall(name: page, expected: {need}, observed: {data.shape[1]})")
+        stride = data.stride(0) if data.shape[0] > 1 else (data.shape[1] + 15) // 16 * 16
+        c = _lib.Cache(data.data_ptr(), data.shape[0], stride, self.page_tokens, self.heads, self.dim)
+        for name, value in dict(index=index, pages=data.shape[0], _c=c).items():
+            object.__setattr__(self, name, value)
+
+    def c(self):
+        return self._c
+
+    @classmethod
+    def empty(cls, pages, page_tokens, heads, dim, device):
+        """A cache of `pages` pages that holds nothing yet."""
+        data = torch.zeros((pages, cache_page_bytes(heads, dim, page_tokens)), dtype=torch.uint8, device=device)
+        return cls(data, page_tokens, heads, dim)
+
+
+def _head_vectors(t, rows, heads, dim, dtype, index, name):
+    """(address, row stride, head stride, heads) of `rows` rows of `heads` (None: its own) vectors of `dim`."""
+    _same_device(t, index, name)
+    if t.dim() != 3 or t.dtype != dtype or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise SploshError(13, f"{name} must be {dtype} [rows, heads, dim] with contiguous vectors")
+    if t.shape[2] != dim or t.shape[1] == 0 or (heads is not None and t.shape[1] != heads):
+        raise GemmQ4Error(1, f"{name} is {tuple(t.shape)}, [rows, {heads or 'heads'}, {dim}] is needed")
+    if t.shape[0] < rows:
+        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows} rows, observed: {t.shape[0]})")
+    head = t.stride(1) if t.shape[1] > 1 else max(t.stride(1), dim)
+    row = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), dim)
+    return t.data_ptr(), row, head, t.shape[1]
+
+
+def _dense_heads(t, rows, heads, dim, index, name):
+    """(address, row stride) of a bf16 output [rows, heads, dim] whose rows are dense."""
+    ptr, _, head, _ = _head_vectors(t, rows, heads, dim, torch.bfloat16, index, name)
+    if head != dim and heads > 1:
+        raise SploshError(13, f"{name} must have dense rows")
+    return ptr, t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * dim)
+
+
+def _norm_weight(t, dim, index, name):
+    return _vector(t, dim, torch.bfloat16, index, name)
+
+
+def _frequencies(t, index):
+    """(address, rotary dimensions)."""
+    return (None, 0) if t is None else (_vector(t, 0, torch.float32, index, "frequencies"), 2 * t.numel())
+
+
+def rotate_heads(xs, positions, frequencies, weights=None, eps=1e-6, outs=None, rows=None, stream=None):
+    """splosh_rotate_heads: queries and keys (any number of tensors [rows, heads, dim], fp32 or bf16 alike, strided as
+    their projections left them) normed over each head by ``weights`` (bf16 [dim] each; None: no norm) and their
+    pairs (i, i + len(frequencies)) turned by positions[m] * frequencies[i] (int32 [rows], fp32; None: not). Returns bf16
+    [rows, heads, dim] each."""
+    xs = list(xs)
+    if not xs or len(xs) > 8:
+        raise GemmQ4Error(1, "one to eight tensors")
+    index = _index(xs[0], "x")
+    dtype, dim = xs[0].dtype, xs[0].shape[-1]
+    rows = xs[0].shape[0] if rows is None else rows
+    if rows <= 0:
+        raise GemmQ4Error(1, "rows must be positive")
+    weights = [None] * len(xs) if weights is None else list(weights)
+    if len(weights) != len(xs) or (outs is not None and len(outs) != len(xs)):
+        raise GemmQ4Error(1, "a weight and an output for each tensor")
+    code = _dtype_code(dtype)
+    parts = [_head_vectors(x, rows, None, dim, dtype, index, "x") for x in xs]
+    freq, rotary = _frequencies(frequencies, index)
+    with _launch(index):
+        if outs is None:
+            with _allocating(stream):
+                outs = [torch.empty((rows, x.shape[1], dim), dtype=torch.bfloat16, device=x.device) for x in xs]
+        cs = (_lib.Heads * len(xs))(*[
+            _lib.Heads(*p, _norm_weight(w, dim, index, "weight"), *_dense_heads(o, rows, p[3], dim, index, "output"))
+            for p, w, o in zip(parts, weights, outs)])
+        st = _lib.lib().splosh_rotate_heads(cs, len(xs), code, rows, dim,
+                                            _vector(positions, rows, torch.int32, index, "positions"), freq, rotary, eps,
+                                            _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
+    return outs
+
+
+def cache_write(cache, packed, k, v, q=None, frequencies=None, k_weight=None, q_weight=None, eps=1e-6, out=None, rows=None,
+                stream=None):
+    """splosh_cache_write: a step's keys (normed by ``k_weight``, turned by their rows' positions; neither where that is
+    None) and values, [rows, cache.heads, dim] fp32 or bf16, into the cache at the places of ``packed``. With ``q``
+    [rows, heads, dim] also the step's queries normed and turned, in the same launch: returned as bf16 (``out``)."""
+    index = cache.index
+    _same_device(packed.table, index, "table")
+    rows = k.shape[0] if rows is None else rows
+    if rows <= 0:
+        raise GemmQ4Error(1, "rows must be positive")
+    dim, dtype = cache.dim, k.dtype
+    code = _dtype_code(dtype)
+    kc = _lib.Heads(*_head_vectors(k, rows, cache.heads, dim, dtype, index, "k"), _norm_weight(k_weight, dim, index, "k_weight"))
+    vc = _lib.Heads(*_head_vectors(v, rows, cache.heads, dim, dtype, index, "v"))
+    freq, rotary = _frequencies(frequencies, index)
+    qc = None
+    with _launch(index):
+        if q is not None:
+            part = _head_vectors(q, rows, None, dim, dtype, index, "q")
+            if out is None:
+                with _allocating(stream):
+                    out = torch.empty((rows, q.shape[1], dim), dtype=torch.bfloat16, device=q.device)
+            qc = _lib.Heads(*part, _norm_weight(q_weight, dim, index, "q_weight"),
+                            *_dense_heads(out, rows, part[3], dim, index, "output"))
+        st = _lib.lib().splosh_cache_write(cache._c, packed._c, kc, vc, qc, code, rows, freq, rotary, eps,
+                                           _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
+    return out if q is not None else None
+
+
+def cache_read(cache, packed, rows=None, k=None, v=None, stream=None):
+    """splosh_cache_read: what the cache holds at the places of ``packed``'s rows, as bf16 (k, v) [rows, heads, dim]. Of a
+    request with n rows these are its last n tokens. rows: that of k or v where they are given."""
+    index = cache.index
+    _same_device(packed.table, index, "table")
+    if rows is None:
+        if k is None and v is None:
+            raise GemmQ4Error(1, "rows or an output is needed")
+        rows = (k if k is not None else v).shape[0]
+    if rows <= 0:
+        raise GemmQ4Error(1, "rows must be positive")
+    with _launch(index):
+        if k is None and v is None:
+            with _allocating(stream):
+                k, v = (torch.empty((rows, cache.heads, cache.dim), dtype=torch.bfloat16, device=cache.data.device) for _ in "kv")
+        places = [(None, 0) if t is None else _dense_heads(t, rows, cache.heads, cache.dim, index, n) for t, n in ((k, "k"), (v, "v"))]
+        st = _lib.lib().splosh_cache_read(cache._c, packed._c, rows, *places[0], *places[1], _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
+    return k, v
+
+
+def attend_workspace_bytes(cache, packed, rows, q_heads, shared=0):
+    """splosh_attend_workspace_bytes: the scratch an attention call needs (0: not a valid shape)."""
+    with _launch(cache.index):
+        return _lib.lib().splosh_attend_workspace_bytes(cache._c, packed._c, rows, q_heads, shared)
+
+
+def attend(q, cache, packed, shared=0, scale=None, out=None, rows=None, stream=None, workspace=None):
+    """splosh_attend: causal attention of a step's queries (bf16 [rows, heads, dim], strided as they are) over the cache,
+    which holds the step's own keys and values already. shared: the first tokens (whole pages) that all requests have in
+    common, read once for all through request 0's pages. scale None: dim ** -0.5. Returns bf16 [rows, heads, dim] with
+    dense rows, the out projection's activation."""
+    index = cache.index
+    _same_device(packed.table, index, "table")
+    rows = q.shape[0] if rows is None else rows
+    if rows <= 0:
+        raise GemmQ4Error(1, "rows must be positive")
+    dim = cache.dim
+    part = _head_vectors(q, rows, None, dim, torch.bfloat16, index, "q")
+    lib = _lib.lib()
+    with _launch(index):
+        if out is None or workspace is None:
+            with _allocating(stream):
+                out = torch.empty((rows, part[3], dim), dtype=torch.bfloat16, device=q.device) if out is None else out
+                if workspace is None:
+                    need = lib.splosh_attend_workspace_bytes(cache._c, packed._c, rows, part[3], shared)
+                    workspace = torch.empty(max(1, need), dtype=torch.uint8, device=q.device)
+        st = lib.splosh_attend(*part, cache._c, packed._c, rows, shared, dim ** -0.5 if scale is None else scale,
+                               *_dense_heads(out, rows, part[3], dim, index, "output"),
+                               *_given_workspace(workspace, index), _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
+    return out
+
+
+def verify_workspace_bytes(rows, vocab, requests):
+    """splosh_verify_workspace_bytes: the scratch a verification needs (0: not a valid shape)."""
+    return _lib.lib().splosh_verify_workspace_bytes(rows, vocab, requests)
+
+
+def verify(logits, tokens, starts, uniforms, temperature=None, draft=None, out=None, accepted=None, stream=None,
+           workspace=None):
+    """splosh_verify: the drafted tokens of a verify step against the target's logits (fp32 or bf16 [rows, vocab]).
+    ``tokens`` int32 [rows], the ids that the step embedded; ``starts`` int32 [requests + 1]; ``uniforms`` fp32 [rows];
+    ``temperature`` fp32 [requests] (None: 1); ``draft`` the draft's probabilities [rows, vocab] by the row that judges the
+    token (fp32 or bf16; None: drafted by a lookup or greedily). Returns (out int32 [rows], accepted int32 [requests]): from starts[r]
+    on the accepted tokens of request r and the new one, then -1."""
+    index = _index(logits, "logits")
+    ptr = _matrix(logits, 0, 0, index, "logits")
+    rows, vocab = logits.shape
+    requests = starts.numel() - 1
+    if rows == 0 or vocab == 0 or requests < 1:
+        raise GemmQ4Error(1, "rows, vocab and requests must be positive")
+    f32, i32 = torch.float32, torch.int32
+    inputs = (_vector(tokens, rows, i32, index, "tokens"), _vector(starts, requests + 1, i32, index, "starts"), requests,
+              _vector(uniforms, rows, f32, index, "uniforms"), _vector(temperature, requests, f32, index, "temperature"))
+    judged = (None, 0, 0) if draft is None else (_matrix(draft, rows, vocab, index, "draft"), _row_stride(draft), _dtype_code(draft.dtype))
+    code, lib = _dtype_code(logits.dtype), _lib.lib()
+    with _launch(index):
+        if out is None or accepted is None or workspace is None:
+            with _allocating(stream):
+                out = torch.empty(rows, dtype=i32, device=logits.device) if out is None else out
+                accepted = torch.empty(requests, dtype=i32, device=logits.device) if accepted is None else accepted
+                if workspace is None:
+                    workspace = torch.empty(max(1, lib.splosh_verify_workspace_bytes(rows, vocab, requests)), dtype=torch.uint8,
+                                            device=logits.device)
+        st = lib.splosh_verify(ptr, _row_stride(logits), code, rows, vocab, *inputs, *judged,
+                               _vector(out, rows, i32, index, "out"), _vector(accepted, requests, i32, index, "accepted"),
+                               *_given_workspace(workspace, index), _raw_stream(stream, index))
+    if st:
+        _lib.check(st)
+    return out, accepted
