@@ -520,8 +520,8 @@ typedef struct splosh_packed {
 /* Keys and values of one layer in 8 bits, in pages of page_tokens tokens (a multiple of 32) for all
  * `heads` key/value heads of dim 64, 128 or 256. Page i starts at data + i page_stride, page_stride >=
  * splosh_cache_page_bytes(heads, dim, page_tokens) and a multiple of 16, data 16-byte aligned. A page holds for each
- * head and each 32 tokens one record of 64 dim + 256 bytes: the int8 codes of the keys [32][dim], of the
- * values [32][dim], the fp32 scales of the keys [32] and of the values [32]. A vector x is kept as
+ * head and each 32 tokens one record of 64 dim + 256 bytes: the codes of the keys [32][dim], of the
+ * values [32][dim] (a byte each, code + 128), the fp32 scales of the keys [32] and of the values [32]. A vector x is kept as
  * code_i = rint(127 x_i / max|x|) and scale = max|x| / 127 and stands for code_i scale; where max|x| / 127 is below
  * 2^-100, with that as the scale. One with an infinite or NaN element is kept as codes 0 and scale NaN, and
  * stands for NaN. */

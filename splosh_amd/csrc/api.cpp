@@ -1407,7 +1407,7 @@ size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_pac
                                      int64_t q_heads, int64_t shared) {
     if (!cache || !packed || !splosh_cache_page_bytes(cache->heads, cache->dim, cache->page_tokens) || rows <= 0 ||
         rows > kMaxStepRows || q_heads <= 0 || q_heads > kMaxCacheHeads || q_heads % cache->heads != 0 || shared < 0 ||
-        packed->requests <= 0 || packed->requests > SPLOSH_MAX_REQUESTS)
+        packed->requests <= 0 || packed->requests > SPLOSH_MAX_REQUESTS || rows * q_heads >= (int64_t)1 << 30)
         return 0;
     return splosh::attend_workspace_bytes(*cache, packed->requests, rows, q_heads, shared);
 }
@@ -1421,6 +1421,7 @@ int splosh_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, in
     if ((st = check_heads(part, SPLOSH_BF16, rows, cache->dim, true))) return st;
     if (q_heads % cache->heads != 0)
         return fail(SPLOSH_ERR_INVALID_SHAPE, "q_heads must be a multiple of the cache's heads");
+    if (rows * q_heads >= (int64_t)1 << 30) return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows and heads for one launch");
     if (shared < 0 || shared % cache->page_tokens != 0 || shared / cache->page_tokens > packed->table_pages)
         return fail(SPLOSH_ERR_INVALID_SHAPE, "shared must be whole pages of the table");
     if (!(scale > 0.0f) || scale > 3.0e38f) return fail(SPLOSH_ERR_INVALID_SHAPE, "scale must be positive and finite");

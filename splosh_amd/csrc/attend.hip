@@ -1,66 +1,859 @@
 // attend.hip -- causal attention of a packed step's rows over the 8-bit paged cache.
 //
-// A wave takes one (row, query head): its lanes hold dim / 64 dimensions each and go through the keys one after the
-// other with the running maximum and sum of the softmax.
-#include "cache.hpp"
+// With s_j = q . code(k_j), ks_j and vs_j the scales of key and value j, and t_j = s_j ks_j scale log2(e) + log2(vs_j):
+//     a_j = 2^(t_j - M),   out = sum_j a_j code(v_j) / sum_j (a_j / vs_j),
+// M a running maximum of t. The scale of v_j goes into its weight's exponent, so that a_j is what v_j's codes are
+// multiplied with, and lies in [0, 2^8] whatever the scales are: fp16 holds it to 2^-11, and of what is too small for
+// it nothing but 2^-25 of the largest is lost. Codes are whole numbers up to 127 and exact in fp16; so are the values of
+// a row of q, moved by the power of two that brings its largest to 2^14 (what is below 2^-28 of that is cut at 2^-39 of it).
+// Both products run on the fp16 matrix instructions with fp32 sums.
+//
+// Scores are computed transposed, keys by queries: a lane then holds four consecutive keys of one query, and their
+// weights are, as they are, its operand of the second product (values' dimensions by queries), whose order of keys is
+// free as long as both operands have the same. Nothing but sums over the lanes of a query crosses lanes.
+//
+// Two kernels share the work out as attend_plan.hpp says. `few` (up to 64 vectors of a request and key/value head): bound by the
+// cache's bytes. Each of a workgroup's four waves goes through blocks of 32 keys of its own for all vectors, straight
+// from memory to registers; they are joined at the end. `many`: bound by the matrix instructions. Eight waves hold 32
+// vectors each, and go together through blocks that are widened to fp16 once, in LDS.
+#include <climits>
+#include <type_traits>
+
+#include "attend_plan.hpp"
 
 namespace splosh {
 
-constexpr int kAttendThreads = 256;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr size_t kAttendCounterBytes = 16384;  // the workspace's first bytes belong to other kernels' counters
+constexpr float kLowest = -1e30f;              // M before the first key
+constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
+constexpr int kFewThreads = 256, kFewWaves = 4, kManyThreads = 512, kManyRows = 256;
+constexpr int kFewKeys = kFewWaves * kBlock, kManyKeys = 2 * kBlock;  // of a unit
 
 struct AttendArgs {
     const uint16_t *q;
     int64_t row_stride, head_stride;
     uint16_t *out;
     int64_t ld_out;
-    int q_heads, group, shared;
-    float scale;
+    int q_heads, shared, wide;  // wide: 16-byte aligned vectors of q
+    float factor;               // scale log2(e)
+    TileShape tile;
+    int prefix;                 // the launch over the shared prefix
+    int partial;                // whether every piece leaves its partial result
+    float *slots;
+    int64_t segment_slots;
+    int64_t *units;             // the requests' first units, and the total
+    int64_t *segments;          // and first segments
 };
 
-template <int D>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, CacheView cache, PackedView packed) {
-    constexpr int E = D / 64;
-    const int row = blockIdx.x, lane = threadIdx.x & 63;
-    const int r = request_of(packed.starts, packed.requests, row);
-    if (r < 0) return;
-    const int position = packed.lengths[r] - packed.starts[r + 1] + row;
-    for (int h = threadIdx.x >> 6; h < a.q_heads; h += kAttendThreads / 64) {
-        float q[E], o[E] = {}, most = -__builtin_inff(), sum = 0.0f;
-        for (int e = 0; e < E; ++e)
-            q[e] = bf16_bits_to_f32(a.q[row * a.row_stride + h * a.head_stride + lane * E + e]);
-        for (int j = 0; j <= position; ++j) {
-            int page, at;
-            if (!place_of(cache, packed, j < a.shared ? 0 : r, j, page, at)) continue;
-            const uint8_t *record = record_of<D>(cache, page, h / a.group, at / kBlock);
-            const int8_t *k = reinterpret_cast<const int8_t *>(record) + at % kBlock * D + lane * E, *v = k + kBlock * D;
-            const float *scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + at % kBlock;
-            float s = 0.0f;
-            for (int e = 0; e < E; ++e) s += q[e] * (float)k[e];
+// Where a piece's vectors and keys lie.
+struct Piece {
+    Span span;
+    int request, head, tile;
+    int first_block, blocks;  // of 32 keys, from the span's first on
+    int64_t slot;
+    bool direct;              // the whole segment, and nothing to join it with
+};
+
+// Four codes, kept as code + 128, as fp16: 1024 + byte is 0x6400 | byte.
+__device__ __forceinline__ f16x2 as_f16x2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
+__device__ __forceinline__ f16x2 centred(uint32_t v) { return as_f16x2(v) - f16x2{(_Float16)1152, (_Float16)1152}; }
+__device__ __forceinline__ void widen4(uint32_t codes, f16x2 &lo, f16x2 &hi) {
+    lo = centred(perm_bytes(0x64646464u, codes, 0x04010400u));
+    hi = centred(perm_bytes(0x64646464u, codes, 0x04030402u));
+}
+__device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
+    return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4,
+                                   5, 6, 7);
+}
+__device__ __forceinline__ f16x8 widen8(uint32_t lo, uint32_t hi) {
+    f16x2 a, b, c, d;
+    widen4(lo, a, b);
+    widen4(hi, c, d);
+    return join8(a, b, c, d);
+}
+// Four dimensions of eight tokens, transposed: part[c] is dimension c of tokens 0..7.
+__device__ __forceinline__ void widen_turned(const uint32_t (&v)[8], f16x8 (&part)[4]) {
+    f16x2 of[4][4];
 #pragma unroll
-            for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m);
-            s = s * scales[0] * a.scale * 1.4426950408889634f;
-            const float top = __builtin_fmaxf(most, s), keep = exp2f(most - top), w = exp2f(s - top);
-            most = top;
-            sum = sum * keep + w;
-            for (int e = 0; e < E; ++e) o[e] = o[e] * keep + w * scales[kBlock] * (float)v[e];
+    for (int p = 0; p < 4; ++p) {
+        const uint32_t low = perm_bytes(v[2 * p + 1], v[2 * p], 0x05040100u), high = perm_bytes(v[2 * p + 1], v[2 * p], 0x07060302u);
+        of[0][p] = centred(perm_bytes(0x64646464u, low, 0x04020400u));
+        of[1][p] = centred(perm_bytes(0x64646464u, low, 0x04030401u));
+        of[2][p] = centred(perm_bytes(0x64646464u, high, 0x04020400u));
+        of[3][p] = centred(perm_bytes(0x64646464u, high, 0x04030401u));
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) part[c] = join8(of[c][0], of[c][1], of[c][2], of[c][3]);
+}
+
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
+// Eight values of q.
+__device__ __forceinline__ void load_q8(const uint16_t *at, int wide, float *v) {
+    uint32_t w[4];
+    if (wide) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = at[2 * e] | (uint32_t)at[2 * e + 1] << 16;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = bf16_bits_to_f32(w[e]), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+}
+// The power that brings a row's largest value to [2^14, 2^15).
+__device__ __forceinline__ int power_of(float most) { return 141 - (int)(__float_as_uint(most) >> 23); }
+__device__ __forceinline__ u32x4 moved8(const float *v, int power) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = f16_pair(__builtin_ldexpf(v[2 * e], power), __builtin_ldexpf(v[2 * e + 1], power));
+    return w;
+}
+
+// What the sum of a_j is divided by, for the scale of v_j. (1 where it is no scale: t is then NaN, or the key masked.)
+__device__ __forceinline__ float inverse_scale(float vs) {
+    const float r = __builtin_amdgcn_rcpf(vs);
+    return __builtin_fabsf(r) < __builtin_inff() ? r : 1.0f;
+}
+
+// The packed row that vector x of a tile's request is of.
+__device__ __forceinline__ int row_of(const Piece &p, int group, int x) { return p.span.begin + x / group; }
+
+// The last key that packed row `row` sees, of the launch's.
+__device__ __forceinline__ int position_of(const AttendArgs &a, const PackedView &packed, const Piece &p, int row) {
+    if (!a.prefix) return p.span.first + row - p.span.begin;
+    int low = 0, high = packed.requests;  // the last request that starts at or before the row
+    while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (packed.starts[mid] <= row) low = mid;
+        else high = mid;
+    }
+    return packed.lengths[low] - packed.starts[low + 1] + row;
+}
+
+// The page ids of a request, 64 columns at a time in a wave's lanes.
+struct Pages {
+    const int32_t *table;
+    int columns, base, ids;
+    __device__ __forceinline__ Pages(const PackedView &p, int request)
+        : table(p.table + request * p.table_stride), columns(p.table_pages), base(-64), ids(-1) {}
+    __device__ __forceinline__ int operator()(int column) {
+        if (column < base || column >= base + 64) {
+            base = column;
+            const int c = base + (int)(threadIdx.x & 63);
+            ids = c < columns ? table[c] : -1;
         }
-        for (int e = 0; e < E; ++e)
-            a.out[row * a.ld_out + h * D + lane * E + e] = f32_to_bf16(sum == 0.0f ? 0.0f : o[e] / sum);
+        return __builtin_amdgcn_readlane(ids, column - base);
+    }
+};
+
+// The record of a block of the request's keys; `hole`: it lies in no page (some record is given all the same).
+template <int D>
+__device__ __forceinline__ const uint8_t *block_record(const CacheView &cache, Pages &pages, int head, int block, bool &hole) {
+    const int column = block / cache.page_blocks;
+    int page = pages(column);
+    hole = page < 0 || page >= cache.pages;
+    page = hole ? 0 : page;
+    return record_of<D>(cache, page, head, block - column * cache.page_blocks);
+}
+
+// Calls `work` for each piece of the launch's units that workgroup blockIdx.x takes. All threads call it; scratch: a
+// word for each of a few more than the workgroup's threads.
+template <int THREADS, typename F>
+__device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView &cache, const PackedView &packed, F work) {
+    const TileShape &tile = a.tile;
+    const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int request = 0;
+    int64_t total, before = 0, segment = 0;
+    Span span;
+    if (a.prefix) {
+        span = prefix_span(packed, a.shared);
+        total = tile.heads * units_before(span, tile, tiles_of(span, tile));
+    } else {
+        // The units and segments before each request: a run of requests a thread, summed over the threads.
+        __shared__ int64_t wave_units[THREADS / 64], wave_segments[THREADS / 64], found_before, found_segment;
+        __shared__ int found;
+        const int run = (packed.requests + THREADS - 1) / THREADS;
+        const int low = min(tid * run, packed.requests), high = min(low + run, packed.requests);
+        auto units_of = [&](int r, int64_t &units, int &segments) {
+            const Span s = own_span(packed, cache.page_tokens, a.shared, r);
+            const int tiles = tiles_of(s, tile);
+            units = tile.heads * units_before(s, tile, tiles);
+            segments = tile.heads * tiles;
+        };
+        int64_t units = 0, segments = 0, u;
+        int n;
+        for (int r = low; r < high; ++r) units_of(r, u, n), units += u, segments += n;
+        int64_t units_to = units, segments_to = segments;  // own ones included
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int64_t x = __shfl_up(units_to, m), y = __shfl_up(segments_to, m);
+            if (lane >= m) units_to += x, segments_to += y;
+        }
+        if (lane == 63) wave_units[wave] = units_to, wave_segments[wave] = segments_to;
+        if (tid == 0) found = -1;
+        __syncthreads();
+        total = 0;
+        for (int i = 0; i < THREADS / 64; ++i) {
+            if (i < wave) units_to += wave_units[i], segments_to += wave_segments[i];
+            total += wave_units[i];
+        }
+        const int sharers = sharers_of(total, tile.workgroups);
+        const int64_t first = w < sharers ? first_unit(total, sharers, w) : total;
+        int64_t at = units_to - units, at_segment = segments_to - segments;
+        const bool mine = at <= first && first < units_to;
+        if (mine || w == 0) {
+            for (int r = low; r < high; ++r) {
+                units_of(r, u, n);
+                if (w == 0) a.units[r] = at, a.segments[r] = at_segment;  // (for the launch that joins the pieces)
+                if (mine && at <= first && first < at + u) found = r, found_before = at, found_segment = at_segment;
+                at += u, at_segment += n;
+            }
+        }
+        if (w == 0 && tid == 0) a.units[packed.requests] = total;
+        __syncthreads();
+        if (found < 0) return;
+        request = found, before = found_before, segment = found_segment;
+        span = own_span(packed, cache.page_tokens, a.shared, request);
+    }
+    const int sharers = sharers_of(total, tile.workgroups);
+    if (w >= sharers) return;
+    int64_t unit = first_unit(total, sharers, w);
+    const int64_t end = first_unit(total, sharers, w + 1);
+    int tiles = tiles_of(span, tile), head, t = 0, offset;
+    {
+        const int64_t each = units_before(span, tile, tiles);
+        int64_t rest = unit - before;
+        head = (int)(rest / each);
+        rest -= head * each;
+        int units = tile_units(span, tile, 0);
+        while (rest >= units) rest -= units, units = tile_units(span, tile, ++t);
+        offset = (int)rest;
+        segment += head * tiles + t;
+    }
+    while (true) {
+        const int units = tile_units(span, tile, t);
+        const int take = (int)(units - offset < end - unit ? units - offset : end - unit);
+        const int all = tile_end(span, tile, t) - span.from, blocks = all > 0 ? (all + kBlock - 1) / kBlock : 0;
+        const int per = tile.keys / kBlock;
+        Piece p;
+        p.span = span, p.request = request, p.head = head, p.tile = t;
+        p.first_block = offset * per;
+        p.blocks = max(0, min((offset + take) * per, blocks) - p.first_block);
+        p.slot = offset == 0 ? segment : a.segment_slots + w;
+        p.direct = !a.partial && take == units;
+        if (segment < a.segment_slots) work(p);  // (more there are only where starts do not ascend)
+        unit += take;
+        if (unit >= end) return;
+        offset = 0, ++segment;
+        if (++t < tiles) continue;
+        t = 0;
+        if (++head < tile.heads) continue;
+        head = 0;
+        do {  // (there is another one: the units say so)
+            span = own_span(packed, cache.page_tokens, a.shared, ++request);
+            tiles = tiles_of(span, tile);
+        } while (tiles == 0 && request + 1 < packed.requests);
     }
 }
 
-size_t attend_workspace_bytes(const splosh_cache &, int64_t, int64_t, int64_t, int64_t) { return 16384; }
+// The result of vector x, dimensions d .. d + N - 1 of N sums o with maximum M: written, or left in the piece's slot.
+template <int D, int N>
+__device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, int i, int d, const float *o, float total) {
+    if (p.direct) {
+        const int x = p.tile * a.tile.rows + i;
+        if (x >= p.span.n * a.tile.group) return;
+        const int row = row_of(p, a.tile.group, x), h = p.head * a.tile.group + x % a.tile.group;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        uint16_t *at = a.out + row * a.ld_out + (int64_t)h * D + d;
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const uint32_t pair = total == 0.0f ? 0u : f32x2_to_bf16x2(o[e] * inv, o[e + 1] * inv);
+            at[e] = (uint16_t)pair, at[e + 1] = (uint16_t)(pair >> 16);
+        }
+    } else {
+        float *at = a.slots + p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)i * D + d;
+#pragma unroll
+        for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4 *>(at + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+    }
+}
+// And its maximum and sum, where they are left.
+template <int D>
+__device__ __forceinline__ void write_total(const AttendArgs &a, const Piece &p, int i, float most, float total) {
+    if (p.direct) return;
+    float *at = a.slots + p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)a.tile.rows * D;
+    at[i] = most, at[a.tile.rows + i] = total;
+}
+
+// ---- few vectors --------------------------------------------------------------------------------
+
+template <int D, int NT>
+__global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, CacheView cache, PackedView packed) {
+    constexpr int R = 16 * NT, SLABS = D / 64, STEPS = D / 32, TILES = D / 16, CHUNKS = D / 16, PITCH = D + 4;
+    __shared__ __align__(16) u32x4 q_parts[NT * STEPS * 64];
+    __shared__ __align__(16) float joined[kFewWaves][16 * PITCH];
+    __shared__ float wave_most[kFewWaves][R], wave_total[kFewWaves][R], row_factor[R];
+    __shared__ int row_position[R], least;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+
+    for_pieces<kFewThreads>(a, cache, packed, [&](const Piece &p) {
+        const int group = a.tile.group, vectors = p.span.n * group;
+        __syncthreads();  // (the last piece's LDS is read)
+        if (tid == 0) least = INT_MAX;
+        __syncthreads();
+        // The tile's queries as the first product's operand: 16 dimensions of a vector a thread.
+        for (int item = tid; item < R * CHUNKS; item += kFewThreads) {
+            const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
+            const bool valid = x < vectors;
+            const int row = valid ? row_of(p, group, x) : 0;
+            float v[16] = {}, most = 0.0f;
+            if (valid) {
+                const uint16_t *at = a.q + row * a.row_stride + (p.head * group + x % group) * a.head_stride + c * 16;
+                load_q8(at, a.wide, v);
+                load_q8(at + 8, a.wide, v + 8);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
+#pragma unroll
+            for (int m = 1; m < CHUNKS; m <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, m));
+            const int power = power_of(most);
+            u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
+            to[0] = moved8(v, power);
+            to[64] = moved8(v + 8, power);
+            if (c == 0) {
+                row_factor[i] = __builtin_ldexpf(a.factor, -power);
+                row_position[i] = valid ? position_of(a, packed, p, row) : -1;
+                if (valid) atomicMin(&least, row_position[i]);
+            }
+        }
+        __syncthreads();
+        float factor[NT], most[NT], total[NT];
+        int position[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            factor[n] = row_factor[n * 16 + col], position[n] = row_position[n * 16 + col];
+            most[n] = kLowest, total[n] = 0.0f;
+        }
+        const int first_position = least;
+        f32x4 acc[TILES][NT] = {};
+        Pages pages(packed, a.prefix ? 0 : p.request);
+        const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
+
+        u32x4 k[2][SLABS];
+        uint32_t v[8][SLABS];
+        f32x4 ks[2], vs[2];
+        bool hole = false;
+        auto load_keys = [&](const uint8_t *record) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s = 0; s < SLABS; ++s)
+                    k[t][s] = *reinterpret_cast<const u32x4 *>(record + (t * 16 + col) * D + s * 64 + g * 16);
+            const float *scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + 4 * g;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                ks[t] = *reinterpret_cast<const f32x4 *>(scales + 16 * t);
+                vs[t] = *reinterpret_cast<const f32x4 *>(scales + kBlock + 16 * t);
+            }
+        };
+        auto load_values = [&](const uint8_t *record) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint8_t *at = record + (kBlock + (e / 4) * 16 + 4 * g + e % 4) * D + col * (D / 16);
+                if constexpr (SLABS == 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) v[e][s] = x[s];
+                } else if constexpr (SLABS == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                    v[e][0] = x[0], v[e][1] = x[1];
+                } else {
+                    v[e][0] = *reinterpret_cast<const uint32_t *>(at);
+                }
+            }
+        };
+        if (from + wave < to) {
+            const uint8_t *record = block_record<D>(cache, pages, p.head, from + wave, hole);
+            load_keys(record);
+            load_values(record);
+        }
+        for (int block = from + wave; block < to; block += kFewWaves) {
+            const bool more = block + kFewWaves < to, dead = hole;
+            const uint8_t *next = nullptr;
+            if (more) next = block_record<D>(cache, pages, p.head, block + kFewWaves, hole);
+            f32x4 s[2][NT] = {};
+#pragma unroll
+            for (int slab = 0; slab < SLABS; ++slab)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const f16x8 k0 = widen8(k[0][slab][2 * half], k[0][slab][2 * half + 1]);
+                    const f16x8 k1 = widen8(k[1][slab][2 * half], k[1][slab][2 * half + 1]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const f16x8 q = __builtin_bit_cast(f16x8, q_parts[(n * STEPS + slab * 2 + half) * 64 + lane]);
+                        s[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q, s[0][n], 0, 0, 0);
+                        s[1][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q, s[1][n], 0, 0, 0);
+                    }
+                }
+            float key_scale[8], value_log[8], inverse[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                key_scale[e] = ks[e / 4][e % 4];
+                value_log[e] = __builtin_amdgcn_logf(vs[e / 4][e % 4]);
+                inverse[e] = inverse_scale(vs[e / 4][e % 4]);
+            }
+            if (more) load_keys(next);
+            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
+            f16x8 weight[NT];
+            float t[NT][8];
+            bool follow = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    t[n][e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
+                    if (masked)
+                        t[n][e] = !dead && block * kBlock + (e / 4) * 16 + 4 * g + e % 4 <= position[n] ? t[n][e] : -__builtin_inff();
+                    top = __builtin_fmaxf(top, t[n][e]);
+                }
+                top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+                top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                wave_most[wave][n * 16 + col] = top;  // (kept there while `follow` is found out)
+                follow |= top > most[n] + kSlack;
+            }
+            if (__any(follow)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float top = __builtin_fmaxf(most[n], wave_most[wave][n * 16 + col]);
+                    const float keep = __builtin_amdgcn_exp2f(most[n] - top);
+                    most[n] = top;
+                    total[n] *= keep;
+#pragma unroll
+                    for (int j = 0; j < TILES; ++j) acc[j][n] *= keep;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(t[n][e] - most[n]);
+                    total[n] = __builtin_fmaf(w[e], inverse[e], total[n]);
+                }
+                const u32x4 pairs = {f16_pair(w[0], w[1]), f16_pair(w[2], w[3]), f16_pair(w[4], w[5]), f16_pair(w[6], w[7])};
+                weight[n] = __builtin_bit_cast(f16x8, pairs);
+            }
+#pragma unroll
+            for (int slab = 0; slab < SLABS; ++slab) {
+                uint32_t of[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) of[e] = v[e][slab];
+                f16x8 part[4];
+                widen_turned(of, part);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[slab * 4 + c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[c], weight[n], acc[slab * 4 + c][n], 0, 0, 0);
+            }
+            if (more) load_values(next);
+        }
+        // The four waves' sums against the largest of their maxima, added in their order.
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            total[n] += __shfl_xor(total[n], 16);
+            total[n] += __shfl_xor(total[n], 32);
+            if (g == 0) wave_most[wave][n * 16 + col] = most[n], wave_total[wave][n * 16 + col] = total[n];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float top = kLowest;
+#pragma unroll
+            for (int w = 0; w < kFewWaves; ++w) top = __builtin_fmaxf(top, wave_most[w][n * 16 + col]);
+            const float keep = __builtin_amdgcn_exp2f(most[n] - top);
+            if (n) __syncthreads();  // (the last sixteen vectors are read)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < TILES; j += 4)
+                    *reinterpret_cast<f32x4 *>(&joined[wave][col * PITCH + (4 * g + e) * TILES + j]) =
+                        f32x4{acc[j][n][e] * keep, acc[j + 1][n][e] * keep, acc[j + 2][n][e] * keep, acc[j + 3][n][e] * keep};
+            __syncthreads();
+            const int i = tid / 16, d = tid % 16 * (D / 16);
+            float sum[D / 16], row_total = 0.0f, row_most = kLowest;
+#pragma unroll
+            for (int e = 0; e < D / 16; ++e) sum[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kFewWaves; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w][n * 16 + i]);
+#pragma unroll
+            for (int w = 0; w < kFewWaves; ++w) {
+                row_total += wave_total[w][n * 16 + i] * __builtin_amdgcn_exp2f(wave_most[w][n * 16 + i] - row_most);
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) sum[e] += joined[w][i * PITCH + d + e];
+            }
+            write_sums<D, D / 16>(a, p, n * 16 + i, d, sum, row_total);
+            if (tid % 16 == 0) write_total<D>(a, p, n * 16 + i, row_most, row_total);
+        }
+    });
+}
+
+// ---- many vectors -------------------------------------------------------------------------------
+
+template <int D>
+__global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheView cache, PackedView packed) {
+    constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = 1024 + 64;  // (the pitch spreads a quad's writes over the banks)
+    constexpr int K_ITEMS = 2 * D / 256 > 0 ? 2 * D / 256 : 1;
+    __shared__ __align__(16) uint8_t key_parts[2][STEPS * K_PITCH];
+    __shared__ __align__(16) u32x4 value_parts[2][TILES * 2 * 64];
+    __shared__ __align__(16) float scales[2][3][kBlock];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, g = lane >> 5;
+
+    for_pieces<kManyThreads>(a, cache, packed, [&](const Piece &p) {
+        const int group = a.tile.group, vectors = p.span.n * group;
+        const int x = p.tile * kManyRows + wave * 32 + col;
+        const bool valid = x < vectors;
+        const int row = valid ? row_of(p, group, x) : 0;
+        const int position = valid ? position_of(a, packed, p, row) : INT_MAX;
+        int first_position = position;  // of the wave's vectors
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) first_position = min(first_position, __shfl_xor(first_position, m));
+        // The lane's vector, half of its dimensions.
+        f16x8 q[STEPS];
+        float factor;
+        {
+            float most = 0.0f;
+            const uint16_t *at = a.q + row * a.row_stride + (p.head * group + (valid ? x % group : 0)) * a.head_stride + g * 8;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                float v[8];
+                load_q8(at + 16 * s, a.wide, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
+            }
+            most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+            const int power = power_of(most);
+            factor = __builtin_ldexpf(a.factor, -power);
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                float v[8];
+                load_q8(at + 16 * s, a.wide, v);
+                q[s] = __builtin_bit_cast(f16x8, moved8(v, power));
+            }
+        }
+        f32x16 acc[TILES] = {};
+        float most = kLowest, total = 0.0f;
+        Pages pages(packed, a.prefix ? 0 : p.request);
+        const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
+
+        // Staging: threads 0..D-1 four dimensions of eight values each, the last 256 threads runs of 16 bytes of keys.
+        const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
+        const bool stages_values = tid < D, stages_keys = tid >= 256;
+        uint32_t raw_v[8] = {};
+        u32x4 raw_k[K_ITEMS] = {};
+        float raw_scale = 0.0f;
+        bool hole = false;
+        auto fetch = [&](int block) {
+            const uint8_t *record = block_record<D>(cache, pages, p.head, block, hole);
+            if (stages_values) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    raw_v[e] = *reinterpret_cast<const uint32_t *>(
+                        record + (kBlock + 16 * value_step + (e / 4) * 8 + 4 * value_g + e % 4) * D + quad * 4);
+            }
+            if (stages_keys) {
+#pragma unroll
+                for (int n = 0; n < K_ITEMS; ++n) {
+                    const int item = tid - 256 + 256 * n;
+                    if (item < 2 * D)
+                        raw_k[n] = *reinterpret_cast<const u32x4 *>(record + (item / 4 % 32) * D + (item / 128 * 4 + item % 4) * 16);
+                }
+            }
+            if (tid < 2 * kBlock) raw_scale = reinterpret_cast<const float *>(record + 2 * kBlock * D)[tid];
+        };
+        auto stage = [&](int buffer) {
+            if (stages_values) {
+                f16x8 part[4];
+                widen_turned(raw_v, part);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int t = D == 64 ? c >> 1 : quad / 32 * 4 + c, m = D == 64 ? (c & 1) * 16 + quad : quad % 32;
+                    value_parts[buffer][(t * 2 + value_step) * 64 + value_g * 32 + m] = __builtin_bit_cast(u32x4, part[c]);
+                }
+            }
+            if (stages_keys) {
+#pragma unroll
+                for (int n = 0; n < K_ITEMS; ++n) {
+                    const int item = tid - 256 + 256 * n;
+                    if (item < 2 * D) {
+                        uint8_t *at = key_parts[buffer] + (item / 128 * 4 + item % 4) * K_PITCH + (item / 4 % 32) * 16;
+                        *reinterpret_cast<f16x8 *>(at) = widen8(raw_k[n][0], raw_k[n][1]);
+                        *reinterpret_cast<f16x8 *>(at + 512) = widen8(raw_k[n][2], raw_k[n][3]);
+                    }
+                }
+            }
+            if (tid < kBlock) scales[buffer][0][tid] = raw_scale;
+            else if (tid < 2 * kBlock)
+                scales[buffer][1][tid - kBlock] = __builtin_amdgcn_logf(raw_scale), scales[buffer][2][tid - kBlock] = inverse_scale(raw_scale);
+        };
+
+        bool dead = false;
+        __syncthreads();  // (the last piece's LDS is read)
+        if (from < to) {
+            fetch(from);
+            dead = hole;
+            stage(0);
+        }
+        __syncthreads();
+        for (int block = from; block < to; ++block) {
+            const int buffer = (block - from) & 1;
+            if (block + 1 < to) fetch(block + 1);
+            f32x16 s = {};
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                const f16x8 k = *reinterpret_cast<const f16x8 *>(key_parts[buffer] + i * K_PITCH + lane * 16);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], s, 0, 0, 0);
+            }
+            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
+            float t[16], top = -__builtin_inff();
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const f32x4 ks = *reinterpret_cast<const f32x4 *>(&scales[buffer][0][8 * b + 4 * g]);
+                const f32x4 lv = *reinterpret_cast<const f32x4 *>(&scales[buffer][1][8 * b + 4 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[4 * b + e] = __builtin_fmaf(s[4 * b + e], ks[e] * factor, lv[e]);
+            }
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    t[e] = !dead && block * kBlock + e / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, t[e]);
+            top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > most + kSlack)) {
+                top = __builtin_fmaxf(top, most);
+                const float keep = __builtin_amdgcn_exp2f(most - top);
+                most = top;
+                total *= keep;
+#pragma unroll
+                for (int j = 0; j < TILES; ++j) acc[j] *= keep;
+            }
+            uint32_t pairs[8];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const f32x4 inverse = *reinterpret_cast<const f32x4 *>(&scales[buffer][2][8 * b + 4 * g]);
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(t[4 * b + e] - most);
+                    total = __builtin_fmaf(w[e], inverse[e], total);
+                }
+                pairs[2 * b] = f16_pair(w[0], w[1]), pairs[2 * b + 1] = f16_pair(w[2], w[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const u32x4 four = {pairs[4 * i], pairs[4 * i + 1], pairs[4 * i + 2], pairs[4 * i + 3]};
+                const f16x8 weight = __builtin_bit_cast(f16x8, four);
+#pragma unroll
+                for (int j = 0; j < TILES; ++j) {
+                    const f16x8 v = __builtin_bit_cast(f16x8, value_parts[buffer][(j * 2 + i) * 64 + lane]);
+                    acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weight, acc[j], 0, 0, 0);
+                }
+            }
+            if (block + 1 < to) {
+                dead = hole;
+                stage(buffer ^ 1);
+            }
+            __syncthreads();
+        }
+        total += __shfl_xor(total, 32);
+        const int i = wave * 32 + col;
+        if constexpr (D > 64) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < TILES; j += 4) {
+                        const float o[4] = {acc[j][4 * b + e], acc[j + 1][4 * b + e], acc[j + 2][4 * b + e], acc[j + 3][4 * b + e]};
+                        write_sums<D, 4>(a, p, i, 4 * (8 * j + 8 * b + 4 * g + e), o, total);
+                    }
+        } else {
+            // Tile t, row m holds dimension 4 (m % 16) + 2 t + m / 16: rows m and m + 16 of both tiles are four in a row.
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float o[4] = {acc[0][4 * b + e], acc[0][4 * b + 8 + e], acc[1][4 * b + e], acc[1][4 * b + 8 + e]};
+                    write_sums<D, 4>(a, p, i, 4 * (8 * b + 4 * g + e), o, total);
+                }
+        }
+        if (g == 0) write_total<D>(a, p, i, most, total);
+    });
+}
+
+// ---- the pieces joined ----------------------------------------------------------------------------
+
+struct JoinArgs {
+    AttendArgs own, prefix;
+};
+
+// A wave a (row, query head): the weights of its pieces, one a lane, and their sums in the order of the keys.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs a, CacheView cache, PackedView packed) {
+    constexpr int E = D / 64;
+    const AttendArgs &own = a.own;
+    const int64_t vector = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, row = (int)(vector / own.q_heads), h = (int)(vector % own.q_heads);
+    if (row >= packed.rows) return;
+    const int r = request_of(packed.starts, packed.requests, row);
+    if (r < 0) return;
+    float top = kLowest, total = 0.0f, o[E] = {};
+    // The pieces of one segment of a launch; `only`: leave a segment of one piece, which is written already.
+    auto pieces = [&](const AttendArgs &l, const Span &span, int64_t before, int64_t segment, int64_t all, bool only) {
+        const TileShape &tile = l.tile;
+        const int x = (row - span.begin) * tile.group + h % tile.group, t = x / tile.rows, i = x - t * tile.rows, head = h / tile.group;
+        const int tiles = tiles_of(span, tile);
+        if (segment + (int64_t)head * tiles + t >= l.segment_slots) return false;
+        const int64_t start = before + head * units_before(span, tile, tiles) + units_before(span, tile, t);
+        const int sharers = sharers_of(all, tile.workgroups), w0 = owner_of(all, sharers, start);
+        const int count = owner_of(all, sharers, start + tile_units(span, tile, t) - 1) - w0 + 1;
+        if (only && count == 1) return false;
+        const int64_t size = tile.rows * (int64_t)(D + 2);
+        auto slot = [&](int j) { return l.slots + (j == 0 ? segment + (int64_t)head * tiles + t : l.segment_slots + w0 + j) * size; };
+        for (int base = 0; base < count; base += 64) {
+            const int j = base + lane;
+            float most = kLowest, sum = 0.0f;
+            if (j < count) {
+                const float *at = slot(j) + (int64_t)tile.rows * D + i;
+                most = at[0], sum = at[tile.rows];
+            }
+            float now = __builtin_fmaxf(top, most);
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) now = __builtin_fmaxf(now, __shfl_xor(now, m));
+            const float keep = __builtin_amdgcn_exp2f(top - now), weight = __builtin_amdgcn_exp2f(most - now);
+            top = now;
+            total *= keep;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= keep;
+            sum *= weight;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+            total += sum;
+            const int here = min(64, count - base);
+#pragma unroll 4
+            for (int j2 = 0; j2 < here; ++j2) {
+                const float w = __shfl(weight, j2);
+                const float *at = slot(base + j2) + (int64_t)i * D + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += w * at[e];
+            }
+        }
+        return true;
+    };
+    if (own.partial) {
+        const Span span = prefix_span(packed, own.shared);
+        const TileShape &tile = a.prefix.tile;
+        pieces(a.prefix, span, 0, 0, tile.heads * units_before(span, tile, tiles_of(span, tile)), false);
+    }
+    if (!pieces(own, own_span(packed, cache.page_tokens, own.shared, r), own.units[r], own.segments[r], own.units[packed.requests], !own.partial))
+        return;
+    uint16_t *at = own.out + row * own.ld_out + (int64_t)h * D + lane * E;
+    const float inv = 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < E; ++e) at[e] = total == 0.0f ? 0 : f32_to_bf16(o[e] * inv);
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+
+struct AttendPlan {
+    bool few;
+    TileShape tile;
+    int64_t segment_slots;
+    size_t slot_bytes() const { return (size_t)((segment_slots + tile.workgroups) * tile.rows); }  // times (dim + 2) floats
+};
+
+// `vectors`: those of a request and key/value head, on average.
+static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, int64_t q_heads, const splosh_cache &cache) {
+    AttendPlan p;
+    const int cus = device_cus();
+    p.few = vectors <= 64;
+    const int nt = (int)((vectors + 15) / 16);
+    p.tile.rows = p.few ? 16 * nt : kManyRows;
+    p.tile.keys = p.few ? kFewKeys : kManyKeys;
+    p.tile.group = (int)(q_heads / cache.heads);
+    p.tile.heads = (int)cache.heads;
+    p.tile.workgroups = p.few && nt == 1 ? 2 * cus : cus;
+    p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
+    return p;
+}
+static AttendPlan plan_own(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads) {
+    return plan_launch((rows + requests - 1) / requests * (q_heads / cache.heads), requests, rows, q_heads, cache);
+}
+static AttendPlan plan_prefix(const splosh_cache &cache, int64_t rows, int64_t q_heads) {
+    return plan_launch(rows * (q_heads / cache.heads), 1, rows, q_heads, cache);
+}
+static size_t tables_bytes(int64_t requests) { return ((size_t)requests + 1) * 2 * sizeof(int64_t); }
+
+size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t shared) {
+    size_t slots = plan_own(cache, requests, rows, q_heads).slot_bytes();
+    if (shared > 0) slots += plan_prefix(cache, rows, q_heads).slot_bytes();
+    return kAttendCounterBytes + tables_bytes(requests) + slots * (size_t)(cache.dim + 2) * sizeof(float);
+}
+
+template <int D>
+static void launch_part(const AttendPlan &plan, const AttendArgs &a, const CacheView &cache, const PackedView &packed,
+                        hipStream_t stream) {
+    auto go = [&](auto kernel, int threads) { kernel<<<plan.tile.workgroups, threads, 0, stream>>>(a, cache, packed); };
+    if (!plan.few) go(many_kernel<D>, kManyThreads);
+    else if (plan.tile.rows == 16) go(few_kernel<D, 1>, kFewThreads);
+    else if (plan.tile.rows == 32) go(few_kernel<D, 2>, kFewThreads);
+    else if (plan.tile.rows == 48) go(few_kernel<D, 3>, kFewThreads);
+    else go(few_kernel<D, 4>, kFewThreads);
+}
 
 hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
                          const splosh_cache &cache, const splosh_packed &packed, int64_t rows, int64_t shared,
-                         float scale, uint16_t *out, int64_t ld_out, void *, hipStream_t stream) {
-    const AttendArgs a{q, row_stride, head_stride, out, ld_out, (int)q_heads, (int)(q_heads / cache.heads), (int)shared, scale};
-    auto go = [&](auto kernel) {
-        kernel<<<(unsigned)rows, kAttendThreads, 0, stream>>>(a, view_of(cache), view_of(packed, rows));
+                         float scale, uint16_t *out, int64_t ld_out, void *workspace, hipStream_t stream) {
+    const AttendPlan own = plan_own(cache, packed.requests, rows, q_heads);
+    uint8_t *at = static_cast<uint8_t *>(workspace) + kAttendCounterBytes;
+    AttendArgs a{};
+    a.q = q, a.row_stride = row_stride, a.head_stride = head_stride, a.out = out, a.ld_out = ld_out;
+    a.q_heads = (int)q_heads, a.shared = (int)shared;
+    a.wide = reinterpret_cast<uintptr_t>(q) % 16 == 0 && row_stride % 8 == 0 && head_stride % 8 == 0;
+    a.factor = scale * 1.4426950408889634f;
+    a.units = reinterpret_cast<int64_t *>(at);
+    a.segments = a.units + packed.requests + 1;
+    a.slots = reinterpret_cast<float *>(at + tables_bytes(packed.requests));
+    a.tile = own.tile, a.segment_slots = own.segment_slots, a.partial = shared > 0;
+    const CacheView cv = view_of(cache);
+    const PackedView pv = view_of(packed, rows);
+    AttendArgs b = a;
+    AttendPlan prefix = own;
+    if (shared > 0) {
+        prefix = plan_prefix(cache, rows, q_heads);
+        b.tile = prefix.tile, b.segment_slots = prefix.segment_slots, b.prefix = 1;
+        b.slots = a.slots + own.slot_bytes() * (cache.dim + 2);
+    }
+    auto run = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        if (shared > 0) launch_part<D>(prefix, b, cv, pv, stream);
+        launch_part<D>(own, a, cv, pv, stream);
+        join_kernel<D><<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, stream>>>(JoinArgs{a, b}, cv, pv);
     };
-    if (cache.dim == 256) go(attend_kernel<256>);
-    else if (cache.dim == 128) go(attend_kernel<128>);
-    else go(attend_kernel<64>);
+    if (cache.dim == 256) run(std::integral_constant<int, 256>{});
+    else if (cache.dim == 128) run(std::integral_constant<int, 128>{});
+    else run(std::integral_constant<int, 64>{});
     return hipGetLastError();
 }
 

@@ -1,0 +1,78 @@
+// attend_plan.hpp -- how a launch of the attention kernels shares a step's work out, as functions of the step's shape that the
+// kernels and the host both compile.
+#pragma once
+
+#include "cache.hpp"
+
+namespace splosh {
+
+// A tile is `rows` of the (row, query head) vectors of one request that share a key/value head, side by side: vector x
+// is row x / group of the request and head x % group of the group. A segment is a tile with all its keys, counted in units of
+// `keys` keys; the segments lie one behind the other (requests, then key/value heads, then tiles) and workgroup w of
+// `workgroups` takes the units from total w / workgroups on. So every workgroup has the same share, whatever
+// the lengths, and what a segment is cut into follows from the shape alone.
+struct TileShape {
+    int rows, keys, group, heads, workgroups;
+};
+
+// One request's part of a launch: its n rows from packed row `begin` on, the first at position `first`, and the keys
+// [from, to) of those that its rows see. A prefix that all requests share is one such part, of all rows.
+struct Span {
+    int begin, n, first, from, to;
+};
+
+__host__ __device__ __forceinline__ Span own_span(const PackedView &p, int page_tokens, int shared, int request) {
+    const int begin = p.starts[request], end = p.starts[request + 1], length = p.lengths[request];
+    Span s;
+    s.begin = begin < 0 ? 0 : begin;
+    s.n = (end > p.rows ? p.rows : end) - s.begin;
+    if (s.n < 0) s.n = 0;
+    // (Lengths past either end of what a table can hold are as good as these: nothing is seen, or everything.)
+    const int least = -(1 << 22), most = (1 << 30) + (1 << 23);
+    s.first = (length < least ? least : length > most ? most : length) - (s.begin + s.n) + s.begin;
+    s.from = shared;
+    s.to = p.table_pages * page_tokens;
+    return s;
+}
+__host__ __device__ __forceinline__ Span prefix_span(const PackedView &p, int shared) {
+    const int end = p.starts[p.requests];
+    return {0, end < 0 ? 0 : end > p.rows ? p.rows : end, shared, 0, shared};
+}
+
+__host__ __device__ __forceinline__ int tiles_of(const Span &s, const TileShape &t) { return (s.n * t.group + t.rows - 1) / t.rows; }
+
+// The end of the keys that tile i of a span sees.
+__host__ __device__ __forceinline__ int tile_end(const Span &s, const TileShape &t, int i) {
+    const int vectors = s.n * t.group, last = ((i + 1) * t.rows < vectors ? (i + 1) * t.rows : vectors) - 1;
+    const int end = s.first + last / t.group + 1;
+    return end < s.to ? end : s.to;
+}
+// Its units: one at least, so that rows that see nothing are written too.
+__host__ __device__ __forceinline__ int tile_units(const Span &s, const TileShape &t, int i) {
+    const int keys = tile_end(s, t, i) - s.from;
+    return keys <= t.keys ? 1 : (keys - 1) / t.keys + 1;
+}
+// The units of the tiles before tile i, for one key/value head.
+__host__ __device__ __forceinline__ int64_t units_before(const Span &s, const TileShape &t, int i) {
+    int64_t units = 0;
+    for (int j = 0; j < i; ++j) units += tile_units(s, t, j);
+    return units;
+}
+
+// The workgroups that get any of `total` units: one a unit where there are fewer units. Their pieces of a segment are consecutive.
+__host__ __device__ __forceinline__ int sharers_of(int64_t total, int workgroups) {
+    return total < workgroups ? (int)total : workgroups;
+}
+// Of these, workgroup w's first unit, and the workgroup that unit u belongs to.
+__host__ __device__ __forceinline__ int64_t first_unit(int64_t total, int workgroups, int w) { return total * w / workgroups; }
+__host__ __device__ __forceinline__ int owner_of(int64_t total, int workgroups, int64_t u) {
+    return (int)(((u + 1) * workgroups - 1) / total);
+}
+
+// A piece of a segment keeps its partial result in a slot: the one that begins the segment in that of the
+// segment, any other (a workgroup has one such at most, its first) in that of its workgroup.
+__host__ __device__ __forceinline__ int64_t most_segments(int64_t requests, int64_t rows, int64_t q_heads, int64_t heads, int tile_rows) {
+    return heads * ((requests < rows ? requests : rows) + rows * (q_heads / heads) / tile_rows);
+}
+
+}  // namespace splosh

@@ -9,7 +9,8 @@ namespace splosh {
 constexpr int kBlock = 32;  // tokens of a record
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
 
-// A record: codes of 32 keys, of 32 values, their scales. Rows of codes are whole vectors, so that a token is written
+// A record: codes of 32 keys, of 32 values, their scales; a code is kept as the byte code + 128, which takes one instruction less to
+// widen than a signed one. Rows of codes are whole vectors, so that a token is written
 // and read back in runs of `dim` bytes, and a matrix instruction's operand is a run of a row (keys: 16 bytes
 // of dimensions a lane) or the same run of eight rows (values), transposed in the registers while it is widened to fp16.
 constexpr int record_bytes(int dim) { return 2 * kBlock * dim + 2 * kBlock * 4; }

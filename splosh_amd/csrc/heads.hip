@@ -106,7 +106,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[E], float &scale) 
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int c = bad ? 0 : (int)__builtin_rintf(v[e] * times / by);
-        codes |= (uint32_t)(c & 0xff) << 8 * e;
+        codes |= (uint32_t)(c + 128) << 8 * e;
     }
     return codes;
 }
@@ -210,10 +210,10 @@ __global__ __launch_bounds__(kHeadThreads) void cache_read_kernel(ReadArgs a, Ca
         if (placed) {
             const uint8_t *record = record_of<D>(cache, page, head, at / kBlock);
             const int token = at % kBlock;
-            const int8_t *codes = reinterpret_cast<const int8_t *>(record) + (values * kBlock + token) * D + lane * E;
+            const uint8_t *codes = record + (values * kBlock + token) * D + lane * E;
             const float scale = reinterpret_cast<const float *>(record + 2 * kBlock * D)[values * kBlock + token];
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = (float)codes[e] * scale;
+            for (int e = 0; e < E; ++e) v[e] = (float)(codes[e] - 128) * scale;
         }
         store_bf16<E>(a.out[values] + row * a.ld[values] + head * D + lane * E, a.wide[values], v);
     }

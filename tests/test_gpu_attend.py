@@ -147,7 +147,7 @@ def test_what_is_masked_does_not_count(rt, runs, lengths, dim):
     for slot in range(s.pages * 32):
         if slot not in used:
             record = s.cache.data[slot // 32].view(2, -1)
-            record[:, slot % 32 * dim : (slot % 32 + 1) * dim] = 0x80
+            record[:, slot % 32 * dim : (slot % 32 + 1) * dim] = 0x00
             scales = record[:, 64 * dim :].view(torch.float32)
             scales[:, slot % 32], scales[:, 32 + slot % 32] = -math.inf, [0.0, -1.0, math.inf, math.nan][slot % 4]
     s.check(s.run())

@@ -116,7 +116,7 @@ def test_cache_holds_what_it_was_given(rt, dtype, runs, lengths, heads, dim, pag
             for values, x in ((0, st["k"]), (1, st["v"])):
                 codes, scale = kept(x[m, h])
                 at = base + (values * 32 + token) * dim
-                got = data[place[2], at : at + dim].view(torch.int8)
+                got = data[place[2], at : at + dim].int() - 128
                 if dtype == torch.bfloat16:
                     assert torch.equal(got.double(), codes), (m, h, values)
                 else:  # (x 127 / max, each rounded: a code next to the border of two can be either)
