@@ -17,6 +17,7 @@
 // from memory to registers; they are joined at the end. `many`: bound by the matrix instructions. Eight waves hold 32
 // vectors each, and go together through blocks that are widened to fp16 once, in LDS.
 #include <climits>
+#include <mutex>
 #include <type_traits>
 
 #include "attend_plan.hpp"
@@ -29,8 +30,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr size_t kAttendCounterBytes = 16384;  // the workspace's first bytes belong to other kernels' counters
 constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
-constexpr int kFewThreads = 256, kFewWaves = 4, kManyThreads = 512, kManyRows = 256;
-constexpr int kFewKeys = kFewWaves * kBlock, kManyKeys = 2 * kBlock;  // of a unit
+constexpr int kManyThreads = 512, kManyRows = 256, kManyKeys = 2 * kBlock;
 
 struct AttendArgs {
     const uint16_t *q;
@@ -116,6 +116,15 @@ __device__ __forceinline__ u32x4 moved8(const float *v, int power) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = f16_pair(__builtin_ldexpf(v[2 * e], power), __builtin_ldexpf(v[2 * e + 1], power));
     return w;
+}
+
+// A value that all lanes of the wave have, as a scalar.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ Span uniform(const Span &s) {
+    return {uniform(s.begin), uniform(s.n), uniform(s.first), uniform(s.from), uniform(s.to)};
 }
 
 // What the sum of a_j is divided by, for the scale of v_j. (1 where it is no scale: t is then NaN, or the key masked.)
@@ -221,9 +230,11 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         if (w == 0 && tid == 0) a.units[packed.requests] = total;
         __syncthreads();
         if (found < 0) return;
-        request = found, before = found_before, segment = found_segment;
+        request = uniform(found), before = uniform(found_before), segment = uniform(found_segment);
+        total = uniform(total);
         span = own_span(packed, cache.page_tokens, a.shared, request);
     }
+    span = uniform(span);
     const int sharers = sharers_of(total, tile.workgroups);
     if (w >= sharers) return;
     int64_t unit = first_unit(total, sharers, w);
@@ -259,7 +270,7 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         if (++head < tile.heads) continue;
         head = 0;
         do {  // (there is another one: the units say so)
-            span = own_span(packed, cache.page_tokens, a.shared, ++request);
+            span = uniform(own_span(packed, cache.page_tokens, a.shared, ++request));
             tiles = tiles_of(span, tile);
         } while (tiles == 0 && request + 1 < packed.requests);
     }
@@ -294,25 +305,83 @@ __device__ __forceinline__ void write_total(const AttendArgs &a, const Piece &p,
 }
 
 // ---- few vectors --------------------------------------------------------------------------------
+//
+// A wave has two records in LDS: the one it multiplies and the next one, on its way from memory (16 bytes a lane straight into LDS), so
+// that what is in flight takes no registers. Nothing is shared between the waves but the queries, and there is no
+// barrier while a piece runs. Where the sums would take more than 96 registers (256 dimensions of two or more times sixteen
+// vectors), two waves share a record and hold half of the dimensions each: both compute the scores, and a barrier
+// for each record says that both have loaded their half of the next. (One wave with all of them, 512 registers: spills, 460 us
+// for the 320 MB of the verify step.) A row of codes lies in LDS with its 16-byte runs exchanged by `turned`: the sixteen keys of an
+// operand read then hit different banks.
+
+template <int D>
+struct FewRing {
+    static constexpr int kRecord = record_bytes(D), kCodeLoads = 2 * kBlock * D / 1024, kLoads = kCodeLoads + 1;
+    static constexpr int kRuns = D / 16;  // of 16 bytes, of a row
+    static __device__ __forceinline__ int turned(int row, int run) {
+        return run ^ (D == 64 ? (row ^ row >> 2) & 3 : row & (kRuns - 1));
+    }
+};
 
 template <int D, int NT>
-__global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, CacheView cache, PackedView packed) {
-    constexpr int R = 16 * NT, SLABS = D / 64, STEPS = D / 32, TILES = D / 16, CHUNKS = D / 16, PITCH = D + 4;
-    __shared__ __align__(16) u32x4 q_parts[NT * STEPS * 64];
-    __shared__ __align__(16) float joined[kFewWaves][16 * PITCH];
-    __shared__ float wave_most[kFewWaves][R], wave_total[kFewWaves][R], row_factor[R];
-    __shared__ int row_position[R], least;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+struct FewShape {
+    static constexpr int kParts = D / 16 * NT * 4 > 96 ? 2 : 1;      // waves a record
+    static constexpr int kGroups = D == 256 && NT == 4 ? 3 : 4;       // records at a time (four would leave no room for the queries)
+    static constexpr int kThreads = 64 * kParts * kGroups, kRows = 16 * NT, kPitch = D + 4;
+    static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kQueryBytes = kRows * D * 2;
+    static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions
+    static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
+    static_assert(kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
+};
 
-    for_pieces<kFewThreads>(a, cache, packed, [&](const Piece &p) {
+template <int D, int NT>
+__global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(AttendArgs a, CacheView cache, PackedView packed) {
+    typedef FewShape<D, NT> S;
+    typedef FewRing<D> Ring;
+    constexpr int R = S::kRows, SLABS = D / 64, STEPS = D / 32, TILES = D / 16, CHUNKS = D / 16, PITCH = S::kPitch, GROUPS = S::kGroups;
+    constexpr int PARTS = S::kParts, HELD = TILES / PARTS, WORDS = SLABS / PARTS;  // tiles and dwords of a value's run that the wave holds
+    extern __shared__ __align__(16) char lds[];
+    u32x4 *const q_parts = reinterpret_cast<u32x4 *>(lds + S::kRingBytes);
+    float *const joined = reinterpret_cast<float *>(lds);  // [group][16][PITCH], in the ring's place
+    float *const wave_most = reinterpret_cast<float *>(lds + S::kNumbers), *const wave_total = wave_most + GROUPS * R;
+    float *const row_factor = wave_total + GROUPS * R;
+    int *const row_position = reinterpret_cast<int *>(row_factor + R), *const least = row_position + R;
+    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int record_group = wave / PARTS, half_of = wave % PARTS;
+    const int ring = record_group * 2 * Ring::kRecord;  // where the group's two records lie
+
+    // What load j of a record brings to the lane's 16 bytes of LDS: run (l mod kRuns) of row j (1024 / D) + l / kRuns, from where
+    // `turned` has it. Only with 256 dimensions does that depend on j, and on j mod 4 alone.
+    constexpr int SOURCES = D == 256 ? 4 : 1;
+    uint32_t source[SOURCES];
+#pragma unroll
+    for (int j = 0; j < SOURCES; ++j) {
+        const int row = j * (1024 / D) + lane / Ring::kRuns;
+        source[j] = (uint32_t)(lane / Ring::kRuns * D + Ring::turned(row, lane % Ring::kRuns) * 16);
+    }
+    for_pieces<S::kThreads>(a, cache, packed, [&](const Piece &p) {
         const int group = a.tile.group, vectors = p.span.n * group;
         __syncthreads();  // (the last piece's LDS is read)
-        if (tid == 0) least = INT_MAX;
+        Pages pages(packed, a.prefix ? 0 : p.request);
+        const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
+        bool hole = false;
+        auto load = [&](int block, int buffer) {
+            const uint8_t *record = block_record<D>(cache, pages, p.head, block, hole);
+            const rsrc_t r = make_rsrc(record, Ring::kRecord);
+            char *at = lds + uniform(ring + buffer * Ring::kRecord);
+#pragma unroll
+            for (int j = 0; j < Ring::kCodeLoads; ++j)
+                if (PARTS == 1 || j % 2 == half_of) buffer_load_lds16(r, at + j * 1024, source[j % SOURCES] + j * 1024);
+            if (PARTS == 1 || half_of == 0) buffer_load_lds4(r, at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (from + record_group < to) load(from + record_group, 0);
+        if (tid == 0) *least = INT_MAX;
         __syncthreads();
         // The tile's queries as the first product's operand: 16 dimensions of a vector a thread.
-        for (int item = tid; item < R * CHUNKS; item += kFewThreads) {
+        for (int item = tid; item < (R * CHUNKS + S::kThreads - 1) / S::kThreads * S::kThreads; item += S::kThreads) {
             const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
-            const bool valid = x < vectors;
+            const bool valid = i < R && x < vectors;
             const int row = valid ? row_of(p, group, x) : 0;
             float v[16] = {}, most = 0.0f;
             if (valid) {
@@ -325,13 +394,15 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, CacheVie
 #pragma unroll
             for (int m = 1; m < CHUNKS; m <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, m));
             const int power = power_of(most);
-            u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
-            to[0] = moved8(v, power);
-            to[64] = moved8(v + 8, power);
-            if (c == 0) {
-                row_factor[i] = __builtin_ldexpf(a.factor, -power);
-                row_position[i] = valid ? position_of(a, packed, p, row) : -1;
-                if (valid) atomicMin(&least, row_position[i]);
+            if (i < R) {
+                u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
+                to[0] = moved8(v, power);
+                to[64] = moved8(v + 8, power);
+                if (c == 0) {
+                    row_factor[i] = __builtin_ldexpf(a.factor, -power);
+                    row_position[i] = valid ? position_of(a, packed, p, row) : -1;
+                    if (valid) atomicMin(least, row_position[i]);
+                }
             }
         }
         __syncthreads();
@@ -342,60 +413,36 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, CacheVie
             factor[n] = row_factor[n * 16 + col], position[n] = row_position[n * 16 + col];
             most[n] = kLowest, total[n] = 0.0f;
         }
-        const int first_position = least;
-        f32x4 acc[TILES][NT] = {};
-        Pages pages(packed, a.prefix ? 0 : p.request);
-        const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
-
-        u32x4 k[2][SLABS];
-        uint32_t v[8][SLABS];
-        f32x4 ks[2], vs[2];
-        bool hole = false;
-        auto load_keys = [&](const uint8_t *record) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int s = 0; s < SLABS; ++s)
-                    k[t][s] = *reinterpret_cast<const u32x4 *>(record + (t * 16 + col) * D + s * 64 + g * 16);
-            const float *scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + 4 * g;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                ks[t] = *reinterpret_cast<const f32x4 *>(scales + 16 * t);
-                vs[t] = *reinterpret_cast<const f32x4 *>(scales + kBlock + 16 * t);
+        const int first_position = uniform(*least);
+        f32x4 acc[HELD][NT] = {};
+        int buffer = 0;
+        for (int first = from; first < to; first += GROUPS, buffer ^= 1) {
+            const int block = first + record_group;
+            const bool dead = hole;
+            if (PARTS == 2) {
+                wait_vmcnt<0>();
+                lds_barrier();  // this record has landed for both waves, and both are done with the one before it
             }
-        };
-        auto load_values = [&](const uint8_t *record) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint8_t *at = record + (kBlock + (e / 4) * 16 + 4 * g + e % 4) * D + col * (D / 16);
-                if constexpr (SLABS == 4) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) v[e][s] = x[s];
-                } else if constexpr (SLABS == 2) {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
-                    v[e][0] = x[0], v[e][1] = x[1];
-                } else {
-                    v[e][0] = *reinterpret_cast<const uint32_t *>(at);
-                }
+            if (block + GROUPS < to) {
+                load(block + GROUPS, buffer ^ 1);
+                if (PARTS == 1) wait_vmcnt<Ring::kLoads>();  // this record has landed; the next may be in flight
+            } else if (PARTS == 1) {
+                wait_vmcnt<0>();
             }
-        };
-        if (from + wave < to) {
-            const uint8_t *record = block_record<D>(cache, pages, p.head, from + wave, hole);
-            load_keys(record);
-            load_values(record);
-        }
-        for (int block = from + wave; block < to; block += kFewWaves) {
-            const bool more = block + kFewWaves < to, dead = hole;
-            const uint8_t *next = nullptr;
-            if (more) next = block_record<D>(cache, pages, p.head, block + kFewWaves, hole);
+            asm volatile("" ::: "memory");
+            if (block >= to) continue;
+            const char *const record = lds + ring + buffer * Ring::kRecord;
+            const float *const scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + 4 * g;
             f32x4 s[2][NT] = {};
 #pragma unroll
-            for (int slab = 0; slab < SLABS; ++slab)
+            for (int slab = 0; slab < SLABS; ++slab) {
+                u32x4 k[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    k[t] = *reinterpret_cast<const u32x4 *>(record + (t * 16 + col) * D + Ring::turned(t * 16 + col, slab * 4 + g) * 16);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const f16x8 k0 = widen8(k[0][slab][2 * half], k[0][slab][2 * half + 1]);
-                    const f16x8 k1 = widen8(k[1][slab][2 * half], k[1][slab][2 * half + 1]);
+                    const f16x8 k0 = widen8(k[0][2 * half], k[0][2 * half + 1]), k1 = widen8(k[1][2 * half], k[1][2 * half + 1]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const f16x8 q = __builtin_bit_cast(f16x8, q_parts[(n * STEPS + slab * 2 + half) * 64 + lane]);
@@ -403,57 +450,68 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, CacheVie
                         s[1][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q, s[1][n], 0, 0, 0);
                     }
                 }
+            }
             float key_scale[8], value_log[8], inverse[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                key_scale[e] = ks[e / 4][e % 4];
-                value_log[e] = __builtin_amdgcn_logf(vs[e / 4][e % 4]);
-                inverse[e] = inverse_scale(vs[e / 4][e % 4]);
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 ks = *reinterpret_cast<const f32x4 *>(scales + 16 * t), vs = *reinterpret_cast<const f32x4 *>(scales + kBlock + 16 * t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    key_scale[4 * t + e] = ks[e];
+                    value_log[4 * t + e] = __builtin_amdgcn_logf(vs[e]);
+                    inverse[4 * t + e] = inverse_scale(vs[e]);
+                }
             }
-            if (more) load_keys(next);
             const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
             f16x8 weight[NT];
-            float t[NT][8];
-            bool follow = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float top = -__builtin_inff();
+                float t[8], top = -__builtin_inff();
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    t[n][e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
-                    if (masked)
-                        t[n][e] = !dead && block * kBlock + (e / 4) * 16 + 4 * g + e % 4 <= position[n] ? t[n][e] : -__builtin_inff();
-                    top = __builtin_fmaxf(top, t[n][e]);
+                for (int e = 0; e < 8; ++e) t[e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        t[e] = !dead && block * kBlock + (e / 4) * 16 + 4 * g + e % 4 <= position[n] ? t[e] : -__builtin_inff();
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, t[e]);
                 top = __builtin_fmaxf(top, __shfl_xor(top, 16));
                 top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                wave_most[wave][n * 16 + col] = top;  // (kept there while `follow` is found out)
-                follow |= top > most[n] + kSlack;
-            }
-            if (__any(follow)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float top = __builtin_fmaxf(most[n], wave_most[wave][n * 16 + col]);
+                if (__any(top > most[n] + kSlack)) {
+                    top = __builtin_fmaxf(top, most[n]);
                     const float keep = __builtin_amdgcn_exp2f(most[n] - top);
                     most[n] = top;
                     total[n] *= keep;
 #pragma unroll
-                    for (int j = 0; j < TILES; ++j) acc[j][n] *= keep;
+                    for (int j = 0; j < HELD; ++j) acc[j][n] *= keep;
                 }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(t[n][e] - most[n]);
-                    total[n] = __builtin_fmaf(w[e], inverse[e], total[n]);
+                    t[e] = __builtin_amdgcn_exp2f(t[e] - most[n]);
+                    total[n] = __builtin_fmaf(t[e], inverse[e], total[n]);
                 }
-                const u32x4 pairs = {f16_pair(w[0], w[1]), f16_pair(w[2], w[3]), f16_pair(w[4], w[5]), f16_pair(w[6], w[7])};
+                const u32x4 pairs = {f16_pair(t[0], t[1]), f16_pair(t[2], t[3]), f16_pair(t[4], t[5]), f16_pair(t[6], t[7])};
                 weight[n] = __builtin_bit_cast(f16x8, pairs);
             }
+            uint32_t v[8][WORDS];
 #pragma unroll
-            for (int slab = 0; slab < SLABS; ++slab) {
+            for (int e = 0; e < 8; ++e) {
+                const int token = kBlock + (e / 4) * 16 + 4 * g + e % 4;
+                const char *at = record + token * D + Ring::turned(token, col * Ring::kRuns / 16) * 16 + col * (D / 16) % 16 + half_of * 8;
+                if constexpr (WORDS == 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[e][i] = x[i];
+                } else if constexpr (WORDS == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                    v[e][0] = x[0], v[e][1] = x[1];
+                } else {
+                    v[e][0] = *reinterpret_cast<const uint32_t *>(at);
+                }
+            }
+#pragma unroll
+            for (int slab = 0; slab < WORDS; ++slab) {
                 uint32_t of[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) of[e] = v[e][slab];
@@ -465,44 +523,50 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, CacheVie
                     for (int n = 0; n < NT; ++n)
                         acc[slab * 4 + c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[c], weight[n], acc[slab * 4 + c][n], 0, 0, 0);
             }
-            if (more) load_values(next);
+            // The record is read before the load after the next overwrites it.
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // The four waves' sums against the largest of their maxima, added in their order.
+        // The groups' sums against the largest of their maxima, added in their order.
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             total[n] += __shfl_xor(total[n], 16);
             total[n] += __shfl_xor(total[n], 32);
-            if (g == 0) wave_most[wave][n * 16 + col] = most[n], wave_total[wave][n * 16 + col] = total[n];
+            if (g == 0 && half_of == 0) wave_most[record_group * R + n * 16 + col] = most[n], wave_total[record_group * R + n * 16 + col] = total[n];
         }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float top = kLowest;
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) top = __builtin_fmaxf(top, wave_most[w][n * 16 + col]);
+            for (int w = 0; w < GROUPS; ++w) top = __builtin_fmaxf(top, wave_most[w * R + n * 16 + col]);
             const float keep = __builtin_amdgcn_exp2f(most[n] - top);
             if (n) __syncthreads();  // (the last sixteen vectors are read)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int j = 0; j < TILES; j += 4)
-                    *reinterpret_cast<f32x4 *>(&joined[wave][col * PITCH + (4 * g + e) * TILES + j]) =
+                for (int j = 0; j < HELD; j += 4)
+                    *reinterpret_cast<f32x4 *>(joined + (record_group * 16 + col) * PITCH + (4 * g + e) * TILES + half_of * HELD + j) =
                         f32x4{acc[j][n][e] * keep, acc[j + 1][n][e] * keep, acc[j + 2][n][e] * keep, acc[j + 3][n][e] * keep};
             __syncthreads();
-            const int i = tid / 16, d = tid % 16 * (D / 16);
-            float sum[D / 16], row_total = 0.0f, row_most = kLowest;
+            for (int item = tid; item < 256; item += S::kThreads) {
+                const int i = item / 16, d = item % 16 * (D / 16);
+                float sum[D / 16] = {}, row_total = 0.0f, row_most = kLowest;
 #pragma unroll
-            for (int e = 0; e < D / 16; ++e) sum[e] = 0.0f;
+                for (int w = 0; w < GROUPS; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w * R + n * 16 + i]);
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w][n * 16 + i]);
+                for (int w = 0; w < GROUPS; ++w) {
+                    row_total += wave_total[w * R + n * 16 + i] * __builtin_amdgcn_exp2f(wave_most[w * R + n * 16 + i] - row_most);
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) {
-                row_total += wave_total[w][n * 16 + i] * __builtin_amdgcn_exp2f(wave_most[w][n * 16 + i] - row_most);
+                    for (int e = 0; e < D / 16; e += 4) {
+                        const f32x4 part = *reinterpret_cast<const f32x4 *>(joined + (w * 16 + i) * PITCH + d + e);
 #pragma unroll
-                for (int e = 0; e < D / 16; ++e) sum[e] += joined[w][i * PITCH + d + e];
+                        for (int f = 0; f < 4; ++f) sum[e + f] += part[f];
+                    }
+                }
+                write_sums<D, D / 16>(a, p, n * 16 + i, d, sum, row_total);
+                if (item % 16 == 0) write_total<D>(a, p, n * 16 + i, row_most, row_total);
             }
-            write_sums<D, D / 16>(a, p, n * 16 + i, d, sum, row_total);
-            if (tid % 16 == 0) write_total<D>(a, p, n * 16 + i, row_most, row_total);
         }
     });
 }
@@ -516,7 +580,9 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
     __shared__ __align__(16) uint8_t key_parts[2][STEPS * K_PITCH];
     __shared__ __align__(16) u32x4 value_parts[2][TILES * 2 * 64];
     __shared__ __align__(16) float scales[2][3][kBlock];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, g = lane >> 5;
+    extern __shared__ __align__(16) char lds[];
+    char *const raw = lds;  // the next record
+    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 31, g = lane >> 5;
 
     for_pieces<kManyThreads>(a, cache, packed, [&](const Piece &p) {
         const int group = a.tile.group, vectors = p.span.n * group;
@@ -527,6 +593,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         int first_position = position;  // of the wave's vectors
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1) first_position = min(first_position, __shfl_xor(first_position, m));
+        first_position = uniform(first_position);
         // The lane's vector, half of its dimensions.
         f16x8 q[STEPS];
         float factor;
@@ -555,61 +622,59 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         Pages pages(packed, a.prefix ? 0 : p.request);
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
 
-        // Staging: threads 0..D-1 four dimensions of eight values each, the last 256 threads runs of 16 bytes of keys.
+        // The record of block b goes straight into LDS while block b - 1 is multiplied, and is widened to fp16 after that:
+        // by threads 0..D-1 four dimensions of eight values each, by the last 256 threads 16-byte runs of keys.
         const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
-        const bool stages_values = tid < D, stages_keys = tid >= 256;
-        uint32_t raw_v[8] = {};
-        u32x4 raw_k[K_ITEMS] = {};
-        float raw_scale = 0.0f;
         bool hole = false;
         auto fetch = [&](int block) {
             const uint8_t *record = block_record<D>(cache, pages, p.head, block, hole);
-            if (stages_values) {
+            const rsrc_t r = make_rsrc(record, record_bytes(D));
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    raw_v[e] = *reinterpret_cast<const uint32_t *>(
-                        record + (kBlock + 16 * value_step + (e / 4) * 8 + 4 * value_g + e % 4) * D + quad * 4);
-            }
-            if (stages_keys) {
-#pragma unroll
-                for (int n = 0; n < K_ITEMS; ++n) {
-                    const int item = tid - 256 + 256 * n;
-                    if (item < 2 * D)
-                        raw_k[n] = *reinterpret_cast<const u32x4 *>(record + (item / 4 % 32) * D + (item / 128 * 4 + item % 4) * 16);
-                }
-            }
-            if (tid < 2 * kBlock) raw_scale = reinterpret_cast<const float *>(record + 2 * kBlock * D)[tid];
+            for (int j = 0; j < (2 * kBlock * D / 1024 + 7) / 8; ++j)
+                if (j * 8 + wave < 2 * kBlock * D / 1024) buffer_load_lds16(r, lds + (j * 8 + wave) * 1024, (j * 8 + wave) * 1024 + lane * 16);
+            if (wave == 7) buffer_load_lds4(r, lds + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
+            __builtin_amdgcn_sched_barrier(0);
         };
         auto stage = [&](int buffer) {
-            if (stages_values) {
+            if (tid < D) {
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = *reinterpret_cast<const uint32_t *>(raw + (kBlock + 16 * value_step + (e / 4) * 8 + 4 * value_g + e % 4) * D + quad * 4);
                 f16x8 part[4];
-                widen_turned(raw_v, part);
+                widen_turned(v, part);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int t = D == 64 ? c >> 1 : quad / 32 * 4 + c, m = D == 64 ? (c & 1) * 16 + quad : quad % 32;
                     value_parts[buffer][(t * 2 + value_step) * 64 + value_g * 32 + m] = __builtin_bit_cast(u32x4, part[c]);
                 }
             }
-            if (stages_keys) {
+            if (tid >= 256) {
 #pragma unroll
                 for (int n = 0; n < K_ITEMS; ++n) {
                     const int item = tid - 256 + 256 * n;
                     if (item < 2 * D) {
-                        uint8_t *at = key_parts[buffer] + (item / 128 * 4 + item % 4) * K_PITCH + (item / 4 % 32) * 16;
-                        *reinterpret_cast<f16x8 *>(at) = widen8(raw_k[n][0], raw_k[n][1]);
-                        *reinterpret_cast<f16x8 *>(at + 512) = widen8(raw_k[n][2], raw_k[n][3]);
+                        const int run = item / 128 * 4 + item % 4, token = item / 4 % 32;
+                        const u32x4 k = *reinterpret_cast<const u32x4 *>(raw + token * D + run * 16);
+                        uint8_t *at = key_parts[buffer] + run * K_PITCH + token * 16;
+                        *reinterpret_cast<f16x8 *>(at) = widen8(k[0], k[1]);
+                        *reinterpret_cast<f16x8 *>(at + 512) = widen8(k[2], k[3]);
                     }
                 }
             }
-            if (tid < kBlock) scales[buffer][0][tid] = raw_scale;
-            else if (tid < 2 * kBlock)
-                scales[buffer][1][tid - kBlock] = __builtin_amdgcn_logf(raw_scale), scales[buffer][2][tid - kBlock] = inverse_scale(raw_scale);
+            if (tid < 2 * kBlock) {
+                const float scale = reinterpret_cast<const float *>(raw + 2 * kBlock * D)[tid];
+                if (tid < kBlock) scales[buffer][0][tid] = scale;
+                else scales[buffer][1][tid - kBlock] = __builtin_amdgcn_logf(scale), scales[buffer][2][tid - kBlock] = inverse_scale(scale);
+            }
         };
 
         bool dead = false;
         __syncthreads();  // (the last piece's LDS is read)
         if (from < to) {
             fetch(from);
+            wait_vmcnt<0>();
+            __syncthreads();
             dead = hole;
             stage(0);
         }
@@ -671,10 +736,12 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                 }
             }
             if (block + 1 < to) {
+                wait_vmcnt<0>();
+                lds_barrier();  // every wave's part of the next record has landed
                 dead = hole;
                 stage(buffer ^ 1);
             }
-            __syncthreads();
+            lds_barrier();
         }
         total += __shfl_xor(total, 32);
         const int i = wave * 32 + col;
@@ -790,10 +857,10 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     p.few = vectors <= 64;
     const int nt = (int)((vectors + 15) / 16);
     p.tile.rows = p.few ? 16 * nt : kManyRows;
-    p.tile.keys = p.few ? kFewKeys : kManyKeys;
+    p.tile.keys = !p.few ? kManyKeys : cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups * kBlock : FewShape<64, 1>::kGroups * kBlock;
     p.tile.group = (int)(q_heads / cache.heads);
     p.tile.heads = (int)cache.heads;
-    p.tile.workgroups = p.few && nt == 1 ? 2 * cus : cus;
+    p.tile.workgroups = p.few && cache.dim < 256 ? 2 * cus : cus;
     p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
     return p;
 }
@@ -814,12 +881,23 @@ size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64
 template <int D>
 static void launch_part(const AttendPlan &plan, const AttendArgs &a, const CacheView &cache, const PackedView &packed,
                         hipStream_t stream) {
-    auto go = [&](auto kernel, int threads) { kernel<<<plan.tile.workgroups, threads, 0, stream>>>(a, cache, packed); };
-    if (!plan.few) go(many_kernel<D>, kManyThreads);
-    else if (plan.tile.rows == 16) go(few_kernel<D, 1>, kFewThreads);
-    else if (plan.tile.rows == 32) go(few_kernel<D, 2>, kFewThreads);
-    else if (plan.tile.rows == 48) go(few_kernel<D, 3>, kFewThreads);
-    else go(few_kernel<D, 4>, kFewThreads);
+    auto few = [&](auto tiles) {
+        typedef FewShape<D, decltype(tiles)::value> S;
+        auto kernel = few_kernel<D, decltype(tiles)::value>;
+        // (Allowed once a device: more dynamic LDS than the default 64 KiB.)
+        static std::once_flag allowed[64];
+        int device = 0;
+        (void)hipGetDevice(&device);
+        std::call_once(allowed[device & 63], [&] {
+            (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+        });
+        kernel<<<plan.tile.workgroups, S::kThreads, S::kLds, stream>>>(a, cache, packed);
+    };
+    if (!plan.few) many_kernel<D><<<plan.tile.workgroups, kManyThreads, record_bytes(D), stream>>>(a, cache, packed);
+    else if (plan.tile.rows == 16) few(std::integral_constant<int, 1>{});
+    else if (plan.tile.rows == 32) few(std::integral_constant<int, 2>{});
+    else if (plan.tile.rows == 48) few(std::integral_constant<int, 3>{});
+    else few(std::integral_constant<int, 4>{});
 }
 
 hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
