@@ -30,7 +30,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr size_t kAttendCounterBytes = 16384;  // the workspace's first bytes belong to other kernels' counters
 constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
-constexpr int kManyThreads = 512, kManyRows = 256, kManyKeys = 2 * kBlock;
+constexpr int kManyThreads = 512, kManyRows = 256;
+constexpr int kManyKeys = 2 * kBlock;  // of a unit of the kernel for many vectors
 
 struct AttendArgs {
     const uint16_t *q;
@@ -44,8 +45,15 @@ struct AttendArgs {
     int partial;                // whether every piece leaves its partial result
     float *slots;
     int64_t segment_slots;
-    int64_t *units;             // the requests' first units, and the total
-    int64_t *segments;          // and first segments
+    struct Pieces *pieces;      // of every (row, query head)
+};
+
+// Where the partial results of one (row, query head) lie, for the launch that joins them.
+struct Pieces {
+    int slot;       // the first one's
+    int workgroup;  // the workgroup that took it; the next ones took the next, and have slots by workgroup
+    int count;      // 1 and no prefix: written already
+    int at;         // its vector of the tile
 };
 
 // Where a piece's vectors and keys lie.
@@ -53,7 +61,7 @@ struct Piece {
     Span span;
     int request, head, tile;
     int first_block, blocks;  // of 32 keys, from the span's first on
-    int64_t slot;
+    int slot, count;          // count: the segment's pieces, where this is the first of them; 0 else
     bool direct;              // the whole segment, and nothing to join it with
 };
 
@@ -219,15 +227,13 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         const int64_t first = w < sharers ? first_unit(total, sharers, w) : total;
         int64_t at = units_to - units, at_segment = segments_to - segments;
         const bool mine = at <= first && first < units_to;
-        if (mine || w == 0) {
+        if (mine) {
             for (int r = low; r < high; ++r) {
                 units_of(r, u, n);
-                if (w == 0) a.units[r] = at, a.segments[r] = at_segment;  // (for the launch that joins the pieces)
-                if (mine && at <= first && first < at + u) found = r, found_before = at, found_segment = at_segment;
+                if (at <= first && first < at + u) found = r, found_before = at, found_segment = at_segment;
                 at += u, at_segment += n;
             }
         }
-        if (w == 0 && tid == 0) a.units[packed.requests] = total;
         __syncthreads();
         if (found < 0) return;
         request = uniform(found), before = uniform(found_before), segment = uniform(found_segment);
@@ -259,7 +265,8 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         p.span = span, p.request = request, p.head = head, p.tile = t;
         p.first_block = offset * per;
         p.blocks = max(0, min((offset + take) * per, blocks) - p.first_block);
-        p.slot = offset == 0 ? segment : a.segment_slots + w;
+        p.slot = (int)(offset == 0 ? segment : a.segment_slots + w);
+        p.count = offset > 0 ? 0 : take == units ? 1 : owner_of(total, sharers, unit + units - 1) - w + 1;
         p.direct = !a.partial && take == units;
         if (segment < a.segment_slots) work(p);  // (more there are only where starts do not ascend)
         unit += take;
@@ -296,22 +303,164 @@ __device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, 
         for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4 *>(at + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
     }
 }
-// And its maximum and sum, where they are left.
+// And its maximum and sum, where they are left; with the segment's first piece, where all of its pieces are.
 template <int D>
 __device__ __forceinline__ void write_total(const AttendArgs &a, const Piece &p, int i, float most, float total) {
+    const int x = p.tile * a.tile.rows + i;
+    if (p.count > 0 && x < p.span.n * a.tile.group)
+        a.pieces[(int64_t)row_of(p, a.tile.group, x) * a.q_heads + p.head * a.tile.group + x % a.tile.group] = {p.slot, (int)blockIdx.x, p.count, i};
     if (p.direct) return;
     float *at = a.slots + p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)a.tile.rows * D;
     at[i] = most, at[a.tile.rows + i] = total;
+}
+
+// The tile's queries as the first product's operand, 16 dimensions of a vector a thread; the powers that they are moved back by, their positions
+// and the least of these.
+template <int D, int R, int THREADS>
+__device__ __forceinline__ void stage_queries(const AttendArgs &a, const PackedView &packed, const Piece &p, u32x4 *q_parts, float *row_factor,
+                                              int *row_position, int *least) {
+    constexpr int STEPS = D / 32, CHUNKS = D / 16;
+    const int group = a.tile.group, vectors = p.span.n * group, tid = threadIdx.x;
+                    for (int item = tid; item < (R * CHUNKS + THREADS - 1) / THREADS * THREADS; item += THREADS) {
+                const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
+                const bool valid = i < R && x < vectors;
+                const int row = valid ? row_of(p, group, x) : 0;
+                float v[16] = {}, most = 0.0f;
+                if (valid) {
+                    const uint16_t *at = a.q + row * a.row_stride + (p.head * group + x % group) * a.head_stride + c * 16;
+                    load_q8(at, a.wide, v);
+                    load_q8(at + 8, a.wide, v + 8);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
+#pragma unroll
+                for (int m = 1; m < CHUNKS; m <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, m));
+                const int power = power_of(most);
+                if (i < R) {
+                    u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
+                    to[0] = moved8(v, power);
+                    to[64] = moved8(v + 8, power);
+                    if (c == 0) {
+                        row_factor[i] = __builtin_ldexpf(a.factor, -power);
+                        row_position[i] = valid ? position_of(a, packed, p, row) : -1;
+                        if (valid) atomicMin(least, row_position[i]);
+                    }
+                }
+            }
+}
+
+// The groups' sums against the largest of their maxima, added in their order: vectors 16 at a time, all threads.
+template <int D, int NT, typename S, int HELD>
+__device__ __forceinline__ void join_groups(const AttendArgs &a, const Piece &p, f32x4 (&acc)[HELD][NT], const float (&most)[NT], float (&total)[NT],
+                                            float *joined, float *wave_most, float *wave_total, int record_group, int half_of) {
+    constexpr int R = S::kRows, GROUPS = S::kGroups, PITCH = S::kPitch;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                total[n] += __shfl_xor(total[n], 16);
+                total[n] += __shfl_xor(total[n], 32);
+                if (g == 0 && half_of == 0) wave_most[record_group * R + n * 16 + col] = most[n], wave_total[record_group * R + n * 16 + col] = total[n];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float top = kLowest;
+#pragma unroll
+                for (int w = 0; w < GROUPS; ++w) top = __builtin_fmaxf(top, wave_most[w * R + n * 16 + col]);
+                const float keep = __builtin_amdgcn_exp2f(most[n] - top);
+                if (n) __syncthreads();  // (the last sixteen vectors are read)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < HELD; j += 4)
+                        *reinterpret_cast<f32x4 *>(joined + (record_group * 16 + col) * PITCH + half_of * (D / 2) + (4 * g + e) * HELD + j) =
+                            f32x4{acc[j][n][e] * keep, acc[j + 1][n][e] * keep, acc[j + 2][n][e] * keep, acc[j + 3][n][e] * keep};
+                __syncthreads();
+                for (int item = tid; item < 256; item += S::kThreads) {
+                    const int i = item / 16, d = item % 16 * (D / 16);
+                    float sum[D / 16] = {}, row_total = 0.0f, row_most = kLowest;
+#pragma unroll
+                    for (int w = 0; w < GROUPS; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w * R + n * 16 + i]);
+#pragma unroll
+                    for (int w = 0; w < GROUPS; ++w) {
+                        row_total += wave_total[w * R + n * 16 + i] * __builtin_amdgcn_exp2f(wave_most[w * R + n * 16 + i] - row_most);
+#pragma unroll
+                        for (int e = 0; e < D / 16; e += 4) {
+                            const f32x4 part = *reinterpret_cast<const f32x4 *>(joined + (w * 16 + i) * PITCH + d + e);
+#pragma unroll
+                            for (int f = 0; f < 4; ++f) sum[e + f] += part[f];
+                        }
+                    }
+                    write_sums<D, D / 16>(a, p, n * 16 + i, d, sum, row_total);
+                    if (item % 16 == 0) write_total<D>(a, p, n * 16 + i, row_most, row_total);
+                }
+            }
+}
+
+// The larger of a lane's value and that of the lane 16 (32) further: two registers' rows swapped, in place of a trip through LDS.
+__device__ __forceinline__ float max_rows(float v) {
+    typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+    const u32x2v r = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_halves(float v) {
+    typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+    const u32x2v r = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The weights of a lane's eight scores of each vector: masked, against the running maxima (the sums follow where these move), summed with
+// the scales' inverses, and as the second product's operand.
+template <int NT, int HELD>
+__device__ __forceinline__ void weigh(float (&t)[NT][8], bool masked, bool dead, int block, int g, const int (&position)[NT], const float (&inverse)[8],
+                                      float (&most)[NT], float (&total)[NT], f32x4 (&acc)[HELD][NT], f16x8 (&weight)[NT]) {
+    if (masked) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                t[n][e] = !dead && block * kBlock + (e / 4) * 16 + 4 * g + e % 4 <= position[n] ? t[n][e] : -__builtin_inff();
+    }
+    float top[NT];
+    bool follow = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        top[n] = t[n][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top[n] = __builtin_fmaxf(top[n], t[n][e]);
+        top[n] = max_halves(max_rows(top[n]));
+        follow |= top[n] > most[n] + kSlack;
+    }
+    if (__any(follow)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float now = __builtin_fmaxf(top[n], most[n]), keep = __builtin_amdgcn_exp2f(most[n] - now);
+            most[n] = now;
+            total[n] *= keep;
+#pragma unroll
+            for (int j = 0; j < HELD; ++j) acc[j][n] *= keep;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        uint32_t pairs[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float a = __builtin_amdgcn_exp2f(t[n][e] - most[n]), b = __builtin_amdgcn_exp2f(t[n][e + 1] - most[n]);
+            total[n] = __builtin_fmaf(a, inverse[e], total[n]);
+            total[n] = __builtin_fmaf(b, inverse[e + 1], total[n]);
+            pairs[e / 2] = f16_pair(a, b);
+        }
+        const u32x4 four = {pairs[0], pairs[1], pairs[2], pairs[3]};
+        weight[n] = __builtin_bit_cast(f16x8, four);
+    }
 }
 
 // ---- few vectors --------------------------------------------------------------------------------
 //
 // A wave has two records in LDS: the one it multiplies and the next one, on its way from memory (16 bytes a lane straight into LDS), so
 // that what is in flight takes no registers. Nothing is shared between the waves but the queries, and there is no
-// barrier while a piece runs. Where the sums would take more than 96 registers (256 dimensions of two or more times sixteen
-// vectors), two waves share a record and hold half of the dimensions each: both compute the scores, and a barrier
-// for each record says that both have loaded their half of the next. (One wave with all of them, 512 registers: spills, 460 us
-// for the 320 MB of the verify step.) A row of codes lies in LDS with its 16-byte runs exchanged by `turned`: the sixteen keys of an
+// barrier while a piece runs. A row of codes lies in LDS with its 16-byte runs exchanged by `turned`: the sixteen keys of an
 // operand read then hit different banks.
 
 template <int D>
@@ -325,9 +474,7 @@ struct FewRing {
 
 template <int D, int NT>
 struct FewShape {
-    static constexpr int kParts = D / 16 * NT * 4 > 96 ? 2 : 1;      // waves a record
-    static constexpr int kGroups = D == 256 && NT == 4 ? 3 : 4;       // records at a time (four would leave no room for the queries)
-    static constexpr int kThreads = 64 * kParts * kGroups, kRows = 16 * NT, kPitch = D + 4;
+    static constexpr int kGroups = 4, kThreads = 64 * kGroups, kRows = 16 * NT, kPitch = D + 4;
     static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kQueryBytes = kRows * D * 2;
     static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions
     static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
@@ -338,8 +485,7 @@ template <int D, int NT>
 __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(AttendArgs a, CacheView cache, PackedView packed) {
     typedef FewShape<D, NT> S;
     typedef FewRing<D> Ring;
-    constexpr int R = S::kRows, SLABS = D / 64, STEPS = D / 32, TILES = D / 16, CHUNKS = D / 16, PITCH = S::kPitch, GROUPS = S::kGroups;
-    constexpr int PARTS = S::kParts, HELD = TILES / PARTS, WORDS = SLABS / PARTS;  // tiles and dwords of a value's run that the wave holds
+    constexpr int R = S::kRows, SLABS = D / 64, STEPS = D / 32, GROUPS = S::kGroups, HELD = D / 16;
     extern __shared__ __align__(16) char lds[];
     u32x4 *const q_parts = reinterpret_cast<u32x4 *>(lds + S::kRingBytes);
     float *const joined = reinterpret_cast<float *>(lds);  // [group][16][PITCH], in the ring's place
@@ -347,8 +493,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
     float *const row_factor = wave_total + GROUPS * R;
     int *const row_position = reinterpret_cast<int *>(row_factor + R), *const least = row_position + R;
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
-    const int record_group = wave / PARTS, half_of = wave % PARTS;
-    const int ring = record_group * 2 * Ring::kRecord;  // where the group's two records lie
+    const int record_group = wave, ring = record_group * 2 * Ring::kRecord;  // where the group's two records lie
 
     // What load j of a record brings to the lane's 16 bytes of LDS: run (l mod kRuns) of row j (1024 / D) + l / kRuns, from where
     // `turned` has it. Only with 256 dimensions does that depend on j, and on j mod 4 alone.
@@ -360,7 +505,6 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
         source[j] = (uint32_t)(lane / Ring::kRuns * D + Ring::turned(row, lane % Ring::kRuns) * 16);
     }
     for_pieces<S::kThreads>(a, cache, packed, [&](const Piece &p) {
-        const int group = a.tile.group, vectors = p.span.n * group;
         __syncthreads();  // (the last piece's LDS is read)
         Pages pages(packed, a.prefix ? 0 : p.request);
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
@@ -371,40 +515,14 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
             char *at = lds + uniform(ring + buffer * Ring::kRecord);
 #pragma unroll
             for (int j = 0; j < Ring::kCodeLoads; ++j)
-                if (PARTS == 1 || j % 2 == half_of) buffer_load_lds16(r, at + j * 1024, source[j % SOURCES] + j * 1024);
-            if (PARTS == 1 || half_of == 0) buffer_load_lds4(r, at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
+                buffer_load_lds16(r, at + j * 1024, source[j % SOURCES] + j * 1024);
+            buffer_load_lds4(r, at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
             __builtin_amdgcn_sched_barrier(0);
         };
         if (from + record_group < to) load(from + record_group, 0);
         if (tid == 0) *least = INT_MAX;
         __syncthreads();
-        // The tile's queries as the first product's operand: 16 dimensions of a vector a thread.
-        for (int item = tid; item < (R * CHUNKS + S::kThreads - 1) / S::kThreads * S::kThreads; item += S::kThreads) {
-            const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
-            const bool valid = i < R && x < vectors;
-            const int row = valid ? row_of(p, group, x) : 0;
-            float v[16] = {}, most = 0.0f;
-            if (valid) {
-                const uint16_t *at = a.q + row * a.row_stride + (p.head * group + x % group) * a.head_stride + c * 16;
-                load_q8(at, a.wide, v);
-                load_q8(at + 8, a.wide, v + 8);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
-#pragma unroll
-            for (int m = 1; m < CHUNKS; m <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, m));
-            const int power = power_of(most);
-            if (i < R) {
-                u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
-                to[0] = moved8(v, power);
-                to[64] = moved8(v + 8, power);
-                if (c == 0) {
-                    row_factor[i] = __builtin_ldexpf(a.factor, -power);
-                    row_position[i] = valid ? position_of(a, packed, p, row) : -1;
-                    if (valid) atomicMin(least, row_position[i]);
-                }
-            }
-        }
+        stage_queries<D, R, S::kThreads>(a, packed, p, q_parts, row_factor, row_position, least);
         __syncthreads();
         float factor[NT], most[NT], total[NT];
         int position[NT];
@@ -416,21 +534,15 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
         const int first_position = uniform(*least);
         f32x4 acc[HELD][NT] = {};
         int buffer = 0;
-        for (int first = from; first < to; first += GROUPS, buffer ^= 1) {
-            const int block = first + record_group;
+        for (int block = from + record_group; block < to; block += GROUPS, buffer ^= 1) {
             const bool dead = hole;
-            if (PARTS == 2) {
-                wait_vmcnt<0>();
-                lds_barrier();  // this record has landed for both waves, and both are done with the one before it
-            }
             if (block + GROUPS < to) {
                 load(block + GROUPS, buffer ^ 1);
-                if (PARTS == 1) wait_vmcnt<Ring::kLoads>();  // this record has landed; the next may be in flight
-            } else if (PARTS == 1) {
+                wait_vmcnt<Ring::kLoads>();  // this record has landed; the next may be in flight
+            } else {
                 wait_vmcnt<0>();
             }
             asm volatile("" ::: "memory");
-            if (block >= to) continue;
             const char *const record = lds + ring + buffer * Ring::kRecord;
             const float *const scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + 4 * g;
             f32x4 s[2][NT] = {};
@@ -464,46 +576,22 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
             }
             const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
             f16x8 weight[NT];
+            float t[NT][8];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float t[8], top = -__builtin_inff();
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
-                if (masked) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        t[e] = !dead && block * kBlock + (e / 4) * 16 + 4 * g + e % 4 <= position[n] ? t[e] : -__builtin_inff();
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, t[e]);
-                top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-                top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                if (__any(top > most[n] + kSlack)) {
-                    top = __builtin_fmaxf(top, most[n]);
-                    const float keep = __builtin_amdgcn_exp2f(most[n] - top);
-                    most[n] = top;
-                    total[n] *= keep;
-#pragma unroll
-                    for (int j = 0; j < HELD; ++j) acc[j][n] *= keep;
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    t[e] = __builtin_amdgcn_exp2f(t[e] - most[n]);
-                    total[n] = __builtin_fmaf(t[e], inverse[e], total[n]);
-                }
-                const u32x4 pairs = {f16_pair(t[0], t[1]), f16_pair(t[2], t[3]), f16_pair(t[4], t[5]), f16_pair(t[6], t[7])};
-                weight[n] = __builtin_bit_cast(f16x8, pairs);
-            }
-            uint32_t v[8][WORDS];
+                for (int e = 0; e < 8; ++e) t[n][e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
+            weigh<NT, HELD>(t, masked, dead, block, g, position, inverse, most, total, acc, weight);
+            uint32_t v[8][SLABS];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int token = kBlock + (e / 4) * 16 + 4 * g + e % 4;
-                const char *at = record + token * D + Ring::turned(token, col * Ring::kRuns / 16) * 16 + col * (D / 16) % 16 + half_of * 8;
-                if constexpr (WORDS == 4) {
+                const char *at = record + token * D + Ring::turned(token, col * Ring::kRuns / 16) * 16 + col * (D / 16) % 16;
+                if constexpr (SLABS == 4) {
                     const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[e][i] = x[i];
-                } else if constexpr (WORDS == 2) {
+                } else if constexpr (SLABS == 2) {
                     const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
                     v[e][0] = x[0], v[e][1] = x[1];
                 } else {
@@ -511,7 +599,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
                 }
             }
 #pragma unroll
-            for (int slab = 0; slab < WORDS; ++slab) {
+            for (int slab = 0; slab < SLABS; ++slab) {
                 uint32_t of[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) of[e] = v[e][slab];
@@ -527,47 +615,186 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
         }
-        // The groups' sums against the largest of their maxima, added in their order.
+        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group, 0);
+    });
+}
+
+// ---- few vectors, many sums -----------------------------------------------------------------------
+//
+// Two waves share a record where one wave's sums would take more than 96 registers (256 dimensions of two or more times sixteen
+// vectors): each holds half of the values' dimensions, and both compute the scores. They load half of each record each, so that a
+// barrier has to say what has landed and what is used up; there are two for a record, after the scores (its keys' place is
+// free: those of the record after the next are asked for) and before the next ones (the same for values), so that
+// a whole record a group is in flight at every wait. (Measured on the verify step, 320 MB: one wave with all sums, 512 registers,
+// 150 us; one barrier and one wait a record 110; half records straight to registers, the scores of either half exchanged, 131.)
+
+template <int D, int NT>
+struct PairShape {
+    static constexpr int kGroups = D == 256 && NT == 4 ? 3 : 4;  // (four would leave no room for the queries)
+    static constexpr int kThreads = 128 * kGroups, kRows = 16 * NT, kPitch = D + 4;
+    static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kNumbers = kRingBytes + kRows * D * 2;
+    static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
+    static_assert(kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
+};
+
+template <int D, int NT>
+__global__ __launch_bounds__((PairShape<D, NT>::kThreads)) void pair_kernel(AttendArgs a, CacheView cache, PackedView packed) {
+    typedef PairShape<D, NT> S;
+    typedef FewRing<D> Ring;
+    constexpr int R = S::kRows, SLABS = D / 64, STEPS = D / 32, GROUPS = S::kGroups;
+    constexpr int HELD = D / 32, WORDS = D / 128;  // tiles, and dwords of a value's run, of half of the dimensions
+    constexpr int KEY_LOADS = kBlock * D / 2048, VALUE_LOADS = KEY_LOADS + 1;  // of a wave: half of the codes; the scales with the values
+    extern __shared__ __align__(16) char lds[];
+    float *const joined = reinterpret_cast<float *>(lds);  // [group][16][PITCH], in the ring's place
+    u32x4 *const q_parts = reinterpret_cast<u32x4 *>(lds + S::kRingBytes);
+    float *const wave_most = reinterpret_cast<float *>(lds + S::kNumbers), *const wave_total = wave_most + GROUPS * R;
+    float *const row_factor = wave_total + GROUPS * R;
+    int *const row_position = reinterpret_cast<int *>(row_factor + R), *const least = row_position + R;
+    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int record_group = wave >> 1, half_of = wave & 1, ring = record_group * 2 * Ring::kRecord;
+
+    // (The sources of a record's loads as in few_kernel.)
+    constexpr int SOURCES = D == 256 ? 4 : 1;
+    uint32_t source[SOURCES];
+#pragma unroll
+    for (int j = 0; j < SOURCES; ++j)
+        source[j] = (uint32_t)(lane / Ring::kRuns * D + Ring::turned(j * (1024 / D) + lane / Ring::kRuns, lane % Ring::kRuns) * 16);
+
+    for_pieces<S::kThreads>(a, cache, packed, [&](const Piece &p) {
+        Pages pages(packed, a.prefix ? 0 : p.request);
+        const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
+        bool hole;
+        // (Past the last block nothing is read: every lane's offset is past the end. The counts stay the same.)
+        auto source_of = [&](int block) {
+            hole = false;
+            const uint8_t *record = block < to ? block_record<D>(cache, pages, p.head, block, hole) : cache.data;
+            return make_rsrc(record, block < to ? Ring::kRecord : 0);
+        };
+        auto load_keys = [&](int block, int buffer) {
+            const rsrc_t r = source_of(block);
+            char *at = lds + uniform(ring + buffer * Ring::kRecord);
+#pragma unroll
+            for (int i = 0; i < KEY_LOADS; ++i) {
+                const int j = 2 * i + half_of;
+                buffer_load_lds16(r, at + j * 1024, source[SOURCES == 1 ? 0 : (2 * i) % 4 + half_of] + j * 1024);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto load_values = [&](int block, int buffer) {
+            const rsrc_t r = source_of(block);
+            char *at = lds + uniform(ring + buffer * Ring::kRecord);
+#pragma unroll
+            for (int i = 0; i < KEY_LOADS; ++i) {
+                const int j = 2 * KEY_LOADS + 2 * i + half_of;
+                buffer_load_lds16(r, at + j * 1024, source[SOURCES == 1 ? 0 : (2 * i) % 4 + half_of] + j * 1024);
+            }
+            buffer_load_lds4(r, at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);  // (both waves: the same)
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        __syncthreads();  // (the last piece's LDS is read)
+        load_keys(from + record_group, 0);
+        load_values(from + record_group, 0);
+        bool dead_next = hole;
+        load_keys(from + record_group + GROUPS, 1);
+        if (tid == 0) *least = INT_MAX;
+        lds_barrier();
+        stage_queries<D, R, S::kThreads>(a, packed, p, q_parts, row_factor, row_position, least);
+        lds_barrier();
+        float factor[NT], most[NT], total[NT];
+        int position[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            total[n] += __shfl_xor(total[n], 16);
-            total[n] += __shfl_xor(total[n], 32);
-            if (g == 0 && half_of == 0) wave_most[record_group * R + n * 16 + col] = most[n], wave_total[record_group * R + n * 16 + col] = total[n];
+            factor[n] = row_factor[n * 16 + col], position[n] = row_position[n * 16 + col];
+            most[n] = kLowest, total[n] = 0.0f;
         }
-        __syncthreads();
+        const int first_position = uniform(*least);
+        f32x4 acc[HELD][NT] = {};
+        int buffer = 0;
+        // Groups from the third on are one barrier behind: while the others compute scores (LDS and matrix instructions), they weigh values
+        // (vector instructions), on the same SIMDs.
+        if (record_group >= 2) lds_barrier();
+        for (int first = from; first < to; first += GROUPS, buffer ^= 1) {
+            const int block = first + record_group;
+            const bool here = block < to, dead = dead_next;
+            const char *const record = lds + ring + buffer * Ring::kRecord;
+            wait_vmcnt<VALUE_LOADS + KEY_LOADS>();
+            lds_barrier();  // this record's keys are here, and the last one's values used up
+            load_values(block + GROUPS, buffer ^ 1);
+            dead_next = hole;
+            f32x4 s[2][NT] = {};
+            if (here) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float top = kLowest;
+                for (int slab = 0; slab < SLABS; ++slab) {
+                    u32x4 k[2];
 #pragma unroll
-            for (int w = 0; w < GROUPS; ++w) top = __builtin_fmaxf(top, wave_most[w * R + n * 16 + col]);
-            const float keep = __builtin_amdgcn_exp2f(most[n] - top);
-            if (n) __syncthreads();  // (the last sixteen vectors are read)
+                    for (int t = 0; t < 2; ++t)
+                        k[t] = *reinterpret_cast<const u32x4 *>(record + (t * 16 + col) * D + Ring::turned(t * 16 + col, slab * 4 + g) * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+                    for (int half = 0; half < 2; ++half) {
+                        const f16x8 k0 = widen8(k[0][2 * half], k[0][2 * half + 1]), k1 = widen8(k[1][2 * half], k[1][2 * half + 1]);
 #pragma unroll
-                for (int j = 0; j < HELD; j += 4)
-                    *reinterpret_cast<f32x4 *>(joined + (record_group * 16 + col) * PITCH + (4 * g + e) * TILES + half_of * HELD + j) =
-                        f32x4{acc[j][n][e] * keep, acc[j + 1][n][e] * keep, acc[j + 2][n][e] * keep, acc[j + 3][n][e] * keep};
-            __syncthreads();
-            for (int item = tid; item < 256; item += S::kThreads) {
-                const int i = item / 16, d = item % 16 * (D / 16);
-                float sum[D / 16] = {}, row_total = 0.0f, row_most = kLowest;
-#pragma unroll
-                for (int w = 0; w < GROUPS; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w * R + n * 16 + i]);
-#pragma unroll
-                for (int w = 0; w < GROUPS; ++w) {
-                    row_total += wave_total[w * R + n * 16 + i] * __builtin_amdgcn_exp2f(wave_most[w * R + n * 16 + i] - row_most);
-#pragma unroll
-                    for (int e = 0; e < D / 16; e += 4) {
-                        const f32x4 part = *reinterpret_cast<const f32x4 *>(joined + (w * 16 + i) * PITCH + d + e);
-#pragma unroll
-                        for (int f = 0; f < 4; ++f) sum[e + f] += part[f];
+                        for (int n = 0; n < NT; ++n) {
+                            const f16x8 q = __builtin_bit_cast(f16x8, q_parts[(n * STEPS + slab * 2 + half) * 64 + lane]);
+                            s[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q, s[0][n], 0, 0, 0);
+                            s[1][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q, s[1][n], 0, 0, 0);
+                        }
                     }
                 }
-                write_sums<D, D / 16>(a, p, n * 16 + i, d, sum, row_total);
-                if (item % 16 == 0) write_total<D>(a, p, n * 16 + i, row_most, row_total);
+            }
+            wait_vmcnt<VALUE_LOADS + KEY_LOADS>();
+            lds_barrier();  // its values and scales are here, and its keys used up
+            load_keys(block + 2 * GROUPS, buffer);
+            if (!here) continue;
+            const float *const scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + 4 * g;
+            float key_scale[8], value_log[8], inverse[8];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 ks = *reinterpret_cast<const f32x4 *>(scales + 16 * t), vs = *reinterpret_cast<const f32x4 *>(scales + kBlock + 16 * t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    key_scale[4 * t + e] = ks[e];
+                    value_log[4 * t + e] = __builtin_amdgcn_logf(vs[e]);
+                    inverse[4 * t + e] = inverse_scale(vs[e]);
+                }
+            }
+            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
+            f16x8 weight[NT];
+            float t[NT][8];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[n][e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
+            weigh<NT, HELD>(t, masked, dead, block, g, position, inverse, most, total, acc, weight);
+            uint32_t v[8][WORDS];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int token = kBlock + (e / 4) * 16 + 4 * g + e % 4, byte = half_of * (D / 2) + col * 4 * WORDS;
+                const char *at = record + token * D + Ring::turned(token, byte / 16) * 16 + byte % 16;
+                if constexpr (WORDS == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                    v[e][0] = x[0], v[e][1] = x[1];
+                } else {
+                    v[e][0] = *reinterpret_cast<const uint32_t *>(at);
+                }
+            }
+#pragma unroll
+            for (int word = 0; word < WORDS; ++word) {
+                uint32_t of[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) of[e] = v[e][word];
+                f16x8 part[4];
+                widen_turned(of, part);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[word * 4 + c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[c], weight[n], acc[word * 4 + c][n], 0, 0, 0);
             }
         }
+        if (record_group < 2) lds_barrier();
+        wait_vmcnt<0>();
+        __syncthreads();
+        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group, half_of);
     });
 }
 
@@ -704,7 +931,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, t[e]);
-            top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+            top = max_halves(top);
             if (__any(top > most + kSlack)) {
                 top = __builtin_fmaxf(top, most);
                 const float keep = __builtin_amdgcn_exp2f(most - top);
@@ -771,70 +998,66 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 
 // ---- the pieces joined ----------------------------------------------------------------------------
 
-struct JoinArgs {
-    AttendArgs own, prefix;
-};
-
-// A wave a (row, query head): the weights of its pieces, one a lane, and their sums in the order of the keys.
+// A wave a (row, query head): the weights of its pieces, one a lane, and their sums in the order of the keys, sixteen pieces' loads
+// at a time.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(JoinArgs a, CacheView cache, PackedView packed) {
-    constexpr int E = D / 64;
-    const AttendArgs &own = a.own;
-    const int64_t vector = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs prefix, PackedView packed) {
+    constexpr int E = D / 64, BATCH = 16;
+    typedef float Sums __attribute__((ext_vector_type(E == 1 ? 2 : E)));
+    const int64_t vector = (int64_t)blockIdx.x * (blockDim.x / 64) + uniform((int)threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, row = (int)(vector / own.q_heads), h = (int)(vector % own.q_heads);
-    if (row >= packed.rows) return;
-    const int r = request_of(packed.starts, packed.requests, row);
-    if (r < 0) return;
+    if (row >= packed.rows || row >= packed.starts[packed.requests] || row < packed.starts[0]) return;
+    Pieces mine = own.pieces[vector];
+    if (mine.count == 1 && !own.partial) return;
     float top = kLowest, total = 0.0f, o[E] = {};
-    // The pieces of one segment of a launch; `only`: leave a segment of one piece, which is written already.
-    auto pieces = [&](const AttendArgs &l, const Span &span, int64_t before, int64_t segment, int64_t all, bool only) {
-        const TileShape &tile = l.tile;
-        const int x = (row - span.begin) * tile.group + h % tile.group, t = x / tile.rows, i = x - t * tile.rows, head = h / tile.group;
-        const int tiles = tiles_of(span, tile);
-        if (segment + (int64_t)head * tiles + t >= l.segment_slots) return false;
-        const int64_t start = before + head * units_before(span, tile, tiles) + units_before(span, tile, t);
-        const int sharers = sharers_of(all, tile.workgroups), w0 = owner_of(all, sharers, start);
-        const int count = owner_of(all, sharers, start + tile_units(span, tile, t) - 1) - w0 + 1;
-        if (only && count == 1) return false;
-        const int64_t size = tile.rows * (int64_t)(D + 2);
-        auto slot = [&](int j) { return l.slots + (j == 0 ? segment + (int64_t)head * tiles + t : l.segment_slots + w0 + j) * size; };
-        for (int base = 0; base < count; base += 64) {
-            const int j = base + lane;
+    auto join = [&](const AttendArgs &l, const Pieces &p) {
+        const int rows = l.tile.rows, last = (int)l.segment_slots + l.tile.workgroups;
+        const int64_t size = rows * (int64_t)(D + 2);
+        // (Of rows that no request has, where starts do not ascend, this is what the workspace happened to hold.)
+        if (p.slot < 0 || p.slot >= last || p.workgroup < 0 || p.count < 1 || p.count > l.tile.workgroups - p.workgroup || p.at < 0 || p.at >= rows) return;
+        auto slot = [&](int j) { return l.slots + (j == 0 ? p.slot : l.segment_slots + p.workgroup + j) * size; };
+        for (int base = 0; base < p.count; base += 64) {
+            const int j = base + lane, here = min(64, p.count - base);
             float most = kLowest, sum = 0.0f;
-            if (j < count) {
-                const float *at = slot(j) + (int64_t)tile.rows * D + i;
-                most = at[0], sum = at[tile.rows];
+            if (j < p.count) {
+                const float *at = slot(j) + (int64_t)rows * D + p.at;
+                most = at[0], sum = at[rows];
             }
             float now = __builtin_fmaxf(top, most);
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) now = __builtin_fmaxf(now, __shfl_xor(now, m));
             const float keep = __builtin_amdgcn_exp2f(top - now), weight = __builtin_amdgcn_exp2f(most - now);
             top = now;
-            total *= keep;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= keep;
             sum *= weight;
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-            total += sum;
-            const int here = min(64, count - base);
-#pragma unroll 4
-            for (int j2 = 0; j2 < here; ++j2) {
-                const float w = __shfl(weight, j2);
-                const float *at = slot(base + j2) + (int64_t)i * D + lane * E;
+            total = total * keep + sum;
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[e] += w * at[e];
+            for (int e = 0; e < E; ++e) o[e] *= keep;
+            for (int first = 0; first < here; first += BATCH) {
+                float part[BATCH][E];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const float *at = slot(base + min(first + k, here - 1)) + (int64_t)p.at * D + lane * E;
+                    if constexpr (E == 1) {
+                        part[k][0] = *at;
+                    } else {
+                        const Sums v = *reinterpret_cast<const Sums *>(at);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) part[k][e] = v[e];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const float w = __shfl(weight, (first + k) & 63);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = first + k < here ? o[e] + w * part[k][e] : o[e];
+                }
             }
         }
-        return true;
     };
-    if (own.partial) {
-        const Span span = prefix_span(packed, own.shared);
-        const TileShape &tile = a.prefix.tile;
-        pieces(a.prefix, span, 0, 0, tile.heads * units_before(span, tile, tiles_of(span, tile)), false);
-    }
-    if (!pieces(own, own_span(packed, cache.page_tokens, own.shared, r), own.units[r], own.segments[r], own.units[packed.requests], !own.partial))
-        return;
+    if (own.partial) join(prefix, prefix.pieces[vector]);
+    join(own, mine);
     uint16_t *at = own.out + row * own.ld_out + (int64_t)h * D + lane * E;
     const float inv = 1.0f / total;
 #pragma unroll
@@ -857,7 +1080,7 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     p.few = vectors <= 64;
     const int nt = (int)((vectors + 15) / 16);
     p.tile.rows = p.few ? 16 * nt : kManyRows;
-    p.tile.keys = !p.few ? kManyKeys : cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups * kBlock : FewShape<64, 1>::kGroups * kBlock;
+    p.tile.keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? PairShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
     p.tile.group = (int)(q_heads / cache.heads);
     p.tile.heads = (int)cache.heads;
     p.tile.workgroups = p.few && cache.dim < 256 ? 2 * cus : cus;
@@ -870,28 +1093,34 @@ static AttendPlan plan_own(const splosh_cache &cache, int64_t requests, int64_t 
 static AttendPlan plan_prefix(const splosh_cache &cache, int64_t rows, int64_t q_heads) {
     return plan_launch(rows * (q_heads / cache.heads), 1, rows, q_heads, cache);
 }
-static size_t tables_bytes(int64_t requests) { return ((size_t)requests + 1) * 2 * sizeof(int64_t); }
+// Where the vectors' pieces are, of each launch.
+static size_t pieces_bytes(int64_t rows, int64_t q_heads) { return (size_t)(rows * q_heads) * sizeof(Pieces); }
 
 size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t shared) {
     size_t slots = plan_own(cache, requests, rows, q_heads).slot_bytes();
     if (shared > 0) slots += plan_prefix(cache, rows, q_heads).slot_bytes();
-    return kAttendCounterBytes + tables_bytes(requests) + slots * (size_t)(cache.dim + 2) * sizeof(float);
+    return kAttendCounterBytes + (shared > 0 ? 2 : 1) * pieces_bytes(rows, q_heads) + slots * (size_t)(cache.dim + 2) * sizeof(float);
+}
+
+// (More dynamic LDS than the default 64 KiB has to be allowed, once a device.)
+template <typename S, typename K>
+static void launch_lds(K kernel, int grid, hipStream_t stream, const AttendArgs &a, const CacheView &cache, const PackedView &packed) {
+    static std::once_flag allowed[64];
+    int device = 0;
+    (void)hipGetDevice(&device);
+    std::call_once(allowed[device & 63], [&] {
+        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+    });
+    kernel<<<grid, S::kThreads, S::kLds, stream>>>(a, cache, packed);
 }
 
 template <int D>
 static void launch_part(const AttendPlan &plan, const AttendArgs &a, const CacheView &cache, const PackedView &packed,
                         hipStream_t stream) {
     auto few = [&](auto tiles) {
-        typedef FewShape<D, decltype(tiles)::value> S;
-        auto kernel = few_kernel<D, decltype(tiles)::value>;
-        // (Allowed once a device: more dynamic LDS than the default 64 KiB.)
-        static std::once_flag allowed[64];
-        int device = 0;
-        (void)hipGetDevice(&device);
-        std::call_once(allowed[device & 63], [&] {
-            (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
-        });
-        kernel<<<plan.tile.workgroups, S::kThreads, S::kLds, stream>>>(a, cache, packed);
+        constexpr int NT = decltype(tiles)::value;
+        if constexpr (D / 16 * NT * 4 > 96) launch_lds<PairShape<D, NT>>(pair_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
+        else launch_lds<FewShape<D, NT>>(few_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
     };
     if (!plan.few) many_kernel<D><<<plan.tile.workgroups, kManyThreads, record_bytes(D), stream>>>(a, cache, packed);
     else if (plan.tile.rows == 16) few(std::integral_constant<int, 1>{});
@@ -910,9 +1139,8 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
     a.q_heads = (int)q_heads, a.shared = (int)shared;
     a.wide = reinterpret_cast<uintptr_t>(q) % 16 == 0 && row_stride % 8 == 0 && head_stride % 8 == 0;
     a.factor = scale * 1.4426950408889634f;
-    a.units = reinterpret_cast<int64_t *>(at);
-    a.segments = a.units + packed.requests + 1;
-    a.slots = reinterpret_cast<float *>(at + tables_bytes(packed.requests));
+    a.pieces = reinterpret_cast<Pieces *>(at);
+    a.slots = reinterpret_cast<float *>(at + (shared > 0 ? 2 : 1) * pieces_bytes(rows, q_heads));
     a.tile = own.tile, a.segment_slots = own.segment_slots, a.partial = shared > 0;
     const CacheView cv = view_of(cache);
     const PackedView pv = view_of(packed, rows);
@@ -921,13 +1149,16 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
     if (shared > 0) {
         prefix = plan_prefix(cache, rows, q_heads);
         b.tile = prefix.tile, b.segment_slots = prefix.segment_slots, b.prefix = 1;
+        b.pieces = a.pieces + rows * q_heads;
         b.slots = a.slots + own.slot_bytes() * (cache.dim + 2);
     }
     auto run = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         if (shared > 0) launch_part<D>(prefix, b, cv, pv, stream);
         launch_part<D>(own, a, cv, pv, stream);
-        join_kernel<D><<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, stream>>>(JoinArgs{a, b}, cv, pv);
+        // (Few vectors: a workgroup each, so that they spread over the CUs.)
+        const int waves = rows * q_heads <= 4096 ? 1 : 4;
+        join_kernel<D><<<(unsigned)((rows * q_heads + waves - 1) / waves), 64 * waves, 0, stream>>>(a, b, pv);
     };
     if (cache.dim == 256) run(std::integral_constant<int, 256>{});
     else if (cache.dim == 128) run(std::integral_constant<int, 128>{});
