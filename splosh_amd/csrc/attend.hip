@@ -409,11 +409,9 @@ __device__ __forceinline__ float max_halves(float v) {
     return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The weights of a lane's eight scores of each vector: masked, against the running maxima (the sums follow where these move), summed with
-// the scales' inverses, and as the second product's operand.
-template <int NT, int HELD>
-__device__ __forceinline__ void weigh(float (&t)[NT][8], bool masked, bool dead, int block, int g, const int (&position)[NT], const float (&inverse)[8],
-                                      float (&most)[NT], float (&total)[NT], f32x4 (&acc)[HELD][NT], f16x8 (&weight)[NT]) {
+// A lane's eight scores of each vector masked, and the largest of all lanes' of the vector.
+template <int NT>
+__device__ __forceinline__ void mask_scores(float (&t)[NT][8], bool masked, bool dead, int block, int g, const int (&position)[NT], float (&top)[NT]) {
     if (masked) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -421,26 +419,18 @@ __device__ __forceinline__ void weigh(float (&t)[NT][8], bool masked, bool dead,
             for (int e = 0; e < 8; ++e)
                 t[n][e] = !dead && block * kBlock + (e / 4) * 16 + 4 * g + e % 4 <= position[n] ? t[n][e] : -__builtin_inff();
     }
-    float top[NT];
-    bool follow = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         top[n] = t[n][0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) top[n] = __builtin_fmaxf(top[n], t[n][e]);
         top[n] = max_halves(max_rows(top[n]));
-        follow |= top[n] > most[n] + kSlack;
     }
-    if (__any(follow)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float now = __builtin_fmaxf(top[n], most[n]), keep = __builtin_amdgcn_exp2f(most[n] - now);
-            most[n] = now;
-            total[n] *= keep;
-#pragma unroll
-            for (int j = 0; j < HELD; ++j) acc[j][n] *= keep;
-        }
-    }
+}
+
+// Their weights against the running maxima, summed with the scales' inverses, and as the second product's operand.
+template <int NT>
+__device__ __forceinline__ void weigh(const float (&t)[NT][8], const float (&inverse)[8], const float (&most)[NT], float (&total)[NT], f16x8 (&weight)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         uint32_t pairs[4];
@@ -472,9 +462,12 @@ struct FewRing {
     }
 };
 
+// (A wave a record; four would leave no room for the queries of four tiles of 256 dimensions. Where a wave's sums take more than
+// 96 registers it has its SIMD for itself, and they lie in accumulation registers.)
 template <int D, int NT>
 struct FewShape {
-    static constexpr int kGroups = 4, kThreads = 64 * kGroups, kRows = 16 * NT, kPitch = D + 4;
+    static constexpr bool kAlone = D / 16 * NT * 4 > 96;
+    static constexpr int kGroups = D == 256 && NT == 4 ? 3 : 4, kThreads = 64 * kGroups, kRows = 16 * NT, kPitch = D + 4;
     static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kQueryBytes = kRows * D * 2;
     static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions
     static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
@@ -482,7 +475,7 @@ struct FewShape {
 };
 
 template <int D, int NT>
-__global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(AttendArgs a, CacheView cache, PackedView packed) {
+__global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlone ? 1 : 2)) void few_kernel(AttendArgs a, CacheView cache, PackedView packed) {
     typedef FewShape<D, NT> S;
     typedef FewRing<D> Ring;
     constexpr int R = S::kRows, SLABS = D / 64, STEPS = D / 32, GROUPS = S::kGroups, HELD = D / 16;
@@ -534,13 +527,23 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
         const int first_position = uniform(*least);
         f32x4 acc[HELD][NT] = {};
         int buffer = 0;
-        for (int block = from + record_group; block < to; block += GROUPS, buffer ^= 1) {
-            const bool dead = hole;
-            if (block + GROUPS < to) {
-                load(block + GROUPS, buffer ^ 1);
-                wait_vmcnt<Ring::kLoads>();  // this record has landed; the next may be in flight
-            } else {
-                wait_vmcnt<0>();
+        bool waited = false, dead = false;
+        // Where a maximum moves by more than kSlack the loop over the records is left, the sums scaled, and the record
+        // begun again: inside of it nothing but the matrix instructions touches the sums. (Scaled in a branch of the loop, the compiler holds
+        // them twice, and copies 192 registers a record: 150 us for the 320 MB of the verify step.)
+        for (int block = from + record_group; block < to;) {
+        float top[NT];
+        bool moved = false;
+        do {
+            if (!waited) {
+                dead = hole;
+                if (block + GROUPS < to) {
+                    load(block + GROUPS, buffer ^ 1);
+                    wait_vmcnt<Ring::kLoads>();  // this record has landed; the next may be in flight
+                } else {
+                    wait_vmcnt<0>();
+                }
+                waited = true;
             }
             asm volatile("" ::: "memory");
             const char *const record = lds + ring + buffer * Ring::kRecord;
@@ -581,7 +584,12 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[n][e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
-            weigh<NT, HELD>(t, masked, dead, block, g, position, inverse, most, total, acc, weight);
+            mask_scores<NT>(t, masked, dead, block, g, position, top);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) moved |= top[n] > most[n] + kSlack;
+            moved = __any(moved);
+            if (moved) break;
+            weigh<NT>(t, inverse, most, total, weight);
             uint32_t v[8][SLABS];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -614,187 +622,20 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), 2) void few_kernel(Att
             // The record is read before the load after the next overwrites it.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
+            block += GROUPS, buffer ^= 1, waited = false;
+        } while (block < to);
+        if (moved) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float now = __builtin_fmaxf(top[n], most[n]), keep = __builtin_amdgcn_exp2f(most[n] - now);
+                most[n] = now;
+                total[n] *= keep;
+#pragma unroll
+                for (int j = 0; j < HELD; ++j) acc[j][n] *= keep;
+            }
+        }
         }
         join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group, 0);
-    });
-}
-
-// ---- few vectors, many sums -----------------------------------------------------------------------
-//
-// Two waves share a record where one wave's sums would take more than 96 registers (256 dimensions of two or more times sixteen
-// vectors): each holds half of the values' dimensions, and both compute the scores. They load half of each record each, so that a
-// barrier has to say what has landed and what is used up; there are two for a record, after the scores (its keys' place is
-// free: those of the record after the next are asked for) and before the next ones (the same for values), so that
-// a whole record a group is in flight at every wait. (Measured on the verify step, 320 MB: one wave with all sums, 512 registers,
-// 150 us; one barrier and one wait a record 110; half records straight to registers, the scores of either half exchanged, 131.)
-
-template <int D, int NT>
-struct PairShape {
-    static constexpr int kGroups = D == 256 && NT == 4 ? 3 : 4;  // (four would leave no room for the queries)
-    static constexpr int kThreads = 128 * kGroups, kRows = 16 * NT, kPitch = D + 4;
-    static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kNumbers = kRingBytes + kRows * D * 2;
-    static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
-    static_assert(kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
-};
-
-template <int D, int NT>
-__global__ __launch_bounds__((PairShape<D, NT>::kThreads)) void pair_kernel(AttendArgs a, CacheView cache, PackedView packed) {
-    typedef PairShape<D, NT> S;
-    typedef FewRing<D> Ring;
-    constexpr int R = S::kRows, SLABS = D / 64, STEPS = D / 32, GROUPS = S::kGroups;
-    constexpr int HELD = D / 32, WORDS = D / 128;  // tiles, and dwords of a value's run, of half of the dimensions
-    constexpr int KEY_LOADS = kBlock * D / 2048, VALUE_LOADS = KEY_LOADS + 1;  // of a wave: half of the codes; the scales with the values
-    extern __shared__ __align__(16) char lds[];
-    float *const joined = reinterpret_cast<float *>(lds);  // [group][16][PITCH], in the ring's place
-    u32x4 *const q_parts = reinterpret_cast<u32x4 *>(lds + S::kRingBytes);
-    float *const wave_most = reinterpret_cast<float *>(lds + S::kNumbers), *const wave_total = wave_most + GROUPS * R;
-    float *const row_factor = wave_total + GROUPS * R;
-    int *const row_position = reinterpret_cast<int *>(row_factor + R), *const least = row_position + R;
-    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
-    const int record_group = wave >> 1, half_of = wave & 1, ring = record_group * 2 * Ring::kRecord;
-
-    // (The sources of a record's loads as in few_kernel.)
-    constexpr int SOURCES = D == 256 ? 4 : 1;
-    uint32_t source[SOURCES];
-#pragma unroll
-    for (int j = 0; j < SOURCES; ++j)
-        source[j] = (uint32_t)(lane / Ring::kRuns * D + Ring::turned(j * (1024 / D) + lane / Ring::kRuns, lane % Ring::kRuns) * 16);
-
-    for_pieces<S::kThreads>(a, cache, packed, [&](const Piece &p) {
-        Pages pages(packed, a.prefix ? 0 : p.request);
-        const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
-        bool hole;
-        // (Past the last block nothing is read: every lane's offset is past the end. The counts stay the same.)
-        auto source_of = [&](int block) {
-            hole = false;
-            const uint8_t *record = block < to ? block_record<D>(cache, pages, p.head, block, hole) : cache.data;
-            return make_rsrc(record, block < to ? Ring::kRecord : 0);
-        };
-        auto load_keys = [&](int block, int buffer) {
-            const rsrc_t r = source_of(block);
-            char *at = lds + uniform(ring + buffer * Ring::kRecord);
-#pragma unroll
-            for (int i = 0; i < KEY_LOADS; ++i) {
-                const int j = 2 * i + half_of;
-                buffer_load_lds16(r, at + j * 1024, source[SOURCES == 1 ? 0 : (2 * i) % 4 + half_of] + j * 1024);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        auto load_values = [&](int block, int buffer) {
-            const rsrc_t r = source_of(block);
-            char *at = lds + uniform(ring + buffer * Ring::kRecord);
-#pragma unroll
-            for (int i = 0; i < KEY_LOADS; ++i) {
-                const int j = 2 * KEY_LOADS + 2 * i + half_of;
-                buffer_load_lds16(r, at + j * 1024, source[SOURCES == 1 ? 0 : (2 * i) % 4 + half_of] + j * 1024);
-            }
-            buffer_load_lds4(r, at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);  // (both waves: the same)
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        __syncthreads();  // (the last piece's LDS is read)
-        load_keys(from + record_group, 0);
-        load_values(from + record_group, 0);
-        bool dead_next = hole;
-        load_keys(from + record_group + GROUPS, 1);
-        if (tid == 0) *least = INT_MAX;
-        lds_barrier();
-        stage_queries<D, R, S::kThreads>(a, packed, p, q_parts, row_factor, row_position, least);
-        lds_barrier();
-        float factor[NT], most[NT], total[NT];
-        int position[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            factor[n] = row_factor[n * 16 + col], position[n] = row_position[n * 16 + col];
-            most[n] = kLowest, total[n] = 0.0f;
-        }
-        const int first_position = uniform(*least);
-        f32x4 acc[HELD][NT] = {};
-        int buffer = 0;
-        // Groups from the third on are one barrier behind: while the others compute scores (LDS and matrix instructions), they weigh values
-        // (vector instructions), on the same SIMDs.
-        if (record_group >= 2) lds_barrier();
-        for (int first = from; first < to; first += GROUPS, buffer ^= 1) {
-            const int block = first + record_group;
-            const bool here = block < to, dead = dead_next;
-            const char *const record = lds + ring + buffer * Ring::kRecord;
-            wait_vmcnt<VALUE_LOADS + KEY_LOADS>();
-            lds_barrier();  // this record's keys are here, and the last one's values used up
-            load_values(block + GROUPS, buffer ^ 1);
-            dead_next = hole;
-            f32x4 s[2][NT] = {};
-            if (here) {
-#pragma unroll
-                for (int slab = 0; slab < SLABS; ++slab) {
-                    u32x4 k[2];
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        k[t] = *reinterpret_cast<const u32x4 *>(record + (t * 16 + col) * D + Ring::turned(t * 16 + col, slab * 4 + g) * 16);
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const f16x8 k0 = widen8(k[0][2 * half], k[0][2 * half + 1]), k1 = widen8(k[1][2 * half], k[1][2 * half + 1]);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const f16x8 q = __builtin_bit_cast(f16x8, q_parts[(n * STEPS + slab * 2 + half) * 64 + lane]);
-                            s[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q, s[0][n], 0, 0, 0);
-                            s[1][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q, s[1][n], 0, 0, 0);
-                        }
-                    }
-                }
-            }
-            wait_vmcnt<VALUE_LOADS + KEY_LOADS>();
-            lds_barrier();  // its values and scales are here, and its keys used up
-            load_keys(block + 2 * GROUPS, buffer);
-            if (!here) continue;
-            const float *const scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + 4 * g;
-            float key_scale[8], value_log[8], inverse[8];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const f32x4 ks = *reinterpret_cast<const f32x4 *>(scales + 16 * t), vs = *reinterpret_cast<const f32x4 *>(scales + kBlock + 16 * t);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    key_scale[4 * t + e] = ks[e];
-                    value_log[4 * t + e] = __builtin_amdgcn_logf(vs[e]);
-                    inverse[4 * t + e] = inverse_scale(vs[e]);
-                }
-            }
-            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
-            f16x8 weight[NT];
-            float t[NT][8];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) t[n][e] = __builtin_fmaf(s[e / 4][n][e % 4], key_scale[e] * factor[n], value_log[e]);
-            weigh<NT, HELD>(t, masked, dead, block, g, position, inverse, most, total, acc, weight);
-            uint32_t v[8][WORDS];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int token = kBlock + (e / 4) * 16 + 4 * g + e % 4, byte = half_of * (D / 2) + col * 4 * WORDS;
-                const char *at = record + token * D + Ring::turned(token, byte / 16) * 16 + byte % 16;
-                if constexpr (WORDS == 2) {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
-                    v[e][0] = x[0], v[e][1] = x[1];
-                } else {
-                    v[e][0] = *reinterpret_cast<const uint32_t *>(at);
-                }
-            }
-#pragma unroll
-            for (int word = 0; word < WORDS; ++word) {
-                uint32_t of[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) of[e] = v[e][word];
-                f16x8 part[4];
-                widen_turned(of, part);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        acc[word * 4 + c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[c], weight[n], acc[word * 4 + c][n], 0, 0, 0);
-            }
-        }
-        if (record_group < 2) lds_barrier();
-        wait_vmcnt<0>();
-        __syncthreads();
-        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group, half_of);
     });
 }
 
@@ -1080,7 +921,7 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     p.few = vectors <= 64;
     const int nt = (int)((vectors + 15) / 16);
     p.tile.rows = p.few ? 16 * nt : kManyRows;
-    p.tile.keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? PairShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
+    p.tile.keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
     p.tile.group = (int)(q_heads / cache.heads);
     p.tile.heads = (int)cache.heads;
     p.tile.workgroups = p.few && cache.dim < 256 ? 2 * cus : cus;
@@ -1119,8 +960,7 @@ static void launch_part(const AttendPlan &plan, const AttendArgs &a, const Cache
                         hipStream_t stream) {
     auto few = [&](auto tiles) {
         constexpr int NT = decltype(tiles)::value;
-        if constexpr (D / 16 * NT * 4 > 96) launch_lds<PairShape<D, NT>>(pair_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
-        else launch_lds<FewShape<D, NT>>(few_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
+        launch_lds<FewShape<D, NT>>(few_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
     };
     if (!plan.few) many_kernel<D><<<plan.tile.workgroups, kManyThreads, record_bytes(D), stream>>>(a, cache, packed);
     else if (plan.tile.rows == 16) few(std::integral_constant<int, 1>{});
