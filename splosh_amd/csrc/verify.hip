@@ -51,23 +51,20 @@ struct VerifyArgs {
     StripSums *strips;
 };
 
-// 2^x, x <= 0, to 1e-13: the whole part as the exponent, the fraction (|f| <= 1/2) by its series in f ln 2.
+// 2^x, x <= 0, to 1e-9 of it: the whole part as the exponent, and of the fraction (|f| <= 1/2) the series in f ln 2, from the third power on
+// in fp32 (that part is below 0.008: off by 5e-10 at most, where it ends with the eighth power by 2e-10). All of it in 64 bits
+// takes twice the time: 30 us for the 64 rows of 248320, and the sums gain nothing by it.
 __device__ __forceinline__ double power2(double x) {
-    if (!(x > -1000.0)) return 0.0;
-    const double n = __builtin_rint(x), f = (x - n) * 0.6931471805599453;
-    double e = 1.0 / 479001600.0;
-    e = e * f + 1.0 / 39916800.0;
-    e = e * f + 1.0 / 3628800.0;
-    e = e * f + 1.0 / 362880.0;
-    e = e * f + 1.0 / 40320.0;
-    e = e * f + 1.0 / 5040.0;
-    e = e * f + 1.0 / 720.0;
-    e = e * f + 1.0 / 120.0;
-    e = e * f + 1.0 / 24.0;
-    e = e * f + 1.0 / 6.0;
-    e = e * f + 0.5;
-    e = e * f + 1.0;
-    e = e * f + 1.0;
+    x = __builtin_fmax(x, -2000.0);  // (0 from 2^-1075 on)
+    const double n = __builtin_rint(x), f = x - n;
+    const float g = (float)f;
+    float h = 1.3215487e-6f;
+    h = __builtin_fmaf(h, g, 1.5252734e-5f);
+    h = __builtin_fmaf(h, g, 1.5403530e-4f);
+    h = __builtin_fmaf(h, g, 1.3333558e-3f);
+    h = __builtin_fmaf(h, g, 9.6181291e-3f);
+    h = __builtin_fmaf(h, g, 5.5504109e-2f);
+    const double e = __builtin_fma(__builtin_fma(__builtin_fma((double)h, f, 0.24022650695910072), f, 0.6931471805599453), f, 1.0);
     return __builtin_ldexp(e, (int)n);
 }
 
@@ -84,6 +81,34 @@ __device__ __forceinline__ double weight_of(float v, float most, double by, bool
     if (by == 0.0) return first ? 1.0 : 0.0;
     if (v == most) return 1.0;
     return most == __builtin_inff() ? 0.0 : power2(((double)v - (double)most) * by);
+}
+
+// Four entries in a row, of a row of any alignment, the first `here` of which are its.
+struct __attribute__((packed, aligned(4))) Four32 {
+    float v[4];
+};
+struct __attribute__((packed, aligned(2))) Four16 {
+    uint16_t v[4];
+};
+__device__ __forceinline__ void entries(const float *p, int here, float (&v)[4]) {
+    if (here >= 4) {
+        const Four32 x = *reinterpret_cast<const Four32 *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x.v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < here ? p[e] : -__builtin_inff();
+    }
+}
+__device__ __forceinline__ void entries(const uint16_t *p, int here, float (&v)[4]) {
+    if (here >= 4) {
+        const Four16 x = *reinterpret_cast<const Four16 *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = bf16_bits_to_f32(x.v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < here ? bf16_bits_to_f32(p[e]) : -__builtin_inff();
+    }
 }
 
 __device__ __forceinline__ float entry(const float *p) { return *p; }
@@ -115,13 +140,15 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
     const int r = row_request(a.starts, a.requests, row);
     if (r < 0) return;
     const T *logits = (const T *)a.logits + row * a.ld;
-    const int begin = piece * kPiece + wave * kStrip + lane;
-    float v[kPer], most = -__builtin_inff();
+    const int begin = piece * kPiece + wave * kStrip + lane * 4;  // its entries: four in a row, 256 further the next four
+    float v[kPer / 4][4], most = -__builtin_inff();
     int first = INT_MAX;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = begin + 64 * e < a.vocab ? entry(logits + begin + 64 * e) : -__builtin_inff();
+    for (int k = 0; k < kPer / 4; ++k) entries(logits + begin + 256 * k, a.vocab - begin - 256 * k, v[k]);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) keep_first(most, first, v[e], begin + 64 * e);
+    for (int k = 0; k < kPer / 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keep_first(most, first, v[k][e], begin + 256 * k + e);
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) keep_first(most, first, __shfl_xor(most, m), __shfl_xor(first, m));
     if (lane == 0) wave_most[wave] = most, wave_first[wave] = first;
@@ -130,7 +157,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
     const double by = factor_of(a.temperature, r);
     double sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) sum += weight_of(v[e], most, by, begin + 64 * e == first);
+    for (int k = 0; k < kPer / 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += weight_of(v[k][e], most, by, begin + 256 * k + e == first);
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
     if (lane == 0) wave_total[wave] = sum;
@@ -166,18 +195,39 @@ __device__ __forceinline__ double draft_of(const VerifyArgs &a, int row, int tok
 // u of a row: below 0 or NaN as 0.
 __device__ __forceinline__ double uniform_of(const VerifyArgs &a, int row) { return __builtin_fmax((double)a.uniforms[row], 0.0); }
 
-// (weight of max(p - q, 0), of p) of one entry of the decided row.
-template <typename T>
-__device__ __forceinline__ StripSums rest_of(const VerifyArgs &a, const Decision &d, int drafted, int token) {
-    if (token >= a.vocab || !(d.total > 0.0)) return {0.0, 0.0};
-    const double p = weight_of(entry((const T *)a.logits + d.row * a.ld + token), d.most, d.by, token == d.top) / d.total;
-    return {d.last ? p : __builtin_fmax(p - draft_of(a, d.row, token, drafted), 0.0), p};
+// (weight of max(p - q, 0), of p) of N entries of the decided row from `token` on, four in a row and `step` further the next four.
+template <typename T, int N>
+__device__ __forceinline__ void rests_of(const VerifyArgs &a, const Decision &d, int drafted, int token, int step, StripSums (&w)[N]) {
+    float v[N / 4][4], q[N / 4][4];
+    const T *logits = (const T *)a.logits + d.row * a.ld;
+    const bool whole = d.last || !a.draft;
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) entries(logits + token + k * step, a.vocab - token - k * step, v[k]);
+    if (!whole) {
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+            const int64_t at = d.row * a.ld_draft + token + k * step;
+            if (a.draft_f32) entries((const float *)a.draft + at, a.vocab - token - k * step, q[k]);
+            else entries((const uint16_t *)a.draft + at, a.vocab - token - k * step, q[k]);
+        }
+    }
+    const double inv = d.total > 0.0 ? 1.0 / d.total : 0.0;
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = token + k * step + e;
+            const double p = weight_of(v[k][e], d.most, d.by, i == d.top) * inv;
+            const double taken = d.last ? 0.0 : !a.draft ? (i == drafted ? 1.0 : 0.0) : (double)q[k][e];
+            w[4 * k + e] = {p > 0.0 ? __builtin_fmax(p - taken, 0.0) : 0.0, p};  // (past the vocabulary p is 0)
+        }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
+    constexpr int kKept = 64;
     __shared__ int stop;
-    __shared__ Decision decision;
+    __shared__ PieceStats kept[kKept];
     const int r = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int begin = max(a.starts[r], 0), end = min(a.starts[r + 1], a.rows);
     if (begin >= end) {
@@ -187,35 +237,35 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
     if (tid == 0) stop = end - 1;
     __syncthreads();
     const double by = factor_of(a.temperature, r);
-    for (int row = begin + wave; row < end - 1; row += kWaves) {
-        const PieceStats s = row_stats(a, row, by);
-        const int t = a.tokens[row + 1];
+    // A wave a row; what the deciding row's numbers are is kept for as many rows as there is room for.
+    for (int row = begin + wave; row < end; row += kWaves) {
+        const int t = row + 1 < end ? a.tokens[row + 1] : -1;
         bool accept = t >= 0 && t < a.vocab;
-        if (accept) {
-            const double p = weight_of(entry((const T *)a.logits + row * a.ld + t), s.most, by, t == s.first);
-            accept = s.sum > 0.0 && uniform_of(a, row) * draft_of(a, row, t, t) < p / s.sum;
+        const float logit = accept ? entry((const T *)a.logits + row * a.ld + t) : 0.0f;
+        const double u = uniform_of(a, row), q = accept ? draft_of(a, row, t, t) : 0.0;
+        const PieceStats s = row_stats(a, row, by);
+        if (accept) accept = s.sum > 0.0 && u * q < weight_of(logit, s.most, by, t == s.first) / s.sum;
+        if (lane == 0) {
+            if (!accept) atomicMin(&stop, row);
+            if (row - begin < kKept) kept[row - begin] = s;
         }
-        if (!accept && lane == 0) atomicMin(&stop, row);
     }
     __syncthreads();
-    if (wave == 0) {
-        const PieceStats s = row_stats(a, stop, by);
-        if (lane == 0) decision = {stop, stop == end - 1, s.first, s.most, s.sum, by};
-    }
-    __syncthreads();
-    const Decision d = decision;
+    const int last = stop;
+    PieceStats s;
+    if (last - begin < kKept) s = kept[last - begin];
+    else s = row_stats(a, last, by);
+    const Decision d = {last, last == end - 1, s.first, s.most, s.sum, by};
     const int drafted = d.last ? -1 : a.tokens[d.row + 1];
     if (piece == 0) {
         if (tid == 0) a.decisions[r] = d, a.accepted[r] = d.row - begin;
         for (int row = begin + tid; row < end; row += kThreads)
             if (row != d.row) a.out[row] = row < d.row ? a.tokens[row + 1] : -1;
     }
-    StripSums sum{0.0, 0.0};
+    StripSums sum{0.0, 0.0}, w[kPer];
+    rests_of<T, kPer>(a, d, drafted, piece * kPiece + wave * kStrip + lane * 4, 256, w);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const StripSums w = rest_of<T>(a, d, drafted, piece * kPiece + wave * kStrip + 64 * e + lane);
-        sum.rest += w.rest, sum.whole += w.whole;
-    }
+    for (int e = 0; e < kPer; ++e) sum.rest += w[e].rest, sum.whole += w[e].whole;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) sum.rest += __shfl_xor(sum.rest, m), sum.whole += __shfl_xor(sum.whole, m);
     if (lane == 0) a.strips[((int64_t)r * a.pieces + piece) * kWaves + wave] = sum;
@@ -232,44 +282,64 @@ __device__ __forceinline__ double wave_running(double v) {
     return v;
 }
 
-// One wave a request: strips by the lane, then the strip's entries 64 at a time.
+// One wave a request. The strips, and then the entries of the one that the draw falls into, lie in runs over the lanes: the lane whose
+// run the draw falls into goes through it.
 template <typename T>
 __global__ __launch_bounds__(64) void finish_kernel(VerifyArgs a) {
     const int r = blockIdx.x, lane = threadIdx.x;
     const Decision d = a.decisions[r];
     if (d.row < 0) return;
     const StripSums *strips = a.strips + (int64_t)r * a.pieces * kWaves;
-    const int count = a.pieces * kWaves, drafted = d.last ? -1 : a.tokens[d.row + 1];
+    const int count = a.pieces * kWaves, drafted = d.last ? -1 : a.tokens[d.row + 1], run = (count + 63) / 64;
+    const int low = min(lane * run, count), high = min(low + run, count);
+    const double u = uniform_of(a, min(a.starts[r + 1], a.rows) - 1);
     double rest = 0.0, whole = 0.0;
-    for (int i = lane; i < count; i += 64) rest += strips[i].rest, whole += strips[i].whole;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) rest += __shfl_xor(rest, m), whole += __shfl_xor(whole, m);
-    const bool from_rest = rest > 0.0;
-    const double most = uniform_of(a, min(a.starts[r + 1], a.rows) - 1) * (from_rest ? rest : whole);
-    // The strip whose running weight passes the draw; the last one with weight if none does.
-    double before = 0.0, strip_before = 0.0;
-    int strip = -1;
-    for (int base = 0; base < count; base += 64) {
-        const int i = base + lane;
-        const double w = i < count ? (from_rest ? strips[i].rest : strips[i].whole) : 0.0;
-        const double running = before + wave_running(w);
-        const uint64_t passed = __ballot(w > 0.0 && running > most), with = __ballot(w > 0.0);
-        const int at = passed ? __builtin_ctzll(passed) : with ? 63 - __builtin_clzll(with) : -1;
-        if (at >= 0) strip = base + at, strip_before = __shfl(running - w, at);
-        if (passed) break;
-        before = __shfl(running, 63);
-    }
+#pragma unroll 4
+    for (int i = low; i < high; ++i) rest += strips[i].rest, whole += strips[i].whole;
+    const double rests = wave_running(rest), wholes = wave_running(whole);
+    const bool from_rest = __shfl(rests, 63) > 0.0;
+    const double total = from_rest ? __shfl(rests, 63) : __shfl(wholes, 63), draw = u * total;
+    // The lane that the draw falls into: the first whose running weight passes it, or, if none does, the last with weight.
+    auto lane_of = [&](double own, double running) {
+        const uint64_t passed = __ballot(own > 0.0 && running > draw), with = __ballot(own > 0.0);
+        return passed ? __builtin_ctzll(passed) : with ? 63 - __builtin_clzll(with) : -1;
+    };
+    const double mine = from_rest ? rest : whole, running = from_rest ? rests : wholes;
+    const int at = lane_of(mine, running);
     int token = -1;
-    if (strip >= 0) {
-        before = strip_before;
-        for (int e = 0; e < kPer; ++e) {
-            const StripSums s = rest_of<T>(a, d, drafted, strip * kStrip + 64 * e + lane);
-            const double w = from_rest ? s.rest : s.whole, running = before + wave_running(w);
-            const uint64_t passed = __ballot(w > 0.0 && running > most), with = __ballot(w > 0.0);
-            const int at = passed ? __builtin_ctzll(passed) : with ? 63 - __builtin_clzll(with) : -1;
-            if (at >= 0) token = strip * kStrip + 64 * e + at;
-            if (passed) break;
-            before = __shfl(running, 63);
+    if (at >= 0) {
+        // That lane's strips one by one (all lanes go along with it).
+        const int first = __shfl(low, at), end = __shfl(high, at);
+        double before = __shfl(running - mine, at), strip_before = before;
+        int strip = -1;
+        for (int i = first; i < end; ++i) {
+            const double w = from_rest ? strips[i].rest : strips[i].whole;
+            if (w > 0.0) {
+                strip = i, strip_before = before;
+                if (before + w > draw) break;
+            }
+            before += w;
+        }
+        if (strip >= 0) {
+            StripSums w[kPer];
+            rests_of<T, kPer>(a, d, drafted, strip * kStrip + lane * kPer, 4, w);
+            double own = 0.0;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) own += from_rest ? w[e].rest : w[e].whole;
+            const double to = strip_before + wave_running(own);
+            const int found = lane_of(own, to);
+            double sum = to - own;
+            int entry_of = -1;
+            bool done = false;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const double x = from_rest ? w[e].rest : w[e].whole;
+                if (x > 0.0 && !done) entry_of = e;
+                sum += x;
+                done |= x > 0.0 && sum > draw;
+            }
+            const int entry_there = __shfl(entry_of, found < 0 ? 0 : found);
+            if (found >= 0 && entry_there >= 0) token = strip * kStrip + found * kPer + entry_there;
         }
     }
     if (lane == 0) a.out[d.row] = token;
