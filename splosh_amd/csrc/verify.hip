@@ -111,6 +111,26 @@ __device__ __forceinline__ void entries(const uint16_t *p, int here, float (&v)[
     }
 }
 
+// The weights of N entries in fours from index `first` on, `step` further the next four. With a finite `most` and a T, NaN and -inf go the way of
+// what is far below it: 2^-2000.
+template <int N>
+__device__ __forceinline__ void weights_of(const float (&v)[N / 4][4], float most, double by, int first, int step, int top, double (&w)[N]) {
+    if (by > 0.0 && __builtin_fabsf(most) < __builtin_inff()) {
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * k + e] = power2(((double)v[k][e] - (double)most) * by);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool one = by == 0.0 ? first + k * step + e == top : v[k][e] == most;
+                w[4 * k + e] = one && v[k][e] > -__builtin_inff() ? 1.0 : 0.0;
+            }
+    }
+}
+
 __device__ __forceinline__ float entry(const float *p) { return *p; }
 __device__ __forceinline__ float entry(const uint16_t *p) { return bf16_bits_to_f32(*p); }
 
@@ -142,30 +162,39 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
     const T *logits = (const T *)a.logits + row * a.ld;
     const int begin = piece * kPiece + wave * kStrip + lane * 4;  // its entries: four in a row, 256 further the next four
     float v[kPer / 4][4], most = -__builtin_inff();
-    int first = INT_MAX;
 #pragma unroll
     for (int k = 0; k < kPer / 4; ++k) entries(logits + begin + 256 * k, a.vocab - begin - 256 * k, v[k]);
 #pragma unroll
     for (int k = 0; k < kPer / 4; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) keep_first(most, first, v[k][e], begin + 256 * k + e);
+        for (int e = 0; e < 4; ++e) most = __builtin_fmaxf(most, v[k][e]);
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) keep_first(most, first, __shfl_xor(most, m), __shfl_xor(first, m));
-    if (lane == 0) wave_most[wave] = most, wave_first[wave] = first;
+    for (int m = 1; m < 64; m <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, m));
+    if (lane == 0) wave_most[wave] = most;
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) keep_first(most, first, wave_most[w], wave_first[w]);
-    const double by = factor_of(a.temperature, r);
-    double sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most = __builtin_fmaxf(most, wave_most[w]);
+    int first = INT_MAX;
 #pragma unroll
     for (int k = 0; k < kPer / 4; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += weight_of(v[k][e], most, by, begin + 256 * k + e == first);
+        for (int e = 0; e < 4; ++e) first = min(first, v[k][e] == most ? begin + 256 * k + e : INT_MAX);
+    const double by = factor_of(a.temperature, r);
+    double sum = 0.0, w[kPer];
+    // (Of a greedy row any one entry of the largest value stands for the piece: its first is found below.)
+    if (by > 0.0) {
+        weights_of<kPer>(v, most, by, begin, 256, -1, w);
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+        for (int e = 0; e < kPer; ++e) sum += w[e];
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m), first = min(first, __shfl_xor(first, m));
+    if (lane == 0) wave_first[wave] = first;
     if (lane == 0) wave_total[wave] = sum;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kWaves; ++w) sum += wave_total[w];
+        for (int w = 1; w < kWaves; ++w) sum += wave_total[w], first = min(first, wave_first[w]);
+        if (by == 0.0) sum = most > -__builtin_inff() ? 1.0 : 0.0;
         a.stats[(int64_t)row * a.pieces + piece] = {sum, most, first};
     }
 }
@@ -212,12 +241,14 @@ __device__ __forceinline__ void rests_of(const VerifyArgs &a, const Decision &d,
         }
     }
     const double inv = d.total > 0.0 ? 1.0 / d.total : 0.0;
+    double weight[N];
+    weights_of<N>(v, d.most, d.by, token, step, d.top, weight);
 #pragma unroll
     for (int k = 0; k < N / 4; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = token + k * step + e;
-            const double p = weight_of(v[k][e], d.most, d.by, i == d.top) * inv;
+            const double p = weight[4 * k + e] * inv;
             const double taken = d.last ? 0.0 : !a.draft ? (i == drafted ? 1.0 : 0.0) : (double)q[k][e];
             w[4 * k + e] = {p > 0.0 ? __builtin_fmax(p - taken, 0.0) : 0.0, p};  // (past the vocabulary p is 0)
         }
