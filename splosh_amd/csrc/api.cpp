@@ -1421,7 +1421,9 @@ int splosh_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, in
     if ((st = check_heads(part, SPLOSH_BF16, rows, cache->dim, true))) return st;
     if (q_heads % cache->heads != 0)
         return fail(SPLOSH_ERR_INVALID_SHAPE, "q_heads must be a multiple of the cache's heads");
-    if (rows * q_heads >= (int64_t)1 << 30) return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    if (rows * q_heads >= (int64_t)1 << 30 ||
+        !splosh::attend_fits(*cache, packed->requests, rows, q_heads, packed->table_pages * cache->page_tokens))
+        return fail(SPLOSH_ERR_UNSUPPORTED, "too many rows, heads and tokens for one launch");
     if (shared < 0 || shared % cache->page_tokens != 0 || shared / cache->page_tokens > packed->table_pages)
         return fail(SPLOSH_ERR_INVALID_SHAPE, "shared must be whole pages of the table");
     if (!(scale > 0.0f) || scale > 3.0e38f) return fail(SPLOSH_ERR_INVALID_SHAPE, "scale must be positive and finite");

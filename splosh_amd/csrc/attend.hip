@@ -32,6 +32,7 @@ constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
 constexpr int kManyThreads = 512, kManyRows = 256;
 constexpr int kManyKeys = 2 * kBlock;  // of a unit of the kernel for many vectors
+constexpr int kExtra = 1;             // units that a segment costs beside its keys
 
 struct AttendArgs {
     const uint16_t *q;
@@ -41,6 +42,7 @@ struct AttendArgs {
     int q_heads, shared, wide;  // wide: 16-byte aligned vectors of q
     float factor;               // scale log2(e)
     TileShape tile;
+    Divisor by_blocks;          // a page's
     int prefix;                 // the launch over the shared prefix
     int partial;                // whether every piece leaves its partial result
     float *slots;
@@ -135,6 +137,18 @@ __device__ __forceinline__ Span uniform(const Span &s) {
     return {uniform(s.begin), uniform(s.n), uniform(s.first), uniform(s.from), uniform(s.to)};
 }
 
+// The larger of a lane's value and that of the lane 16 (32) further: two registers' rows swapped, in place of a trip through LDS.
+__device__ __forceinline__ float max_rows(float v) {
+    typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+    const u32x2v r = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_halves(float v) {
+    typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+    const u32x2v r = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // What the sum of a_j is divided by, for the scale of v_j. (1 where it is no scale: t is then NaN, or the key masked.)
 __device__ __forceinline__ float inverse_scale(float vs) {
     const float r = __builtin_amdgcn_rcpf(vs);
@@ -142,7 +156,11 @@ __device__ __forceinline__ float inverse_scale(float vs) {
 }
 
 // The packed row that vector x of a tile's request is of.
-__device__ __forceinline__ int row_of(const Piece &p, int group, int x) { return p.span.begin + x / group; }
+__device__ __forceinline__ int row_of(const Piece &p, const TileShape &tile, int x) { return p.span.begin + tile.by_group.of(x); }
+// And its query head.
+__device__ __forceinline__ int head_of(const Piece &p, const TileShape &tile, int x) {
+    return p.head * tile.group + x - tile.by_group.of(x) * tile.group;
+}
 
 // The last key that packed row `row` sees, of the launch's.
 __device__ __forceinline__ int position_of(const AttendArgs &a, const PackedView &packed, const Piece &p, int row) {
@@ -174,98 +192,128 @@ struct Pages {
 
 // The record of a block of the request's keys; `hole`: it lies in no page (some record is given all the same).
 template <int D>
-__device__ __forceinline__ const uint8_t *block_record(const CacheView &cache, Pages &pages, int head, int block, bool &hole) {
-    const int column = block / cache.page_blocks;
+__device__ __forceinline__ const uint8_t *block_record(const AttendArgs &a, const CacheView &cache, Pages &pages, int head, int block, bool &hole) {
+    const int column = a.by_blocks.of(block);
     int page = pages(column);
     hole = page < 0 || page >= cache.pages;
     page = hole ? 0 : page;
     return record_of<D>(cache, page, head, block - column * cache.page_blocks);
 }
 
-// Calls `work` for each piece of the launch's units that workgroup blockIdx.x takes. All threads call it; scratch: a
-// word for each of a few more than the workgroup's threads.
+// Over the wave's lanes, the running sum of v, each lane's own included: within rows of sixteen lanes, then from row to row.
+__device__ __forceinline__ int running_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+// The largest of a lane's value and those of the lanes beside it, in groups of N (4, 8 or 16).
+template <int N>
+__device__ __forceinline__ float group_max(float v) {
+    auto other = [](float x, auto ctrl) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    v = __builtin_fmaxf(v, other(v, std::integral_constant<int, 0xb1>{}));                      // lanes 1 0 3 2
+    v = __builtin_fmaxf(v, other(v, std::integral_constant<int, 0x4e>{}));                      // lanes 2 3 0 1
+    if constexpr (N >= 8) v = __builtin_fmaxf(v, other(v, std::integral_constant<int, 0x141>{}));   // eight lanes turned round
+    if constexpr (N >= 16) v = __builtin_fmaxf(v, other(v, std::integral_constant<int, 0x140>{}));  // sixteen
+    return v;
+}
+
+// Calls `work` for each piece of the launch's units that workgroup blockIdx.x takes. All threads call it.
 template <int THREADS, typename F>
 __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView &cache, const PackedView &packed, F work) {
     const TileShape &tile = a.tile;
-    const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int request = 0;
-    int64_t total, before = 0, segment = 0;
+    const int w = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    // Up to 64 requests lie in a wave's lanes, and every wave sums them up by itself; more of them are runs of the workgroup's threads.
+    const bool few = packed.requests <= 64;
+    Span mine{};  // the lane's request
+    auto span_at = [&](int r) {
+        if (!few) return uniform(own_span(packed, cache.page_tokens, a.shared, r));
+        return Span{__builtin_amdgcn_readlane(mine.begin, r), __builtin_amdgcn_readlane(mine.n, r), __builtin_amdgcn_readlane(mine.first, r),
+                    a.shared, packed.table_pages * cache.page_tokens};
+    };
+    int request = 0, total, before = 0, segment = 0;
     Span span;
     if (a.prefix) {
-        span = prefix_span(packed, a.shared);
+        span = uniform(prefix_span(packed, a.shared));
         total = tile.heads * units_before(span, tile, tiles_of(span, tile));
+    } else if (few) {
+        int units = 0, segments = 0;
+        if (lane < packed.requests) {
+            mine = own_span(packed, cache.page_tokens, a.shared, lane);
+            const int tiles = tiles_of(mine, tile);
+            units = tile.heads * units_before(mine, tile, tiles), segments = tile.heads * tiles;
+        }
+        const int units_to = running_sum(units), segments_to = running_sum(segments);
+        total = __builtin_amdgcn_readlane(units_to, 63);
+        const int sharers = sharers_of(total, tile.workgroups);
+        if (w >= sharers) return;
+        const int first = first_unit(total, sharers, w);
+        request = __builtin_ctzll(__ballot(first < units_to));
+        before = __builtin_amdgcn_readlane(units_to - units, request), segment = __builtin_amdgcn_readlane(segments_to - segments, request);
+        span = span_at(request);
     } else {
-        // The units and segments before each request: a run of requests a thread, summed over the threads.
-        __shared__ int64_t wave_units[THREADS / 64], wave_segments[THREADS / 64], found_before, found_segment;
-        __shared__ int found;
+        __shared__ int wave_units[THREADS / 64], wave_segments[THREADS / 64], found[3];
         const int run = (packed.requests + THREADS - 1) / THREADS;
         const int low = min(tid * run, packed.requests), high = min(low + run, packed.requests);
-        auto units_of = [&](int r, int64_t &units, int &segments) {
+        auto units_of = [&](int r, int &segments) {
             const Span s = own_span(packed, cache.page_tokens, a.shared, r);
             const int tiles = tiles_of(s, tile);
-            units = tile.heads * units_before(s, tile, tiles);
             segments = tile.heads * tiles;
+            return tile.heads * units_before(s, tile, tiles);
         };
-        int64_t units = 0, segments = 0, u;
-        int n;
-        for (int r = low; r < high; ++r) units_of(r, u, n), units += u, segments += n;
-        int64_t units_to = units, segments_to = segments;  // own ones included
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int64_t x = __shfl_up(units_to, m), y = __shfl_up(segments_to, m);
-            if (lane >= m) units_to += x, segments_to += y;
-        }
+        int units = 0, segments = 0, n;
+        for (int r = low; r < high; ++r) units += units_of(r, n), segments += n;
+        int units_to = running_sum(units), segments_to = running_sum(segments);
         if (lane == 63) wave_units[wave] = units_to, wave_segments[wave] = segments_to;
-        if (tid == 0) found = -1;
+        if (tid == 0) found[0] = -1;
         __syncthreads();
         total = 0;
         for (int i = 0; i < THREADS / 64; ++i) {
             if (i < wave) units_to += wave_units[i], segments_to += wave_segments[i];
             total += wave_units[i];
         }
-        const int sharers = sharers_of(total, tile.workgroups);
-        const int64_t first = w < sharers ? first_unit(total, sharers, w) : total;
-        int64_t at = units_to - units, at_segment = segments_to - segments;
-        const bool mine = at <= first && first < units_to;
-        if (mine) {
+        total = uniform(total);
+        const int sharers = sharers_of(total, tile.workgroups), first = w < sharers ? first_unit(total, sharers, w) : total;
+        int at = units_to - units, at_segment = segments_to - segments;
+        if (at <= first && first < units_to) {
             for (int r = low; r < high; ++r) {
-                units_of(r, u, n);
-                if (at <= first && first < at + u) found = r, found_before = at, found_segment = at_segment;
+                const int u = units_of(r, n);
+                if (at <= first && first < at + u) found[0] = r, found[1] = at, found[2] = at_segment;
                 at += u, at_segment += n;
             }
         }
         __syncthreads();
-        if (found < 0) return;
-        request = uniform(found), before = uniform(found_before), segment = uniform(found_segment);
-        total = uniform(total);
-        span = own_span(packed, cache.page_tokens, a.shared, request);
+        request = uniform(found[0]), before = uniform(found[1]), segment = uniform(found[2]);
+        if (request < 0) return;
+        span = span_at(request);
     }
-    span = uniform(span);
     const int sharers = sharers_of(total, tile.workgroups);
     if (w >= sharers) return;
-    int64_t unit = first_unit(total, sharers, w);
-    const int64_t end = first_unit(total, sharers, w + 1);
-    int tiles = tiles_of(span, tile), head, t = 0, offset;
+    int unit = first_unit(total, sharers, w);
+    const int end = first_unit(total, sharers, w + 1);
+    int tiles = tiles_of(span, tile), head, t = 0, offset = unit - before;
     {
-        const int64_t each = units_before(span, tile, tiles);
-        int64_t rest = unit - before;
-        head = (int)(rest / each);
-        rest -= head * each;
+        const int each = units_before(span, tile, tiles);
+        head = offset / each;
+        offset -= head * each;
         int units = tile_units(span, tile, 0);
-        while (rest >= units) rest -= units, units = tile_units(span, tile, ++t);
-        offset = (int)rest;
+        while (offset >= units) offset -= units, units = tile_units(span, tile, ++t);
         segment += head * tiles + t;
     }
     while (true) {
-        const int units = tile_units(span, tile, t);
-        const int take = (int)(units - offset < end - unit ? units - offset : end - unit);
-        const int all = tile_end(span, tile, t) - span.from, blocks = all > 0 ? (all + kBlock - 1) / kBlock : 0;
+        const int units = tile_units(span, tile, t), take = min(units - offset, end - unit);
+        const int keys = tile_end(span, tile, t) - span.from, blocks = keys > 0 ? (keys + kBlock - 1) / kBlock : 0;
         const int per = tile.keys / kBlock;
         Piece p;
         p.span = span, p.request = request, p.head = head, p.tile = t;
-        p.first_block = offset * per;
-        p.blocks = max(0, min((offset + take) * per, blocks) - p.first_block);
-        p.slot = (int)(offset == 0 ? segment : a.segment_slots + w);
+        p.first_block = max(0, offset - tile.extra) * per;
+        p.blocks = max(0, min((offset + take - tile.extra) * per, blocks) - p.first_block);
+        p.slot = offset == 0 ? segment : (int)a.segment_slots + w;
         p.count = offset > 0 ? 0 : take == units ? 1 : owner_of(total, sharers, unit + units - 1) - w + 1;
         p.direct = !a.partial && take == units;
         if (segment < a.segment_slots) work(p);  // (more there are only where starts do not ascend)
@@ -277,7 +325,7 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         if (++head < tile.heads) continue;
         head = 0;
         do {  // (there is another one: the units say so)
-            span = uniform(own_span(packed, cache.page_tokens, a.shared, ++request));
+            span = span_at(++request);
             tiles = tiles_of(span, tile);
         } while (tiles == 0 && request + 1 < packed.requests);
     }
@@ -289,7 +337,7 @@ __device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, 
     if (p.direct) {
         const int x = p.tile * a.tile.rows + i;
         if (x >= p.span.n * a.tile.group) return;
-        const int row = row_of(p, a.tile.group, x), h = p.head * a.tile.group + x % a.tile.group;
+        const int row = row_of(p, a.tile, x), h = head_of(p, a.tile, x);
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         uint16_t *at = a.out + row * a.ld_out + (int64_t)h * D + d;
 #pragma unroll
@@ -308,7 +356,7 @@ template <int D>
 __device__ __forceinline__ void write_total(const AttendArgs &a, const Piece &p, int i, float most, float total) {
     const int x = p.tile * a.tile.rows + i;
     if (p.count > 0 && x < p.span.n * a.tile.group)
-        a.pieces[(int64_t)row_of(p, a.tile.group, x) * a.q_heads + p.head * a.tile.group + x % a.tile.group] = {p.slot, (int)blockIdx.x, p.count, i};
+        a.pieces[(int64_t)row_of(p, a.tile, x) * a.q_heads + head_of(p, a.tile, x)] = {p.slot, (int)blockIdx.x, p.count, i};
     if (p.direct) return;
     float *at = a.slots + p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)a.tile.rows * D;
     at[i] = most, at[a.tile.rows + i] = total;
@@ -320,21 +368,20 @@ template <int D, int R, int THREADS>
 __device__ __forceinline__ void stage_queries(const AttendArgs &a, const PackedView &packed, const Piece &p, u32x4 *q_parts, float *row_factor,
                                               int *row_position, int *least) {
     constexpr int STEPS = D / 32, CHUNKS = D / 16;
-    const int group = a.tile.group, vectors = p.span.n * group, tid = threadIdx.x;
+    const int vectors = p.span.n * a.tile.group, tid = threadIdx.x;
                     for (int item = tid; item < (R * CHUNKS + THREADS - 1) / THREADS * THREADS; item += THREADS) {
                 const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
                 const bool valid = i < R && x < vectors;
-                const int row = valid ? row_of(p, group, x) : 0;
+                const int row = valid ? row_of(p, a.tile, x) : 0;
                 float v[16] = {}, most = 0.0f;
                 if (valid) {
-                    const uint16_t *at = a.q + row * a.row_stride + (p.head * group + x % group) * a.head_stride + c * 16;
+                    const uint16_t *at = a.q + row * a.row_stride + head_of(p, a.tile, x) * a.head_stride + c * 16;
                     load_q8(at, a.wide, v);
                     load_q8(at + 8, a.wide, v + 8);
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
-#pragma unroll
-                for (int m = 1; m < CHUNKS; m <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, m));
+most = group_max<CHUNKS>(most);
                 const int power = power_of(most);
                 if (i < R) {
                     u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
@@ -349,64 +396,59 @@ __device__ __forceinline__ void stage_queries(const AttendArgs &a, const PackedV
             }
 }
 
-// The groups' sums against the largest of their maxima, added in their order: vectors 16 at a time, all threads.
+// The groups' sums against the largest of their maxima, added in their order: 32 vectors at a time (what the ring has room for), all threads.
 template <int D, int NT, typename S, int HELD>
 __device__ __forceinline__ void join_groups(const AttendArgs &a, const Piece &p, f32x4 (&acc)[HELD][NT], const float (&most)[NT], float (&total)[NT],
-                                            float *joined, float *wave_most, float *wave_total, int record_group, int half_of) {
+                                            float *joined, float *wave_most, float *wave_total, int record_group) {
     constexpr int R = S::kRows, GROUPS = S::kGroups, PITCH = S::kPitch;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                total[n] += __shfl_xor(total[n], 16);
-                total[n] += __shfl_xor(total[n], 32);
-                if (g == 0 && half_of == 0) wave_most[record_group * R + n * 16 + col] = most[n], wave_total[record_group * R + n * 16 + col] = total[n];
-            }
-            __syncthreads();
+    for (int n = 0; n < NT; ++n) {
+        total[n] += __shfl_xor(total[n], 16);
+        total[n] += __shfl_xor(total[n], 32);
+        if (g == 0) wave_most[record_group * R + n * 16 + col] = most[n], wave_total[record_group * R + n * 16 + col] = total[n];
+    }
+    __syncthreads();
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float top = kLowest;
+    for (int n0 = 0; n0 < NT; n0 += 2) {
+        constexpr int MOST = NT > 1 ? 2 : 1;
+        const int here = NT - n0 < MOST ? NT - n0 : MOST;
+        if (n0) __syncthreads();  // (the last vectors are read)
 #pragma unroll
-                for (int w = 0; w < GROUPS; ++w) top = __builtin_fmaxf(top, wave_most[w * R + n * 16 + col]);
-                const float keep = __builtin_amdgcn_exp2f(most[n] - top);
-                if (n) __syncthreads();  // (the last sixteen vectors are read)
+        for (int k = 0; k < MOST; ++k) {
+            const int n = n0 + k;
+            if (n >= NT) break;
+            float top = kLowest;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+            for (int w = 0; w < GROUPS; ++w) top = __builtin_fmaxf(top, wave_most[w * R + n * 16 + col]);
+            const float keep = __builtin_amdgcn_exp2f(most[n] - top);
 #pragma unroll
-                    for (int j = 0; j < HELD; j += 4)
-                        *reinterpret_cast<f32x4 *>(joined + (record_group * 16 + col) * PITCH + half_of * (D / 2) + (4 * g + e) * HELD + j) =
-                            f32x4{acc[j][n][e] * keep, acc[j + 1][n][e] * keep, acc[j + 2][n][e] * keep, acc[j + 3][n][e] * keep};
-                __syncthreads();
-                for (int item = tid; item < 256; item += S::kThreads) {
-                    const int i = item / 16, d = item % 16 * (D / 16);
-                    float sum[D / 16] = {}, row_total = 0.0f, row_most = kLowest;
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int w = 0; w < GROUPS; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w * R + n * 16 + i]);
+                for (int j = 0; j < HELD; j += 4)
+                    *reinterpret_cast<f32x4 *>(joined + ((k * GROUPS + record_group) * 16 + col) * PITCH + (4 * g + e) * HELD + j) =
+                        f32x4{acc[j][n][e] * keep, acc[j + 1][n][e] * keep, acc[j + 2][n][e] * keep, acc[j + 3][n][e] * keep};
+        }
+        __syncthreads();
+        for (int item = tid; item < here * 256; item += S::kThreads) {
+            const int k = item / 256, i = item / 16 % 16, d = item % 16 * (D / 16), row = (n0 + k) * 16 + i;
+            float sum[D / 16] = {}, row_total = 0.0f, row_most = kLowest;
 #pragma unroll
-                    for (int w = 0; w < GROUPS; ++w) {
-                        row_total += wave_total[w * R + n * 16 + i] * __builtin_amdgcn_exp2f(wave_most[w * R + n * 16 + i] - row_most);
+            for (int w = 0; w < GROUPS; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w * R + row]);
 #pragma unroll
-                        for (int e = 0; e < D / 16; e += 4) {
-                            const f32x4 part = *reinterpret_cast<const f32x4 *>(joined + (w * 16 + i) * PITCH + d + e);
+            for (int w = 0; w < GROUPS; ++w) {
+                row_total += wave_total[w * R + row] * __builtin_amdgcn_exp2f(wave_most[w * R + row] - row_most);
 #pragma unroll
-                            for (int f = 0; f < 4; ++f) sum[e + f] += part[f];
-                        }
-                    }
-                    write_sums<D, D / 16>(a, p, n * 16 + i, d, sum, row_total);
-                    if (item % 16 == 0) write_total<D>(a, p, n * 16 + i, row_most, row_total);
+                for (int e = 0; e < D / 16; e += 4) {
+                    const f32x4 part = *reinterpret_cast<const f32x4 *>(joined + ((k * GROUPS + w) * 16 + i) * PITCH + d + e);
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) sum[e + f] += part[f];
                 }
             }
-}
-
-// The larger of a lane's value and that of the lane 16 (32) further: two registers' rows swapped, in place of a trip through LDS.
-__device__ __forceinline__ float max_rows(float v) {
-    typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
-    const u32x2v r = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
-    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float max_halves(float v) {
-    typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
-    const u32x2v r = __builtin_bit_cast(u32x2v, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
-    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            write_sums<D, D / 16>(a, p, row, d, sum, row_total);
+            if (item % 16 == 0) write_total<D>(a, p, row, row_most, row_total);
+        }
+    }
 }
 
 // A lane's eight scores of each vector masked, and the largest of all lanes' of the vector.
@@ -471,7 +513,7 @@ struct FewShape {
     static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kQueryBytes = kRows * D * 2;
     static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions
     static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
-    static_assert(kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
+    static_assert((NT > 1 ? 2 : 1) * kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
 };
 
 template <int D, int NT>
@@ -503,7 +545,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
         bool hole = false;
         auto load = [&](int block, int buffer) {
-            const uint8_t *record = block_record<D>(cache, pages, p.head, block, hole);
+            const uint8_t *record = block_record<D>(a, cache, pages, p.head, block, hole);
             const rsrc_t r = make_rsrc(record, Ring::kRecord);
             char *at = lds + uniform(ring + buffer * Ring::kRecord);
 #pragma unroll
@@ -635,7 +677,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
             }
         }
         }
-        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group, 0);
+        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group);
     });
 }
 
@@ -653,10 +695,10 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 31, g = lane >> 5;
 
     for_pieces<kManyThreads>(a, cache, packed, [&](const Piece &p) {
-        const int group = a.tile.group, vectors = p.span.n * group;
+        const int vectors = p.span.n * a.tile.group;
         const int x = p.tile * kManyRows + wave * 32 + col;
         const bool valid = x < vectors;
-        const int row = valid ? row_of(p, group, x) : 0;
+        const int row = valid ? row_of(p, a.tile, x) : 0;
         const int position = valid ? position_of(a, packed, p, row) : INT_MAX;
         int first_position = position;  // of the wave's vectors
 #pragma unroll
@@ -667,7 +709,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         float factor;
         {
             float most = 0.0f;
-            const uint16_t *at = a.q + row * a.row_stride + (p.head * group + (valid ? x % group : 0)) * a.head_stride + g * 8;
+            const uint16_t *at = a.q + row * a.row_stride + head_of(p, a.tile, valid ? x : 0) * a.head_stride + g * 8;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 float v[8];
@@ -675,7 +717,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 #pragma unroll
                 for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
             }
-            most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+            most = max_halves(most);
             const int power = power_of(most);
             factor = __builtin_ldexpf(a.factor, -power);
 #pragma unroll
@@ -695,7 +737,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
         bool hole = false;
         auto fetch = [&](int block) {
-            const uint8_t *record = block_record<D>(cache, pages, p.head, block, hole);
+            const uint8_t *record = block_record<D>(a, cache, pages, p.head, block, hole);
             const rsrc_t r = make_rsrc(record, record_bytes(D));
 #pragma unroll
             for (int j = 0; j < (2 * kBlock * D / 1024 + 7) / 8; ++j)
@@ -920,11 +962,8 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     const int cus = device_cus();
     p.few = vectors <= 64;
     const int nt = (int)((vectors + 15) / 16);
-    p.tile.rows = p.few ? 16 * nt : kManyRows;
-    p.tile.keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
-    p.tile.group = (int)(q_heads / cache.heads);
-    p.tile.heads = (int)cache.heads;
-    p.tile.workgroups = p.few && cache.dim < 256 ? 2 * cus : cus;
+    const int keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
+    p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, kExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
     p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
     return p;
 }
@@ -936,6 +975,12 @@ static AttendPlan plan_prefix(const splosh_cache &cache, int64_t rows, int64_t q
 }
 // Where the vectors' pieces are, of each launch.
 static size_t pieces_bytes(int64_t rows, int64_t q_heads) { return (size_t)(rows * q_heads) * sizeof(Pieces); }
+
+// Units are counted in 32 bits: whether a launch of this size can have no more.
+bool attend_fits(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t tokens) {
+    const AttendPlan p = plan_own(cache, requests, rows, q_heads);
+    return p.segment_slots * (tokens / p.tile.keys + 2 + p.tile.extra) < INT32_MAX && p.segment_slots + p.tile.workgroups < INT32_MAX;
+}
 
 size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t shared) {
     size_t slots = plan_own(cache, requests, rows, q_heads).slot_bytes();
@@ -978,6 +1023,7 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
     a.q = q, a.row_stride = row_stride, a.head_stride = head_stride, a.out = out, a.ld_out = ld_out;
     a.q_heads = (int)q_heads, a.shared = (int)shared;
     a.wide = reinterpret_cast<uintptr_t>(q) % 16 == 0 && row_stride % 8 == 0 && head_stride % 8 == 0;
+    a.by_blocks = divisor((int)(cache.page_tokens / kBlock));
     a.factor = scale * 1.4426950408889634f;
     a.pieces = reinterpret_cast<Pieces *>(at);
     a.slots = reinterpret_cast<float *>(at + (shared > 0 ? 2 : 1) * pieces_bytes(rows, q_heads));

@@ -323,6 +323,7 @@ hipError_t launch_cache_read(const splosh_cache &cache, const splosh_packed &pac
                              int64_t ldk, uint16_t *v, int64_t ldv, hipStream_t stream);
 
 // Attention over the cache (attend.hip).
+bool attend_fits(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t tokens);
 size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t shared);
 hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
                          const splosh_cache &cache, const splosh_packed &packed, int64_t rows, int64_t shared,
