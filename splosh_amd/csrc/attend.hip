@@ -39,7 +39,7 @@ struct AttendArgs {
     int64_t row_stride, head_stride;
     uint16_t *out;
     int64_t ld_out;
-    int q_heads, shared, wide;  // wide: 16-byte aligned vectors of q
+    int q_heads, shared, wide, wide_out;  // whether vectors of q are 16-byte aligned, and of out 8-byte
     float factor;               // scale log2(e)
     TileShape tile;
     Divisor by_blocks;          // a page's
@@ -338,12 +338,17 @@ __device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, 
         const int x = p.tile * a.tile.rows + i;
         if (x >= p.span.n * a.tile.group) return;
         const int row = row_of(p, a.tile, x), h = head_of(p, a.tile, x);
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const float inv = 1.0f / total;
         uint16_t *at = a.out + row * a.ld_out + (int64_t)h * D + d;
+        uint32_t pair[N / 2];
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-            const uint32_t pair = total == 0.0f ? 0u : f32x2_to_bf16x2(o[e] * inv, o[e + 1] * inv);
-            at[e] = (uint16_t)pair, at[e + 1] = (uint16_t)(pair >> 16);
+        for (int e = 0; e < N / 2; ++e) pair[e] = total == 0.0f ? 0u : f32x2_to_bf16x2(o[2 * e] * inv, o[2 * e + 1] * inv);
+        if (a.wide_out) {
+#pragma unroll
+            for (int e = 0; e < N / 4; ++e) reinterpret_cast<u32x2 *>(at)[e] = u32x2{pair[2 * e], pair[2 * e + 1]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) at[e] = (uint16_t)(pair[e / 2] >> 16 * (e & 1));
         }
     } else {
         float *at = a.slots + p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)i * D + d;
@@ -390,7 +395,7 @@ most = group_max<CHUNKS>(most);
                     if (c == 0) {
                         row_factor[i] = __builtin_ldexpf(a.factor, -power);
                         row_position[i] = valid ? position_of(a, packed, p, row) : -1;
-                        if (valid) atomicMin(least, row_position[i]);
+                        if (valid && a.prefix) atomicMin(least, row_position[i]);
                     }
                 }
             }
@@ -555,8 +560,10 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
             __builtin_amdgcn_sched_barrier(0);
         };
         if (from + record_group < to) load(from + record_group, 0);
-        if (tid == 0) *least = INT_MAX;
-        __syncthreads();
+        if (a.prefix) {
+            if (tid == 0) *least = INT_MAX;
+            __syncthreads();
+        }
         stage_queries<D, R, S::kThreads>(a, packed, p, q_parts, row_factor, row_position, least);
         __syncthreads();
         float factor[NT], most[NT], total[NT];
@@ -566,7 +573,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
             factor[n] = row_factor[n * 16 + col], position[n] = row_position[n * 16 + col];
             most[n] = kLowest, total[n] = 0.0f;
         }
-        const int first_position = uniform(*least);
+        const int first_position = a.prefix ? uniform(*least) : p.span.first + a.tile.by_group.of(p.tile * R);
         f32x4 acc[HELD][NT] = {};
         int buffer = 0;
         bool waited = false, dead = false;
@@ -630,7 +637,12 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
 #pragma unroll
             for (int n = 0; n < NT; ++n) moved |= top[n] > most[n] + kSlack;
             moved = __any(moved);
-            if (moved) break;
+            if (moved) {
+                if (block != from + record_group) break;
+                moved = false;  // (the first record: there are no sums yet)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) most[n] = __builtin_fmaxf(top[n], most[n]);
+            }
             weigh<NT>(t, inverse, most, total, weight);
             uint32_t v[8][SLABS];
 #pragma unroll
@@ -1023,6 +1035,7 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
     a.q = q, a.row_stride = row_stride, a.head_stride = head_stride, a.out = out, a.ld_out = ld_out;
     a.q_heads = (int)q_heads, a.shared = (int)shared;
     a.wide = reinterpret_cast<uintptr_t>(q) % 16 == 0 && row_stride % 8 == 0 && head_stride % 8 == 0;
+    a.wide_out = reinterpret_cast<uintptr_t>(out) % 8 == 0 && ld_out % 4 == 0;
     a.by_blocks = divisor((int)(cache.page_tokens / kBlock));
     a.factor = scale * 1.4426950408889634f;
     a.pieces = reinterpret_cast<Pieces *>(at);
