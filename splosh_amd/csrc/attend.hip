@@ -695,6 +695,19 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
 
 // ---- many vectors -------------------------------------------------------------------------------
 
+// N products' operands read from LDS four ahead of them.
+template <int N>
+__device__ __forceinline__ void interleave() {
+    constexpr int AHEAD = N < 4 ? N : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 template <int D>
 __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheView cache, PackedView packed) {
     constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = 1024 + 64;  // (the pitch spreads a quad's writes over the banks)
@@ -702,8 +715,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
     __shared__ __align__(16) uint8_t key_parts[2][STEPS * K_PITCH];
     __shared__ __align__(16) u32x4 value_parts[2][TILES * 2 * 64];
     __shared__ __align__(16) float scales[2][3][kBlock];
-    extern __shared__ __align__(16) char lds[];
-    char *const raw = lds;  // the next record
+    extern __shared__ __align__(16) char lds[];  // two records as they are
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 31, g = lane >> 5;
 
     for_pieces<kManyThreads>(a, cache, packed, [&](const Piece &p) {
@@ -744,20 +756,24 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         Pages pages(packed, a.prefix ? 0 : p.request);
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
 
-        // The record of block b goes straight into LDS while block b - 1 is multiplied, and is widened to fp16 after that:
+        // A record goes straight into LDS two blocks before it is multiplied, and is widened to fp16 one block before:
         // by threads 0..D-1 four dimensions of eight values each, by the last 256 threads 16-byte runs of keys.
-        const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
         bool hole = false;
-        auto fetch = [&](int block) {
+        auto fetch = [&](int block, int buffer) {
+            const int at = buffer * record_bytes(D);
             const uint8_t *record = block_record<D>(a, cache, pages, p.head, block, hole);
             const rsrc_t r = make_rsrc(record, record_bytes(D));
 #pragma unroll
             for (int j = 0; j < (2 * kBlock * D / 1024 + 7) / 8; ++j)
-                if (j * 8 + wave < 2 * kBlock * D / 1024) buffer_load_lds16(r, lds + (j * 8 + wave) * 1024, (j * 8 + wave) * 1024 + lane * 16);
-            if (wave == 7) buffer_load_lds4(r, lds + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
+                if (j * 8 + wave < 2 * kBlock * D / 1024) buffer_load_lds16(r, lds + at + (j * 8 + wave) * 1024, (j * 8 + wave) * 1024 + lane * 16);
+            if (wave == 7) buffer_load_lds4(r, lds + at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
             __builtin_amdgcn_sched_barrier(0);
         };
         auto stage = [&](int buffer) {
+            const char *const raw = lds + buffer * record_bytes(D);
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));  // (the places are found anew each time: kept, they would be spilled)
+            const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
             if (tid < D) {
                 uint32_t v[8];
 #pragma unroll
@@ -791,26 +807,35 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             }
         };
 
-        bool dead = false;
+        bool dead = false, dead_next = false;
         __syncthreads();  // (the last piece's LDS is read)
         if (from < to) {
-            fetch(from);
-            wait_vmcnt<0>();
-            __syncthreads();
+            fetch(from, 0);
             dead = hole;
-            stage(0);
+            if (from + 1 < to) fetch(from + 1, 1);
+            dead_next = hole;
+            wait_vmcnt<0>();
         }
         __syncthreads();
+        if (from < to) stage(0);
+        lds_barrier();
         for (int block = from; block < to; ++block) {
             const int buffer = (block - from) & 1;
-            if (block + 1 < to) fetch(block + 1);
+            const bool more = block + 1 < to;
+            hole = false;
+            if (block + 2 < to) fetch(block + 2, buffer);
+            // The waves of a SIMD take turns: one widens the next record while the other multiplies.
+            if (more && wave >= 4) stage(buffer ^ 1);
             f32x16 s = {};
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
                 const f16x8 k = *reinterpret_cast<const f16x8 *>(key_parts[buffer] + i * K_PITCH + lane * 16);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], s, 0, 0, 0);
             }
-            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
+            interleave<STEPS>();
+            if (more && wave < 4) stage(buffer ^ 1);
+            const bool here_dead = dead, masked = dead || block * kBlock + kBlock - 1 > first_position;
+            dead = dead_next, dead_next = hole;
             float t[16], top = -__builtin_inff();
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -822,7 +847,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    t[e] = !dead && block * kBlock + e / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
+                    t[e] = !here_dead && block * kBlock + e / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, t[e]);
@@ -835,7 +860,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) acc[j] *= keep;
             }
-            uint32_t pairs[8];
+            u32x4 pairs[2];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const f32x4 inverse = *reinterpret_cast<const f32x4 *>(&scales[buffer][2][8 * b + 4 * g]);
@@ -845,25 +870,19 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                     w[e] = __builtin_amdgcn_exp2f(t[4 * b + e] - most);
                     total = __builtin_fmaf(w[e], inverse[e], total);
                 }
-                pairs[2 * b] = f16_pair(w[0], w[1]), pairs[2 * b + 1] = f16_pair(w[2], w[3]);
+                pairs[b / 2][2 * (b % 2)] = f16_pair(w[0], w[1]), pairs[b / 2][2 * (b % 2) + 1] = f16_pair(w[2], w[3]);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const u32x4 four = {pairs[4 * i], pairs[4 * i + 1], pairs[4 * i + 2], pairs[4 * i + 3]};
-                const f16x8 weight = __builtin_bit_cast(f16x8, four);
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) {
                     const f16x8 v = __builtin_bit_cast(f16x8, value_parts[buffer][(j * 2 + i) * 64 + lane]);
-                    acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weight, acc[j], 0, 0, 0);
+                    acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pairs[i]), acc[j], 0, 0, 0);
                 }
-            }
-            if (block + 1 < to) {
-                wait_vmcnt<0>();
-                lds_barrier();  // every wave's part of the next record has landed
-                dead = hole;
-                stage(buffer ^ 1);
-            }
-            lds_barrier();
+            interleave<2 * TILES>();
+            wait_vmcnt<0>();
+            lds_barrier();  // the record after the next has landed, the next one is widened, and this one used up
         }
         total += __shfl_xor(total, 32);
         const int i = wave * 32 + col;
@@ -1019,7 +1038,7 @@ static void launch_part(const AttendPlan &plan, const AttendArgs &a, const Cache
         constexpr int NT = decltype(tiles)::value;
         launch_lds<FewShape<D, NT>>(few_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
     };
-    if (!plan.few) many_kernel<D><<<plan.tile.workgroups, kManyThreads, record_bytes(D), stream>>>(a, cache, packed);
+    if (!plan.few) many_kernel<D><<<plan.tile.workgroups, kManyThreads, 2 * record_bytes(D), stream>>>(a, cache, packed);
     else if (plan.tile.rows == 16) few(std::integral_constant<int, 1>{});
     else if (plan.tile.rows == 32) few(std::integral_constant<int, 2>{});
     else if (plan.tile.rows == 48) few(std::integral_constant<int, 3>{});
