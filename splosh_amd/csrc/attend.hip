@@ -106,25 +106,27 @@ __device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
 }
 
 // Eight values of q.
-__device__ __forceinline__ void load_q8(const uint16_t *at, int wide, float *v) {
-    uint32_t w[4];
-    if (wide) {
-        const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+__device__ __forceinline__ u32x4 load_q8(const uint16_t *at, int wide) {
+    if (wide) return *reinterpret_cast<const u32x4 *>(at);
+    u32x4 w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = x[e];
-    } else {
+    for (int e = 0; e < 4; ++e) w[e] = at[2 * e] | (uint32_t)at[2 * e + 1] << 16;
+    return w;
+}
+__device__ __forceinline__ float largest8(const u32x4 &w) {
+    float most = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = at[2 * e] | (uint32_t)at[2 * e + 1] << 16;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[2 * e] = bf16_bits_to_f32(w[e]), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    for (int e = 0; e < 4; ++e)
+        most = __builtin_fmaxf(most, __builtin_fmaxf(__builtin_fabsf(bf16_bits_to_f32(w[e])), __builtin_fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+    return most;
 }
 // The power that brings a row's largest value to [2^14, 2^15).
 __device__ __forceinline__ int power_of(float most) { return 141 - (int)(__float_as_uint(most) >> 23); }
-__device__ __forceinline__ u32x4 moved8(const float *v, int power) {
+__device__ __forceinline__ u32x4 moved8(const u32x4 &v, int power) {
     u32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = f16_pair(__builtin_ldexpf(v[2 * e], power), __builtin_ldexpf(v[2 * e + 1], power));
+    for (int e = 0; e < 4; ++e)
+        w[e] = f16_pair(__builtin_ldexpf(bf16_bits_to_f32(v[e]), power), __builtin_ldexpf(__uint_as_float(v[e] & 0xffff0000u), power));
     return w;
 }
 
@@ -135,6 +137,13 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 }
 __device__ __forceinline__ Span uniform(const Span &s) {
     return {uniform(s.begin), uniform(s.n), uniform(s.first), uniform(s.from), uniform(s.to)};
+}
+
+// The lane's number, found anew: where every register is taken, a kept one is spilled, and its reload waits for all loads into LDS.
+__device__ __forceinline__ int lane_anew() {
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+    return lane;
 }
 
 // The larger of a lane's value and that of the lane 16 (32) further: two registers' rows swapped, in place of a trip through LDS.
@@ -374,31 +383,28 @@ __device__ __forceinline__ void stage_queries(const AttendArgs &a, const PackedV
                                               int *row_position, int *least) {
     constexpr int STEPS = D / 32, CHUNKS = D / 16;
     const int vectors = p.span.n * a.tile.group, tid = threadIdx.x;
-                    for (int item = tid; item < (R * CHUNKS + THREADS - 1) / THREADS * THREADS; item += THREADS) {
-                const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
-                const bool valid = i < R && x < vectors;
-                const int row = valid ? row_of(p, a.tile, x) : 0;
-                float v[16] = {}, most = 0.0f;
-                if (valid) {
-                    const uint16_t *at = a.q + row * a.row_stride + head_of(p, a.tile, x) * a.head_stride + c * 16;
-                    load_q8(at, a.wide, v);
-                    load_q8(at + 8, a.wide, v + 8);
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
-most = group_max<CHUNKS>(most);
-                const int power = power_of(most);
-                if (i < R) {
-                    u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
-                    to[0] = moved8(v, power);
-                    to[64] = moved8(v + 8, power);
-                    if (c == 0) {
-                        row_factor[i] = __builtin_ldexpf(a.factor, -power);
-                        row_position[i] = valid ? position_of(a, packed, p, row) : -1;
-                        if (valid && a.prefix) atomicMin(least, row_position[i]);
-                    }
-                }
+    for (int item = tid; item < (R * CHUNKS + THREADS - 1) / THREADS * THREADS; item += THREADS) {
+        const int i = item / CHUNKS, c = item % CHUNKS, x = p.tile * R + i;
+        const bool valid = i < R && x < vectors;
+        const int row = valid ? row_of(p, a.tile, x) : 0;
+        u32x4 low = {}, high = {};
+        if (valid) {
+            const uint16_t *at = a.q + row * a.row_stride + head_of(p, a.tile, x) * a.head_stride + c * 16;
+            low = load_q8(at, a.wide), high = load_q8(at + 8, a.wide);
+        }
+        const float most = group_max<CHUNKS>(__builtin_fmaxf(largest8(low), largest8(high)));
+        const int power = power_of(most);
+        if (i < R) {
+            u32x4 *to = q_parts + (i / 16 * STEPS + c / 4 * 2) * 64 + (c % 4) * 16 + i % 16;
+            to[0] = moved8(low, power);
+            to[64] = moved8(high, power);
+            if (c == 0) {
+                row_factor[i] = __builtin_ldexpf(a.factor, -power);
+                row_position[i] = valid ? position_of(a, packed, p, row) : -1;
+                if (valid && a.prefix) atomicMin(least, row_position[i]);
             }
+        }
+    }
 }
 
 // The groups' sums against the largest of their maxima, added in their order: 32 vectors at a time (what the ring has room for), all threads.
@@ -709,13 +715,23 @@ __device__ __forceinline__ void interleave() {
 }
 
 template <int D>
+struct ManyShape {
+    static constexpr int kPitch = 1024 + 64;  // of a step of keys: spreads a quad's writes over the banks
+    static constexpr int kLoads = D == 64 ? 2 : D / 128;  // of a wave, of its eighth of a record's codes
+    static constexpr int kKeys = 2 * record_bytes(D), kValues = kKeys + 3 * (D / 16) * kPitch, kScales = kValues + 4 * (D / 32) * 2048;
+    static constexpr int kThreads = kManyThreads, kLds = kScales + 4 * 3 * kBlock * 4;
+    static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+template <int D>
 __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheView cache, PackedView packed) {
-    constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = 1024 + 64;  // (the pitch spreads a quad's writes over the banks)
+    constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = ManyShape<D>::kPitch;
     constexpr int K_ITEMS = 2 * D / 256 > 0 ? 2 * D / 256 : 1;
-    __shared__ __align__(16) uint8_t key_parts[2][STEPS * K_PITCH];
-    __shared__ __align__(16) u32x4 value_parts[2][TILES * 2 * 64];
-    __shared__ __align__(16) float scales[2][3][kBlock];
-    extern __shared__ __align__(16) char lds[];  // two records as they are
+    typedef ManyShape<D> S;
+    extern __shared__ __align__(16) char lds[];  // two records as they are, then three of keys, four of values and of scales as they are used
+    uint8_t *const key_parts = reinterpret_cast<uint8_t *>(lds + S::kKeys);
+    u32x4 *const value_parts = reinterpret_cast<u32x4 *>(lds + S::kValues);
+    float *const scales = reinterpret_cast<float *>(lds + S::kScales);
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 31, g = lane >> 5;
 
     for_pieces<kManyThreads>(a, cache, packed, [&](const Piece &p) {
@@ -734,45 +750,44 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         {
             float most = 0.0f;
             const uint16_t *at = a.q + row * a.row_stride + head_of(p, a.tile, valid ? x : 0) * a.head_stride + g * 8;
+            u32x4 held[STEPS];
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                float v[8];
-                load_q8(at + 16 * s, a.wide, v);
+            for (int s = 0; s < STEPS; ++s) held[s] = load_q8(at + 16 * s, a.wide);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
-            }
+            for (int s = 0; s < STEPS; ++s) most = __builtin_fmaxf(most, largest8(held[s]));
             most = max_halves(most);
             const int power = power_of(most);
             factor = __builtin_ldexpf(a.factor, -power);
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                float v[8];
-                load_q8(at + 16 * s, a.wide, v);
-                q[s] = __builtin_bit_cast(f16x8, moved8(v, power));
-            }
+            for (int s = 0; s < STEPS; ++s) q[s] = __builtin_bit_cast(f16x8, moved8(held[s], power));
         }
         f32x16 acc[TILES] = {};
         float most = kLowest, total = 0.0f;
         Pages pages(packed, a.prefix ? 0 : p.request);
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
 
-        // A record goes straight into LDS two blocks before it is multiplied, and is widened to fp16 one block before:
-        // by threads 0..D-1 four dimensions of eight values each, by the last 256 threads 16-byte runs of keys.
+        // A record goes straight into LDS three steps before it is multiplied, and is widened to fp16 two steps before. Waves 0 to 3 do that
+        // with the values (a thread four dimensions of eight of them) and the scales, waves 4 to 7 with the keys (16-byte runs).
         bool hole = false;
         auto fetch = [&](int block, int buffer) {
-            const int at = buffer * record_bytes(D);
+            const int lane = lane_anew();
             const uint8_t *record = block_record<D>(a, cache, pages, p.head, block, hole);
             const rsrc_t r = make_rsrc(record, record_bytes(D));
+            const int part = (wave < 4 ? kBlock * D : 0) + (wave & 3) * (kBlock * D / 4), at = buffer * record_bytes(D) + part;
+            if constexpr (D == 64) {
 #pragma unroll
-            for (int j = 0; j < (2 * kBlock * D / 1024 + 7) / 8; ++j)
-                if (j * 8 + wave < 2 * kBlock * D / 1024) buffer_load_lds16(r, lds + at + (j * 8 + wave) * 1024, (j * 8 + wave) * 1024 + lane * 16);
-            if (wave == 7) buffer_load_lds4(r, lds + at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
+                for (int n = 0; n < S::kLoads; ++n) buffer_load_lds4(r, lds + at + n * 256, part + n * 256 + lane * 4);
+            } else {
+#pragma unroll
+                for (int n = 0; n < S::kLoads; ++n) buffer_load_lds16(r, lds + at + n * 1024, part + n * 1024 + lane * 16);
+            }
+            // (All four waves the same, so that they count the same loads.)
+            if (wave < 4) buffer_load_lds4(r, lds + buffer * record_bytes(D) + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto stage = [&](int buffer) {
+        auto stage = [&](int buffer, int third, int fourth) {  // the record's place among two, three and four
             const char *const raw = lds + buffer * record_bytes(D);
-            int tid = threadIdx.x;
-            asm volatile("" : "+v"(tid));  // (the places are found anew each time: kept, they would be spilled)
+            const int tid = wave * 64 + lane_anew();
             const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
             if (tid < D) {
                 uint32_t v[8];
@@ -784,7 +799,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int t = D == 64 ? c >> 1 : quad / 32 * 4 + c, m = D == 64 ? (c & 1) * 16 + quad : quad % 32;
-                    value_parts[buffer][(t * 2 + value_step) * 64 + value_g * 32 + m] = __builtin_bit_cast(u32x4, part[c]);
+                    value_parts[(fourth * TILES * 2 + t * 2 + value_step) * 64 + value_g * 32 + m] = __builtin_bit_cast(u32x4, part[c]);
                 }
             }
             if (tid >= 256) {
@@ -794,7 +809,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                     if (item < 2 * D) {
                         const int run = item / 128 * 4 + item % 4, token = item / 4 % 32;
                         const u32x4 k = *reinterpret_cast<const u32x4 *>(raw + token * D + run * 16);
-                        uint8_t *at = key_parts[buffer] + run * K_PITCH + token * 16;
+                        uint8_t *at = key_parts + (third * STEPS + run) * K_PITCH + token * 16;
                         *reinterpret_cast<f16x8 *>(at) = widen8(k[0], k[1]);
                         *reinterpret_cast<f16x8 *>(at + 512) = widen8(k[2], k[3]);
                     }
@@ -802,52 +817,36 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             }
             if (tid < 2 * kBlock) {
                 const float scale = reinterpret_cast<const float *>(raw + 2 * kBlock * D)[tid];
-                if (tid < kBlock) scales[buffer][0][tid] = scale;
-                else scales[buffer][1][tid - kBlock] = __builtin_amdgcn_logf(scale), scales[buffer][2][tid - kBlock] = inverse_scale(scale);
+                float *at = scales + fourth * 3 * kBlock;
+                if (tid < kBlock) at[tid] = scale;
+                else at[tid] = __builtin_amdgcn_logf(scale), at[tid + kBlock] = inverse_scale(scale);
             }
         };
 
-        bool dead = false, dead_next = false;
-        __syncthreads();  // (the last piece's LDS is read)
-        if (from < to) {
-            fetch(from, 0);
-            dead = hole;
-            if (from + 1 < to) fetch(from + 1, 1);
-            dead_next = hole;
-            wait_vmcnt<0>();
-        }
-        __syncthreads();
-        if (from < to) stage(0);
-        lds_barrier();
-        for (int block = from; block < to; ++block) {
-            const int buffer = (block - from) & 1;
-            const bool more = block + 1 < to;
-            hole = false;
-            if (block + 2 < to) fetch(block + 2, buffer);
-            // The waves of a SIMD take turns: one widens the next record while the other multiplies.
-            if (more && wave >= 4) stage(buffer ^ 1);
-            f32x16 s = {};
+        f32x16 s;
+        auto score = [&](int third) {
+            s = f32x16{};
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                const f16x8 k = *reinterpret_cast<const f16x8 *>(key_parts[buffer] + i * K_PITCH + lane * 16);
+                const f16x8 k = *reinterpret_cast<const f16x8 *>(key_parts + (third * STEPS + i) * K_PITCH + lane * 16);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], s, 0, 0, 0);
             }
             interleave<STEPS>();
-            if (more && wave < 4) stage(buffer ^ 1);
-            const bool here_dead = dead, masked = dead || block * kBlock + kBlock - 1 > first_position;
-            dead = dead_next, dead_next = hole;
+        };
+        auto weigh_values = [&](int block, int fourth, bool dead) {
+            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
+            const float *const at = scales + fourth * 3 * kBlock + 4 * g;
             float t[16], top = -__builtin_inff();
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const f32x4 ks = *reinterpret_cast<const f32x4 *>(&scales[buffer][0][8 * b + 4 * g]);
-                const f32x4 lv = *reinterpret_cast<const f32x4 *>(&scales[buffer][1][8 * b + 4 * g]);
+                const f32x4 ks = *reinterpret_cast<const f32x4 *>(at + 8 * b), lv = *reinterpret_cast<const f32x4 *>(at + kBlock + 8 * b);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) t[4 * b + e] = __builtin_fmaf(s[4 * b + e], ks[e] * factor, lv[e]);
             }
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    t[e] = !here_dead && block * kBlock + e / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
+                    t[e] = !dead && block * kBlock + e / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, t[e]);
@@ -860,30 +859,62 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) acc[j] *= keep;
             }
-            u32x4 pairs[2];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const f32x4 inverse = *reinterpret_cast<const f32x4 *>(&scales[buffer][2][8 * b + 4 * g]);
-                float w[4];
+            for (int i = 0; i < 2; ++i) {
+                u32x4 pairs;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(t[4 * b + e] - most);
-                    total = __builtin_fmaf(w[e], inverse[e], total);
+                for (int b = 0; b < 2; ++b) {
+                    const f32x4 inverse = *reinterpret_cast<const f32x4 *>(at + 2 * kBlock + 16 * i + 8 * b);
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = __builtin_amdgcn_exp2f(t[8 * i + 4 * b + e] - most);
+                        total = __builtin_fmaf(w[e], inverse[e], total);
+                    }
+                    pairs[2 * b] = f16_pair(w[0], w[1]), pairs[2 * b + 1] = f16_pair(w[2], w[3]);
                 }
-                pairs[b / 2][2 * (b % 2)] = f16_pair(w[0], w[1]), pairs[b / 2][2 * (b % 2) + 1] = f16_pair(w[2], w[3]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) {
-                    const f16x8 v = __builtin_bit_cast(f16x8, value_parts[buffer][(j * 2 + i) * 64 + lane]);
-                    acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pairs[i]), acc[j], 0, 0, 0);
+                    const f16x8 v = __builtin_bit_cast(f16x8, value_parts[(fourth * TILES * 2 + j * 2 + i) * 64 + lane]);
+                    acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pairs), acc[j], 0, 0, 0);
                 }
-            interleave<2 * TILES>();
+            }
+        };
+
+        bool dead[4] = {};  // of the step's record and of the next ones
+        lds_barrier();  // (the last piece's LDS is read)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (from + n < to) fetch(from + n, n), dead[n] = hole;
+        wait_vmcnt<0>();
+        lds_barrier();
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (from + n < to) stage(n, n, n);
+        lds_barrier();
+        if (from + 2 < to) fetch(from + 2, 0), dead[2] = hole;
+        wait_vmcnt<0>();
+        // A step is the scores of one record, while the one after the next is widened, and then its values. Waves 4 to 7 are half a step
+        // behind: of a SIMD's two waves one has vector instructions where the other has few.
+        lds_barrier();
+        if (wave >= 4) lds_barrier();
+        int third = 0;
+        for (int block = from; block < to; ++block) {
+            hole = false;
+            const int step = block - from;
+            if (block + 3 < to) fetch(block + 3, (step + 1) & 1);
+            dead[3] = hole;
+            if (block + 2 < to) stage(step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3);
+            score(third);
+            lds_barrier();
+            weigh_values(block, step & 3, dead[0]);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) dead[n] = dead[n + 1];
+            third = third == 2 ? 0 : third + 1;
             wait_vmcnt<0>();
-            lds_barrier();  // the record after the next has landed, the next one is widened, and this one used up
+            lds_barrier();
         }
+        if (wave < 4) lds_barrier();
         total += __shfl_xor(total, 32);
         const int i = wave * 32 + col;
         if constexpr (D > 64) {
@@ -1038,7 +1069,7 @@ static void launch_part(const AttendPlan &plan, const AttendArgs &a, const Cache
         constexpr int NT = decltype(tiles)::value;
         launch_lds<FewShape<D, NT>>(few_kernel<D, NT>, plan.tile.workgroups, stream, a, cache, packed);
     };
-    if (!plan.few) many_kernel<D><<<plan.tile.workgroups, kManyThreads, 2 * record_bytes(D), stream>>>(a, cache, packed);
+    if (!plan.few) launch_lds<ManyShape<D>>(many_kernel<D>, plan.tile.workgroups, stream, a, cache, packed);
     else if (plan.tile.rows == 16) few(std::integral_constant<int, 1>{});
     else if (plan.tile.rows == 32) few(std::integral_constant<int, 2>{});
     else if (plan.tile.rows == 48) few(std::integral_constant<int, 3>{});
