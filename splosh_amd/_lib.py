@@ -4,6 +4,7 @@ The library is loaded from this package directory; if it is missing, every call 
 ``SploshLibraryError`` -- there is no fallback path.
 """
 import ctypes
+import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -87,6 +88,10 @@ class Heads(ctypes.Structure):
                 ("ld_out", _i64)]
 
 
+HEADS = struct.Struct("PqqqPPq")  # a Heads struct
+assert HEADS.size == ctypes.sizeof(Heads)
+
+
 # name -> (restype, argtypes); every symbol include/splosh_q4.h declares.
 SIGNATURES = {
     "splosh_q4_layout_init": (_int, [_i64, _i64, _int, _i64, _i64, ctypes.POINTER(Layout)]),
@@ -146,14 +151,12 @@ SIGNATURES = {
     "splosh_sample_workspace_bytes": (_sz, [_i64, _i64]),
     "splosh_sample": (_int, [_vp, _i64, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "splosh_cache_page_bytes": (_sz, [_i64, _i64, _i64]),
-    "splosh_rotate_heads": (_int, [ctypes.POINTER(Heads), _int, _int, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp]),
-    "splosh_cache_write": (_int, [ctypes.POINTER(Cache), ctypes.POINTER(Packed), ctypes.POINTER(Heads),
-                                  ctypes.POINTER(Heads), ctypes.POINTER(Heads), _int, _i64, _vp, _i64, ctypes.c_float,
-                                  _vp]),
-    "splosh_cache_read": (_int, [ctypes.POINTER(Cache), ctypes.POINTER(Packed), _i64, _vp, _i64, _vp, _i64, _vp]),
-    "splosh_attend_workspace_bytes": (_sz, [ctypes.POINTER(Cache), ctypes.POINTER(Packed), _i64, _i64, _i64]),
-    "splosh_attend": (_int, [_vp, _i64, _i64, _i64, ctypes.POINTER(Cache), ctypes.POINTER(Packed), _i64, _i64,
-                             ctypes.c_float, _vp, _i64, _vp, _sz, _vp]),
+    # (The structs of these are passed by address: a handle keeps its own, a list of heads is packed for the call.)
+    "splosh_rotate_heads": (_int, [_vp, _int, _int, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp]),
+    "splosh_cache_write": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _vp, _i64, ctypes.c_float, _vp]),
+    "splosh_cache_read": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "splosh_attend_workspace_bytes": (_sz, [_vp, _vp, _i64, _i64, _i64]),
+    "splosh_attend": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _vp, _sz, _vp]),
     "splosh_verify_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "splosh_verify": (_int, [_vp, _i64, _int, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _int, _vp, _vp, _vp, _sz,
                              _vp]),

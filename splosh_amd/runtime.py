@@ -816,13 +816,6 @@ def sample(logits, uniforms=None, temperature=None, top_k=None, top_p=None, min_
 # ---- the attention layers of a packed step, and its drafted tokens ---------------------------------
 
 
-def _same_device(t, index, name):
-    if not t.is_cuda:
-        raise SploshError(12, f"{name} is not a device tensor")
-    if t.get_device() != index:
-        raise SploshError(13, f"{name} is on {t.device}, the operands on cuda:{index}")
-
-
 @dataclass(frozen=True)
 class Packed:
     """How a step's rows are packed (splosh_packed): ``starts`` int32 [requests + 1], the first row of each request
@@ -843,7 +836,7 @@ class Packed:
         starts = _vector(self.starts, requests + 1, torch.int32, index, "starts")
         lengths = _vector(self.lengths, requests, torch.int32, index, "lengths")
         c = _lib.Packed(starts, lengths, table.data_ptr(), requests, _row_stride(table), pages)
-        for name, value in dict(index=index, requests=requests, _c=c).items():
+        for name, value in dict(index=index, requests=requests, _c=c, _at=ctypes.addressof(c)).items():
             object.__setattr__(self, name, value)
 
     def c(self):
@@ -877,7 +870,7 @@ class Cache:
             raise GemmQ4Error(8, f"bufferTooSmall(name: page, expected: {need}, observed: {data.shape[1]})")
         stride = data.stride(0) if data.shape[0] > 1 else (data.shape[1] + 15) // 16 * 16
         c = _lib.Cache(data.data_ptr(), data.shape[0], stride, self.page_tokens, self.heads, self.dim)
-        for name, value in dict(index=index, pages=data.shape[0], _c=c).items():
+        for name, value in dict(index=index, pages=data.shape[0], _c=c, _at=ctypes.addressof(c)).items():
             object.__setattr__(self, name, value)
 
     def c(self):
@@ -892,33 +885,31 @@ class Cache:
 
 def _head_vectors(t, rows, heads, dim, dtype, index, name):
     """(address, row stride, head stride, heads) of `rows` rows of `heads` (None: its own) vectors of `dim`."""
-    _same_device(t, index, name)
-    if t.dim() != 3 or t.dtype != dtype or (t.stride(2) != 1 and t.shape[2] > 1):
+    shape, strides = t.shape, t.stride()
+    if t.get_device() != index:
+        raise SploshError(13 if t.is_cuda else 12, f"{name} is on {t.device}, the operands on cuda:{index}")
+    if len(shape) != 3 or t.dtype != dtype or (strides[2] != 1 and shape[2] > 1):
         raise SploshError(13, f"{name} must be {dtype} [rows, heads, dim] with contiguous vectors")
-    if t.shape[2] != dim or t.shape[1] == 0 or (heads is not None and t.shape[1] != heads):
-        raise GemmQ4Error(1, f"{name} is {tuple(t.shape)}, [rows, {heads or 'heads'}, {dim}] is needed")
-    if t.shape[0] < rows:
-        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows} rows, observed: {t.shape[0]})")
-    head = t.stride(1) if t.shape[1] > 1 else max(t.stride(1), dim)
-    row = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), dim)
-    return t.data_ptr(), row, head, t.shape[1]
+    have, count, size = shape
+    if size != dim or count == 0 or (heads is not None and count != heads):
+        raise GemmQ4Error(1, f"{name} is {tuple(shape)}, [rows, {heads or 'heads'}, {dim}] is needed")
+    if have < rows:
+        raise GemmQ4Error(8, f"bufferTooSmall(name: {name}, expected: {rows} rows, observed: {have})")
+    # (The stride of a dimension of one can be anything.)
+    return t.data_ptr(), strides[0] if have > 1 else max(strides[0], dim), strides[1] if count > 1 else max(strides[1], dim), count
 
 
 def _dense_heads(t, rows, heads, dim, index, name):
     """(address, row stride) of a bf16 output [rows, heads, dim] whose rows are dense."""
-    ptr, _, head, _ = _head_vectors(t, rows, heads, dim, torch.bfloat16, index, name)
+    ptr, row, head, _ = _head_vectors(t, rows, heads, dim, torch.bfloat16, index, name)
     if head != dim and heads > 1:
         raise SploshError(13, f"{name} must have dense rows")
-    return ptr, t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * dim)
+    return ptr, row if t.shape[0] > 1 else max(row, heads * dim)
 
 
-def _norm_weight(t, dim, index, name):
-    return _vector(t, dim, torch.bfloat16, index, name)
-
-
-def _frequencies(t, index):
-    """(address, rotary dimensions)."""
-    return (None, 0) if t is None else (_vector(t, 0, torch.float32, index, "frequencies"), 2 * t.numel())
+def _address(t, rows, dtype, index, name):
+    """_vector with 0 for None."""
+    return 0 if t is None else _vector(t, rows, dtype, index, name)
 
 
 def rotate_heads(xs, positions, frequencies, weights=None, eps=1e-6, outs=None, rows=None, stream=None):
@@ -926,30 +917,30 @@ def rotate_heads(xs, positions, frequencies, weights=None, eps=1e-6, outs=None, 
     their projections left them) normed over each head by ``weights`` (bf16 [dim] each; None: no norm) and their
     pairs (i, i + len(frequencies)) turned by positions[m] * frequencies[i] (int32 [rows], fp32; None: not). Returns bf16
     [rows, heads, dim] each."""
-    xs = list(xs)
-    if not xs or len(xs) > 8:
+    count = len(xs)
+    if not 0 < count <= 8:
         raise GemmQ4Error(1, "one to eight tensors")
-    index = _index(xs[0], "x")
-    dtype, dim = xs[0].dtype, xs[0].shape[-1]
-    rows = xs[0].shape[0] if rows is None else rows
+    if (weights is not None and len(weights) != count) or (outs is not None and len(outs) != count):
+        raise GemmQ4Error(1, "a weight and an output for each tensor")
+    first = xs[0]
+    index = _index(first, "x")
+    dtype, dim = first.dtype, first.shape[-1]
+    rows = first.shape[0] if rows is None else rows
     if rows <= 0:
         raise GemmQ4Error(1, "rows must be positive")
-    weights = [None] * len(xs) if weights is None else list(weights)
-    if len(weights) != len(xs) or (outs is not None and len(outs) != len(xs)):
-        raise GemmQ4Error(1, "a weight and an output for each tensor")
-    code = _dtype_code(dtype)
-    parts = [_head_vectors(x, rows, None, dim, dtype, index, "x") for x in xs]
-    freq, rotary = _frequencies(frequencies, index)
+    code, bf16 = _dtype_code(dtype), torch.bfloat16
+    if outs is None:
+        with _launch(index), _allocating(stream):
+            outs = [torch.empty((rows, x.shape[1], dim), dtype=bf16, device=x.device) for x in xs]
+    parts = b""
+    for i, x in enumerate(xs):
+        part = _head_vectors(x, rows, None, dim, dtype, index, "x")
+        weight = 0 if weights is None else _address(weights[i], dim, bf16, index, "weight")
+        parts += _lib.HEADS.pack(*part, weight, *_dense_heads(outs[i], rows, part[3], dim, index, "output"))
+    at = _address(positions, rows, torch.int32, index, "positions")
+    freq, rotary = (0, 0) if frequencies is None else (_vector(frequencies, 0, torch.float32, index, "frequencies"), 2 * frequencies.numel())
     with _launch(index):
-        if outs is None:
-            with _allocating(stream):
-                outs = [torch.empty((rows, x.shape[1], dim), dtype=torch.bfloat16, device=x.device) for x in xs]
-        cs = (_lib.Heads * len(xs))(*[
-            _lib.Heads(*p, _norm_weight(w, dim, index, "weight"), *_dense_heads(o, rows, p[3], dim, index, "output"))
-            for p, w, o in zip(parts, weights, outs)])
-        st = _lib.lib().splosh_rotate_heads(cs, len(xs), code, rows, dim,
-                                            _vector(positions, rows, torch.int32, index, "positions"), freq, rotary, eps,
-                                            _raw_stream(stream, index))
+        st = _lib.lib().splosh_rotate_heads(parts, count, code, rows, dim, at, freq, rotary, eps, _raw_stream(stream, index))
     if st:
         _lib.check(st)
     return outs
@@ -960,27 +951,25 @@ def cache_write(cache, packed, k, v, q=None, frequencies=None, k_weight=None, q_
     """splosh_cache_write: a step's keys (normed by ``k_weight``, turned by their rows' positions; neither where that is
     None) and values, [rows, cache.heads, dim] fp32 or bf16, into the cache at the places of ``packed``. With ``q``
     [rows, heads, dim] also the step's queries normed and turned, in the same launch: returned as bf16 (``out``)."""
-    index = cache.index
-    _same_device(packed.table, index, "table")
+    index, dim, dtype = cache.index, cache.dim, k.dtype
+    if packed.index != index:
+        raise SploshError(13, f"the table is on cuda:{packed.index}, the cache on cuda:{index}")
     rows = k.shape[0] if rows is None else rows
     if rows <= 0:
         raise GemmQ4Error(1, "rows must be positive")
-    dim, dtype = cache.dim, k.dtype
-    code = _dtype_code(dtype)
-    kc = _lib.Heads(*_head_vectors(k, rows, cache.heads, dim, dtype, index, "k"), _norm_weight(k_weight, dim, index, "k_weight"))
-    vc = _lib.Heads(*_head_vectors(v, rows, cache.heads, dim, dtype, index, "v"))
-    freq, rotary = _frequencies(frequencies, index)
+    code, bf16, pack = _dtype_code(dtype), torch.bfloat16, _lib.HEADS.pack
+    kc = pack(*_head_vectors(k, rows, cache.heads, dim, dtype, index, "k"), _address(k_weight, dim, bf16, index, "k_weight"), 0, 0)
+    vc = pack(*_head_vectors(v, rows, cache.heads, dim, dtype, index, "v"), 0, 0, 0)
+    freq, rotary = (0, 0) if frequencies is None else (_vector(frequencies, 0, torch.float32, index, "frequencies"), 2 * frequencies.numel())
     qc = None
+    if q is not None:
+        part = _head_vectors(q, rows, None, dim, dtype, index, "q")
+        if out is None:
+            with _launch(index), _allocating(stream):
+                out = torch.empty((rows, part[3], dim), dtype=bf16, device=q.device)
+        qc = pack(*part, _address(q_weight, dim, bf16, index, "q_weight"), *_dense_heads(out, rows, part[3], dim, index, "output"))
     with _launch(index):
-        if q is not None:
-            part = _head_vectors(q, rows, None, dim, dtype, index, "q")
-            if out is None:
-                with _allocating(stream):
-                    out = torch.empty((rows, q.shape[1], dim), dtype=torch.bfloat16, device=q.device)
-            qc = _lib.Heads(*part, _norm_weight(q_weight, dim, index, "q_weight"),
-                            *_dense_heads(out, rows, part[3], dim, index, "output"))
-        st = _lib.lib().splosh_cache_write(cache._c, packed._c, kc, vc, qc, code, rows, freq, rotary, eps,
-                                           _raw_stream(stream, index))
+        st = _lib.lib().splosh_cache_write(cache._at, packed._at, kc, vc, qc, code, rows, freq, rotary, eps, _raw_stream(stream, index))
     if st:
         _lib.check(st)
     return out if q is not None else None
@@ -989,20 +978,22 @@ def cache_write(cache, packed, k, v, q=None, frequencies=None, k_weight=None, q_
 def cache_read(cache, packed, rows=None, k=None, v=None, stream=None):
     """splosh_cache_read: what the cache holds at the places of ``packed``'s rows, as bf16 (k, v) [rows, heads, dim]. Of a
     request with n rows these are its last n tokens. rows: that of k or v where they are given."""
-    index = cache.index
-    _same_device(packed.table, index, "table")
+    index, heads, dim = cache.index, cache.heads, cache.dim
+    if packed.index != index:
+        raise SploshError(13, f"the table is on cuda:{packed.index}, the cache on cuda:{index}")
     if rows is None:
         if k is None and v is None:
             raise GemmQ4Error(1, "rows or an output is needed")
         rows = (k if k is not None else v).shape[0]
     if rows <= 0:
         raise GemmQ4Error(1, "rows must be positive")
+    if k is None and v is None:
+        with _launch(index), _allocating(stream):
+            k, v = (torch.empty((rows, heads, dim), dtype=torch.bfloat16, device=cache.data.device) for _ in "kv")
+    kp = (None, 0) if k is None else _dense_heads(k, rows, heads, dim, index, "k")
+    vp = (None, 0) if v is None else _dense_heads(v, rows, heads, dim, index, "v")
     with _launch(index):
-        if k is None and v is None:
-            with _allocating(stream):
-                k, v = (torch.empty((rows, cache.heads, cache.dim), dtype=torch.bfloat16, device=cache.data.device) for _ in "kv")
-        places = [(None, 0) if t is None else _dense_heads(t, rows, cache.heads, cache.dim, index, n) for t, n in ((k, "k"), (v, "v"))]
-        st = _lib.lib().splosh_cache_read(cache._c, packed._c, rows, *places[0], *places[1], _raw_stream(stream, index))
+        st = _lib.lib().splosh_cache_read(cache._at, packed._at, rows, *kp, *vp, _raw_stream(stream, index))
     if st:
         _lib.check(st)
     return k, v
@@ -1011,7 +1002,7 @@ def cache_read(cache, packed, rows=None, k=None, v=None, stream=None):
 def attend_workspace_bytes(cache, packed, rows, q_heads, shared=0):
     """splosh_attend_workspace_bytes: the scratch an attention call needs (0: not a valid shape)."""
     with _launch(cache.index):
-        return _lib.lib().splosh_attend_workspace_bytes(cache._c, packed._c, rows, q_heads, shared)
+        return _lib.lib().splosh_attend_workspace_bytes(cache._at, packed._at, rows, q_heads, shared)
 
 
 def attend(q, cache, packed, shared=0, scale=None, out=None, rows=None, stream=None, workspace=None):
@@ -1019,12 +1010,12 @@ def attend(q, cache, packed, shared=0, scale=None, out=None, rows=None, stream=N
     which holds the step's own keys and values already. shared: the first tokens (whole pages) that all requests have in
     common, read once for all through request 0's pages. scale None: dim ** -0.5. Returns bf16 [rows, heads, dim] with
     dense rows, the out projection's activation."""
-    index = cache.index
-    _same_device(packed.table, index, "table")
+    index, dim = cache.index, cache.dim
+    if packed.index != index:
+        raise SploshError(13, f"the table is on cuda:{packed.index}, the cache on cuda:{index}")
     rows = q.shape[0] if rows is None else rows
     if rows <= 0:
         raise GemmQ4Error(1, "rows must be positive")
-    dim = cache.dim
     part = _head_vectors(q, rows, None, dim, torch.bfloat16, index, "q")
     lib = _lib.lib()
     with _launch(index):
@@ -1032,9 +1023,9 @@ def attend(q, cache, packed, shared=0, scale=None, out=None, rows=None, stream=N
             with _allocating(stream):
                 out = torch.empty((rows, part[3], dim), dtype=torch.bfloat16, device=q.device) if out is None else out
                 if workspace is None:
-                    need = lib.splosh_attend_workspace_bytes(cache._c, packed._c, rows, part[3], shared)
+                    need = lib.splosh_attend_workspace_bytes(cache._at, packed._at, rows, part[3], shared)
                     workspace = torch.empty(max(1, need), dtype=torch.uint8, device=q.device)
-        st = lib.splosh_attend(*part, cache._c, packed._c, rows, shared, dim ** -0.5 if scale is None else scale,
+        st = lib.splosh_attend(*part, cache._at, packed._at, rows, shared, dim ** -0.5 if scale is None else scale,
                                *_dense_heads(out, rows, part[3], dim, index, "output"),
                                *_given_workspace(workspace, index), _raw_stream(stream, index))
     if st:

@@ -34,22 +34,30 @@ def queries(**change):
     return heads(**{**dict(x=P[5], row_stride=1024, heads=8, out=P[6], ld_out=1024), **change})
 
 
+def at(x):
+    """The address of a struct."""
+    return ctypes.addressof(x) if isinstance(x, ctypes.Structure) else x
+
+
 def name(st):
     return _lib.STATUS_NAMES.get(st, st)
 
 
 def write(c=None, p=None, k=None, v=None, q=None, dtype=_lib.BF16, rows=7, frequencies=P[7], rotary=64):
-    return name(_lib.lib().splosh_cache_write(c or cache(), p or packed(), k or heads(), v or heads(), q or queries(), dtype, rows,
+    args = (c or cache(), p or packed(), k or heads(), v or heads(), q or queries())
+    return name(_lib.lib().splosh_cache_write(*map(at, args), dtype, rows,
                                               frequencies, rotary, 1e-6, None))
 
 
 def read(c=None, p=None, rows=7, k=P[4], ldk=512, v=P[5], ldv=512):
-    return name(_lib.lib().splosh_cache_read(c or cache(), p or packed(), rows, k, ldk, v, ldv, None))
+    args = (c or cache(), p or packed())
+    return name(_lib.lib().splosh_cache_read(*map(at, args), rows, k, ldk, v, ldv, None))
 
 
 def attend(c=None, p=None, q=P[5], row=1024, head=128, heads=8, rows=7, shared=64, scale=0.1, out=P[6], ld=1024, ws=P[8],
            ws_bytes=1 << 40):
-    return name(_lib.lib().splosh_attend(q, row, head, heads, c or cache(), p or packed(), rows, shared, scale, out, ld, ws, ws_bytes, None))
+    args = (c or cache(), p or packed())
+    return name(_lib.lib().splosh_attend(q, row, head, heads, *map(at, args), rows, shared, scale, out, ld, ws, ws_bytes, None))
 
 
 @pytest.mark.parametrize("change,case", [
@@ -104,8 +112,8 @@ def test_calls(call, case):
 def test_rotation(change, case):
     a = dict(count=2, dtype=_lib.BF16, rows=5, dim=128, positions=P[7], frequencies=P[8], rotary=64)
     same = change.pop("same", False)
-    parts = (_lib.Heads * 2)(queries(), queries(x=P[4], out=P[6] if same else P[9]))
-    parts = change.pop("parts", parts)
+    listed = (_lib.Heads * 2)(queries(), queries(x=P[4], out=P[6] if same else P[9]))
+    parts = change.pop("parts", ctypes.addressof(listed))
     a.update(change)
     assert name(_lib.lib().splosh_rotate_heads(parts, a["count"], a["dtype"], a["rows"], a["dim"], a["positions"], a["frequencies"],
                                                a["rotary"], 1e-6, None)) == case
@@ -129,9 +137,10 @@ def test_sizes():
     lib = _lib.lib()
     assert lib.splosh_cache_page_bytes(4, 256, 256) == 4 * 8 * (64 * 256 + 256)
     assert [lib.splosh_cache_page_bytes(*a) for a in ((0, 64, 32), (1, 65, 32), (1, 64, 33), (1, 64, 0))] == [0] * 4
-    assert lib.splosh_attend_workspace_bytes(cache(), packed(), 7, 6, 0) == 0 and lib.splosh_attend_workspace_bytes(cache(), packed(), 0, 8, 0) == 0
-    assert lib.splosh_attend_workspace_bytes(None, packed(), 7, 8, 0) == 0 and lib.splosh_verify_workspace_bytes(1, 1 << 22, 1) == 0
-    assert lib.splosh_attend_workspace_bytes(cache(), packed(), 7, 8, 0) >= 16384 <= lib.splosh_verify_workspace_bytes(8, 1000, 2)
+    c, p = cache(), packed()
+    assert lib.splosh_attend_workspace_bytes(at(c), at(p), 7, 6, 0) == 0 and lib.splosh_attend_workspace_bytes(at(c), at(p), 0, 8, 0) == 0
+    assert lib.splosh_attend_workspace_bytes(None, at(p), 7, 8, 0) == 0 and lib.splosh_verify_workspace_bytes(1, 1 << 22, 1) == 0
+    assert lib.splosh_attend_workspace_bytes(at(c), at(p), 7, 8, 0) >= 16384 <= lib.splosh_verify_workspace_bytes(8, 1000, 2)
 
 
 PLACES = """
