@@ -2,7 +2,7 @@
 // rotation by position in one pass, keys and values into the 8-bit cache, and the cache read back.
 //
 // All of it is bound by memory or, for few rows, by the launch. A workgroup takes one row: its first threads compute
-// the row's cosines and sines, once for all heads, and then each wave takes one (row, head) vector at a time, dim / 64
+// the row's cosines and sines, once for all heads, and then each wave takes four (row, head) vectors at a time, dim / 64
 // consecutive elements a lane. The two halves of a rotated pair meet through the wave's own LDS.
 #include "cache.hpp"
 
@@ -29,18 +29,6 @@ struct HeadArgs {
     int half;
     float eps;
 };
-
-// Every lane's sum, largest value.
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-    return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, m));
-    return v;
-}
 
 template <int E, typename T>
 __device__ __forceinline__ void load_elements(const T *at, int wide, float (&v)[E]) {
@@ -94,7 +82,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[E], float &scale) 
         most = __builtin_fmaxf(most, __builtin_fabsf(v[e]));
         bad |= !(__builtin_fabsf(v[e]) < __builtin_inff());
     }
-    most = wave_max(most);
+    most = wave_max(most);  // (the same in every lane)
     scale = most / 127.0f;
     const bool small = scale < kLeastScale;
     if (small) scale = kLeastScale;
@@ -113,10 +101,28 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[E], float &scale) 
 
 template <typename T, int D, bool kCache>
 __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, CacheView cache, PackedView packed) {
-    constexpr int E = D / 64;
+    constexpr int E = D / 64, BATCH = 4;  // vectors that a wave has in hand at a time
     __shared__ float2 turn[D / 2];
-    __shared__ float vector[kHeadWaves][D];
-    const int row = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    __shared__ float vector[kHeadWaves][BATCH][D];
+    const int row = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int end = min(a.units, (int)(blockIdx.y + 1) * a.chunk);
+    int unit = blockIdx.y * a.chunk + wave;
+    auto part_of = [&](int u) {
+        int which = 0;
+        while (which + 1 < a.parts && u >= a.part[which + 1].first) ++which;
+        return which;
+    };
+    float v[BATCH][E];
+    auto load = [&]() {
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            const int u = unit + n * kHeadWaves;
+            if (u >= end) break;
+            const HeadPart &part = a.part[part_of(u)];
+            load_elements<E>((const T *)part.x + row * part.row_stride + (u - part.first) * part.head_stride + lane * E, part.wide, v[n]);
+        }
+    };
+    load();  // (on its way while the row's place is looked up)
     int position, page = 0, at = 0;
     bool placed = false;
     if (kCache) {
@@ -135,57 +141,69 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, CacheVi
         turn[tid] = make_float2(c, s);
     }
     __syncthreads();
-    const int end = min(a.units, (int)(blockIdx.y + 1) * a.chunk);
-    for (int unit = blockIdx.y * a.chunk + wave; unit < end; unit += kHeadWaves) {
-        int which = 0;
-        while (which + 1 < a.parts && unit >= a.part[which + 1].first) ++which;
-        const HeadPart &part = a.part[which];
-        const int head = unit - part.first;
-        if (kCache && part.kept && !placed) continue;
-        float v[E];
-        load_elements<E>((const T *)part.x + row * part.row_stride + head * part.head_stride + lane * E, part.wide, v);
-        if (part.weight) {
-            float sum = 0.0f;
+    while (true) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += v[e] * v[e];
-            const float inv = 1.0f / sqrtf(wave_sum(sum) * (1.0f / D) + a.eps);
-            float w[E];
-            load_elements<E>(part.weight + lane * E, 0, w);
+        for (int n = 0; n < BATCH; ++n) {
+            const int u = unit + n * kHeadWaves;
+            if (u >= end) break;
+            const HeadPart &part = a.part[part_of(u)];
+            if (part.weight) {
+                float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = v[e] * inv * w[e];
+                for (int e = 0; e < E; ++e) sum += v[n][e] * v[n][e];
+                const float inv = 1.0f / sqrtf(wave_sum(sum) * (1.0f / D) + a.eps);
+                float w[E];
+                load_elements<E>(part.weight + lane * E, 0, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[n][e] = v[n][e] * inv * w[e];
+            }
+            if (part.rotated) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) vector[wave][n][lane * E + e] = v[n][e];
+            }
         }
-        if (part.rotated) {
+        // (What the wave's lanes wrote for each other: nothing of it is another wave's.)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int e = 0; e < E; ++e) vector[wave][lane * E + e] = v[e];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+        for (int n = 0; n < BATCH; ++n) {
+            const int u = unit + n * kHeadWaves;
+            if (u >= end) break;
+            const HeadPart &part = a.part[part_of(u)];
+            const int head = u - part.first;
+            if (part.rotated) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = lane * E + e;
-                if (i < a.half) {
-                    const float2 t = turn[i];
-                    v[e] = v[e] * t.x - vector[wave][i + a.half] * t.y;
-                } else if (i < 2 * a.half) {
-                    const float2 t = turn[i - a.half];
-                    v[e] = v[e] * t.x + vector[wave][i - a.half] * t.y;
+                for (int e = 0; e < E; ++e) {
+                    const int i = lane * E + e;
+                    if (i < a.half) {
+                        const float2 t = turn[i];
+                        v[n][e] = v[n][e] * t.x - vector[wave][n][i + a.half] * t.y;
+                    } else if (i < 2 * a.half) {
+                        const float2 t = turn[i - a.half];
+                        v[n][e] = v[n][e] * t.x + vector[wave][n][i - a.half] * t.y;
+                    }
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            if (!kCache || !part.kept) {
+                store_bf16<E>(part.out + row * part.ld_out + head * D + lane * E, part.wide, v[n]);
+                continue;
+            }
+            if (!placed) continue;
+            float scale;
+            const uint32_t codes = codes_of<E>(v[n], scale);
+            uint8_t *record = record_of<D>(cache, page, head, at / kBlock);
+            const int token = at % kBlock, values = part.kept - 1;
+            uint8_t *to = record + (values * kBlock + token) * D + lane * E;
+            if constexpr (E == 4) *reinterpret_cast<uint32_t *>(to) = codes;
+            else if constexpr (E == 2) *reinterpret_cast<uint16_t *>(to) = (uint16_t)codes;
+            else *to = (uint8_t)codes;
+            if (lane == 0) reinterpret_cast<float *>(record + 2 * kBlock * D)[values * kBlock + token] = scale;
         }
-        if (!kCache || !part.kept) {
-            store_bf16<E>(part.out + row * part.ld_out + head * D + lane * E, part.wide, v);
-            continue;
-        }
-        float scale;
-        const uint32_t codes = codes_of<E>(v, scale);
-        uint8_t *record = record_of<D>(cache, page, head, at / kBlock);
-        const int token = at % kBlock, values = part.kept - 1;
-        uint8_t *to = record + (values * kBlock + token) * D + lane * E;
-        if constexpr (E == 4) *reinterpret_cast<uint32_t *>(to) = codes;
-        else if constexpr (E == 2) *reinterpret_cast<uint16_t *>(to) = (uint16_t)codes;
-        else *to = (uint8_t)codes;
-        if (lane == 0) reinterpret_cast<float *>(record + 2 * kBlock * D)[values * kBlock + token] = scale;
+        unit += BATCH * kHeadWaves;
+        if (unit >= end) return;
+        load();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -198,11 +216,12 @@ struct ReadArgs {
 template <int D>
 __global__ __launch_bounds__(kHeadThreads) void cache_read_kernel(ReadArgs a, CacheView cache, PackedView packed) {
     constexpr int E = D / 64;
-    const int row = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int row = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r = request_of(packed.starts, packed.requests, row);
     if (r < 0) return;
     int page = 0, at = 0;
     const bool placed = place_of(cache, packed, r, packed.lengths[r] - packed.starts[r + 1] + row, page, at);
+#pragma unroll 4
     for (int unit = wave; unit < 2 * cache.heads; unit += kHeadWaves) {
         const int values = unit & 1, head = unit >> 1;
         if (!a.out[values]) continue;
@@ -210,10 +229,13 @@ __global__ __launch_bounds__(kHeadThreads) void cache_read_kernel(ReadArgs a, Ca
         if (placed) {
             const uint8_t *record = record_of<D>(cache, page, head, at / kBlock);
             const int token = at % kBlock;
-            const uint8_t *codes = record + (values * kBlock + token) * D + lane * E;
+            struct alignas(E) Codes {
+                uint8_t of[E];
+            };
+            const Codes codes = *reinterpret_cast<const Codes *>(record + (values * kBlock + token) * D + lane * E);
             const float scale = reinterpret_cast<const float *>(record + 2 * kBlock * D)[values * kBlock + token];
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = (float)(codes[e] - 128) * scale;
+            for (int e = 0; e < E; ++e) v[e] = (float)(codes.of[e] - 128) * scale;
         }
         store_bf16<E>(a.out[values] + row * a.ld[values] + head * D + lane * E, a.wide[values], v);
     }
