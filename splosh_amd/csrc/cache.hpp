@@ -35,29 +35,6 @@ inline PackedView view_of(const splosh_packed &p, int64_t rows) {
     return {p.starts, p.lengths, p.table, p.table_stride, (int)p.table_pages, (int)p.requests, (int)rows};
 }
 
-// The sum, and the largest, of a value over the wave's lanes, in every lane: within rows of sixteen lanes, then from row to row, and the last
-// lane's result read back.
-template <typename F>
-__device__ __forceinline__ float wave_fold(float v, float none, F fold) {
-    auto step = [&](auto ctrl, auto rows) {
-        const int other = __builtin_amdgcn_update_dpp((int)__float_as_uint(none), (int)__float_as_uint(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
-        v = fold(v, __uint_as_float((uint32_t)other));
-    };
-    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
-    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    return wave_fold(v, 0.0f, [](float a, float b) { return a + b; });
-}
-__device__ __forceinline__ float wave_max(float v) {
-    return wave_fold(v, 0.0f, [](float a, float b) { return __builtin_fmaxf(a, b); });  // (of values that are not negative)
-}
-
 // The request that packed row `row` belongs to, -1: none. All lanes of a wave call it with the same row: 64 starts at a time.
 __device__ __forceinline__ int request_of(const int32_t *starts, int requests, int row) {
     const int lane = threadIdx.x & 63;
