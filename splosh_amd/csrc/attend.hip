@@ -32,7 +32,10 @@ constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
 constexpr int kManyThreads = 512, kManyRows = 256;
 constexpr int kManyKeys = 2 * kBlock;  // of a unit of the kernel for many vectors
-constexpr int kExtra = 1;             // units that a segment costs beside its keys
+constexpr int64_t kJoinApart = 4096;  // (row, query head) vectors that are joined a wave each
+// Units that a segment costs beside its keys. (Few vectors: 3, where 1 is 119 instead of 116 us for the 64 requests of 512 MB, 108 instead of
+// 106 for the verify step; many: 1 to 6 are the same within 1 %.)
+constexpr int kFewExtra = 3, kManyExtra = 1;
 
 struct AttendArgs {
     const uint16_t *q;
@@ -232,6 +235,28 @@ __device__ __forceinline__ float group_max(float v) {
     return v;
 }
 
+// A span's units, and the tile that unit `offset` of them is in (offset: then in that tile), 64 tiles at a time in a wave's lanes. (One after the other,
+// the 48 tiles of 2048 rows with 24 heads on 4 took every workgroup 13 us.)
+__device__ __forceinline__ int wave_units(const Span &span, const TileShape &tile, int tiles) {
+    const int lane = threadIdx.x & 63;
+    int units = 0;
+    for (int base = 0; base < tiles; base += 64) units += base + lane < tiles ? tile_units(span, tile, base + lane) : 0;
+    return __builtin_amdgcn_readlane(running_sum(units), 63);
+}
+__device__ __forceinline__ int wave_tile(const Span &span, const TileShape &tile, int tiles, int &offset) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0;; base += 64) {
+        const int units = base + lane < tiles ? tile_units(span, tile, base + lane) : 0, units_to = running_sum(units);
+        const int all = __builtin_amdgcn_readlane(units_to, 63);
+        if (offset < all || base + 64 >= tiles) {
+            const int t = __builtin_ctzll(__ballot(offset < units_to) | 1ull << 63);
+            offset -= __builtin_amdgcn_readlane(units_to - units, t);
+            return base + t;
+        }
+        offset -= all;
+    }
+}
+
 // Calls `work` for each piece of the launch's units that workgroup blockIdx.x takes. All threads call it.
 template <int THREADS, typename F>
 __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView &cache, const PackedView &packed, F work) {
@@ -249,13 +274,25 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
     Span span;
     if (a.prefix) {
         span = uniform(prefix_span(packed, a.shared));
-        total = tile.heads * units_before(span, tile, tiles_of(span, tile));
+        total = tile.heads * wave_units(span, tile, tiles_of(span, tile));
     } else if (few) {
         int units = 0, segments = 0;
         if (lane < packed.requests) {
             mine = own_span(packed, cache.page_tokens, a.shared, lane);
-            const int tiles = tiles_of(mine, tile);
-            units = tile.heads * units_before(mine, tile, tiles), segments = tile.heads * tiles;
+            segments = tile.heads * tiles_of(mine, tile);
+        }
+        // (A lane each, or all lanes for one after the other, whichever takes fewer steps.)
+        int longest = segments;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) longest = max(longest, __shfl_xor(longest, m));
+        if (uniform(longest) > tile.heads * packed.requests) {
+            for (int r = 0; r < packed.requests; ++r) {
+                const Span s = span_at(r);
+                const int all = tile.heads * wave_units(s, tile, tiles_of(s, tile));
+                units = lane == r ? all : units;
+            }
+        } else if (lane < packed.requests) {
+            units = tile.heads * units_before(mine, tile, tiles_of(mine, tile));
         }
         const int units_to = running_sum(units), segments_to = running_sum(segments);
         total = __builtin_amdgcn_readlane(units_to, 63);
@@ -305,15 +342,11 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
     if (w >= sharers) return;
     int unit = first_unit(total, sharers, w);
     const int end = first_unit(total, sharers, w + 1);
-    int tiles = tiles_of(span, tile), head, t = 0, offset = unit - before;
-    {
-        const int each = units_before(span, tile, tiles);
-        head = offset / each;
-        offset -= head * each;
-        int units = tile_units(span, tile, 0);
-        while (offset >= units) offset -= units, units = tile_units(span, tile, ++t);
-        segment += head * tiles + t;
-    }
+    const int each = wave_units(span, tile, tiles_of(span, tile));
+    int tiles = tiles_of(span, tile), offset = unit - before, head = offset / each;
+    offset -= head * each;
+    int t = wave_tile(span, tile, tiles, offset);
+    segment += head * tiles + t;
     while (true) {
         const int units = tile_units(span, tile, t), take = min(units - offset, end - unit);
         const int keys = tile_end(span, tile, t) - span.from, blocks = keys > 0 ? (keys + kBlock - 1) / kBlock : 0;
@@ -343,9 +376,9 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
 // The result of vector x, dimensions d .. d + N - 1 of N sums o with maximum M: written, or left in the piece's slot.
 template <int D, int N>
 __device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, int i, int d, const float *o, float total) {
+    const int x = p.tile * a.tile.rows + i;
+    if (x >= p.span.n * a.tile.group) return;
     if (p.direct) {
-        const int x = p.tile * a.tile.rows + i;
-        if (x >= p.span.n * a.tile.group) return;
         const int row = row_of(p, a.tile, x), h = head_of(p, a.tile, x);
         const float inv = 1.0f / total;
         uint16_t *at = a.out + row * a.ld_out + (int64_t)h * D + d;
@@ -369,7 +402,8 @@ __device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, 
 template <int D>
 __device__ __forceinline__ void write_total(const AttendArgs &a, const Piece &p, int i, float most, float total) {
     const int x = p.tile * a.tile.rows + i;
-    if (p.count > 0 && x < p.span.n * a.tile.group)
+    if (x >= p.span.n * a.tile.group) return;
+    if (p.count > 0)
         a.pieces[(int64_t)row_of(p, a.tile, x) * a.q_heads + head_of(p, a.tile, x)] = {p.slot, (int)blockIdx.x, p.count, i};
     if (p.direct) return;
     float *at = a.slots + p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)a.tile.rows * D;
@@ -720,7 +754,8 @@ struct ManyShape {
     static constexpr int kLoads = D == 64 ? 2 : D / 128;  // of a wave, of its eighth of a record's codes
     static constexpr int kKeys = 2 * record_bytes(D), kValues = kKeys + 3 * (D / 16) * kPitch, kScales = kValues + 4 * (D / 32) * 2048;
     static constexpr int kThreads = kManyThreads, kLds = kScales + 4 * 3 * kBlock * 4;
-    static_assert(kLds <= 160 * 1024, "LDS");
+    static constexpr int kSumPitch = D + 4;
+    static_assert(kLds <= 160 * 1024 && 8 * 16 * kSumPitch * 4 <= kLds, "LDS");
 };
 
 template <int D>
@@ -916,44 +951,65 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         }
         if (wave < 4) lds_barrier();
         total += __shfl_xor(total, 32);
-        const int i = wave * 32 + col;
-        if constexpr (D > 64) {
+        // The wave's sums go through its eighth of the LDS, sixteen vectors at a time, and out in whole rows: as the lanes have them, 16 bytes
+        // of 32 rows at once, 256 vectors of 256 dimensions took 9.7 us.
+        float *const turned = reinterpret_cast<float *>(lds) + wave * 16 * S::kSumPitch;
+        constexpr int ROWS = 256 / D;  // at once, 16 bytes a lane
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            if (col >> 4 == half) {
+                float *const at = turned + (col & 15) * S::kSumPitch;
+                if constexpr (D > 64) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+                    for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                        for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int j = 0; j < TILES; j += 4) {
-                        const float o[4] = {acc[j][4 * b + e], acc[j + 1][4 * b + e], acc[j + 2][4 * b + e], acc[j + 3][4 * b + e]};
-                        write_sums<D, 4>(a, p, i, 4 * (8 * j + 8 * b + 4 * g + e), o, total);
-                    }
-        } else {
-            // Tile t, row m holds dimension 4 (m % 16) + 2 t + m / 16: rows m and m + 16 of both tiles are four in a row.
+                            for (int j = 0; j < TILES; j += 4)
+                                *reinterpret_cast<f32x4 *>(at + 4 * (8 * j + 8 * b + 4 * g + e)) =
+                                    f32x4{acc[j][4 * b + e], acc[j + 1][4 * b + e], acc[j + 2][4 * b + e], acc[j + 3][4 * b + e]};
+                } else {
+                    // Tile t, row m holds dimension 4 (m % 16) + 2 t + m / 16: rows m and m + 16 of both tiles are four in a row.
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float o[4] = {acc[0][4 * b + e], acc[0][4 * b + 8 + e], acc[1][4 * b + e], acc[1][4 * b + 8 + e]};
-                    write_sums<D, 4>(a, p, i, 4 * (8 * b + 4 * g + e), o, total);
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<f32x4 *>(at + 4 * (8 * b + 4 * g + e)) =
+                                f32x4{acc[0][4 * b + e], acc[0][4 * b + 8 + e], acc[1][4 * b + e], acc[1][4 * b + 8 + e]};
                 }
+            }
+            // (What the wave's lanes wrote for each other: nothing of it is another wave's.)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+            for (int n = 0; n < 16; n += ROWS) {
+                const int i = n + lane / (D / 4), d = lane % (D / 4) * 4;
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(turned + i * S::kSumPitch + d);
+                const float o[4] = {x[0], x[1], x[2], x[3]};
+                write_sums<D, 4>(a, p, wave * 32 + 16 * half + i, d, o, __shfl(total, 16 * half + i));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
-        if (g == 0) write_total<D>(a, p, i, most, total);
+        if (g == 0) write_total<D>(a, p, wave * 32 + col, most, total);
     });
 }
 
 // ---- the pieces joined ----------------------------------------------------------------------------
 
-// A wave a (row, query head): the weights of its pieces, one a lane, and their sums in the order of the keys, sixteen pieces' loads
-// at a time.
-template <int D>
+// LANES lanes a (row, query head): the weights of its pieces, one a lane, and their sums in the order of the keys, BATCH pieces'
+// loads at a time. All 64 where there are few vectors, of many pieces each: what it takes is then three loads one after the other.
+// Sixteen where there are many: four vectors' loads are under way in a wave at once.
+template <int D, int LANES>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs prefix, PackedView packed) {
-    constexpr int E = D / 64, BATCH = 16;
-    typedef float Sums __attribute__((ext_vector_type(E == 1 ? 2 : E)));
-    const int64_t vector = (int64_t)blockIdx.x * (blockDim.x / 64) + uniform((int)threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, row = (int)(vector / own.q_heads), h = (int)(vector % own.q_heads);
-    if (row >= packed.rows || row >= packed.starts[packed.requests] || row < packed.starts[0]) return;
-    Pieces mine = own.pieces[vector];
-    if (mine.count == 1 && !own.partial) return;
+    constexpr int E = D / LANES, BATCH = LANES == 64 ? 16 : 64 / E < 4 ? 64 / E : 4;
+    typedef float Sums __attribute__((ext_vector_type(E == 1 ? 2 : E < 4 ? E : 4)));
+    const int64_t vector = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+    const int lane = threadIdx.x % LANES, row = (int)(vector / own.q_heads), h = (int)(vector % own.q_heads);
+    if (row >= packed.rows) return;
+    const int begin = packed.starts[0], end = packed.starts[packed.requests];  // (all four loads at once)
+    const Pieces mine = own.pieces[vector], theirs = prefix.pieces[vector];
+    if (row >= end | row < begin | (mine.count == 1 && !own.partial)) return;
     float top = kLowest, total = 0.0f, o[E] = {};
     auto join = [&](const AttendArgs &l, const Pieces &p) {
         const int rows = l.tile.rows, last = (int)l.segment_slots + l.tile.workgroups;
@@ -961,50 +1017,66 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
         // (Of rows that no request has, where starts do not ascend, this is what the workspace happened to hold.)
         if (p.slot < 0 || p.slot >= last || p.workgroup < 0 || p.count < 1 || p.count > l.tile.workgroups - p.workgroup || p.at < 0 || p.at >= rows) return;
         auto slot = [&](int j) { return l.slots + (j == 0 ? p.slot : l.segment_slots + p.workgroup + j) * size; };
-        for (int base = 0; base < p.count; base += 64) {
-            const int j = base + lane, here = min(64, p.count - base);
+        for (int base = 0; base < p.count; base += LANES) {
+            const int j = base + lane, here = min(LANES, p.count - base);
             float most = kLowest, sum = 0.0f;
             if (j < p.count) {
                 const float *at = slot(j) + (int64_t)rows * D + p.at;
                 most = at[0], sum = at[rows];
             }
-            float now = __builtin_fmaxf(top, most);
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) now = __builtin_fmaxf(now, __shfl_xor(now, m));
-            const float keep = __builtin_amdgcn_exp2f(top - now), weight = __builtin_amdgcn_exp2f(most - now);
-            top = now;
-            sum *= weight;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-            total = total * keep + sum;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= keep;
-            for (int first = 0; first < here; first += BATCH) {
-                float part[BATCH][E];
+            float part[BATCH][E];
+            auto load = [&](int first) {
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
                     const float *at = slot(base + min(first + k, here - 1)) + (int64_t)p.at * D + lane * E;
                     if constexpr (E == 1) {
                         part[k][0] = *at;
                     } else {
-                        const Sums v = *reinterpret_cast<const Sums *>(at);
+                        constexpr int RUN = E < 4 ? E : 4;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) part[k][e] = v[e];
+                        for (int e = 0; e < E; e += RUN) {
+                            const Sums v = *reinterpret_cast<const Sums *>(at + e);
+#pragma unroll
+                            for (int f = 0; f < RUN; ++f) part[k][e + f] = v[f];
+                        }
                     }
                 }
+            };
+            float now = __builtin_fmaxf(top, most);
+#pragma unroll
+            for (int m = 1; m < LANES; m <<= 1) now = __builtin_fmaxf(now, __shfl_xor(now, m));
+            const float keep = __builtin_amdgcn_exp2f(top - now), weight = __builtin_amdgcn_exp2f(most - now);
+            top = now;
+            sum *= weight;
+#pragma unroll
+            for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor(sum, m);
+            total = total * keep + sum;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= keep;
+            for (int first = 0; first < here; first += BATCH) {
+                load(first);
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
-                    const float w = __shfl(weight, (first + k) & 63);
+                    const float w = __shfl(weight, (first + k) % LANES, LANES);
 #pragma unroll
                     for (int e = 0; e < E; ++e) o[e] = first + k < here ? o[e] + w * part[k][e] : o[e];
                 }
             }
         }
     };
-    if (own.partial) join(prefix, prefix.pieces[vector]);
+    if (own.partial) join(prefix, theirs);
     join(own, mine);
     uint16_t *at = own.out + row * own.ld_out + (int64_t)h * D + lane * E;
     const float inv = 1.0f / total;
+    if constexpr (E >= 4) {
+        if (own.wide_out) {
+#pragma unroll
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<u32x2 *>(at + e) = total == 0.0f ? u32x2{} : u32x2{f32x2_to_bf16x2(o[e] * inv, o[e + 1] * inv),
+                                                                                    f32x2_to_bf16x2(o[e + 2] * inv, o[e + 3] * inv)};
+            return;
+        }
+    }
 #pragma unroll
     for (int e = 0; e < E; ++e) at[e] = total == 0.0f ? 0 : f32_to_bf16(o[e] * inv);
 }
@@ -1025,7 +1097,7 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     p.few = vectors <= 64;
     const int nt = (int)((vectors + 15) / 16);
     const int keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
-    p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, kExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
+    p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, p.few ? kFewExtra : kManyExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
     p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
     return p;
 }
@@ -1105,9 +1177,10 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
         constexpr int D = decltype(dim)::value;
         if (shared > 0) launch_part<D>(prefix, b, cv, pv, stream);
         launch_part<D>(own, a, cv, pv, stream);
-        // (Few vectors: a workgroup each, so that they spread over the CUs.)
-        const int waves = rows * q_heads <= 4096 ? 1 : 4;
-        join_kernel<D><<<(unsigned)((rows * q_heads + waves - 1) / waves), 64 * waves, 0, stream>>>(a, b, pv);
+        if (rows * q_heads <= kJoinApart)  // a workgroup each, so that they spread over the CUs
+            join_kernel<D, 64><<<(unsigned)(rows * q_heads), 64, 0, stream>>>(a, b, pv);
+        else
+            join_kernel<D, 16><<<(unsigned)((rows * q_heads + 15) / 16), 256, 0, stream>>>(a, b, pv);
     };
     if (cache.dim == 256) run(std::integral_constant<int, 256>{});
     else if (cache.dim == 128) run(std::integral_constant<int, 128>{});
