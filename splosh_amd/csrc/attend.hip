@@ -12,10 +12,10 @@
 // weights are, as they are, its operand of the second product (values' dimensions by queries), whose order of keys is
 // free as long as both operands have the same. Nothing but sums over the lanes of a query crosses lanes.
 //
-// Two kernels share the work out as attend_plan.hpp says. `few` (up to 64 vectors of a request and key/value head): bound by the
-// cache's bytes. Each of a workgroup's four waves goes through blocks of 32 keys of its own for all vectors, straight
-// from memory to registers; they are joined at the end. `many`: bound by the matrix instructions. Eight waves hold 32
-// vectors each, and go together through blocks that are widened to fp16 once, in LDS.
+// Two kernels share the work out as attend_plan.hpp says. `few` (up to 48 or 64 vectors of a request and key/value head): bound
+// by the cache's bytes. Each of a workgroup's four waves goes through blocks of 32 keys of its own for all vectors, each block on
+// its way into LDS while the one before is multiplied; the waves are joined at the end. `many`: bound by the matrix instructions
+// and what feeds them. Eight waves hold 32 vectors each, and go together through blocks that are widened to fp16 once, in LDS.
 #include <climits>
 #include <mutex>
 #include <type_traits>
@@ -135,9 +135,6 @@ __device__ __forceinline__ u32x4 moved8(const u32x4 &v, int power) {
 
 // A value that all lanes of the wave have, as a scalar.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
-}
 __device__ __forceinline__ Span uniform(const Span &s) {
     return {uniform(s.begin), uniform(s.n), uniform(s.first), uniform(s.from), uniform(s.to)};
 }
@@ -549,12 +546,12 @@ struct FewRing {
     }
 };
 
-// (A wave a record; four would leave no room for the queries of four tiles of 256 dimensions. Where a wave's sums take more than
-// 96 registers it has its SIMD for itself, and they lie in accumulation registers.)
+// (A wave a record. Where a wave's sums take more than 96 registers it has its SIMD for itself, and they lie in accumulation registers.)
+constexpr int kFewGroups = 4;
 template <int D, int NT>
 struct FewShape {
     static constexpr bool kAlone = D / 16 * NT * 4 > 96;
-    static constexpr int kGroups = D == 256 && NT == 4 ? 3 : 4, kThreads = 64 * kGroups, kRows = 16 * NT, kPitch = D + 4;
+    static constexpr int kGroups = kFewGroups, kThreads = 64 * kGroups, kRows = 16 * NT, kPitch = D + 4;
     static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kQueryBytes = kRows * D * 2;
     static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions
     static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
@@ -1090,13 +1087,14 @@ struct AttendPlan {
     size_t slot_bytes() const { return (size_t)((segment_slots + tile.workgroups) * tile.rows); }  // times (dim + 2) floats
 };
 
-// `vectors`: those of a request and key/value head, on average.
+// `vectors`: those of a request and key/value head, on average. (Few and many, eight requests of 8192 tokens with 24 heads on 4, us, at 18, 30,
+// 48 and 60 vectors: 256 dimensions 46, 47, 63 and 200, where a wave's sums no longer fit into its registers, against 101 at each of them;
+// 128 dimensions 28, 29, 37 and 60 against 66 to 68; 64 dimensions 22, 22, 27 and 31 against 53.)
 static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, int64_t q_heads, const splosh_cache &cache) {
     AttendPlan p;
     const int cus = device_cus();
-    p.few = vectors <= 64;
-    const int nt = (int)((vectors + 15) / 16);
-    const int keys = !p.few ? kManyKeys : (cache.dim == 256 && nt == 4 ? FewShape<256, 4>::kGroups : FewShape<64, 1>::kGroups) * kBlock;
+    p.few = vectors <= (cache.dim == 256 ? 48 : 64);
+    const int nt = (int)((vectors + 15) / 16), keys = p.few ? kFewGroups * kBlock : kManyKeys;
     p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, p.few ? kFewExtra : kManyExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
     p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
     return p;
@@ -1145,7 +1143,7 @@ static void launch_part(const AttendPlan &plan, const AttendArgs &a, const Cache
     else if (plan.tile.rows == 16) few(std::integral_constant<int, 1>{});
     else if (plan.tile.rows == 32) few(std::integral_constant<int, 2>{});
     else if (plan.tile.rows == 48) few(std::integral_constant<int, 3>{});
-    else few(std::integral_constant<int, 4>{});
+    else if constexpr (D < 256) few(std::integral_constant<int, 4>{});
 }
 
 hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,

@@ -13,7 +13,7 @@
 //   finish (requests)                    the strip that the draw falls into, and the token in it.
 #include <climits>
 
-#include "common.hpp"
+#include "cache.hpp"
 #include "launch.hpp"
 
 namespace splosh {
@@ -134,18 +134,6 @@ __device__ __forceinline__ void weights_of(const float (&v)[N / 4][4], float mos
 __device__ __forceinline__ float entry(const float *p) { return *p; }
 __device__ __forceinline__ float entry(const uint16_t *p) { return bf16_bits_to_f32(*p); }
 
-// The request of row `row`, -1: none.
-__device__ __forceinline__ int row_request(const int32_t *starts, int requests, int row) {
-    const int lane = threadIdx.x & 63;
-    int count = 0;
-    for (int base = 0; base <= requests; base += 64) {
-        const int i = base + lane, n = __popcll(__ballot(i <= requests && starts[i] <= row));
-        count += n;
-        if (n < 64) break;
-    }
-    return count - 1 < requests ? count - 1 : -1;
-}
-
 // (v, i): the larger value, of equal ones the lower index. NaN is no value.
 __device__ __forceinline__ void keep_first(float &v, int &i, float w, int j) {
     if (w > v || (w == v && j < i)) v = w, i = j;
@@ -157,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
     __shared__ int wave_first[kWaves];
     __shared__ double wave_total[kWaves];
     const int row = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int r = row_request(a.starts, a.requests, row);
+    const int r = request_of(a.starts, a.requests, row);
     if (r < 0) return;
     const T *logits = (const T *)a.logits + row * a.ld;
     const int begin = piece * kPiece + wave * kStrip + lane * 4;  // its entries: four in a row, 256 further the next four
@@ -319,14 +307,15 @@ template <typename T>
 __global__ __launch_bounds__(64) void finish_kernel(VerifyArgs a) {
     const int r = blockIdx.x, lane = threadIdx.x;
     const Decision d = a.decisions[r];
-    if (d.row < 0) return;
     const StripSums *strips = a.strips + (int64_t)r * a.pieces * kWaves;
-    const int count = a.pieces * kWaves, drafted = d.last ? -1 : a.tokens[d.row + 1], run = (count + 63) / 64;
+    const int count = a.pieces * kWaves, run = (count + 63) / 64;
     const int low = min(lane * run, count), high = min(low + run, count);
-    const double u = uniform_of(a, min(a.starts[r + 1], a.rows) - 1);
+    const double u = uniform_of(a, max(min(a.starts[r + 1], a.rows) - 1, 0));
     double rest = 0.0, whole = 0.0;
 #pragma unroll 4
     for (int i = low; i < high; ++i) rest += strips[i].rest, whole += strips[i].whole;
+    if (d.row < 0) return;  // (no rows; the loads above do not wait for it)
+    const int drafted = d.last ? -1 : a.tokens[d.row + 1];
     const double rests = wave_running(rest), wholes = wave_running(whole);
     const bool from_rest = __shfl(rests, 63) > 0.0;
     const double total = from_rest ? __shfl(rests, 63) : __shfl(wholes, 63), draw = u * total;
