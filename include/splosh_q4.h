@@ -563,7 +563,7 @@ int splosh_rotate_heads(const splosh_heads *parts, int count, int dtype, int64_t
 /* A step's keys and values into the cache at their rows' places: keys as splosh_rotate_heads makes them
  * (by the rows' own positions) but not rounded to bf16, values as they are. v's weight and the `out` of both must be NULL.
  * q (NULL: none): the step's queries, to q->out as splosh_rotate_heads makes them, in the same launch. Two rows of one place
- * (requests that share a page they both write) leave one or the other's bytes there. */
+ * (requests that share a page they both write) leave some bytes of either there. */
 int splosh_cache_write(const splosh_cache *cache, const splosh_packed *packed, const splosh_heads *k,
                        const splosh_heads *v, const splosh_heads *q, int dtype, int64_t rows,
                        const float *frequencies, int64_t rotary, float eps, hipStream_t stream);
@@ -584,9 +584,11 @@ size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_pac
  * values, row stride ld_out. A row that sees no key gets zeros.
  * shared: the first `shared` tokens (a multiple of page_tokens, 0: none) are the same for all requests of the call: they
  * are read through the pages of request 0, once for all rows; the table's entries of other requests for
- * them are not used. Scores and sums are fp32, q's values enter the first product as they are, the weights the second one in fp16 (relative
- * to the largest, 2^-11). Nothing is added in an order that changes: the result depends on the step's
- * shape and on the device's count of CUs, and on no other call. The workspace need not be zeroed; its first
+ * them are not used. Scores and sums are fp32; q's values enter the first product in fp16 after a power of two that leaves them
+ * as they are (what is below 2^-28 of its vector's largest: to 2^-39 of that), the weights the second one rounded to
+ * fp16 (2^-11 of each). out may be q itself, with the same strides. Nothing is added in an order that changes: the result depends
+ * on the step's shape and on the device's count of CUs, and on no other call. SPLOSH_ERR_UNSUPPORTED where rows, heads and the
+ * table's tokens are so many that their pieces could pass 2^31. The workspace need not be zeroed; its first
  * 16 KiB stay as they are, so one that other calls use serves here too, in stream order. */
 int splosh_attend(const uint16_t *q, int64_t row_stride, int64_t head_stride, int64_t q_heads,
                   const splosh_cache *cache, const splosh_packed *packed, int64_t rows, int64_t shared, float scale,
@@ -615,7 +617,8 @@ size_t splosh_verify_workspace_bytes(int64_t rows, int64_t vocab, int64_t reques
  *   - u below 0 or NaN counts as 0; u >= 1: the last entry with weight. A drafted id that is negative or not below
  *     vocab is not accepted. A NaN q is not accepted and leaves no weight.
  *   - A request without rows has accepted 0; rows of `out` past starts[requests] are left as they were.
- * Weights and their sums are 64-bit floating point in a fixed order. vocab <= 2^21, rows and requests <= 65535.
+ * Weights are good to 1e-9 and added in 64 bits in an order that the shape alone gives, so the result is the same each time.
+ * `out` and `accepted` must not overlap each other, `tokens` or `starts`. vocab <= 2^21, rows and requests <= 65535.
  * The workspace need not be zeroed; its first 16 KiB stay as they are. */
 int splosh_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const int32_t *tokens,
                   const int32_t *starts, int64_t requests, const float *uniforms, const float *temperature,

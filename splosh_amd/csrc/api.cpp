@@ -1463,7 +1463,10 @@ int splosh_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64
         !aligned(tokens, 4) || !aligned(starts, 4) || !aligned(uniforms, 4) || !aligned(temperature, 4) || !aligned(out, 4) ||
         !aligned(accepted, 4))
         return fail(SPLOSH_ERR_UNSUPPORTED, "operands are not aligned to their elements");
-    if (out == tokens || accepted == out) return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "outputs must not overlap the tokens");
+    auto overlap = [](const int32_t *a, int64_t n, const int32_t *b, int64_t m) { return a < b + m && b < a + n; };
+    if (overlap(out, rows, accepted, requests) || overlap(out, rows, tokens, rows) || overlap(out, rows, starts, requests + 1) ||
+        overlap(accepted, requests, tokens, rows) || overlap(accepted, requests, starts, requests + 1))
+        return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "outputs must not overlap each other, tokens or starts");
     const size_t need = splosh::verify_workspace_bytes(rows, vocab, requests);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(SPLOSH_ERR_WORKSPACE_TOO_SMALL,

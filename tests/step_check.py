@@ -45,8 +45,9 @@ def places(starts, lengths, table, page, pages, rows):
 def rotated(x, weight, frequencies, positions, eps):
     """(y, bound): the norm and the rotation in 64 bits, and what fp32 and one rounding to bf16 may leave of it.
 
-    fp32: the mean of squares, its root and the products are off by (dim / 64 + 16) 2^-24 at most (a lane adds dim / 64
-    squares, six additions across the wave); an angle's fraction, cosine and sine by 2^-22 of the pair."""
+    fp32: the mean of squares is off by (dim / 16 + 5) 2^-24 at most (a lane adds dim / 16 squares, four additions across a
+    vector's lanes), of which the root leaves half, and the root, the quotient and the products by six more: below (dim / 64 + 16) 2^-24
+    in all; an angle's fraction, cosine and sine by 2^-22 of the pair."""
     y = x.double()
     dim = y.shape[-1]
     off = torch.zeros_like(y)

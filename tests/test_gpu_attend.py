@@ -70,10 +70,10 @@ class Step:
 
 @pytest.mark.parametrize("runs,lengths,q_heads,heads,dim,page", [
     ([1], [1], 1, 1, 64, 32), ([1], [31], 4, 2, 128, 32), ([1], [33], 24, 4, 256, 64), ([1], [700], 6, 1, 256, 96),
-    ([1] * 5, [1, 32, 64, 65, 500], 8, 2, 128, 32), ([8] * 4, [8, 40, 129, 1000], 12, 2, 256, 256), ([3, 0, 7, 1], [10, 77, 7, 333], 10, 2, 128, 96),
+    ([1] * 5, [1, 32, 64, 65, 500], 8, 2, 128, 32), ([8] * 4, [8, 40, 129, 1000], 10, 2, 256, 256), ([11] * 3, [300, 40, 11], 5, 1, 256, 64), ([3, 0, 7, 1], [10, 77, 7, 333], 10, 2, 128, 96),
     ([5], [5], 7, 7, 64, 32), ([2, 9], [300, 41], 32, 1, 64, 64), ([40], [40], 6, 1, 256, 64), ([100, 3], [150, 9], 5, 1, 128, 32),
     ([333], [400], 8, 2, 64, 64), ([300], [1000], 6, 1, 256, 256), ([64, 64, 64], [64, 200, 65], 4, 4, 128, 32),
-    ([700, 1, 2], [700, 2000, 2], 4, 1, 128, 96), ([513], [513], 3, 3, 256, 32)])
+    ([700, 1, 2], [700, 2000, 2], 4, 1, 128, 96), ([513], [513], 3, 3, 256, 32), ([1] * 300, [1 + 7 * i % 190 for i in range(300)], 4, 2, 64, 32)])
 def test_attend(rt, runs, lengths, q_heads, heads, dim, page):
     s = Step(rt, runs, lengths, q_heads, heads, dim, page, seed=len(runs) + dim, more=2, layout="gated" if dim == 128 else "dense", pad=3)
     s.check(s.run())
@@ -220,3 +220,12 @@ def test_far_pages(rt):
         some = torch.arange(n - rows, n)
         out, off = attended(q[-rows:], kc * ks, vc * vs, some, dim ** -0.5)
         check_bf16(got, out, off)
+
+
+def test_in_place(rt):
+    """The output in its queries' place: written by one piece, joined from several, and with a shared prefix."""
+    for runs, lengths, shared in (([2, 5], [900, 30], 0), ([300], [900], 0), ([4, 4], [140, 200], 128)):
+        s = Step(rt, runs, lengths, 6, 2, 128, 32, seed=14, shared=shared)
+        want = s.run()
+        got = rt.attend(s.q_gpu, s.cache, s.packed, shared=shared, out=s.q_gpu)
+        assert got.data_ptr() == s.q_gpu.data_ptr() and torch.equal(got, want)

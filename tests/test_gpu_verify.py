@@ -62,7 +62,7 @@ def verified(logits, tokens, u, temperature, draft):
 
 
 def check(rt, logits, tokens, runs, u, temperature, draft, more=0, **kw):
-    """Every request's result; decisions that lie within 1e-12 are left out (there are none in these inputs)."""
+    """Every request's result; weights are good to 1e-9, and no decision in these inputs is within 4e-9 of the row's weight."""
     starts = torch.tensor([sum(runs[:r]) for r in range(len(runs) + 1)], dtype=torch.int32)
     out = torch.full((len(tokens),), 77, dtype=torch.int32, device="cuda")
     cuda = lambda t: t.cuda() if t is not None else None  # noqa: E731
@@ -77,7 +77,7 @@ def check(rt, logits, tokens, runs, u, temperature, draft, more=0, **kw):
             continue
         want, count, margin = verified(host[s : s + n], tokens[s : s + n], u[s : s + n].tolist(),
                                        1.0 if temperature is None else float(temperature[r]), hd[s : s + n] if hd is not None else None)
-        assert margin > 1e-12, "inputs on a border"
+        assert margin > 4e-9, "inputs on a border"
         assert got[s : s + n] == want and accepted[r] == count, (r, got[s : s + n], want)
     assert got[sum(runs):] == [77] * (len(tokens) - sum(runs))
 

@@ -125,7 +125,8 @@ def test_rotation(change, case):
     ({"requests": 0}, "invalidShape"), ({"ld": 999}, "invalidRowStride"), ({"ldd": 999}, "invalidRowStride"), ({"dtype": 4}, "unsupported"),
     ({"ddtype": 4}, "unsupported"), ({"vocab": (1 << 21) + 1, "ld": 1 << 22, "ldd": 1 << 22}, "unsupported"), ({"rows": 65536}, "unsupported"),
     ({"requests": 65536}, "unsupported"), ({"ld": 1 << 62}, "arithmeticOverflow"), ({"logits": ODD}, "unsupported"), ({"out": ODD}, "unsupported"),
-    ({"out": P[2]}, "layoutMismatch"), ({"accepted": P[5]}, "layoutMismatch"), ({"ws": None}, "workspaceTooSmall"), ({"ws_bytes": 16400}, "workspaceTooSmall")])
+    ({"out": P[2]}, "layoutMismatch"), ({"accepted": P[5]}, "layoutMismatch"), ({"out": ctypes.c_void_p(0x30000 - 4 * 7)}, "layoutMismatch"),
+    ({"out": ctypes.c_void_p(0x30000 + 4 * 7)}, "layoutMismatch"), ({"accepted": ctypes.c_void_p(0x40000 + 4 * 2)}, "layoutMismatch"), ({"ws": None}, "workspaceTooSmall"), ({"ws_bytes": 16400}, "workspaceTooSmall")])
 def test_verification(change, case):
     a = dict(logits=P[0], ld=1000, dtype=_lib.F32, rows=8, vocab=1000, tokens=P[2], starts=P[3], requests=2, u=P[4], t=P[7], draft=P[1], ldd=1000,
              ddtype=_lib.F32, out=P[5], accepted=P[6], ws=P[8], ws_bytes=1 << 30)
