@@ -348,14 +348,16 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         const int units = tile_units(span, tile, t), take = min(units - offset, end - unit);
         const int keys = tile_end(span, tile, t) - span.from, blocks = keys > 0 ? (keys + kBlock - 1) / kBlock : 0;
         const int per = tile.keys / kBlock;
+        const bool first = offset <= tile.extra;  // (who has nothing but units before the keys leaves the segment to the next one)
         Piece p;
         p.span = span, p.request = request, p.head = head, p.tile = t;
         p.first_block = max(0, offset - tile.extra) * per;
         p.blocks = max(0, min((offset + take - tile.extra) * per, blocks) - p.first_block);
-        p.slot = offset == 0 ? segment : (int)a.segment_slots + w;
-        p.count = offset > 0 ? 0 : take == units ? 1 : owner_of(total, sharers, unit + units - 1) - w + 1;
-        p.direct = !a.partial && take == units;
-        if (segment < a.segment_slots) work(p);  // (more there are only where starts do not ascend)
+        p.slot = first ? segment : (int)a.segment_slots + w;
+        p.count = !first ? 0 : offset + take == units ? 1 : owner_of(total, sharers, unit + units - offset - 1) - w + 1;
+        p.direct = !a.partial && first && offset + take == units;
+        // (More segments than slots there are only where starts do not ascend.)
+        if (offset + take > tile.extra && segment < a.segment_slots) work(p);
         unit += take;
         if (unit >= end) return;
         offset = 0, ++segment;
