@@ -734,18 +734,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
 
 // ---- many vectors -------------------------------------------------------------------------------
 
-// N products' operands read from LDS four ahead of them.
-template <int N>
-__device__ __forceinline__ void interleave() {
-    constexpr int AHEAD = N < 4 ? N : 4;
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-    for (int i = 0; i < N - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-}
+constexpr int kWidenValues = 1, kWidenKeys = 2;  // what a wave widens
 
 template <int D>
 struct ManyShape {
@@ -761,6 +750,9 @@ template <int D>
 __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheView cache, PackedView packed) {
     constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = ManyShape<D>::kPitch;
     constexpr int K_ITEMS = 2 * D / 256 > 0 ? 2 * D / 256 : 1;
+    // Operands are read from LDS this many products ahead of their own, and the order is kept: left to the compiler's scheduler, each was
+    // read right before its product, and half of a step went by waiting for LDS.
+    constexpr int KEYS_AHEAD = 4;
     typedef ManyShape<D> S;
     extern __shared__ __align__(16) char lds[];  // two records as they are, then three of keys, four of values and of scales as they are used
     uint8_t *const key_parts = reinterpret_cast<uint8_t *>(lds + S::kKeys);
@@ -800,13 +792,19 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         Pages pages(packed, a.prefix ? 0 : p.request);
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
 
-        // A record goes straight into LDS three steps before it is multiplied, and is widened to fp16 two steps before. Waves 0 to 3 do that
-        // with the values (a thread four dimensions of eight of them) and the scales, waves 4 to 7 with the keys (16-byte runs).
+        // A record goes straight into LDS three steps before it is multiplied, and is widened to fp16 two steps before. The first waves do that
+        // with the values (a thread four dimensions of eight of them) and the scales, waves from the fourth on with the keys (16-byte runs).
         bool hole = false;
+        int left = 0;  // records of the page behind `next`, itself included
+        const uint8_t *next = nullptr;
         auto fetch = [&](int block, int buffer) {
             const int lane = lane_anew();
-            const uint8_t *record = block_record<D>(a, cache, pages, p.head, block, hole);
-            const rsrc_t r = make_rsrc(record, record_bytes(D));
+            if (left == 0) {
+                next = block_record<D>(a, cache, pages, p.head, block, hole);
+                left = cache.page_blocks - (block - a.by_blocks.of(block) * cache.page_blocks);
+            }
+            const rsrc_t r = make_rsrc(next, record_bytes(D));
+            next += record_bytes(D), --left;
             const int part = (wave < 4 ? kBlock * D : 0) + (wave & 3) * (kBlock * D / 4), at = buffer * record_bytes(D) + part;
             if constexpr (D == 64) {
 #pragma unroll
@@ -819,55 +817,100 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             if (wave < 4) buffer_load_lds4(r, lds + buffer * record_bytes(D) + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto stage = [&](int buffer, int third, int fourth) {  // the record's place among two, three and four
+
+        // The wave's part of the record in `buffer` widened to place `third` of the keys or `fourth` of the values and scales, and between that
+        // (MULTIPLY) the scores of the keys at place `keys`: the products run while the codes are widened. One after the other, the two
+        // took 1800 cycles of a step's 5200; the values of a step of 256 dimensions are 1440.
+        f32x16 s;
+        auto widen_and_score = [&](auto role, auto multiply, int buffer, int third, int fourth, int keys) {
+            constexpr int ROLE = decltype(role)::value, PIECES = ROLE == kWidenValues ? 4 : ROLE == kWidenKeys ? 2 * K_ITEMS : 0;
+            constexpr bool MULTIPLY = decltype(multiply)::value;
             const char *const raw = lds + buffer * record_bytes(D);
-            const int tid = wave * 64 + lane_anew();
+            const int lane = lane_anew(), tid = wave * 64 + lane;
             const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
-            if (tid < D) {
-                uint32_t v[8];
+            uint32_t v[8];
+            u32x4 run[K_ITEMS];
+            float scale = 0.0f;
+            if constexpr (ROLE == kWidenValues) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     v[e] = *reinterpret_cast<const uint32_t *>(raw + (kBlock + 16 * value_step + (e / 4) * 8 + 4 * value_g + e % 4) * D + quad * 4);
-                f16x8 part[4];
-                widen_turned(v, part);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int t = D == 64 ? c >> 1 : quad / 32 * 4 + c, m = D == 64 ? (c & 1) * 16 + quad : quad % 32;
-                    value_parts[(fourth * TILES * 2 + t * 2 + value_step) * 64 + value_g * 32 + m] = __builtin_bit_cast(u32x4, part[c]);
-                }
+                scale = reinterpret_cast<const float *>(raw + 2 * kBlock * D)[lane];
             }
-            if (tid >= 256) {
+            if constexpr (ROLE == kWidenKeys) {
 #pragma unroll
                 for (int n = 0; n < K_ITEMS; ++n) {
                     const int item = tid - 256 + 256 * n;
-                    if (item < 2 * D) {
-                        const int run = item / 128 * 4 + item % 4, token = item / 4 % 32;
-                        const u32x4 k = *reinterpret_cast<const u32x4 *>(raw + token * D + run * 16);
-                        uint8_t *at = key_parts + (third * STEPS + run) * K_PITCH + token * 16;
-                        *reinterpret_cast<f16x8 *>(at) = widen8(k[0], k[1]);
-                        *reinterpret_cast<f16x8 *>(at + 512) = widen8(k[2], k[3]);
-                    }
+                    run[n] = *reinterpret_cast<const u32x4 *>(raw + item / 4 % 32 * D + (item / 128 * 4 + item % 4) * 16);
                 }
             }
-            if (tid < 2 * kBlock) {
-                const float scale = reinterpret_cast<const float *>(raw + 2 * kBlock * D)[tid];
-                float *at = scales + fourth * 3 * kBlock;
-                if (tid < kBlock) at[tid] = scale;
-                else at[tid] = __builtin_amdgcn_logf(scale), at[tid + kBlock] = inverse_scale(scale);
+            auto turn = [&] {  // pairs of tokens: v[2p] and v[2p + 1] to their bytes 0, 1 and 2, 3
+                if constexpr (ROLE == kWidenValues) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        const uint32_t low = perm_bytes(v[2 * p + 1], v[2 * p], 0x05040100u), high = perm_bytes(v[2 * p + 1], v[2 * p], 0x07060302u);
+                        v[2 * p] = low, v[2 * p + 1] = high;
+                    }
+                }
+            };
+            auto piece = [&](int c) {
+                if constexpr (ROLE == kWidenValues) {
+                    f16x2 of[4];
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) of[p] = centred(perm_bytes(0x64646464u, v[2 * p + c / 2], c % 2 ? 0x04030401u : 0x04020400u));
+                    const int t = D == 64 ? c >> 1 : quad / 32 * 4 + c, m = D == 64 ? (c & 1) * 16 + quad : quad % 32;
+                    value_parts[(fourth * TILES * 2 + t * 2 + value_step) * 64 + value_g * 32 + m] =
+                        __builtin_bit_cast(u32x4, join8(of[0], of[1], of[2], of[3]));
+                }
+                if constexpr (ROLE == kWidenKeys) {
+                    const int item = tid - 256 + 256 * (c / 2), half = c % 2;
+                    uint8_t *const to = key_parts + (third * STEPS + item / 128 * 4 + item % 4) * K_PITCH + item / 4 % 32 * 16;
+                    *reinterpret_cast<f16x8 *>(to + 512 * half) = widen8(run[c / 2][2 * half], run[c / 2][2 * half + 1]);
+                }
+            };
+            if constexpr (MULTIPLY) {
+                const uint8_t *const at = key_parts + keys * STEPS * K_PITCH + lane * 16;
+                auto key = [&](int i) { return *reinterpret_cast<const f16x8 *>(at + i * K_PITCH); };
+                f16x8 k[KEYS_AHEAD];
+#pragma unroll
+                for (int i = 0; i < KEYS_AHEAD; ++i) k[i] = key(i);
+                s = f32x16{};
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % KEYS_AHEAD], q[i], s, 0, 0, 0);
+                    if (i + KEYS_AHEAD < STEPS) k[i % KEYS_AHEAD] = key(i + KEYS_AHEAD);
+                    if (i == STEPS / 4) turn();
+#pragma unroll
+                    for (int c = 0; c < PIECES; ++c)
+                        if (i == STEPS / 4 + 1 + c * (STEPS * 3 / 4 - 1) / PIECES) piece(c);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                turn();
+#pragma unroll
+                for (int c = 0; c < PIECES; ++c) piece(c);
             }
+            if constexpr (ROLE == kWidenValues) {
+                if (wave == 0) {
+                    float *const to = scales + fourth * 3 * kBlock + lane;
+                    to[0] = lane < kBlock ? scale : __builtin_amdgcn_logf(scale);
+                    if (lane >= kBlock) to[kBlock] = inverse_scale(scale);
+                }
+            }
+        };
+        auto part_of_step = [&](auto multiply, int buffer, int third, int fourth, int keys) {
+            if (wave < D / 64) widen_and_score(std::integral_constant<int, kWidenValues>{}, multiply, buffer, third, fourth, keys);
+            else if (wave >= 4 && wave < 4 + 2 * D / 64 / K_ITEMS)
+                widen_and_score(std::integral_constant<int, kWidenKeys>{}, multiply, buffer, third, fourth, keys);
+            else widen_and_score(std::integral_constant<int, 0>{}, multiply, buffer, third, fourth, keys);
         };
 
-        f32x16 s;
-        auto score = [&](int third) {
-            s = f32x16{};
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const f16x8 k = *reinterpret_cast<const f16x8 *>(key_parts + (third * STEPS + i) * K_PITCH + lane * 16);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], s, 0, 0, 0);
-            }
-            interleave<STEPS>();
-        };
         auto weigh_values = [&](int block, int fourth, bool dead) {
+            const int lane = lane_anew(), g = lane >> 5;
+            auto value = [&](int n) {  // tile n % TILES, keys 16 (n / TILES) on
+                return __builtin_bit_cast(f16x8, value_parts[(fourth * TILES * 2 + n % TILES * 2 + n / TILES) * 64 + lane]);
+            };
             const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
             const float *const at = scales + fourth * 3 * kBlock + 4 * g;
             float t[16], top = -__builtin_inff();
@@ -893,26 +936,44 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) acc[j] *= keep;
             }
+            // Half of the weights, and the other half between the products with the first.
+            f32x4 inverse[4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                u32x4 pairs;
+            for (int b = 0; b < 4; ++b) inverse[b] = *reinterpret_cast<const f32x4 *>(at + 2 * kBlock + 8 * b);
+            float w[16];
+            auto weigh = [&](int e) {
+                w[e] = __builtin_amdgcn_exp2f(t[e] - most);
+                total = __builtin_fmaf(w[e], inverse[e / 4][e % 4], total);
+            };
+            u32x4 pairs;
+            auto pack = [&](int half) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const f32x4 inverse = *reinterpret_cast<const f32x4 *>(at + 2 * kBlock + 16 * i + 8 * b);
-                    float w[4];
+                for (int e = 0; e < 4; ++e) pairs[e] = f16_pair(w[8 * half + 2 * e], w[8 * half + 2 * e + 1]);
+            };
+            f16x8 v[2 * TILES];
+            // (How many are read once product n is begun: with 256 dimensions there is room for two ahead until weights are done with.)
+            auto read = [](int n) {
+                const int ahead = D < 256 ? 4 : n < TILES ? 2 : 4;
+                return n + 1 + ahead < 2 * TILES ? n + 1 + ahead : 2 * TILES;
+            };
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        w[e] = __builtin_amdgcn_exp2f(t[8 * i + 4 * b + e] - most);
-                        total = __builtin_fmaf(w[e], inverse[e], total);
-                    }
-                    pairs[2 * b] = f16_pair(w[0], w[1]), pairs[2 * b + 1] = f16_pair(w[2], w[3]);
-                }
+            for (int n = 0; n < read(-1); ++n) v[n] = value(n);
 #pragma unroll
-                for (int j = 0; j < TILES; ++j) {
-                    const f16x8 v = __builtin_bit_cast(f16x8, value_parts[(fourth * TILES * 2 + j * 2 + i) * 64 + lane]);
-                    acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pairs), acc[j], 0, 0, 0);
+            for (int e = 0; e < 8; ++e) weigh(e);
+            pack(0);
+#pragma unroll
+            for (int n = 0; n < 2 * TILES; ++n) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (n == TILES) pack(1);
+                acc[n % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[n], __builtin_bit_cast(f16x8, pairs), acc[n % TILES], 0, 0, 0);
+#pragma unroll
+                for (int m = read(n - 1); m < read(n); ++m) v[m] = value(m);
+                if (n < TILES) {
+#pragma unroll
+                    for (int e = 8 + 8 * n / TILES; e < 8 + 8 * (n + 1) / TILES; ++e) weigh(e);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         };
 
         bool dead[4] = {};  // of the step's record and of the next ones
@@ -924,7 +985,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         lds_barrier();
 #pragma unroll
         for (int n = 0; n < 2; ++n)
-            if (from + n < to) stage(n, n, n);
+            if (from + n < to) part_of_step(std::false_type{}, n, n, n, 0);
         lds_barrier();
         if (from + 2 < to) fetch(from + 2, 0), dead[2] = hole;
         wait_vmcnt<0>();
@@ -938,8 +999,8 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             const int step = block - from;
             if (block + 3 < to) fetch(block + 3, (step + 1) & 1);
             dead[3] = hole;
-            if (block + 2 < to) stage(step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3);
-            score(third);
+            // (Behind the last records something that nothing reads is widened once more.)
+            part_of_step(std::true_type{}, step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3, third);
             lds_barrier();
             weigh_values(block, step & 3, dead[0]);
 #pragma unroll
