@@ -751,7 +751,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
     constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = ManyShape<D>::kPitch;
     constexpr int K_ITEMS = 2 * D / 256 > 0 ? 2 * D / 256 : 1;
     // Operands are read from LDS this many products ahead of their own, and the order is kept: left to the compiler's scheduler, each was
-    // read right before its product, and half of a step went by waiting for LDS.
+    // read right before its product, and half of a step went by waiting (prompt chunk 462 us instead of 437).
     constexpr int KEYS_AHEAD = 4;
     typedef ManyShape<D> S;
     extern __shared__ __align__(16) char lds[];  // two records as they are, then three of keys, four of values and of scales as they are used
@@ -819,8 +819,8 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         };
 
         // The wave's part of the record in `buffer` widened to place `third` of the keys or `fourth` of the values and scales, and between that
-        // (MULTIPLY) the scores of the keys at place `keys`: the products run while the codes are widened. One after the other, the two
-        // took 1800 cycles of a step's 5200; the values of a step of 256 dimensions are 1440.
+        // (MULTIPLY) the scores of the keys at place `keys`: the products run while the codes are widened (one after the other, the prompt
+        // chunk took 437 us instead of 426).
         f32x16 s;
         auto widen_and_score = [&](auto role, auto multiply, int buffer, int third, int fourth, int keys) {
             constexpr int ROLE = decltype(role)::value, PIECES = ROLE == kWidenValues ? 4 : ROLE == kWidenKeys ? 2 * K_ITEMS : 0;
