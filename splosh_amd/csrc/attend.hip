@@ -31,7 +31,6 @@ constexpr size_t kAttendCounterBytes = 16384;  // the workspace's first bytes be
 constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
 constexpr int kManyThreads = 512, kManyRows = 256;
-constexpr int kManyKeys = 2 * kBlock;  // of a unit of the kernel for many vectors
 constexpr int64_t kJoinApart = 4096;  // (row, query head) vectors that are joined a wave each
 // Units that a segment costs beside its keys. (Few vectors: 3, where 1 is 119 instead of 116 us for the 64 requests of 512 MB, 108 instead of
 // 106 for the verify step; many: 1 to 6 are the same within 1 %.)
@@ -734,27 +733,27 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
 
 // ---- many vectors -------------------------------------------------------------------------------
 
-constexpr int kWidenValues = 1, kWidenKeys = 2;  // what a wave widens
-
 template <int D>
 struct ManyShape {
+    // Records of a step: what the eight waves widen and multiply in one is the same for every dim. (With one, a step of fewer dimensions
+    // is shorter than the way of its loads from memory: 2048 rows on 6144 with 24 heads on 4 took 272 us instead of 247 with 128
+    // dimensions, 204 instead of 180 with 64.)
+    static constexpr int kRecords = 256 / D;
     static constexpr int kPitch = 1024 + 64;  // of a step of keys: spreads a quad's writes over the banks
-    static constexpr int kLoads = D == 64 ? 2 : D / 128;  // of a wave, of its eighth of a record's codes
-    static constexpr int kKeys = 2 * record_bytes(D), kValues = kKeys + 3 * (D / 16) * kPitch, kScales = kValues + 4 * (D / 32) * 2048;
-    static constexpr int kThreads = kManyThreads, kLds = kScales + 4 * 3 * kBlock * 4;
+    static constexpr int kRaw = kRecords * record_bytes(D), kKeys = 2 * kRaw, kValues = kKeys + 3 * 16 * kPitch, kScales = kValues + 4 * 16 * 1024;
+    static constexpr int kThreads = kManyThreads, kLds = kScales + 4 * kRecords * 3 * kBlock * 4;
     static constexpr int kSumPitch = D + 4;
     static_assert(kLds <= 160 * 1024 && 8 * 16 * kSumPitch * 4 <= kLds, "LDS");
 };
 
 template <int D>
 __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheView cache, PackedView packed) {
-    constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = ManyShape<D>::kPitch;
-    constexpr int K_ITEMS = 2 * D / 256 > 0 ? 2 * D / 256 : 1;
+    constexpr int STEPS = D / 16, TILES = D / 32, K_PITCH = ManyShape<D>::kPitch, RECORDS = ManyShape<D>::kRecords;
     // Operands are read from LDS this many products ahead of their own, and the order is kept: left to the compiler's scheduler, each was
     // read right before its product, and half of a step went by waiting (prompt chunk 462 us instead of 437).
-    constexpr int KEYS_AHEAD = 4;
+    constexpr int KEYS_AHEAD = D == 256 ? 2 : 4;  // (256: more of them push queries out of the registers)
     typedef ManyShape<D> S;
-    extern __shared__ __align__(16) char lds[];  // two records as they are, then three of keys, four of values and of scales as they are used
+    extern __shared__ __align__(16) char lds[];  // two steps' records as they are, then three of keys, four of values and of scales as they are used
     uint8_t *const key_parts = reinterpret_cast<uint8_t *>(lds + S::kKeys);
     u32x4 *const value_parts = reinterpret_cast<u32x4 *>(lds + S::kValues);
     float *const scales = reinterpret_cast<float *>(lds + S::kScales);
@@ -792,60 +791,57 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         Pages pages(packed, a.prefix ? 0 : p.request);
         const int from = p.span.from / kBlock + p.first_block, to = from + p.blocks;
 
-        // A record goes straight into LDS three steps before it is multiplied, and is widened to fp16 two steps before. The first waves do that
-        // with the values (a thread four dimensions of eight of them) and the scales, waves from the fourth on with the keys (16-byte runs).
-        bool hole = false;
-        int left = 0;  // records of the page behind `next`, itself included
+        // A step's records go straight into LDS three steps before they are multiplied, and are widened to fp16 two steps before. Waves 0 to 3
+        // do that with the values (a thread four dimensions of eight of them) and the scales, waves 4 to 7 with the keys (16-byte runs).
+        const int quarter = wave & 3, record_at = quarter * RECORDS / 4;  // what the wave loads: 2 KiB of codes of this record of a step
+        bool none = false, hole = false;  // whether its page is none; whether its record is
+        int left = 0;                     // records of the page behind `next`, itself included
         const uint8_t *next = nullptr;
-        auto fetch = [&](int block, int buffer) {
-            const int lane = lane_anew();
-            if (left == 0) {
-                next = block_record<D>(a, cache, pages, p.head, block, hole);
+        auto fetch = [&](int first, int buffer) {
+            const int lane = lane_anew(), block = first + record_at;
+            hole = true;
+            if (block >= to) return;
+            if (left <= 0) {
+                next = block_record<D>(a, cache, pages, p.head, block, none);
                 left = cache.page_blocks - (block - a.by_blocks.of(block) * cache.page_blocks);
             }
+            hole = none;
             const rsrc_t r = make_rsrc(next, record_bytes(D));
-            next += record_bytes(D), --left;
-            const int part = (wave < 4 ? kBlock * D : 0) + (wave & 3) * (kBlock * D / 4), at = buffer * record_bytes(D) + part;
-            if constexpr (D == 64) {
+            next += RECORDS * record_bytes(D), left -= RECORDS;
+            const int part = (wave < 4 ? kBlock * D : 0) + quarter % (4 / RECORDS) * 2048;
+            char *const at = lds + (buffer * RECORDS + record_at) * record_bytes(D);
 #pragma unroll
-                for (int n = 0; n < S::kLoads; ++n) buffer_load_lds4(r, lds + at + n * 256, part + n * 256 + lane * 4);
-            } else {
-#pragma unroll
-                for (int n = 0; n < S::kLoads; ++n) buffer_load_lds16(r, lds + at + n * 1024, part + n * 1024 + lane * 16);
-            }
-            // (All four waves the same, so that they count the same loads.)
-            if (wave < 4) buffer_load_lds4(r, lds + buffer * record_bytes(D) + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
+            for (int n = 0; n < 2; ++n) buffer_load_lds16(r, at + part + n * 1024, part + n * 1024 + lane * 16);
+            if (wave < 4) buffer_load_lds4(r, at + 2 * kBlock * D, 2 * kBlock * D + lane * 4);
             __builtin_amdgcn_sched_barrier(0);
         };
 
-        // The wave's part of the record in `buffer` widened to place `third` of the keys or `fourth` of the values and scales, and between that
+        // The wave's part of the records in `buffer` widened to place `third` of the keys or `fourth` of the values and scales, and between that
         // (MULTIPLY) the scores of the keys at place `keys`: the products run while the codes are widened (one after the other, the prompt
-        // chunk took 437 us instead of 426).
-        f32x16 s;
-        auto widen_and_score = [&](auto role, auto multiply, int buffer, int third, int fourth, int keys) {
-            constexpr int ROLE = decltype(role)::value, PIECES = ROLE == kWidenValues ? 4 : ROLE == kWidenKeys ? 2 * K_ITEMS : 0;
-            constexpr bool MULTIPLY = decltype(multiply)::value;
-            const char *const raw = lds + buffer * record_bytes(D);
-            const int lane = lane_anew(), tid = wave * 64 + lane;
-            const int combo = tid / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
+        // chunk took 437 us instead of 426). `dead`: the record whose scales are the wave's is none.
+        f32x16 s[RECORDS];
+        auto widen_and_score = [&](auto values, auto multiply, int buffer, int third, int fourth, int keys, bool dead) {
+            constexpr bool VALUES = decltype(values)::value, MULTIPLY = decltype(multiply)::value;
+            const char *const raw = lds + buffer * S::kRaw;
+            const int lane = lane_anew(), tid = quarter * 64 + lane;
+            const int record = tid / D, combo = tid % D / (D / 4), quad = tid % (D / 4), value_step = combo >> 1, value_g = combo & 1;
             uint32_t v[8];
-            u32x4 run[K_ITEMS];
+            u32x4 run[2];
             float scale = 0.0f;
-            if constexpr (ROLE == kWidenValues) {
+            if constexpr (VALUES) {
+                const char *const at = raw + record * record_bytes(D) + (kBlock + 16 * value_step + 4 * value_g) * D + quad * 4;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    v[e] = *reinterpret_cast<const uint32_t *>(raw + (kBlock + 16 * value_step + (e / 4) * 8 + 4 * value_g + e % 4) * D + quad * 4);
-                scale = reinterpret_cast<const float *>(raw + 2 * kBlock * D)[lane];
-            }
-            if constexpr (ROLE == kWidenKeys) {
+                for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const uint32_t *>(at + (e / 4 * 8 + e % 4) * D);
+                scale = reinterpret_cast<const float *>(raw + record_at * record_bytes(D) + 2 * kBlock * D)[lane];
+            } else {
 #pragma unroll
-                for (int n = 0; n < K_ITEMS; ++n) {
-                    const int item = tid - 256 + 256 * n;
-                    run[n] = *reinterpret_cast<const u32x4 *>(raw + item / 4 % 32 * D + (item / 128 * 4 + item % 4) * 16);
+                for (int n = 0; n < 2; ++n) {
+                    const int all = tid + 256 * n, item = all % (2 * D);
+                    run[n] = *reinterpret_cast<const u32x4 *>(raw + all / (2 * D) * record_bytes(D) + item / 4 % 32 * D + (item / 128 * 4 + item % 4) * 16);
                 }
             }
             auto turn = [&] {  // pairs of tokens: v[2p] and v[2p + 1] to their bytes 0, 1 and 2, 3
-                if constexpr (ROLE == kWidenValues) {
+                if constexpr (VALUES) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const uint32_t low = perm_bytes(v[2 * p + 1], v[2 * p], 0x05040100u), high = perm_bytes(v[2 * p + 1], v[2 * p], 0x07060302u);
@@ -854,79 +850,85 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                 }
             };
             auto piece = [&](int c) {
-                if constexpr (ROLE == kWidenValues) {
+                if constexpr (VALUES) {
                     f16x2 of[4];
 #pragma unroll
                     for (int p = 0; p < 4; ++p) of[p] = centred(perm_bytes(0x64646464u, v[2 * p + c / 2], c % 2 ? 0x04030401u : 0x04020400u));
                     const int t = D == 64 ? c >> 1 : quad / 32 * 4 + c, m = D == 64 ? (c & 1) * 16 + quad : quad % 32;
-                    value_parts[(fourth * TILES * 2 + t * 2 + value_step) * 64 + value_g * 32 + m] =
+                    value_parts[(((fourth * RECORDS + record) * TILES + t) * 2 + value_step) * 64 + value_g * 32 + m] =
                         __builtin_bit_cast(u32x4, join8(of[0], of[1], of[2], of[3]));
-                }
-                if constexpr (ROLE == kWidenKeys) {
-                    const int item = tid - 256 + 256 * (c / 2), half = c % 2;
-                    uint8_t *const to = key_parts + (third * STEPS + item / 128 * 4 + item % 4) * K_PITCH + item / 4 % 32 * 16;
-                    *reinterpret_cast<f16x8 *>(to + 512 * half) = widen8(run[c / 2][2 * half], run[c / 2][2 * half + 1]);
+                } else {
+                    const int all = tid + 256 * (c / 2), item = all % (2 * D), half = c % 2;
+                    uint8_t *const at = key_parts + ((third * RECORDS + all / (2 * D)) * STEPS + item / 128 * 4 + item % 4) * K_PITCH + item / 4 % 32 * 16;
+                    *reinterpret_cast<f16x8 *>(at + 512 * half) = widen8(run[c / 2][2 * half], run[c / 2][2 * half + 1]);
                 }
             };
             if constexpr (MULTIPLY) {
-                const uint8_t *const at = key_parts + keys * STEPS * K_PITCH + lane * 16;
+                const uint8_t *const at = key_parts + keys * 16 * K_PITCH + lane * 16;
                 auto key = [&](int i) { return *reinterpret_cast<const f16x8 *>(at + i * K_PITCH); };
                 f16x8 k[KEYS_AHEAD];
 #pragma unroll
                 for (int i = 0; i < KEYS_AHEAD; ++i) k[i] = key(i);
-                s = f32x16{};
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
+                for (int r = 0; r < RECORDS; ++r) s[r] = f32x16{};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     __builtin_amdgcn_sched_barrier(0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % KEYS_AHEAD], q[i], s, 0, 0, 0);
-                    if (i + KEYS_AHEAD < STEPS) k[i % KEYS_AHEAD] = key(i + KEYS_AHEAD);
-                    if (i == STEPS / 4) turn();
-#pragma unroll
-                    for (int c = 0; c < PIECES; ++c)
-                        if (i == STEPS / 4 + 1 + c * (STEPS * 3 / 4 - 1) / PIECES) piece(c);
+                    s[i / STEPS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % KEYS_AHEAD], q[i % STEPS], s[i / STEPS], 0, 0, 0);
+                    if (i + KEYS_AHEAD < 16) k[i % KEYS_AHEAD] = key(i + KEYS_AHEAD);
+                    if (i == 4) turn();
+                    if (i == 5 || i == 7 || i == 10 || i == 13) piece(i / 3 - 1);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             } else {
                 turn();
 #pragma unroll
-                for (int c = 0; c < PIECES; ++c) piece(c);
+                for (int c = 0; c < 4; ++c) piece(c);
             }
-            if constexpr (ROLE == kWidenValues) {
-                if (wave == 0) {
-                    float *const to = scales + fourth * 3 * kBlock + lane;
-                    to[0] = lane < kBlock ? scale : __builtin_amdgcn_logf(scale);
-                    if (lane >= kBlock) to[kBlock] = inverse_scale(scale);
+            if constexpr (VALUES) {
+                // (A record that is none: its values' logarithms are -inf, which no kept scale has.)
+                if (quarter % (4 / RECORDS) == 0) {
+                    float *const at = scales + (fourth * RECORDS + record_at) * 3 * kBlock + lane;
+                    at[0] = lane < kBlock ? scale : dead ? -__builtin_inff() : __builtin_amdgcn_logf(scale);
+                    if (lane >= kBlock) at[kBlock] = inverse_scale(scale);
                 }
             }
         };
-        auto part_of_step = [&](auto multiply, int buffer, int third, int fourth, int keys) {
-            if (wave < D / 64) widen_and_score(std::integral_constant<int, kWidenValues>{}, multiply, buffer, third, fourth, keys);
-            else if (wave >= 4 && wave < 4 + 2 * D / 64 / K_ITEMS)
-                widen_and_score(std::integral_constant<int, kWidenKeys>{}, multiply, buffer, third, fourth, keys);
-            else widen_and_score(std::integral_constant<int, 0>{}, multiply, buffer, third, fourth, keys);
+        auto part_of_step = [&](auto multiply, int buffer, int third, int fourth, int keys, bool dead) {
+            if (wave < 4) widen_and_score(std::true_type{}, multiply, buffer, third, fourth, keys, dead);
+            else widen_and_score(std::false_type{}, multiply, buffer, third, fourth, keys, dead);
         };
 
-        auto weigh_values = [&](int block, int fourth, bool dead) {
+        auto weigh_values = [&](int block, int fourth) {
+            constexpr int KEYS = 16 * RECORDS, PRODUCTS = 2 * TILES * RECORDS, GROUPS = 2 * RECORDS;  // a lane's; groups of eight weights
             const int lane = lane_anew(), g = lane >> 5;
-            auto value = [&](int n) {  // tile n % TILES, keys 16 (n / TILES) on
-                return __builtin_bit_cast(f16x8, value_parts[(fourth * TILES * 2 + n % TILES * 2 + n / TILES) * 64 + lane]);
+            auto value = [&](int n) {  // group n / TILES, tile n % TILES
+                return __builtin_bit_cast(f16x8, value_parts[(((fourth * RECORDS + n / TILES / 2) * TILES + n % TILES) * 2 + n / TILES % 2) * 64 + lane]);
             };
-            const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
-            const float *const at = scales + fourth * 3 * kBlock + 4 * g;
-            float t[16], top = -__builtin_inff();
+            const float *const at = scales + fourth * RECORDS * 3 * kBlock + 4 * g;
+            bool masked = (block + RECORDS) * kBlock - 1 > first_position;
+            float t[KEYS], top = -__builtin_inff();
+            uint32_t seen = ~0u;  // a bit a record
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const f32x4 ks = *reinterpret_cast<const f32x4 *>(at + 8 * b), lv = *reinterpret_cast<const f32x4 *>(at + kBlock + 8 * b);
+            for (int r = 0; r < RECORDS; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[4 * b + e] = __builtin_fmaf(s[4 * b + e], ks[e] * factor, lv[e]);
-            }
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4 ks = *reinterpret_cast<const f32x4 *>(at + r * 3 * kBlock + 8 * b);
+                    const f32x4 lv = *reinterpret_cast<const f32x4 *>(at + r * 3 * kBlock + kBlock + 8 * b);
+                    if (b == 0) {
+                        const bool dead = uniform((int)__float_as_uint(lv[0])) == (int)0xff800000u;
+                        masked |= dead, seen &= dead ? ~(1u << r) : ~0u;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[16 * r + 4 * b + e] = __builtin_fmaf(s[r][4 * b + e], ks[e] * factor, lv[e]);
+                }
             if (masked) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    t[e] = !dead && block * kBlock + e / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
+                for (int e = 0; e < KEYS; ++e)
+                    t[e] = (seen >> e / 16 & 1) && (block + e / 16) * kBlock + e % 16 / 4 * 8 + 4 * g + e % 4 <= position ? t[e] : -__builtin_inff();
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, t[e]);
+            for (int e = 0; e < KEYS; ++e) top = __builtin_fmaxf(top, t[e]);
             top = max_halves(top);
             if (__any(top > most + kSlack)) {
                 top = __builtin_fmaxf(top, most);
@@ -936,75 +938,81 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) acc[j] *= keep;
             }
-            // Half of the weights, and the other half between the products with the first.
-            f32x4 inverse[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) inverse[b] = *reinterpret_cast<const f32x4 *>(at + 2 * kBlock + 8 * b);
-            float w[16];
-            auto weigh = [&](int e) {
-                w[e] = __builtin_amdgcn_exp2f(t[e] - most);
-                total = __builtin_fmaf(w[e], inverse[e / 4][e % 4], total);
+            // The first eight weights, and each next eight between the products with those before.
+            auto weigh = [&](int e, float inverse) {
+                t[e] = __builtin_amdgcn_exp2f(t[e] - most);
+                total = __builtin_fmaf(t[e], inverse, total);
             };
+            auto inverses = [&](int e) { return *reinterpret_cast<const f32x4 *>(at + e / 16 * 3 * kBlock + 2 * kBlock + e % 16 / 4 * 8); };
             u32x4 pairs;
-            auto pack = [&](int half) {
+            auto pack = [&](int group) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pairs[e] = f16_pair(w[8 * half + 2 * e], w[8 * half + 2 * e + 1]);
+                for (int e = 0; e < 4; ++e) pairs[e] = f16_pair(t[8 * group + 2 * e], t[8 * group + 2 * e + 1]);
             };
-            f16x8 v[2 * TILES];
+            f16x8 v[PRODUCTS];
             // (How many are read once product n is begun: with 256 dimensions there is room for two ahead until weights are done with.)
             auto read = [](int n) {
                 const int ahead = D < 256 ? 4 : n < TILES ? 2 : 4;
-                return n + 1 + ahead < 2 * TILES ? n + 1 + ahead : 2 * TILES;
+                return n + 1 + ahead < PRODUCTS ? n + 1 + ahead : PRODUCTS;
             };
 #pragma unroll
             for (int n = 0; n < read(-1); ++n) v[n] = value(n);
+            f32x4 inverse[2 * GROUPS];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) weigh(e);
+            for (int b = 0; b < 2; ++b) inverse[b] = inverses(4 * b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) weigh(e, inverse[e / 4][e % 4]);
             pack(0);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < 2 * TILES; ++n) {
+            for (int b = 2; b < 4; ++b) inverse[b] = inverses(4 * b);
+#pragma unroll
+            for (int n = 0; n < PRODUCTS; ++n) {
+                constexpr int EACH = 8 / TILES;
+                const int group = n / TILES;
                 __builtin_amdgcn_sched_barrier(0);
-                if (n == TILES) pack(1);
+                if (n % TILES == 0 && group > 0) pack(group);
                 acc[n % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[n], __builtin_bit_cast(f16x8, pairs), acc[n % TILES], 0, 0, 0);
 #pragma unroll
                 for (int m = read(n - 1); m < read(n); ++m) v[m] = value(m);
-                if (n < TILES) {
+                if (n % TILES == 0 && group + 2 < GROUPS)  // those of the weights after the next
 #pragma unroll
-                    for (int e = 8 + 8 * n / TILES; e < 8 + 8 * (n + 1) / TILES; ++e) weigh(e);
+                    for (int b = 2 * group + 4; b < 2 * group + 6; ++b) inverse[b] = inverses(4 * b);
+                if (group + 1 < GROUPS) {
+#pragma unroll
+                    for (int e = 8 * (group + 1) + n % TILES * EACH; e < 8 * (group + 1) + (n % TILES + 1) * EACH; ++e) weigh(e, inverse[e / 4][e % 4]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         };
 
-        bool dead[4] = {};  // of the step's record and of the next ones
         lds_barrier();  // (the last piece's LDS is read)
+        bool staged_hole = true;  // of the record that is widened next
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-            if (from + n < to) fetch(from + n, n), dead[n] = hole;
+        for (int n = 0; n < 2; ++n) {
+            if (from + n * RECORDS < to) fetch(from + n * RECORDS, n);
+            if (n == 0) staged_hole = hole;
+        }
         wait_vmcnt<0>();
         lds_barrier();
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-            if (from + n < to) part_of_step(std::false_type{}, n, n, n, 0);
+        part_of_step(std::false_type{}, 0, 0, 0, 0, staged_hole);
+        if (from + RECORDS < to) part_of_step(std::false_type{}, 1, 1, 1, 0, hole);
         lds_barrier();
-        if (from + 2 < to) fetch(from + 2, 0), dead[2] = hole;
+        if (from + 2 * RECORDS < to) fetch(from + 2 * RECORDS, 0);
+        staged_hole = hole;
         wait_vmcnt<0>();
-        // A step is the scores of one record, while the one after the next is widened, and then its values. Waves 4 to 7 are half a step
-        // behind: of a SIMD's two waves one has vector instructions where the other has few.
+        // A step is the scores of its records, while those of the step after the next are widened, and then its values. Waves 4 to 7 are half
+        // a step behind: of a SIMD's two waves one has vector instructions where the other has few.
         lds_barrier();
         if (wave >= 4) lds_barrier();
-        int third = 0;
-        for (int block = from; block < to; ++block) {
-            hole = false;
-            const int step = block - from;
-            if (block + 3 < to) fetch(block + 3, (step + 1) & 1);
-            dead[3] = hole;
+        int third = 0, step = 0;
+        for (int block = from; block < to; block += RECORDS, ++step) {
+            if (block + 3 * RECORDS < to) fetch(block + 3 * RECORDS, (step + 1) & 1);
             // (Behind the last records something that nothing reads is widened once more.)
-            part_of_step(std::true_type{}, step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3, third);
+            part_of_step(std::true_type{}, step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3, third, staged_hole);
+            staged_hole = hole;
             lds_barrier();
-            weigh_values(block, step & 3, dead[0]);
-#pragma unroll
-            for (int n = 0; n < 3; ++n) dead[n] = dead[n + 1];
+            weigh_values(block, step & 3);
             third = third == 2 ? 0 : third + 1;
             wait_vmcnt<0>();
             lds_barrier();
@@ -1157,7 +1165,7 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     AttendPlan p;
     const int cus = device_cus();
     p.few = vectors <= (cache.dim == 256 ? 48 : 64);
-    const int nt = (int)((vectors + 15) / 16), keys = p.few ? kFewGroups * kBlock : kManyKeys;
+    const int nt = (int)((vectors + 15) / 16), keys = (p.few ? kFewGroups : cache.dim == 64 ? 4 : 2) * kBlock;  // (whole steps)
     p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, p.few ? kFewExtra : kManyExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
     p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
     return p;
