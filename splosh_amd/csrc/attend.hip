@@ -32,9 +32,10 @@ constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
 constexpr int kManyThreads = 512, kManyRows = 256;
 constexpr int64_t kJoinApart = 4096;  // (row, query head) vectors that are joined a wave each
-// Units that a segment costs beside its keys. (Few vectors: 3, where 1 is 119 instead of 116 us for the 64 requests of 512 MB, 108 instead of
+// Units that a segment costs beside its keys. (Few vectors: 3, where 1 is 119 instead of 116 us for 64 requests of 600 MB, 108 instead of
 // 106 for the verify step; many: 1 to 6 are the same within 1 %.)
 constexpr int kFewExtra = 3, kManyExtra = 1;
+constexpr uint32_t kNoRecord = 0xffe5a7d3;     // in place of a scale: a NaN that no arithmetic gives
 
 struct AttendArgs {
     const uint16_t *q;
@@ -886,10 +887,10 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                 for (int c = 0; c < 4; ++c) piece(c);
             }
             if constexpr (VALUES) {
-                // (A record that is none: its values' logarithms are -inf, which no kept scale has.)
+                // (A record that is none: a key's scale that no record holds.)
                 if (quarter % (4 / RECORDS) == 0) {
                     float *const at = scales + (fourth * RECORDS + record_at) * 3 * kBlock + lane;
-                    at[0] = lane < kBlock ? scale : dead ? -__builtin_inff() : __builtin_amdgcn_logf(scale);
+                    at[0] = lane >= kBlock ? __builtin_amdgcn_logf(scale) : dead ? __uint_as_float(kNoRecord) : scale;
                     if (lane >= kBlock) at[kBlock] = inverse_scale(scale);
                 }
             }
@@ -916,7 +917,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                     const f32x4 ks = *reinterpret_cast<const f32x4 *>(at + r * 3 * kBlock + 8 * b);
                     const f32x4 lv = *reinterpret_cast<const f32x4 *>(at + r * 3 * kBlock + kBlock + 8 * b);
                     if (b == 0) {
-                        const bool dead = uniform((int)__float_as_uint(lv[0])) == (int)0xff800000u;
+                        const bool dead = (uint32_t)uniform((int)__float_as_uint(ks[0])) == kNoRecord;
                         masked |= dead, seen &= dead ? ~(1u << r) : ~0u;
                     }
 #pragma unroll

@@ -73,7 +73,7 @@ class Step:
     ([1] * 5, [1, 32, 64, 65, 500], 8, 2, 128, 32), ([8] * 4, [8, 40, 129, 1000], 10, 2, 256, 256), ([11] * 3, [300, 40, 11], 5, 1, 256, 64), ([3, 0, 7, 1], [10, 77, 7, 333], 10, 2, 128, 96),
     ([5], [5], 7, 7, 64, 32), ([2, 9], [300, 41], 32, 1, 64, 64), ([40], [40], 6, 1, 256, 64), ([100, 3], [150, 9], 5, 1, 128, 32),
     ([333], [400], 8, 2, 64, 64), ([300], [1000], 6, 1, 256, 256), ([64, 64, 64], [64, 200, 65], 4, 4, 128, 32),
-    ([700, 1, 2], [700, 2000, 2], 4, 1, 128, 96), ([513], [513], 3, 3, 256, 32), ([1] * 300, [1 + 7 * i % 190 for i in range(300)], 4, 2, 64, 32)])
+    ([700, 1, 2], [700, 2000, 2], 4, 1, 128, 96), ([200, 70], [1500, 70], 6, 1, 64, 96), ([130], [900], 4, 2, 64, 32), ([513], [513], 3, 3, 256, 32), ([1] * 300, [1 + 7 * i % 190 for i in range(300)], 4, 2, 64, 32)])
 def test_attend(rt, runs, lengths, q_heads, heads, dim, page):
     s = Step(rt, runs, lengths, q_heads, heads, dim, page, seed=len(runs) + dim, more=2, layout="gated" if dim == 128 else "dense", pad=3)
     s.check(s.run())
@@ -81,7 +81,7 @@ def test_attend(rt, runs, lengths, q_heads, heads, dim, page):
 
 @pytest.mark.parametrize("runs,own,shared,q_heads,heads,dim,page", [
     ([1, 1, 1], [5, 1, 40], 64, 4, 2, 128, 32), ([4] * 6, [4, 30, 64, 5, 100, 4], 512, 6, 1, 256, 256), ([3, 0, 2], [3, 9, 200], 96, 8, 2, 64, 96),
-    ([40] * 5, [40, 41, 80, 333, 64], 1024, 6, 2, 128, 64), ([1] * 70, [1 + i for i in range(70)], 256, 2, 1, 256, 32)])
+    ([40] * 5, [40, 41, 80, 333, 64], 1024, 6, 2, 128, 64), ([50, 50], [50, 70], 96, 4, 2, 64, 96), ([60, 9], [60, 70], 160, 4, 1, 128, 32), ([1] * 70, [1 + i for i in range(70)], 256, 2, 1, 256, 32)])
 def test_shared_prefix(rt, runs, own, shared, q_heads, heads, dim, page):
     """The same as without saying so, to the bounds of both; and other requests' entries for it are not used."""
     s = Step(rt, runs, [shared + n for n in own], q_heads, heads, dim, page, seed=dim, shared=shared, more=1)
@@ -118,6 +118,21 @@ def test_rows_without_keys(rt):
     slots = (s.table[2, 1:].long()[:, None] * 32 + torch.arange(32)).flatten()[: 70 - 32]
     out, off = attended(s.q[5:6], s.k64[slots], s.v64[slots], torch.tensor([70 - 33]), 128 ** -0.5)
     check_bf16(got[5:6], out, off)
+
+
+@pytest.mark.parametrize("rows,length,dim,page", [(3, 700, 128, 32), (100, 700, 64, 32), (100, 700, 128, 32), (90, 500, 256, 32), (130, 900, 64, 96)])
+def test_holes_between_pages(rt, rows, length, dim, page):
+    """Pages that are none, alone and side by side, first and last, below every kind of tile: their keys are masked."""
+    s = Step(rt, [rows], [length], 2, 1, dim, page, seed=15)
+    columns = -(-length // page)
+    none = sorted({0, 2, 3, 4, 7, columns - 3, columns - 1})
+    for i, column in enumerate(none):
+        s.packed.table[0, column] = (-1, s.pages, -(2 ** 31), 2 ** 31 - 1)[i % 4]
+    seen = torch.tensor([i // page not in none for i in range(length)])
+    slots = (s.table[0].long()[:, None] * page + torch.arange(page)).flatten()[:length][seen]
+    position = seen.long().cumsum(0)[length - rows + torch.arange(rows)] - 1
+    out, off = attended(s.q, s.k64[slots], s.v64[slots], position, dim ** -0.5)
+    check_bf16(s.run().cpu(), out, off)
 
 
 @pytest.mark.parametrize("runs,lengths,dim", [([1], [50], 256), ([4, 8], [37, 65], 128), ([200], [230], 256), ([150], [230], 64)])
