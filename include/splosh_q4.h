@@ -579,8 +579,8 @@ size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_pac
                                      int64_t q_heads, int64_t shared);
 
 /* out[m][h] = sum_j w_j v_j, w = softmax over j <= position(m) of scale q[m][h] . k_j, keys and values those
- * that head h / (q_heads / cache->heads) keeps for row m's request; the step's own have to be written before
- * (splosh_cache_write). q: bf16, vector (m, h) at q + m row_stride + h head_stride; out: bf16, dense rows of q_heads dim
+ * that head h / (q_heads / cache->heads) keeps for row m's request; all that lengths counts has to be written before, the
+ * step's own too (splosh_cache_write). q: bf16, vector (m, h) at q + m row_stride + h head_stride; out: bf16, dense rows of q_heads dim
  * values, row stride ld_out. A row that sees no key gets zeros.
  * shared: the first `shared` tokens (a multiple of page_tokens, 0: none) are the same for all requests of the call: they
  * are read through the pages of request 0, once for all rows; the table's entries of other requests for
