@@ -6,10 +6,10 @@
 // order that the shape alone gives: the neighbours of a draw on a vocabulary of 250000 lie 1e-9 of the weight apart, which fp32
 // would not tell.
 //
-// Three launches; a workgroup takes a piece of 8192 entries of a row, or a request:
+// Three launches; a workgroup takes a piece of 4096 entries of a row, or a request:
 //   scan   (pieces of every row)         the piece's largest entry and the weight of its entries against it;
 //   rest   (pieces of every request's row) which row ends the request's accepted run, from the pieces' numbers and one
-//          probability a row, and the weights max(p - q, 0) and p of that row by strips of 1024;
+//          probability a row, and the weights max(p - q, 0) and p of that row by strips of 512;
 //   finish (requests)                    the strip that the draw falls into, and the token in it.
 #include <climits>
 
@@ -19,8 +19,11 @@
 namespace splosh {
 
 constexpr size_t kVerifyCounterBytes = 16384;  // the workspace's first bytes belong to other kernels' counters
-constexpr int kThreads = 512, kWaves = kThreads / 64, kPer = 16;
+constexpr int kThreads = 512, kWaves = kThreads / 64, kPer = 8;  // of the workgroup for a piece of a request's row
 constexpr int kStrip = 64 * kPer, kPiece = kThreads * kPer;
+// The scan has sixteen entries a thread, so half the threads: 64 rows of 248320 fp32 16.9 us (512 threads of sixteen 18.3, of eight 21.3), where
+// the one row a request, mostly round trips, is 9.0 us with eight a thread (sixteen: 9.6, 256 threads of sixteen 11.5).
+constexpr int kScanPer = 16, kScanThreads = kPiece / kScanPer, kScanWaves = kScanThreads / 64;
 
 struct PieceStats {
     double sum;
@@ -140,20 +143,20 @@ __device__ __forceinline__ void keep_first(float &v, int &i, float w, int j) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
-    __shared__ float wave_most[kWaves];
-    __shared__ int wave_first[kWaves];
-    __shared__ double wave_total[kWaves];
+__global__ __launch_bounds__(kScanThreads) void scan_kernel(VerifyArgs a) {
+    __shared__ float wave_most[kScanWaves];
+    __shared__ int wave_first[kScanWaves];
+    __shared__ double wave_total[kScanWaves];
     const int row = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int r = request_of(a.starts, a.requests, row);
     if (r < 0) return;
     const T *logits = (const T *)a.logits + row * a.ld;
-    const int begin = piece * kPiece + wave * kStrip + lane * 4;  // its entries: four in a row, 256 further the next four
-    float v[kPer / 4][4], most = -__builtin_inff();
+    const int begin = piece * kPiece + wave * 64 * kScanPer + lane * 4;  // its entries: four in a row, 256 further the next four
+    float v[kScanPer / 4][4], most = -__builtin_inff();
 #pragma unroll
-    for (int k = 0; k < kPer / 4; ++k) entries(logits + begin + 256 * k, a.vocab - begin - 256 * k, v[k]);
+    for (int k = 0; k < kScanPer / 4; ++k) entries(logits + begin + 256 * k, a.vocab - begin - 256 * k, v[k]);
 #pragma unroll
-    for (int k = 0; k < kPer / 4; ++k)
+    for (int k = 0; k < kScanPer / 4; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = __builtin_fmaxf(most, v[k][e]);
 #pragma unroll
@@ -161,19 +164,19 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
     if (lane == 0) wave_most[wave] = most;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) most = __builtin_fmaxf(most, wave_most[w]);
+    for (int w = 0; w < kScanWaves; ++w) most = __builtin_fmaxf(most, wave_most[w]);
     int first = INT_MAX;
 #pragma unroll
-    for (int k = 0; k < kPer / 4; ++k)
+    for (int k = 0; k < kScanPer / 4; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) first = min(first, v[k][e] == most ? begin + 256 * k + e : INT_MAX);
     const double by = factor_of(a.temperature, r);
-    double sum = 0.0, w[kPer];
+    double sum = 0.0, w[kScanPer];
     // (Of a greedy row any one entry of the largest value stands for the piece: its first is found below.)
     if (by > 0.0) {
-        weights_of<kPer>(v, most, by, begin, 256, -1, w);
+        weights_of<kScanPer>(v, most, by, begin, 256, -1, w);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum += w[e];
+        for (int e = 0; e < kScanPer; ++e) sum += w[e];
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m), first = min(first, __shfl_xor(first, m));
@@ -181,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(VerifyArgs a) {
     if (lane == 0) wave_total[wave] = sum;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kWaves; ++w) sum += wave_total[w], first = min(first, wave_first[w]);
+        for (int w = 1; w < kScanWaves; ++w) sum += wave_total[w], first = min(first, wave_first[w]);
         if (by == 0.0) sum = most > -__builtin_inff() ? 1.0 : 0.0;
         a.stats[(int64_t)row * a.pieces + piece] = {sum, most, first};
     }
@@ -388,7 +391,7 @@ hipError_t launch_verify(const void *logits, int64_t ld, int dtype, int64_t rows
     a.strips = reinterpret_cast<StripSums *>(at);
     const dim3 rows_grid(a.pieces, (unsigned)rows), requests_grid(a.pieces, (unsigned)requests);
     auto go = [&](auto scan, auto rest, auto finish) {
-        scan<<<rows_grid, kThreads, 0, stream>>>(a);
+        scan<<<rows_grid, kScanThreads, 0, stream>>>(a);
         rest<<<requests_grid, kThreads, 0, stream>>>(a);
         finish<<<(unsigned)requests, 64, 0, stream>>>(a);
     };
