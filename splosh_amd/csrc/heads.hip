@@ -261,32 +261,38 @@ struct ReadArgs {
     int wide[2];
 };
 
+// A wave four heads of a row, keys and values: one way through the table for both, and both under way at once.
 template <int D>
 __global__ __launch_bounds__(kHeadThreads) void cache_read_kernel(ReadArgs a, CacheView cache, PackedView packed) {
     constexpr int E = D / kLanes;
-    const int row = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int which = lane / kLanes, first = lane % kLanes * E;
+    const int units = (cache.heads + kVectors - 1) / kVectors;
+    const int64_t item = (int64_t)blockIdx.x * kHeadWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = (int)(item / units), lane = threadIdx.x & 63;
+    const int head = (int)(item % units) * kVectors + lane / kLanes, first = lane % kLanes * E;
+    if (row >= packed.rows) return;
     const int r = request_of(packed.starts, packed.requests, row);
     if (r < 0) return;
     int page = 0, at = 0;
     const bool placed = place_of(cache, packed, r, packed.lengths[r] - packed.starts[r + 1] + row, page, at);
-    const int units = (cache.heads + kVectors - 1) / kVectors;
-#pragma unroll 2
-    for (int unit = wave; unit < 2 * units; unit += kHeadWaves) {
-        const int values = unit & 1, head = (unit >> 1) * kVectors + which;
-        if (!a.out[values] || head >= cache.heads) continue;
-        float v[E] = {};
-        if (placed) {
-            const uint8_t *record = record_of<D>(cache, page, head, at / kBlock);
-            const int token = at % kBlock;
-            struct alignas(E) Codes {
-                uint8_t of[E];
-            };
-            const Codes codes = *reinterpret_cast<const Codes *>(record + (values * kBlock + token) * D + first);
-            const float scale = reinterpret_cast<const float *>(record + 2 * kBlock * D)[values * kBlock + token];
+    if (head >= cache.heads) return;
+    struct alignas(E) Codes {
+        uint8_t of[E];
+    } codes[2] = {};
+    float scale[2] = {};
+    const uint8_t *record = record_of<D>(cache, placed ? page : 0, head, placed ? at / kBlock : 0);
+    const int token = placed ? at % kBlock : 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = (float)(codes.of[e] - 128) * scale;
-        }
+    for (int values = 0; values < 2; ++values) {
+        if (!a.out[values]) continue;
+        codes[values] = *reinterpret_cast<const Codes *>(record + (values * kBlock + token) * D + first);
+        scale[values] = reinterpret_cast<const float *>(record + 2 * kBlock * D)[values * kBlock + token];
+    }
+#pragma unroll
+    for (int values = 0; values < 2; ++values) {
+        if (!a.out[values]) continue;
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = placed ? (float)(codes[values].of[e] - 128) * scale[values] : 0.0f;
         store_bf16<E>(a.out[values] + row * a.ld[values] + (int64_t)head * D + first, a.wide[values], v);
     }
 }
@@ -361,7 +367,8 @@ hipError_t launch_cache_read(const splosh_cache &cache, const splosh_packed &pac
     const int64_t bytes = run_bytes(cache.dim, 2);
     const ReadArgs a{{k, v}, {ldk, ldv}, {fits(k, ldk, 2, bytes), fits(v, ldv, 2, bytes)}};
     auto go = [&](auto kernel) {
-        kernel<<<(unsigned)rows, kHeadThreads, 0, stream>>>(a, view_of(cache), view_of(packed, rows));
+        const int64_t items = rows * ((cache.heads + kVectors - 1) / kVectors);
+        kernel<<<(unsigned)((items + kHeadWaves - 1) / kHeadWaves), kHeadThreads, 0, stream>>>(a, view_of(cache), view_of(packed, rows));
     };
     if (cache.dim == 256) go(cache_read_kernel<256>);
     else if (cache.dim == 128) go(cache_read_kernel<128>);
