@@ -96,6 +96,46 @@ def test_prefix_longer_than_a_request(rt):
     s.check(s.run())
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_any_step(rt, seed):
+    """Steps of any shape: requests with no, one and many rows, groups of one to fifteen, pages of 32 to 1024 tokens, with and
+    without a shared prefix, and rows before the first request and behind the last."""
+    gen = torch.Generator().manual_seed(500 + seed)
+    pick = lambda *v: v[int(torch.randint(0, len(v), (1,), generator=gen))]  # noqa: E731
+    dim, heads, page, requests = pick(64, 128, 256), pick(1, 2, 3), pick(32, 64, 96, 1024), pick(1, 2, 5, 9, 67)
+    group = pick(1, 2, 3, 5, 7, 15)
+    shared = pick(0, 0, 1, 3) * page if page < 1024 else 0
+    runs = [pick(0, 1, 1, 2, 4, 7) if requests > 2 else pick(1, 9, 33, 150) for _ in range(requests)]
+    runs[-1] = max(runs[-1], 1)
+    lengths = [shared + n + pick(0, 0, 1, 31, 100, 333) for n in runs]
+    s = Step(rt, runs, lengths, heads * group, heads, dim, page, seed=seed, shared=shared, more=pick(0, 3), layout=pick("dense", "gated"),
+             pad=pick(0, 1))
+    scale = pick(None, 0.3)
+    s.check(s.run(scale=scale), scale)
+
+
+def test_rows_before_the_first_request(rt):
+    """starts[0] above zero: those rows belong to no request."""
+    s = Step(rt, [3, 50], [40, 90], 4, 2, 64, 32, seed=16)
+    want = s.run()
+    s.packed.starts[0] = 2
+    for shared in (0, 32):
+        got = rt.attend(s.q_gpu, s.cache, s.packed, shared=shared, out=torch.full_like(want, 9.0))
+        assert bool((got[:2] == 9).all())
+        if shared == 0:  # (request 0 has one row of the same position)
+            assert torch.equal(got[2:], want[2:])
+
+
+def test_lengths_past_the_table(rt):
+    """A length of more tokens than the table has pages for: its rows see those that are there."""
+    for rows in (2, 90):
+        s = Step(rt, [rows], [96], 4, 2, 128, 32, seed=17)
+        s.packed.lengths[0] = 96 + 1000
+        slots = (s.table[0].long()[:, None] * 32 + torch.arange(32)).flatten()
+        out, off = attended(s.q, s.k64[slots], s.v64[slots], torch.full((rows,), 95), 128 ** -0.5)
+        check_bf16(s.run().cpu(), out, off)
+
+
 def test_scales_far_apart(rt):
     """Values whose sizes differ by orders of magnitude, among them vectors of zeros, and sharp and flat weights."""
     for spread, scale in ((4.0, 0.01), (2.0, 3.0)):
