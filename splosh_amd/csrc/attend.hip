@@ -49,7 +49,7 @@ struct AttendArgs {
     int prefix;                 // the launch over the shared prefix
     int partial;                // whether every piece leaves its partial result
     float *slots;
-    int64_t segment_slots;
+    int64_t first_slots;        // where the slots begin of pieces that are not their segment's first
     struct Pieces *pieces;      // of every (row, query head)
 };
 
@@ -353,11 +353,11 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
         p.span = span, p.request = request, p.head = head, p.tile = t;
         p.first_block = max(0, offset - tile.extra) * per;
         p.blocks = max(0, min((offset + take - tile.extra) * per, blocks) - p.first_block);
-        p.slot = first ? segment : (int)a.segment_slots + w;
+        p.slot = !first ? (int)a.first_slots + w : a.partial ? segment : w;
         p.count = !first ? 0 : offset + take == units ? 1 : owner_of(total, sharers, unit + units - offset - 1) - w + 1;
         p.direct = !a.partial && first && offset + take == units;
-        // (More segments than slots there are only where starts do not ascend.)
-        if (offset + take > tile.extra && segment < a.segment_slots) work(p);
+        // (More segments than slots for them there are only where starts do not ascend.)
+        if (offset + take > tile.extra && (!a.partial || segment < a.first_slots)) work(p);
         unit += take;
         if (unit >= end) return;
         offset = 0, ++segment;
@@ -1081,11 +1081,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
     if (row >= end | row < begin | (mine.count == 1 && !own.partial)) return;
     float top = kLowest, total = 0.0f, o[E] = {};
     auto join = [&](const AttendArgs &l, const Pieces &p) {
-        const int rows = l.tile.rows, last = (int)l.segment_slots + l.tile.workgroups;
+        const int rows = l.tile.rows, last = (int)l.first_slots + l.tile.workgroups;
         const int64_t size = rows * (int64_t)(D + 2);
         // (Of rows that no request has, where starts do not ascend, this is what the workspace happened to hold.)
         if (p.slot < 0 || p.slot >= last || p.workgroup < 0 || p.count < 1 || p.count > l.tile.workgroups - p.workgroup || p.at < 0 || p.at >= rows) return;
-        auto slot = [&](int j) { return l.slots + (j == 0 ? p.slot : l.segment_slots + p.workgroup + j) * size; };
+        auto slot = [&](int j) { return l.slots + (j == 0 ? p.slot : l.first_slots + p.workgroup + j) * size; };
         for (int base = 0; base < p.count; base += LANES) {
             const int j = base + lane, here = min(LANES, p.count - base);
             float most = kLowest, sum = 0.0f;
@@ -1155,8 +1155,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
 struct AttendPlan {
     bool few;
     TileShape tile;
-    int64_t segment_slots;
-    size_t slot_bytes() const { return (size_t)((segment_slots + tile.workgroups) * tile.rows); }  // times (dim + 2) floats
+    int64_t segments;  // at most
+    // A workgroup leaves one piece at most that ends before its segment does, and one that does not begin with it; where every
+    // segment leaves its sums (a prefix is to be joined), each has a slot.
+    int64_t first_slots(bool partial) const { return partial ? segments : tile.workgroups; }
+    size_t slot_rows(bool partial) const { return (size_t)((first_slots(partial) + tile.workgroups) * tile.rows); }  // of dim + 2 floats
 };
 
 // `vectors`: those of a request and key/value head, on average. (Few and many, eight requests of 8192 tokens with 24 heads on 4, us, at 18, 30,
@@ -1168,7 +1171,7 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     p.few = vectors <= (cache.dim == 256 ? 48 : 64);
     const int nt = (int)((vectors + 15) / 16), keys = (p.few ? kFewGroups : cache.dim == 64 ? 4 : 2) * kBlock;  // (whole steps)
     p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, p.few ? kFewExtra : kManyExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
-    p.segment_slots = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
+    p.segments = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
     return p;
 }
 static AttendPlan plan_own(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads) {
@@ -1183,12 +1186,12 @@ static size_t pieces_bytes(int64_t rows, int64_t q_heads) { return (size_t)(rows
 // Units are counted in 32 bits: whether a launch of this size can have no more.
 bool attend_fits(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t tokens) {
     const AttendPlan p = plan_own(cache, requests, rows, q_heads);
-    return p.segment_slots * (tokens / p.tile.keys + 2 + p.tile.extra) < INT32_MAX && p.segment_slots + p.tile.workgroups < INT32_MAX;
+    return p.segments * (tokens / p.tile.keys + 2 + p.tile.extra) < INT32_MAX && p.segments + p.tile.workgroups < INT32_MAX;
 }
 
 size_t attend_workspace_bytes(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads, int64_t shared) {
-    size_t slots = plan_own(cache, requests, rows, q_heads).slot_bytes();
-    if (shared > 0) slots += plan_prefix(cache, rows, q_heads).slot_bytes();
+    size_t slots = plan_own(cache, requests, rows, q_heads).slot_rows(shared > 0);
+    if (shared > 0) slots += plan_prefix(cache, rows, q_heads).slot_rows(true);
     return kAttendCounterBytes + (shared > 0 ? 2 : 1) * pieces_bytes(rows, q_heads) + slots * (size_t)(cache.dim + 2) * sizeof(float);
 }
 
@@ -1232,16 +1235,16 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
     a.factor = scale * 1.4426950408889634f;
     a.pieces = reinterpret_cast<Pieces *>(at);
     a.slots = reinterpret_cast<float *>(at + (shared > 0 ? 2 : 1) * pieces_bytes(rows, q_heads));
-    a.tile = own.tile, a.segment_slots = own.segment_slots, a.partial = shared > 0;
+    a.tile = own.tile, a.partial = shared > 0, a.first_slots = own.first_slots(a.partial);
     const CacheView cv = view_of(cache);
     const PackedView pv = view_of(packed, rows);
     AttendArgs b = a;
     AttendPlan prefix = own;
     if (shared > 0) {
         prefix = plan_prefix(cache, rows, q_heads);
-        b.tile = prefix.tile, b.segment_slots = prefix.segment_slots, b.prefix = 1;
+        b.tile = prefix.tile, b.first_slots = prefix.first_slots(true), b.prefix = 1;
         b.pieces = a.pieces + rows * q_heads;
-        b.slots = a.slots + own.slot_bytes() * (cache.dim + 2);
+        b.slots = a.slots + own.slot_rows(true) * (cache.dim + 2);
     }
     auto run = [&](auto dim) {
         constexpr int D = decltype(dim)::value;

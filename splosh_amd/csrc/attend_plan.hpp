@@ -92,8 +92,7 @@ __host__ __device__ __forceinline__ int owner_of(int total, int workgroups, int 
     return (int)(((double)(u + 1) * workgroups - 1.0) / total);
 }
 
-// A piece of a segment keeps its partial result in a slot: the one that begins the segment in that of the
-// segment, any other (a workgroup has one such at most, its first) in that of its workgroup.
+// The most segments that a step of so many requests and rows can have.
 __host__ __device__ __forceinline__ int64_t most_segments(int64_t requests, int64_t rows, int64_t q_heads, int64_t heads, int tile_rows) {
     return heads * ((requests < rows ? requests : rows) + rows * (q_heads / heads) / tile_rows);
 }

@@ -48,6 +48,13 @@ def test_attend(rt, st):
     assert bool((st["out"] == 3).all())
 
 
+def test_workspace_of_long_prompts(rt, st):
+    """Beside sixteen bytes a (row, query head) the scratch is a matter of the device, not of the prompt's length."""
+    one = rt.Packed(st["packed"].starts[:2].contiguous(), st["packed"].lengths[:1].contiguous(), st["packed"].table[:1].contiguous())
+    need = {rows: rt.attend_workspace_bytes(st["cache"], one, rows, HEADS) for rows in (2048, 1 << 17)}
+    assert need[1 << 17] - need[2048] == 16 * HEADS * ((1 << 17) - 2048)
+
+
 def test_heads_and_cache(rt, st):
     write = lambda k=st["k"], v=st["v"], q=st["q"], **kw: rt.cache_write(st["cache"], st["packed"], k, v, q, out=st["out"], **kw)  # noqa: E731
     for kw in (dict(k=st["q"]), dict(v=st["v"].float()), dict(q=st["q"].float()), dict(k=st["k"].cpu()), dict(v=st["v"][:4]), dict(q=st["q"][..., :32]),
