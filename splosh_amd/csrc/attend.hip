@@ -32,9 +32,6 @@ constexpr float kLowest = -1e30f;              // M before the first key
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
 constexpr int kManyThreads = 512, kManyRows = 256;
 constexpr int64_t kJoinApart = 4096;  // (row, query head) vectors that are joined a wave each
-// Units that a segment costs beside its keys. (Few vectors: 3, where 1 is 119 instead of 116 us for 64 requests of 600 MB, 108 instead of
-// 106 for the verify step; many: 1 to 6 are the same within 1 %.)
-constexpr int kFewExtra = 3, kManyExtra = 1;
 constexpr uint32_t kNoRecord = 0xffe5a7d3;     // in place of a scale: a NaN that no arithmetic gives
 
 struct AttendArgs {
@@ -1170,8 +1167,15 @@ static AttendPlan plan_launch(int64_t vectors, int64_t requests, int64_t rows, i
     const int cus = device_cus();
     p.few = vectors <= (cache.dim == 256 ? 48 : 64);
     const int nt = (int)((vectors + 15) / 16), keys = (p.few ? kFewGroups : cache.dim == 64 ? 4 : 2) * kBlock;  // (whole steps)
-    p.tile = tile_shape(p.few ? 16 * nt : kManyRows, keys, p.few ? kFewExtra : kManyExtra, (int)(q_heads / cache.heads), (int)cache.heads, p.few && cache.dim < 256 ? 2 * cus : cus);
-    p.segments = most_segments(requests, rows, q_heads, cache.heads, p.tile.rows);
+    const int tile = p.few ? 16 * nt : kManyRows, workgroups = p.few && cache.dim < 256 ? 2 * cus : cus;
+    p.segments = most_segments(requests, rows, q_heads, cache.heads, tile);
+    // What a segment costs beside its keys (its queries, filling the pipeline, its sums out), in units of keys. Few vectors: 3 (with 1 the
+    // decode step of 64 requests is 119 us instead of 116, the verify step 108 instead of 106). Many: 5, with dim 64, whose units are
+    // twice as long, 3 (with 1 a prompt of 8192 rows of 24 heads on 4 takes 1190 us instead of 944, with 64 dimensions 478 instead of 395; 7 and 10 are
+    // level or slower). Where segments are so few that each is cut over four workgroups or more, 1: a unit more or less is a large part of
+    // a share then (7 requests of 333 rows, heads of 128: 31.5 us instead of 33.6).
+    const int extra = p.few ? 3 : p.segments * 4 < workgroups ? 1 : cache.dim == 64 ? 3 : 5;
+    p.tile = tile_shape(tile, keys, extra, (int)(q_heads / cache.heads), (int)cache.heads, workgroups);
     return p;
 }
 static AttendPlan plan_own(const splosh_cache &cache, int64_t requests, int64_t rows, int64_t q_heads) {
