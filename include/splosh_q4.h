@@ -617,7 +617,8 @@ size_t splosh_verify_workspace_bytes(int64_t rows, int64_t vocab, int64_t reques
  *   - u below 0 or NaN counts as 0; u >= 1: the last entry with weight. A drafted id that is negative or not below
  *     vocab is not accepted. A NaN q is not accepted and leaves no weight.
  *   - A request without rows has accepted 0; rows of `out` past starts[requests] are left as they were.
- * Weights are good to 1e-9 and added in 64 bits in an order that the shape alone gives, so the result is the same each time.
+ * The weights that a draw goes through are good to 1e-13, a row's whole weight to 1e-9, all added in 64 bits in an order
+ * that the shape alone gives, so the result is the same each time.
  * `out` and `accepted` must not overlap each other, `tokens` or `starts`. vocab <= 2^21, rows and requests <= 65535.
  * The workspace need not be zeroed; its first 16 KiB stay as they are. */
 int splosh_verify(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const int32_t *tokens,

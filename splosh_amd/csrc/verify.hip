@@ -54,10 +54,35 @@ struct VerifyArgs {
     StripSums *strips;
 };
 
-// 2^x, x <= 0, to 1e-9 of it: the whole part as the exponent, and of the fraction (|f| <= 1/2) the series in f ln 2, from the third power on
-// in fp32 (that part is below 0.008: off by 5e-10 at most, where it ends with the eighth power by 2e-10). All of it in 64 bits
-// takes twice the time: 30 us for the 64 rows of 248320, and the sums gain nothing by it.
-__device__ __forceinline__ double power2(double x) {
+// 2^(j / 64): each thread below 64 puts one into LDS.
+constexpr int kSteps = 64;
+__constant__ const double kPowers[kSteps] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284, 1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418, 1.1387886347566916, 1.1511892299529827, 1.1637248587775775,
+    1.1763969916502812, 1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687, 1.241857812073484, 1.255380757024691,
+    1.2690509571917332, 1.2828700160787783, 1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303, 1.3542555469368927,
+    1.3690024229745905, 1.383909881963832, 1.3989796725383112, 1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384, 1.5422108254079407, 1.559004400237837, 1.5759808451078865,
+    1.593142151342267, 1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364, 1.681792830507429, 1.7001063537185235,
+    1.718619298122478, 1.7373338352737062, 1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989, 1.8340080864093424,
+    1.8539791250833855, 1.8741676341103, 1.8945759815869656, 1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+
+// 2^(x / 64), x <= 0, to 1e-13 of it: x is a whole number and a rest |r| <= 1/2; of the whole number the last six bits are looked up and the
+// others are the exponent, and of the rest comes the series in r ln 2 / 64 (the fifth power left out by 4e-14). Borders between tokens lie
+// close: with the entries of a draw good to 1e-9, one draw of 8000 over 248320 of them could fall to another token than in 64 bits.
+__device__ __forceinline__ double power2(double x, const double *powers) {
+    x = __builtin_fmax(x, -128000.0);  // (0 from 2^-1075 on)
+    const double shifted = x + 0x1.8p52, r = x - (shifted - 0x1.8p52);  // (the low bits of `shifted` are the whole number)
+    const int whole = (int)(uint32_t)__double_as_longlong(shifted);
+    const double e = r * __builtin_fma(__builtin_fma(__builtin_fma(5.732851688640402e-10, r, 2.1173137155464776e-07), r, 5.86490495505617e-05), r, 0.010830424696249145);
+    const double power = powers[whole & (kSteps - 1)];
+    return __builtin_ldexp(__builtin_fma(power, e, power), whole >> 6);
+}
+
+// 2^x, x <= 0, to 1e-9 of it, for the sums of the scan, whose errors even out: the whole part as the exponent, and of the fraction (|f| <= 1/2)
+// the series in f ln 2, from the third power on in fp32 (that part is below 0.008: off by 5e-10 at most, where it ends with the eighth
+// power by 2e-10). 64 rows of 248320 fp32 take 16.9 us so, 19.0 with the function above.
+__device__ __forceinline__ double power2_near(double x) {
     x = __builtin_fmax(x, -2000.0);  // (0 from 2^-1075 on)
     const double n = __builtin_rint(x), f = x - n;
     const float g = (float)f;
@@ -79,11 +104,11 @@ __device__ __forceinline__ double factor_of(const float *temperature, int reques
 }
 
 // The weight of an entry against the largest, `most`; `first`: whether it is the first of that value.
-__device__ __forceinline__ double weight_of(float v, float most, double by, bool first) {
+__device__ __forceinline__ double weight_of(float v, float most, double by, bool first, const double *powers) {
     if (!(v > -__builtin_inff())) return 0.0;  // (NaN and -inf)
     if (by == 0.0) return first ? 1.0 : 0.0;
     if (v == most) return 1.0;
-    return most == __builtin_inff() ? 0.0 : power2(((double)v - (double)most) * by);
+    return most == __builtin_inff() ? 0.0 : power2(((double)v - (double)most) * (kSteps * by), powers);
 }
 
 // Four entries in a row, of a row of any alignment, the first `here` of which are its.
@@ -116,13 +141,16 @@ __device__ __forceinline__ void entries(const uint16_t *p, int here, float (&v)[
 
 // The weights of N entries in fours from index `first` on, `step` further the next four. With a finite `most` and a T, NaN and -inf go the way of
 // what is far below it: 2^-2000.
-template <int N>
-__device__ __forceinline__ void weights_of(const float (&v)[N / 4][4], float most, double by, int first, int step, int top, double (&w)[N]) {
+template <int N, bool NEAR>
+__device__ __forceinline__ void weights_of(const float (&v)[N / 4][4], float most, double by, int first, int step, int top, const double *powers, double (&w)[N]) {
     if (by > 0.0 && __builtin_fabsf(most) < __builtin_inff()) {
 #pragma unroll
         for (int k = 0; k < N / 4; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[4 * k + e] = power2(((double)v[k][e] - (double)most) * by);
+            for (int e = 0; e < 4; ++e) {
+                const double x = (double)v[k][e] - (double)most;
+                w[4 * k + e] = NEAR ? power2_near(x * by) : power2(x * (kSteps * by), powers);
+            }
     } else {
 #pragma unroll
         for (int k = 0; k < N / 4; ++k)
@@ -174,7 +202,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(VerifyArgs a) {
     double sum = 0.0, w[kScanPer];
     // (Of a greedy row any one entry of the largest value stands for the piece: its first is found below.)
     if (by > 0.0) {
-        weights_of<kScanPer>(v, most, by, begin, 256, -1, w);
+        weights_of<kScanPer, true>(v, most, by, begin, 256, -1, nullptr, w);
 #pragma unroll
         for (int e = 0; e < kScanPer; ++e) sum += w[e];
     }
@@ -191,7 +219,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(VerifyArgs a) {
 }
 
 // The whole row from its pieces, by one wave: the largest entry, the first of that value, and the weight against it.
-__device__ __forceinline__ PieceStats row_stats(const VerifyArgs &a, int row, double by) {
+__device__ __forceinline__ PieceStats row_stats(const VerifyArgs &a, int row, double by, const double *powers) {
     const int lane = threadIdx.x & 63;
     const PieceStats *stats = a.stats + (int64_t)row * a.pieces;
     float most = -__builtin_inff();
@@ -200,7 +228,7 @@ __device__ __forceinline__ PieceStats row_stats(const VerifyArgs &a, int row, do
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) keep_first(most, first, __shfl_xor(most, m), __shfl_xor(first, m));
     double sum = 0.0;
-    for (int i = lane; i < a.pieces; i += 64) sum += stats[i].sum * weight_of(stats[i].most, most, by, stats[i].first == first);
+    for (int i = lane; i < a.pieces; i += 64) sum += stats[i].sum * weight_of(stats[i].most, most, by, stats[i].first == first, powers);
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
     return {sum, most, first};
@@ -217,7 +245,7 @@ __device__ __forceinline__ double uniform_of(const VerifyArgs &a, int row) { ret
 
 // (weight of max(p - q, 0), of p) of N entries of the decided row from `token` on, four in a row and `step` further the next four.
 template <typename T, int N>
-__device__ __forceinline__ void rests_of(const VerifyArgs &a, const Decision &d, int drafted, int token, int step, StripSums (&w)[N]) {
+__device__ __forceinline__ void rests_of(const VerifyArgs &a, const Decision &d, int drafted, int token, int step, const double *powers, StripSums (&w)[N]) {
     float v[N / 4][4], q[N / 4][4];
     const T *logits = (const T *)a.logits + d.row * a.ld;
     const bool whole = d.last || !a.draft;
@@ -233,7 +261,7 @@ __device__ __forceinline__ void rests_of(const VerifyArgs &a, const Decision &d,
     }
     const double inv = d.total > 0.0 ? 1.0 / d.total : 0.0;
     double weight[N];
-    weights_of<N>(v, d.most, d.by, token, step, d.top, weight);
+    weights_of<N, false>(v, d.most, d.by, token, step, d.top, powers, weight);
 #pragma unroll
     for (int k = 0; k < N / 4; ++k)
 #pragma unroll
@@ -250,6 +278,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
     constexpr int kKept = 64;
     __shared__ int stop;
     __shared__ PieceStats kept[kKept];
+    __shared__ double powers[kSteps];
     const int r = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int begin = max(a.starts[r], 0), end = min(a.starts[r + 1], a.rows);
     if (begin >= end) {
@@ -257,6 +286,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
         return;
     }
     if (tid == 0) stop = end - 1;
+    if (tid < kSteps) powers[tid] = kPowers[tid];
     __syncthreads();
     const double by = factor_of(a.temperature, r);
     // A wave a row; what the deciding row's numbers are is kept for as many rows as there is room for.
@@ -265,8 +295,8 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
         bool accept = t >= 0 && t < a.vocab;
         const float logit = accept ? entry((const T *)a.logits + row * a.ld + t) : 0.0f;
         const double u = uniform_of(a, row), q = accept ? draft_of(a, row, t, t) : 0.0;
-        const PieceStats s = row_stats(a, row, by);
-        if (accept) accept = s.sum > 0.0 && u * q < weight_of(logit, s.most, by, t == s.first) / s.sum;
+        const PieceStats s = row_stats(a, row, by, powers);
+        if (accept) accept = s.sum > 0.0 && u * q < weight_of(logit, s.most, by, t == s.first, powers) / s.sum;
         if (lane == 0) {
             if (!accept) atomicMin(&stop, row);
             if (row - begin < kKept) kept[row - begin] = s;
@@ -276,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
     const int last = stop;
     PieceStats s;
     if (last - begin < kKept) s = kept[last - begin];
-    else s = row_stats(a, last, by);
+    else s = row_stats(a, last, by, powers);
     const Decision d = {last, last == end - 1, s.first, s.most, s.sum, by};
     const int drafted = d.last ? -1 : a.tokens[d.row + 1];
     if (piece == 0) {
@@ -285,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(VerifyArgs a) {
             if (row != d.row) a.out[row] = row < d.row ? a.tokens[row + 1] : -1;
     }
     StripSums sum{0.0, 0.0}, w[kPer];
-    rests_of<T, kPer>(a, d, drafted, piece * kPiece + wave * kStrip + lane * 4, 256, w);
+    rests_of<T, kPer>(a, d, drafted, piece * kPiece + wave * kStrip + lane * 4, 256, powers, w);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum.rest += w[e].rest, sum.whole += w[e].whole;
 #pragma unroll
@@ -308,8 +338,11 @@ __device__ __forceinline__ double wave_running(double v) {
 // run the draw falls into goes through it.
 template <typename T>
 __global__ __launch_bounds__(64) void finish_kernel(VerifyArgs a) {
+    __shared__ double powers[kSteps];
     const int r = blockIdx.x, lane = threadIdx.x;
     const Decision d = a.decisions[r];
+    powers[lane] = kPowers[lane];
+    __syncthreads();
     const StripSums *strips = a.strips + (int64_t)r * a.pieces * kWaves;
     const int count = a.pieces * kWaves, run = (count + 63) / 64;
     const int low = min(lane * run, count), high = min(low + run, count);
@@ -345,7 +378,7 @@ __global__ __launch_bounds__(64) void finish_kernel(VerifyArgs a) {
         }
         if (strip >= 0) {
             StripSums w[kPer];
-            rests_of<T, kPer>(a, d, drafted, strip * kStrip + lane * kPer, 4, w);
+            rests_of<T, kPer>(a, d, drafted, strip * kStrip + lane * kPer, 4, powers, w);
             double own = 0.0;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) own += from_rest ? w[e].rest : w[e].whole;

@@ -62,7 +62,7 @@ def verified(logits, tokens, u, temperature, draft):
 
 
 def check(rt, logits, tokens, runs, u, temperature, draft, more=0, **kw):
-    """Every request's result; weights are good to 1e-9, and no decision in these inputs is within 4e-9 of the row's weight."""
+    """Every request's result; a row's weight is good to 1e-9, and no decision in these inputs is within 4e-9 of it."""
     starts = torch.tensor([sum(runs[:r]) for r in range(len(runs) + 1)], dtype=torch.int32)
     out = torch.full((len(tokens),), 77, dtype=torch.int32, device="cuda")
     cuda = lambda t: t.cuda() if t is not None else None  # noqa: E731
@@ -164,3 +164,21 @@ def test_layouts_and_graph(rt):
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(accepted, want[1])
         assert bool((ws[:16384] == 0xff).all())
+
+
+def test_many_draws(rt):
+    """Draws over a whole vocabulary, a thousand of them: every token is the one of 64 bits on the host."""
+    gen = torch.Generator().manual_seed(4)
+    rows, vocab = 256, 100003
+    starts = torch.arange(rows + 1, dtype=torch.int32)
+    for turn in range(4):
+        x = 2.0 * torch.randn(rows, vocab, generator=gen)
+        u, t = torch.rand(rows, generator=gen), 0.5 + torch.rand(rows, generator=gen)
+        got, _ = rt.verify(x.cuda(), torch.zeros(rows, dtype=torch.int32).cuda(), starts.cuda(), u.cuda(), t.cuda())
+        got = got.cpu().long()
+        running = ((x.double() - x.amax(1, keepdim=True)) / t.double()[:, None]).exp().cumsum(1)
+        draw = u.double()[:, None] * running[:, -1:]
+        want = (running > draw).to(torch.uint8).argmax(1)
+        # (The order of the sums alone moves a draw by 1e-11 of the weight at most: 100003 additions of 2^-53.)
+        for r in (got != want).nonzero()[:, 0].tolist():
+            assert abs(float(running[r, min(int(got[r]), int(want[r]))] - draw[r, 0])) < 1e-11 * float(running[r, -1]), (turn, r)
