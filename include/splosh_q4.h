@@ -586,7 +586,8 @@ size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_pac
  * are read through the pages of request 0, once for all rows; the table's entries of other requests for
  * them are not used. Scores and sums are fp32; q's values enter the first product in fp16 after a power of two that leaves them
  * as they are (what is below 2^-28 of its vector's largest: to 2^-39 of that), the weights the second one rounded to
- * fp16 (2^-11 of each). out may be q itself, with the same strides. Nothing is added in an order that changes: the result depends
+ * fp16 (2^-11 of each). Every key has its weight, whatever the sizes of the values; where a request's values hold vectors above 508 beside some
+ * below 2^-55 (zeros too), or above 2^47 at all, it is some 20 to 30 times slower. out may be q itself, with the same strides. Nothing is added in an order that changes: the result depends
  * on the step's shape and on the device's count of CUs, and on no other call. SPLOSH_ERR_UNSUPPORTED where rows, heads and the
  * table's tokens are so many that their pieces could pass 2^31. The workspace need not be zeroed; its first
  * 16 KiB stay as they are, so one that other calls use serves here too, in stream order. */

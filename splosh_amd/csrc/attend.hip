@@ -8,6 +8,14 @@
 // a row of q, moved by the power of two that brings its largest to 2^14 (what is below 2^-28 of that is cut at 2^-39 of it).
 // Both products run on the fp16 matrix instructions with fp32 sums.
 //
+// Beside a key whose value has a large scale, a_j of one with a small scale (2^-100 for a value of zeros) may be below what fp32 holds, where
+// its a_j / vs_j is not. What is lost so of the sum is below 2^(-126 - log2(vs_j)), and the key that M is from has 2^-log2(vs) of it: below 2^-24 of
+// the whole while the scales of a piece are within 2^102 of each other, as they are where none is above 4, or none below 2^-62 and none above 2^40. The loops
+// note whether that is so. Where it is not, a piece leaves its vectors to the last launch, which goes through all of their keys by itself
+// (apart_vector: 20 to 30 times the time). Made good in these kernels, in the loop, behind it or in an instance of its own, it took registers from the sums, or
+// parted what is scheduled together: the verify step took 107 to 168 us instead of 103, with the notes alone 106.
+// Where M moves, and where pieces are joined, the sum is scaled by 2^(x / 2) twice: for scales from 2^-100 to 2^122 it is between 2^-122 and 2^108 a key.
+//
 // Scores are computed transposed, keys by queries: a lane then holds four consecutive keys of one query, and their
 // weights are, as they are, its operand of the second product (values' dimensions by queries), whose order of keys is
 // free as long as both operands have the same. Nothing but sums over the lanes of a query crosses lanes.
@@ -35,6 +43,10 @@ constexpr int kManyThreads = 512, kManyRows = 256;
 // or three: 51 us, sixteen lanes 25.)
 constexpr int64_t kJoinApart = 4096;
 constexpr uint32_t kNoRecord = 0xffe5a7d3;     // in place of a scale: a NaN that no arithmetic gives
+constexpr float kFarApart = 0x1p102f;          // the most that scales may lie apart
+constexpr float kSmallScale = 0x1p-62f, kLargeScale = 4.0f;             // with one below and one above they may be
+constexpr uint32_t kSmallBits = 0x20800000u, kLargeBits = 0x40800000u;  // of these
+constexpr float kApart = -1.0f;                // in place of a sum, which is not negative
 
 struct AttendArgs {
     const uint16_t *q;
@@ -56,7 +68,7 @@ struct AttendArgs {
 struct Pieces {
     int slot;       // the first one's
     int workgroup;  // the workgroup that took it; the next ones took the next, and have slots by workgroup
-    int count;      // 1 and no prefix: written already
+    int count;      // 1 and no prefix: written already; -1: of a whole segment whose scales lie far apart
     int at;         // its vector of the tile
 };
 
@@ -161,6 +173,12 @@ __device__ __forceinline__ float max_halves(float v) {
 __device__ __forceinline__ float inverse_scale(float vs) {
     const float r = __builtin_amdgcn_rcpf(vs);
     return __builtin_fabsf(r) < __builtin_inff() ? r : 1.0f;
+}
+
+// A sum against another maximum: v 2^x.
+__device__ __forceinline__ float scaled(float v, float x) {
+    const float root = __builtin_amdgcn_exp2f(0.5f * x);
+    return v * root * root;
 }
 
 // The packed row that vector x of a tile's request is of.
@@ -396,6 +414,15 @@ __device__ __forceinline__ void write_sums(const AttendArgs &a, const Piece &p, 
         for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4 *>(at + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
     }
 }
+// A vector whose piece's scales lie far apart.
+template <int D>
+__device__ __forceinline__ void write_apart(const AttendArgs &a, const Piece &p, int i) {
+    const int x = p.tile * a.tile.rows + i;
+    if (x >= p.span.n * a.tile.group) return;
+    if (p.count > 0)
+        a.pieces[(int64_t)row_of(p, a.tile, x) * a.q_heads + head_of(p, a.tile, x)] = {p.slot, (int)blockIdx.x, p.direct ? -1 : p.count, i};
+    if (!p.direct) a.slots[p.slot * (a.tile.rows * (int64_t)(D + 2)) + (int64_t)a.tile.rows * (D + 1) + i] = kApart;
+}
 // And its maximum and sum, where they are left; with the segment's first piece, where all of its pieces are.
 template <int D>
 __device__ __forceinline__ void write_total(const AttendArgs &a, const Piece &p, int i, float most, float total) {
@@ -442,7 +469,7 @@ __device__ __forceinline__ void stage_queries(const AttendArgs &a, const PackedV
 // The groups' sums against the largest of their maxima, added in their order: 32 vectors at a time (what the ring has room for), all threads.
 template <int D, int NT, typename S, int HELD>
 __device__ __forceinline__ void join_groups(const AttendArgs &a, const Piece &p, f32x4 (&acc)[HELD][NT], const float (&most)[NT], float (&total)[NT],
-                                            float *joined, float *wave_most, float *wave_total, int record_group) {
+                                            float *joined, float *wave_most, float *wave_total, int record_group, const int *apart) {
     constexpr int R = S::kRows, GROUPS = S::kGroups, PITCH = S::kPitch;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -452,6 +479,12 @@ __device__ __forceinline__ void join_groups(const AttendArgs &a, const Piece &p,
         if (g == 0) wave_most[record_group * R + n * 16 + col] = most[n], wave_total[record_group * R + n * 16 + col] = total[n];
     }
     __syncthreads();
+    static_assert(GROUPS == 4, "a word of `apart` each");
+    const u32x4 any_apart = *reinterpret_cast<const u32x4 *>(apart);
+    if (__builtin_expect(uniform((int)(any_apart[0] | any_apart[1] | any_apart[2] | any_apart[3])), 0)) {
+        if (tid < R) write_apart<D>(a, p, tid);
+        return;
+    }
 #pragma unroll
     for (int n0 = 0; n0 < NT; n0 += 2) {
         constexpr int MOST = NT > 1 ? 2 : 1;
@@ -480,7 +513,7 @@ __device__ __forceinline__ void join_groups(const AttendArgs &a, const Piece &p,
             for (int w = 0; w < GROUPS; ++w) row_most = __builtin_fmaxf(row_most, wave_most[w * R + row]);
 #pragma unroll
             for (int w = 0; w < GROUPS; ++w) {
-                row_total += wave_total[w * R + row] * __builtin_amdgcn_exp2f(wave_most[w * R + row] - row_most);
+                row_total += scaled(wave_total[w * R + row], wave_most[w * R + row] - row_most);
 #pragma unroll
                 for (int e = 0; e < D / 16; e += 4) {
                     const f32x4 part = *reinterpret_cast<const f32x4 *>(joined + ((k * GROUPS + w) * 16 + i) * PITCH + d + e);
@@ -554,8 +587,8 @@ struct FewShape {
     static constexpr bool kAlone = D / 16 * NT * 4 > 96;
     static constexpr int kGroups = kFewGroups, kThreads = 64 * kGroups, kRows = 16 * NT, kPitch = D + 4;
     static constexpr int kRingBytes = kGroups * 2 * FewRing<D>::kRecord, kQueryBytes = kRows * D * 2;
-    static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions
-    static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 16;
+    static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions, their least, a word a wave
+    static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 32;
     static_assert((NT > 1 ? 2 : 1) * kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
 };
 
@@ -569,7 +602,7 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
     float *const joined = reinterpret_cast<float *>(lds);  // [group][16][PITCH], in the ring's place
     float *const wave_most = reinterpret_cast<float *>(lds + S::kNumbers), *const wave_total = wave_most + GROUPS * R;
     float *const row_factor = wave_total + GROUPS * R;
-    int *const row_position = reinterpret_cast<int *>(row_factor + R), *const least = row_position + R;
+    int *const row_position = reinterpret_cast<int *>(row_factor + R), *const least = row_position + R, *const apart = least + 4;
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int record_group = wave, ring = record_group * 2 * Ring::kRecord;  // where the group's two records lie
 
@@ -612,9 +645,11 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
             most[n] = kLowest, total[n] = 0.0f;
         }
         const int first_position = a.prefix ? uniform(*least) : p.span.first + a.tile.by_group.of(p.tile * R);
+        const int seen_to = tile_end(p.span, a.tile, p.tile);  // (keys that no row of the tile sees were never written)
         f32x4 acc[HELD][NT] = {};
         int buffer = 0;
         bool waited = false, dead = false;
+        float least_scale = 1.0f, most_scale = 1.0f;  // of the lane's key of each record
         // Where a maximum moves by more than kSlack the loop over the records is left, the sums scaled, and the record
         // begun again: inside of it nothing but the matrix instructions touches the sums. (Scaled in a branch of the loop, the compiler holds
         // them twice, and copies 192 registers a record: 150 us for the 320 MB of the verify step.)
@@ -665,6 +700,10 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
                 }
             }
             const bool masked = dead || block * kBlock + kBlock - 1 > first_position;
+            float value_scale = __builtin_fmaxf((scales - 4 * g)[kBlock + (lane & (kBlock - 1))], kLeastScale);
+            asm("" : "+v"(value_scale));  // (read whatever the lane: a branch around it parts what is scheduled together)
+            const float counted = (lane & (kBlock - 1)) < (dead ? 0 : seen_to - block * kBlock) ? value_scale : 1.0f;
+            least_scale = __builtin_fminf(least_scale, counted), most_scale = __builtin_fmaxf(most_scale, counted);
             f16x8 weight[NT];
             float t[NT][8];
 #pragma unroll
@@ -720,14 +759,15 @@ __global__ __launch_bounds__((FewShape<D, NT>::kThreads), (FewShape<D, NT>::kAlo
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float now = __builtin_fmaxf(top[n], most[n]), keep = __builtin_amdgcn_exp2f(most[n] - now);
+                total[n] = scaled(total[n], most[n] - now);
                 most[n] = now;
-                total[n] *= keep;
 #pragma unroll
                 for (int j = 0; j < HELD; ++j) acc[j][n] *= keep;
             }
         }
         }
-        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group);
+        apart[wave] = __any(most_scale > kSmallScale * kFarApart) | (__any(most_scale > kLargeScale) & __any(least_scale < kSmallScale));
+        join_groups<D, NT, S, HELD>(a, p, acc, most, total, joined, wave_most, wave_total, record_group, apart);
     });
 }
 
@@ -741,7 +781,8 @@ struct ManyShape {
     static constexpr int kRecords = 256 / D;
     static constexpr int kPitch = 1024 + 64;  // of a step of keys: spreads a quad's writes over the banks
     static constexpr int kRaw = kRecords * record_bytes(D), kKeys = 2 * kRaw, kValues = kKeys + 3 * 16 * kPitch, kScales = kValues + 4 * 16 * 1024;
-    static constexpr int kThreads = kManyThreads, kLds = kScales + 4 * kRecords * 3 * kBlock * 4;
+    static constexpr int kEnds = kScales + 4 * kRecords * 3 * kBlock * 4;  // the bits of the least and of the largest scale
+    static constexpr int kThreads = kManyThreads, kLds = kEnds + 16;
     static constexpr int kSumPitch = D + 4;
     static_assert(kLds <= 160 * 1024 && 8 * 16 * kSumPitch * 4 <= kLds, "LDS");
 };
@@ -757,6 +798,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
     uint8_t *const key_parts = reinterpret_cast<uint8_t *>(lds + S::kKeys);
     u32x4 *const value_parts = reinterpret_cast<u32x4 *>(lds + S::kValues);
     float *const scales = reinterpret_cast<float *>(lds + S::kScales);
+    uint32_t *const scale_ends = reinterpret_cast<uint32_t *>(lds + S::kEnds);
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, col = lane & 31, g = lane >> 5;
 
     for_pieces<kManyThreads>(a, cache, packed, [&](const Piece &p) {
@@ -818,9 +860,10 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 
         // The wave's part of the records in `buffer` widened to place `third` of the keys or `fourth` of the values and scales, and between that
         // (MULTIPLY) the scores of the keys at place `keys`: the products run while the codes are widened (one after the other, the prompt
-        // chunk took 437 us instead of 426). `dead`: the record whose scales are the wave's is none.
+        // chunk took 437 us instead of 426). `first`: the first of the records' blocks; `dead`: the one whose
+        // scales are the wave's is none.
         f32x16 s[RECORDS];
-        auto widen_and_score = [&](auto values, auto multiply, int buffer, int third, int fourth, int keys, bool dead) {
+        auto widen_and_score = [&](auto values, auto multiply, int first, int buffer, int third, int fourth, int keys, bool dead) {
             constexpr bool VALUES = decltype(values)::value, MULTIPLY = decltype(multiply)::value;
             const char *const raw = lds + buffer * S::kRaw;
             const int lane = lane_anew(), tid = quarter * 64 + lane;
@@ -891,12 +934,17 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
                     float *const at = scales + (fourth * RECORDS + record_at) * 3 * kBlock + lane;
                     at[0] = lane >= kBlock ? __builtin_amdgcn_logf(scale) : dead ? __uint_as_float(kNoRecord) : scale;
                     if (lane >= kBlock) at[kBlock] = inverse_scale(scale);
+                    const uint32_t bits = __float_as_uint(scale);  // (0, and less than 0 as a float, are not looked at either)
+                    if (__builtin_expect(__any((lane >= kBlock) & (bits - kSmallBits > kLargeBits - kSmallBits) & (bits - 1 < 0x7f800000u)), 0)) {
+                        if (!dead & (lane >= kBlock) & (bits - 1 < 0x7f800000u) & ((first + record_at) * kBlock + lane - kBlock < tile_end(p.span, a.tile, p.tile)))
+                            atomicMin(&scale_ends[0], bits), atomicMax(&scale_ends[1], bits);
+                    }
                 }
             }
         };
-        auto part_of_step = [&](auto multiply, int buffer, int third, int fourth, int keys, bool dead) {
-            if (wave < 4) widen_and_score(std::true_type{}, multiply, buffer, third, fourth, keys, dead);
-            else widen_and_score(std::false_type{}, multiply, buffer, third, fourth, keys, dead);
+        auto part_of_step = [&](auto multiply, int first, int buffer, int third, int fourth, int keys, bool dead) {
+            if (wave < 4) widen_and_score(std::true_type{}, multiply, first, buffer, third, fourth, keys, dead);
+            else widen_and_score(std::false_type{}, multiply, first, buffer, third, fourth, keys, dead);
         };
 
         auto weigh_values = [&](int block, int fourth) {
@@ -933,8 +981,8 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             if (__any(top > most + kSlack)) {
                 top = __builtin_fmaxf(top, most);
                 const float keep = __builtin_amdgcn_exp2f(most - top);
+                total = scaled(total, most - top);
                 most = top;
-                total *= keep;
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) acc[j] *= keep;
             }
@@ -987,6 +1035,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         };
 
         lds_barrier();  // (the last piece's LDS is read)
+        if (tid == 0) scale_ends[0] = kSmallBits, scale_ends[1] = kLargeBits;
         bool staged_hole = true;  // of the record that is widened next
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -995,8 +1044,8 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         }
         wait_vmcnt<0>();
         lds_barrier();
-        part_of_step(std::false_type{}, 0, 0, 0, 0, staged_hole);
-        if (from + RECORDS < to) part_of_step(std::false_type{}, 1, 1, 1, 0, hole);
+        part_of_step(std::false_type{}, from, 0, 0, 0, 0, staged_hole);
+        if (from + RECORDS < to) part_of_step(std::false_type{}, from + RECORDS, 1, 1, 1, 0, hole);
         lds_barrier();
         if (from + 2 * RECORDS < to) fetch(from + 2 * RECORDS, 0);
         staged_hole = hole;
@@ -1009,7 +1058,7 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
         for (int block = from; block < to; block += RECORDS, ++step) {
             if (block + 3 * RECORDS < to) fetch(block + 3 * RECORDS, (step + 1) & 1);
             // (Behind the last records something that nothing reads is widened once more.)
-            part_of_step(std::true_type{}, step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3, third, staged_hole);
+            part_of_step(std::true_type{}, block + 2 * RECORDS, step & 1, third == 0 ? 2 : third - 1, (step + 2) & 3, third, staged_hole);
             staged_hole = hole;
             lds_barrier();
             weigh_values(block, step & 3);
@@ -1018,6 +1067,10 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
             lds_barrier();
         }
         if (wave < 4) lds_barrier();
+        if (__builtin_expect(__uint_as_float(uniform((int)scale_ends[0])) < __uint_as_float(uniform((int)scale_ends[1])) / kFarApart, 0)) {
+            if (g == 0) write_apart<D>(a, p, wave * 32 + col);
+            return;
+        }
         total += __shfl_xor(total, 32);
         // The wave's sums go through its eighth of the LDS, sixteen vectors at a time, and out in whole rows: as the lanes have them, 16 bytes
         // of 32 rows at once, 256 vectors of 256 dimensions took 9.7 us.
@@ -1068,8 +1121,79 @@ __global__ __launch_bounds__(kManyThreads) void many_kernel(AttendArgs a, CacheV
 // LANES lanes a (row, query head): the weights of its pieces, one a lane, and their sums in the order of the keys, BATCH pieces'
 // loads at a time. All 64 where there are few vectors, of many pieces each: what it takes is then three loads one after the other.
 // Sixteen where there are many: four vectors' loads are under way in a wave at once.
+//
+// A vector whose scales lie far apart: its keys, LANES at a time, a lane a key for the scores and a lane E dimensions for the sums, with a maximum of the
+// scores of its own for what is divided by. (Eight requests of 4096 tokens with 24 heads of 256 on 4: 768 us, 30 where nothing is left to this; 1024 rows on
+// 1024 before them: 3.4 ms, 105.)
 template <int D, int LANES>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs prefix, PackedView packed) {
+__device__ __forceinline__ void apart_vector(const AttendArgs &a, const CacheView &cache, const PackedView &packed, int row, int h, float (&o)[D / LANES], float &total) {
+    constexpr int E = D / LANES;
+    struct alignas(E) Codes {
+        uint8_t of[E];
+    };
+    const int lane = threadIdx.x % LANES;
+    int request = 0;  // the last that starts at or before the row
+    for (int step = 1 << 16; step; step >>= 1)
+        if (request + step < packed.requests && packed.starts[request + step] <= row) request += step;
+    const Span span = own_span(packed, cache.page_tokens, 0, request);
+    const int end = min(span.first + row - span.begin + 1, span.to), head = h / a.tile.group;
+    const uint16_t *const q = a.q + row * a.row_stride + h * a.head_stride;
+    float largest = 0.0f;
+    for (int d = 0; d < D; d += 8) largest = __builtin_fmaxf(largest, largest8(load_q8(q + d, a.wide)));
+    const int power = power_of(largest);
+    const float factor = __builtin_ldexpf(a.factor, -power);
+    float most = kLowest, top = kLowest;  // of the weights' exponents, of the scores
+    total = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    for (int first = 0; first < end; first += LANES) {
+        const int key = first + lane;
+        const uint8_t *record = nullptr;  // of the lane's key, where it has one
+        int page, at, token = 0;
+        if (key < end && place_of(cache, packed, key < a.shared ? 0 : request, key, page, at)) record = record_of<D>(cache, page, head, at / kBlock), token = at % kBlock;
+        float score = -__builtin_inff(), t = score;
+        if (record) {
+            float s = 0.0f;
+#pragma unroll 4
+            for (int d = 0; d < D; d += 8) {
+                const u32x4 x = load_q8(q + d, a.wide);
+                const u32x2 k = *reinterpret_cast<const u32x2 *>(record + token * D + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float v = e % 2 ? __uint_as_float(x[e / 2] & 0xffff0000u) : bf16_bits_to_f32(x[e / 2]);
+                    s += __builtin_ldexpf(v, power) * (float)((int)(k[e / 4] >> 8 * (e % 4) & 0xff) - 128);
+                }
+            }
+            const float *const scales = reinterpret_cast<const float *>(record + 2 * kBlock * D) + token;
+            score = s * (scales[0] * factor);
+            t = score + __builtin_amdgcn_logf(scales[kBlock]);
+        }
+        float now = __builtin_fmaxf(most, t), now_top = __builtin_fmaxf(top, score);
+#pragma unroll
+        for (int m = 1; m < LANES; m <<= 1) now = __builtin_fmaxf(now, __shfl_xor(now, m)), now_top = __builtin_fmaxf(now_top, __shfl_xor(now_top, m));
+        const float keep = __builtin_amdgcn_exp2f(most - now), weight = __builtin_amdgcn_exp2f(t - now);
+        float sum = __builtin_amdgcn_exp2f(score - now_top);
+#pragma unroll
+        for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor(sum, m);
+        total = total * __builtin_amdgcn_exp2f(top - now_top) + sum;
+        most = now, top = now_top;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= keep;
+        // The values of each key in turn, from where that key's lane found them. (Where it found none its weight is 0.)
+        const int64_t where = reinterpret_cast<int64_t>(record ? record + (kBlock + token) * D : cache.data);
+#pragma unroll 4
+        for (int j = 0; j < LANES; ++j) {
+            const Codes codes = reinterpret_cast<const Codes *>(__shfl(where, j, LANES))[lane];
+            const float w = __shfl(weight, j, LANES);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += w * (float)((int)codes.of[e] - 128);
+        }
+    }
+    total = scaled(total, top - most);  // (against the same maximum as the sums)
+}
+
+template <int D, int LANES>
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs prefix, CacheView cache, PackedView packed) {
     constexpr int E = D / LANES, BATCH = LANES == 64 ? 16 : 64 / E < 4 ? 64 / E : 4;
     typedef float Sums __attribute__((ext_vector_type(E == 1 ? 2 : E < 4 ? E : 4)));
     const int64_t vector = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
@@ -1079,6 +1203,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
     const Pieces mine = own.pieces[vector], theirs = prefix.pieces[vector];
     if (row >= end | row < begin | (mine.count == 1 && !own.partial)) return;
     float top = kLowest, total = 0.0f, o[E] = {};
+    bool apart = mine.count < 0;
     auto join = [&](const AttendArgs &l, const Pieces &p) {
         const int rows = l.tile.rows, last = (int)l.first_slots + l.tile.workgroups;
         const int64_t size = rows * (int64_t)(D + 2);
@@ -1092,6 +1217,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
                 const float *at = slot(j) + (int64_t)rows * D + p.at;
                 most = at[0], sum = at[rows];
             }
+            const uint64_t marked = __ballot(sum == kApart);
+            if (__builtin_expect(marked != 0, 0)) apart |= (marked >> (threadIdx.x & 63 & ~(LANES - 1)) & (~0ull >> (64 - LANES))) != 0;
             float part[BATCH][E];
             auto load = [&](int first) {
 #pragma unroll
@@ -1114,11 +1241,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
 #pragma unroll
             for (int m = 1; m < LANES; m <<= 1) now = __builtin_fmaxf(now, __shfl_xor(now, m));
             const float keep = __builtin_amdgcn_exp2f(top - now), weight = __builtin_amdgcn_exp2f(most - now);
+            sum = scaled(sum, most - now), total = scaled(total, top - now);
             top = now;
-            sum *= weight;
 #pragma unroll
             for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor(sum, m);
-            total = total * keep + sum;
+            total += sum;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] *= keep;
             for (int first = 0; first < here; first += BATCH) {
@@ -1134,6 +1261,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs pr
     };
     if (own.partial) join(prefix, theirs);
     join(own, mine);
+    if (__builtin_expect(apart, 0)) apart_vector<D, LANES>(own, cache, packed, row, h, o, total);
     uint16_t *at = own.out + row * own.ld_out + (int64_t)h * D + lane * E;
     const float inv = 1.0f / total;
     if constexpr (E >= 4) {
@@ -1257,9 +1385,9 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
         if (shared > 0) launch_part<D>(prefix, b, cv, pv, stream);
         launch_part<D>(own, a, cv, pv, stream);
         if (rows * q_heads <= kJoinApart)  // a workgroup each, so that they spread over the CUs
-            join_kernel<D, 64><<<(unsigned)(rows * q_heads), 64, 0, stream>>>(a, b, pv);
+            join_kernel<D, 64><<<(unsigned)(rows * q_heads), 64, 0, stream>>>(a, b, cv, pv);
         else
-            join_kernel<D, 16><<<(unsigned)((rows * q_heads + 15) / 16), 256, 0, stream>>>(a, b, pv);
+            join_kernel<D, 16><<<(unsigned)((rows * q_heads + 15) / 16), 256, 0, stream>>>(a, b, cv, pv);
     };
     if (cache.dim == 256) run(std::integral_constant<int, 256>{});
     else if (cache.dim == 128) run(std::integral_constant<int, 128>{});

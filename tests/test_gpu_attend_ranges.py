@@ -1,0 +1,58 @@
+"""splosh_attend at the ends of its numbers: values whose sizes lie as far apart as the cache can hold them."""
+import pytest
+import torch
+
+from test_gpu_attend import Step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def rt():
+    from splosh_amd import runtime
+    return runtime
+
+
+# few vectors and many, one record, one wave's and all waves', a segment cut over workgroups, each kind of join, and a shared prefix
+SHAPES = [([1], [2], 1, 1, 64, 32, 0), ([1, 3], [70, 300], 2, 1, 128, 32, 0), ([1], [1500], 3, 1, 256, 96, 0), ([20], [700], 2, 1, 64, 64, 0), ([2, 2], [3000, 40], 6, 2, 128, 32, 0),
+          ([4] * 150, [40] * 150, 8, 2, 128, 32, 0), ([600], [640], 8, 1, 64, 64, 0), ([700], [800], 6, 1, 256, 32, 0),
+          ([90], [200], 1, 1, 256, 32, 0), ([100, 80], [1000, 80], 2, 1, 128, 32, 0), ([300], [400], 1, 1, 64, 96, 0), ([700], [900], 8, 1, 128, 64, 0),
+          ([1, 2, 1], [300, 220, 290], 4, 2, 128, 32, 192), ([40, 60], [300, 700], 2, 1, 256, 32, 256), ([50, 70], [230, 200], 2, 1, 64, 96, 96)]
+
+
+@pytest.mark.parametrize("order", ["by turns", "small first", "large first", "one small"])
+@pytest.mark.parametrize("small,large", [(0.0, 1e10), (0.0, 1e30), (0.0, 3e38), (1e-27, 1e4), (1e-20, 1e25)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_values_of_any_size(rt, shape, small, large, order):
+    """Every key has its weight, whatever the size of its value: a value of zeros beside one of 1e30 leaves half of it, in one record,
+    in two, in two pieces and in a prefix and behind it.
+
+    The bound is step_check's: an exponent is a logarithm of a scale (up to 2^7, 2^-17 for its last place) and two roundings of sums of that
+    size (2^-18 each), 2^-16 in all, beside the weights' 2^-11 and the output's 2^-8."""
+    runs, lengths, q_heads, heads, dim, page, shared = shape
+    s = Step(rt, runs, lengths, q_heads, heads, dim, page, seed=dim + len(order), shared=shared)
+    unit = s.v.double() / s.v.double().abs().amax(-1, keepdim=True)
+    for r, length in enumerate(lengths):
+        i = torch.arange(length)
+        slots = s.table[r].long()[i // page] * page + i % page
+        pick = {"by turns": i % 2 == 1, "small first": i >= length // 2, "large first": i < length // 2, "one small": i != length // 3}[order]
+        size = torch.where(pick, large, small).double()
+        s.v[slots] = (unit[slots] * size[:, None, None]).to(torch.bfloat16)
+    s.fill()
+    s.check(s.run(scale=0.01), 0.01)
+
+
+@pytest.mark.parametrize("runs,lengths,shared", [([1, 2], [40, 9], 0), ([8], [900], 0), ([300], [420], 0), ([40, 30], [140, 200], 128)])
+def test_in_place_and_again(rt, runs, lengths, shared):
+    """Values far apart with the output in its queries' place, in a workspace of garbage, and behind a key that only later rows see."""
+    s = Step(rt, runs, lengths, 4, 2, 128, 32, seed=2, shared=shared)
+    s.v[::2] = 0
+    for r, length in enumerate(lengths):
+        s.v[int(s.table[r, (length - 1) // 32]) * 32 + (length - 1) % 32] = 1e30
+    s.fill()
+    want = s.run()
+    s.check(want)
+    ws = torch.full((rt.attend_workspace_bytes(s.cache, s.packed, s.rows, 4, shared),), 0xff, dtype=torch.uint8, device="cuda")
+    assert torch.equal(s.run(workspace=ws), want)
+    got = rt.attend(s.q_gpu, s.cache, s.packed, shared=shared, out=s.q_gpu, workspace=ws)
+    assert torch.equal(got, want)
