@@ -499,8 +499,8 @@ int splosh_sample(const void *logits, int64_t ld, int dtype, int64_t rows, int64
  *
  * How a step is packed: row m belongs to request r where starts[r] <= m < starts[r + 1] (starts[0] = 0,
  * ascending; a request may have no row), and stands for that request's token at position
- * lengths[r] - starts[r + 1] + m: lengths[r] counts the request's tokens in the cache once the step's own
- * are in it. Position p of request r lies at place p % page_tokens of page table[r table_stride +
+ * lengths[r] - min(starts[r + 1], rows) + m: lengths[r] counts the request's tokens in the cache once the
+ * step's own are in it. Position p of request r lies at place p % page_tokens of page table[r table_stride +
  * p / page_tokens]. All three are device arrays that a kernel reads when it runs, so a captured call may
  * find others at each replay. Rows from starts[requests] on belong to no request: what they would
  * write is left as it was. A row with a negative position, or one past the table, has no place in the

@@ -197,7 +197,7 @@ __device__ __forceinline__ int position_of(const AttendArgs &a, const PackedView
         if (packed.starts[mid] <= row) low = mid;
         else high = mid;
     }
-    return packed.lengths[low] - packed.starts[low + 1] + row;
+    return position_in(packed, low, row);
 }
 
 // The page ids of a request, 64 columns at a time in a wave's lanes.

@@ -49,6 +49,14 @@ __device__ __forceinline__ int request_of(const int32_t *starts, int requests, i
     return r < requests ? r : -1;
 }
 
+// The position of packed row `row`, one of request `request`'s: starts past the step's rows count as those, as everywhere (and those below 0: this one's
+// end is past the row), and a position below 32 bits is as good as their least.
+__host__ __device__ __forceinline__ int position_in(const PackedView &p, int request, int row) {
+    const int end = p.starts[request + 1] < p.rows ? p.starts[request + 1] : p.rows;
+    const int64_t position = (int64_t)p.lengths[request] - end + row;
+    return position < INT32_MIN ? INT32_MIN : (int)position;
+}
+
 // Where token `position` of request `request` lies: its page's id and its place there; false where it has none.
 __host__ __device__ __forceinline__ bool place_of(const CacheView &c, const PackedView &p, int request, int position, int &page, int &at) {
     if (request < 0 || position < 0) return false;

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, CacheVi
     if (kCache) {
         const int r = request_of(packed.starts, packed.requests, row);
         if (r < 0) return;  // (the same for the whole workgroup)
-        position = packed.lengths[r] - packed.starts[r + 1] + row;
+        position = position_in(packed, r, row);
         placed = place_of(cache, packed, r, position, page, at);
     } else {
         position = a.positions ? a.positions[row] : 0;
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kHeadThreads) void cache_read_kernel(ReadArgs a, Ca
     const int r = request_of(packed.starts, packed.requests, row);
     if (r < 0) return;
     int page = 0, at = 0;
-    const bool placed = place_of(cache, packed, r, packed.lengths[r] - packed.starts[r + 1] + row, page, at);
+    const bool placed = place_of(cache, packed, r, position_in(packed, r, row), page, at);
     if (head >= cache.heads) return;
     struct alignas(E) Codes {
         uint8_t of[E];
