@@ -354,7 +354,9 @@ __global__ __launch_bounds__(64) void finish_kernel(VerifyArgs a) {
     const int drafted = d.last ? -1 : a.tokens[d.row + 1];
     const double rests = wave_running(rest), wholes = wave_running(whole);
     const bool from_rest = __shfl(rests, 63) > 0.0;
-    const double total = from_rest ? __shfl(rests, 63) : __shfl(wholes, 63), draw = u * total;
+    const double total = from_rest ? __shfl(rests, 63) : __shfl(wholes, 63);
+    // (u >= 1 is past the whole weight. The product would be the sum in one order, which sums in the others' orders pass before the last entry.)
+    const double draw = u < 1.0 ? u * total : __builtin_inf();
     // The lane that the draw falls into: the first whose running weight passes it, or, if none does, the last with weight.
     auto lane_of = [&](double own, double running) {
         const uint64_t passed = __ballot(own > 0.0 && running > draw), with = __ballot(own > 0.0);
