@@ -36,7 +36,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr size_t kAttendCounterBytes = 16384;  // the workspace's first bytes belong to other kernels' counters
-constexpr float kLowest = -1e30f;              // M before the first key
+constexpr float kLowest = -0x1.fffffep+127f;   // M before the first key: no finite t is lower
 constexpr float kSlack = 8.0f;                 // how far t may pass M before M follows
 constexpr int kManyThreads = 512, kManyRows = 256;
 // (Row, query head) vectors that are joined a wave each; more, sixteen lanes each. (1536 of some 35 pieces: 14 us, sixteen lanes 19; 49152 of two

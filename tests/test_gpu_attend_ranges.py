@@ -1,7 +1,9 @@
-"""splosh_attend at the ends of its numbers: values whose sizes lie as far apart as the cache can hold them."""
+"""splosh_attend at the ends of its numbers: values whose sizes lie as far apart as the cache can hold them, and scores near the ends of
+fp32."""
 import pytest
 import torch
 
+from step_check import HALF
 from test_gpu_attend import Step
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +58,32 @@ def test_in_place_and_again(rt, runs, lengths, shared):
     assert torch.equal(s.run(workspace=ws), want)
     got = rt.attend(s.q_gpu, s.cache, s.packed, shared=shared, out=s.q_gpu, workspace=ws)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("runs,lengths,dim", [([3], [40], 64), ([2], [900], 128), ([1, 2], [300, 33], 256), ([80], [200], 64), ([90], [130], 128), ([150], [700], 256)])
+def test_scores_of_any_size(rt, runs, lengths, dim):
+    """Scores far below -1e30 and above 1e30: all of a row's weight is at its largest score, and the row is that key's value, to the rounding of
+    its scale's reciprocal (2^-22) and the output's."""
+    for sign in (-1.0, 1.0):
+        s = Step(rt, runs, lengths, 2, 2, dim, 32, seed=3)
+        s.q[:] = 1e17
+        s.q_gpu.copy_(s.q)
+        want = []
+        for r, length in enumerate(lengths):
+            i = torch.arange(length)
+            slots = s.table[r].long()[i // 32] * 32 + i % 32
+            # (The largest score is that of the row's first key or of its last one.)
+            s.k[slots] = (sign * 1e17 * (1 + i / 64.0)).to(torch.bfloat16)[:, None, None].expand(-1, 2, dim)
+            for m in range(runs[r]):
+                want.append(int(slots[length - runs[r] + m if sign > 0 else 0]))
+        s.fill()
+        k = s.k64[torch.tensor(want)][:, :, 0]
+        assert bool((k.abs() * 1e17 * dim * dim ** -0.5 > 1e34).all())
+        got = s.run().cpu().double()
+        for m, slot in enumerate(want):
+            if sign > 0:  # (bf16 keys: neighbours of the last one may be equal to it)
+                same = (s.k64[:, :, 0] == s.k64[slot, :, 0]).all(1).nonzero()[:, 0]
+                if len(same) > 1:
+                    continue
+            v = s.v64[slot]
+            assert bool(((got[m] - v).abs() <= v.abs() * (HALF + 2.0 ** -20)).all()), (sign, m)
