@@ -1196,9 +1196,9 @@ template <int D, int LANES>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs own, AttendArgs prefix, CacheView cache, PackedView packed) {
     constexpr int E = D / LANES, BATCH = LANES == 64 ? 16 : 64 / E < 4 ? 64 / E : 4;
     typedef float Sums __attribute__((ext_vector_type(E == 1 ? 2 : E < 4 ? E : 4)));
-    const int64_t vector = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+    const int64_t vector = (long_block() * blockDim.x + threadIdx.x) / LANES;
+    if (vector >= (int64_t)packed.rows * own.q_heads) return;
     const int lane = threadIdx.x % LANES, row = (int)(vector / own.q_heads), h = (int)(vector % own.q_heads);
-    if (row >= packed.rows) return;
     const int begin = packed.starts[0], end = packed.starts[packed.requests];  // (all four loads at once)
     const Pieces mine = own.pieces[vector], theirs = prefix.pieces[vector];
     if (row >= end | row < begin | (mine.count == 1 && !own.partial)) return;
@@ -1387,7 +1387,7 @@ hipError_t launch_attend(const uint16_t *q, int64_t row_stride, int64_t head_str
         if (rows * q_heads <= kJoinApart)  // a workgroup each, so that they spread over the CUs
             join_kernel<D, 64><<<(unsigned)(rows * q_heads), 64, 0, stream>>>(a, b, cv, pv);
         else
-            join_kernel<D, 16><<<(unsigned)((rows * q_heads + 15) / 16), 256, 0, stream>>>(a, b, cv, pv);
+            join_kernel<D, 16><<<long_grid((rows * q_heads + 15) / 16), 256, 0, stream>>>(a, b, cv, pv);
     };
     if (cache.dim == 256) run(std::integral_constant<int, 256>{});
     else if (cache.dim == 128) run(std::integral_constant<int, 128>{});

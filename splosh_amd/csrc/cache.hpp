@@ -11,6 +11,14 @@ namespace splosh {
 constexpr int kBlock = 32;  // tokens of a record
 constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
 
+// A launch has at most 2^32 threads a dimension: this many workgroups of 256 go along x, and more of them in rows of so many along y.
+constexpr int kGridLog = 22;
+inline dim3 long_grid(int64_t workgroups) {
+    const int64_t row = (int64_t)1 << kGridLog;
+    return workgroups <= row ? dim3((unsigned)workgroups) : dim3((unsigned)row, (unsigned)((workgroups + row - 1) / row));
+}
+__device__ __forceinline__ int64_t long_block() { return (int64_t)blockIdx.y << kGridLog | blockIdx.x; }
+
 // A record: codes of 32 keys, of 32 values, their scales; a code is kept as the byte code + 128, which takes one instruction less to
 // widen than a signed one. Rows of codes are whole vectors, so that a token is written
 // and read back in runs of `dim` bytes, and a matrix instruction's operand is a run of a row (keys: 16 bytes

@@ -266,10 +266,10 @@ template <int D>
 __global__ __launch_bounds__(kHeadThreads) void cache_read_kernel(ReadArgs a, CacheView cache, PackedView packed) {
     constexpr int E = D / kLanes;
     const int units = (cache.heads + kVectors - 1) / kVectors;
-    const int64_t item = (int64_t)blockIdx.x * kHeadWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t item = long_block() * kHeadWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (item >= (int64_t)packed.rows * units) return;
     const int row = (int)(item / units), lane = threadIdx.x & 63;
     const int head = (int)(item % units) * kVectors + lane / kLanes, first = lane % kLanes * E;
-    if (row >= packed.rows) return;
     const int r = request_of(packed.starts, packed.requests, row);
     if (r < 0) return;
     int page = 0, at = 0;
@@ -368,7 +368,7 @@ hipError_t launch_cache_read(const splosh_cache &cache, const splosh_packed &pac
     const ReadArgs a{{k, v}, {ldk, ldv}, {fits(k, ldk, 2, bytes), fits(v, ldv, 2, bytes)}};
     auto go = [&](auto kernel) {
         const int64_t items = rows * ((cache.heads + kVectors - 1) / kVectors);
-        kernel<<<(unsigned)((items + kHeadWaves - 1) / kHeadWaves), kHeadThreads, 0, stream>>>(a, view_of(cache), view_of(packed, rows));
+        kernel<<<long_grid((items + kHeadWaves - 1) / kHeadWaves), kHeadThreads, 0, stream>>>(a, view_of(cache), view_of(packed, rows));
     };
     if (cache.dim == 256) go(cache_read_kernel<256>);
     else if (cache.dim == 128) go(cache_read_kernel<128>);
