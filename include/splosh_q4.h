@@ -582,6 +582,7 @@ size_t splosh_attend_workspace_bytes(const splosh_cache *cache, const splosh_pac
  * that head h / (q_heads / cache->heads) keeps for row m's request; all that lengths counts has to be written before, the
  * step's own too (splosh_cache_write). q: bf16, vector (m, h) at q + m row_stride + h head_stride; out: bf16, dense rows of q_heads dim
  * values, row stride ld_out. A row that sees no key gets zeros.
+ * Where starts do not ascend, what a request's rows get is not defined (nothing else is written).
  * shared: the first `shared` tokens (a multiple of page_tokens, 0: none) are the same for all requests of the call: they
  * are read through the pages of request 0, once for all rows; the table's entries of other requests for
  * them are not used. Scores and sums are fp32; q's values enter the first product in fp16 after a power of two that leaves them

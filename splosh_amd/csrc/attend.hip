@@ -327,13 +327,16 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
             return tile.heads * units_before(s, tile, tiles);
         };
         int units = 0, segments = 0, n;
-        for (int r = low; r < high; ++r) units += units_of(r, n), segments += n;
+        bool ascending = true;
+        for (int r = low; r < high; ++r) units += units_of(r, n), segments += n, ascending &= ascends(packed, r);
         int units_to = running_sum(units), segments_to = running_sum(segments);
-        if (lane == 63) wave_units[wave] = units_to, wave_segments[wave] = segments_to;
+        const bool sound = __all(ascending);
+        if (lane == 63) wave_units[wave] = sound ? units_to : -1, wave_segments[wave] = segments_to;
         if (tid == 0) found[0] = -1;
         __syncthreads();
         total = 0;
         for (int i = 0; i < THREADS / 64; ++i) {
+            if (wave_units[i] < 0) return;  // (starts that do not ascend: nothing is computed)
             if (i < wave) units_to += wave_units[i], segments_to += wave_segments[i];
             total += wave_units[i];
         }
