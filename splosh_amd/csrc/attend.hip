@@ -365,20 +365,13 @@ __device__ __forceinline__ void for_pieces(const AttendArgs &a, const CacheView 
     int t = wave_tile(span, tile, tiles, offset);
     segment += head * tiles + t;
     while (true) {
-        const int units = tile_units(span, tile, t), take = min(units - offset, end - unit);
-        const int keys = tile_end(span, tile, t) - span.from, blocks = keys > 0 ? (keys + kBlock - 1) / kBlock : 0;
-        const int per = tile.keys / kBlock;
-        const bool first = offset <= tile.extra;  // (who has nothing but units before the keys leaves the segment to the next one)
+        const Cut cut = cut_of(span, tile, t, segment, offset, unit, end, w, sharers, total, a.partial, a.first_slots);
         Piece p;
         p.span = span, p.request = request, p.head = head, p.tile = t;
-        p.first_block = max(0, offset - tile.extra) * per;
-        p.blocks = max(0, min((offset + take - tile.extra) * per, blocks) - p.first_block);
-        p.slot = !first ? (int)a.first_slots + w : a.partial ? segment : w;
-        p.count = !first ? 0 : offset + take == units ? 1 : owner_of(total, sharers, unit + units - offset - 1) - w + 1;
-        p.direct = !a.partial && first && offset + take == units;
+        p.first_block = cut.first_block, p.blocks = cut.blocks, p.slot = cut.slot, p.count = cut.count, p.direct = cut.direct;
         // (More segments than slots for them there are only where starts do not ascend.)
-        if (offset + take > tile.extra && (!a.partial || segment < a.first_slots)) work(p);
-        unit += take;
+        if (cut.any && (!a.partial || segment < a.first_slots)) work(p);
+        unit += cut.take;
         if (unit >= end) return;
         offset = 0, ++segment;
         if (++t < tiles) continue;

@@ -96,6 +96,30 @@ __host__ __device__ __forceinline__ int owner_of(int total, int workgroups, int 
     return (int)(((double)(u + 1) * workgroups - 1.0) / total);
 }
 
+// What workgroup w of `sharers` takes of a segment from unit `offset` on, which is unit `unit` of the launch's `total`.
+struct Cut {
+    int take;                 // units
+    bool any;                 // whether it has keys, or all there is of a segment without: who has nothing but units before the keys leaves the segment to the next
+    int first_block, blocks;  // of 32 keys, from the span's first on
+    int slot, count;          // where partial results go; of the segment's first piece, how many workgroups have one
+    bool direct;              // the whole segment, and nothing to join it with
+};
+__host__ __device__ __forceinline__ Cut cut_of(const Span &s, const TileShape &t, int i, int segment, int offset, int unit, int end, int w, int sharers, int total,
+                                               bool partial, int64_t first_slots) {
+    const int units = tile_units(s, t, i), keys = tile_end(s, t, i) - s.from;
+    const int blocks = keys > 0 ? (keys + kBlock - 1) / kBlock : 0, per = t.keys / kBlock;
+    Cut c;
+    c.take = units - offset < end - unit ? units - offset : end - unit;
+    c.any = offset + c.take > t.extra;
+    const bool first = offset <= t.extra, whole = offset + c.take == units;
+    const int from = offset > t.extra ? (offset - t.extra) * per : 0, to = (offset + c.take - t.extra) * per < blocks ? (offset + c.take - t.extra) * per : blocks;
+    c.first_block = from, c.blocks = to > from ? to - from : 0;
+    c.slot = !first ? (int)first_slots + w : partial ? segment : w;
+    c.count = !first ? 0 : whole ? 1 : owner_of(total, sharers, unit + units - offset - 1) - w + 1;
+    c.direct = !partial && first && whole;
+    return c;
+}
+
 // The most segments that a step of so many requests and rows can have.
 __host__ __device__ __forceinline__ int64_t most_segments(int64_t requests, int64_t rows, int64_t q_heads, int64_t heads, int tile_rows) {
     return heads * ((requests < rows ? requests : rows) + rows * (q_heads / heads) / tile_rows);
