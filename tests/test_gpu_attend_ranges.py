@@ -3,7 +3,7 @@ fp32."""
 import pytest
 import torch
 
-from step_check import HALF
+from step_check import HALF, attended, check_bf16
 from test_gpu_attend import Step
 
 pytestmark = pytest.mark.gpu
@@ -58,6 +58,42 @@ def test_in_place_and_again(rt, runs, lengths, shared):
     assert torch.equal(s.run(workspace=ws), want)
     got = rt.attend(s.q_gpu, s.cache, s.packed, shared=shared, out=s.q_gpu, workspace=ws)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows,length,dim,page", [(3, 700, 128, 32), (100, 700, 64, 32), (90, 500, 256, 64), (1000, 1100, 64, 32)])
+@pytest.mark.parametrize("layout", ["dense", "gated"])
+def test_far_apart_between_holes(rt, rows, length, dim, page, layout):
+    """Values far apart with pages that are none between them, keys that are NaN behind all rows but the last, a table shorter than the length, and queries
+    and outputs that are not aligned."""
+    s = Step(rt, [rows], [length], 8, 2, dim, page, seed=15, layout=layout)
+    columns = -(-length // page)
+    none = sorted({0, 2, 3, columns - 3})
+    for i, column in enumerate(none):
+        s.packed.table[0, column] = (-1, s.pages, -(2 ** 31), 2 ** 31 - 1)[i]
+    i = torch.arange(length)
+    all_slots = s.table[0].long()[i // page] * page + i % page
+    s.v[all_slots[::3]] = 0
+    s.v[all_slots[1::5]] *= 1e12
+    last = int(all_slots[-1])
+    s.k[last] = float("nan")
+    s.fill()
+    seen = torch.tensor([j // page not in none for j in range(length)])
+    seen[-1] = False
+    slots = all_slots[seen]
+    position = seen.long().cumsum(0)[length - rows + torch.arange(rows)] - 1
+    out, off = attended(s.q, s.k64[slots], s.v64[slots], position, 0.01)
+    got = s.run(scale=0.01)
+    check_bf16(got[:-1].cpu(), out[:-1], off[:-1])
+    assert torch.isnan(got[-1]).all()
+    # One element off: no vector of q, and no row of the output, is where wide loads and stores could take it.
+    wide = torch.zeros(rows, 8 * dim + 3, dtype=torch.bfloat16, device="cuda")
+    q = wide[:, 1 : 1 + 8 * dim].unflatten(1, (8, dim))
+    q.copy_(s.q_gpu)
+    held = torch.full((rows, 8 * dim + 3), 9.0, dtype=torch.bfloat16, device="cuda")
+    rt.attend(q, s.cache, s.packed, scale=0.01, out=held[:, 1 : 1 + 8 * dim].unflatten(1, (8, dim)))
+    same = held[:, 1 : 1 + 8 * dim].unflatten(1, (8, dim))
+    assert torch.equal(same[:-1], got[:-1]) and torch.isnan(same[-1]).all()
+    assert bool((held[:, :1] == 9).all()) and bool((held[:, 1 + 8 * dim :] == 9).all())
 
 
 @pytest.mark.parametrize("runs,lengths,dim", [([3], [40], 64), ([2], [900], 128), ([1, 2], [300, 33], 256), ([80], [200], 64), ([90], [130], 128), ([150], [700], 256)])
