@@ -540,7 +540,7 @@ size_t splosh_cache_page_bytes(int64_t heads, int64_t dim, int64_t page_tokens);
 /* The heads of one projection: vector (row m, head h) of `dim` elements at x + m row_stride + h
  * head_stride (elements of the call's dtype), so that queries may lie beside their gates. weight: bf16
  * [dim], the norm's; NULL: no norm. out: bf16, dense rows of heads dim values, row stride ld_out;
- * it may be x itself where x is bf16 with the same strides. */
+ * it may be x itself where x is bf16 with the same strides (refused with others). */
 typedef struct splosh_heads {
     const void *x;
     int64_t row_stride;

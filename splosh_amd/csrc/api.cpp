@@ -1326,6 +1326,9 @@ int check_heads(const splosh_heads &h, int dtype, int64_t rows, int64_t dim, boo
         return fail(SPLOSH_ERR_ARITHMETIC_OVERFLOW, "heads: size overflows");
     if (!aligned(h.x, dtype == SPLOSH_F32 ? 4 : 2) || !aligned(h.weight, 2) || !aligned(h.out, 2))
         return fail(SPLOSH_ERR_UNSUPPORTED, "heads are not aligned to their elements");
+    // In place, a vector is read and written by the same threads only where both lie alike.
+    if (written && h.x == h.out && (dtype != SPLOSH_BF16 || (rows > 1 && h.ld_out != h.row_stride) || (h.heads > 1 && h.head_stride != dim)))
+        return fail(SPLOSH_ERR_LAYOUT_MISMATCH, "an output in its input's place must be bf16 with the same strides");
     return SPLOSH_OK;
 }
 

@@ -587,6 +587,8 @@ struct FewShape {
     static constexpr int kNumbers = kRingBytes + kQueryBytes;  // then: maxima and sums of each group, factors, positions, their least, a word a wave
     static constexpr int kLds = kNumbers + (2 * kGroups + 2) * kRows * 4 + 32;
     static_assert((NT > 1 ? 2 : 1) * kGroups * 16 * kPitch * 4 <= kRingBytes && kLds <= 160 * 1024, "LDS");
+    // (LDS is given out in pieces of 1280 bytes; 48 are for_pieces' own.)
+    static_assert(D == 256 || kAlone || 2 * ((kLds + 48 + 1279) / 1280 * 1280) <= 160 * 1024, "two workgroups a CU");
 };
 
 template <int D, int NT>
