@@ -61,9 +61,12 @@ __host__ __device__ __forceinline__ Span prefix_span(const PackedView &p, int sh
     return {0, end < 0 ? 0 : end > p.rows ? p.rows : end, shared, 0, shared};
 }
 
-// Whether a request ends where it begins or later. Where all do, no row is two requests', and the units of all of them are what the host has
+// Whether a request ends where it begins or later, with starts past the step's rows as those. Where all do, no row is two requests', and the units of all of them are what the host has
 // found to fit into 32 bits; where one does not, they can be many times that, and with sums that wrap two requests can have the same unit.
-__host__ __device__ __forceinline__ bool ascends(const PackedView &p, int request) { return p.starts[request] <= p.starts[request + 1]; }
+__host__ __device__ __forceinline__ bool ascends(const PackedView &p, int request) {
+    const int begin = p.starts[request], end = p.starts[request + 1];
+    return begin <= end || begin <= 0 || end >= p.rows;
+}
 
 __host__ __device__ __forceinline__ int tiles_of(const Span &s, const TileShape &t) { return t.by_rows.of(s.n * t.group + t.rows - 1); }
 

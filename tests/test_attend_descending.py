@@ -15,9 +15,9 @@ int main() {
     // 4096 requests of up to 4096 rows and 32768 tokens, four key/value heads of six queries each, tiles of 16 and units of 128 keys.
     const int requests = 4096, rows = 4096, page = 256, pages = 128;
     const TileShape t = tile_shape(16, 128, 3, 6, 4, 256);
-    for (int down = 0; down < 2; ++down) {
+    for (int down = 0; down < 3; ++down) {
         std::vector<int32_t> starts(requests + 1), lengths(requests, page * pages);
-        for (int r = 0; r <= requests; ++r) starts[r] = down ? (r % 2 ? rows : 0) : r;
+        for (int r = 0; r <= requests; ++r) starts[r] = down == 1 ? (r % 2 ? rows : 0) : down == 2 ? (r < 9 ? -r : r < 99 ? r : 3 * rows - r) : r;
         const PackedView p{starts.data(), lengths.data(), nullptr, pages, pages, requests, rows};
         int64_t total = 0;
         bool sound = true;
@@ -40,6 +40,7 @@ def test_units_of_descending_starts(tmp_path):
     source.write_text(PROGRAM)
     subprocess.run([wc.HIPCC, "-x", "hip", "--offload-arch=gfx950", "-O1", "-std=c++17", f"-I{wc.ROOT / 'include'}", f"-I{wc.ROOT / 'splosh_amd/csrc'}",
                     str(source), "-o", str(program)], check=True, capture_output=True)
-    up, down = (tuple(map(int, line.split())) for line in subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout.splitlines())
+    up, down, outside = (tuple(map(int, line.split())) for line in subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout.splitlines())
     assert up == (1, 1, 1)
     assert down == (1, 0, 0)
+    assert outside == (1, 1, 1)  # (below 0 and past the rows, in any order, they are all the same)

@@ -32,3 +32,13 @@ def test_descending(rt, requests, rows, shared):
         assert torch.equal(s.cache.data, before) and bool((held[:32] == 9).all()) and bool((held[-32:] == 9).all())
         s.packed.starts.copy_(good)
         assert torch.equal(s.run(), want)
+
+
+@pytest.mark.parametrize("requests", [5, 70])
+def test_outside_of_the_rows(rt, requests):
+    """starts below 0 and past the call's rows, in any order, count as 0 and as the rows."""
+    s = Step(rt, [0, 0] + [2] * (requests - 4) + [0, 0], [9] * requests, 4, 2, 64, 32, seed=3)
+    want = s.run()
+    s.packed.starts[0], s.packed.starts[1] = -3, -7
+    s.packed.starts[-3:] = torch.tensor([s.rows + 9, s.rows + 900, s.rows + 5], dtype=torch.int32)
+    assert torch.equal(s.run(), want)
